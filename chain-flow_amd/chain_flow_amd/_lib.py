@@ -92,6 +92,16 @@ SIGNATURES = {
     "cfh_gdn_tree": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _VP, _VP, _VP]),
     "cfh_gdn_tree_vllm": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _VP, _VP, _I, _I, _I, _I, _I, _I, _I,
                                C.c_float, _VP, _VP, _VP]),
+    "cfh_kv_write": (_I, [_VP, _I64, _VP, _I64, _I, _I, _I, _I, _VP, _I64, _VP, _I64, _VP, _VP, _I, _I, _VP, _VP, _VP]),
+    "cfh_kv_read": (_I, [_VP, _I64, _VP, _I64, _VP, _VP, _I, _I, _VP, _I, _I, _I, _I, _VP, _VP, _VP, _VP]),
+    "cfh_paged_attn_ws_bytes": (_I64, [_I, _I, _I, _I, _I, _I]),
+    "cfh_paged_attn": (_I, [_VP, _I64, _I, _I, _I, _I, _I, _VP, _I64, _VP, _I64, _VP, _VP, _I, _I, _VP, _I, _I, _VP,
+                            _VP, _I, C.c_float, _I, _I, _VP, _I64, _VP, _VP, _VP, _VP]),
+    "cfh_gdn_decode": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _VP, _I, _I, _I, _I, _I, _I, C.c_float, _VP, _VP,
+                            _VP]),
+    "cfh_gdn_prefill_ws_bytes": (_I64, [_I, _I, _I]),
+    "cfh_gdn_prefill": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, C.c_float,
+                             _VP, _VP, _VP, _VP]),
 }
 
 
@@ -138,6 +148,25 @@ def check(status: int, what: str) -> None:
 def ptr(t) -> int | None:
     """Device (or host) address of a tensor, None for None."""
     return None if t is None else t.data_ptr()
+
+
+def device_of(first, *others, status=None):
+    """The one GPU that the tensors (None: skipped) lie on, which has to be the current device: a launch goes to
+    the current device's stream.  ``status`` words are int32 [1]."""
+    import torch
+    dev = first.device
+    if dev.type != "cuda" or any(t is not None and t.device != dev for t in others):
+        raise ValueError("the tensors must lie on one GPU")
+    if dev.index != torch.cuda.current_device():
+        raise ValueError(f"the tensors lie on {dev}, but the current device is cuda:{torch.cuda.current_device()}")
+    if status is not None and (status.dtype != torch.int32 or status.device != dev or status.numel() < 1):
+        raise ValueError("status must be an int32 tensor on the same device")
+    return dev
+
+
+def aligned(t):
+    """The tensor, or a copy of it that starts on a 16-byte boundary as the vector loads need."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def stream_handle(stream=None):

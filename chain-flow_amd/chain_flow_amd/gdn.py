@@ -1,4 +1,5 @@
-"""Host side of the tree gated delta net (GDN) state update used in tree verification.
+"""Host side of the gated delta net (GDN): the tree state update used in tree verification, and the
+committed tokens' forms (``gdn_prefill``, ``gdn_decode``) that make the states its roots start from.
 
 Mirrors ``tree_gated_delta_scan`` (``cf/kernels/tree_scan.py:41-73``): every node of a BFS-ordered
 draft tree (``parent[n] < n``, -1 = root) applies the gated delta rule to its parent's state (roots
@@ -86,4 +87,85 @@ def tree_gdn_vllm(mixed_qkv, a, b, A_log, dt_bias, ssm_state, node_slots, parent
         int(ssm_state.dtype == torch.bfloat16), nslots, slots.data_ptr(), parent.data_ptr(), int(prefix_slot), N,
         H, HV, K, V, int(bool(use_qk_l2norm)), float(K ** -0.5 if scale is None else scale), out.data_ptr(),
         _lib.ptr(status), _lib.stream_handle()), "cfh_gdn_tree_vllm")
+    return out
+
+
+def _seq_args(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, H, out, status, initial=None):
+    """The checks that ``gdn_prefill`` and ``gdn_decode`` share -> (x, a, b, A_log, dt_bias, slots, out)."""
+    T, conv = mixed_qkv.shape
+    nslots, HV, V, K = ssm_state.shape
+    if H < 1 or HV % H:
+        raise ValueError(f"{HV} value heads are no multiple of {H} q/k heads")
+    if K != 128 or V % 16 or V < 16:
+        raise ValueError(f"ssm_state must be [slots, HV, V, 128] with V a multiple of 16, not {tuple(ssm_state.shape)}")
+    if conv != 2 * H * K + HV * V:
+        raise ValueError(f"mixed_qkv width {conv} != 2*{H}*{K} + {HV}*{V}")
+    if any(t.dtype != torch.bfloat16 for t in (mixed_qkv, a, b)):
+        raise ValueError("mixed_qkv, a, b must be bf16")
+    if ssm_state.dtype not in (torch.bfloat16, torch.float32) or not ssm_state.is_contiguous():
+        raise ValueError("ssm_state must be a contiguous bf16 or fp32 [slots, HV, V, K] tensor")
+    if a.shape != (T, HV) or b.shape != (T, HV) or A_log.shape != (HV,) or dt_bias.shape != (HV,):
+        raise ValueError("a, b must be [T, HV] and A_log, dt_bias [HV]")
+    if slots.dim() != 1 or slots.shape[0] > 4096:
+        raise ValueError("slots must be [S], S <= 4096")
+    dev = _lib.device_of(mixed_qkv, a, b, A_log, dt_bias, ssm_state, status=status)
+    if out is None:
+        out = torch.empty(T, HV, V, dtype=torch.bfloat16, device=dev)
+    elif out.shape != (T, HV, V) or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.device != dev:
+        raise ValueError(f"out must be a contiguous bf16 [{T}, {HV}, {V}] tensor on {dev}")
+    f32 = lambda t: t.to(torch.float32).contiguous()  # noqa: E731
+    return (_lib.aligned(mixed_qkv.contiguous()), a.contiguous(), b.contiguous(), f32(A_log), f32(dt_bias),
+            slots.to(dev, torch.int32).contiguous(), out)
+
+
+def gdn_decode(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, *, num_q_heads: int, scale: float | None = None,
+               use_qk_l2norm: bool = True, out=None, status: torch.Tensor | None = None):
+    """One token of each of S sequences through the gated delta rule (the recurrent step of a decode batch),
+    in ``tree_gdn_vllm``'s layout and gates: mixed_qkv [S, 2 H K + HV V] bf16, a, b [S, HV] bf16, A_log,
+    dt_bias [HV], ssm_state [slots, HV, V, K] bf16 or fp32 (sequence s's slot slots[s] is updated in place).
+    -> o [S, HV, V] bf16.  One launch of ``cfh_gdn_decode``, no host synchronisation.
+
+    Slot -1 marks a padding row: nothing is read or written for it (its row of ``out`` stays as it was).  A
+    slot outside ssm_state or shared by two rows gives NaN outputs, stays as it was, and sets ``status``
+    (int32 [1] on the device, zeroed by the caller), if given, to 1."""
+    H = int(num_q_heads)
+    S = mixed_qkv.shape[0]
+    if slots.shape != (S,):
+        raise ValueError(f"slots must be [{S}]")
+    x, a, b, A_log, dt_bias, slots, out = _seq_args(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, H, out, status)
+    nslots, HV, V, K = ssm_state.shape
+    _lib.check(_lib.lib().cfh_gdn_decode(
+        x.data_ptr(), a.data_ptr(), b.data_ptr(), A_log.data_ptr(), dt_bias.data_ptr(), ssm_state.data_ptr(),
+        int(ssm_state.dtype == torch.bfloat16), nslots, slots.data_ptr(), S, H, HV, K, V, int(bool(use_qk_l2norm)),
+        float(K ** -0.5 if scale is None else scale), out.data_ptr(), _lib.ptr(status), _lib.stream_handle()),
+        "cfh_gdn_decode")
+    return out
+
+
+def gdn_prefill(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, cu_seqlens, *, num_q_heads: int, initial=None,
+                scale: float | None = None, use_qk_l2norm: bool = True, out=None, status: torch.Tensor | None = None):
+    """The rows of S sequences (or chunks of them) through the gated delta rule: sequence s has the rows
+    cu_seqlens[s] .. cu_seqlens[s + 1] of mixed_qkv [T, 2 H K + HV V], starts from slot slots[s] of ssm_state
+    (from zero where ``initial`` [S] bool is given and false) and leaves its state there, rounded to the
+    slot's type once.  Layout, gates and slots as in ``gdn_decode``; the state a draft tree's roots start
+    from (``tree_gdn_vllm``'s prefix slot).  -> o [T, HV, V] bf16.  ``cfh_gdn_prefill``, no host
+    synchronisation; rows of no sequence stay as they were in ``out``."""
+    H = int(num_q_heads)
+    x, a, b, A_log, dt_bias, slots, out = _seq_args(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, H, out, status)
+    S, T = slots.shape[0], x.shape[0]
+    nslots, HV, V, K = ssm_state.shape
+    if cu_seqlens.shape != (S + 1,):
+        raise ValueError(f"cu_seqlens must be [{S + 1}]")
+    cu = cu_seqlens.to(x.device, torch.int32).contiguous()
+    if initial is not None:
+        if initial.shape != (S,) or initial.dtype not in (torch.bool, torch.uint8):
+            raise ValueError(f"initial must be a bool [{S}] tensor")
+        initial = initial.to(x.device).contiguous()
+    L = _lib.lib()
+    ws = torch.empty(int(L.cfh_gdn_prefill_ws_bytes(T, S, HV)), dtype=torch.uint8, device=x.device)
+    _lib.check(L.cfh_gdn_prefill(
+        x.data_ptr(), a.data_ptr(), b.data_ptr(), A_log.data_ptr(), dt_bias.data_ptr(), ssm_state.data_ptr(),
+        int(ssm_state.dtype == torch.bfloat16), nslots, slots.data_ptr(), cu.data_ptr(), _lib.ptr(initial), S, T, H, HV,
+        K, V, int(bool(use_qk_l2norm)), float(K ** -0.5 if scale is None else scale), out.data_ptr(), ws.data_ptr(),
+        _lib.ptr(status), _lib.stream_handle()), "cfh_gdn_prefill")
     return out

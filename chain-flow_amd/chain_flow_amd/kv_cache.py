@@ -1,0 +1,158 @@
+"""Host side of the committed prefix's attention: the paged key / value cache and the attention over it.
+
+* ``kv_cache_write`` -- new keys and values into cache slots, as they are or quantised to 8 bits;
+* ``kv_cache_read`` -- slots back as rows of the model's type;
+* ``paged_attention`` -- new rows (a prefill chunk, single tokens, a draft tree's nodes) over each
+  sequence's pages; with ``causal=False`` and a tree's nodes it gives the prefix half that
+  ``tree_attn_merge`` merges with.
+
+A cache is [blocks, page, Hkv, D] of the model's type (bf16 or fp16), or of ``torch.float8_e4m3fn`` with a
+byte [blocks, page, Hkv] (uint8) per slot and head: byte c stands for the scale 2^(c - 127).  Slot n is row
+n % page of block n / page.  The blocks of a cache may be strided (two halves of one allocation); within a
+block it is contiguous.  No call synchronises with the host.
+"""
+from __future__ import annotations
+
+import torch
+
+from chain_flow_amd import _lib
+
+_TYPES = (torch.bfloat16, torch.float16)
+
+
+def _check_cache(k_cache, v_cache, k_exp, v_exp, dtype):
+    """-> (blocks, page, Hkv, D) of a cache that serves rows of ``dtype``."""
+    blocks, page, Hkv, D = k_cache.shape
+    if v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+        raise ValueError("k_cache and v_cache must share one shape and type")
+    if D not in (64, 128, 256):
+        raise ValueError(f"head width {D} is not 64, 128 or 256")
+    if k_cache.dtype == torch.float8_e4m3fn:
+        for e in (k_exp, v_exp):
+            if e is None or e.dtype != torch.uint8 or e.shape != (blocks, page, Hkv) or not e.is_contiguous():
+                raise ValueError(f"an 8-bit cache needs contiguous uint8 k_exp and v_exp [{blocks}, {page}, {Hkv}]")
+    elif k_cache.dtype != dtype or k_exp is not None or v_exp is not None:
+        raise ValueError(f"the cache must be {dtype} without exponents, or float8_e4m3fn with them")
+    for c in (k_cache, v_cache):
+        if c.stride()[1:] != (Hkv * D, D, 1) or (blocks > 1 and (c.stride(0) < page * Hkv * D or c.stride(0) % 16)) \
+                or c.data_ptr() % 16:
+            raise ValueError("cache blocks must be contiguous [page, Hkv, D], on strides of 16 elements and 16-byte "
+                             "boundaries")
+    return blocks, page, Hkv, D
+
+
+def _block_stride(c):
+    return c.stride(0) if c.shape[0] > 1 else c[0].numel()
+
+
+def _rows(t, name):
+    """Rows [T, heads, D] with contiguous heads whose vector loads are aligned (copied where they are not)."""
+    T, h, D = t.shape
+    if t.stride(2) == 1 and t.stride(1) == D and (T < 2 or (t.stride(0) >= h * D and t.stride(0) % 8 == 0)) \
+            and t.data_ptr() % 16 == 0:
+        return t, t.stride(0) if T > 1 else h * D
+    t = _lib.aligned(t.contiguous())
+    return t, h * D
+
+
+def kv_cache_write(key, value, k_cache, v_cache, slots, *, k_exp=None, v_exp=None, status=None) -> None:
+    """key, value [T, Hkv, D] bf16 or fp16 (rows may be strided) into ``slots`` [T] of the cache, in place.
+
+    With an 8-bit cache each (row, head) gets the least power-of-two scale, from 2^-126 up, that brings its
+    largest finite magnitude to 448 or below; its elements are rounded to e4m3 once (nearest even; they end
+    at 240 where 256 times the scale exceeds the type's largest value, so that what was finite reads back
+    finite), NaN and infinities are stored as NaN.
+
+    A negative slot is a padding row (skipped).  A slot past the cache is skipped and sets ``status`` (int32
+    [1] on the device, zeroed by the caller), if given, to 1.  Slots of one call must differ: rows that share
+    one race, and either's elements may stay (a host tensor's are checked here)."""
+    if key.dtype not in _TYPES or value.dtype != key.dtype or value.shape != key.shape:
+        raise ValueError("key and value must be bf16 or fp16 tensors of one shape [T, Hkv, D]")
+    blocks, page, Hkv, D = _check_cache(k_cache, v_cache, k_exp, v_exp, key.dtype)
+    T = key.shape[0]
+    if key.shape != (T, Hkv, D) or slots.shape != (T,):
+        raise ValueError(f"key and value must be [T, {Hkv}, {D}] and slots [T]")
+    dev = _lib.device_of(key, value, k_cache, v_cache, k_exp, v_exp, status=status)
+    if not slots.is_cuda:
+        used = slots[slots >= 0]
+        if used.unique().numel() != used.numel() or (used >= blocks * page).any():
+            raise ValueError(f"slots must be distinct and below {blocks * page}")
+    slots = slots.to(dev, torch.int32).contiguous()
+    key, ld_k = _rows(key, "key")
+    value, ld_v = _rows(value, "value")
+    _lib.check(_lib.lib().cfh_kv_write(
+        key.data_ptr(), ld_k, value.data_ptr(), ld_v, T, Hkv, D, int(key.dtype == torch.bfloat16), k_cache.data_ptr(),
+        _block_stride(k_cache), v_cache.data_ptr(), _block_stride(v_cache), _lib.ptr(k_exp), _lib.ptr(v_exp), blocks,
+        page, slots.data_ptr(), _lib.ptr(status), _lib.stream_handle()), "cfh_kv_write")
+
+
+def kv_cache_read(k_cache, v_cache, slots, *, dtype=None, k_exp=None, v_exp=None, status=None):
+    """``slots`` [T] of the cache as rows -> (key, value) [T, Hkv, D] of ``dtype`` (default: the cache's type, bf16
+    for an 8-bit cache); 8-bit elements are multiplied by their scale and rounded to nearest even.  A negative
+    slot, and one past the cache (which sets ``status``), gives a zero row."""
+    if dtype is None:
+        dtype = torch.bfloat16 if k_cache.dtype == torch.float8_e4m3fn else k_cache.dtype
+    if dtype not in _TYPES:
+        raise ValueError("rows are read as bf16 or fp16")
+    blocks, page, Hkv, D = _check_cache(k_cache, v_cache, k_exp, v_exp, dtype)
+    if slots.dim() != 1:
+        raise ValueError("slots must be [T]")
+    dev = _lib.device_of(k_cache, v_cache, k_exp, v_exp, status=status)
+    slots = slots.to(dev, torch.int32).contiguous()
+    T = slots.shape[0]
+    key = torch.empty(T, Hkv, D, dtype=dtype, device=dev)
+    value = torch.empty(T, Hkv, D, dtype=dtype, device=dev)
+    _lib.check(_lib.lib().cfh_kv_read(
+        k_cache.data_ptr(), _block_stride(k_cache), v_cache.data_ptr(), _block_stride(v_cache), _lib.ptr(k_exp),
+        _lib.ptr(v_exp), blocks, page, slots.data_ptr(), T, Hkv, D, int(dtype == torch.bfloat16), key.data_ptr(),
+        value.data_ptr(), _lib.ptr(status), _lib.stream_handle()), "cfh_kv_read")
+    return key, value
+
+
+def paged_attention(query, k_cache, v_cache, block_table, seq_lens, cu_q, *, scale: float, causal: bool = True,
+                    k_exp=None, v_exp=None, max_len: int | None = None, out=None, status=None):
+    """query [T, H, D] (rows may be strided; H a multiple of Hkv) over the cache: sequence s has the query rows
+    cu_q[s] .. cu_q[s + 1] and seq_lens[s] tokens in blocks block_table[s]; row i of its n sees token j where
+    j < len and, if ``causal``, j <= len - n + i (the rows' own keys and values are the cache's last n, written
+    before the call).  -> (out [T, H, D] of the query's type, lse [H, T] fp32: ``tree_attn_merge``'s prefix_lse).
+
+    A row that sees no token gives 0 and -inf.  Rows of no sequence stay as they were in ``out``.  Lengths, tables
+    and bounds are read on the device only: a negative length or one past the table, and rows that see a token of
+    a block outside the cache, give NaN; a sequence whose rows do not lie in the query is skipped; each sets
+    ``status`` (int32 [1], zeroed by the caller), if given, to 1.  ``max_len``: an upper bound of the lengths
+    (default: what the table holds); it only plans how the work is split."""
+    if query.dtype not in _TYPES:
+        raise ValueError("query must be bf16 or fp16")
+    blocks, page, Hkv, D = _check_cache(k_cache, v_cache, k_exp, v_exp, query.dtype)
+    T, H, Dq = query.shape
+    if Dq != D or H % Hkv:
+        raise ValueError(f"query must be [T, H, {D}] with H a multiple of {Hkv}")
+    S = seq_lens.shape[0]
+    if seq_lens.shape != (S,) or cu_q.shape != (S + 1,) or block_table.dim() != 2 or block_table.shape[0] != S:
+        raise ValueError("seq_lens must be [S], cu_q [S + 1] and block_table [S, blocks]")
+    dev = _lib.device_of(query, k_cache, v_cache, k_exp, v_exp, status=status)
+    if out is None:
+        out = torch.empty(T, H, D, dtype=query.dtype, device=dev)
+    elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev or out.stride()[1:] != (D, 1) \
+            or (T > 1 and (out.stride(0) < H * D or out.stride(0) % 8)) or out.data_ptr() % 16:
+        raise ValueError(f"out must be a {query.dtype} [{T}, {H}, {D}] tensor on {dev} with contiguous heads, 16-byte "
+                         "aligned")
+    table = block_table.to(dev, torch.int32)
+    if table.stride(1) != 1 or table.stride(0) < table.shape[1]:
+        table = table.contiguous()
+    width = table.shape[1]
+    lens, cu = seq_lens.to(dev, torch.int32).contiguous(), cu_q.to(dev, torch.int32).contiguous()
+    most = width * page
+    most = most if max_len is None else max(0, min(int(max_len), most))
+    lse = torch.empty(H, T, dtype=torch.float32, device=dev)
+    query, q_ld = _rows(query, "query")
+    L = _lib.lib()
+    nws = int(L.cfh_paged_attn_ws_bytes(T, H, Hkv, D, S, most))
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws > 0 else None
+    _lib.check(L.cfh_paged_attn(
+        query.data_ptr(), q_ld, T, H, Hkv, D, int(query.dtype == torch.bfloat16), k_cache.data_ptr(),
+        _block_stride(k_cache), v_cache.data_ptr(), _block_stride(v_cache), _lib.ptr(k_exp), _lib.ptr(v_exp), blocks,
+        page, table.data_ptr(), max(table.stride(0), width), width, lens.data_ptr(), cu.data_ptr(), S, float(scale),
+        int(bool(causal)), most, out.data_ptr(), out.stride(0) if T > 1 else H * D, lse.data_ptr(), _lib.ptr(ws),
+        _lib.ptr(status), _lib.stream_handle()), "cfh_paged_attn")
+    return out, lse

@@ -486,6 +486,73 @@ int cfh_tree_greedy_accept(const void* logits, long long ld, int V, int n_rows, 
                            int max_spec, int32_t* out_tokens, int32_t* accepted_path, int32_t* accepted_len,
                            int32_t* row_argmax, void* ws, void* stream);
 
+/* ---------------------------------------------------------------- the committed prefix: paged cache
+ * The key / value cache of a target's attention layers: k_cache, v_cache [blocks][page][Hkv][D], slot n =
+ * row n % page of block n / page; block strides bs_k / bs_v in elements (multiples of 16, at least
+ * page Hkv D: the two may be views of one allocation), rows within a block contiguous.  With k_exp and
+ * v_exp NULL the elements are 2-byte (bf16 or fp16: is_bf16); with both given they are e4m3, and byte
+ * c = exp[blocks][page][Hkv] is the scale 2^(c - 127) of its (slot, head).  Any page size; D in
+ * {64, 128, 256}; blocks * page < 2^31.  Pointers 16-byte aligned, row strides multiples of 8 elements.
+ *
+ * cfh_kv_write: rows key / value [T][Hkv][D] (row strides ld_k / ld_v, heads contiguous) into slots[T].
+ * A negative slot is a padding row (skipped); one past the cache is skipped and sets status[0] to 1
+ * (status: one int32 the caller zeroes, or NULL).  Two rows of one call in the same slot race: either's
+ * elements may stay.  8-bit form: the scale is the least power of two, from 2^-126 up, that brings the
+ * row's largest finite magnitude to 448 or below; elements are x / scale rounded to nearest even (they end
+ * at 240 where 256 times the scale exceeds the source type's largest value); NaN and infinities become
+ * NaN. */
+int cfh_kv_write(const void* key, long long ld_k, const void* value, long long ld_v, int T, int Hkv, int D,
+                 int is_bf16, void* k_cache, long long bs_k, void* v_cache, long long bs_v, uint8_t* k_exp,
+                 uint8_t* v_exp, int blocks, int page, const int32_t* slots, int32_t* status, void* stream);
+
+/* slots[T] of the cache back as contiguous rows key / value [T][Hkv][D] of the 2-byte type, 8-bit elements
+ * times their scale rounded to nearest even.  Slots outside the cache give zero rows (past it: status 1). */
+int cfh_kv_read(const void* k_cache, long long bs_k, const void* v_cache, long long bs_v, const uint8_t* k_exp,
+                const uint8_t* v_exp, int blocks, int page, const int32_t* slots, int T, int Hkv, int D, int is_bf16,
+                void* key, void* value, int32_t* status, void* stream);
+
+/* Attention of new rows over the cache: sequence s has the query rows cu_q[s] .. cu_q[s+1] of q [T][H][D]
+ * (row stride q_ld) and seq_lens[s] tokens in the blocks table[s][..] (S rows of stride table_ld,
+ * max_blocks entries usable).  Its row i of n sees token j where j < len and, if causal, j <= len - n + i:
+ *   out = sum_j softmax_j(scale q.k_j) v_j (row stride o_ld), lse [H][T] fp32 = log sum_j exp(scale q.k_j)
+ * over kv head h / (H / Hkv); a row that sees nothing gives 0 and -inf.  causal = 0 with a draft tree's
+ * nodes as rows gives the prefix_out / prefix_lse that cfh_tree_attn_merge takes.  Lengths, tables and
+ * row bounds are read on the device only, so the call never synchronises and can be captured.  Rows of no
+ * sequence are left as they were; a sequence whose bounds do not lie in [0, T] is skipped; one whose
+ * length is negative or exceeds max_blocks * page, and rows that see a token of a block outside the cache,
+ * give NaN; each of these sets status[0] to 1.  max_len: an upper bound of the lengths (it only plans how
+ * the work is split).  ws: cfh_paged_attn_ws_bytes(...) bytes, 256-byte aligned (NULL where that is 0). */
+int64_t cfh_paged_attn_ws_bytes(int T, int H, int Hkv, int D, int S, int max_len);
+int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, int is_bf16, const void* k_cache,
+                   long long bs_k, const void* v_cache, long long bs_v, const uint8_t* k_exp, const uint8_t* v_exp,
+                   int blocks, int page, const int32_t* table, int table_ld, int max_blocks, const int32_t* seq_lens,
+                   const int32_t* cu_q, int S, float scale, int causal, int max_len, void* out, long long o_ld,
+                   float* lse, void* ws, int32_t* status, void* stream);
+
+/* ---------------------------------------------------------------- the committed prefix: recurrent state
+ * The gated delta rule over committed tokens, in the layout of cfh_gdn_tree_vllm (mixed_qkv, a, b, A_log,
+ * dt_bias, gates, normalisation, scale, ssm_state [nslots][HV][V][K] bf16 or fp32), each sequence from and
+ * to its slot: S = exp(g) S; d = beta (v - S k); S += d k^T; o = S q.  The state is carried in fp32 and
+ * rounded to the slot's type once, when the call ends; out [T][HV][V] bf16.  K == 128, V % 16 == 0,
+ * S <= 4096.  Slot -1 is a padding sequence (nothing is read or written for it).  A slot outside the state
+ * or shared with another sequence of the call gives NaN rows, leaves the slot as it was and sets status[0]
+ * to 1 (status: one int32 the caller zeroes, or NULL); checked on the device, so the calls never
+ * synchronise and can be captured.
+ *
+ * cfh_gdn_decode: one token a sequence, row s of mixed_qkv [S].
+ * cfh_gdn_prefill: sequence s has the rows cu_seqlens[s] .. cu_seqlens[s+1] of mixed_qkv [T] (a sequence
+ * whose bounds do not lie in [0, T] is skipped and sets status; one of no rows leaves its slot as it was;
+ * rows of no sequence are left as they were).  initial [S] (or NULL: all 1): 0 = start from a zero state
+ * instead of the slot's.  ws: cfh_gdn_prefill_ws_bytes(T, S, HV) bytes, 256-byte aligned. */
+int cfh_gdn_decode(const void* mixed_qkv, const void* a, const void* b, const float* A_log, const float* dt_bias,
+                   void* ssm_state, int state_bf16, int nslots, const int32_t* slots, int S, int H, int HV, int K,
+                   int V, int use_l2norm, float scale, void* out, int32_t* status, void* stream);
+int64_t cfh_gdn_prefill_ws_bytes(int T, int S, int HV);
+int cfh_gdn_prefill(const void* mixed_qkv, const void* a, const void* b, const float* A_log, const float* dt_bias,
+                    void* ssm_state, int state_bf16, int nslots, const int32_t* slots, const int32_t* cu_seqlens,
+                    const uint8_t* initial, int S, int T, int H, int HV, int K, int V, int use_l2norm, float scale,
+                    void* out, void* ws, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -195,3 +195,32 @@ def vllm_gates_f32(a, b, A_log, dt_bias, threshold=20.0):
 
 def _round_bf16_f32(x):
     return _round_bf16(x).astype(np.float32)
+
+
+def gdn_sequences(mixed_qkv, a, b, A_log, dt_bias, state, slots, cu, H, scale, initial=None, use_qk_l2norm=True):
+    """The serving layout's gated delta rule over committed tokens, one after another, in float64: sequence s has
+    rows cu[s] .. cu[s + 1], starts from state[slots[s]] ([HV, V, K]; zero where initial[s] is false) and leaves
+    its state there.  -> (out [T, HV, V] (NaN rows: of no sequence), new state array), nothing rounded but beta."""
+    X = np.asarray(mixed_qkv, np.float64)
+    st = np.array(state, dtype=np.float64, copy=True)
+    _, HV, V, K = st.shape
+    g, beta = vllm_gating(a, b, A_log, dt_bias)
+    out = np.full((X.shape[0], HV, V), np.nan)
+    heads = np.arange(HV) * H // HV
+    for s, slot in enumerate(slots):
+        if slot < 0 or cu[s] == cu[s + 1]:
+            continue
+        S = st[slot] if initial is None or initial[s] else np.zeros((HV, V, K))
+        for t in range(cu[s], cu[s + 1]):
+            q, k = X[t, :H * K].reshape(H, K), X[t, H * K:2 * H * K].reshape(H, K)
+            v = X[t, 2 * H * K:].reshape(HV, V)
+            if use_qk_l2norm:
+                q = q / np.sqrt((q * q).sum(-1, keepdims=True) + 1e-6)
+                k = k / np.sqrt((k * k).sum(-1, keepdims=True) + 1e-6)
+            q, k = q[heads] * scale, k[heads]
+            S = S * np.exp(g[t])[:, None, None]
+            d = (v - np.einsum("hvk,hk->hv", S, k)) * beta[t][:, None]
+            S = S + d[:, :, None] * k[:, None, :]
+            out[t] = np.einsum("hvk,hk->hv", S, q)
+        st[slot] = S
+    return out, st
