@@ -44,19 +44,16 @@ __device__ __forceinline__ unsigned pack_e4m3(float a, float b, float c, float d
   return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 
-// Eight e4m3 elements times s, rounded to the 2-byte type.
+// Eight e4m3 elements times 2^(code - 127), rounded to the 2-byte type (nearest even): one conversion for two.
 template <bool BF>
-__device__ __forceinline__ uint4 dequant8(const uint2& w, float s) {
-  uint4 o;
-  auto two = [&](int word, auto hi) {
-    const f32x2k v = __builtin_amdgcn_cvt_pk_f32_fp8(word, hi.value);
-    return pack2<BF>(v[0] * s, v[1] * s);
+__device__ __forceinline__ uint4 dequant8(const uint2& w, int code) {
+  const float s = __uint_as_float((unsigned)code << 23);
+  auto two = [&](unsigned word, auto hi) {
+    if constexpr (BF) return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, s, hi.value));
+    else return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, s, hi.value));
   };
-  o.x = two((int)w.x, std::false_type{});
-  o.y = two((int)w.x, std::true_type{});
-  o.z = two((int)w.y, std::false_type{});
-  o.w = two((int)w.y, std::true_type{});
-  return o;
+  return make_uint4(two(w.x, std::false_type{}), two(w.x, std::true_type{}), two(w.y, std::false_type{}),
+                    two(w.y, std::true_type{}));
 }
 
 // f(bf16?, 8-bit cache?, head width) with the three as types.

@@ -102,8 +102,7 @@ __global__ void __launch_bounds__(256) k_kv_read(KvRowsArgs a) {
       out = *(const uint4*)((const u16*)(val ? a.vc : a.kc) + src);
     } else {
       const uint2 w = *(const uint2*)((const uint8_t*)(val ? a.vc : a.kc) + src);
-      const float s = __uint_as_float((unsigned)(val ? a.ve : a.ke)[(size_t)slot * a.Hkv + h] << 23);
-      out = dequant8<BF>(w, s);
+      out = dequant8<BF>(w, (val ? a.ve : a.ke)[(size_t)slot * a.Hkv + h]);
     }
   } else if (slot >= 0 && a.status && c == 0) {
     a.status[0] = 1;

@@ -3,13 +3,29 @@
 //
 // Sequence s has the query rows cu_q[s] .. cu_q[s + 1] and seq_lens[s] tokens in its pages table[s][..].
 // Its row i of n sees token j where j < len and, if causal, j <= len - n + i (the chunk's own rows are the
-// cache's last ones).  Head h reads kv head h / (H / Hkv).
+// cache's last ones).  Head h reads kv head h / G, G = H / Hkv.
 //     o = sum_j softmax_j(scale q.k_j) v_j,   lse = log sum_j exp(scale q.k_j)
 // A row that sees nothing gives o = 0 and lse = -inf.
+//
+// The G heads of a kv head are packed beside each other as rows (row r = token r / G, head r % G), so each
+// cache row is read once for all of them.  Both kernels compute the transposed scores S^T = K Q^T with MFMA:
+// a lane then holds one query row's scores, the running maximum and sum of its softmax are lane-local but
+// for one exchange, and the probabilities are already where the next MFMA wants its second operand
+// (O^T += V^T P^T), only in another order of the tokens, which the first operand's loads follow.
+// Probabilities are rounded to the 2-byte type once for that product; statistics and sums are fp32.
+//   k_attn_tiles  many rows: workgroups of NW waves x 32 rows over tiles of tokens staged in LDS
+//   k_attn_rows   few rows (decode): one tile of 16 rows, each wave its own tokens, no barrier but the join's
+// The long axis is cut into pieces of `piece` tokens where the rows alone do not fill the chip; k_attn_join
+// then merges the pieces' (max, sum, O).
 #include "cfh_host.h"
 #include "cfh_kv.h"
 
 namespace {
+
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 struct PagedArgs {
   const u16* q;                // [T][H][D], row stride q_ld
@@ -21,94 +37,707 @@ struct PagedArgs {
   const int* lens;             // [S]
   const int* cu;               // [S + 1]
   int* status;
+  float* po;                   // pieces' O [npiece][T][H][D] (npiece > 1)
+  float2* pml;                 // pieces' (max in log2 units, sum) [npiece][T][H]
   long long q_ld, o_ld, bs_k, bs_v;
-  int T, H, Hkv, S, blocks, page, table_ld, max_blocks, causal;
-  float scale;
+  unsigned long long pmagic;   // j / page = j * pmagic >> pshift, j < 2^31
+  int pshift;
+  int T, H, Hkv, G, S, blocks, page, table_ld, max_blocks, causal;
+  int piece, npiece, tiles;    // tokens a piece, pieces, row-tile slots
+  int few;                     // rows (tokens * G) up to which a sequence is k_attn_rows' (0: none)
+  int qsign;                   // of the scale: the sign goes into q, so that the scores' maximum scales
+  float c;                     // |scale| log2(e)
 };
 
 // Whether a sequence's rows lie in the query.
 __device__ __forceinline__ bool bounds_ok(const PagedArgs& a, int c0, int c1) { return c0 >= 0 && c0 <= c1 && c1 <= a.T; }
 
-// The simplest form: a wave per (row, head), lane l the elements l * EPL .., one token after another with
-// the running maximum and sum of the softmax.
+__device__ __forceinline__ int page_of(const PagedArgs& a, int j) { return (int)(((unsigned long long)(unsigned)j * a.pmagic) >> a.pshift); }
+
+// Row-tile slot -> (sequence, tile): sequence s has the slots from floor(cu[s] G / R) + s on, at most
+// ceil(n G / R) of them used, so no two sequences share one.  A search over 64 sequences a step.
+template <int R>
+__device__ __forceinline__ bool find_tile(const PagedArgs& a, int slot, int& s, int& tile) {
+  const int lane = threadIdx.x & 63;
+  auto start = [&](int i) { return (int)(((long long)a.cu[i] * a.G) / R) + i; };   // (of bounds past T: any value)
+  int lo = 0, n = a.S;                       // the last i in [lo, lo + n) with start(i) <= slot
+  while (n > 1) {
+    const int step = (n + 63) / 64, i = lo + lane * step;
+    const bool le = i < lo + n && start(i) <= slot;
+    const unsigned long long m = __ballot(le);
+    const int k = m ? 63 - __builtin_clzll(m) : 0;
+    n = min(step, lo + n - (lo + k * step));
+    lo += k * step;
+  }
+  s = lo;
+  tile = slot - start(lo);
+  return tile >= 0;
+}
+
+// What one workgroup works on: rows [r0, r0 + R) of the n * G packed rows of sequence s and kv head hk, and
+// the tokens [j0, j1) of one piece.
+struct Work {
+  int s, c0, n, len, hk, piece, r0, j0, j1, jend;   // jend: tokens any of the tile's rows sees
+  bool bad;                                         // a length the table cannot hold
+};
+
+// The number of tokens row token i of n sees.
+__device__ __forceinline__ int seen(const PagedArgs& a, int len, int n, int i) {
+  return a.causal ? max(0, min(len, len - n + i + 1)) : len;
+}
+
+template <int R, bool FEW>
+__device__ __forceinline__ bool find_work(const PagedArgs& a, Work& w) {
+  // (kv head, piece) groups and row tiles: consecutive workgroups go to the eight XCDs in turn, and each XCD
+  // has its own L2, so a group's row tiles, which read the same tokens, are kept on one XCD (or an even share
+  // of the XCDs) where the group count allows
+  const int groups = a.Hkv * a.npiece;
+  int g, t;
+  const int b = blockIdx.x;
+  if (8 % groups == 0) {
+    const int per = 8 / groups, x = b % 8;
+    g = x / per;
+    t = b / 8 * per + x % per;
+  } else if (groups % 8 == 0) {
+    g = b % 8 + 8 * (b / 8 / a.tiles);
+    t = b / 8 % a.tiles;
+  } else {
+    g = b % groups;
+    t = b / groups;
+  }
+  if (g >= groups || t >= a.tiles) return false;
+  w.hk = g % a.Hkv;
+  w.piece = g / a.Hkv;
+  int tile;
+  if (!find_tile<R>(a, a.tiles - 1 - t, w.s, tile)) return false;   // (late rows see the most: first)
+  w.c0 = a.cu[w.s];
+  const int c1 = a.cu[w.s + 1];
+  if (!bounds_ok(a, w.c0, c1)) return false;
+  w.n = c1 - w.c0;
+  if (FEW ? (a.few && (long long)w.n * a.G > a.few) : (long long)w.n * a.G <= a.few) return false;
+  w.r0 = tile * R;
+  if (w.r0 >= w.n * a.G) return false;
+  w.len = a.lens[w.s];
+  w.bad = w.len < 0 || w.len > (long long)a.max_blocks * a.page;
+  if (w.bad) w.len = 0;
+  w.jend = seen(a, w.len, w.n, min(w.n * a.G - 1, w.r0 + R - 1) / a.G);
+  w.j0 = min(w.piece * a.piece, w.jend);
+  w.j1 = w.piece + 1 == a.npiece ? w.jend : min(w.j0 + a.piece, w.jend);
+  // a piece past the tile's tokens has nothing to do; the first one also answers for rows that see nothing
+  return w.piece == 0 || w.j0 < w.j1;
+}
+
+// Sequences whose rows do not lie in the query are skipped: the status word says so.
+__device__ __forceinline__ void check_bounds(const PagedArgs& a) {
+  if (a.status && blockIdx.x == 0)
+    for (int i = threadIdx.x; i < a.S; i += blockDim.x)
+      if (!bounds_ok(a, a.cu[i], a.cu[i + 1])) a.status[0] = 1;
+}
+
+// The block of token j, or -1 where j is not below j1; a block outside the cache is noted.
+__device__ __forceinline__ int block_of(const PagedArgs& a, const Work& w, int j, int* first_bad) {
+  if (j >= w.j1) return -1;
+  const int b = a.table[(size_t)w.s * a.table_ld + page_of(a, j)];
+  if (b >= 0 && b < a.blocks) return b;
+  atomicMin(first_bad, j);
+  return -1;
+}
+
+// 8 elements of the row of token j (block b >= 0) as the 2-byte type; zero where b < 0, so that nothing that
+// lies past a sequence's tokens reaches a product.
+template <bool F8>
+__device__ __forceinline__ uint4 load_row(const PagedArgs& a, const void* c, long long bs, int b, int j, int hk, int D, int col) {
+  if (b < 0) return make_uint4(0, 0, 0, 0);
+  const int at = j - page_of(a, j) * a.page;
+  const size_t i = (size_t)b * bs + ((size_t)at * a.Hkv + hk) * D + col;
+  if constexpr (F8) {
+    const uint2 r = *(const uint2*)((const uint8_t*)c + i);
+    return make_uint4(r.x, r.y, 0, 0);
+  } else {
+    return *(const uint4*)((const u16*)c + i);
+  }
+}
+template <bool F8>
+__device__ __forceinline__ int load_exp(const PagedArgs& a, const uint8_t* ex, int b, int j, int hk) {
+  if (!F8 || b < 0) return 127;
+  const int at = j - page_of(a, j) * a.page;
+  return ex[((size_t)b * a.page + at) * a.Hkv + hk];
+}
+template <bool BF, bool F8>
+__device__ __forceinline__ uint4 to_rows(const uint4& r, int code) {
+  if constexpr (F8) return dequant8<BF>(make_uint2(r.x, r.y), code);
+  else return r;
+}
+
+template <bool BF>
+__device__ __forceinline__ f32x16 mfma32(const uint4& x, const uint4& y, f32x16 acc) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b16x8, x), __builtin_bit_cast(b16x8, y), acc, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h16x8, x), __builtin_bit_cast(h16x8, y), acc, 0, 0, 0);
+}
+
+// Four elements of one column from four rows of 16-lane blocks in LDS (lane l of a block points at row l / 4,
+// columns 4 (l % 4) .. + 3 and receives column l of rows 0 .. 3).
+__device__ __forceinline__ uint2 read_tr(const u16* p) {
+  typedef __attribute__((address_space(3))) s16x4* lptr;
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)p));
+}
+
+// 16-byte chunk order within a token's row in LDS: chunk c of token t lies at c ^ swz(t).  Eight tokens with
+// one chunk (K's operand reads), and four tokens with two neighbouring chunks (V's transposed reads), each
+// cover all 128 bytes of the banks.
+__device__ __forceinline__ int swz(int t) { return ((t & 3) << 1) | ((t >> 2) & 1); }
+
+__device__ __forceinline__ float swap_max(float x) {
+  const u32x2 s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float swap_sum(float x) {
+  const u32x2 s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+// Whether any of the eight 2-byte elements is infinite or NaN.
+template <bool BF>
+__device__ __forceinline__ bool any_nonfinite(const uint4& r) {
+  constexpr unsigned E = BF ? 0x7f80u : 0x7c00u;
+  bool f = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned w = i == 0 ? r.x : i == 1 ? r.y : i == 2 ? r.z : r.w;
+    f |= (w & E) == E || (w & (E << 16)) == (E << 16);
+  }
+  return f;
+}
+// The same elements with what is not finite replaced: kind 0 by zero; kinds 1 and 2 keep only that, as 1 where
+// the element is +inf or NaN (1), or -inf or NaN (2), and 0 elsewhere.
+template <bool BF>
+__device__ __forceinline__ unsigned only_finite(unsigned w, int kind) {
+  constexpr unsigned E = BF ? 0x7f80u : 0x7c00u, M = BF ? 0x7fu : 0x3ffu, ONE = BF ? 0x3f80u : 0x3c00u;
+  unsigned o = 0;
+#pragma unroll
+  for (int h = 0; h < 32; h += 16) {
+    const unsigned e = (w >> h) & 0xffffu;
+    const bool inf = (e & E) == E, nan = inf && (e & M), neg = e >> 15;
+    const unsigned x = kind == 0 ? (inf ? 0u : e) : (inf && (nan || neg == (kind == 2)) ? ONE : 0u);
+    o |= x << h;
+  }
+  return o;
+}
+
+constexpr float LAZY = 8.f;   // log2 units the running maximum may lag behind (probabilities up to 2^8)
+
+// Many rows.  Wave v of a workgroup takes rows 32 v .. 32 v + 31 of its tile; lane l of a wave holds query
+// row l % 32, and of every group of eight tokens the four with (t / 4) % 2 == l / 32.  Token tiles of TK go
+// global -> registers -> LDS one tile ahead (the 8-bit cache is widened on that way), double-buffered, one
+// barrier a tile.
+template <bool BF, bool F8, int D, int NW, int TK>
+__global__ void __launch_bounds__(NW * 64) k_attn_tiles(PagedArgs a) {
+  constexpr int R = NW * 32, NT = NW * 64;
+  constexpr int CH = D / 8;                       // 16-byte chunks a token's row
+  constexpr int CPT = TK * CH / NT;               // chunks a thread stages (of K, and of V)
+  constexpr int RS = NT / CH;                     // tokens between a thread's chunks
+  static_assert(CPT >= 1 && TK % 32 == 0, "a tile is at least a chunk a thread");
+  __shared__ __align__(16) u16 lds[2][2][TK * D];
+  __shared__ int first_bad, odd[2];
+  check_bounds(a);
+  Work w;
+  if (!find_work<R, false>(a, w)) return;         // (the whole workgroup)
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5;
+  if (tid == 0) { first_bad = 0x7fffffff; odd[0] = odd[1] = -1; }
+  __syncthreads();
+
+  const int r = w.r0 + wave * 32 + (lane & 31), rows = w.n * a.G;
+  const bool live = r < rows;
+  const int i = min(r, rows - 1) / a.G, hh = min(r, rows - 1) % a.G;
+  const int t = w.c0 + i, h = w.hk * a.G + hh;
+  const int vis = min(seen(a, w.len, w.n, i), w.j1);
+  // the fewest tokens a row of the wave, and of the workgroup, sees: tiles below need no mask
+  const int vis_wave = min(seen(a, w.len, w.n, min(w.r0 + wave * 32, rows - 1) / a.G), w.j1);
+  const int vis_wg = min(seen(a, w.len, w.n, w.r0 / a.G), w.j1);
+  uint4 qf[D / 16];
+  {
+    const u16* q = a.q + (size_t)t * a.q_ld + (size_t)h * D + 8 * half;
+    const unsigned flip = a.qsign < 0 ? 0x80008000u : 0u, keep = a.qsign ? 0xffffffffu : 0u;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      uint4 x = *(const uint4*)(q + 16 * s);
+      qf[s] = make_uint4((x.x ^ flip) & keep, (x.y ^ flip) & keep, (x.z ^ flip) & keep, (x.w ^ flip) & keep);
+    }
+  }
+
+  const int srow = tid / CH, scol = tid % CH;     // this thread's chunks: tokens srow + RS x, chunk scol
+  uint4 kr[CPT], vr[CPT];
+  int kx[CPT], vx[CPT], blk[CPT];
+  auto blocks = [&](int jt) {
+#pragma unroll
+    for (int x = 0; x < CPT; ++x) blk[x] = block_of(a, w, jt + srow + RS * x, &first_bad);
+  };
+  auto fetch = [&](int jt) {
+#pragma unroll
+    for (int x = 0; x < CPT; ++x) {
+      const int j = jt + srow + RS * x;
+      kr[x] = load_row<F8>(a, a.kc, a.bs_k, blk[x], j, w.hk, D, scol * 8);
+      vr[x] = load_row<F8>(a, a.vc, a.bs_v, blk[x], j, w.hk, D, scol * 8);
+      kx[x] = load_exp<F8>(a, a.ke, blk[x], j, w.hk);
+      vx[x] = load_exp<F8>(a, a.ve, blk[x], j, w.hk);
+    }
+  };
+  auto stage = [&](int jt, int buf) {
+    bool f = false;
+#pragma unroll
+    for (int x = 0; x < CPT; ++x) {
+      const int tok = srow + RS * x, at = tok * D + ((scol ^ swz(tok)) * 8);
+      const uint4 v = to_rows<BF, F8>(vr[x], vx[x]);
+      *(uint4*)&lds[buf][0][at] = to_rows<BF, F8>(kr[x], kx[x]);
+      *(uint4*)&lds[buf][1][at] = v;
+      if (jt + TK > vis_wg) f |= any_nonfinite<BF>(v);
+    }
+    if (f) odd[buf] = jt;                         // a tile that some rows see in part holds what is not finite
+  };
+
+  f32x16 o[D / 32] = {};
+  float m = -INFINITY, l = 0.f;                   // (m in log2 units; l: this half's tokens)
+  if (w.j0 < w.j1) {
+    blocks(w.j0);
+    fetch(w.j0);
+    blocks(w.j0 + TK);
+    stage(w.j0, 0);
+  }
+  int buf = 0;
+  for (int jt = w.j0; jt < w.j1; jt += TK, buf ^= 1) {
+    __syncthreads();
+    const bool more = jt + TK < w.j1;
+    if (more) {
+      fetch(jt + TK);
+      blocks(jt + 2 * TK);
+    }
+    if (jt < w.j1 && w.r0 + wave * 32 < rows) {
+      const u16* kt = lds[buf][0];
+      const u16* vt = lds[buf][1];
+      f32x16 sc[TK / 32];
+#pragma unroll
+      for (int b = 0; b < TK / 32; ++b) {
+        sc[b] = f32x16{};
+        const int tok = 32 * b + (lane & 31);
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+          const uint4 kf = *(const uint4*)&kt[tok * D + (((2 * s + half) ^ swz(tok)) * 8)];
+          sc[b] = mfma32<BF>(kf, qf[s], sc[b]);
+        }
+      }
+      if (jt + TK > vis_wave) {
+#pragma unroll
+        for (int b = 0; b < TK / 32; ++b)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (jt + 32 * b + 8 * (e / 4) + 4 * half + e % 4 >= vis) sc[b][e] = -INFINITY;
+      }
+      float mx = sc[0][0];
+#pragma unroll
+      for (int b = 0; b < TK / 32; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[b][e]);
+      mx = swap_max(mx) * a.c;
+      if (__any(mx > m + LAZY || (m == -INFINITY && mx > m))) {
+        const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[d][e] *= f;
+        m = mn;
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+      uint4 pf[TK / 16];
+#pragma unroll
+      for (int b = 0; b < TK / 32; ++b) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          sc[b][e] = __builtin_amdgcn_exp2f(fmaf(sc[b][e], a.c, -base));
+          l += sc[b][e];
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+          pf[2 * b + s] = make_uint4(pack2<BF>(sc[b][8 * s], sc[b][8 * s + 1]), pack2<BF>(sc[b][8 * s + 2], sc[b][8 * s + 3]),
+                                     pack2<BF>(sc[b][8 * s + 4], sc[b][8 * s + 5]), pack2<BF>(sc[b][8 * s + 6], sc[b][8 * s + 7]));
+      }
+      // the transposed reads: lane block (lane / 16) % 2 takes 16 of the 32 columns, half the tokens 4 half ..
+      const int tr = 4 * half + (lane & 15) / 4, cl = 2 * ((lane >> 4) & 1) + (lane & 3) / 2, by = 4 * (lane & 1);
+      auto vfrag = [&](int d, int s) {
+        const int t0 = 16 * s + tr, t1 = t0 + 8;
+        const uint2 x = read_tr(&vt[t0 * D + (((4 * d + cl) ^ swz(t0)) * 8) + by]);
+        const uint2 y = read_tr(&vt[t1 * D + (((4 * d + cl) ^ swz(t1)) * 8) + by]);
+        return make_uint4(x.x, x.y, y.x, y.y);
+      };
+      if (odd[buf] != jt) {
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+          for (int s = 0; s < TK / 16; ++s) o[d] = mfma32<BF>(vfrag(d, s), pf[s], o[d]);
+      } else {
+        // a value that is not finite and that some of the rows do not see: 0 * NaN must not reach those.  The
+        // finite values as ever; then the others as ones, times ones where a row sees the token
+        uint4 pi[TK / 16];
+        constexpr unsigned ONE = BF ? 0x3f80u : 0x3c00u;
+#pragma unroll
+        for (int s = 0; s < TK / 16; ++s) {
+          unsigned b[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = jt + 16 * s + 8 * (e / 2) + 4 * half + 2 * (e % 2);
+            b[e] = (j < vis ? ONE : 0u) | (j + 1 < vis ? ONE << 16 : 0u);
+          }
+          pi[s] = make_uint4(b[0], b[1], b[2], b[3]);
+        }
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) {
+          f32x16 up = {}, down = {};
+#pragma unroll
+          for (int s = 0; s < TK / 16; ++s) {
+            const uint4 v = vfrag(d, s);
+            auto as = [&](int kind) {
+              return make_uint4(only_finite<BF>(v.x, kind), only_finite<BF>(v.y, kind), only_finite<BF>(v.z, kind),
+                                only_finite<BF>(v.w, kind));
+            };
+            o[d] = mfma32<BF>(as(0), pf[s], o[d]);
+            up = mfma32<BF>(as(1), pi[s], up);
+            down = mfma32<BF>(as(2), pi[s], down);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[d][e] += (up[e] > 0.f ? INFINITY : 0.f) + (down[e] > 0.f ? -INFINITY : 0.f);
+        }
+      }
+    }
+    if (more) stage(jt + TK, buf ^ 1);
+  }
+  __syncthreads();
+  l = swap_sum(l);
+  if (w.bad || first_bad < vis) {
+    l = __builtin_nanf("");
+    if (a.status && live) a.status[0] = 1;
+  }
+  if (!live) return;
+  if (a.npiece == 1) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    u16* out = a.out + (size_t)t * a.o_ld + (size_t)h * D + 4 * half;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *(uint2*)(out + 32 * d + 8 * g) = make_uint2(pack2<BF>(o[d][4 * g] * inv, o[d][4 * g + 1] * inv),
+                                                     pack2<BF>(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
+    if (half == 0) a.lse[(size_t)h * a.T + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
+  } else {
+    const size_t at = ((size_t)w.piece * a.T + t) * a.H + h;
+    float* po = a.po + at * D + 4 * half;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *(float4*)(po + 32 * d + 8 * g) = make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+    if (half == 0) a.pml[at] = make_float2(m, l);
+  }
+}
+
+// Few rows: a tile of 16, one workgroup of four waves a (row tile, kv head, piece), each wave the tokens of
+// every fourth group of 16.  K goes from memory straight into the first operand's registers (16 tokens x
+// 64-byte segments a load), V through the wave's own 16 rows of LDS for the transposed reads; both one group
+// ahead.  Waves do not wait for each other before the join of their (max, sum, O) at the end.
+template <bool BF>
+__device__ __forceinline__ f32x4 mfma16(const uint4& x, const uint4& y, f32x4 acc) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, x), __builtin_bit_cast(b16x8, y), acc, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, x), __builtin_bit_cast(h16x8, y), acc, 0, 0, 0);
+}
+template <bool BF>
+__device__ __forceinline__ f32x4 mfma16h(const uint2& x, const uint2& y, f32x4 acc) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, x), __builtin_bit_cast(s16x4, y), acc, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(h16x4, x), __builtin_bit_cast(h16x4, y), acc, 0, 0, 0);
+}
+
 template <bool BF, bool F8, int D>
-__global__ void __launch_bounds__(256) k_paged_rows(PagedArgs a) {
-  constexpr int EPL = D / 64;
+__global__ void __launch_bounds__(256) k_attn_rows(PagedArgs a) {
+  constexpr int R = 16, NW = 4, KS = D / 32;      // MFMA steps of 32 along the head
+  constexpr int CH = D / 8, VPT = 16 * CH / 64;   // V's 16-byte chunks a lane stages
+  constexpr int KL = F8 ? KS / 2 : KS;            // 16-byte loads of a lane's share of K
+  __shared__ __align__(16) union { u16 v[NW][16 * D]; float o[NW][16 * D]; } sh;
+  __shared__ float2 ml[NW][16];
+  __shared__ int first_bad;
+  check_bounds(a);
+  Work w;
+  if (!find_work<R, true>(a, w)) return;          // (the whole workgroup)
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, tl = lane & 15;
+  if (tid == 0) first_bad = 0x7fffffff;
+  __syncthreads();
+  const int rows = w.n * a.G, r = w.r0 + tl;
+  const int i = min(r, rows - 1) / a.G, hh = min(r, rows - 1) % a.G;
+  const int t = w.c0 + i, h = w.hk * a.G + hh;
+  const int vis = min(seen(a, w.len, w.n, i), w.j1);
+  const int vis_all = min(seen(a, w.len, w.n, w.r0 / a.G), w.j1);
+  // contraction order: step s, lane group g, element e is column 32 s + 8 g + e, or with an 8-bit cache, whose
+  // 16-byte loads hold two steps' elements, column 64 (s / 2) + 16 g + 8 (s % 2) + e
+  uint4 qf[KS];
+  {
+    const u16* q = a.q + (size_t)t * a.q_ld + (size_t)h * D;
+    const unsigned flip = a.qsign < 0 ? 0x80008000u : 0u, keep = a.qsign ? 0xffffffffu : 0u;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const uint4 x = *(const uint4*)(q + (F8 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g));
+      qf[s] = make_uint4((x.x ^ flip) & keep, (x.y ^ flip) & keep, (x.z ^ flip) & keep, (x.w ^ flip) & keep);
+    }
+  }
+  u16* const vt = sh.v[wave];
+  uint4 kr[KL], vr[VPT];
+  int kx = 127, vx[VPT], kb = -1, vb[VPT];
+  // this lane's token of K is tl; its chunks of V are tokens (lane + 64 x) / CH
+  auto blocks = [&](int jt) {
+    kb = block_of(a, w, jt + tl, &first_bad);
+#pragma unroll
+    for (int x = 0; x < VPT; ++x) vb[x] = block_of(a, w, jt + (lane + 64 * x) / CH, &first_bad);
+  };
+  auto fetch = [&](int jt) {
+#pragma unroll
+    for (int s = 0; s < KL; ++s) {
+      if constexpr (F8) {
+        kr[s] = make_uint4(0, 0, 0, 0);
+        if (kb >= 0) {
+          const int j = jt + tl, at = j - page_of(a, j) * a.page;
+          kr[s] = *(const uint4*)((const uint8_t*)a.kc + (size_t)kb * a.bs_k + ((size_t)at * a.Hkv + w.hk) * D + 64 * s + 16 * g);
+        }
+      } else {
+        kr[s] = load_row<false>(a, a.kc, a.bs_k, kb, jt + tl, w.hk, D, 32 * s + 8 * g);
+      }
+    }
+    kx = load_exp<F8>(a, a.ke, kb, jt + tl, w.hk);
+#pragma unroll
+    for (int x = 0; x < VPT; ++x) {
+      const int c = lane + 64 * x, j = jt + c / CH;
+      vr[x] = load_row<F8>(a, a.vc, a.bs_v, vb[x], j, w.hk, D, (c % CH) * 8);
+      vx[x] = load_exp<F8>(a, a.ve, vb[x], j, w.hk);
+    }
+  };
+  f32x4 o[D / 16] = {};
+  float m = -INFINITY, l = 0.f;
+  const int step = 16 * NW;
+  int jt = w.j0 + 16 * wave;
+  if (jt < w.j1) {
+    blocks(jt);
+    fetch(jt);
+    blocks(jt + step);
+  }
+  for (; jt < w.j1; jt += step) {
+    bool f = false;
+#pragma unroll
+    for (int x = 0; x < VPT; ++x) {
+      const int c = lane + 64 * x, tok = c / CH;
+      const uint4 v = to_rows<BF, F8>(vr[x], vx[x]);
+      *(uint4*)&vt[tok * D + (((c % CH) ^ swz(tok)) * 8)] = v;
+      f |= jt + 16 > vis_all && any_nonfinite<BF>(v);
+    }
+    const bool odd = __any(f);
+    uint4 kf[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      if constexpr (F8) kf[s] = dequant8<BF>(s % 2 ? make_uint2(kr[s / 2].z, kr[s / 2].w) : make_uint2(kr[s / 2].x, kr[s / 2].y), kx);
+      else kf[s] = kr[s];
+    }
+    if (jt + step < w.j1) {
+      fetch(jt + step);
+      blocks(jt + 2 * step);
+    }
+    f32x4 sc = {};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) sc = mfma16<BF>(kf[s], qf[s], sc);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (jt + 4 * g + e >= vis) sc[e] = -INFINITY;
+      mx = fmaxf(mx, sc[e]);
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 16));
+    mx = swap_max(mx) * a.c;
+    if (__any(mx > m + LAZY || (m == -INFINITY && mx > m))) {
+      const float mn = fmaxf(m, mx), fac = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= fac;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][e] *= fac;
+      m = mn;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], a.c, -base));
+      l += sc[e];
+    }
+    const uint2 pf = make_uint2(pack2<BF>(sc[0], sc[1]), pack2<BF>(sc[2], sc[3]));
+    // (a wave's LDS accesses complete in order: its reads see its own writes above)
+    const int tr = 4 * g + tl / 4;
+    auto vfrag = [&](int d) { return read_tr(&vt[tr * D + (((2 * d + (tl & 3) / 2) ^ swz(tr)) * 8) + 4 * (tl & 1)]); };
+    if (!odd) {
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) o[d] = mfma16h<BF>(vfrag(d), pf, o[d]);
+    } else {                                      // (as in k_attn_tiles)
+      constexpr unsigned ONE = BF ? 0x3f80u : 0x3c00u;
+      const int j = jt + 4 * g;
+      const uint2 pi = make_uint2((j < vis ? ONE : 0u) | (j + 1 < vis ? ONE << 16 : 0u),
+                                  (j + 2 < vis ? ONE : 0u) | (j + 3 < vis ? ONE << 16 : 0u));
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        const uint2 v = vfrag(d);
+        auto as = [&](int kind) { return make_uint2(only_finite<BF>(v.x, kind), only_finite<BF>(v.y, kind)); };
+        o[d] = mfma16h<BF>(as(0), pf, o[d]);
+        const f32x4 up = mfma16h<BF>(as(1), pi, f32x4{}), down = mfma16h<BF>(as(2), pi, f32x4{});
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][e] += (up[e] > 0.f ? INFINITY : 0.f) + (down[e] > 0.f ? -INFINITY : 0.f);
+      }
+    }
+  }
+  // the four waves' join: each row's maximum, then the sums of what the waves hold under it
+  l += __shfl_xor(l, 16);
+  l = swap_sum(l);
+  if (lane < 16) ml[wave][lane] = make_float2(m, l);
+  __syncthreads();                                // (and the waves are done with sh.v)
+  float mj = -INFINITY;
+#pragma unroll
+  for (int v = 0; v < NW; ++v) mj = fmaxf(mj, ml[v][tl].x);
+  const float mine = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mj);
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d)
+    *(f32x4*)&sh.o[wave][tl * D + 16 * (d ^ (tl & (D / 16 - 1))) + 4 * g] = o[d] * mine;
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < 16 * D / 4 / 256; ++x) {
+    const int c = tid + 256 * x, row = c / (D / 4), col = c % (D / 4) * 4;
+    const int rr = w.r0 + row;
+    if (rr >= rows) break;
+    const int ti = rr / a.G, tt = w.c0 + ti, th = w.hk * a.G + rr % a.G;
+    f32x4 sum = {};
+    float ls = 0.f, mr = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < NW; ++v) mr = fmaxf(mr, ml[v][row].x);
+#pragma unroll
+    for (int v = 0; v < NW; ++v) {
+      sum += *(const f32x4*)&sh.o[v][row * D + 16 * ((col / 16) ^ (row & (D / 16 - 1))) + col % 16];
+      ls += ml[v][row].x == -INFINITY ? ml[v][row].y : ml[v][row].y * __builtin_amdgcn_exp2f(ml[v][row].x - mr);
+    }
+    if (w.bad || first_bad < min(seen(a, w.len, w.n, ti), w.j1)) {
+      ls = __builtin_nanf("");
+      if (a.status) a.status[0] = 1;
+    }
+    if (a.npiece == 1) {
+      const float inv = ls == 0.f ? 0.f : 1.f / ls;
+      *(uint2*)(a.out + (size_t)tt * a.o_ld + (size_t)th * D + col) =
+          make_uint2(pack2<BF>(sum[0] * inv, sum[1] * inv), pack2<BF>(sum[2] * inv, sum[3] * inv));
+      if (col == 0) a.lse[(size_t)th * a.T + tt] = ls == 0.f ? -INFINITY : (mr + log2f(ls)) * 0.69314718055994530942f;
+    } else {
+      const size_t at = ((size_t)w.piece * a.T + tt) * a.H + th;
+      *(f32x4*)(a.po + at * D + col) = sum;
+      if (col == 0) a.pml[at] = make_float2(mr, ls);
+    }
+  }
+}
+
+// The pieces of each (row, head) in piece order: the largest maximum, then the sums under it.  A wave a
+// (row, head), D / 64 columns a lane.
+template <bool BF, int D>
+__global__ void __launch_bounds__(256) k_attn_join(PagedArgs a) {
+  constexpr int E = D / 64;
   const int lane = threadIdx.x & 63;
   const long long gw = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int t = (int)(gw / a.H), h = (int)(gw - (long long)t * a.H);
-  if (a.status && gw == 0)
-    for (int i = lane; i < a.S; i += 64)
-      if (!bounds_ok(a, a.cu[i], a.cu[i + 1])) a.status[0] = 1;
   if (t >= a.T) return;
-  int lo = 0, hi = a.S;                         // the first i >= 1 with cu[i] > t, less one
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu[mid] <= t) lo = mid; else hi = mid;
+  int s = 0, n = a.S;                             // the last sequence with cu[s] <= t (64 a step)
+  while (n > 1) {
+    const int step = (n + 63) / 64, i = s + lane * step;
+    const unsigned long long mk = __ballot(i < s + n && a.cu[i] <= t);
+    const int k = mk ? 63 - __builtin_clzll(mk) : 0;
+    n = min(step, s + n - (s + k * step));
+    s += k * step;
   }
-  const int s = lo, c0 = a.cu[s], c1 = a.cu[s + 1];
+  const int c0 = a.cu[s], c1 = a.cu[s + 1];
   if (t < c0 || t >= c1 || !bounds_ok(a, c0, c1)) return;   // a row of no sequence
-  const int hk = h / (a.H / a.Hkv);
   int len = a.lens[s];
-  const long long most = (long long)a.max_blocks * a.page;
-  bool bad = len < 0 || len > most;
-  len = bad ? 0 : len;
-  const int vis = a.causal ? min(len, len - (c1 - c0) + (t - c0) + 1) : len;
-  float q[EPL], acc[EPL], m = -INFINITY, l = 0.f;
-  auto ld = [&](const void* p, size_t i) {
-    if constexpr (BF) return __uint_as_float((unsigned)((const u16*)p)[i] << 16);
-    else return (float)__builtin_bit_cast(_Float16, ((const u16*)p)[i]);
-  };
-  for (int e = 0; e < EPL; ++e) {
-    q[e] = ld(a.q, (size_t)t * a.q_ld + (size_t)h * D + lane * EPL + e);
-    acc[e] = 0.f;
+  if (len < 0 || len > (long long)a.max_blocks * a.page) len = 0;
+  // a piece of the row's tile exists while it starts below what the row itself sees (and the first always)
+  const int vis = seen(a, len, c1 - c0, t - c0);
+  const int np = max(1, min(a.npiece, (vis + a.piece - 1) / a.piece));
+  float m = -INFINITY;
+  for (int p = lane; p < np; p += 64) m = fmaxf(m, a.pml[((size_t)p * a.T + t) * a.H + h].x);
+  m = wave_max(m);
+  float l = 0.f, o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  for (int p = 0; p < np; ++p) {
+    const size_t at = ((size_t)p * a.T + t) * a.H + h;
+    const float2 x = a.pml[at];
+    const float f = x.x == -INFINITY ? (x.y == 0.f ? 0.f : x.y) : __builtin_amdgcn_exp2f(x.x - m);
+    l += x.x == -INFINITY ? x.y : x.y * f;
+    const float* po = a.po + at * D + lane * E;
+    if (x.x != -INFINITY || x.y != 0.f)
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] += po[e] * f;
   }
-  for (int j = 0; j < vis; ++j) {
-    const int b = j / a.page, at = j - b * a.page;
-    const int blk = a.table[(size_t)s * a.table_ld + b];
-    if (blk < 0 || blk >= a.blocks) { bad = true; break; }
-    auto row = [&](const void* c, const uint8_t* ex, long long bs, float (&x)[EPL]) {
-      const size_t i = (size_t)blk * bs + ((size_t)at * a.Hkv + hk) * D + lane * EPL;
-      for (int e = 0; e < EPL; ++e) {
-        if constexpr (F8) {
-          const float sc = __uint_as_float((unsigned)ex[((size_t)blk * a.page + at) * a.Hkv + hk] << 23);
-          const f32x2k v = __builtin_amdgcn_cvt_pk_f32_fp8((int)((const uint8_t*)c)[i + e], false);
-          const unsigned w = pack2<BF>(v[0] * sc, 0.f);
-          x[e] = ld(&w, 0);
-        } else {
-          x[e] = ld(c, i + e);
-        }
-      }
-    };
-    float k[EPL], v[EPL], d = 0.f;
-    row(a.kc, a.ke, a.bs_k, k);
-    row(a.vc, a.ve, a.bs_v, v);
-    for (int e = 0; e < EPL; ++e) d += q[e] * k[e];
-    const float x = wave_sum(d) * a.scale;
-    const float mn = fmaxf(m, x);
-    const float base = mn == -INFINITY ? 0.f : mn;
-    const float w = expf(m - base), p = expf(x - base);
-    l = l * w + p;
-    for (int e = 0; e < EPL; ++e) acc[e] = acc[e] * w + p * v[e];
-    m = mn;
-  }
-  float inv = l == 0.f ? 0.f : 1.f / l, lse = l == 0.f ? -INFINITY : m + logf(l);
-  if (bad) {
-    inv = lse = __builtin_nanf("");
-    if (a.status && lane == 0) a.status[0] = 1;
-  }
-  for (int e = 0; e < EPL; ++e)
-    a.out[(size_t)t * a.o_ld + (size_t)h * D + lane * EPL + e] = (u16)pack2<BF>(acc[e] * inv, 0.f);
-  if (lane == 0) a.lse[(size_t)h * a.T + t] = lse;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  u16* out = a.out + (size_t)t * a.o_ld + (size_t)h * D + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) out[e] = (u16)pack2<BF>(o[e] * inv, 0.f);
+  if (lane == 0) a.lse[(size_t)h * a.T + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
 }
+
+// How a call is split, from what the host knows (sizes and an upper bound of the lengths).
+struct Plan {
+  bool rows, tiles;      // which kernels run
+  int few;               // (both: the rows up to which a sequence is k_attn_rows')
+  int nrow, ntile;       // row-tile slots of each
+  int piece, npiece;
+};
+
+constexpr int TILE_ROWS = 128, FEW_ROWS = 16, PIECE_MIN = 256, FILL = 512;
+
+Plan plan(int T, int H, int Hkv, int S, int max_len) {
+  const int G = H / Hkv;
+  Plan p = {};
+  const long long packed = (long long)T * G;
+  // on average at most one tile of 16 rows a sequence: all sequences are few-row ones
+  p.rows = packed <= (long long)FEW_ROWS * S || packed <= FEW_ROWS;
+  p.tiles = !p.rows;
+  p.few = 0;
+  if (p.tiles && S > 1) {         // some sequences may be few-row ones
+    p.rows = true;
+    p.few = FEW_ROWS;
+  }
+  p.nrow = (int)(packed / FEW_ROWS) + S;
+  p.ntile = (int)(packed / TILE_ROWS) + S;
+  // pieces so that (rows' tiles) x (kv heads) x pieces fill the chip: FILL workgroups, none shorter than
+  // PIECE_MIN tokens
+  const long long items = (long long)Hkv * (p.tiles ? (packed + TILE_ROWS - 1) / TILE_ROWS : S);
+  const long long want = std::max(1ll, (FILL + items - 1) / items);
+  long long piece = ((long long)max_len + want - 1) / want;
+  piece = std::max<long long>(PIECE_MIN, (piece + 63) / 64 * 64);
+  p.npiece = (int)std::max(1ll, ((long long)max_len + piece - 1) / piece);
+  p.piece = (int)std::min<long long>(piece, 0x40000000);
+  return p;
+}
+
+int64_t po_bytes(const Plan& p, int T, int H, int D) { return cfh::align256((size_t)p.npiece * T * H * D * sizeof(float)); }
 
 }  // namespace
 
 extern "C" {
 
 int64_t cfh_paged_attn_ws_bytes(int T, int H, int Hkv, int D, int S, int max_len) {
-  if (T < 0 || H < 1 || Hkv < 1 || H % Hkv || S < 0 || max_len < 0) return -1;
-  return 0;
+  if (T < 0 || H < 1 || Hkv < 1 || H % Hkv || S < 0 || max_len < 0 || D < 1) return -1;
+  if (T == 0 || S == 0) return 0;
+  const Plan p = plan(T, H, Hkv, S, max_len);
+  if (p.npiece == 1) return 0;
+  return po_bytes(p, T, H, D) + (int64_t)cfh::align256((size_t)p.npiece * T * H * sizeof(float2));
 }
 
 int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, int is_bf16, const void* k_cache,
@@ -120,7 +749,9 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
       table_ld < max_blocks || max_len < 0)
     return CFH_E_INVALID;
   if (D != 64 && D != 128 && D != 256) return CFH_E_UNSUPPORTED;
-  if ((long long)blocks * page > 0x7fffffffll || (long long)max_blocks * page > 0x7fffffffll) return CFH_E_UNSUPPORTED;
+  if ((long long)blocks * page > 0x7fffffffll || (long long)max_blocks * page > 0x3fffffffll ||
+      (long long)T * H > 0x3fffffffll || S > 1 << 20)
+    return CFH_E_UNSUPPORTED;
   const bool f8 = k_exp || v_exp;
   if (!k_cache || !v_cache || (f8 && (!k_exp || !v_exp))) return CFH_E_INVALID;
   const long long inner = (long long)page * Hkv * D;
@@ -130,18 +761,53 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
   if (!q || !out || !lse || !seq_lens || !cu_q || (max_blocks && !table) || q_ld < (long long)H * D ||
       o_ld < (long long)H * D || q_ld % 8 || o_ld % 8 || ((uintptr_t)q | (uintptr_t)out) % 16)
     return CFH_E_INVALID;
+  const Plan p = plan(T, H, Hkv, S, max_len);
+  if (p.npiece > 1 && (!ws || (uintptr_t)ws % 256)) return CFH_E_INVALID;
   PagedArgs a = {};
   a.q = (const u16*)q; a.out = (u16*)out; a.lse = lse; a.kc = k_cache; a.vc = v_cache; a.ke = k_exp; a.ve = v_exp;
   a.table = table; a.lens = seq_lens; a.cu = cu_q; a.status = status; a.q_ld = q_ld; a.o_ld = o_ld; a.bs_k = bs_k;
-  a.bs_v = bs_v; a.T = T; a.H = H; a.Hkv = Hkv; a.S = S; a.blocks = blocks; a.page = page; a.table_ld = table_ld;
-  a.max_blocks = max_blocks; a.causal = causal ? 1 : 0; a.scale = scale;
-  const long long waves = (long long)T * H;
-  const dim3 grid((unsigned)((waves + 3) / 4));
+  a.bs_v = bs_v; a.T = T; a.H = H; a.Hkv = Hkv; a.G = H / Hkv; a.S = S; a.blocks = blocks; a.page = page;
+  a.table_ld = table_ld; a.max_blocks = max_blocks; a.causal = causal ? 1 : 0;
+  a.qsign = scale > 0.f ? 1 : scale < 0.f ? -1 : 0;
+  a.c = scale == 0.f ? 1.f : fabsf(scale) * 1.44269504088896340736f;
+  a.po = (float*)ws;
+  a.pml = (float2*)((char*)ws + (p.npiece > 1 ? po_bytes(p, T, H, D) : 0));
+  a.piece = p.piece; a.npiece = p.npiece; a.few = p.few;
+  int l = 0;                                      // ceil(log2(page)): j * floor(2^(31 + l) / page + 1) >> (31 + l)
+  while ((1ll << l) < page) ++l;
+  a.pshift = 31 + l;
+  a.pmagic = (1ull << a.pshift) / (unsigned)page + 1;
   hipStream_t st = (hipStream_t)stream;
-  kv_dispatch(is_bf16, f8, D, [&](auto bf, auto e8, auto d) {
-    hipLaunchKernelGGL((k_paged_rows<bf.value, e8.value, d.value>), grid, dim3(256), 0, st, a);
-  });
-  CFH_LAUNCH_CHECK();
+  const long long groups = (long long)Hkv * p.npiece;
+  auto grid_of = [&](int tiles) {                 // (whole rounds of the XCD mapping)
+    const long long per = 8 % groups == 0 ? 8 / groups : 1;
+    return 8 % groups == 0 ? (tiles + per - 1) / per * 8 : groups * tiles;
+  };
+  if (std::max(grid_of(p.nrow), grid_of(p.ntile)) > 0x7fffffffll) return CFH_E_UNSUPPORTED;
+  if (p.tiles) {
+    a.tiles = p.ntile;
+    const dim3 grid((unsigned)grid_of(p.ntile));
+    kv_dispatch(is_bf16, f8, D, [&](auto bf, auto e8, auto d) {
+      constexpr int TK = d.value == 256 ? 32 : 64;
+      hipLaunchKernelGGL((k_attn_tiles<bf.value, e8.value, d.value, 4, TK>), grid, dim3(256), 0, st, a);
+    });
+    CFH_LAUNCH_CHECK();
+  }
+  if (p.rows) {
+    a.tiles = p.nrow;
+    const dim3 grid((unsigned)grid_of(p.nrow));
+    kv_dispatch(is_bf16, f8, D, [&](auto bf, auto e8, auto d) {
+      hipLaunchKernelGGL((k_attn_rows<bf.value, e8.value, d.value>), grid, dim3(256), 0, st, a);
+    });
+    CFH_LAUNCH_CHECK();
+  }
+  if (p.npiece > 1) {
+    const dim3 grid((unsigned)(((long long)T * H + 3) / 4));
+    kv_dispatch(is_bf16, false, D, [&](auto bf, auto, auto d) {
+      hipLaunchKernelGGL((k_attn_join<bf.value, d.value>), grid, dim3(256), 0, st, a);
+    });
+    CFH_LAUNCH_CHECK();
+  }
   return CFH_OK;
 }
 
