@@ -5,8 +5,23 @@
 //     S = e^g S;  d = beta (v - S k^);  S += d k^T;  o = S q^
 // with k^ = k / sqrt(|k|^2 + 1e-6), q^ = scale q / sqrt(|q|^2 + 1e-6) and S a slot [V][K] of the state.
 // The state is carried in fp32 and rounded to the slot's type once, at the end of the call.
+//
+// Whole chunks (k_gdn_prep, k_gdn_chunks).  Over a chunk of C = 64 rows, with G_i the sum of g up to row i and
+// D_ij = e^(G_i - G_j), the rows' updates d_i solve one triangular system and everything else is products:
+//     (I + L) d = R,   L_ij = beta_i D_ij k^_i.k^_j (j < i),   R_i = beta_i (v_i - e^G_i S k^_i)
+//     o_i = e^G_i S q^_i + sum_(j <= i) D_ij (q^_i.k^_j) d_j,   S = e^G_C S + sum_j D_Cj d_j k^_j^T
+// L and its inverse, and the matrix of the second term, do not depend on S: k_gdn_prep makes them for all
+// chunks at once.  k_gdn_chunks then carries S through the chunks of each (sequence, value head), 16 value
+// columns a workgroup (they do not mix).
+//   Precision: q and k enter MFMA as the bf16 numbers they are, their norms and decays are fp32 factors of the
+// rows; fp32 operands (S, R, d, the two matrices) are split into two bf16 parts, the product of the low parts
+// dropped: 2^-17 of a factor, so that fp32 states keep about 5 digits more than one bf16 product has.
+// Differences of G are taken in 64 bits: a strong decay earlier in the chunk must not cost a weak one later its
+// digits (decays below e^-200 are taken as that: both are 0 in fp32).
 #include "cfh_gdn.h"
 #include "cfh_host.h"
+#include "cfh_kernels.h"
+#include "cfh_tr.h"
 
 namespace {
 
@@ -145,6 +160,437 @@ __global__ void __launch_bounds__(64) k_gdn_rows(GdnSeqArgs a) {
   }
 }
 
+// ---------------------------------------------------------------- whole chunks
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int GC = 64;                             // rows a chunk
+constexpr int GW_FRAG = 4 * 2 * 2 * 64 * 16;       // a matrix [64][64]: [row tile][k-step][hi, lo][lane] 16 B
+constexpr int GW_VEC = 2 * GW_FRAG;                // then the rows' factors: fp32 [4][64] and e^G_C
+constexpr int GW_BYTES = GW_VEC + 4 * GC * 4 + 256;
+
+__device__ __forceinline__ f32x4 mfma_b(const uint4& x, const uint4& y, f32x4 acc) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, x), __builtin_bit_cast(b16x8, y), acc, 0, 0, 0);
+}
+
+// x = hi + lo to 2^-17, both bf16.
+__device__ __forceinline__ void split4(const f32x4& x, uint2& hi, uint2& lo) {
+  hi = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+  lo = make_uint2(pack_bf16(x[0] - __uint_as_float(hi.x << 16), x[1] - __uint_as_float(hi.x & 0xffff0000u)),
+                  pack_bf16(x[2] - __uint_as_float(hi.y << 16), x[3] - __uint_as_float(hi.y & 0xffff0000u)));
+}
+
+// Chunk slots: sequence s has those from floor(cu[s] / 64) + s on, ceil(n / 64) of them used, so no two
+// sequences share one.
+__device__ __forceinline__ int chunk_start(const int* cu, int s) { return cu[s] / GC + s; }
+
+// The order of a contraction over 32 k-slots, element e of lane group g: 16-row MFMA results (row 4 g + r of two
+// tiles, r = e % 4, tile e / 4) are operands as they stand.  The other operand follows it.
+//   slot (g, e) = row 16 (e / 4) + 4 g + e % 4
+
+// L, (I + L)^-1, the attention matrix and the rows' factors of one chunk and value head.  Four waves, a
+// 16-row tile each.
+__global__ void __launch_bounds__(256) k_gdn_prep(GdnSeqArgs a, char* ws) {
+  __shared__ __align__(16) float Ls[GC][GC + 4], Ts[GC][GC + 4];
+  __shared__ __align__(16) float rks[GC], rqs[GC], bts[GC];
+  __shared__ double Gs[GC];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, tl = lane & 15;
+  const int slot = blockIdx.x / a.HV, hv = blockIdx.x % a.HV;
+  int s = 0, cnt = a.S;                            // the last sequence with chunk_start <= slot, 64 a step
+  while (cnt > 1) {
+    const int step = (cnt + 63) / 64, i = s + lane * step;
+    const unsigned long long m = __ballot(i < s + cnt && chunk_start(a.cu, i) <= slot);
+    const int k = m ? 63 - __builtin_clzll(m) : 0;
+    cnt = min(step, s + cnt - (s + k * step));
+    s += k * step;
+  }
+  const int c0 = a.cu[s], c1 = a.cu[s + 1];
+  if (c0 < 0 || c0 > c1 || c1 > a.T) return;
+  const int chunk = slot - chunk_start(a.cu, s);
+  if (chunk < 0 || chunk >= (c1 - c0 + GC - 1) / GC) return;
+  const int t0 = c0 + chunk * GC, n = min(GC, c1 - t0);
+  const int h = hv / (a.HV / a.H);
+  char* const w = ws + ((size_t)slot * a.HV + hv) * GW_BYTES;
+
+  // this lane's share of row tl of each tile: columns 32 ks + 8 g .. + 7, the operand of either side
+  uint4 kf[4][4], qf[4];
+#pragma unroll
+  for (int tile = 0; tile < 4; ++tile) {
+    const int row = 16 * tile + tl;
+    const uint16_t* p = a.qkv + (size_t)(t0 + min(row, n - 1)) * a.ld + ((size_t)a.H + h) * GDN_DK + 8 * g;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      kf[tile][ks] = make_uint4(0, 0, 0, 0);
+      if (tile <= wave) {
+        kf[tile][ks] = *(const uint4*)(p + 32 * ks);
+        if (row >= n) kf[tile][ks] = make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
+  {
+    const int row = 16 * wave + tl;
+    const uint16_t* p = a.qkv + (size_t)(t0 + min(row, n - 1)) * a.ld + (size_t)h * GDN_DK + 8 * g;
+    float kk = 0.f, qq = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      qf[ks] = *(const uint4*)(p + 32 * ks);
+      if (row >= n) qf[ks] = make_uint4(0, 0, 0, 0);
+      // (the wave's own tile of kf: selected without an index that varies)
+      uint4 own = kf[0][ks];
+#pragma unroll
+      for (int tile = 1; tile < 4; ++tile)
+        if (tile == wave) own = kf[tile][ks];
+      auto sq = [](const uint4& r) {
+        float x = 0.f;
+        const unsigned v[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float lo = __uint_as_float(v[e] << 16), hi = __uint_as_float(v[e] & 0xffff0000u);
+          x += lo * lo;
+          x += hi * hi;
+        }
+        return x;
+      };
+      kk += sq(own);
+      qq += sq(qf[ks]);
+    }
+    kk += __shfl_xor(kk, 16); kk += __shfl_xor(kk, 32);
+    qq += __shfl_xor(qq, 16); qq += __shfl_xor(qq, 32);
+    if (lane < 16) {
+      rks[row] = a.l2norm ? 1.0f / sqrtf(kk + 1e-6f) : 1.0f;
+      rqs[row] = a.l2norm ? a.scale / sqrtf(qq + 1e-6f) : a.scale;
+    }
+  }
+  if (wave == 0) {
+    float gl = 0.f, bt = 0.f;
+    if (lane < n) {
+      const size_t m = (size_t)(t0 + lane) * a.HV + hv;
+      seq_gates(bf16f(a.ga[m]) + a.dt_bias[hv], expf(a.A_log[hv]), bf16f(a.gb[m]), gl, bt);
+      gl = gl < -200.f ? -200.f : gl;
+    }
+    double G = gl;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double x = __shfl_up(G, o);
+      if (lane >= o) G += x;
+    }
+    Gs[lane] = G;
+    bts[lane] = bt;
+  }
+  __syncthreads();
+
+  // L into LDS, the attention matrix A kept for later: element (row 16 wave + 4 g + r, column 16 tile + tl)
+  const float4 rk4 = *(const float4*)&rks[16 * wave + 4 * g], rq4 = *(const float4*)&rqs[16 * wave + 4 * g];
+  const float4 bt4 = *(const float4*)&bts[16 * wave + 4 * g];
+  const float rkr[4] = {rk4.x, rk4.y, rk4.z, rk4.w}, rqr[4] = {rq4.x, rq4.y, rq4.z, rq4.w};
+  const float btr[4] = {bt4.x, bt4.y, bt4.z, bt4.w};
+  f32x4 att[4];
+#pragma unroll
+  for (int tile = 0; tile < 4; ++tile) {
+    att[tile] = f32x4{};
+    f32x4 kk = {}, qk = {};
+    if (tile <= wave) {
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        uint4 own = kf[0][ks];
+#pragma unroll
+        for (int x = 1; x < 4; ++x)
+          if (x == wave) own = kf[x][ks];
+        kk = mfma_b(own, kf[tile][ks], kk);
+        qk = mfma_b(qf[ks], kf[tile][ks], qk);
+      }
+      const int j = 16 * tile + tl;
+      const double Gj = Gs[j];
+      const float rkj = rks[j];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = 16 * wave + 4 * g + r;
+        const float d = expf((float)(Gs[i] - Gj));
+        kk[r] = j < i ? btr[r] * d * (rkr[r] * rkj) * kk[r] : 0.f;
+        att[tile][r] = j <= i ? d * (rqr[r] * rkj) * qk[r] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) Ls[16 * wave + 4 * g + r][16 * tile + tl] = kk[r];
+  }
+  if (wave == 0) {
+    // the rows' factors: beta, beta e^G |k|^-1, e^G |q|^-1 scale, e^(G_C - G) |k|^-1
+    float* v = (float*)(w + GW_VEC);
+    const float e = expf((float)Gs[lane]);
+    v[lane] = bts[lane];
+    v[GC + lane] = bts[lane] * e * rks[lane];
+    v[2 * GC + lane] = e * rqs[lane];
+    v[3 * GC + lane] = expf((float)(Gs[GC - 1] - Gs[lane])) * rks[lane];
+    if (lane == 0) v[4 * GC] = expf((float)Gs[GC - 1]);
+  }
+  // the inverse, by 16 x 16 blocks.  Diagonal: column tl by substitution down the rows, in registers (the four
+  // lane groups do the same work)
+  float x[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float d = i == tl ? 1.f : 0.f;
+#pragma unroll
+    for (int l = 0; l < i; ++l) d -= Ls[16 * wave + i][16 * wave + l] * x[l];
+    x[i] = d;
+  }
+  if (g == 0) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) Ts[16 * wave + i][16 * wave + tl] = x[i];
+  }
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+    if (b > wave)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) Ts[16 * wave + 4 * g + r][16 * b + tl] = 0.f;
+  // below it: T_ab = -T_aa sum_(b <= c < a) L_ac T_cb, in fp32 MFMA (16 x 16 x 4: operand lanes tl = row or
+  // column, g = k), block diagonal by block diagonal; the sum's result is the second product's operand as it is
+#pragma unroll
+  for (int d = 1; d < 4; ++d) {
+    __syncthreads();
+    if (wave >= d) {
+      const int b = wave - d;
+      f32x4 m = {}, t = {};
+      for (int c = b; c < wave; ++c)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          m = __builtin_amdgcn_mfma_f32_16x16x4f32(Ls[16 * wave + tl][16 * c + 4 * k + g], Ts[16 * c + 4 * k + g][16 * b + tl], m, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        t = __builtin_amdgcn_mfma_f32_16x16x4f32(Ts[16 * wave + tl][16 * wave + 4 * g + r], m[r], t, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) Ts[16 * wave + 4 * g + r][16 * b + tl] = -t[r];
+    }
+  }
+  __syncthreads();
+  // both matrices as operands, split (A by way of L's place)
+#pragma unroll
+  for (int tile = 0; tile < 4; ++tile)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) Ls[16 * wave + 4 * g + r][16 * tile + tl] = att[tile][r];
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const float(*M)[GC + 4] = m ? Ls : Ts;
+    uint4* out = (uint4*)(w + m * GW_FRAG) + (size_t)wave * 4 * 64 + lane;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      if (ks > wave / 2) break;                     // (the columns past the tile's rows are zero: never read)
+      uint2 h0, l0, h1, l1;
+      split4(*(const f32x4*)&M[16 * wave + tl][32 * ks + 4 * g], h0, l0);
+      split4(*(const f32x4*)&M[16 * wave + tl][32 * ks + 16 + 4 * g], h1, l1);
+      out[(ks * 2) * 64] = make_uint4(h0.x, h0.y, h1.x, h1.y);
+      out[(ks * 2 + 1) * 64] = make_uint4(l0.x, l0.y, l1.x, l1.y);
+    }
+  }
+}
+
+// One chunk's inputs of one lane, loaded while the chunk before it is worked on.
+struct ChunkIn {
+  uint4 k[4];                      // the chunk's K rows for LDS: row tid / 16 + 16 x, columns 8 (tid % 16) ..
+  uint2 q[4][2];                   // row 16 wave + tl of Q, slot order
+  uint4 t[2][2], at[2][2];         // the wave's rows of the two matrices: [k-step][hi, lo]
+  uint16_t v[4];                   // rows 16 wave + 4 g + r, this lane's value column
+  float4 b, cx, cq, ce;            // the rows' factors
+  float eg;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) k_gdn_chunks(GdnSeqArgs a, const char* ws) {
+  __shared__ __align__(16) uint16_t kl[2][GC * GDN_DK];
+  __shared__ __align__(16) uint4 sS[4][2][64];              // S: [k-step = wave][hi, lo][lane]
+  __shared__ __align__(16) uint2 sR[2][2][64][2], sD[2][2][64][2], sE[2][2][64][2];   // [hi, lo][k-step][lane][tile of it]
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, tl = lane & 15;
+  const int nsl = a.V / 16;
+  // the column slices of a (sequence, value head) read the same chunks: on one XCD, whose L2 holds them
+  const int pair = (blockIdx.x / 8 / nsl) * 8 + blockIdx.x % 8, sl = blockIdx.x / 8 % nsl;
+  if (pair >= a.S * a.HV) return;
+  const int s = pair / a.HV, hv = pair % a.HV;
+  const int c0 = a.cu[s], c1 = a.cu[s + 1];
+  const bool rows = c0 >= 0 && c0 <= c1 && c1 <= a.T;
+  const int ok = slot_verdict(a.slots, a.S, s, a.nslots);
+  if (ok == 0) return;
+  if (ok < 0 || !rows) {
+    if (a.status && tid == 0) a.status[0] = 1;
+    if (rows)
+      for (int t = c0 + tid / 16; t < c1; t += 16) a.out[((size_t)t * a.HV + hv) * a.V + sl * 16 + tid % 16] = 0x7fc0;
+    return;
+  }
+  if (c0 == c1) return;
+  const int h = hv / (a.HV / a.H), nc = (c1 - c0 + GC - 1) / GC;
+  const uint16_t* const qb = a.qkv + (size_t)h * GDN_DK;
+  const uint16_t* const kb = qb + (size_t)a.H * GDN_DK;
+  const uint16_t* const vb = a.qkv + 2 * (size_t)a.H * GDN_DK + (size_t)hv * a.V + sl * 16 + tl;
+  const char* const wb = ws + ((size_t)chunk_start(a.cu, s) * a.HV + hv) * GW_BYTES;
+
+  auto load = [&](int c, ChunkIn& in) {
+    const int t0 = c0 + c * GC, n = min(GC, c1 - t0);
+    const char* w = wb + (size_t)c * a.HV * GW_BYTES;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int row = tid / 16 + 16 * x;
+      in.k[x] = *(const uint4*)(kb + (size_t)(t0 + min(row, n - 1)) * a.ld + (tid % 16) * 8);
+      if (row >= n) in.k[x] = make_uint4(0, 0, 0, 0);
+    }
+    const uint16_t* q = qb + (size_t)(t0 + min(16 * wave + tl, n - 1)) * a.ld + 4 * g;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      in.q[ks][0] = *(const uint2*)(q + 32 * ks);
+      in.q[ks][1] = *(const uint2*)(q + 32 * ks + 16);
+    }
+    const uint4* tf = (const uint4*)w + (size_t)wave * 4 * 64 + lane;
+    const uint4* af = (const uint4*)(w + GW_FRAG) + (size_t)wave * 4 * 64 + lane;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const int kk = min(ks, wave / 2);           // (past the tile's rows: loaded again, never used)
+        in.t[ks][p] = tf[(kk * 2 + p) * 64];
+        in.at[ks][p] = af[(kk * 2 + p) * 64];
+      }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = 16 * wave + 4 * g + r;
+      in.v[r] = vb[(size_t)(t0 + min(row, n - 1)) * a.ld];
+      if (row >= n) in.v[r] = 0;
+    }
+    const float* f = (const float*)(w + GW_VEC);
+    in.b = *(const float4*)(f + 16 * wave + 4 * g);
+    in.cx = *(const float4*)(f + GC + 16 * wave + 4 * g);
+    in.cq = *(const float4*)(f + 2 * GC + 16 * wave + 4 * g);
+    in.ce = *(const float4*)(f + 3 * GC + 16 * wave + 4 * g);
+    in.eg = f[4 * GC];
+  };
+  auto stage = [&](const ChunkIn& in, int buf) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int row = tid / 16 + 16 * x;
+      *(uint4*)&kl[buf][row * GDN_DK + (((tid % 16) ^ swz(row)) * 8)] = in.k[x];
+    }
+  };
+
+  // S^T: this wave's k rows 32 wave + 16 u + 4 g + r, value column tl
+  T* const st = (T*)a.state + (((size_t)a.slots[s] * a.HV + hv) * a.V + sl * 16 + tl) * GDN_DK + 32 * wave + 4 * g;
+  f32x4 S[2] = {};
+  if (!a.initial || a.initial[s]) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if constexpr (sizeof(T) == 4) {
+        S[u] = *(const f32x4*)(st + 16 * u);
+      } else {
+        const uint2 x = *(const uint2*)(st + 16 * u);
+        S[u] = f32x4{__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xffff0000u), __uint_as_float(x.y << 16),
+                     __uint_as_float(x.y & 0xffff0000u)};
+      }
+    }
+  }
+
+  auto work = [&](int c, const ChunkIn& in, ChunkIn& next) {
+    const uint16_t* kt = kl[c & 1];
+    const int t0 = c0 + c * GC, n = min(GC, c1 - t0);
+    uint2 h0, l0, h1, l1;
+    split4(S[0], h0, l0);
+    split4(S[1], h1, l1);
+    sS[wave][0][lane] = make_uint4(h0.x, h0.y, h1.x, h1.y);
+    sS[wave][1][lane] = make_uint4(l0.x, l0.y, l1.x, l1.y);
+    if (c + 1 < nc) load(c + 1, next);
+    lds_barrier();
+    // X = K S, Y = Q S for the wave's 16 rows
+    f32x4 X[2] = {}, Y[2] = {};
+    const int row = 16 * wave + tl;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      const int ch = 4 * ks + g / 2, by = 4 * (g & 1);
+      const uint2 ka = *(const uint2*)&kt[row * GDN_DK + ((ch ^ swz(row)) * 8) + by];
+      const uint2 kc = *(const uint2*)&kt[row * GDN_DK + (((ch + 2) ^ swz(row)) * 8) + by];
+      const uint4 kf = make_uint4(ka.x, ka.y, kc.x, kc.y);
+      const uint4 qf = make_uint4(in.q[ks][0].x, in.q[ks][0].y, in.q[ks][1].x, in.q[ks][1].y);
+      const uint4 hi = sS[ks][0][lane], lo = sS[ks][1][lane];
+      X[0] = mfma_b(kf, hi, X[0]);
+      X[1] = mfma_b(kf, lo, X[1]);
+      Y[0] = mfma_b(qf, hi, Y[0]);
+      Y[1] = mfma_b(qf, lo, Y[1]);
+    }
+    const float bb[4] = {in.b.x, in.b.y, in.b.z, in.b.w}, cx[4] = {in.cx.x, in.cx.y, in.cx.z, in.cx.w};
+    const float cq[4] = {in.cq.x, in.cq.y, in.cq.z, in.cq.w}, ce[4] = {in.ce.x, in.ce.y, in.ce.z, in.ce.w};
+    f32x4 R, O;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      R[r] = bb[r] * bf16f(in.v[r]) - cx[r] * (X[0][r] + X[1][r]);
+      O[r] = cq[r] * (Y[0][r] + Y[1][r]);
+    }
+    split4(R, h0, l0);
+    sR[0][wave >> 1][lane][wave & 1] = h0;
+    sR[1][wave >> 1][lane][wave & 1] = l0;
+    lds_barrier();
+    f32x4 d[3] = {};
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      if (ks > wave / 2) break;
+      const uint4 hi = *(const uint4*)sR[0][ks][lane], lo = *(const uint4*)sR[1][ks][lane];
+      d[0] = mfma_b(in.t[ks][0], hi, d[0]);
+      d[1] = mfma_b(in.t[ks][0], lo, d[1]);
+      d[2] = mfma_b(in.t[ks][1], hi, d[2]);
+    }
+    f32x4 D = d[0] + (d[1] + d[2]), E;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) E[r] = D[r] * ce[r];
+    split4(E, h0, l0);
+    split4(D, h1, l1);
+    sE[0][wave >> 1][lane][wave & 1] = h0;
+    sE[1][wave >> 1][lane][wave & 1] = l0;
+    sD[0][wave >> 1][lane][wave & 1] = h1;
+    sD[1][wave >> 1][lane][wave & 1] = l1;
+    lds_barrier();
+    // S: tiles u of the wave's k rows; K's columns as rows by transposed reads
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      f32x4 up[2] = {};
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const int r0 = 32 * ks + 4 * g + tl / 4, r1 = r0 + 16, ch = 4 * wave + 2 * u + (tl & 3) / 2, by = 4 * (tl & 1);
+        const uint2 x = read_tr(&kt[r0 * GDN_DK + ((ch ^ swz(r0)) * 8) + by]);
+        const uint2 y = read_tr(&kt[r1 * GDN_DK + ((ch ^ swz(r1)) * 8) + by]);
+        const uint4 kf = make_uint4(x.x, x.y, y.x, y.y);
+        up[0] = mfma_b(kf, *(const uint4*)sE[0][ks][lane], up[0]);
+        up[1] = mfma_b(kf, *(const uint4*)sE[1][ks][lane], up[1]);
+      }
+      S[u] = S[u] * in.eg + (up[0] + up[1]);
+    }
+    f32x4 o[3] = {};
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      if (ks > wave / 2) break;
+      const uint4 hi = *(const uint4*)sD[0][ks][lane], lo = *(const uint4*)sD[1][ks][lane];
+      o[0] = mfma_b(in.at[ks][0], hi, o[0]);
+      o[1] = mfma_b(in.at[ks][0], lo, o[1]);
+      o[2] = mfma_b(in.at[ks][1], hi, o[2]);
+    }
+    O += o[0] + (o[1] + o[2]);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = 16 * wave + 4 * g + r;
+      if (i < n) a.out[((size_t)(t0 + i) * a.HV + hv) * a.V + sl * 16 + tl] = to_bf16(O[r]);
+    }
+    if (c + 1 < nc) stage(next, (c + 1) & 1);
+  };
+  ChunkIn A, B;
+  load(0, A);
+  stage(A, 0);
+  for (int c = 0; c < nc; c += 2) {
+    work(c, A, B);
+    if (c + 1 < nc) work(c + 1, B, A);
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    if constexpr (sizeof(T) == 4) *(f32x4*)(st + 16 * u) = S[u];
+    else *(uint2*)(st + 16 * u) = make_uint2(pack_bf16(S[u][0], S[u][1]), pack_bf16(S[u][2], S[u][3]));
+  }
+}
+
+// Rows a sequence, on average, up to which they go one after another (k_gdn_rows).
+constexpr int GDN_ROWS_MAX = 8;
+
+inline long long chunk_slots(int T, int S) { return (long long)T / GC + S; }
+
 constexpr int GDN_SEQS = 4096;   // sequences a call (every wave looks for its slot among theirs)
 
 int seq_args(GdnSeqArgs& g, const void* mixed_qkv, const void* a, const void* b, const float* A_log,
@@ -188,7 +634,7 @@ int cfh_gdn_decode(const void* mixed_qkv, const void* a, const void* b, const fl
 
 int64_t cfh_gdn_prefill_ws_bytes(int T, int S, int HV) {
   if (T < 0 || S < 0 || HV < 1) return -1;
-  return 0;
+  return (long long)T <= (long long)GDN_ROWS_MAX * S ? 0 : chunk_slots(T, S) * HV * GW_BYTES;
 }
 
 int cfh_gdn_prefill(const void* mixed_qkv, const void* a, const void* b, const float* A_log, const float* dt_bias,
@@ -203,7 +649,17 @@ int cfh_gdn_prefill(const void* mixed_qkv, const void* a, const void* b, const f
   if (!cu_seqlens) return CFH_E_INVALID;
   g.cu = cu_seqlens;
   g.initial = initial;
-  return launch_rows(g, state_bf16, (hipStream_t)stream);
+  hipStream_t st = (hipStream_t)stream;
+  if ((long long)T <= (long long)GDN_ROWS_MAX * S) return launch_rows(g, state_bf16, st);
+  if (!ws || (uintptr_t)ws % 256) return CFH_E_INVALID;
+  const long long prep = chunk_slots(T, S) * HV, blocks = ((long long)S * HV + 7) / 8 * 8 * (V / 16);
+  if (prep > 0x7fffffffll || blocks > 0x7fffffffll) return CFH_E_UNSUPPORTED;
+  hipLaunchKernelGGL(k_gdn_prep, dim3((unsigned)prep), dim3(256), 0, st, g, (char*)ws);
+  CFH_LAUNCH_CHECK();
+  if (state_bf16) hipLaunchKernelGGL(k_gdn_chunks<uint16_t>, dim3((unsigned)blocks), dim3(256), 0, st, g, (const char*)ws);
+  else hipLaunchKernelGGL(k_gdn_chunks<float>, dim3((unsigned)blocks), dim3(256), 0, st, g, (const char*)ws);
+  CFH_LAUNCH_CHECK();
+  return CFH_OK;
 }
 
 }  // extern "C"

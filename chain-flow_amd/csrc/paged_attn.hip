@@ -19,11 +19,11 @@
 // then merges the pieces' (max, sum, O).
 #include "cfh_host.h"
 #include "cfh_kv.h"
+#include "cfh_tr.h"
 
 namespace {
 
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
@@ -176,18 +176,6 @@ __device__ __forceinline__ f32x16 mfma32(const uint4& x, const uint4& y, f32x16 
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h16x8, x), __builtin_bit_cast(h16x8, y), acc, 0, 0, 0);
 }
-
-// Four elements of one column from four rows of 16-lane blocks in LDS (lane l of a block points at row l / 4,
-// columns 4 (l % 4) .. + 3 and receives column l of rows 0 .. 3).
-__device__ __forceinline__ uint2 read_tr(const u16* p) {
-  typedef __attribute__((address_space(3))) s16x4* lptr;
-  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)p));
-}
-
-// 16-byte chunk order within a token's row in LDS: chunk c of token t lies at c ^ swz(t).  Eight tokens with
-// one chunk (K's operand reads), and four tokens with two neighbouring chunks (V's transposed reads), each
-// cover all 128 bytes of the banks.
-__device__ __forceinline__ int swz(int t) { return ((t & 3) << 1) | ((t >> 2) & 1); }
 
 __device__ __forceinline__ float swap_max(float x) {
   const u32x2 s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
