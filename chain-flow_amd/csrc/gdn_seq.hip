@@ -14,8 +14,8 @@
 // chunks at once.  k_gdn_chunks then carries S through the chunks of each (sequence, value head), 16 value
 // columns a workgroup (they do not mix).
 //   Precision: q and k enter MFMA as the bf16 numbers they are, their norms and decays are fp32 factors of the
-// rows; fp32 operands (S, R, d, the two matrices) are split into two bf16 parts, the product of the low parts
-// dropped: 2^-17 of a factor, so that fp32 states keep about 5 digits more than one bf16 product has.
+// rows; fp32 operands on the way to the state (S, R, d, the inverse) are split into three bf16 parts, products
+// below 2^-24 dropped, so that fp32 states keep fp32 digits; what only the bf16 output sees into two (2^-17).
 // Differences of G are taken in 64 bits: a strong decay earlier in the chunk must not cost a weak one later its
 // digits (decays below e^-200 are taken as that: both are 0 in fp32).
 #include "cfh_gdn.h"
@@ -164,8 +164,9 @@ __global__ void __launch_bounds__(64) k_gdn_rows(GdnSeqArgs a) {
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int GC = 64;                             // rows a chunk
-constexpr int GW_FRAG = 4 * 2 * 2 * 64 * 16;       // a matrix [64][64]: [row tile][k-step][hi, lo][lane] 16 B
-constexpr int GW_VEC = 2 * GW_FRAG;                // then the rows' factors: fp32 [4][64] and e^G_C
+// a chunk and value head's place in the workspace: the inverse in three parts and the attention matrix in two,
+// [row tile][k-step][part][lane] 16 B each; then the rows' factors, fp32 [4][64], and e^G_C
+constexpr int GW_ATT = 4 * 2 * 3 * 64 * 16, GW_VEC = GW_ATT + 4 * 2 * 2 * 64 * 16;
 constexpr int GW_BYTES = GW_VEC + 4 * GC * 4 + 256;
 
 __device__ __forceinline__ f32x4 mfma_b(const uint4& x, const uint4& y, f32x4 acc) {
@@ -177,6 +178,19 @@ __device__ __forceinline__ void split4(const f32x4& x, uint2& hi, uint2& lo) {
   hi = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
   lo = make_uint2(pack_bf16(x[0] - __uint_as_float(hi.x << 16), x[1] - __uint_as_float(hi.x & 0xffff0000u)),
                   pack_bf16(x[2] - __uint_as_float(hi.y << 16), x[3] - __uint_as_float(hi.y & 0xffff0000u)));
+}
+
+// x = hi + mid + lo to 2^-25, all bf16.
+__device__ __forceinline__ void split4(const f32x4& x, uint2 (&p)[3]) {
+  f32x4 r = x;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    p[i] = make_uint2(pack_bf16(r[0], r[1]), pack_bf16(r[2], r[3]));
+    if (i < 2) {
+      r[0] -= __uint_as_float(p[i].x << 16); r[1] -= __uint_as_float(p[i].x & 0xffff0000u);
+      r[2] -= __uint_as_float(p[i].y << 16); r[3] -= __uint_as_float(p[i].y & 0xffff0000u);
+    }
+  }
 }
 
 // Chunk slots: sequence s has those from floor(cu[s] / 64) + s on, ceil(n / 64) of them used, so no two
@@ -193,7 +207,7 @@ __global__ void __launch_bounds__(256) k_gdn_prep(GdnSeqArgs a, char* ws) {
   __shared__ __align__(16) float Ls[GC][GC + 4], Ts[GC][GC + 4];
   __shared__ __align__(16) float rks[GC], rqs[GC], bts[GC];
   __shared__ double Gs[GC];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, tl = lane & 15;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, tl = lane & 15;
   const int slot = blockIdx.x / a.HV, hv = blockIdx.x % a.HV;
   int s = 0, cnt = a.S;                            // the last sequence with chunk_start <= slot, 64 a step
   while (cnt > 1) {
@@ -361,44 +375,54 @@ __global__ void __launch_bounds__(256) k_gdn_prep(GdnSeqArgs a, char* ws) {
     }
   }
   __syncthreads();
-  // both matrices as operands, split (A by way of L's place)
+  // both matrices as operands, split (A by way of L's place); columns past the tile's rows are zero, never read
 #pragma unroll
   for (int tile = 0; tile < 4; ++tile)
 #pragma unroll
     for (int r = 0; r < 4; ++r) Ls[16 * wave + 4 * g + r][16 * tile + tl] = att[tile][r];
   __syncthreads();
+  uint4* const tf = (uint4*)w + (size_t)wave * 6 * 64 + lane;
+  uint4* const af = (uint4*)(w + GW_ATT) + (size_t)wave * 4 * 64 + lane;
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    const float(*M)[GC + 4] = m ? Ls : Ts;
-    uint4* out = (uint4*)(w + m * GW_FRAG) + (size_t)wave * 4 * 64 + lane;
+  for (int ks = 0; ks < 2; ++ks) {
+    if (ks > wave / 2) break;
+    uint2 p0[3], p1[3], h0, l0, h1, l1;
+    split4(*(const f32x4*)&Ts[16 * wave + tl][32 * ks + 4 * g], p0);
+    split4(*(const f32x4*)&Ts[16 * wave + tl][32 * ks + 16 + 4 * g], p1);
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      if (ks > wave / 2) break;                     // (the columns past the tile's rows are zero: never read)
-      uint2 h0, l0, h1, l1;
-      split4(*(const f32x4*)&M[16 * wave + tl][32 * ks + 4 * g], h0, l0);
-      split4(*(const f32x4*)&M[16 * wave + tl][32 * ks + 16 + 4 * g], h1, l1);
-      out[(ks * 2) * 64] = make_uint4(h0.x, h0.y, h1.x, h1.y);
-      out[(ks * 2 + 1) * 64] = make_uint4(l0.x, l0.y, l1.x, l1.y);
-    }
+    for (int p = 0; p < 3; ++p) tf[(ks * 3 + p) * 64] = make_uint4(p0[p].x, p0[p].y, p1[p].x, p1[p].y);
+    split4(*(const f32x4*)&Ls[16 * wave + tl][32 * ks + 4 * g], h0, l0);
+    split4(*(const f32x4*)&Ls[16 * wave + tl][32 * ks + 16 + 4 * g], h1, l1);
+    af[(ks * 2) * 64] = make_uint4(h0.x, h0.y, h1.x, h1.y);
+    af[(ks * 2 + 1) * 64] = make_uint4(l0.x, l0.y, l1.x, l1.y);
   }
 }
 
-// One chunk's inputs of one lane, loaded while the chunk before it is worked on.
-struct ChunkIn {
-  uint4 k[4];                      // the chunk's K rows for LDS: row tid / 16 + 16 x, columns 8 (tid % 16) ..
-  uint2 q[4][2];                   // row 16 wave + tl of Q, slot order
-  uint4 t[2][2], at[2][2];         // the wave's rows of the two matrices: [k-step][hi, lo]
-  uint16_t v[4];                   // rows 16 wave + 4 g + r, this lane's value column
-  float4 b, cx, cq, ce;            // the rows' factors
+// S through the chunks of one (sequence, value head), 16 value columns, in a chain that no other workgroup can
+// shorten: what counts is the time from one chunk's S to the next one's.  Waves 0 - 3 carry the chain (a 16-row
+// tile of the chunk each, and 32 k rows of S), waves 4 - 7 compute the outputs and stage K beside it.  Three
+// barriers a chunk: S published, R published, d published.  Inputs come a chunk ahead.
+// Rows of S in a wave's MFMA tiles: tile u, row 4 g + r is k row 32 wave + 8 g + 4 u + r, so that the two tiles
+// of a lane make eight neighbouring k rows, the natural operand order of K and Q.
+struct ChainIn {                   // a lane of a chain wave, one chunk
+  uint4 t[2][3];                   // its rows of the inverse: [k-step][part]
+  uint2 v;                         // 4 columns of row 16 wave + lane / 4 (to LDS and back transposed)
+  float4 b, cx, ce;                // factors of rows 16 wave + 4 g + r
   float eg;
+};
+struct OutIn {                     // a lane of an output wave
+  uint4 q[4], at[2][2];            // row 16 wave + tl of Q; its rows of the attention matrix
+  float4 cq;
 };
 
 template <typename T>
-__global__ void __launch_bounds__(256) k_gdn_chunks(GdnSeqArgs a, const char* ws) {
-  __shared__ __align__(16) uint16_t kl[2][GC * GDN_DK];
-  __shared__ __align__(16) uint4 sS[4][2][64];              // S: [k-step = wave][hi, lo][lane]
-  __shared__ __align__(16) uint2 sR[2][2][64][2], sD[2][2][64][2], sE[2][2][64][2];   // [hi, lo][k-step][lane][tile of it]
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, tl = lane & 15;
+__global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws) {
+  __shared__ __align__(16) uint16_t kl[2][GC * GDN_DK];     // K, chunks of 16 bytes in swz order
+  __shared__ __align__(16) uint4 sS[4][3][64];              // S: [k-step = wave][part][lane]
+  __shared__ __align__(16) uint2 sR[3][2][64][2], sE[3][2][64][2], sD[2][2][64][2];   // [part][k-step][lane][tile of it]
+  __shared__ __align__(16) uint2 sV[4][64];
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, tl = lane & 15;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), wave = wv & 3;
   const int nsl = a.V / 16;
   // the column slices of a (sequence, value head) read the same chunks: on one XCD, whose L2 holds them
   const int pair = (blockIdx.x / 8 / nsl) * 8 + blockIdx.x % 8, sl = blockIdx.x / 8 % nsl;
@@ -411,178 +435,210 @@ __global__ void __launch_bounds__(256) k_gdn_chunks(GdnSeqArgs a, const char* ws
   if (ok < 0 || !rows) {
     if (a.status && tid == 0) a.status[0] = 1;
     if (rows)
-      for (int t = c0 + tid / 16; t < c1; t += 16) a.out[((size_t)t * a.HV + hv) * a.V + sl * 16 + tid % 16] = 0x7fc0;
+      for (int t = c0 + tid / 16; t < c1; t += 32) a.out[((size_t)t * a.HV + hv) * a.V + sl * 16 + tid % 16] = 0x7fc0;
     return;
   }
   if (c0 == c1) return;
   const int h = hv / (a.HV / a.H), nc = (c1 - c0 + GC - 1) / GC;
   const uint16_t* const qb = a.qkv + (size_t)h * GDN_DK;
   const uint16_t* const kb = qb + (size_t)a.H * GDN_DK;
-  const uint16_t* const vb = a.qkv + 2 * (size_t)a.H * GDN_DK + (size_t)hv * a.V + sl * 16 + tl;
+  const uint16_t* const vb = a.qkv + 2 * (size_t)a.H * GDN_DK + (size_t)hv * a.V + sl * 16;
   const char* const wb = ws + ((size_t)chunk_start(a.cu, s) * a.HV + hv) * GW_BYTES;
+  auto place = [&](int c) { return wb + (size_t)c * a.HV * GW_BYTES; };
+  // Loads of a chunk past the last one load the last one again: behind a branch the compiler would count them
+  // as perhaps not issued, and a wait for an older load would become a wait for these.  For the same reason
+  // rows behind the sequence are cleared where they are used.
 
-  auto load = [&](int c, ChunkIn& in) {
-    const int t0 = c0 + c * GC, n = min(GC, c1 - t0);
-    const char* w = wb + (size_t)c * a.HV * GW_BYTES;
+  if (wv >= 4) {
+    uint4 kr[4];
+    auto load_k = [&](int c) {
+      const int t0 = c0 + c * GC, n = min(GC, c1 - t0);
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int row = tid / 16 + 16 * x;
-      in.k[x] = *(const uint4*)(kb + (size_t)(t0 + min(row, n - 1)) * a.ld + (tid % 16) * 8);
-      if (row >= n) in.k[x] = make_uint4(0, 0, 0, 0);
-    }
-    const uint16_t* q = qb + (size_t)(t0 + min(16 * wave + tl, n - 1)) * a.ld + 4 * g;
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      in.q[ks][0] = *(const uint2*)(q + 32 * ks);
-      in.q[ks][1] = *(const uint2*)(q + 32 * ks + 16);
-    }
-    const uint4* tf = (const uint4*)w + (size_t)wave * 4 * 64 + lane;
-    const uint4* af = (const uint4*)(w + GW_FRAG) + (size_t)wave * 4 * 64 + lane;
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const int kk = min(ks, wave / 2);           // (past the tile's rows: loaded again, never used)
-        in.t[ks][p] = tf[(kk * 2 + p) * 64];
-        in.at[ks][p] = af[(kk * 2 + p) * 64];
+      for (int x = 0; x < 4; ++x) {
+        const int row = 16 * x + (tid - 256) / 16;
+        kr[x] = *(const uint4*)(kb + (size_t)(t0 + min(row, n - 1)) * a.ld + (tid % 16) * 8);
       }
+    };
+    auto stage_k = [&](int c) {
+      const int n = c1 - c0 - c * GC;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = 16 * wave + 4 * g + r;
-      in.v[r] = vb[(size_t)(t0 + min(row, n - 1)) * a.ld];
-      if (row >= n) in.v[r] = 0;
-    }
-    const float* f = (const float*)(w + GW_VEC);
-    in.b = *(const float4*)(f + 16 * wave + 4 * g);
-    in.cx = *(const float4*)(f + GC + 16 * wave + 4 * g);
-    in.cq = *(const float4*)(f + 2 * GC + 16 * wave + 4 * g);
-    in.ce = *(const float4*)(f + 3 * GC + 16 * wave + 4 * g);
-    in.eg = f[4 * GC];
-  };
-  auto stage = [&](const ChunkIn& in, int buf) {
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int row = tid / 16 + 16 * x;
-      *(uint4*)&kl[buf][row * GDN_DK + (((tid % 16) ^ swz(row)) * 8)] = in.k[x];
-    }
-  };
-
-  // S^T: this wave's k rows 32 wave + 16 u + 4 g + r, value column tl
-  T* const st = (T*)a.state + (((size_t)a.slots[s] * a.HV + hv) * a.V + sl * 16 + tl) * GDN_DK + 32 * wave + 4 * g;
-  f32x4 S[2] = {};
-  if (!a.initial || a.initial[s]) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if constexpr (sizeof(T) == 4) {
-        S[u] = *(const f32x4*)(st + 16 * u);
-      } else {
-        const uint2 x = *(const uint2*)(st + 16 * u);
-        S[u] = f32x4{__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xffff0000u), __uint_as_float(x.y << 16),
-                     __uint_as_float(x.y & 0xffff0000u)};
+      for (int x = 0; x < 4; ++x) {
+        const int row = 16 * x + (tid - 256) / 16;
+        *(uint4*)&kl[c & 1][row * GDN_DK + (((tid % 16) ^ swz(row)) * 8)] = row < n ? kr[x] : make_uint4(0, 0, 0, 0);
       }
+    };
+    auto load = [&](int c, OutIn& in) {
+      const int t0 = c0 + c * GC, n = min(GC, c1 - t0);
+      const uint16_t* q = qb + (size_t)(t0 + min(16 * wave + tl, n - 1)) * a.ld + 8 * g;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) in.q[ks] = *(const uint4*)(q + 32 * ks);
+      const uint4* af = (const uint4*)(place(c) + GW_ATT) + (size_t)wave * 4 * 64 + lane;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) in.at[ks][p] = af[(min(ks, wave / 2) * 2 + p) * 64];
+      in.cq = *(const float4*)((const float*)(place(c) + GW_VEC) + 2 * GC + 16 * wave + 4 * g);
+    };
+    auto work = [&](int c, const OutIn& in, OutIn& next) {
+      const int t0 = c0 + c * GC, n = min(GC, c1 - t0);
+      lds_barrier();                                         // S is there
+      load_k(min(c + 1, nc - 1));
+      f32x4 Y[2] = {};
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        Y[0] = mfma_b(in.q[ks], sS[ks][0][lane], Y[0]);
+        Y[1] = mfma_b(in.q[ks], sS[ks][1][lane], Y[1]);
+      }
+      lds_barrier();                                         // R is there
+      load(min(c + 1, nc - 1), next);
+      stage_k(min(c + 1, nc - 1));
+      lds_barrier();                                         // d is there
+      f32x4 o[3] = {};
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        if (ks > wave / 2) break;
+        const uint4 hi = *(const uint4*)sD[0][ks][lane], lo = *(const uint4*)sD[1][ks][lane];
+        o[0] = mfma_b(in.at[ks][0], hi, o[0]);
+        o[1] = mfma_b(in.at[ks][0], lo, o[1]);
+        o[2] = mfma_b(in.at[ks][1], hi, o[2]);
+      }
+      const float cq[4] = {in.cq.x, in.cq.y, in.cq.z, in.cq.w};
+      uint16_t* out = a.out + ((size_t)(t0 + 16 * wave + 4 * g) * a.HV + hv) * a.V + sl * 16 + tl;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (16 * wave + 4 * g + r < n)
+          out[(size_t)r * a.HV * a.V] = to_bf16(cq[r] * (Y[0][r] + Y[1][r]) + (o[0][r] + (o[1][r] + o[2][r])));
+    };
+    OutIn A, B;
+    load_k(0);
+    load(0, A);
+    stage_k(0);
+    for (int c = 0;;) {
+      work(c, A, B);
+      if (++c >= nc) return;
+      work(c, B, A);
+      if (++c >= nc) return;
     }
   }
 
-  auto work = [&](int c, const ChunkIn& in, ChunkIn& next) {
-    const uint16_t* kt = kl[c & 1];
+  auto load = [&](int c, ChainIn& in) {
     const int t0 = c0 + c * GC, n = min(GC, c1 - t0);
-    uint2 h0, l0, h1, l1;
-    split4(S[0], h0, l0);
-    split4(S[1], h1, l1);
-    sS[wave][0][lane] = make_uint4(h0.x, h0.y, h1.x, h1.y);
-    sS[wave][1][lane] = make_uint4(l0.x, l0.y, l1.x, l1.y);
-    if (c + 1 < nc) load(c + 1, next);
-    lds_barrier();
-    // X = K S, Y = Q S for the wave's 16 rows
-    f32x4 X[2] = {}, Y[2] = {};
-    const int row = 16 * wave + tl;
+    const uint4* tf = (const uint4*)place(c) + (size_t)wave * 6 * 64 + lane;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int p = 0; p < 3; ++p) in.t[ks][p] = tf[(min(ks, wave / 2) * 3 + p) * 64];
+    in.v = *(const uint2*)(vb + (size_t)(t0 + min(16 * wave + lane / 4, n - 1)) * a.ld + 4 * (lane & 3));
+    const float* f = (const float*)(place(c) + GW_VEC) + 16 * wave + 4 * g;
+    in.b = *(const float4*)f;
+    in.cx = *(const float4*)(f + GC);
+    in.ce = *(const float4*)(f + 3 * GC);
+    in.eg = *((const float*)(place(c) + GW_VEC) + 4 * GC);
+  };
+  T* const st = (T*)a.state + (((size_t)a.slots[s] * a.HV + hv) * a.V + sl * 16 + tl) * GDN_DK + 32 * wave + 8 * g;
+  f32x4 S[2] = {};
+  if (!a.initial || a.initial[s]) {
+    if constexpr (sizeof(T) == 4) {
+      S[0] = *(const f32x4*)st;
+      S[1] = *(const f32x4*)(st + 4);
+    } else {
+      const uint4 x = *(const uint4*)st;
+      S[0] = f32x4{__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xffff0000u), __uint_as_float(x.y << 16),
+                   __uint_as_float(x.y & 0xffff0000u)};
+      S[1] = f32x4{__uint_as_float(x.z << 16), __uint_as_float(x.z & 0xffff0000u), __uint_as_float(x.w << 16),
+                   __uint_as_float(x.w & 0xffff0000u)};
+    }
+  }
+  auto work = [&](int c, const ChainIn& in, ChainIn& next) {
+    const uint16_t* kt = kl[c & 1];
+    const int n = c1 - c0 - c * GC, row = 16 * wave + tl;
+    uint2 p0[3], p1[3];
+    split4(S[0], p0);
+    split4(S[1], p1);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) sS[wave][p][lane] = make_uint4(p0[p].x, p0[p].y, p1[p].x, p1[p].y);
+    sV[wave][lane] = 16 * wave + lane / 4 < n ? in.v : make_uint2(0, 0);
+    lds_barrier();                                           // S is there, and K
+    f32x4 X[3] = {};
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      const int ch = 4 * ks + g / 2, by = 4 * (g & 1);
-      const uint2 ka = *(const uint2*)&kt[row * GDN_DK + ((ch ^ swz(row)) * 8) + by];
-      const uint2 kc = *(const uint2*)&kt[row * GDN_DK + (((ch + 2) ^ swz(row)) * 8) + by];
-      const uint4 kf = make_uint4(ka.x, ka.y, kc.x, kc.y);
-      const uint4 qf = make_uint4(in.q[ks][0].x, in.q[ks][0].y, in.q[ks][1].x, in.q[ks][1].y);
-      const uint4 hi = sS[ks][0][lane], lo = sS[ks][1][lane];
-      X[0] = mfma_b(kf, hi, X[0]);
-      X[1] = mfma_b(kf, lo, X[1]);
-      Y[0] = mfma_b(qf, hi, Y[0]);
-      Y[1] = mfma_b(qf, lo, Y[1]);
-    }
-    const float bb[4] = {in.b.x, in.b.y, in.b.z, in.b.w}, cx[4] = {in.cx.x, in.cx.y, in.cx.z, in.cx.w};
-    const float cq[4] = {in.cq.x, in.cq.y, in.cq.z, in.cq.w}, ce[4] = {in.ce.x, in.ce.y, in.ce.z, in.ce.w};
-    f32x4 R, O;
+      const uint4 kf = *(const uint4*)&kt[row * GDN_DK + (((4 * ks + g) ^ swz(row)) * 8)];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      R[r] = bb[r] * bf16f(in.v[r]) - cx[r] * (X[0][r] + X[1][r]);
-      O[r] = cq[r] * (Y[0][r] + Y[1][r]);
+      for (int p = 0; p < 3; ++p) X[p] = mfma_b(kf, sS[ks][p][lane], X[p]);
     }
-    split4(R, h0, l0);
-    sR[0][wave >> 1][lane][wave & 1] = h0;
-    sR[1][wave >> 1][lane][wave & 1] = l0;
-    lds_barrier();
+    // (the wave's own sV: in order behind its write) rows 4 g .. 4 g + 3 of its tile, column tl
+    const uint2 vv = read_tr((const uint16_t*)&sV[wave][16 * g] + 4 * tl);
+    load(min(c + 1, nc - 1), next);
+    const float bb[4] = {in.b.x, in.b.y, in.b.z, in.b.w}, cx[4] = {in.cx.x, in.cx.y, in.cx.z, in.cx.w};
+    const float ce[4] = {in.ce.x, in.ce.y, in.ce.z, in.ce.w};
+    const float v[4] = {__uint_as_float(vv.x << 16), __uint_as_float(vv.x & 0xffff0000u), __uint_as_float(vv.y << 16),
+                        __uint_as_float(vv.y & 0xffff0000u)};
+    f32x4 R;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) R[r] = bb[r] * v[r] - cx[r] * (X[0][r] + (X[1][r] + X[2][r]));
+    split4(R, p0);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) sR[p][wave >> 1][lane][wave & 1] = p0[p];
+    lds_barrier();                                           // R is there
     f32x4 d[3] = {};
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       if (ks > wave / 2) break;
-      const uint4 hi = *(const uint4*)sR[0][ks][lane], lo = *(const uint4*)sR[1][ks][lane];
-      d[0] = mfma_b(in.t[ks][0], hi, d[0]);
-      d[1] = mfma_b(in.t[ks][0], lo, d[1]);
-      d[2] = mfma_b(in.t[ks][1], hi, d[2]);
+      uint4 x[3];
+#pragma unroll
+      for (int p = 0; p < 3; ++p) x[p] = *(const uint4*)sR[p][ks][lane];
+      d[0] = mfma_b(in.t[ks][0], x[0], d[0]);
+      d[1] = mfma_b(in.t[ks][0], x[1], d[1]);
+      d[2] = mfma_b(in.t[ks][1], x[0], d[2]);
+      d[1] = mfma_b(in.t[ks][1], x[1], d[1]);
+      d[2] = mfma_b(in.t[ks][0], x[2], d[2]);
+      d[1] = mfma_b(in.t[ks][2], x[0], d[1]);
     }
-    f32x4 D = d[0] + (d[1] + d[2]), E;
+    const f32x4 D = d[0] + (d[1] + d[2]);
+    f32x4 E;
 #pragma unroll
     for (int r = 0; r < 4; ++r) E[r] = D[r] * ce[r];
-    split4(E, h0, l0);
-    split4(D, h1, l1);
-    sE[0][wave >> 1][lane][wave & 1] = h0;
-    sE[1][wave >> 1][lane][wave & 1] = l0;
-    sD[0][wave >> 1][lane][wave & 1] = h1;
-    sD[1][wave >> 1][lane][wave & 1] = l1;
-    lds_barrier();
-    // S: tiles u of the wave's k rows; K's columns as rows by transposed reads
+    split4(E, p0);
+    split4(D, p1[0], p1[1]);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      f32x4 up[2] = {};
+    for (int p = 0; p < 3; ++p) sE[p][wave >> 1][lane][wave & 1] = p0[p];
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        const int r0 = 32 * ks + 4 * g + tl / 4, r1 = r0 + 16, ch = 4 * wave + 2 * u + (tl & 3) / 2, by = 4 * (tl & 1);
-        const uint2 x = read_tr(&kt[r0 * GDN_DK + ((ch ^ swz(r0)) * 8) + by]);
-        const uint2 y = read_tr(&kt[r1 * GDN_DK + ((ch ^ swz(r1)) * 8) + by]);
-        const uint4 kf = make_uint4(x.x, x.y, y.x, y.y);
-        up[0] = mfma_b(kf, *(const uint4*)sE[0][ks][lane], up[0]);
-        up[1] = mfma_b(kf, *(const uint4*)sE[1][ks][lane], up[1]);
-      }
-      S[u] = S[u] * in.eg + (up[0] + up[1]);
-    }
-    f32x4 o[3] = {};
+    for (int p = 0; p < 2; ++p) sD[p][wave >> 1][lane][wave & 1] = p1[p];
+    lds_barrier();                                           // d is there
+    // S: K's columns as rows by transposed reads
+    f32x4 up[2][3] = {};
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      if (ks > wave / 2) break;
-      const uint4 hi = *(const uint4*)sD[0][ks][lane], lo = *(const uint4*)sD[1][ks][lane];
-      o[0] = mfma_b(in.at[ks][0], hi, o[0]);
-      o[1] = mfma_b(in.at[ks][0], lo, o[1]);
-      o[2] = mfma_b(in.at[ks][1], hi, o[2]);
-    }
-    O += o[0] + (o[1] + o[2]);
+      uint4 x[3];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = 16 * wave + 4 * g + r;
-      if (i < n) a.out[((size_t)(t0 + i) * a.HV + hv) * a.V + sl * 16 + tl] = to_bf16(O[r]);
+      for (int p = 0; p < 3; ++p) x[p] = *(const uint4*)sE[p][ks][lane];
+      const int r0 = 32 * ks + 4 * g + tl / 4, r1 = r0 + 16, ch = 4 * wave + (tl & 3);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint2 y = read_tr(&kt[r0 * GDN_DK + ((ch ^ swz(r0)) * 8) + 4 * u]);
+        const uint2 z = read_tr(&kt[r1 * GDN_DK + ((ch ^ swz(r1)) * 8) + 4 * u]);
+        const uint4 kf = make_uint4(y.x, y.y, z.x, z.y);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) up[u][p] = mfma_b(kf, x[p], up[u][p]);
+      }
     }
-    if (c + 1 < nc) stage(next, (c + 1) & 1);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) S[u] = S[u] * in.eg + (up[u][0] + (up[u][1] + up[u][2]));
   };
-  ChunkIn A, B;
+  ChainIn A, B;
   load(0, A);
-  stage(A, 0);
-  for (int c = 0; c < nc; c += 2) {
+  for (int c = 0;;) {
     work(c, A, B);
-    if (c + 1 < nc) work(c + 1, B, A);
+    if (++c >= nc) break;
+    work(c, B, A);
+    if (++c >= nc) break;
   }
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    if constexpr (sizeof(T) == 4) *(f32x4*)(st + 16 * u) = S[u];
-    else *(uint2*)(st + 16 * u) = make_uint2(pack_bf16(S[u][0], S[u][1]), pack_bf16(S[u][2], S[u][3]));
+  if constexpr (sizeof(T) == 4) {
+    *(f32x4*)st = S[0];
+    *(f32x4*)(st + 4) = S[1];
+  } else {
+    *(uint4*)st = make_uint4(pack_bf16(S[0][0], S[0][1]), pack_bf16(S[0][2], S[0][3]), pack_bf16(S[1][0], S[1][1]),
+                             pack_bf16(S[1][2], S[1][3]));
   }
 }
 
@@ -656,8 +712,8 @@ int cfh_gdn_prefill(const void* mixed_qkv, const void* a, const void* b, const f
   if (prep > 0x7fffffffll || blocks > 0x7fffffffll) return CFH_E_UNSUPPORTED;
   hipLaunchKernelGGL(k_gdn_prep, dim3((unsigned)prep), dim3(256), 0, st, g, (char*)ws);
   CFH_LAUNCH_CHECK();
-  if (state_bf16) hipLaunchKernelGGL(k_gdn_chunks<uint16_t>, dim3((unsigned)blocks), dim3(256), 0, st, g, (const char*)ws);
-  else hipLaunchKernelGGL(k_gdn_chunks<float>, dim3((unsigned)blocks), dim3(256), 0, st, g, (const char*)ws);
+  if (state_bf16) hipLaunchKernelGGL(k_gdn_chunks<uint16_t>, dim3((unsigned)blocks), dim3(512), 0, st, g, (const char*)ws);
+  else hipLaunchKernelGGL(k_gdn_chunks<float>, dim3((unsigned)blocks), dim3(512), 0, st, g, (const char*)ws);
   CFH_LAUNCH_CHECK();
   return CFH_OK;
 }
