@@ -14,10 +14,12 @@
 // chunks at once.  k_gdn_chunks then carries S through the chunks of each (sequence, value head), 16 value
 // columns a workgroup (they do not mix).
 //   Precision: q and k enter MFMA as the bf16 numbers they are, their norms and decays are fp32 factors of the
-// rows; fp32 operands on the way to the state (S, R, d, the inverse) are split into three bf16 parts, products
-// below 2^-24 dropped, so that fp32 states keep fp32 digits; what only the bf16 output sees into two (2^-17).
+// rows; fp32 operands on the way to the state (S, R, d) are split into three bf16 parts, so that fp32 states keep
+// fp32 digits; the inverse, whose diagonal is exactly 1, and what only the bf16 output sees into two (2^-18).
 // Differences of G are taken in 64 bits: a strong decay earlier in the chunk must not cost a weak one later its
 // digits (decays below e^-200 are taken as that: both are 0 in fp32).
+#include <type_traits>
+
 #include "cfh_gdn.h"
 #include "cfh_host.h"
 #include "cfh_kernels.h"
@@ -164,9 +166,9 @@ __global__ void __launch_bounds__(64) k_gdn_rows(GdnSeqArgs a) {
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int GC = 64;                             // rows a chunk
-// a chunk and value head's place in the workspace: the inverse in three parts and the attention matrix in two,
-// [row tile][k-step][part][lane] 16 B each; then the rows' factors, fp32 [4][64], and e^G_C
-constexpr int GW_ATT = 4 * 2 * 3 * 64 * 16, GW_VEC = GW_ATT + 4 * 2 * 2 * 64 * 16;
+// a chunk and value head's place in the workspace: the inverse and the attention matrix in two parts each,
+// [row tile][k-step][part][lane] 16 B; then the rows' factors, fp32 [4][64], and e^G_C
+constexpr int GW_ATT = 4 * 2 * 2 * 64 * 16, GW_VEC = 2 * GW_ATT;
 constexpr int GW_BYTES = GW_VEC + 4 * GC * 4 + 256;
 
 __device__ __forceinline__ f32x4 mfma_b(const uint4& x, const uint4& y, f32x4 acc) {
@@ -381,20 +383,19 @@ __global__ void __launch_bounds__(256) k_gdn_prep(GdnSeqArgs a, char* ws) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) Ls[16 * wave + 4 * g + r][16 * tile + tl] = att[tile][r];
   __syncthreads();
-  uint4* const tf = (uint4*)w + (size_t)wave * 6 * 64 + lane;
-  uint4* const af = (uint4*)(w + GW_ATT) + (size_t)wave * 4 * 64 + lane;
 #pragma unroll
-  for (int ks = 0; ks < 2; ++ks) {
-    if (ks > wave / 2) break;
-    uint2 p0[3], p1[3], h0, l0, h1, l1;
-    split4(*(const f32x4*)&Ts[16 * wave + tl][32 * ks + 4 * g], p0);
-    split4(*(const f32x4*)&Ts[16 * wave + tl][32 * ks + 16 + 4 * g], p1);
+  for (int m = 0; m < 2; ++m) {
+    const float(*M)[GC + 4] = m ? Ls : Ts;
+    uint4* out = (uint4*)(w + m * GW_ATT) + (size_t)wave * 4 * 64 + lane;
 #pragma unroll
-    for (int p = 0; p < 3; ++p) tf[(ks * 3 + p) * 64] = make_uint4(p0[p].x, p0[p].y, p1[p].x, p1[p].y);
-    split4(*(const f32x4*)&Ls[16 * wave + tl][32 * ks + 4 * g], h0, l0);
-    split4(*(const f32x4*)&Ls[16 * wave + tl][32 * ks + 16 + 4 * g], h1, l1);
-    af[(ks * 2) * 64] = make_uint4(h0.x, h0.y, h1.x, h1.y);
-    af[(ks * 2 + 1) * 64] = make_uint4(l0.x, l0.y, l1.x, l1.y);
+    for (int ks = 0; ks < 2; ++ks) {
+      if (ks > wave / 2) break;
+      uint2 h0, l0, h1, l1;
+      split4(*(const f32x4*)&M[16 * wave + tl][32 * ks + 4 * g], h0, l0);
+      split4(*(const f32x4*)&M[16 * wave + tl][32 * ks + 16 + 4 * g], h1, l1);
+      out[(ks * 2) * 64] = make_uint4(h0.x, h0.y, h1.x, h1.y);
+      out[(ks * 2 + 1) * 64] = make_uint4(l0.x, l0.y, l1.x, l1.y);
+    }
   }
 }
 
@@ -405,7 +406,7 @@ __global__ void __launch_bounds__(256) k_gdn_prep(GdnSeqArgs a, char* ws) {
 // Rows of S in a wave's MFMA tiles: tile u, row 4 g + r is k row 32 wave + 8 g + 4 u + r, so that the two tiles
 // of a lane make eight neighbouring k rows, the natural operand order of K and Q.
 struct ChainIn {                   // a lane of a chain wave, one chunk
-  uint4 t[2][3];                   // its rows of the inverse: [k-step][part]
+  uint4 t[2][2];                   // its rows of the inverse: [k-step][part]
   uint2 v;                         // 4 columns of row 16 wave + lane / 4 (to LDS and back transposed)
   float4 b, cx, ce;                // factors of rows 16 wave + 4 g + r
   float eg;
@@ -467,22 +468,24 @@ __global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws
         *(uint4*)&kl[c & 1][row * GDN_DK + (((tid % 16) ^ swz(row)) * 8)] = row < n ? kr[x] : make_uint4(0, 0, 0, 0);
       }
     };
-    auto load = [&](int c, OutIn& in) {
+    // (nk: the k-steps of the wave's rows of a triangular matrix, one for the first two row tiles)
+    auto load_q = [&](int c, OutIn& in) {
       const int t0 = c0 + c * GC, n = min(GC, c1 - t0);
       const uint16_t* q = qb + (size_t)(t0 + min(16 * wave + tl, n - 1)) * a.ld + 8 * g;
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) in.q[ks] = *(const uint4*)(q + 32 * ks);
+    };
+    auto load_a = [&](int c, OutIn& in, auto nk) {
       const uint4* af = (const uint4*)(place(c) + GW_ATT) + (size_t)wave * 4 * 64 + lane;
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-        for (int p = 0; p < 2; ++p) in.at[ks][p] = af[(min(ks, wave / 2) * 2 + p) * 64];
+      for (int x = 0; x < 2 * nk.value; ++x) in.at[x / 2][x % 2] = af[x * 64];
       in.cq = *(const float4*)((const float*)(place(c) + GW_VEC) + 2 * GC + 16 * wave + 4 * g);
     };
-    auto work = [&](int c, const OutIn& in, OutIn& next) {
+    auto work = [&](int c, const OutIn& in, OutIn& next, auto nk) {
       const int t0 = c0 + c * GC, n = min(GC, c1 - t0);
       lds_barrier();                                         // S is there
-      load_k(min(c + 1, nc - 1));
+      stage_k(min(c + 1, nc - 1));
+      load_k(min(c + 2, nc - 1));
       f32x4 Y[2] = {};
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
@@ -490,13 +493,12 @@ __global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws
         Y[1] = mfma_b(in.q[ks], sS[ks][1][lane], Y[1]);
       }
       lds_barrier();                                         // R is there
-      load(min(c + 1, nc - 1), next);
-      stage_k(min(c + 1, nc - 1));
+      load_q(min(c + 1, nc - 1), next);
       lds_barrier();                                         // d is there
+      load_a(min(c + 1, nc - 1), next, nk);
       f32x4 o[3] = {};
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        if (ks > wave / 2) break;
+      for (int ks = 0; ks < nk.value; ++ks) {
         const uint4 hi = *(const uint4*)sD[0][ks][lane], lo = *(const uint4*)sD[1][ks][lane];
         o[0] = mfma_b(in.at[ks][0], hi, o[0]);
         o[1] = mfma_b(in.at[ks][0], lo, o[1]);
@@ -510,24 +512,31 @@ __global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws
           out[(size_t)r * a.HV * a.V] = to_bf16(cq[r] * (Y[0][r] + Y[1][r]) + (o[0][r] + (o[1][r] + o[2][r])));
     };
     OutIn A, B;
-    load_k(0);
-    load(0, A);
-    stage_k(0);
-    for (int c = 0;;) {
-      work(c, A, B);
-      if (++c >= nc) return;
-      work(c, B, A);
-      if (++c >= nc) return;
-    }
+    auto chunks = [&](auto nk) {
+      load_k(0);
+      stage_k(0);
+      load_k(min(1, nc - 1));
+      load_q(0, A);
+      load_a(0, A, nk);
+      for (int c = 0;;) {
+        work(c, A, B, nk);
+        if (++c >= nc) break;
+        work(c, B, A, nk);
+        if (++c >= nc) break;
+      }
+    };
+    if (wave < 2) chunks(std::integral_constant<int, 1>{});
+    else chunks(std::integral_constant<int, 2>{});
+    return;
   }
 
-  auto load = [&](int c, ChainIn& in) {
+  auto load_t = [&](int c, ChainIn& in, auto nk) {
+    const uint4* tf = (const uint4*)place(c) + (size_t)wave * 4 * 64 + lane;
+#pragma unroll
+    for (int x = 0; x < 2 * nk.value; ++x) in.t[x / 2][x % 2] = tf[x * 64];
+  };
+  auto load_v = [&](int c, ChainIn& in) {
     const int t0 = c0 + c * GC, n = min(GC, c1 - t0);
-    const uint4* tf = (const uint4*)place(c) + (size_t)wave * 6 * 64 + lane;
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-      for (int p = 0; p < 3; ++p) in.t[ks][p] = tf[(min(ks, wave / 2) * 3 + p) * 64];
     in.v = *(const uint2*)(vb + (size_t)(t0 + min(16 * wave + lane / 4, n - 1)) * a.ld + 4 * (lane & 3));
     const float* f = (const float*)(place(c) + GW_VEC) + 16 * wave + 4 * g;
     in.b = *(const float4*)f;
@@ -549,7 +558,7 @@ __global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws
                    __uint_as_float(x.w & 0xffff0000u)};
     }
   }
-  auto work = [&](int c, const ChainIn& in, ChainIn& next) {
+  auto work = [&](int c, const ChainIn& in, ChainIn& next, auto nk) {
     const uint16_t* kt = kl[c & 1];
     const int n = c1 - c0 - c * GC, row = 16 * wave + tl;
     uint2 p0[3], p1[3];
@@ -568,7 +577,7 @@ __global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws
     }
     // (the wave's own sV: in order behind its write) rows 4 g .. 4 g + 3 of its tile, column tl
     const uint2 vv = read_tr((const uint16_t*)&sV[wave][16 * g] + 4 * tl);
-    load(min(c + 1, nc - 1), next);
+    load_v(min(c + 1, nc - 1), next);
     const float bb[4] = {in.b.x, in.b.y, in.b.z, in.b.w}, cx[4] = {in.cx.x, in.cx.y, in.cx.z, in.cx.w};
     const float ce[4] = {in.ce.x, in.ce.y, in.ce.z, in.ce.w};
     const float v[4] = {__uint_as_float(vv.x << 16), __uint_as_float(vv.x & 0xffff0000u), __uint_as_float(vv.y << 16),
@@ -582,18 +591,17 @@ __global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws
     lds_barrier();                                           // R is there
     f32x4 d[3] = {};
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      if (ks > wave / 2) break;
+    for (int ks = 0; ks < nk.value; ++ks) {
       uint4 x[3];
 #pragma unroll
       for (int p = 0; p < 3; ++p) x[p] = *(const uint4*)sR[p][ks][lane];
       d[0] = mfma_b(in.t[ks][0], x[0], d[0]);
       d[1] = mfma_b(in.t[ks][0], x[1], d[1]);
       d[2] = mfma_b(in.t[ks][1], x[0], d[2]);
-      d[1] = mfma_b(in.t[ks][1], x[1], d[1]);
-      d[2] = mfma_b(in.t[ks][0], x[2], d[2]);
-      d[1] = mfma_b(in.t[ks][2], x[0], d[1]);
+      d[1] = mfma_b(in.t[ks][0], x[2], d[1]);
+      d[2] = mfma_b(in.t[ks][1], x[1], d[2]);
     }
+    load_t(min(c + 1, nc - 1), next, nk);
     const f32x4 D = d[0] + (d[1] + d[2]);
     f32x4 E;
 #pragma unroll
@@ -625,14 +633,20 @@ __global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws
 #pragma unroll
     for (int u = 0; u < 2; ++u) S[u] = S[u] * in.eg + (up[u][0] + (up[u][1] + up[u][2]));
   };
+  __builtin_amdgcn_s_setprio(3);     // (the outputs fill what the chain leaves)
   ChainIn A, B;
-  load(0, A);
-  for (int c = 0;;) {
-    work(c, A, B);
-    if (++c >= nc) break;
-    work(c, B, A);
-    if (++c >= nc) break;
-  }
+  auto chunks = [&](auto nk) {
+    load_t(0, A, nk);
+    load_v(0, A);
+    for (int c = 0;;) {
+      work(c, A, B, nk);
+      if (++c >= nc) break;
+      work(c, B, A, nk);
+      if (++c >= nc) break;
+    }
+  };
+  if (wave < 2) chunks(std::integral_constant<int, 1>{});
+  else chunks(std::integral_constant<int, 2>{});
   if constexpr (sizeof(T) == 4) {
     *(f32x4*)st = S[0];
     *(f32x4*)(st + 4) = S[1];
