@@ -400,28 +400,46 @@ __global__ void __launch_bounds__(256) k_gdn_prep(GdnSeqArgs a, char* ws) {
 }
 
 // S through the chunks of one (sequence, value head), 16 value columns, in a chain that no other workgroup can
-// shorten: what counts is the time from one chunk's S to the next one's.  Waves 0 - 3 carry the chain (a 16-row
-// tile of the chunk each, and 32 k rows of S), waves 4 - 7 compute the outputs and stage K beside it.  Three
-// barriers a chunk: S published, R published, d published.  Inputs come a chunk ahead.
+// shorten: what counts is the time from one chunk's S to the next one's.  Waves 0 - 3 carry the chain, waves
+// 4 - 7 compute the outputs beside it and bring K, v and the rows' factors into LDS.  Three barriers a chunk.
+//   B1  every chain wave multiplies all of K with its own 32 k rows of S (from registers), the partial products
+//       meet in LDS
+//   B2  each chain wave makes R of its 16 rows of them
+//   B3  and d of its rows of the inverse and R; then its 32 k rows of S from all d
+// What a phase reads of LDS but does not wait for is read before the barrier in front of it.
 // Rows of S in a wave's MFMA tiles: tile u, row 4 g + r is k row 32 wave + 8 g + 4 u + r, so that the two tiles
 // of a lane make eight neighbouring k rows, the natural operand order of K and Q.
-struct ChainIn {                   // a lane of a chain wave, one chunk
-  uint4 t[2][2];                   // its rows of the inverse: [k-step][part]
-  uint2 v;                         // 4 columns of row 16 wave + lane / 4 (to LDS and back transposed)
-  float4 b, cx, ce;                // factors of rows 16 wave + 4 g + r
-  float eg;
+// Global accesses go through buffer descriptors of the chunk (base and size in scalar registers, one lane offset
+// for all chunks): rows behind the sequence read as zero and are not written, with no branch and no select.  A
+// branch around a load or store has the compiler count it as perhaps not issued, and a wait for an older load
+// becomes a wait for everything behind it.
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2b __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t span(const void* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, bytes, 0x27000);
+}
+__device__ __forceinline__ uint4 span_load16(__amdgpu_buffer_rsrc_t b, int at) {
+  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0));
+}
+
+struct KeyIn {                     // a lane of an output wave, a chunk on its way to LDS
+  uint4 k[4];
+  uint2 v;
+  float f;
 };
-struct OutIn {                     // a lane of an output wave
-  uint4 q[4], at[2][2];            // row 16 wave + tl of Q; its rows of the attention matrix
-  float4 cq;
+struct OutIn {                     // a lane of an output wave, one chunk
+  uint4 q[4], at[2][2];            // row 16 wave + tl of Q; its rows of the attention matrix: [k-step][part]
+  float4 cq;                       // factors of rows 16 wave + 4 g + r
 };
 
 template <typename T>
 __global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws) {
   __shared__ __align__(16) uint16_t kl[2][GC * GDN_DK];     // K, chunks of 16 bytes in swz order
-  __shared__ __align__(16) uint4 sS[4][3][64];              // S: [k-step = wave][part][lane]
+  __shared__ __align__(16) f32x4 sX[4][4][64];              // partial K S: [chain wave][row tile][lane]
+  __shared__ __align__(16) uint4 sS[4][2][64];              // S for the outputs: [k-step = wave][part][lane]
   __shared__ __align__(16) uint2 sR[3][2][64][2], sE[3][2][64][2], sD[2][2][64][2];   // [part][k-step][lane][tile of it]
-  __shared__ __align__(16) uint2 sV[4][64];
+  __shared__ __align__(16) uint2 sV[2][4][64];              // v: [row tile][row, 4 columns]
+  __shared__ __align__(16) float sF[2][4][GC];              // beta, beta e^G |k|^-1, e^(G_C - G) |k|^-1, e^G_C
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, tl = lane & 15;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), wave = wv & 3;
   const int nsl = a.V / 16;
@@ -441,61 +459,65 @@ __global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws
   }
   if (c0 == c1) return;
   const int h = hv / (a.HV / a.H), nc = (c1 - c0 + GC - 1) / GC;
-  const uint16_t* const qb = a.qkv + (size_t)h * GDN_DK;
-  const uint16_t* const kb = qb + (size_t)a.H * GDN_DK;
-  const uint16_t* const vb = a.qkv + 2 * (size_t)a.H * GDN_DK + (size_t)hv * a.V + sl * 16;
   const char* const wb = ws + ((size_t)chunk_start(a.cu, s) * a.HV + hv) * GW_BYTES;
   auto place = [&](int c) { return wb + (size_t)c * a.HV * GW_BYTES; };
-  // Loads of a chunk past the last one load the last one again: behind a branch the compiler would count them
-  // as perhaps not issued, and a wait for an older load would become a wait for these.  For the same reason
-  // rows behind the sequence are cleared where they are used.
+  // (chunks past the last one: the last one again)
+  auto rows_of = [&](int c) {      // the chunk's rows of mixed_qkv
+    const int t0 = c0 + c * GC, n = min(GC, c1 - t0);
+    return span(a.qkv + (size_t)t0 * a.ld, n * a.ld * 2);
+  };
 
   if (wv >= 4) {
-    uint4 kr[4];
-    auto load_k = [&](int c) {
-      const int t0 = c0 + c * GC, n = min(GC, c1 - t0);
+    const int koff = ((tid - 256) / 16 * a.ld + (a.H + h) * GDN_DK + (tid % 16) * 8) * 2, krow = 16 * a.ld * 2;
+    const int voff = ((16 * wave + lane / 4) * a.ld + 2 * a.H * GDN_DK + hv * a.V + sl * 16 + 4 * (lane & 3)) * 2;
+    const int qoff = ((16 * wave + tl) * a.ld + h * GDN_DK + 8 * g) * 2;
+    const int foff = GW_VEC + (wave == 3 ? 4 * GC : (wave == 2 ? 3 : wave) * GC + lane) * 4;
+    auto load_in = [&](int c, KeyIn& in) {
+      const auto b = rows_of(c);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int row = 16 * x + (tid - 256) / 16;
-        kr[x] = *(const uint4*)(kb + (size_t)(t0 + min(row, n - 1)) * a.ld + (tid % 16) * 8);
-      }
+      for (int x = 0; x < 4; ++x) in.k[x] = span_load16(b, koff + x * krow);
+      in.v = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(b, voff, 0, 0));
+      in.f = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(span(place(c), GW_BYTES), foff, 0, 0));
     };
-    auto stage_k = [&](int c) {
-      const int n = c1 - c0 - c * GC;
+    auto stage_in = [&](int c, const KeyIn& in) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const int row = 16 * x + (tid - 256) / 16;
-        *(uint4*)&kl[c & 1][row * GDN_DK + (((tid % 16) ^ swz(row)) * 8)] = row < n ? kr[x] : make_uint4(0, 0, 0, 0);
+        *(uint4*)&kl[c & 1][row * GDN_DK + (((tid % 16) ^ swz(row)) * 8)] = in.k[x];
       }
+      sV[c & 1][wave][lane] = in.v;
+      sF[c & 1][wave][lane] = in.f;
     };
     // (nk: the k-steps of the wave's rows of a triangular matrix, one for the first two row tiles)
     auto load_q = [&](int c, OutIn& in) {
-      const int t0 = c0 + c * GC, n = min(GC, c1 - t0);
-      const uint16_t* q = qb + (size_t)(t0 + min(16 * wave + tl, n - 1)) * a.ld + 8 * g;
+      const auto b = rows_of(c);
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) in.q[ks] = *(const uint4*)(q + 32 * ks);
+      for (int ks = 0; ks < 4; ++ks) in.q[ks] = span_load16(b, qoff + 64 * ks);
     };
     auto load_a = [&](int c, OutIn& in, auto nk) {
-      const uint4* af = (const uint4*)(place(c) + GW_ATT) + (size_t)wave * 4 * 64 + lane;
+      const auto b = span(place(c), GW_BYTES);
 #pragma unroll
-      for (int x = 0; x < 2 * nk.value; ++x) in.at[x / 2][x % 2] = af[x * 64];
-      in.cq = *(const float4*)((const float*)(place(c) + GW_VEC) + 2 * GC + 16 * wave + 4 * g);
+      for (int x = 0; x < 2 * nk.value; ++x) in.at[x / 2][x % 2] = span_load16(b, GW_ATT + ((wave * 4 + x) * 64 + lane) * 16);
+      in.cq = __builtin_bit_cast(float4, span_load16(b, GW_VEC + (2 * GC + 16 * wave + 4 * g) * 4));
     };
-    auto work = [&](int c, const OutIn& in, OutIn& next, auto nk) {
-      const int t0 = c0 + c * GC, n = min(GC, c1 - t0);
-      lds_barrier();                                         // S is there
-      stage_k(min(c + 1, nc - 1));
-      load_k(min(c + 2, nc - 1));
+    const size_t rs = (size_t)a.HV * a.V;
+    const int ooff = ((16 * wave + 4 * g) * (int)rs + hv * a.V + sl * 16 + tl) * 2;
+    auto work = [&](int c, const OutIn& in, OutIn& next, KeyIn& key, const KeyIn& next_key, auto nk) {
+      lds_barrier();                                         // B1
       f32x4 Y[2] = {};
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
         Y[0] = mfma_b(in.q[ks], sS[ks][0][lane], Y[0]);
         Y[1] = mfma_b(in.q[ks], sS[ks][1][lane], Y[1]);
       }
-      lds_barrier();                                         // R is there
+      const float cq[4] = {in.cq.x, in.cq.y, in.cq.z, in.cq.w};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) Y[0][r] = cq[r] * (Y[0][r] + Y[1][r]);
+      lds_barrier();                                         // B2
+      stage_in(c + 1, next_key);
+      load_in(min(c + 2, nc - 1), key);
       load_q(min(c + 1, nc - 1), next);
-      lds_barrier();                                         // d is there
-      load_a(min(c + 1, nc - 1), next, nk);
+      lds_barrier();                                         // B3
       f32x4 o[3] = {};
 #pragma unroll
       for (int ks = 0; ks < nk.value; ++ks) {
@@ -504,24 +526,26 @@ __global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws
         o[1] = mfma_b(in.at[ks][0], lo, o[1]);
         o[2] = mfma_b(in.at[ks][1], hi, o[2]);
       }
-      const float cq[4] = {in.cq.x, in.cq.y, in.cq.z, in.cq.w};
-      uint16_t* out = a.out + ((size_t)(t0 + 16 * wave + 4 * g) * a.HV + hv) * a.V + sl * 16 + tl;
+      load_a(min(c + 1, nc - 1), next, nk);
+      const f32x4 O = Y[0] + (o[0] + (o[1] + o[2]));
+      const int t0 = c0 + c * GC;
+      const auto b = span(a.out + (size_t)t0 * rs, min(GC, c1 - t0) * (int)rs * 2);
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (16 * wave + 4 * g + r < n)
-          out[(size_t)r * a.HV * a.V] = to_bf16(cq[r] * (Y[0][r] + Y[1][r]) + (o[0][r] + (o[1][r] + o[2][r])));
+      for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b16(to_bf16(O[r]), b, ooff + r * (int)rs * 2, 0, 0);
     };
+    KeyIn KA, KB;
     OutIn A, B;
     auto chunks = [&](auto nk) {
-      load_k(0);
-      stage_k(0);
-      load_k(min(1, nc - 1));
+      load_in(0, KA);
+      load_in(min(1, nc - 1), KB);
       load_q(0, A);
       load_a(0, A, nk);
+      stage_in(0, KA);
+      lds_barrier();                                         // the first chunk's K, v and factors are there
       for (int c = 0;;) {
-        work(c, A, B, nk);
+        work(c, A, B, KA, KB, nk);
         if (++c >= nc) break;
-        work(c, B, A, nk);
+        work(c, B, A, KB, KA, nk);
         if (++c >= nc) break;
       }
     };
@@ -530,20 +554,6 @@ __global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws
     return;
   }
 
-  auto load_t = [&](int c, ChainIn& in, auto nk) {
-    const uint4* tf = (const uint4*)place(c) + (size_t)wave * 4 * 64 + lane;
-#pragma unroll
-    for (int x = 0; x < 2 * nk.value; ++x) in.t[x / 2][x % 2] = tf[x * 64];
-  };
-  auto load_v = [&](int c, ChainIn& in) {
-    const int t0 = c0 + c * GC, n = min(GC, c1 - t0);
-    in.v = *(const uint2*)(vb + (size_t)(t0 + min(16 * wave + lane / 4, n - 1)) * a.ld + 4 * (lane & 3));
-    const float* f = (const float*)(place(c) + GW_VEC) + 16 * wave + 4 * g;
-    in.b = *(const float4*)f;
-    in.cx = *(const float4*)(f + GC);
-    in.ce = *(const float4*)(f + 3 * GC);
-    in.eg = *((const float*)(place(c) + GW_VEC) + 4 * GC);
-  };
   T* const st = (T*)a.state + (((size_t)a.slots[s] * a.HV + hv) * a.V + sl * 16 + tl) * GDN_DK + 32 * wave + 8 * g;
   f32x4 S[2] = {};
   if (!a.initial || a.initial[s]) {
@@ -558,86 +568,110 @@ __global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws
                    __uint_as_float(x.w & 0xffff0000u)};
     }
   }
-  auto work = [&](int c, const ChainIn& in, ChainIn& next, auto nk) {
+  auto load_t = [&](int c, uint4 (&t)[2][2], auto nk) {      // its rows of the inverse: [k-step][part]
+    const auto b = span(place(c), GW_BYTES);
+#pragma unroll
+    for (int x = 0; x < 2 * nk.value; ++x) t[x / 2][x % 2] = span_load16(b, ((wave * 4 + x) * 64 + lane) * 16);
+  };
+  // a chunk's K at the wave's k columns, rows 16 i + tl; v of rows 16 wave + 4 g + r, column tl; the factors
+  uint4 kx[4];
+  uint2 vv;
+  f32x4 fb, fx, fe;
+  float eg;
+  auto read_in = [&](int c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      kx[i] = *(const uint4*)&kl[c & 1][(16 * i + tl) * GDN_DK + (((4 * wave + g) ^ swz(tl)) * 8)];
+    vv = read_tr((const uint16_t*)&sV[c & 1][wave][16 * g] + 4 * tl);
+    fb = *(const f32x4*)&sF[c & 1][0][16 * wave + 4 * g];
+    fx = *(const f32x4*)&sF[c & 1][1][16 * wave + 4 * g];
+    fe = *(const f32x4*)&sF[c & 1][2][16 * wave + 4 * g];
+    eg = sF[c & 1][3][0];
+  };
+  auto work = [&](int c, const uint4 (&t)[2][2], uint4 (&tnext)[2][2], auto nk) {
     const uint16_t* kt = kl[c & 1];
-    const int n = c1 - c0 - c * GC, row = 16 * wave + tl;
     uint2 p0[3], p1[3];
+    uint4 sp[3];
     split4(S[0], p0);
     split4(S[1], p1);
 #pragma unroll
-    for (int p = 0; p < 3; ++p) sS[wave][p][lane] = make_uint4(p0[p].x, p0[p].y, p1[p].x, p1[p].y);
-    sV[wave][lane] = 16 * wave + lane / 4 < n ? in.v : make_uint2(0, 0);
-    lds_barrier();                                           // S is there, and K
-    f32x4 X[3] = {};
+    for (int p = 0; p < 3; ++p) sp[p] = make_uint4(p0[p].x, p0[p].y, p1[p].x, p1[p].y);
+    f32x4 X[4] = {};
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      const uint4 kf = *(const uint4*)&kt[row * GDN_DK + (((4 * ks + g) ^ swz(row)) * 8)];
+    for (int p = 2; p >= 0; --p)
 #pragma unroll
-      for (int p = 0; p < 3; ++p) X[p] = mfma_b(kf, sS[ks][p][lane], X[p]);
-    }
-    // (the wave's own sV: in order behind its write) rows 4 g .. 4 g + 3 of its tile, column tl
-    const uint2 vv = read_tr((const uint16_t*)&sV[wave][16 * g] + 4 * tl);
-    load_v(min(c + 1, nc - 1), next);
-    const float bb[4] = {in.b.x, in.b.y, in.b.z, in.b.w}, cx[4] = {in.cx.x, in.cx.y, in.cx.z, in.cx.w};
-    const float ce[4] = {in.ce.x, in.ce.y, in.ce.z, in.ce.w};
-    const float v[4] = {__uint_as_float(vv.x << 16), __uint_as_float(vv.x & 0xffff0000u), __uint_as_float(vv.y << 16),
-                        __uint_as_float(vv.y & 0xffff0000u)};
+      for (int i = 0; i < 4; ++i) X[i] = mfma_b(kx[i], sp[p], X[i]);
+    sS[wave][0][lane] = sp[0];
+    sS[wave][1][lane] = sp[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sX[wave][i][lane] = X[i];
+    lds_barrier();                                           // B1
+    const f32x4 x = (sX[0][wave][lane] + sX[1][wave][lane]) + (sX[2][wave][lane] + sX[3][wave][lane]);
+    const f32x4 v = {__uint_as_float(vv.x << 16), __uint_as_float(vv.x & 0xffff0000u), __uint_as_float(vv.y << 16),
+                     __uint_as_float(vv.y & 0xffff0000u)};
     f32x4 R;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) R[r] = bb[r] * v[r] - cx[r] * (X[0][r] + (X[1][r] + X[2][r]));
+    for (int r = 0; r < 4; ++r) R[r] = fb[r] * v[r] - fx[r] * x[r];
     split4(R, p0);
 #pragma unroll
     for (int p = 0; p < 3; ++p) sR[p][wave >> 1][lane][wave & 1] = p0[p];
-    lds_barrier();                                           // R is there
+    lds_barrier();                                           // B2
     f32x4 d[3] = {};
 #pragma unroll
     for (int ks = 0; ks < nk.value; ++ks) {
-      uint4 x[3];
+      uint4 y[3];
 #pragma unroll
-      for (int p = 0; p < 3; ++p) x[p] = *(const uint4*)sR[p][ks][lane];
-      d[0] = mfma_b(in.t[ks][0], x[0], d[0]);
-      d[1] = mfma_b(in.t[ks][0], x[1], d[1]);
-      d[2] = mfma_b(in.t[ks][1], x[0], d[2]);
-      d[1] = mfma_b(in.t[ks][0], x[2], d[1]);
-      d[2] = mfma_b(in.t[ks][1], x[1], d[2]);
+      for (int p = 0; p < 3; ++p) y[p] = *(const uint4*)sR[p][ks][lane];
+      d[0] = mfma_b(t[ks][0], y[0], d[0]);
+      d[1] = mfma_b(t[ks][0], y[1], d[1]);
+      d[2] = mfma_b(t[ks][1], y[0], d[2]);
+      d[1] = mfma_b(t[ks][0], y[2], d[1]);
+      d[2] = mfma_b(t[ks][1], y[1], d[2]);
     }
-    load_t(min(c + 1, nc - 1), next, nk);
-    const f32x4 D = d[0] + (d[1] + d[2]);
-    f32x4 E;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) E[r] = D[r] * ce[r];
-    split4(E, p0);
-    split4(D, p1[0], p1[1]);
-#pragma unroll
-    for (int p = 0; p < 3; ++p) sE[p][wave >> 1][lane][wave & 1] = p0[p];
-#pragma unroll
-    for (int p = 0; p < 2; ++p) sD[p][wave >> 1][lane][wave & 1] = p1[p];
-    lds_barrier();                                           // d is there
-    // S: K's columns as rows by transposed reads
-    f32x4 up[2][3] = {};
+    load_t(min(c + 1, nc - 1), tnext, nk);
+    // K's columns as rows, by transposed reads: row of S 16 u + tl, tokens in slot order
+    uint4 kf[2][2];
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      uint4 x[3];
-#pragma unroll
-      for (int p = 0; p < 3; ++p) x[p] = *(const uint4*)sE[p][ks][lane];
       const int r0 = 32 * ks + 4 * g + tl / 4, r1 = r0 + 16, ch = 4 * wave + (tl & 3);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const uint2 y = read_tr(&kt[r0 * GDN_DK + ((ch ^ swz(r0)) * 8) + 4 * u]);
         const uint2 z = read_tr(&kt[r1 * GDN_DK + ((ch ^ swz(r1)) * 8) + 4 * u]);
-        const uint4 kf = make_uint4(y.x, y.y, z.x, z.y);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) up[u][p] = mfma_b(kf, x[p], up[u][p]);
+        kf[ks][u] = make_uint4(y.x, y.y, z.x, z.y);
       }
     }
+    const f32x4 D = d[0] + (d[1] + d[2]);
+    split4(D * fe, p0);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) S[u] = S[u] * in.eg + (up[u][0] + (up[u][1] + up[u][2]));
+    for (int p = 0; p < 3; ++p) sE[p][wave >> 1][lane][wave & 1] = p0[p];
+    split4(D, p1[0], p1[1]);
+#pragma unroll
+    for (int p = 0; p < 2; ++p) sD[p][wave >> 1][lane][wave & 1] = p1[p];
+    const float keep = eg;
+    lds_barrier();                                           // B3
+    f32x4 up[2][2] = {};
+    uint4 y[2][3];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int p = 0; p < 3; ++p) y[ks][p] = *(const uint4*)sE[p][ks][lane];
+    read_in(min(c + 1, nc - 1));
+#pragma unroll
+    for (int p = 2; p >= 0; --p)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) up[u][ks] = mfma_b(kf[ks][u], y[ks][p], up[u][ks]);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) S[u] = S[u] * keep + (up[u][0] + up[u][1]);
   };
   __builtin_amdgcn_s_setprio(3);     // (the outputs fill what the chain leaves)
-  ChainIn A, B;
+  uint4 A[2][2], B[2][2];
   auto chunks = [&](auto nk) {
     load_t(0, A, nk);
-    load_v(0, A);
+    lds_barrier();
+    read_in(0);
     for (int c = 0;;) {
       work(c, A, B, nk);
       if (++c >= nc) break;
