@@ -14,8 +14,9 @@
 // chunks at once.  k_gdn_chunks then carries S through the chunks of each (sequence, value head), 16 value
 // columns a workgroup (they do not mix).
 //   Precision: q and k enter MFMA as the bf16 numbers they are, their norms and decays are fp32 factors of the
-// rows; fp32 operands on the way to the state (S, R, d) are split into three bf16 parts, so that fp32 states keep
-// fp32 digits; the inverse, whose diagonal is exactly 1, and what only the bf16 output sees into two (2^-18).
+// rows; fp32 operands are split into bf16 parts: R and d, on the way to an fp32 state, into three, the others into two
+// (2^-18; the state's error is 1.3e-7 over 8,000 rows, 5 to 7 times that with two parts of R or d, the same with
+// three of S).
 // Differences of G are taken in 64 bits: a strong decay earlier in the chunk must not cost a weak one later its
 // digits (decays below e^-200 are taken as that: both are 0 in fp32).
 #include <type_traits>
@@ -175,20 +176,14 @@ __device__ __forceinline__ f32x4 mfma_b(const uint4& x, const uint4& y, f32x4 ac
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, x), __builtin_bit_cast(b16x8, y), acc, 0, 0, 0);
 }
 
-// x = hi + lo to 2^-17, both bf16.
-__device__ __forceinline__ void split4(const f32x4& x, uint2& hi, uint2& lo) {
-  hi = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
-  lo = make_uint2(pack_bf16(x[0] - __uint_as_float(hi.x << 16), x[1] - __uint_as_float(hi.x & 0xffff0000u)),
-                  pack_bf16(x[2] - __uint_as_float(hi.y << 16), x[3] - __uint_as_float(hi.y & 0xffff0000u)));
-}
-
-// x = hi + mid + lo to 2^-25, all bf16.
-__device__ __forceinline__ void split4(const f32x4& x, uint2 (&p)[3]) {
+// x = the sum of N bf16 parts, to 2^-(8 N + 1).
+template <int N>
+__device__ __forceinline__ void split4(const f32x4& x, uint2 (&p)[N]) {
   f32x4 r = x;
 #pragma unroll
-  for (int i = 0; i < 3; ++i) {
+  for (int i = 0; i < N; ++i) {
     p[i] = make_uint2(pack_bf16(r[0], r[1]), pack_bf16(r[2], r[3]));
-    if (i < 2) {
+    if (i + 1 < N) {
       r[0] -= __uint_as_float(p[i].x << 16); r[1] -= __uint_as_float(p[i].x & 0xffff0000u);
       r[2] -= __uint_as_float(p[i].y << 16); r[3] -= __uint_as_float(p[i].y & 0xffff0000u);
     }
@@ -390,18 +385,19 @@ __global__ void __launch_bounds__(256) k_gdn_prep(GdnSeqArgs a, char* ws) {
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       if (ks > wave / 2) break;
-      uint2 h0, l0, h1, l1;
-      split4(*(const f32x4*)&M[16 * wave + tl][32 * ks + 4 * g], h0, l0);
-      split4(*(const f32x4*)&M[16 * wave + tl][32 * ks + 16 + 4 * g], h1, l1);
-      out[(ks * 2) * 64] = make_uint4(h0.x, h0.y, h1.x, h1.y);
-      out[(ks * 2 + 1) * 64] = make_uint4(l0.x, l0.y, l1.x, l1.y);
+      uint2 p0[2], p1[2];
+      split4(*(const f32x4*)&M[16 * wave + tl][32 * ks + 4 * g], p0);
+      split4(*(const f32x4*)&M[16 * wave + tl][32 * ks + 16 + 4 * g], p1);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) out[(ks * 2 + p) * 64] = make_uint4(p0[p].x, p0[p].y, p1[p].x, p1[p].y);
     }
   }
 }
 
 // S through the chunks of one (sequence, value head), 16 value columns, in a chain that no other workgroup can
 // shorten: what counts is the time from one chunk's S to the next one's.  Waves 0 - 3 carry the chain, waves
-// 4 - 7 compute the outputs beside it and bring K, v and the rows' factors into LDS.  Three barriers a chunk.
+// 4 - 7 compute the outputs beside it, waves 8 - 11 bring K, v and the rows' factors into LDS.  Three barriers a
+// chunk.
 //   B1  every chain wave multiplies all of K with its own 32 k rows of S (from registers), the partial products
 //       meet in LDS
 //   B2  each chain wave makes R of its 16 rows of them
@@ -422,7 +418,7 @@ __device__ __forceinline__ uint4 span_load16(__amdgpu_buffer_rsrc_t b, int at) {
   return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0));
 }
 
-struct KeyIn {                     // a lane of an output wave, a chunk on its way to LDS
+struct KeyIn {                     // a lane of a staging wave, one chunk
   uint4 k[4];
   uint2 v;
   float f;
@@ -433,11 +429,12 @@ struct OutIn {                     // a lane of an output wave, one chunk
 };
 
 template <typename T>
-__global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws) {
+__global__ void __launch_bounds__(768) k_gdn_chunks(GdnSeqArgs a, const char* ws) {
+  constexpr int NP = sizeof(T) == 4 ? 3 : 2;                // parts of R and d
   __shared__ __align__(16) uint16_t kl[2][GC * GDN_DK];     // K, chunks of 16 bytes in swz order
   __shared__ __align__(16) f32x4 sX[4][4][64];              // partial K S: [chain wave][row tile][lane]
   __shared__ __align__(16) uint4 sS[4][2][64];              // S for the outputs: [k-step = wave][part][lane]
-  __shared__ __align__(16) uint2 sR[3][2][64][2], sE[3][2][64][2], sD[2][2][64][2];   // [part][k-step][lane][tile of it]
+  __shared__ __align__(16) uint2 sR[NP][2][64][2], sE[NP][2][64][2], sD[2][2][64][2];   // [part][k-step][lane][tile of it]
   __shared__ __align__(16) uint2 sV[2][4][64];              // v: [row tile][row, 4 columns]
   __shared__ __align__(16) float sF[2][4][GC];              // beta, beta e^G |k|^-1, e^(G_C - G) |k|^-1, e^G_C
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, tl = lane & 15;
@@ -454,7 +451,7 @@ __global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws
   if (ok < 0 || !rows) {
     if (a.status && tid == 0) a.status[0] = 1;
     if (rows)
-      for (int t = c0 + tid / 16; t < c1; t += 32) a.out[((size_t)t * a.HV + hv) * a.V + sl * 16 + tid % 16] = 0x7fc0;
+      for (int t = c0 + tid / 16; t < c1; t += 48) a.out[((size_t)t * a.HV + hv) * a.V + sl * 16 + tid % 16] = 0x7fc0;
     return;
   }
   if (c0 == c1) return;
@@ -467,27 +464,48 @@ __global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws
     return span(a.qkv + (size_t)t0 * a.ld, n * a.ld * 2);
   };
 
-  if (wv >= 4) {
-    const int koff = ((tid - 256) / 16 * a.ld + (a.H + h) * GDN_DK + (tid % 16) * 8) * 2, krow = 16 * a.ld * 2;
+  if (wv >= 8) {
+    const int koff = ((tid - 512) / 16 * a.ld + (a.H + h) * GDN_DK + (tid % 16) * 8) * 2, krow = 16 * a.ld * 2;
     const int voff = ((16 * wave + lane / 4) * a.ld + 2 * a.H * GDN_DK + hv * a.V + sl * 16 + 4 * (lane & 3)) * 2;
-    const int qoff = ((16 * wave + tl) * a.ld + h * GDN_DK + 8 * g) * 2;
     const int foff = GW_VEC + (wave == 3 ? 4 * GC : (wave == 2 ? 3 : wave) * GC + lane) * 4;
-    auto load_in = [&](int c, KeyIn& in) {
+    auto load = [&](int c, KeyIn& in) {
       const auto b = rows_of(c);
 #pragma unroll
       for (int x = 0; x < 4; ++x) in.k[x] = span_load16(b, koff + x * krow);
       in.v = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(b, voff, 0, 0));
       in.f = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(span(place(c), GW_BYTES), foff, 0, 0));
     };
-    auto stage_in = [&](int c, const KeyIn& in) {
+    auto stage = [&](int c, const KeyIn& in) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const int row = 16 * x + (tid - 256) / 16;
+        const int row = 16 * x + (tid - 512) / 16;
         *(uint4*)&kl[c & 1][row * GDN_DK + (((tid % 16) ^ swz(row)) * 8)] = in.k[x];
       }
       sV[c & 1][wave][lane] = in.v;
       sF[c & 1][wave][lane] = in.f;
     };
+    auto work = [&](int c, KeyIn& in, const KeyIn& next) {
+      lds_barrier();                                         // B1
+      load(min(c + 2, nc - 1), in);
+      lds_barrier();                                         // B2: the other buffer's readers are done
+      stage(c + 1, next);
+      lds_barrier();                                         // B3: and it holds the next chunk
+    };
+    KeyIn A, B;
+    load(0, A);
+    load(min(1, nc - 1), B);
+    stage(0, A);
+    lds_barrier();                                           // the first chunk's K, v and factors are there
+    for (int c = 0;;) {
+      work(c, A, B);
+      if (++c >= nc) return;
+      work(c, B, A);
+      if (++c >= nc) return;
+    }
+  }
+
+  if (wv >= 4) {
+    const int qoff = ((16 * wave + tl) * a.ld + h * GDN_DK + 8 * g) * 2;
     // (nk: the k-steps of the wave's rows of a triangular matrix, one for the first two row tiles)
     auto load_q = [&](int c, OutIn& in) {
       const auto b = rows_of(c);
@@ -502,7 +520,7 @@ __global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws
     };
     const size_t rs = (size_t)a.HV * a.V;
     const int ooff = ((16 * wave + 4 * g) * (int)rs + hv * a.V + sl * 16 + tl) * 2;
-    auto work = [&](int c, const OutIn& in, OutIn& next, KeyIn& key, const KeyIn& next_key, auto nk) {
+    auto work = [&](int c, const OutIn& in, OutIn& next, auto nk) {
       lds_barrier();                                         // B1
       f32x4 Y[2] = {};
 #pragma unroll
@@ -514,8 +532,6 @@ __global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws
 #pragma unroll
       for (int r = 0; r < 4; ++r) Y[0][r] = cq[r] * (Y[0][r] + Y[1][r]);
       lds_barrier();                                         // B2
-      stage_in(c + 1, next_key);
-      load_in(min(c + 2, nc - 1), key);
       load_q(min(c + 1, nc - 1), next);
       lds_barrier();                                         // B3
       f32x4 o[3] = {};
@@ -533,19 +549,15 @@ __global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws
 #pragma unroll
       for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b16(to_bf16(O[r]), b, ooff + r * (int)rs * 2, 0, 0);
     };
-    KeyIn KA, KB;
     OutIn A, B;
     auto chunks = [&](auto nk) {
-      load_in(0, KA);
-      load_in(min(1, nc - 1), KB);
       load_q(0, A);
       load_a(0, A, nk);
-      stage_in(0, KA);
-      lds_barrier();                                         // the first chunk's K, v and factors are there
+      lds_barrier();
       for (int c = 0;;) {
-        work(c, A, B, KA, KB, nk);
+        work(c, A, B, nk);
         if (++c >= nc) break;
-        work(c, B, A, KB, KA, nk);
+        work(c, B, A, nk);
         if (++c >= nc) break;
       }
     };
@@ -590,15 +602,15 @@ __global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws
   };
   auto work = [&](int c, const uint4 (&t)[2][2], uint4 (&tnext)[2][2], auto nk) {
     const uint16_t* kt = kl[c & 1];
-    uint2 p0[3], p1[3];
-    uint4 sp[3];
+    uint2 p0[2], p1[2], pn[NP];
+    uint4 sp[2];
     split4(S[0], p0);
     split4(S[1], p1);
 #pragma unroll
-    for (int p = 0; p < 3; ++p) sp[p] = make_uint4(p0[p].x, p0[p].y, p1[p].x, p1[p].y);
+    for (int p = 0; p < 2; ++p) sp[p] = make_uint4(p0[p].x, p0[p].y, p1[p].x, p1[p].y);
     f32x4 X[4] = {};
 #pragma unroll
-    for (int p = 2; p >= 0; --p)
+    for (int p = 1; p >= 0; --p)
 #pragma unroll
       for (int i = 0; i < 4; ++i) X[i] = mfma_b(kx[i], sp[p], X[i]);
     sS[wave][0][lane] = sp[0];
@@ -612,21 +624,23 @@ __global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws
     f32x4 R;
 #pragma unroll
     for (int r = 0; r < 4; ++r) R[r] = fb[r] * v[r] - fx[r] * x[r];
-    split4(R, p0);
+    split4(R, pn);
 #pragma unroll
-    for (int p = 0; p < 3; ++p) sR[p][wave >> 1][lane][wave & 1] = p0[p];
+    for (int p = 0; p < NP; ++p) sR[p][wave >> 1][lane][wave & 1] = pn[p];
     lds_barrier();                                           // B2
     f32x4 d[3] = {};
 #pragma unroll
     for (int ks = 0; ks < nk.value; ++ks) {
-      uint4 y[3];
+      uint4 y[NP];
 #pragma unroll
-      for (int p = 0; p < 3; ++p) y[p] = *(const uint4*)sR[p][ks][lane];
+      for (int p = 0; p < NP; ++p) y[p] = *(const uint4*)sR[p][ks][lane];
       d[0] = mfma_b(t[ks][0], y[0], d[0]);
       d[1] = mfma_b(t[ks][0], y[1], d[1]);
       d[2] = mfma_b(t[ks][1], y[0], d[2]);
-      d[1] = mfma_b(t[ks][0], y[2], d[1]);
-      d[2] = mfma_b(t[ks][1], y[1], d[2]);
+      if constexpr (NP == 3) {
+        d[1] = mfma_b(t[ks][0], y[2], d[1]);
+        d[2] = mfma_b(t[ks][1], y[1], d[2]);
+      }
     }
     load_t(min(c + 1, nc - 1), tnext, nk);
     // K's columns as rows, by transposed reads: row of S 16 u + tl, tokens in slot order
@@ -642,23 +656,23 @@ __global__ void __launch_bounds__(512) k_gdn_chunks(GdnSeqArgs a, const char* ws
       }
     }
     const f32x4 D = d[0] + (d[1] + d[2]);
-    split4(D * fe, p0);
+    split4(D * fe, pn);
 #pragma unroll
-    for (int p = 0; p < 3; ++p) sE[p][wave >> 1][lane][wave & 1] = p0[p];
-    split4(D, p1[0], p1[1]);
+    for (int p = 0; p < NP; ++p) sE[p][wave >> 1][lane][wave & 1] = pn[p];
+    split4(D, p1);
 #pragma unroll
     for (int p = 0; p < 2; ++p) sD[p][wave >> 1][lane][wave & 1] = p1[p];
     const float keep = eg;
     lds_barrier();                                           // B3
     f32x4 up[2][2] = {};
-    uint4 y[2][3];
+    uint4 y[2][NP];
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-      for (int p = 0; p < 3; ++p) y[ks][p] = *(const uint4*)sE[p][ks][lane];
+      for (int p = 0; p < NP; ++p) y[ks][p] = *(const uint4*)sE[p][ks][lane];
     read_in(min(c + 1, nc - 1));
 #pragma unroll
-    for (int p = 2; p >= 0; --p)
+    for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
@@ -701,7 +715,7 @@ int seq_args(GdnSeqArgs& g, const void* mixed_qkv, const void* a, const void* b,
              const float* dt_bias, void* ssm_state, int nslots, const int32_t* slots, int S, int T, int H, int HV, int K,
              int V, int use_l2norm, float scale, void* out, int32_t* status) {
   if (T < 0 || S < 0 || H < 1 || HV < H || HV % H || V < 16 || V % 16 || nslots < 1) return CFH_E_INVALID;
-  if (K != GDN_DK || S > GDN_SEQS) return CFH_E_UNSUPPORTED;
+  if (K != GDN_DK || S > GDN_SEQS || 2ll * H * K + (long long)HV * V > 1 << 20) return CFH_E_UNSUPPORTED;
   if (T == 0 || S == 0) return CFH_OK;
   if (!mixed_qkv || !a || !b || !A_log || !dt_bias || !ssm_state || !slots || !out) return CFH_E_INVALID;
   if (((uintptr_t)mixed_qkv | (uintptr_t)ssm_state) % 16 || (uintptr_t)out % 2) return CFH_E_INVALID;
@@ -760,8 +774,8 @@ int cfh_gdn_prefill(const void* mixed_qkv, const void* a, const void* b, const f
   if (prep > 0x7fffffffll || blocks > 0x7fffffffll) return CFH_E_UNSUPPORTED;
   hipLaunchKernelGGL(k_gdn_prep, dim3((unsigned)prep), dim3(256), 0, st, g, (char*)ws);
   CFH_LAUNCH_CHECK();
-  if (state_bf16) hipLaunchKernelGGL(k_gdn_chunks<uint16_t>, dim3((unsigned)blocks), dim3(512), 0, st, g, (const char*)ws);
-  else hipLaunchKernelGGL(k_gdn_chunks<float>, dim3((unsigned)blocks), dim3(512), 0, st, g, (const char*)ws);
+  if (state_bf16) hipLaunchKernelGGL(k_gdn_chunks<uint16_t>, dim3((unsigned)blocks), dim3(768), 0, st, g, (const char*)ws);
+  else hipLaunchKernelGGL(k_gdn_chunks<float>, dim3((unsigned)blocks), dim3(768), 0, st, g, (const char*)ws);
   CFH_LAUNCH_CHECK();
   return CFH_OK;
 }
