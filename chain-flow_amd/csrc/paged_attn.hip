@@ -18,6 +18,7 @@
 // The long axis is cut into pieces of `piece` tokens where the rows alone do not fill the chip; k_attn_join
 // then merges the pieces' (max, sum, O).
 #include "cfh_host.h"
+#include "cfh_kernels.h"
 #include "cfh_kv.h"
 #include "cfh_tr.h"
 
@@ -40,7 +41,7 @@ struct PagedArgs {
   float* po;                   // pieces' O [npiece][T][H][D] (npiece > 1)
   float2* pml;                 // pieces' (max in log2 units, sum) [npiece][T][H]
   long long q_ld, o_ld, bs_k, bs_v;
-  unsigned long long pmagic;   // j / page = j * pmagic >> pshift, j < 2^31
+  unsigned pmagic;             // j / page = (2 j * pmagic >> 32) >> pshift, j < 2^30
   int pshift;
   int T, H, Hkv, G, S, blocks, page, table_ld, max_blocks, causal;
   int piece, npiece, tiles;    // tokens a piece, pieces, row-tile slots
@@ -52,7 +53,7 @@ struct PagedArgs {
 // Whether a sequence's rows lie in the query.
 __device__ __forceinline__ bool bounds_ok(const PagedArgs& a, int c0, int c1) { return c0 >= 0 && c0 <= c1 && c1 <= a.T; }
 
-__device__ __forceinline__ int page_of(const PagedArgs& a, int j) { return (int)(((unsigned long long)(unsigned)j * a.pmagic) >> a.pshift); }
+__device__ __forceinline__ int page_of(const PagedArgs& a, int j) { return (int)(__umulhi((unsigned)j << 1, a.pmagic) >> a.pshift); }
 
 // Row-tile slot -> (sequence, tile): sequence s has the slots from floor(cu[s] G / R) + s on, at most
 // ceil(n G / R) of them used, so no two sequences share one.  A search over 64 sequences a step.
@@ -86,7 +87,7 @@ __device__ __forceinline__ int seen(const PagedArgs& a, int len, int n, int i) {
   return a.causal ? max(0, min(len, len - n + i + 1)) : len;
 }
 
-template <int R, bool FEW>
+template <int R, bool ROWS>
 __device__ __forceinline__ bool find_work(const PagedArgs& a, Work& w) {
   // (kv head, piece) groups and row tiles: consecutive workgroups go to the eight XCDs in turn, and each XCD
   // has its own L2, so a group's row tiles, which read the same tokens, are kept on one XCD (or an even share
@@ -108,13 +109,14 @@ __device__ __forceinline__ bool find_work(const PagedArgs& a, Work& w) {
   if (g >= groups || t >= a.tiles) return false;
   w.hk = g % a.Hkv;
   w.piece = g / a.Hkv;
-  int tile;
-  if (!find_tile<R>(a, a.tiles - 1 - t, w.s, tile)) return false;   // (late rows see the most: first)
+  int tile = 0;
+  if (ROWS && a.few) w.s = t;      // (beside k_attn_tiles: one tile of a.few rows a sequence)
+  else if (!find_tile<R>(a, a.tiles - 1 - t, w.s, tile)) return false;   // (late rows see the most: first)
   w.c0 = a.cu[w.s];
   const int c1 = a.cu[w.s + 1];
   if (!bounds_ok(a, w.c0, c1)) return false;
   w.n = c1 - w.c0;
-  if (FEW ? (a.few && (long long)w.n * a.G > a.few) : (long long)w.n * a.G <= a.few) return false;
+  if (ROWS ? (a.few && (long long)w.n * a.G > a.few) : (long long)w.n * a.G <= a.few) return false;
   w.r0 = tile * R;
   if (w.r0 >= w.n * a.G) return false;
   w.len = a.lens[w.s];
@@ -134,34 +136,43 @@ __device__ __forceinline__ void check_bounds(const PagedArgs& a) {
       if (!bounds_ok(a, a.cu[i], a.cu[i + 1])) a.status[0] = 1;
 }
 
-// The block of token j, or -1 where j is not below j1; a block outside the cache is noted.
-__device__ __forceinline__ int block_of(const PagedArgs& a, const Work& w, int j, int* first_bad) {
-  if (j >= w.j1) return -1;
-  const int b = a.table[(size_t)w.s * a.table_ld + page_of(a, j)];
-  if (b >= 0 && b < a.blocks) return b;
-  atomicMin(first_bad, j);
-  return -1;
+// Where token j lies: its block (-1 where j is not below j1, or the block outside the cache, which is noted) and
+// its row in the block.
+struct Place { int blk, row; };
+__device__ __forceinline__ Place place_of(const PagedArgs& a, const Work& w, int j, int* first_bad) {
+  const int p = page_of(a, j);
+  Place at = {-1, j - p * a.page};
+  if (j < w.j1) {
+    at.blk = a.table[(size_t)w.s * a.table_ld + p];
+    if ((unsigned)at.blk >= (unsigned)a.blocks) {
+      atomicMin(first_bad, j);
+      at.blk = -1;
+    }
+  }
+  return at;
 }
 
-// 8 elements of the row of token j (block b >= 0) as the 2-byte type; zero where b < 0, so that nothing that
-// lies past a sequence's tokens reaches a product.
+// 8 elements of a token's row as they lie in memory; zero where there is no block, so that nothing that lies past
+// a sequence's tokens reaches a product.
 template <bool F8>
-__device__ __forceinline__ uint4 load_row(const PagedArgs& a, const void* c, long long bs, int b, int j, int hk, int D, int col) {
-  if (b < 0) return make_uint4(0, 0, 0, 0);
-  const int at = j - page_of(a, j) * a.page;
-  const size_t i = (size_t)b * bs + ((size_t)at * a.Hkv + hk) * D + col;
-  if constexpr (F8) {
-    const uint2 r = *(const uint2*)((const uint8_t*)c + i);
-    return make_uint4(r.x, r.y, 0, 0);
-  } else {
-    return *(const uint4*)((const u16*)c + i);
+__device__ __forceinline__ uint4 load_row(const PagedArgs& a, const void* c, long long bs, const Place& at, int hk, int D, int col) {
+  uint4 r = make_uint4(0, 0, 0, 0);
+  if (at.blk >= 0) {
+    const size_t i = (size_t)(unsigned)at.blk * (size_t)bs + (unsigned)((at.row * a.Hkv + hk) * D + col);
+    if constexpr (F8) {
+      const uint2 x = *(const uint2*)((const uint8_t*)c + i);
+      r.x = x.x;
+      r.y = x.y;
+    } else {
+      r = *(const uint4*)((const u16*)c + i);
+    }
   }
+  return r;
 }
 template <bool F8>
-__device__ __forceinline__ int load_exp(const PagedArgs& a, const uint8_t* ex, int b, int j, int hk) {
-  if (!F8 || b < 0) return 127;
-  const int at = j - page_of(a, j) * a.page;
-  return ex[((size_t)b * a.page + at) * a.Hkv + hk];
+__device__ __forceinline__ int load_exp(const PagedArgs& a, const uint8_t* ex, const Place& at, int hk) {
+  if (!F8 || at.blk < 0) return 127;
+  return ex[((size_t)at.blk * a.page + at.row) * a.Hkv + hk];
 }
 template <bool BF, bool F8>
 __device__ __forceinline__ uint4 to_rows(const uint4& r, int code) {
@@ -198,20 +209,35 @@ __device__ __forceinline__ bool any_nonfinite(const uint4& r) {
   }
   return f;
 }
-// The same elements with what is not finite replaced: kind 0 by zero; kinds 1 and 2 keep only that, as 1 where
-// the element is +inf or NaN (1), or -inf or NaN (2), and 0 elsewhere.
+// The same elements with zeros for those.
 template <bool BF>
-__device__ __forceinline__ unsigned only_finite(unsigned w, int kind) {
-  constexpr unsigned E = BF ? 0x7f80u : 0x7c00u, M = BF ? 0x7fu : 0x3ffu, ONE = BF ? 0x3f80u : 0x3c00u;
-  unsigned o = 0;
+__device__ __forceinline__ uint4 only_finite(const uint4& r) {
+  constexpr unsigned E = BF ? 0x7f80u : 0x7c00u;
+  auto two = [](unsigned w) { return ((w & E) == E ? 0u : w & 0xffffu) | ((w & (E << 16)) == (E << 16) ? 0u : w & 0xffff0000u); };
+  return make_uint4(two(r.x), two(r.y), two(r.z), two(r.w));
+}
+
+// Values that are not finite and that some rows of the tile do not see: 0 * NaN must not reach those.  In token
+// tiles that not every row sees whole they enter LDS as zeros and their tokens are noted (bit j - base of
+// `odd`); at the end each row adds those it sees to its results, where they decide by themselves.
+template <bool BF, bool F8>
+__device__ __forceinline__ void add_odd(const PagedArgs& a, const Work& w, unsigned* odd, int words, int base, int vis, int col,
+                                        int D, float (&o)[4]) {
+  for (int i = 0; i < words; ++i)
+    for (unsigned m = odd[i]; m; m &= m - 1) {
+      const int j = base + 32 * i + __builtin_ctz(m);
+      if (j >= vis) break;
+      const int p = page_of(a, j);                                       // (noted tokens lie in blocks of the cache)
+      const Place at = {a.table[(size_t)w.s * a.table_ld + p], j - p * a.page};
+      const uint4 r = to_rows<BF, F8>(load_row<F8>(a, a.vc, a.bs_v, at, w.hk, D, col & ~7), load_exp<F8>(a, a.ve, at, w.hk));
+      float x[8];
+      widen8<BF>(r, x);
 #pragma unroll
-  for (int h = 0; h < 32; h += 16) {
-    const unsigned e = (w >> h) & 0xffffu;
-    const bool inf = (e & E) == E, nan = inf && (e & M), neg = e >> 15;
-    const unsigned x = kind == 0 ? (inf ? 0u : e) : (inf && (nan || neg == (kind == 2)) ? ONE : 0u);
-    o |= x << h;
-  }
-  return o;
+      for (int e = 0; e < 4; ++e) {
+        const float v = col & 4 ? x[4 + e] : x[e];
+        if (!(fabsf(v) < INFINITY)) o[e] += v;
+      }
+    }
 }
 
 constexpr float LAZY = 8.f;   // log2 units the running maximum may lag behind (probabilities up to 2^8)
@@ -221,19 +247,23 @@ constexpr float LAZY = 8.f;   // log2 units the running maximum may lag behind (
 // global -> registers -> LDS one tile ahead (the 8-bit cache is widened on that way), double-buffered, one
 // barrier a tile.
 template <bool BF, bool F8, int D, int NW, int TK>
-__global__ void __launch_bounds__(NW * 64) k_attn_tiles(PagedArgs a) {
+__global__ void __launch_bounds__(NW * 64, 2) k_attn_tiles(PagedArgs a) {
   constexpr int R = NW * 32, NT = NW * 64;
   constexpr int CH = D / 8;                       // 16-byte chunks a token's row
   constexpr int CPT = TK * CH / NT;               // chunks a thread stages (of K, and of V)
   constexpr int RS = NT / CH;                     // tokens between a thread's chunks
-  static_assert(CPT >= 1 && TK % 32 == 0, "a tile is at least a chunk a thread");
+  static_assert(CPT >= 1 && TK % 32 == 0 && RS % 8 == 0, "a tile is at least a chunk a thread; one chunk order a thread");
   __shared__ __align__(16) u16 lds[2][2][TK * D];
-  __shared__ int first_bad, odd[2];
+  // the tokens that some but not all rows see lie within R of each other, and a tile on either side
+  constexpr int OW = (R + 2 * TK + 31) / 32;
+  __shared__ int first_bad;
+  __shared__ unsigned odd[OW];
   check_bounds(a);
   Work w;
   if (!find_work<R, false>(a, w)) return;         // (the whole workgroup)
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5;
-  if (tid == 0) { first_bad = 0x7fffffff; odd[0] = odd[1] = -1; }
+  if (tid == 0) first_bad = 0x7fffffff;
+  if (tid < OW) odd[tid] = 0;
   __syncthreads();
 
   const int r = w.r0 + wave * 32 + (lane & 31), rows = w.n * a.G;
@@ -256,49 +286,62 @@ __global__ void __launch_bounds__(NW * 64) k_attn_tiles(PagedArgs a) {
   }
 
   const int srow = tid / CH, scol = tid % CH;     // this thread's chunks: tokens srow + RS x, chunk scol
+  const int sat = srow * D + ((scol ^ swz(srow)) * 8);   // (swz has a period of 8 tokens)
+  // Operand addresses: chunk c of a token lies at c ^ z, z below 8, so only c % 8 takes part and the rest, like
+  // the rows of a tile, is an offset in the instruction
+  int ka[4], va[2];
+  {
+    const int kt = lane & 31, vt = 4 * half + (lane & 15) / 4, vc = 2 * ((lane >> 4) & 1) + (lane & 3) / 2;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ka[i] = kt * D + (((2 * i + half) ^ swz(kt)) * 8);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) va[i] = vt * D + (((4 * i + vc) ^ swz(vt)) * 8) + 4 * (lane & 1);
+  }
   uint4 kr[CPT], vr[CPT];
-  int kx[CPT], vx[CPT], blk[CPT];
+  int kx[CPT], vx[CPT];
+  Place pl[CPT];
   auto blocks = [&](int jt) {
 #pragma unroll
-    for (int x = 0; x < CPT; ++x) blk[x] = block_of(a, w, jt + srow + RS * x, &first_bad);
+    for (int x = 0; x < CPT; ++x) pl[x] = place_of(a, w, jt + srow + RS * x, &first_bad);
   };
-  auto fetch = [&](int jt) {
+  auto fetch = [&]() {
 #pragma unroll
     for (int x = 0; x < CPT; ++x) {
-      const int j = jt + srow + RS * x;
-      kr[x] = load_row<F8>(a, a.kc, a.bs_k, blk[x], j, w.hk, D, scol * 8);
-      vr[x] = load_row<F8>(a, a.vc, a.bs_v, blk[x], j, w.hk, D, scol * 8);
-      kx[x] = load_exp<F8>(a, a.ke, blk[x], j, w.hk);
-      vx[x] = load_exp<F8>(a, a.ve, blk[x], j, w.hk);
+      kr[x] = load_row<F8>(a, a.kc, a.bs_k, pl[x], w.hk, D, scol * 8);
+      vr[x] = load_row<F8>(a, a.vc, a.bs_v, pl[x], w.hk, D, scol * 8);
+      kx[x] = load_exp<F8>(a, a.ke, pl[x], w.hk);
+      vx[x] = load_exp<F8>(a, a.ve, pl[x], w.hk);
     }
   };
+  const int odd_base = w.j0 + max(0, vis_wg - w.j0) / TK * TK;   // the first tile that not every row sees whole
   auto stage = [&](int jt, int buf) {
-    bool f = false;
 #pragma unroll
     for (int x = 0; x < CPT; ++x) {
-      const int tok = srow + RS * x, at = tok * D + ((scol ^ swz(tok)) * 8);
-      const uint4 v = to_rows<BF, F8>(vr[x], vx[x]);
+      const int tok = srow + RS * x, at = sat + RS * x * D;
+      uint4 v = to_rows<BF, F8>(vr[x], vx[x]);
       *(uint4*)&lds[buf][0][at] = to_rows<BF, F8>(kr[x], kx[x]);
+      if (jt + TK > vis_wg && any_nonfinite<BF>(v)) {
+        v = only_finite<BF>(v);
+        atomicOr(&odd[(jt + tok - odd_base) / 32], 1u << ((jt + tok - odd_base) & 31));
+      }
       *(uint4*)&lds[buf][1][at] = v;
-      if (jt + TK > vis_wg) f |= any_nonfinite<BF>(v);
     }
-    if (f) odd[buf] = jt;                         // a tile that some rows see in part holds what is not finite
   };
 
   f32x16 o[D / 32] = {};
   float m = -INFINITY, l = 0.f;                   // (m in log2 units; l: this half's tokens)
   if (w.j0 < w.j1) {
     blocks(w.j0);
-    fetch(w.j0);
+    fetch();
     blocks(w.j0 + TK);
     stage(w.j0, 0);
   }
   int buf = 0;
   for (int jt = w.j0; jt < w.j1; jt += TK, buf ^= 1) {
-    __syncthreads();
+    lds_barrier();
     const bool more = jt + TK < w.j1;
     if (more) {
-      fetch(jt + TK);
+      fetch();
       blocks(jt + 2 * TK);
     }
     if (jt < w.j1 && w.r0 + wave * 32 < rows) {
@@ -308,12 +351,9 @@ __global__ void __launch_bounds__(NW * 64) k_attn_tiles(PagedArgs a) {
 #pragma unroll
       for (int b = 0; b < TK / 32; ++b) {
         sc[b] = f32x16{};
-        const int tok = 32 * b + (lane & 31);
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-          const uint4 kf = *(const uint4*)&kt[tok * D + (((2 * s + half) ^ swz(tok)) * 8)];
-          sc[b] = mfma32<BF>(kf, qf[s], sc[b]);
-        }
+        for (int s = 0; s < D / 16; ++s)
+          sc[b] = mfma32<BF>(*(const uint4*)&kt[ka[s & 3] + 32 * b * D + s / 4 * 64], qf[s], sc[b]);
       }
       if (jt + TK > vis_wave) {
 #pragma unroll
@@ -352,51 +392,15 @@ __global__ void __launch_bounds__(NW * 64) k_attn_tiles(PagedArgs a) {
                                      pack2<BF>(sc[b][8 * s + 4], sc[b][8 * s + 5]), pack2<BF>(sc[b][8 * s + 6], sc[b][8 * s + 7]));
       }
       // the transposed reads: lane block (lane / 16) % 2 takes 16 of the 32 columns, half the tokens 4 half ..
-      const int tr = 4 * half + (lane & 15) / 4, cl = 2 * ((lane >> 4) & 1) + (lane & 3) / 2, by = 4 * (lane & 1);
       auto vfrag = [&](int d, int s) {
-        const int t0 = 16 * s + tr, t1 = t0 + 8;
-        const uint2 x = read_tr(&vt[t0 * D + (((4 * d + cl) ^ swz(t0)) * 8) + by]);
-        const uint2 y = read_tr(&vt[t1 * D + (((4 * d + cl) ^ swz(t1)) * 8) + by]);
+        const u16* p = &vt[va[d & 1] + 16 * s * D + d / 2 * 64];
+        const uint2 x = read_tr(p), y = read_tr(p + 8 * D);
         return make_uint4(x.x, x.y, y.x, y.y);
       };
-      if (odd[buf] != jt) {
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d)
+      for (int s = 0; s < TK / 16; ++s)
 #pragma unroll
-          for (int s = 0; s < TK / 16; ++s) o[d] = mfma32<BF>(vfrag(d, s), pf[s], o[d]);
-      } else {
-        // a value that is not finite and that some of the rows do not see: 0 * NaN must not reach those.  The
-        // finite values as ever; then the others as ones, times ones where a row sees the token
-        uint4 pi[TK / 16];
-        constexpr unsigned ONE = BF ? 0x3f80u : 0x3c00u;
-#pragma unroll
-        for (int s = 0; s < TK / 16; ++s) {
-          unsigned b[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = jt + 16 * s + 8 * (e / 2) + 4 * half + 2 * (e % 2);
-            b[e] = (j < vis ? ONE : 0u) | (j + 1 < vis ? ONE << 16 : 0u);
-          }
-          pi[s] = make_uint4(b[0], b[1], b[2], b[3]);
-        }
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) {
-          f32x16 up = {}, down = {};
-#pragma unroll
-          for (int s = 0; s < TK / 16; ++s) {
-            const uint4 v = vfrag(d, s);
-            auto as = [&](int kind) {
-              return make_uint4(only_finite<BF>(v.x, kind), only_finite<BF>(v.y, kind), only_finite<BF>(v.z, kind),
-                                only_finite<BF>(v.w, kind));
-            };
-            o[d] = mfma32<BF>(as(0), pf[s], o[d]);
-            up = mfma32<BF>(as(1), pi[s], up);
-            down = mfma32<BF>(as(2), pi[s], down);
-          }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[d][e] += (up[e] > 0.f ? INFINITY : 0.f) + (down[e] > 0.f ? -INFINITY : 0.f);
-        }
-      }
+        for (int d = 0; d < D / 32; ++d) o[d] = mfma32<BF>(vfrag(d, s), pf[s], o[d]);
     }
     if (more) stage(jt + TK, buf ^ 1);
   }
@@ -427,6 +431,27 @@ __global__ void __launch_bounds__(NW * 64) k_attn_tiles(PagedArgs a) {
         *(float4*)(po + 32 * d + 8 * g) = make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
     if (half == 0) a.pml[at] = make_float2(m, l);
   }
+  unsigned any = 0;
+#pragma unroll
+  for (int x = 0; x < OW; ++x) any |= odd[x];
+  if (any) {                                      // (to what was just stored: the sums stay in registers)
+#pragma unroll 1
+    for (int c = 4 * half; c < D; c += 8) {
+      float y[4] = {0.f, 0.f, 0.f, 0.f};
+      add_odd<BF, F8>(a, w, odd, OW, odd_base, vis, c, D, y);
+      if (a.npiece == 1) {
+        u16* out = a.out + (size_t)t * a.o_ld + (size_t)h * D + c;
+        for (int e = 0; e < 4; ++e) {
+          float was[8];
+          widen8<BF>(make_uint4(out[e], 0, 0, 0), was);
+          out[e] = (u16)pack2<BF>(was[0] + y[e], 0.f);
+        }
+      } else {
+        float* po = a.po + (((size_t)w.piece * a.T + t) * a.H + h) * D + c;
+        for (int e = 0; e < 4; ++e) po[e] += y[e];
+      }
+    }
+  }
 }
 
 // Few rows: a tile of 16, one workgroup of four waves a (row tile, kv head, piece), each wave the tokens of
@@ -456,11 +481,12 @@ __global__ void __launch_bounds__(256) k_attn_rows(PagedArgs a) {
   __shared__ __align__(16) union { u16 v[NW][16 * D]; float o[NW][16 * D]; } sh;
   __shared__ float2 ml[NW][16];
   __shared__ int first_bad;
+  __shared__ unsigned odd[2];                     // (the tokens not all rows see: 16, and a group on either side)
   check_bounds(a);
   Work w;
   if (!find_work<R, true>(a, w)) return;          // (the whole workgroup)
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, tl = lane & 15;
-  if (tid == 0) first_bad = 0x7fffffff;
+  if (tid == 0) { first_bad = 0x7fffffff; odd[0] = odd[1] = 0; }
   __syncthreads();
   const int rows = w.n * a.G, r = w.r0 + tl;
   const int i = min(r, rows - 1) / a.G, hh = min(r, rows - 1) % a.G;
@@ -480,54 +506,61 @@ __global__ void __launch_bounds__(256) k_attn_rows(PagedArgs a) {
     }
   }
   u16* const vt = sh.v[wave];
+  int va[4];                                      // (as in k_attn_tiles)
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int tr = 4 * g + tl / 4;
+    va[i] = tr * D + (((2 * i + (tl & 3) / 2) ^ swz(tr)) * 8) + 4 * (tl & 1);
+  }
   uint4 kr[KL], vr[VPT];
-  int kx = 127, vx[VPT], kb = -1, vb[VPT];
+  int kx = 127, vx[VPT];
+  Place kb, vb[VPT];
   // this lane's token of K is tl; its chunks of V are tokens (lane + 64 x) / CH
   auto blocks = [&](int jt) {
-    kb = block_of(a, w, jt + tl, &first_bad);
+    kb = place_of(a, w, jt + tl, &first_bad);
 #pragma unroll
-    for (int x = 0; x < VPT; ++x) vb[x] = block_of(a, w, jt + (lane + 64 * x) / CH, &first_bad);
+    for (int x = 0; x < VPT; ++x) vb[x] = place_of(a, w, jt + (lane + 64 * x) / CH, &first_bad);
   };
-  auto fetch = [&](int jt) {
+  auto fetch = [&]() {
 #pragma unroll
     for (int s = 0; s < KL; ++s) {
       if constexpr (F8) {
         kr[s] = make_uint4(0, 0, 0, 0);
-        if (kb >= 0) {
-          const int j = jt + tl, at = j - page_of(a, j) * a.page;
-          kr[s] = *(const uint4*)((const uint8_t*)a.kc + (size_t)kb * a.bs_k + ((size_t)at * a.Hkv + w.hk) * D + 64 * s + 16 * g);
-        }
+        if (kb.blk >= 0)
+          kr[s] = *(const uint4*)((const uint8_t*)a.kc + (size_t)(unsigned)kb.blk * (size_t)a.bs_k +
+                                  (unsigned)((kb.row * a.Hkv + w.hk) * D + 64 * s + 16 * g));
       } else {
-        kr[s] = load_row<false>(a, a.kc, a.bs_k, kb, jt + tl, w.hk, D, 32 * s + 8 * g);
+        kr[s] = load_row<false>(a, a.kc, a.bs_k, kb, w.hk, D, 32 * s + 8 * g);
       }
     }
-    kx = load_exp<F8>(a, a.ke, kb, jt + tl, w.hk);
+    kx = load_exp<F8>(a, a.ke, kb, w.hk);
 #pragma unroll
     for (int x = 0; x < VPT; ++x) {
-      const int c = lane + 64 * x, j = jt + c / CH;
-      vr[x] = load_row<F8>(a, a.vc, a.bs_v, vb[x], j, w.hk, D, (c % CH) * 8);
-      vx[x] = load_exp<F8>(a, a.ve, vb[x], j, w.hk);
+      vr[x] = load_row<F8>(a, a.vc, a.bs_v, vb[x], w.hk, D, (lane + 64 * x) % CH * 8);
+      vx[x] = load_exp<F8>(a, a.ve, vb[x], w.hk);
     }
   };
   f32x4 o[D / 16] = {};
   float m = -INFINITY, l = 0.f;
   const int step = 16 * NW;
+  const int odd_base = w.j0 + max(0, vis_all - w.j0) / 16 * 16;   // the first group that not every row sees whole
   int jt = w.j0 + 16 * wave;
   if (jt < w.j1) {
     blocks(jt);
-    fetch(jt);
+    fetch();
     blocks(jt + step);
   }
   for (; jt < w.j1; jt += step) {
-    bool f = false;
 #pragma unroll
     for (int x = 0; x < VPT; ++x) {
       const int c = lane + 64 * x, tok = c / CH;
-      const uint4 v = to_rows<BF, F8>(vr[x], vx[x]);
+      uint4 v = to_rows<BF, F8>(vr[x], vx[x]);
+      if (jt + 16 > vis_all && any_nonfinite<BF>(v)) {
+        v = only_finite<BF>(v);
+        atomicOr(&odd[(jt + tok - odd_base) / 32], 1u << ((jt + tok - odd_base) & 31));
+      }
       *(uint4*)&vt[tok * D + (((c % CH) ^ swz(tok)) * 8)] = v;
-      f |= jt + 16 > vis_all && any_nonfinite<BF>(v);
     }
-    const bool odd = __any(f);
     uint4 kf[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -535,7 +568,7 @@ __global__ void __launch_bounds__(256) k_attn_rows(PagedArgs a) {
       else kf[s] = kr[s];
     }
     if (jt + step < w.j1) {
-      fetch(jt + step);
+      fetch();
       blocks(jt + 2 * step);
     }
     f32x4 sc = {};
@@ -566,26 +599,9 @@ __global__ void __launch_bounds__(256) k_attn_rows(PagedArgs a) {
     }
     const uint2 pf = make_uint2(pack2<BF>(sc[0], sc[1]), pack2<BF>(sc[2], sc[3]));
     // (a wave's LDS accesses complete in order: its reads see its own writes above)
-    const int tr = 4 * g + tl / 4;
-    auto vfrag = [&](int d) { return read_tr(&vt[tr * D + (((2 * d + (tl & 3) / 2) ^ swz(tr)) * 8) + 4 * (tl & 1)]); };
-    if (!odd) {
+    auto vfrag = [&](int d) { return read_tr(&vt[va[d & 3] + d / 4 * 64]); };
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d) o[d] = mfma16h<BF>(vfrag(d), pf, o[d]);
-    } else {                                      // (as in k_attn_tiles)
-      constexpr unsigned ONE = BF ? 0x3f80u : 0x3c00u;
-      const int j = jt + 4 * g;
-      const uint2 pi = make_uint2((j < vis ? ONE : 0u) | (j + 1 < vis ? ONE << 16 : 0u),
-                                  (j + 2 < vis ? ONE : 0u) | (j + 3 < vis ? ONE << 16 : 0u));
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
-        const uint2 v = vfrag(d);
-        auto as = [&](int kind) { return make_uint2(only_finite<BF>(v.x, kind), only_finite<BF>(v.y, kind)); };
-        o[d] = mfma16h<BF>(as(0), pf, o[d]);
-        const f32x4 up = mfma16h<BF>(as(1), pi, f32x4{}), down = mfma16h<BF>(as(2), pi, f32x4{});
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[d][e] += (up[e] > 0.f ? INFINITY : 0.f) + (down[e] > 0.f ? -INFINITY : 0.f);
-      }
-    }
+    for (int d = 0; d < D / 16; ++d) o[d] = mfma16h<BF>(vfrag(d), pf, o[d]);
   }
   // the four waves' join: each row's maximum, then the sums of what the waves hold under it
   l += __shfl_xor(l, 16);
@@ -615,6 +631,11 @@ __global__ void __launch_bounds__(256) k_attn_rows(PagedArgs a) {
       sum += *(const f32x4*)&sh.o[v][row * D + 16 * ((col / 16) ^ (row & (D / 16 - 1))) + col % 16];
       ls += ml[v][row].x == -INFINITY ? ml[v][row].y : ml[v][row].y * __builtin_amdgcn_exp2f(ml[v][row].x - mr);
     }
+    if (odd[0] | odd[1]) {
+      float y[4] = {sum[0], sum[1], sum[2], sum[3]};
+      add_odd<BF, F8>(a, w, odd, 2, odd_base, min(seen(a, w.len, w.n, ti), w.j1), col, D, y);
+      sum = f32x4{y[0], y[1], y[2], y[3]};
+    }
     if (w.bad || first_bad < min(seen(a, w.len, w.n, ti), w.j1)) {
       ls = __builtin_nanf("");
       if (a.status) a.status[0] = 1;
@@ -632,15 +653,15 @@ __global__ void __launch_bounds__(256) k_attn_rows(PagedArgs a) {
   }
 }
 
-// The pieces of each (row, head) in piece order: the largest maximum, then the sums under it.  A wave a
-// (row, head), D / 64 columns a lane.
+// The pieces of each (row, head): the largest maximum, then the sums under it, in piece order.  A workgroup of
+// four waves a (row, head), the waves a quarter of the pieces each, 4 pieces' loads in flight, D / 64 columns a
+// lane.
 template <bool BF, int D>
 __global__ void __launch_bounds__(256) k_attn_join(PagedArgs a) {
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63;
-  const long long gw = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int t = (int)(gw / a.H), h = (int)(gw - (long long)t * a.H);
-  if (t >= a.T) return;
+  constexpr int E = D / 64, B = 4;
+  __shared__ float so[4][D], sl[4];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int t = blockIdx.x / a.H, h = blockIdx.x % a.H;
   int s = 0, n = a.S;                             // the last sequence with cu[s] <= t (64 a step)
   while (n > 1) {
     const int step = (n + 63) / 64, i = s + lane * step;
@@ -653,30 +674,49 @@ __global__ void __launch_bounds__(256) k_attn_join(PagedArgs a) {
   if (t < c0 || t >= c1 || !bounds_ok(a, c0, c1)) return;   // a row of no sequence
   int len = a.lens[s];
   if (len < 0 || len > (long long)a.max_blocks * a.page) len = 0;
-  // a piece of the row's tile exists while it starts below what the row itself sees (and the first always)
-  const int vis = seen(a, len, c1 - c0, t - c0);
-  const int np = max(1, min(a.npiece, (vis + a.piece - 1) / a.piece));
+  // the row's pieces: those that start below what it sees, and the first always
+  const int np = max(1, min(a.npiece, (seen(a, len, c1 - c0, t - c0) + a.piece - 1) / a.piece));
+  const size_t row = (size_t)t * a.H + h, rows = (size_t)a.T * a.H;
   float m = -INFINITY;
-  for (int p = lane; p < np; p += 64) m = fmaxf(m, a.pml[((size_t)p * a.T + t) * a.H + h].x);
+  for (int p = lane; p < np; p += 64) m = fmaxf(m, a.pml[p * rows + row].x);
   m = wave_max(m);
   float l = 0.f, o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int p = 0; p < np; ++p) {
-    const size_t at = ((size_t)p * a.T + t) * a.H + h;
-    const float2 x = a.pml[at];
-    const float f = x.x == -INFINITY ? (x.y == 0.f ? 0.f : x.y) : __builtin_amdgcn_exp2f(x.x - m);
-    l += x.x == -INFINITY ? x.y : x.y * f;
-    const float* po = a.po + at * D + lane * E;
-    if (x.x != -INFINITY || x.y != 0.f)
+  const int per = (np + 3) / 4, p1 = min(np, (wave + 1) * per);
+  for (int p = wave * per; p < p1; p += B) {
+    float2 x[B];
+    float y[B][E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] += po[e] * f;
+    for (int i = 0; i < B; ++i) {
+      const size_t at = min(p + i, p1 - 1) * rows + row;
+      x[i] = a.pml[at];
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[i][e] = a.po[at * D + lane * E + e];
+    }
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      if (p + i >= p1) break;
+      // (a piece that saw nothing: maximum -inf, sum 0, or NaN for a bad table)
+      const float f = x[i].x == -INFINITY ? x[i].y : __builtin_amdgcn_exp2f(x[i].x - m);
+      l += x[i].x == -INFINITY ? x[i].y : x[i].y * f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] += y[i][e] * f;
+    }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  u16* out = a.out + (size_t)t * a.o_ld + (size_t)h * D + lane * E;
 #pragma unroll
-  for (int e = 0; e < E; ++e) out[e] = (u16)pack2<BF>(o[e] * inv, 0.f);
-  if (lane == 0) a.lse[(size_t)h * a.T + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
+  for (int e = 0; e < E; ++e) so[wave][lane * E + e] = o[e];
+  if (lane == 0) sl[wave] = l;
+  __syncthreads();
+  l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (threadIdx.x < D / 2) {
+    const int c = threadIdx.x * 2;
+    const float x = (so[0][c] + so[1][c]) + (so[2][c] + so[3][c]);
+    const float y = (so[0][c + 1] + so[1][c + 1]) + (so[2][c + 1] + so[3][c + 1]);
+    *(unsigned*)(a.out + (size_t)t * a.o_ld + (size_t)h * D + c) = pack2<BF>(x * inv, y * inv);
+  }
+  if (threadIdx.x == 0) a.lse[(size_t)h * a.T + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
 }
 
 // How a call is split, from what the host knows (sizes and an upper bound of the lengths).
@@ -687,9 +727,11 @@ struct Plan {
   int piece, npiece;
 };
 
-constexpr int TILE_ROWS = 128, FEW_ROWS = 16, PIECE_MIN = 256, FILL = 512;
+constexpr int FEW_ROWS = 16, PIECE_MIN = 256, FILL = 512;
 
-Plan plan(int T, int H, int Hkv, int S, int max_len) {
+constexpr int tile_rows(int D) { return D == 256 ? 256 : 128; }
+
+Plan plan(int T, int H, int Hkv, int D, int S, int max_len) {
   const int G = H / Hkv;
   Plan p = {};
   const long long packed = (long long)T * G;
@@ -701,12 +743,12 @@ Plan plan(int T, int H, int Hkv, int S, int max_len) {
     p.rows = true;
     p.few = FEW_ROWS;
   }
-  p.nrow = (int)(packed / FEW_ROWS) + S;
-  p.ntile = (int)(packed / TILE_ROWS) + S;
+  p.nrow = p.few ? S : (int)(packed / FEW_ROWS) + S;
+  p.ntile = (int)(packed / tile_rows(D)) + S;
   // pieces so that (rows' tiles) x (kv heads) x pieces fill the chip: FILL workgroups, none shorter than
   // PIECE_MIN tokens
-  const long long items = (long long)Hkv * (p.tiles ? (packed + TILE_ROWS - 1) / TILE_ROWS : S);
-  const long long want = std::max(1ll, (FILL + items - 1) / items);
+  const long long items = (long long)Hkv * (p.tiles ? (packed + tile_rows(D) - 1) / tile_rows(D) : S);
+  const long long want = items >= FILL / 2 ? 1 : (FILL + items - 1) / items;
   long long piece = ((long long)max_len + want - 1) / want;
   piece = std::max<long long>(PIECE_MIN, (piece + 63) / 64 * 64);
   p.npiece = (int)std::max(1ll, ((long long)max_len + piece - 1) / piece);
@@ -723,7 +765,7 @@ extern "C" {
 int64_t cfh_paged_attn_ws_bytes(int T, int H, int Hkv, int D, int S, int max_len) {
   if (T < 0 || H < 1 || Hkv < 1 || H % Hkv || S < 0 || max_len < 0 || D < 1) return -1;
   if (T == 0 || S == 0) return 0;
-  const Plan p = plan(T, H, Hkv, S, max_len);
+  const Plan p = plan(T, H, Hkv, D, S, max_len);
   if (p.npiece == 1) return 0;
   return po_bytes(p, T, H, D) + (int64_t)cfh::align256((size_t)p.npiece * T * H * sizeof(float2));
 }
@@ -743,13 +785,14 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
   const bool f8 = k_exp || v_exp;
   if (!k_cache || !v_cache || (f8 && (!k_exp || !v_exp))) return CFH_E_INVALID;
   const long long inner = (long long)page * Hkv * D;
+  if (inner > 0x7fffffffll) return CFH_E_UNSUPPORTED;
   if (bs_k < inner || bs_v < inner || bs_k % 16 || bs_v % 16 || ((uintptr_t)k_cache | (uintptr_t)v_cache) % 16)
     return CFH_E_INVALID;
   if (T == 0 || S == 0) return CFH_OK;
   if (!q || !out || !lse || !seq_lens || !cu_q || (max_blocks && !table) || q_ld < (long long)H * D ||
       o_ld < (long long)H * D || q_ld % 8 || o_ld % 8 || ((uintptr_t)q | (uintptr_t)out) % 16)
     return CFH_E_INVALID;
-  const Plan p = plan(T, H, Hkv, S, max_len);
+  const Plan p = plan(T, H, Hkv, D, S, max_len);
   if (p.npiece > 1 && (!ws || (uintptr_t)ws % 256)) return CFH_E_INVALID;
   PagedArgs a = {};
   a.q = (const u16*)q; a.out = (u16*)out; a.lse = lse; a.kc = k_cache; a.vc = v_cache; a.ke = k_exp; a.ve = v_exp;
@@ -761,10 +804,12 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
   a.po = (float*)ws;
   a.pml = (float2*)((char*)ws + (p.npiece > 1 ? po_bytes(p, T, H, D) : 0));
   a.piece = p.piece; a.npiece = p.npiece; a.few = p.few;
-  int l = 0;                                      // ceil(log2(page)): j * floor(2^(31 + l) / page + 1) >> (31 + l)
+  // j / page for j < 2^30 as j M >> (31 + l), 2^l >= page > 2^(l - 1), M = floor(2^(31 + l) / page) + 1 < 2^32: M is
+  // above 2^(31 + l) / page by at most 1, which adds less than 2^30 / 2^(31 + l) < 1 / page to the quotient
+  int l = 0;
   while ((1ll << l) < page) ++l;
-  a.pshift = 31 + l;
-  a.pmagic = (1ull << a.pshift) / (unsigned)page + 1;
+  a.pshift = l;
+  a.pmagic = (unsigned)((1ull << (31 + l)) / (unsigned)page + 1);
   hipStream_t st = (hipStream_t)stream;
   const long long groups = (long long)Hkv * p.npiece;
   auto grid_of = [&](int tiles) {                 // (whole rounds of the XCD mapping)
@@ -776,8 +821,8 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
     a.tiles = p.ntile;
     const dim3 grid((unsigned)grid_of(p.ntile));
     kv_dispatch(is_bf16, f8, D, [&](auto bf, auto e8, auto d) {
-      constexpr int TK = d.value == 256 ? 32 : 64;
-      hipLaunchKernelGGL((k_attn_tiles<bf.value, e8.value, d.value, 4, TK>), grid, dim3(256), 0, st, a);
+      constexpr int NW = tile_rows(d.value) / 32, TK = d.value == 256 ? 32 : 64;
+      hipLaunchKernelGGL((k_attn_tiles<bf.value, e8.value, d.value, NW, TK>), grid, dim3(NW * 64), 0, st, a);
     });
     CFH_LAUNCH_CHECK();
   }
@@ -790,7 +835,7 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
     CFH_LAUNCH_CHECK();
   }
   if (p.npiece > 1) {
-    const dim3 grid((unsigned)(((long long)T * H + 3) / 4));
+    const dim3 grid((unsigned)(T * H));
     kv_dispatch(is_bf16, false, D, [&](auto bf, auto, auto d) {
       hipLaunchKernelGGL((k_attn_join<bf.value, d.value>), grid, dim3(256), 0, st, a);
     });
