@@ -136,43 +136,44 @@ __device__ __forceinline__ void check_bounds(const PagedArgs& a) {
       if (!bounds_ok(a, a.cu[i], a.cu[i + 1])) a.status[0] = 1;
 }
 
-// Where token j lies: its block (-1 where j is not below j1, or the block outside the cache, which is noted) and
-// its row in the block.
+// Where token j lies: the table's entry for its page, as loaded, and its row in the block.  Looked at only when
+// the token's own loads are issued (a check at once would wait for the table).  Past the work's tokens: the last
+// one's.
 struct Place { int blk, row; };
-__device__ __forceinline__ Place place_of(const PagedArgs& a, const Work& w, int j, int* first_bad) {
+__device__ __forceinline__ Place look_up(const PagedArgs& a, const Work& w, int j) {
+  j = min(j, w.j1 - 1);
   const int p = page_of(a, j);
-  Place at = {-1, j - p * a.page};
-  if (j < w.j1) {
-    at.blk = a.table[(size_t)w.s * a.table_ld + p];
-    if ((unsigned)at.blk >= (unsigned)a.blocks) {
-      atomicMin(first_bad, j);
-      at.blk = -1;
-    }
+  return {a.table[(size_t)w.s * a.table_ld + p], j - p * a.page};
+}
+// Whether token j is one of the work's and its block one of the cache's (one that is not is noted); if not, the
+// place becomes one that can be read.
+__device__ __forceinline__ bool resolve(const PagedArgs& a, const Work& w, int j, Place& at, int* first_bad) {
+  const bool in = (unsigned)at.blk < (unsigned)a.blocks;
+  if (!in) {
+    if (j < w.j1) atomicMin(first_bad, j);
+    at.blk = 0;
   }
-  return at;
+  return in && j < w.j1;
 }
 
-// 8 elements of a token's row as they lie in memory; zero where there is no block, so that nothing that lies past
-// a sequence's tokens reaches a product.
+// 16 bytes (8 elements of a 2-byte cache, 16 of an 8-bit one) of a token's row, or 8 of an 8-bit one.
+template <int ES>
+__device__ __forceinline__ const char* row_at(const PagedArgs& a, const void* c, long long bs, const Place& at, int hk, int D, int col) {
+  return (const char*)c + ((size_t)(unsigned)at.blk * (size_t)bs + (unsigned)((at.row * a.Hkv + hk) * D + col)) * ES;
+}
 template <bool F8>
 __device__ __forceinline__ uint4 load_row(const PagedArgs& a, const void* c, long long bs, const Place& at, int hk, int D, int col) {
-  uint4 r = make_uint4(0, 0, 0, 0);
-  if (at.blk >= 0) {
-    const size_t i = (size_t)(unsigned)at.blk * (size_t)bs + (unsigned)((at.row * a.Hkv + hk) * D + col);
-    if constexpr (F8) {
-      const uint2 x = *(const uint2*)((const uint8_t*)c + i);
-      r.x = x.x;
-      r.y = x.y;
-    } else {
-      r = *(const uint4*)((const u16*)c + i);
-    }
+  if constexpr (F8) {
+    const uint2 x = *(const uint2*)row_at<1>(a, c, bs, at, hk, D, col);
+    return make_uint4(x.x, x.y, 0, 0);
+  } else {
+    return *(const uint4*)row_at<2>(a, c, bs, at, hk, D, col);
   }
-  return r;
 }
 template <bool F8>
 __device__ __forceinline__ int load_exp(const PagedArgs& a, const uint8_t* ex, const Place& at, int hk) {
-  if (!F8 || at.blk < 0) return 127;
-  return ex[((size_t)at.blk * a.page + at.row) * a.Hkv + hk];
+  if constexpr (F8) return ex[((size_t)at.blk * a.page + at.row) * a.Hkv + hk];
+  return 127;
 }
 template <bool BF, bool F8>
 __device__ __forceinline__ uint4 to_rows(const uint4& r, int code) {
@@ -299,14 +300,16 @@ __global__ void __launch_bounds__(NW * 64, 2) k_attn_tiles(PagedArgs a) {
   }
   uint4 kr[CPT], vr[CPT];
   int kx[CPT], vx[CPT];
+  bool ok[CPT];
   Place pl[CPT];
-  auto blocks = [&](int jt) {
+  auto places = [&](int jt) {
 #pragma unroll
-    for (int x = 0; x < CPT; ++x) pl[x] = place_of(a, w, jt + srow + RS * x, &first_bad);
+    for (int x = 0; x < CPT; ++x) pl[x] = look_up(a, w, jt + srow + RS * x);
   };
-  auto fetch = [&]() {
+  auto fetch = [&](int jt) {
 #pragma unroll
     for (int x = 0; x < CPT; ++x) {
+      ok[x] = resolve(a, w, jt + srow + RS * x, pl[x], &first_bad);
       kr[x] = load_row<F8>(a, a.kc, a.bs_k, pl[x], w.hk, D, scol * 8);
       vr[x] = load_row<F8>(a, a.vc, a.bs_v, pl[x], w.hk, D, scol * 8);
       kx[x] = load_exp<F8>(a, a.ke, pl[x], w.hk);
@@ -318,7 +321,9 @@ __global__ void __launch_bounds__(NW * 64, 2) k_attn_tiles(PagedArgs a) {
 #pragma unroll
     for (int x = 0; x < CPT; ++x) {
       const int tok = srow + RS * x, at = sat + RS * x * D;
+      // (V's rows of no token enter as zeros: 0 * NaN would reach the sums.  K's scores are masked)
       uint4 v = to_rows<BF, F8>(vr[x], vx[x]);
+      v = ok[x] ? v : make_uint4(0, 0, 0, 0);
       *(uint4*)&lds[buf][0][at] = to_rows<BF, F8>(kr[x], kx[x]);
       if (jt + TK > vis_wg && any_nonfinite<BF>(v)) {
         v = only_finite<BF>(v);
@@ -331,9 +336,9 @@ __global__ void __launch_bounds__(NW * 64, 2) k_attn_tiles(PagedArgs a) {
   f32x16 o[D / 32] = {};
   float m = -INFINITY, l = 0.f;                   // (m in log2 units; l: this half's tokens)
   if (w.j0 < w.j1) {
-    blocks(w.j0);
-    fetch();
-    blocks(w.j0 + TK);
+    places(w.j0);
+    fetch(w.j0);
+    places(w.j0 + TK);
     stage(w.j0, 0);
   }
   int buf = 0;
@@ -341,8 +346,8 @@ __global__ void __launch_bounds__(NW * 64, 2) k_attn_tiles(PagedArgs a) {
     lds_barrier();
     const bool more = jt + TK < w.j1;
     if (more) {
-      fetch();
-      blocks(jt + 2 * TK);
+      fetch(jt + TK);
+      places(jt + 2 * TK);
     }
     if (jt < w.j1 && w.r0 + wave * 32 < rows) {
       const u16* kt = lds[buf][0];
@@ -455,9 +460,10 @@ __global__ void __launch_bounds__(NW * 64, 2) k_attn_tiles(PagedArgs a) {
 }
 
 // Few rows: a tile of 16, one workgroup of four waves a (row tile, kv head, piece), each wave the tokens of
-// every fourth group of 16.  K goes from memory straight into the first operand's registers (16 tokens x
-// 64-byte segments a load), V through the wave's own 16 rows of LDS for the transposed reads; both one group
-// ahead.  Waves do not wait for each other before the join of their (max, sum, O) at the end.
+// every fourth group of TG.  K goes from memory straight into the first operand's registers (16 tokens x
+// 64-byte segments a load), V through the wave's own rows of LDS for the transposed reads; both one group
+// ahead, 16 KB a wave (8 for D = 64 in 8 bits), with no branch around a load: behind one the compiler waits
+// for everything.  Waves do not wait for each other before the join of their (max, sum, O) at the end.
 template <bool BF>
 __device__ __forceinline__ f32x4 mfma16(const uint4& x, const uint4& y, f32x4 acc) {
   if constexpr (BF)
@@ -474,19 +480,21 @@ __device__ __forceinline__ f32x4 mfma16h(const uint2& x, const uint2& y, f32x4 a
 }
 
 template <bool BF, bool F8, int D>
-__global__ void __launch_bounds__(256) k_attn_rows(PagedArgs a) {
+__global__ void __launch_bounds__(256, 2) k_attn_rows(PagedArgs a) {
   constexpr int R = 16, NW = 4, KS = D / 32;      // MFMA steps of 32 along the head
-  constexpr int CH = D / 8, VPT = 16 * CH / 64;   // V's 16-byte chunks a lane stages
-  constexpr int KL = F8 ? KS / 2 : KS;            // 16-byte loads of a lane's share of K
-  __shared__ __align__(16) union { u16 v[NW][16 * D]; float o[NW][16 * D]; } sh;
+  constexpr int U = F8 ? (D == 256 ? 2 : 4) : 256 / D, TG = 16 * U;   // 16-token tiles a group, its tokens
+  constexpr int CE = F8 ? 16 : 8, CH = D / CE;    // elements of a 16-byte load, loads a token's row
+  constexpr int KL = D / (4 * CE), VL = TG * CH / 64;   // a lane's 16-byte loads: of K a tile, of V a group
+  __shared__ __align__(16) union { u16 v[NW][TG * D]; float o[NW][16 * D]; } sh;
   __shared__ float2 ml[NW][16];
   __shared__ int first_bad;
-  __shared__ unsigned odd[2];                     // (the tokens not all rows see: 16, and a group on either side)
+  __shared__ unsigned odd[4];                     // (the tokens not all rows see: 16, and a group on either side)
   check_bounds(a);
   Work w;
   if (!find_work<R, true>(a, w)) return;          // (the whole workgroup)
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, tl = lane & 15;
-  if (tid == 0) { first_bad = 0x7fffffff; odd[0] = odd[1] = 0; }
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, tl = lane & 15;
+  if (tid == 0) first_bad = 0x7fffffff;
+  if (tid < 4) odd[tid] = 0;
   __syncthreads();
   const int rows = w.n * a.G, r = w.r0 + tl;
   const int i = min(r, rows - 1) / a.G, hh = min(r, rows - 1) % a.G;
@@ -508,78 +516,94 @@ __global__ void __launch_bounds__(256) k_attn_rows(PagedArgs a) {
   u16* const vt = sh.v[wave];
   int va[4];                                      // (as in k_attn_tiles)
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int x = 0; x < 4; ++x) {
     const int tr = 4 * g + tl / 4;
-    va[i] = tr * D + (((2 * i + (tl & 3) / 2) ^ swz(tr)) * 8) + 4 * (tl & 1);
+    va[x] = tr * D + (((2 * x + (tl & 3) / 2) ^ swz(tr)) * 8) + 4 * (tl & 1);
   }
-  uint4 kr[KL], vr[VPT];
-  int kx = 127, vx[VPT];
-  Place kb, vb[VPT];
-  // this lane's token of K is tl; its chunks of V are tokens (lane + 64 x) / CH
-  auto blocks = [&](int jt) {
-    kb = place_of(a, w, jt + tl, &first_bad);
+  // this lane's token of K's tile u is 16 u + tl; its chunks of V are of tokens (lane + 64 x) / CH
+  uint4 kr[U][KL], vr[VL];
+  int kx[U], vx[VL];
+  bool vok[VL];
+  Place kp[U], vp[VL];
+  auto k_places = [&](int jt) {
 #pragma unroll
-    for (int x = 0; x < VPT; ++x) vb[x] = place_of(a, w, jt + (lane + 64 * x) / CH, &first_bad);
+    for (int u = 0; u < U; ++u) kp[u] = look_up(a, w, jt + 16 * u + tl);
   };
-  auto fetch = [&]() {
+  auto v_places = [&](int jt) {
 #pragma unroll
-    for (int s = 0; s < KL; ++s) {
-      if constexpr (F8) {
-        kr[s] = make_uint4(0, 0, 0, 0);
-        if (kb.blk >= 0)
-          kr[s] = *(const uint4*)((const uint8_t*)a.kc + (size_t)(unsigned)kb.blk * (size_t)a.bs_k +
-                                  (unsigned)((kb.row * a.Hkv + w.hk) * D + 64 * s + 16 * g));
-      } else {
-        kr[s] = load_row<false>(a, a.kc, a.bs_k, kb, w.hk, D, 32 * s + 8 * g);
-      }
+    for (int x = 0; x < VL; ++x) vp[x] = look_up(a, w, jt + (lane + 64 * x) / CH);
+  };
+  auto k_fetch = [&](int jt) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      resolve(a, w, jt + 16 * u + tl, kp[u], &first_bad);
+#pragma unroll
+      for (int s = 0; s < KL; ++s)
+        kr[u][s] = *(const uint4*)row_at<F8 ? 1 : 2>(a, a.kc, a.bs_k, kp[u], w.hk, D, 4 * CE * s + CE * g);
+      kx[u] = load_exp<F8>(a, a.ke, kp[u], w.hk);
     }
-    kx = load_exp<F8>(a, a.ke, kb, w.hk);
+  };
+  auto v_fetch = [&](int jt) {
 #pragma unroll
-    for (int x = 0; x < VPT; ++x) {
-      vr[x] = load_row<F8>(a, a.vc, a.bs_v, vb[x], w.hk, D, (lane + 64 * x) % CH * 8);
-      vx[x] = load_exp<F8>(a, a.ve, vb[x], w.hk);
+    for (int x = 0; x < VL; ++x) {
+      vok[x] = resolve(a, w, jt + (lane + 64 * x) / CH, vp[x], &first_bad);
+      vr[x] = *(const uint4*)row_at<F8 ? 1 : 2>(a, a.vc, a.bs_v, vp[x], w.hk, D, (lane + 64 * x) % CH * CE);
+      vx[x] = load_exp<F8>(a, a.ve, vp[x], w.hk);
     }
   };
   f32x4 o[D / 16] = {};
   float m = -INFINITY, l = 0.f;
-  const int step = 16 * NW;
-  const int odd_base = w.j0 + max(0, vis_all - w.j0) / 16 * 16;   // the first group that not every row sees whole
-  int jt = w.j0 + 16 * wave;
+  const int step = TG * NW;
+  const int odd_base = w.j0 + max(0, vis_all - w.j0) / TG * TG;   // the first group that not every row sees whole
+  int jt = w.j0 + TG * wave;
   if (jt < w.j1) {
-    blocks(jt);
-    fetch();
-    blocks(jt + step);
+    k_places(jt);
+    v_places(jt);
+    k_fetch(jt);
+    v_fetch(jt);
+    k_places(jt + step);
+    v_places(jt + step);
   }
   for (; jt < w.j1; jt += step) {
+    const bool edge = jt + TG > vis_all;          // (uniform)
 #pragma unroll
-    for (int x = 0; x < VPT; ++x) {
-      const int c = lane + 64 * x, tok = c / CH;
-      uint4 v = to_rows<BF, F8>(vr[x], vx[x]);
-      if (jt + 16 > vis_all && any_nonfinite<BF>(v)) {
-        v = only_finite<BF>(v);
-        atomicOr(&odd[(jt + tok - odd_base) / 32], 1u << ((jt + tok - odd_base) & 31));
+    for (int x = 0; x < VL; ++x) {
+      const int c = lane + 64 * x, tok = c / CH, ch = c % CH * (CE / 8);
+#pragma unroll
+      for (int y = 0; y < CE / 8; ++y) {
+        uint4 v = F8 ? dequant8<BF>(y ? make_uint2(vr[x].z, vr[x].w) : make_uint2(vr[x].x, vr[x].y), vx[x]) : vr[x];
+        v = vok[x] ? v : make_uint4(0, 0, 0, 0);
+        if (edge && any_nonfinite<BF>(v)) {
+          v = only_finite<BF>(v);
+          atomicOr(&odd[(jt + tok - odd_base) / 32], 1u << ((jt + tok - odd_base) & 31));
+        }
+        *(uint4*)&vt[tok * D + (((ch + y) ^ swz(tok)) * 8)] = v;
       }
-      *(uint4*)&vt[tok * D + (((c % CH) ^ swz(tok)) * 8)] = v;
     }
-    uint4 kf[KS];
+    v_fetch(jt + step);                           // (past the work's tokens: its last ones again, never used)
+    v_places(jt + 2 * step);
+    f32x4 sc[U];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      if constexpr (F8) kf[s] = dequant8<BF>(s % 2 ? make_uint2(kr[s / 2].z, kr[s / 2].w) : make_uint2(kr[s / 2].x, kr[s / 2].y), kx);
-      else kf[s] = kr[s];
-    }
-    if (jt + step < w.j1) {
-      fetch();
-      blocks(jt + 2 * step);
-    }
-    f32x4 sc = {};
+    for (int u = 0; u < U; ++u) {
+      sc[u] = f32x4{};
 #pragma unroll
-    for (int s = 0; s < KS; ++s) sc = mfma16<BF>(kf[s], qf[s], sc);
+      for (int s = 0; s < KS; ++s) {
+        uint4 kf;
+        if constexpr (F8) kf = dequant8<BF>(s % 2 ? make_uint2(kr[u][s / 2].z, kr[u][s / 2].w) : make_uint2(kr[u][s / 2].x, kr[u][s / 2].y), kx[u]);
+        else kf = kr[u][s];
+        sc[u] = mfma16<BF>(kf, qf[s], sc[u]);
+      }
+    }
+    k_fetch(jt + step);
+    k_places(jt + 2 * step);
     float mx = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (jt + 4 * g + e >= vis) sc[e] = -INFINITY;
-      mx = fmaxf(mx, sc[e]);
-    }
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (jt + 16 * u + 4 * g + e >= vis) sc[u][e] = -INFINITY;
+        mx = fmaxf(mx, sc[u][e]);
+      }
     mx = fmaxf(mx, __shfl_xor(mx, 16));
     mx = swap_max(mx) * a.c;
     if (__any(mx > m + LAZY || (m == -INFINITY && mx > m))) {
@@ -592,16 +616,30 @@ __global__ void __launch_bounds__(256) k_attn_rows(PagedArgs a) {
       m = mn;
     }
     const float base = m == -INFINITY ? 0.f : m;
+    uint2 pf[U];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], a.c, -base));
-      l += sc[e];
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sc[u][e] = __builtin_amdgcn_exp2f(fmaf(sc[u][e], a.c, -base));
+        l += sc[u][e];
+      }
+      pf[u] = make_uint2(pack2<BF>(sc[u][0], sc[u][1]), pack2<BF>(sc[u][2], sc[u][3]));
     }
-    const uint2 pf = make_uint2(pack2<BF>(sc[0], sc[1]), pack2<BF>(sc[2], sc[3]));
     // (a wave's LDS accesses complete in order: its reads see its own writes above)
-    auto vfrag = [&](int d) { return read_tr(&vt[va[d & 3] + d / 4 * 64]); };
+    auto vfrag = [&](int d, int u) { return read_tr(&vt[va[d & 3] + 16 * u * D + d / 4 * 64]); };
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) o[d] = mfma16h<BF>(vfrag(d), pf, o[d]);
+    for (int d = 0; d < D / 16; ++d) {
+      if constexpr (U == 1) {
+        o[d] = mfma16h<BF>(vfrag(d, 0), pf[0], o[d]);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; u += 2) {          // two tiles a step: elements 0 - 3 of the first, 4 - 7 of the second
+          const uint2 x = vfrag(d, u), y = vfrag(d, u + 1);
+          o[d] = mfma16<BF>(make_uint4(x.x, x.y, y.x, y.y), make_uint4(pf[u].x, pf[u].y, pf[u + 1].x, pf[u + 1].y), o[d]);
+        }
+      }
+    }
   }
   // the four waves' join: each row's maximum, then the sums of what the waves hold under it
   l += __shfl_xor(l, 16);
@@ -631,9 +669,9 @@ __global__ void __launch_bounds__(256) k_attn_rows(PagedArgs a) {
       sum += *(const f32x4*)&sh.o[v][row * D + 16 * ((col / 16) ^ (row & (D / 16 - 1))) + col % 16];
       ls += ml[v][row].x == -INFINITY ? ml[v][row].y : ml[v][row].y * __builtin_amdgcn_exp2f(ml[v][row].x - mr);
     }
-    if (odd[0] | odd[1]) {
+    if (odd[0] | odd[1] | odd[2] | odd[3]) {
       float y[4] = {sum[0], sum[1], sum[2], sum[3]};
-      add_odd<BF, F8>(a, w, odd, 2, odd_base, min(seen(a, w.len, w.n, ti), w.j1), col, D, y);
+      add_odd<BF, F8>(a, w, odd, 4, odd_base, min(seen(a, w.len, w.n, ti), w.j1), col, D, y);
       sum = f32x4{y[0], y[1], y[2], y[3]};
     }
     if (w.bad || first_bad < min(seen(a, w.len, w.n, ti), w.j1)) {
