@@ -151,17 +151,24 @@ def ptr(t) -> int | None:
 
 
 def device_of(first, *others, status=None):
-    """The one GPU that the tensors (None: skipped) lie on, which has to be the current device: a launch goes to
-    the current device's stream.  ``status`` words are int32 [1]."""
+    """The index of the one GPU that the tensors (None: skipped) lie on, which has to be the current device: a
+    launch goes to the current device's stream.  ``status`` words are int32 [1]."""
     import torch
-    dev = first.device
-    if dev.type != "cuda" or any(t is not None and t.device != dev for t in others):
+    dev = first.get_device()                       # -1: not a GPU's
+    if dev < 0 or any(t is not None and t.get_device() != dev for t in others):
         raise ValueError("the tensors must lie on one GPU")
-    if dev.index != torch.cuda.current_device():
-        raise ValueError(f"the tensors lie on {dev}, but the current device is cuda:{torch.cuda.current_device()}")
-    if status is not None and (status.dtype != torch.int32 or status.device != dev or status.numel() < 1):
+    if dev != torch._C._cuda_getDevice():
+        raise ValueError(f"the tensors lie on cuda:{dev}, but the current device is cuda:{torch.cuda.current_device()}")
+    if status is not None and (status.dtype != torch.int32 or status.get_device() != dev or status.numel() < 1):
         raise ValueError("status must be an int32 tensor on the same device")
     return dev
+
+
+def stream_of(dev: int) -> int:
+    """The current stream of a device, as the address a launch takes (``stream_handle`` builds two objects for it: 3 us
+    of a call's 9)."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def aligned(t):

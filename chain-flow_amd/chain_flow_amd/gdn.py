@@ -91,7 +91,8 @@ def tree_gdn_vllm(mixed_qkv, a, b, A_log, dt_bias, ssm_state, node_slots, parent
 
 
 def _seq_args(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, H, out, status, initial=None):
-    """The checks that ``gdn_prefill`` and ``gdn_decode`` share -> (x, a, b, A_log, dt_bias, slots, out)."""
+    """The checks that ``gdn_prefill`` and ``gdn_decode`` share -> (x, a, b, A_log, dt_bias, slots, out,
+    device)."""
     T, conv = mixed_qkv.shape
     nslots, HV, V, K = ssm_state.shape
     if H < 1 or HV % H:
@@ -110,12 +111,20 @@ def _seq_args(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, H, out, status,
         raise ValueError("slots must be [S], S <= 4096")
     dev = _lib.device_of(mixed_qkv, a, b, A_log, dt_bias, ssm_state, status=status)
     if out is None:
-        out = torch.empty(T, HV, V, dtype=torch.bfloat16, device=dev)
-    elif out.shape != (T, HV, V) or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.device != dev:
-        raise ValueError(f"out must be a contiguous bf16 [{T}, {HV}, {V}] tensor on {dev}")
-    f32 = lambda t: t.to(torch.float32).contiguous()  # noqa: E731
-    return (_lib.aligned(mixed_qkv.contiguous()), a.contiguous(), b.contiguous(), f32(A_log), f32(dt_bias),
-            slots.to(dev, torch.int32).contiguous(), out)
+        out = mixed_qkv.new_empty((T, HV, V))
+    elif out.shape != (T, HV, V) or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.get_device() != dev:
+        raise ValueError(f"out must be a contiguous bf16 [{T}, {HV}, {V}] tensor on cuda:{dev}")
+    if A_log.dtype != torch.float32 or dt_bias.dtype != torch.float32:
+        A_log, dt_bias = A_log.float(), dt_bias.float()
+    return (_lib.aligned(mixed_qkv.contiguous()), a.contiguous(), b.contiguous(), A_log.contiguous(), dt_bias.contiguous(),
+            _on(slots, dev), out, dev)
+
+
+def _on(index, dev):
+    """An index tensor as int32 on the device."""
+    if index.dtype != torch.int32 or index.get_device() != dev:
+        index = index.to(f"cuda:{dev}", torch.int32)
+    return index.contiguous()
 
 
 def gdn_decode(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, *, num_q_heads: int, scale: float | None = None,
@@ -132,13 +141,12 @@ def gdn_decode(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, *, num_q_heads
     S = mixed_qkv.shape[0]
     if slots.shape != (S,):
         raise ValueError(f"slots must be [{S}]")
-    x, a, b, A_log, dt_bias, slots, out = _seq_args(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, H, out, status)
+    x, a, b, A_log, dt_bias, slots, out, dev = _seq_args(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, H, out, status)
     nslots, HV, V, K = ssm_state.shape
     _lib.check(_lib.lib().cfh_gdn_decode(
         x.data_ptr(), a.data_ptr(), b.data_ptr(), A_log.data_ptr(), dt_bias.data_ptr(), ssm_state.data_ptr(),
-        int(ssm_state.dtype == torch.bfloat16), nslots, slots.data_ptr(), S, H, HV, K, V, int(bool(use_qk_l2norm)),
-        float(K ** -0.5 if scale is None else scale), out.data_ptr(), _lib.ptr(status), _lib.stream_handle()),
-        "cfh_gdn_decode")
+        ssm_state.dtype == torch.bfloat16, nslots, slots.data_ptr(), S, H, HV, K, V, bool(use_qk_l2norm),
+        K ** -0.5 if scale is None else scale, out.data_ptr(), _lib.ptr(status), _lib.stream_of(dev)), "cfh_gdn_decode")
     return out
 
 
@@ -151,21 +159,21 @@ def gdn_prefill(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, cu_seqlens, *
     from (``tree_gdn_vllm``'s prefix slot).  -> o [T, HV, V] bf16.  ``cfh_gdn_prefill``, no host
     synchronisation; rows of no sequence stay as they were in ``out``."""
     H = int(num_q_heads)
-    x, a, b, A_log, dt_bias, slots, out = _seq_args(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, H, out, status)
+    x, a, b, A_log, dt_bias, slots, out, dev = _seq_args(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, H, out, status)
     S, T = slots.shape[0], x.shape[0]
     nslots, HV, V, K = ssm_state.shape
     if cu_seqlens.shape != (S + 1,):
         raise ValueError(f"cu_seqlens must be [{S + 1}]")
-    cu = cu_seqlens.to(x.device, torch.int32).contiguous()
+    cu = _on(cu_seqlens, dev)
     if initial is not None:
         if initial.shape != (S,) or initial.dtype not in (torch.bool, torch.uint8):
             raise ValueError(f"initial must be a bool [{S}] tensor")
         initial = initial.to(x.device).contiguous()
     L = _lib.lib()
-    ws = torch.empty(int(L.cfh_gdn_prefill_ws_bytes(T, S, HV)), dtype=torch.uint8, device=x.device)
+    ws = x.new_empty(L.cfh_gdn_prefill_ws_bytes(T, S, HV), dtype=torch.uint8)
     _lib.check(L.cfh_gdn_prefill(
         x.data_ptr(), a.data_ptr(), b.data_ptr(), A_log.data_ptr(), dt_bias.data_ptr(), ssm_state.data_ptr(),
-        int(ssm_state.dtype == torch.bfloat16), nslots, slots.data_ptr(), cu.data_ptr(), _lib.ptr(initial), S, T, H, HV,
-        K, V, int(bool(use_qk_l2norm)), float(K ** -0.5 if scale is None else scale), out.data_ptr(), ws.data_ptr(),
-        _lib.ptr(status), _lib.stream_handle()), "cfh_gdn_prefill")
+        ssm_state.dtype == torch.bfloat16, nslots, slots.data_ptr(), cu.data_ptr(), _lib.ptr(initial), S, T, H, HV, K, V,
+        bool(use_qk_l2norm), K ** -0.5 if scale is None else scale, out.data_ptr(), ws.data_ptr(), _lib.ptr(status),
+        _lib.stream_of(dev)), "cfh_gdn_prefill")
     return out

@@ -21,38 +21,50 @@ _TYPES = (torch.bfloat16, torch.float16)
 
 
 def _check_cache(k_cache, v_cache, k_exp, v_exp, dtype):
-    """-> (blocks, page, Hkv, D) of a cache that serves rows of ``dtype``."""
-    blocks, page, Hkv, D = k_cache.shape
-    if v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+    """-> (blocks, page, Hkv, D, block strides of k and v) of a cache that serves rows of ``dtype``."""
+    shape = k_cache.shape
+    blocks, page, Hkv, D = shape
+    kind = k_cache.dtype
+    if v_cache.shape != shape or v_cache.dtype != kind:
         raise ValueError("k_cache and v_cache must share one shape and type")
-    if D not in (64, 128, 256):
+    if D != 128 and D != 256 and D != 64:
         raise ValueError(f"head width {D} is not 64, 128 or 256")
-    if k_cache.dtype == torch.float8_e4m3fn:
+    if kind == torch.float8_e4m3fn:
         for e in (k_exp, v_exp):
-            if e is None or e.dtype != torch.uint8 or e.shape != (blocks, page, Hkv) or not e.is_contiguous():
+            if e is None or e.dtype != torch.uint8 or e.shape != shape[:3] or not e.is_contiguous():
                 raise ValueError(f"an 8-bit cache needs contiguous uint8 k_exp and v_exp [{blocks}, {page}, {Hkv}]")
-    elif k_cache.dtype != dtype or k_exp is not None or v_exp is not None:
+    elif kind != dtype or k_exp is not None or v_exp is not None:
         raise ValueError(f"the cache must be {dtype} without exponents, or float8_e4m3fn with them")
-    for c in (k_cache, v_cache):
-        if c.stride()[1:] != (Hkv * D, D, 1) or (blocks > 1 and (c.stride(0) < page * Hkv * D or c.stride(0) % 16)) \
-                or c.data_ptr() % 16:
-            raise ValueError("cache blocks must be contiguous [page, Hkv, D], on strides of 16 elements and 16-byte "
-                             "boundaries")
-    return blocks, page, Hkv, D
+    (bs_k, *in_k), (bs_v, *in_v) = k_cache.stride(), v_cache.stride()
+    row = Hkv * D
+    inner = page * row
+    if blocks == 1:
+        bs_k = bs_v = inner
+    want = [row, D, 1]
+    if (in_k != want or in_v != want or bs_k < inner or bs_v < inner or (bs_k | bs_v) % 16
+            or (k_cache.data_ptr() | v_cache.data_ptr()) % 16):
+        raise ValueError("cache blocks must be contiguous [page, Hkv, D], on strides of 16 elements and 16-byte "
+                         "boundaries")
+    return blocks, page, Hkv, D, bs_k, bs_v
 
 
-def _block_stride(c):
-    return c.stride(0) if c.shape[0] > 1 else c[0].numel()
-
-
-def _rows(t, name):
-    """Rows [T, heads, D] with contiguous heads whose vector loads are aligned (copied where they are not)."""
+def _rows(t):
+    """Rows [T, heads, D] with contiguous heads whose vector loads are aligned (copied where they are not), and
+    their stride."""
     T, h, D = t.shape
-    if t.stride(2) == 1 and t.stride(1) == D and (T < 2 or (t.stride(0) >= h * D and t.stride(0) % 8 == 0)) \
-            and t.data_ptr() % 16 == 0:
-        return t, t.stride(0) if T > 1 else h * D
-    t = _lib.aligned(t.contiguous())
-    return t, h * D
+    ld, inner, one = t.stride()
+    if T < 2:
+        ld = h * D
+    if one != 1 or inner != D or ld < h * D or ld % 8 or t.data_ptr() % 16:
+        t, ld = _lib.aligned(t.contiguous()), h * D
+    return t, ld
+
+
+def _i32(t, dev):
+    """An index tensor as int32 on the device."""
+    if t.dtype != torch.int32 or t.get_device() != dev:
+        t = t.to(f"cuda:{dev}", torch.int32)
+    return t.contiguous()
 
 
 def kv_cache_write(key, value, k_cache, v_cache, slots, *, k_exp=None, v_exp=None, status=None) -> None:
@@ -68,7 +80,7 @@ def kv_cache_write(key, value, k_cache, v_cache, slots, *, k_exp=None, v_exp=Non
     one race, and either's elements may stay (a host tensor's are checked here)."""
     if key.dtype not in _TYPES or value.dtype != key.dtype or value.shape != key.shape:
         raise ValueError("key and value must be bf16 or fp16 tensors of one shape [T, Hkv, D]")
-    blocks, page, Hkv, D = _check_cache(k_cache, v_cache, k_exp, v_exp, key.dtype)
+    blocks, page, Hkv, D, bs_k, bs_v = _check_cache(k_cache, v_cache, k_exp, v_exp, key.dtype)
     T = key.shape[0]
     if key.shape != (T, Hkv, D) or slots.shape != (T,):
         raise ValueError(f"key and value must be [T, {Hkv}, {D}] and slots [T]")
@@ -77,13 +89,13 @@ def kv_cache_write(key, value, k_cache, v_cache, slots, *, k_exp=None, v_exp=Non
         used = slots[slots >= 0]
         if used.unique().numel() != used.numel() or (used >= blocks * page).any():
             raise ValueError(f"slots must be distinct and below {blocks * page}")
-    slots = slots.to(dev, torch.int32).contiguous()
-    key, ld_k = _rows(key, "key")
-    value, ld_v = _rows(value, "value")
+    slots = _i32(slots, dev)
+    key, ld_k = _rows(key)
+    value, ld_v = _rows(value)
     _lib.check(_lib.lib().cfh_kv_write(
-        key.data_ptr(), ld_k, value.data_ptr(), ld_v, T, Hkv, D, int(key.dtype == torch.bfloat16), k_cache.data_ptr(),
-        _block_stride(k_cache), v_cache.data_ptr(), _block_stride(v_cache), _lib.ptr(k_exp), _lib.ptr(v_exp), blocks,
-        page, slots.data_ptr(), _lib.ptr(status), _lib.stream_handle()), "cfh_kv_write")
+        key.data_ptr(), ld_k, value.data_ptr(), ld_v, T, Hkv, D, key.dtype == torch.bfloat16, k_cache.data_ptr(), bs_k,
+        v_cache.data_ptr(), bs_v, _lib.ptr(k_exp), _lib.ptr(v_exp), blocks, page, slots.data_ptr(), _lib.ptr(status),
+        _lib.stream_of(dev)), "cfh_kv_write")
 
 
 def kv_cache_read(k_cache, v_cache, slots, *, dtype=None, k_exp=None, v_exp=None, status=None):
@@ -94,18 +106,18 @@ def kv_cache_read(k_cache, v_cache, slots, *, dtype=None, k_exp=None, v_exp=None
         dtype = torch.bfloat16 if k_cache.dtype == torch.float8_e4m3fn else k_cache.dtype
     if dtype not in _TYPES:
         raise ValueError("rows are read as bf16 or fp16")
-    blocks, page, Hkv, D = _check_cache(k_cache, v_cache, k_exp, v_exp, dtype)
+    blocks, page, Hkv, D, bs_k, bs_v = _check_cache(k_cache, v_cache, k_exp, v_exp, dtype)
     if slots.dim() != 1:
         raise ValueError("slots must be [T]")
     dev = _lib.device_of(k_cache, v_cache, k_exp, v_exp, status=status)
-    slots = slots.to(dev, torch.int32).contiguous()
+    slots = _i32(slots, dev)
     T = slots.shape[0]
-    key = torch.empty(T, Hkv, D, dtype=dtype, device=dev)
-    value = torch.empty(T, Hkv, D, dtype=dtype, device=dev)
+    key = k_cache.new_empty((T, Hkv, D), dtype=dtype)
+    value = torch.empty_like(key)
     _lib.check(_lib.lib().cfh_kv_read(
-        k_cache.data_ptr(), _block_stride(k_cache), v_cache.data_ptr(), _block_stride(v_cache), _lib.ptr(k_exp),
-        _lib.ptr(v_exp), blocks, page, slots.data_ptr(), T, Hkv, D, int(dtype == torch.bfloat16), key.data_ptr(),
-        value.data_ptr(), _lib.ptr(status), _lib.stream_handle()), "cfh_kv_read")
+        k_cache.data_ptr(), bs_k, v_cache.data_ptr(), bs_v, _lib.ptr(k_exp), _lib.ptr(v_exp), blocks, page,
+        slots.data_ptr(), T, Hkv, D, dtype == torch.bfloat16, key.data_ptr(), value.data_ptr(), _lib.ptr(status),
+        _lib.stream_of(dev)), "cfh_kv_read")
     return key, value
 
 
@@ -123,7 +135,7 @@ def paged_attention(query, k_cache, v_cache, block_table, seq_lens, cu_q, *, sca
     (default: what the table holds); it only plans how the work is split."""
     if query.dtype not in _TYPES:
         raise ValueError("query must be bf16 or fp16")
-    blocks, page, Hkv, D = _check_cache(k_cache, v_cache, k_exp, v_exp, query.dtype)
+    blocks, page, Hkv, D, bs_k, bs_v = _check_cache(k_cache, v_cache, k_exp, v_exp, query.dtype)
     T, H, Dq = query.shape
     if Dq != D or H % Hkv:
         raise ValueError(f"query must be [T, H, {D}] with H a multiple of {Hkv}")
@@ -132,27 +144,31 @@ def paged_attention(query, k_cache, v_cache, block_table, seq_lens, cu_q, *, sca
         raise ValueError("seq_lens must be [S], cu_q [S + 1] and block_table [S, blocks]")
     dev = _lib.device_of(query, k_cache, v_cache, k_exp, v_exp, status=status)
     if out is None:
-        out = torch.empty(T, H, D, dtype=query.dtype, device=dev)
-    elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev or out.stride()[1:] != (D, 1) \
-            or (T > 1 and (out.stride(0) < H * D or out.stride(0) % 8)) or out.data_ptr() % 16:
-        raise ValueError(f"out must be a {query.dtype} [{T}, {H}, {D}] tensor on {dev} with contiguous heads, 16-byte "
-                         "aligned")
-    table = block_table.to(dev, torch.int32)
-    if table.stride(1) != 1 or table.stride(0) < table.shape[1]:
-        table = table.contiguous()
+        out = query.new_empty((T, H, D))
+        o_ld = H * D
+    else:
+        o_ld = out.stride(0) if T > 1 else H * D
+        if (out.shape != query.shape or out.dtype != query.dtype or out.get_device() != dev or out.stride()[1:] != (D, 1)
+                or o_ld < H * D or o_ld % 8 or out.data_ptr() % 16):
+            raise ValueError(f"out must be a {query.dtype} [{T}, {H}, {D}] tensor on cuda:{dev} with contiguous heads, "
+                             "16-byte aligned")
+    table = block_table
+    if table.dtype != torch.int32 or table.get_device() != dev:
+        table = table.to(f"cuda:{dev}", torch.int32)
     width = table.shape[1]
-    lens, cu = seq_lens.to(dev, torch.int32).contiguous(), cu_q.to(dev, torch.int32).contiguous()
+    if table.stride(1) != 1 or table.stride(0) < width:
+        table = table.contiguous()
+    lens, cu = _i32(seq_lens, dev), _i32(cu_q, dev)
     most = width * page
     most = most if max_len is None else max(0, min(int(max_len), most))
-    lse = torch.empty(H, T, dtype=torch.float32, device=dev)
-    query, q_ld = _rows(query, "query")
+    query, q_ld = _rows(query)
     L = _lib.lib()
-    nws = int(L.cfh_paged_attn_ws_bytes(T, H, Hkv, D, S, most))
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws > 0 else None
+    nws = L.cfh_paged_attn_ws_bytes(T, H, Hkv, D, S, most)
+    lse = query.new_empty((H, T), dtype=torch.float32)
+    ws = query.new_empty(nws, dtype=torch.uint8) if nws > 0 else None
     _lib.check(L.cfh_paged_attn(
-        query.data_ptr(), q_ld, T, H, Hkv, D, int(query.dtype == torch.bfloat16), k_cache.data_ptr(),
-        _block_stride(k_cache), v_cache.data_ptr(), _block_stride(v_cache), _lib.ptr(k_exp), _lib.ptr(v_exp), blocks,
-        page, table.data_ptr(), max(table.stride(0), width), width, lens.data_ptr(), cu.data_ptr(), S, float(scale),
-        int(bool(causal)), most, out.data_ptr(), out.stride(0) if T > 1 else H * D, lse.data_ptr(), _lib.ptr(ws),
-        _lib.ptr(status), _lib.stream_handle()), "cfh_paged_attn")
+        query.data_ptr(), q_ld, T, H, Hkv, D, query.dtype == torch.bfloat16, k_cache.data_ptr(), bs_k, v_cache.data_ptr(),
+        bs_v, _lib.ptr(k_exp), _lib.ptr(v_exp), blocks, page, table.data_ptr(), max(table.stride(0), width), width,
+        lens.data_ptr(), cu.data_ptr(), S, scale, bool(causal), most, out.data_ptr(), o_ld, lse.data_ptr(), _lib.ptr(ws),
+        _lib.ptr(status), _lib.stream_of(dev)), "cfh_paged_attn")
     return out, lse
