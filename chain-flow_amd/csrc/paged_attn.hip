@@ -691,15 +691,17 @@ __global__ void __launch_bounds__(256, 2) k_attn_rows(PagedArgs a) {
   }
 }
 
-// The pieces of each (row, head): the largest maximum, then the sums under it, in piece order.  A workgroup of
-// four waves a (row, head), the waves a quarter of the pieces each, 4 pieces' loads in flight, D / 64 columns a
-// lane.
-template <bool BF, int D>
+// The pieces of each (row, head): the largest maximum, then the sums under it, in piece order.  W waves a (row,
+// head), each a share of the pieces, four of them in flight, D / 64 columns a lane.
+template <bool BF, int D, int W>
 __global__ void __launch_bounds__(256) k_attn_join(PagedArgs a) {
   constexpr int E = D / 64, B = 4;
-  __shared__ float so[4][D], sl[4];
+  typedef float vec __attribute__((ext_vector_type(E)));
+  __shared__ float so[W > 1 ? W : 1][D], sl[W];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int t = blockIdx.x / a.H, h = blockIdx.x % a.H;
+  const int at = W == 1 ? blockIdx.x * 4 + wave : blockIdx.x, part = W == 1 ? 0 : wave;
+  const int t = at / a.H, h = at % a.H;
+  if (t >= a.T) return;
   int s = 0, n = a.S;                             // the last sequence with cu[s] <= t (64 a step)
   while (n > 1) {
     const int step = (n + 63) / 64, i = s + lane * step;
@@ -718,19 +720,17 @@ __global__ void __launch_bounds__(256) k_attn_join(PagedArgs a) {
   float m = -INFINITY;
   for (int p = lane; p < np; p += 64) m = fmaxf(m, a.pml[p * rows + row].x);
   m = wave_max(m);
-  float l = 0.f, o[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-  const int per = (np + 3) / 4, p1 = min(np, (wave + 1) * per);
-  for (int p = wave * per; p < p1; p += B) {
+  float l = 0.f;
+  vec o = {};
+  const int per = (np + W - 1) / W, p1 = min(np, (part + 1) * per);
+  for (int p = part * per; p < p1; p += B) {
     float2 x[B];
-    float y[B][E];
+    vec y[B];
 #pragma unroll
     for (int i = 0; i < B; ++i) {
-      const size_t at = min(p + i, p1 - 1) * rows + row;
-      x[i] = a.pml[at];
-#pragma unroll
-      for (int e = 0; e < E; ++e) y[i][e] = a.po[at * D + lane * E + e];
+      const size_t q = min(p + i, p1 - 1) * rows + row;
+      x[i] = a.pml[q];
+      y[i] = *(const vec*)(a.po + q * D + lane * E);
     }
 #pragma unroll
     for (int i = 0; i < B; ++i) {
@@ -738,23 +738,34 @@ __global__ void __launch_bounds__(256) k_attn_join(PagedArgs a) {
       // (a piece that saw nothing: maximum -inf, sum 0, or NaN for a bad table)
       const float f = x[i].x == -INFINITY ? x[i].y : __builtin_amdgcn_exp2f(x[i].x - m);
       l += x[i].x == -INFINITY ? x[i].y : x[i].y * f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] += y[i][e] * f;
+      o += y[i] * f;
     }
   }
+  if constexpr (W > 1) {
+    *(vec*)&so[part][lane * E] = o;
+    if (lane == 0) sl[part] = l;
+    __syncthreads();
+    if (part) return;
+    o = vec{};
+    l = 0.f;
 #pragma unroll
-  for (int e = 0; e < E; ++e) so[wave][lane * E + e] = o[e];
-  if (lane == 0) sl[wave] = l;
-  __syncthreads();
-  l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (threadIdx.x < D / 2) {
-    const int c = threadIdx.x * 2;
-    const float x = (so[0][c] + so[1][c]) + (so[2][c] + so[3][c]);
-    const float y = (so[0][c + 1] + so[1][c + 1]) + (so[2][c + 1] + so[3][c + 1]);
-    *(unsigned*)(a.out + (size_t)t * a.o_ld + (size_t)h * D + c) = pack2<BF>(x * inv, y * inv);
+    for (int i = 0; i < W; ++i) {
+      o += *(const vec*)&so[i][lane * E];
+      l += sl[i];
+    }
   }
-  if (threadIdx.x == 0) a.lse[(size_t)h * a.T + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  u16* out = a.out + (size_t)t * a.o_ld + (size_t)h * D + lane * E;
+  if constexpr (E == 1) {
+    *out = (u16)pack2<BF>(o[0] * inv, 0.f);
+  } else {
+    unsigned y[E / 2];
+#pragma unroll
+    for (int e = 0; e < E; e += 2) y[e / 2] = pack2<BF>(o[e] * inv, o[e + 1] * inv);
+    if constexpr (E == 2) *(unsigned*)out = y[0];
+    else *(uint2*)out = make_uint2(y[0], y[1]);
+  }
+  if (lane == 0) a.lse[(size_t)h * a.T + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
 }
 
 // How a call is split, from what the host knows (sizes and an upper bound of the lengths).
@@ -785,8 +796,8 @@ Plan plan(int T, int H, int Hkv, int D, int S, int max_len) {
   p.ntile = (int)(packed / tile_rows(D)) + S;
   // pieces so that (rows' tiles) x (kv heads) x pieces fill the chip: FILL workgroups, none shorter than
   // PIECE_MIN tokens
-  const long long items = (long long)Hkv * (p.tiles ? (packed + tile_rows(D) - 1) / tile_rows(D) : S);
-  const long long want = items >= FILL / 2 ? 1 : (FILL + items - 1) / items;
+  const long long items = (long long)Hkv * std::max<long long>(p.tiles ? (packed + tile_rows(D) - 1) / tile_rows(D) : S, std::min(S, T));
+  const long long want = items >= FILL * 3 / 8 ? 1 : (FILL + items - 1) / items;
   long long piece = ((long long)max_len + want - 1) / want;
   piece = std::max<long long>(PIECE_MIN, (piece + 63) / 64 * 64);
   p.npiece = (int)std::max(1ll, ((long long)max_len + piece - 1) / piece);
@@ -873,9 +884,12 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
     CFH_LAUNCH_CHECK();
   }
   if (p.npiece > 1) {
-    const dim3 grid((unsigned)(T * H));
+    // up to 8 pieces a wave takes a (row, head) by itself, above that a workgroup
+    const bool wide = p.npiece > 8;
+    const dim3 grid((unsigned)(wide ? (long long)T * H : ((long long)T * H + 3) / 4));
     kv_dispatch(is_bf16, false, D, [&](auto bf, auto, auto d) {
-      hipLaunchKernelGGL((k_attn_join<bf.value, d.value>), grid, dim3(256), 0, st, a);
+      if (wide) hipLaunchKernelGGL((k_attn_join<bf.value, d.value, 4>), grid, dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((k_attn_join<bf.value, d.value, 1>), grid, dim3(256), 0, st, a);
     });
     CFH_LAUNCH_CHECK();
   }
