@@ -13,9 +13,17 @@ __device__ __forceinline__ uint2 read_tr(const unsigned short* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)p));
 }
 
-// 16-byte chunk order within a row of a multiple of 128 bytes: chunk c of row t lies at c ^ swz(t).  Eight rows
-// with one chunk (operands read along the rows), and four rows with two neighbouring chunks (transposed reads,
-// or 8-byte pieces), each cover all 128 bytes of the banks.
-__device__ __forceinline__ int swz(int t) { return ((t & 3) << 1) | ((t >> 2) & 1); }
+// 16-byte chunk order within rows of D 2-byte elements: chunk c of row t lies at c ^ swz<D>(t).  LDS has 64 banks of
+// 4 bytes, 16 chunks.  A 16-byte read serves 16 lanes a cycle: 16 rows with one chunk fall on different chunks.  A
+// transposed read serves 32: 4 rows with 4 neighbouring chunks, and 8 rows with 2, do too (D = 64, where two rows share
+// the 16 chunks: 4 rows with 4 chunks take two cycles).
+template <int D>
+__device__ __forceinline__ int swz(int t) {
+  if (D == 64) t >>= 1;
+  const int z = ((t & 3) << 2) | ((t >> 1) & 2) | ((t >> 3) & 1);
+  return D == 64 ? z >> 1 : z;
+}
+// The order that repeats after 8 rows: reads take two cycles for one, but half as many operand addresses are kept.
+__device__ __forceinline__ int swz8(int t) { return ((t & 3) << 1) | ((t >> 2) & 1); }
 
 }  // namespace

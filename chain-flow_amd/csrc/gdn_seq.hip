@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(768) k_gdn_chunks(GdnSeqArgs a, const char* ws
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const int row = 16 * x + (tid - 512) / 16;
-        *(uint4*)&kl[c & 1][row * GDN_DK + (((tid % 16) ^ swz(row)) * 8)] = in.k[x];
+        *(uint4*)&kl[c & 1][row * GDN_DK + (((tid % 16) ^ swz<GDN_DK>(row)) * 8)] = in.k[x];
       }
       sV[c & 1][wave][lane] = in.v;
       sF[c & 1][wave][lane] = in.f;
@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(768) k_gdn_chunks(GdnSeqArgs a, const char* ws
   auto read_in = [&](int c) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      kx[i] = *(const uint4*)&kl[c & 1][(16 * i + tl) * GDN_DK + (((4 * wave + g) ^ swz(tl)) * 8)];
+      kx[i] = *(const uint4*)&kl[c & 1][(16 * i + tl) * GDN_DK + (((4 * wave + g) ^ swz<GDN_DK>(tl)) * 8)];
     vv = read_tr((const uint16_t*)&sV[c & 1][wave][16 * g] + 4 * tl);
     fb = *(const f32x4*)&sF[c & 1][0][16 * wave + 4 * g];
     fx = *(const f32x4*)&sF[c & 1][1][16 * wave + 4 * g];
@@ -650,8 +650,8 @@ __global__ void __launch_bounds__(768) k_gdn_chunks(GdnSeqArgs a, const char* ws
       const int r0 = 32 * ks + 4 * g + tl / 4, r1 = r0 + 16, ch = 4 * wave + (tl & 3);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const uint2 y = read_tr(&kt[r0 * GDN_DK + ((ch ^ swz(r0)) * 8) + 4 * u]);
-        const uint2 z = read_tr(&kt[r1 * GDN_DK + ((ch ^ swz(r1)) * 8) + 4 * u]);
+        const uint2 y = read_tr(&kt[r0 * GDN_DK + ((ch ^ swz<GDN_DK>(r0)) * 8) + 4 * u]);
+        const uint2 z = read_tr(&kt[r1 * GDN_DK + ((ch ^ swz<GDN_DK>(r1)) * 8) + 4 * u]);
         kf[ks][u] = make_uint4(y.x, y.y, z.x, z.y);
       }
     }

@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(NW * 64, 2) k_attn_tiles(PagedArgs a) {
   constexpr int CH = D / 8;                       // 16-byte chunks a token's row
   constexpr int CPT = TK * CH / NT;               // chunks a thread stages (of K, and of V)
   constexpr int RS = NT / CH;                     // tokens between a thread's chunks
-  static_assert(CPT >= 1 && TK % 32 == 0 && RS % 8 == 0, "a tile is at least a chunk a thread; one chunk order a thread");
+  static_assert(CPT >= 1 && TK % 32 == 0 && RS % 16 == 0, "a tile is at least a chunk a thread; one chunk order a thread");
   __shared__ __align__(16) u16 lds[2][2][TK * D];
   // the tokens that some but not all rows see lie within R of each other, and a tile on either side
   constexpr int OW = (R + 2 * TK + 31) / 32;
@@ -287,16 +287,24 @@ __global__ void __launch_bounds__(NW * 64, 2) k_attn_tiles(PagedArgs a) {
   }
 
   const int srow = tid / CH, scol = tid % CH;     // this thread's chunks: tokens srow + RS x, chunk scol
-  const int sat = srow * D + ((scol ^ swz(srow)) * 8);   // (swz has a period of 8 tokens)
-  // Operand addresses: chunk c of a token lies at c ^ z, z below 8, so only c % 8 takes part and the rest, like
-  // the rows of a tile, is an offset in the instruction
-  int ka[4], va[2];
+  // Operand addresses: chunk c of token t lies at c ^ z(t), z below 2 KA, so only the low bits of c take part and the
+  // rest, like the rows of a tile, is an offset in the instruction.  At D = 256 the accumulators leave no registers
+  // for the 16 addresses of swz (they spill: 764 us where the 6 of swz8, whose reads take twice the LDS cycles, take
+  // 541; 3,841 rows over 9,001 tokens, 16 / 4 heads)
+  constexpr bool S8 = D == 256;
+  constexpr int KA = S8 || D == 64 ? 4 : 8, VA = KA / 2;
+  auto order = [](int t) { return S8 ? swz8(t) : swz<D>(t); };
+  const int sat = srow * D + ((scol ^ order(srow)) * 8);
+  int ka[KA], va[2][VA];
   {
     const int kt = lane & 31, vt = 4 * half + (lane & 15) / 4, vc = 2 * ((lane >> 4) & 1) + (lane & 3) / 2;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) ka[i] = kt * D + (((2 * i + half) ^ swz(kt)) * 8);
+    for (int i = 0; i < KA; ++i) ka[i] = kt * D + (((2 * i + half) ^ order(kt)) * 8);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) va[i] = vt * D + (((4 * i + vc) ^ swz(vt)) * 8) + 4 * (lane & 1);
+    for (int i = 0; i < VA; ++i) {
+      va[0][i] = vt * D + (((4 * i + vc) ^ order(vt)) * 8) + 4 * (lane & 1);
+      va[1][i] = S8 ? va[0][i] : (vt + 8) * D + (((4 * i + vc) ^ order(vt + 8)) * 8) + 4 * (lane & 1);
+    }
   }
   uint4 kr[CPT], vr[CPT];
   int kx[CPT], vx[CPT];
@@ -354,11 +362,12 @@ __global__ void __launch_bounds__(NW * 64, 2) k_attn_tiles(PagedArgs a) {
       const u16* vt = lds[buf][1];
       f32x16 sc[TK / 32];
 #pragma unroll
-      for (int b = 0; b < TK / 32; ++b) {
-        sc[b] = f32x16{};
+      for (int b = 0; b < TK / 32; ++b) sc[b] = f32x16{};
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s)
-          sc[b] = mfma32<BF>(*(const uint4*)&kt[ka[s & 3] + 32 * b * D + s / 4 * 64], qf[s], sc[b]);
+      for (int s = 0; s < D / 16; ++s) {
+#pragma unroll
+        for (int b = 0; b < TK / 32; ++b)
+          sc[b] = mfma32<BF>(*(const uint4*)&kt[ka[s % KA] + 32 * b * D + s / KA * 16 * KA], qf[s], sc[b]);
       }
       if (jt + TK > vis_wave) {
 #pragma unroll
@@ -398,8 +407,8 @@ __global__ void __launch_bounds__(NW * 64, 2) k_attn_tiles(PagedArgs a) {
       }
       // the transposed reads: lane block (lane / 16) % 2 takes 16 of the 32 columns, half the tokens 4 half ..
       auto vfrag = [&](int d, int s) {
-        const u16* p = &vt[va[d & 1] + 16 * s * D + d / 2 * 64];
-        const uint2 x = read_tr(p), y = read_tr(p + 8 * D);
+        const int at = 16 * s * D + d / VA * 32 * VA;
+        const uint2 x = read_tr(&vt[va[0][d % VA] + at]), y = read_tr(&vt[va[1][d % VA] + at + (S8 ? 8 * D : 0)]);
         return make_uint4(x.x, x.y, y.x, y.y);
       };
 #pragma unroll
@@ -514,11 +523,12 @@ __global__ void __launch_bounds__(256, 2) k_attn_rows(PagedArgs a) {
     }
   }
   u16* const vt = sh.v[wave];
-  int va[4];                                      // (as in k_attn_tiles)
+  constexpr int VA = D == 64 ? 4 : 8;             // (as in k_attn_tiles)
+  int va[VA];
 #pragma unroll
-  for (int x = 0; x < 4; ++x) {
+  for (int x = 0; x < VA; ++x) {
     const int tr = 4 * g + tl / 4;
-    va[x] = tr * D + (((2 * x + (tl & 3) / 2) ^ swz(tr)) * 8) + 4 * (tl & 1);
+    va[x] = tr * D + (((2 * x + (tl & 3) / 2) ^ swz<D>(tr)) * 8) + 4 * (tl & 1);
   }
   // this lane's token of K's tile u is 16 u + tl; its chunks of V are of tokens (lane + 64 x) / CH
   uint4 kr[U][KL], vr[VL];
@@ -577,7 +587,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_rows(PagedArgs a) {
           v = only_finite<BF>(v);
           atomicOr(&odd[(jt + tok - odd_base) / 32], 1u << ((jt + tok - odd_base) & 31));
         }
-        *(uint4*)&vt[tok * D + (((ch + y) ^ swz(tok)) * 8)] = v;
+        *(uint4*)&vt[tok * D + (((ch + y) ^ swz<D>(tok)) * 8)] = v;
       }
     }
     v_fetch(jt + step);                           // (past the work's tokens: its last ones again, never used)
@@ -627,7 +637,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_rows(PagedArgs a) {
       pf[u] = make_uint2(pack2<BF>(sc[u][0], sc[u][1]), pack2<BF>(sc[u][2], sc[u][3]));
     }
     // (a wave's LDS accesses complete in order: its reads see its own writes above)
-    auto vfrag = [&](int d, int u) { return read_tr(&vt[va[d & 3] + 16 * u * D + d / 4 * 64]); };
+    auto vfrag = [&](int d, int u) { return read_tr(&vt[va[d % VA] + 16 * u * D + d / VA * 16 * VA]); };
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) {
       if constexpr (U == 1) {
