@@ -19,6 +19,7 @@
 // three of S).
 // Differences of G are taken in 64 bits: a strong decay earlier in the chunk must not cost a weak one later its
 // digits (decays below e^-200 are taken as that: both are 0 in fp32).
+#include <algorithm>
 #include <type_traits>
 
 #include "cfh_gdn.h"
@@ -704,8 +705,14 @@ __global__ void __launch_bounds__(768) k_gdn_chunks(GdnSeqArgs a, const char* ws
   }
 }
 
-// Rows a sequence, on average, up to which they go one after another (k_gdn_rows).
-constexpr int GDN_ROWS_MAX = 8;
+// Whether the rows go one after another (k_gdn_rows): up to 8 a sequence on average, and 2 more for each round of
+// workgroups that k_gdn_chunks takes, one a CU (32 value heads of 128; one after another / in chunks: one sequence of
+// 8 rows 12.3 / 13.9 us, of 12 16.7 / 14.0; eight of 16 27.9 / 40.9, of 24 38.2 / 42.0, of 32 48.7 / 42.0).
+constexpr int GDN_ROWS_MAX = 8, GDN_CUS = 256;
+inline bool rows_in_turn(long long T, long long S, int HV, int V) {
+  const long long rounds = std::min((S * HV * (V / 16) + GDN_CUS - 1) / GDN_CUS, 8ll);
+  return T <= (GDN_ROWS_MAX + 2 * rounds) * S;
+}
 
 inline long long chunk_slots(int T, int S) { return (long long)T / GC + S; }
 
@@ -768,7 +775,7 @@ int cfh_gdn_prefill(const void* mixed_qkv, const void* a, const void* b, const f
   g.cu = cu_seqlens;
   g.initial = initial;
   hipStream_t st = (hipStream_t)stream;
-  if ((long long)T <= (long long)GDN_ROWS_MAX * S) return launch_rows(g, state_bf16, st);
+  if (rows_in_turn(T, S, HV, V)) return launch_rows(g, state_bf16, st);
   if (!ws || (uintptr_t)ws % 256) return CFH_E_INVALID;
   const long long prep = chunk_slots(T, S) * HV, blocks = ((long long)S * HV + 7) / 8 * 8 * (V / 16);
   if (prep > 0x7fffffffll || blocks > 0x7fffffffll) return CFH_E_UNSUPPORTED;

@@ -704,7 +704,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_rows(PagedArgs a) {
 // The pieces of each (row, head): the largest maximum, then the sums under it, in piece order.  W waves a (row,
 // head), each a share of the pieces, four of them in flight, D / 64 columns a lane.
 template <bool BF, int D, int W>
-__global__ void __launch_bounds__(256) k_attn_join(PagedArgs a) {
+__global__ void __launch_bounds__(W == 1 ? 256 : W * 64) k_attn_join(PagedArgs a) {
   constexpr int E = D / 64, B = 4;
   typedef float vec __attribute__((ext_vector_type(E)));
   __shared__ float so[W > 1 ? W : 1][D], sl[W];
@@ -786,7 +786,7 @@ struct Plan {
   int piece, npiece;
 };
 
-constexpr int FEW_ROWS = 16, PIECE_MIN = 256, FILL = 512;
+constexpr int FEW_ROWS = 16;
 
 constexpr int tile_rows(int D) { return D == 256 ? 256 : 128; }
 
@@ -804,12 +804,15 @@ Plan plan(int T, int H, int Hkv, int D, int S, int max_len) {
   }
   p.nrow = p.few ? S : (int)(packed / FEW_ROWS) + S;
   p.ntile = (int)(packed / tile_rows(D)) + S;
-  // pieces so that (rows' tiles) x (kv heads) x pieces fill the chip: FILL workgroups, none shorter than
-  // PIECE_MIN tokens
+  // Pieces so that (row tiles) x (kv heads) x pieces fill the chip with the workgroups it holds at once, one a CU at
+  // D = 256 with many rows, else two; none from three quarters of a workgroup a CU on (244 of them, 3,841 rows over
+  // 9,001 tokens: cut in two 614 us, whole 551).  Pieces of 512 tokens at least where rows are few (one row over
+  // 30,011: 256 tokens 25 / 29 us at D = 64 / 128, 512 tokens 20 / 24), 256 where they are many.
+  const int fill = p.tiles && D == 256 ? 256 : 512, least = p.tiles ? 256 : 512;
   const long long items = (long long)Hkv * std::max<long long>(p.tiles ? (packed + tile_rows(D) - 1) / tile_rows(D) : S, std::min(S, T));
-  const long long want = items >= FILL * 3 / 8 ? 1 : (FILL + items - 1) / items;
+  const long long want = items >= 192 ? 1 : (fill + items - 1) / items;
   long long piece = ((long long)max_len + want - 1) / want;
-  piece = std::max<long long>(PIECE_MIN, (piece + 63) / 64 * 64);
+  piece = std::max<long long>(least, (piece + 63) / 64 * 64);
   p.npiece = (int)std::max(1ll, ((long long)max_len + piece - 1) / piece);
   p.piece = (int)std::min<long long>(piece, 0x40000000);
   return p;
@@ -894,11 +897,12 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
     CFH_LAUNCH_CHECK();
   }
   if (p.npiece > 1) {
-    // up to 8 pieces a wave takes a (row, head) by itself, above that a workgroup
+    // up to 8 pieces a wave takes a (row, head) by itself, above that a workgroup of 16 (59 pieces of 16 rows and
+    // heads: 14 us with 4 waves)
     const bool wide = p.npiece > 8;
     const dim3 grid((unsigned)(wide ? (long long)T * H : ((long long)T * H + 3) / 4));
     kv_dispatch(is_bf16, false, D, [&](auto bf, auto, auto d) {
-      if (wide) hipLaunchKernelGGL((k_attn_join<bf.value, d.value, 4>), grid, dim3(256), 0, st, a);
+      if (wide) hipLaunchKernelGGL((k_attn_join<bf.value, d.value, 16>), grid, dim3(1024), 0, st, a);
       else hipLaunchKernelGGL((k_attn_join<bf.value, d.value, 1>), grid, dim3(256), 0, st, a);
     });
     CFH_LAUNCH_CHECK();
