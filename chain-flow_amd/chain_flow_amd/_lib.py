@@ -171,6 +171,19 @@ def stream_of(dev: int) -> int:
     return torch._C._cuda_getCurrentRawStream(dev)
 
 
+def index32(t, dev: int):
+    """An index tensor as int32 on device ``dev``, contiguous; 64-bit values that 32 bits do not hold become the
+    nearest that they do (both lie outside whatever they index)."""
+    import torch
+    if t.dtype == torch.int32:
+        if t.get_device() != dev:
+            t = t.to(f"cuda:{dev}")
+        return t.contiguous()
+    if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool:
+        raise ValueError(f"an index tensor must hold integers, not {t.dtype}")
+    return t.to(f"cuda:{dev}", torch.int64).clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32).contiguous()
+
+
 def aligned(t):
     """The tensor, or a copy of it that starts on a 16-byte boundary as the vector loads need."""
     return t if t.data_ptr() % 16 == 0 else t.clone()

@@ -117,14 +117,7 @@ def _seq_args(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, H, out, status,
     if A_log.dtype != torch.float32 or dt_bias.dtype != torch.float32:
         A_log, dt_bias = A_log.float(), dt_bias.float()
     return (_lib.aligned(mixed_qkv.contiguous()), a.contiguous(), b.contiguous(), A_log.contiguous(), dt_bias.contiguous(),
-            _on(slots, dev), out, dev)
-
-
-def _on(index, dev):
-    """An index tensor as int32 on the device."""
-    if index.dtype != torch.int32 or index.get_device() != dev:
-        index = index.to(f"cuda:{dev}", torch.int32)
-    return index.contiguous()
+            _lib.index32(slots, dev), out, dev)
 
 
 def gdn_decode(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, *, num_q_heads: int, scale: float | None = None,
@@ -146,14 +139,14 @@ def gdn_decode(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, *, num_q_heads
     _lib.check(_lib.lib().cfh_gdn_decode(
         x.data_ptr(), a.data_ptr(), b.data_ptr(), A_log.data_ptr(), dt_bias.data_ptr(), ssm_state.data_ptr(),
         ssm_state.dtype == torch.bfloat16, nslots, slots.data_ptr(), S, H, HV, K, V, bool(use_qk_l2norm),
-        K ** -0.5 if scale is None else scale, out.data_ptr(), _lib.ptr(status), _lib.stream_of(dev)), "cfh_gdn_decode")
+        float(K ** -0.5 if scale is None else scale), out.data_ptr(), _lib.ptr(status), _lib.stream_of(dev)), "cfh_gdn_decode")
     return out
 
 
 def gdn_prefill(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, cu_seqlens, *, num_q_heads: int, initial=None,
                 scale: float | None = None, use_qk_l2norm: bool = True, out=None, status: torch.Tensor | None = None):
     """The rows of S sequences (or chunks of them) through the gated delta rule: sequence s has the rows
-    cu_seqlens[s] .. cu_seqlens[s + 1] of mixed_qkv [T, 2 H K + HV V], starts from slot slots[s] of ssm_state
+    cu_seqlens[s] .. cu_seqlens[s + 1] (ascending) of mixed_qkv [T, 2 H K + HV V], starts from slot slots[s] of ssm_state
     (from zero where ``initial`` [S] bool is given and false) and leaves its state there, rounded to the
     slot's type once.  Layout, gates and slots as in ``gdn_decode``; the state a draft tree's roots start
     from (``tree_gdn_vllm``'s prefix slot).  -> o [T, HV, V] bf16.  ``cfh_gdn_prefill``, no host
@@ -164,7 +157,7 @@ def gdn_prefill(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, cu_seqlens, *
     nslots, HV, V, K = ssm_state.shape
     if cu_seqlens.shape != (S + 1,):
         raise ValueError(f"cu_seqlens must be [{S + 1}]")
-    cu = _on(cu_seqlens, dev)
+    cu = _lib.index32(cu_seqlens, dev)
     if initial is not None:
         if initial.shape != (S,) or initial.dtype not in (torch.bool, torch.uint8):
             raise ValueError(f"initial must be a bool [{S}] tensor")
@@ -174,6 +167,6 @@ def gdn_prefill(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, cu_seqlens, *
     _lib.check(L.cfh_gdn_prefill(
         x.data_ptr(), a.data_ptr(), b.data_ptr(), A_log.data_ptr(), dt_bias.data_ptr(), ssm_state.data_ptr(),
         ssm_state.dtype == torch.bfloat16, nslots, slots.data_ptr(), cu.data_ptr(), _lib.ptr(initial), S, T, H, HV, K, V,
-        bool(use_qk_l2norm), K ** -0.5 if scale is None else scale, out.data_ptr(), ws.data_ptr(), _lib.ptr(status),
+        bool(use_qk_l2norm), float(K ** -0.5 if scale is None else scale), out.data_ptr(), ws.data_ptr(), _lib.ptr(status),
         _lib.stream_of(dev)), "cfh_gdn_prefill")
     return out

@@ -7,7 +7,7 @@
   ``tree_attn_merge`` merges with.
 
 A cache is [blocks, page, Hkv, D] of the model's type (bf16 or fp16), or of ``torch.float8_e4m3fn`` with a
-byte [blocks, page, Hkv] (uint8) per slot and head: byte c stands for the scale 2^(c - 127).  Slot n is row
+byte [blocks, page, Hkv] (uint8) per slot and head: byte c, 1 to 254, stands for the scale 2^(c - 127).  Slot n is row
 n % page of block n / page.  The blocks of a cache may be strided (two halves of one allocation); within a
 block it is contiguous.  No call synchronises with the host.
 """
@@ -60,13 +60,6 @@ def _rows(t):
     return t, ld
 
 
-def _i32(t, dev):
-    """An index tensor as int32 on the device."""
-    if t.dtype != torch.int32 or t.get_device() != dev:
-        t = t.to(f"cuda:{dev}", torch.int32)
-    return t.contiguous()
-
-
 def kv_cache_write(key, value, k_cache, v_cache, slots, *, k_exp=None, v_exp=None, status=None) -> None:
     """key, value [T, Hkv, D] bf16 or fp16 (rows may be strided) into ``slots`` [T] of the cache, in place.
 
@@ -89,7 +82,7 @@ def kv_cache_write(key, value, k_cache, v_cache, slots, *, k_exp=None, v_exp=Non
         used = slots[slots >= 0]
         if used.unique().numel() != used.numel() or (used >= blocks * page).any():
             raise ValueError(f"slots must be distinct and below {blocks * page}")
-    slots = _i32(slots, dev)
+    slots = _lib.index32(slots, dev)
     key, ld_k = _rows(key)
     value, ld_v = _rows(value)
     _lib.check(_lib.lib().cfh_kv_write(
@@ -110,7 +103,7 @@ def kv_cache_read(k_cache, v_cache, slots, *, dtype=None, k_exp=None, v_exp=None
     if slots.dim() != 1:
         raise ValueError("slots must be [T]")
     dev = _lib.device_of(k_cache, v_cache, k_exp, v_exp, status=status)
-    slots = _i32(slots, dev)
+    slots = _lib.index32(slots, dev)
     T = slots.shape[0]
     key = k_cache.new_empty((T, Hkv, D), dtype=dtype)
     value = torch.empty_like(key)
@@ -124,7 +117,7 @@ def kv_cache_read(k_cache, v_cache, slots, *, dtype=None, k_exp=None, v_exp=None
 def paged_attention(query, k_cache, v_cache, block_table, seq_lens, cu_q, *, scale: float, causal: bool = True,
                     k_exp=None, v_exp=None, max_len: int | None = None, out=None, status=None):
     """query [T, H, D] (rows may be strided; H a multiple of Hkv) over the cache: sequence s has the query rows
-    cu_q[s] .. cu_q[s + 1] and seq_lens[s] tokens in blocks block_table[s]; row i of its n sees token j where
+    cu_q[s] .. cu_q[s + 1] (ascending) and seq_lens[s] tokens in blocks block_table[s]; row i of its n sees token j where
     j < len and, if ``causal``, j <= len - n + i (the rows' own keys and values are the cache's last n, written
     before the call).  -> (out [T, H, D] of the query's type, lse [H, T] fp32: ``tree_attn_merge``'s prefix_lse).
 
@@ -154,11 +147,11 @@ def paged_attention(query, k_cache, v_cache, block_table, seq_lens, cu_q, *, sca
                              "16-byte aligned")
     table = block_table
     if table.dtype != torch.int32 or table.get_device() != dev:
-        table = table.to(f"cuda:{dev}", torch.int32)
+        table = _lib.index32(table, dev)
     width = table.shape[1]
     if table.stride(1) != 1 or table.stride(0) < width:
         table = table.contiguous()
-    lens, cu = _i32(seq_lens, dev), _i32(cu_q, dev)
+    lens, cu = _lib.index32(seq_lens, dev), _lib.index32(cu_q, dev)
     most = width * page
     most = most if max_len is None else max(0, min(int(max_len), most))
     query, q_ld = _rows(query)
@@ -169,6 +162,6 @@ def paged_attention(query, k_cache, v_cache, block_table, seq_lens, cu_q, *, sca
     _lib.check(L.cfh_paged_attn(
         query.data_ptr(), q_ld, T, H, Hkv, D, query.dtype == torch.bfloat16, k_cache.data_ptr(), bs_k, v_cache.data_ptr(),
         bs_v, _lib.ptr(k_exp), _lib.ptr(v_exp), blocks, page, table.data_ptr(), max(table.stride(0), width), width,
-        lens.data_ptr(), cu.data_ptr(), S, scale, bool(causal), most, out.data_ptr(), o_ld, lse.data_ptr(), _lib.ptr(ws),
+        lens.data_ptr(), cu.data_ptr(), S, float(scale), bool(causal), most, out.data_ptr(), o_ld, lse.data_ptr(), _lib.ptr(ws),
         _lib.ptr(status), _lib.stream_of(dev)), "cfh_paged_attn")
     return out, lse

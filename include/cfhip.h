@@ -491,7 +491,7 @@ int cfh_tree_greedy_accept(const void* logits, long long ld, int V, int n_rows, 
  * row n % page of block n / page; block strides bs_k / bs_v in elements (multiples of 16, at least
  * page Hkv D: the two may be views of one allocation), rows within a block contiguous.  With k_exp and
  * v_exp NULL the elements are 2-byte (bf16 or fp16: is_bf16); with both given they are e4m3, and byte
- * c = exp[blocks][page][Hkv] is the scale 2^(c - 127) of its (slot, head).  Any page size; D in
+ * c = exp[blocks][page][Hkv], 1 to 254, is the scale 2^(c - 127) of its (slot, head).  Any page size; D in
  * {64, 128, 256}; blocks * page < 2^31.  Pointers 16-byte aligned, row strides multiples of 8 elements.
  *
  * cfh_kv_write: rows key / value [T][Hkv][D] (row strides ld_k / ld_v, heads contiguous) into slots[T].
@@ -511,8 +511,8 @@ int cfh_kv_read(const void* k_cache, long long bs_k, const void* v_cache, long l
                 const uint8_t* v_exp, int blocks, int page, const int32_t* slots, int T, int Hkv, int D, int is_bf16,
                 void* key, void* value, int32_t* status, void* stream);
 
-/* Attention of new rows over the cache: sequence s has the query rows cu_q[s] .. cu_q[s+1] of q [T][H][D]
- * (row stride q_ld) and seq_lens[s] tokens in the blocks table[s][..] (S rows of stride table_ld,
+/* Attention of new rows over the cache: sequence s has the query rows cu_q[s] .. cu_q[s+1] (ascending) of
+ * q [T][H][D] (row stride q_ld) and seq_lens[s] tokens in the blocks table[s][..] (S rows of stride table_ld,
  * max_blocks entries usable).  Its row i of n sees token j where j < len and, if causal, j <= len - n + i:
  *   out = sum_j softmax_j(scale q.k_j) v_j (row stride o_ld), lse [H][T] fp32 = log sum_j exp(scale q.k_j)
  * over kv head h / (H / Hkv); a row that sees nothing gives 0 and -inf.  causal = 0 with a draft tree's
@@ -540,7 +540,7 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
  * synchronise and can be captured.
  *
  * cfh_gdn_decode: one token a sequence, row s of mixed_qkv [S].
- * cfh_gdn_prefill: sequence s has the rows cu_seqlens[s] .. cu_seqlens[s+1] of mixed_qkv [T] (a sequence
+ * cfh_gdn_prefill: sequence s has the rows cu_seqlens[s] .. cu_seqlens[s+1] (ascending) of mixed_qkv [T] (a sequence
  * whose bounds do not lie in [0, T] is skipped and sets status; one of no rows leaves its slot as it was;
  * rows of no sequence are left as they were).  initial [S] (or NULL: all 1): 0 = start from a zero state
  * instead of the slot's.  ws: cfh_gdn_prefill_ws_bytes(T, S, HV) bytes, 256-byte aligned. */

@@ -242,11 +242,12 @@ def test_attention_peaked_and_flat_scores(cuda):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,cache", [(BF, BF), (FP, FP), (BF, F8)])
-@pytest.mark.parametrize("new,length", [(40, 40), (70, 200), (1, 90)])
-def test_masked_places_do_not_reach_a_row(cuda, dtype, cache, new, length):
+@pytest.mark.parametrize("new,length,D", [(40, 40, 128), (70, 200, 128), (1, 90, 128), (70, 200, 64), (70, 200, 256),
+                                          (3, 700, 256), (3, 700, 64), (150, 150, 256)])
+def test_masked_places_do_not_reach_a_row(cuda, dtype, cache, new, length, D):
     """NaN and infinities in keys and values of later tokens of the chunk: a row that does not see them is what it is
     without them, a row that does is not finite where they are."""
-    c = Case(cuda, dtype, cache, [new], [length], 4, 2, 128, 16, seed=5)
+    c = Case(cuda, dtype, cache, [new], [length], 4, 2, D, 16, seed=5)
     clean = c.run()
     at = length - 1                                           # the last token: only the last row sees it
     blk, off = int(c.table[0, at // 16]), at % 16
@@ -255,13 +256,13 @@ def test_masked_places_do_not_reach_a_row(cuda, dtype, cache, new, length):
         c.k.view(torch.uint8)[blk, off, 1, 5] = 0x7F
     else:
         c.v[blk, off, 0, 5], c.v[blk, off, 0, 9], c.k[blk, off, 1, 5] = float("nan"), float("inf"), float("nan")
-    print(f"[paged attn NaN] {dtype} {cache} new={new} length={length}", flush=True)
+    print(f"[paged attn NaN] {dtype} {cache} new={new} length={length} D={D}", flush=True)
     out, lse = c.run()
     assert torch.equal(out[:-1], clean[0][:-1]) and torch.equal(lse[:, :-1], clean[1][:, :-1])
     assert out[-1, :2, 5].isnan().all() and out[-1, 2:].isnan().all() and lse[2:, -1].isnan().all()
     if cache != F8:
         assert (out[-1, :2, 9] == float("inf")).all()
-    keep = [d for d in range(128) if d not in (5, 9)]
+    keep = [d for d in range(D) if d not in (5, 9)]
     assert torch.equal(out[-1, :2][:, keep], clean[0][-1, :2][:, keep])
 
 
@@ -417,3 +418,41 @@ def test_two_streams_at_once(cuda):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(o, alone[i][0]) and torch.equal(e, alone[i][1]) for o, e in got[i])
+
+
+@pytest.mark.gpu
+def test_index_tensors_of_64_bits(cuda):
+    """int64 slots, tables, lengths and bounds; a slot past 32 bits is outside the cache, not what its low half says;
+    floats are refused."""
+    c = Case(cuda, BF, BF, [2, 1], [40, 9], 4, 2, 64, 16, seed=21)
+    ref = c.run()
+    i64 = lambda x: torch.as_tensor(x).long().to(cuda)  # noqa: E731
+    got = paged_attention(c.q, c.k, c.v, i64(c.table), i64(c.lens), i64(c.cu), scale=c.scale)
+    assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    before = c.k.clone()
+    key = torch.ones(2, 2, 64, dtype=BF, device=cuda)
+    kv_cache_write(key, key, c.k, c.v, i64([2 ** 32, -2 ** 40]), status=status)
+    assert status.item() == 1 and torch.equal(c.k.nan_to_num(7.0), before.nan_to_num(7.0))
+    with pytest.raises(ValueError, match="integers"):
+        kv_cache_write(key, key, c.k, c.v, torch.zeros(2, device=cuda))
+
+
+@pytest.mark.gpu
+def test_attention_in_place_of_the_query(cuda):
+    """out may be the query itself: every row and head is read by the workgroups that write it, before they do."""
+    for news, lens in (([1, 1], [3000, 40]), ([100], [300])):
+        c = Case(cuda, BF, BF, news, lens, 8, 2, 128, 16, seed=22)
+        ref = c.run()
+        got = c.run(out=c.q)
+        assert got[0].data_ptr() == c.q.data_ptr() and torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+
+
+@pytest.mark.gpu
+def test_attention_mixed_batch_of_few_and_many_rows(cuda):
+    """Decode rows and chunks in one call: each sequence by the kernel for its row count."""
+    c = Case(cuda, BF, BF, [1, 90, 1, 4, 33, 0, 1], [500, 200, 1, 70, 33, 20, 64], 8, 2, 128, 16, seed=23)
+    print("[paged attn mixed]", flush=True)
+    c.check(*c.run())
+    c = Case(cuda, FP, F8, [1] * 20 + [200], [30 + 7 * i for i in range(20)] + [250], 16, 4, 256, 64, seed=24)
+    c.check(*c.run())
