@@ -19,6 +19,9 @@
 // three of S).
 // Differences of G are taken in 64 bits: a strong decay earlier in the chunk must not cost a weak one later its
 // digits (decays below e^-200 are taken as that: both are 0 in fp32).
+//   A row that is not finite must not reach the rows before it, whose triangular products multiply it by zeros.  Entries
+// of R and d past the largest finite bf16 enter the products as that number, and from the first of them on the outputs
+// of their column, and its state, are NaN.
 #include <algorithm>
 #include <type_traits>
 
@@ -172,6 +175,8 @@ constexpr int GC = 64;                             // rows a chunk
 // [row tile][k-step][part][lane] 16 B; then the rows' factors, fp32 [4][64], and e^G_C
 constexpr int GW_ATT = 4 * 2 * 2 * 64 * 16, GW_VEC = 2 * GW_ATT;
 constexpr int GW_BYTES = GW_VEC + 4 * GC * 4 + 256;
+
+constexpr float GDN_RANGE = 0x1.fep127f;           // the largest finite bf16
 
 __device__ __forceinline__ f32x4 mfma_b(const uint4& x, const uint4& y, f32x4 acc) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, x), __builtin_bit_cast(b16x8, y), acc, 0, 0, 0);
@@ -365,6 +370,9 @@ __global__ void __launch_bounds__(256) k_gdn_prep(GdnSeqArgs a, char* ws) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           m = __builtin_amdgcn_mfma_f32_16x16x4f32(Ls[16 * wave + tl][16 * c + 4 * k + g], Ts[16 * c + 4 * k + g][16 * b + tl], m, 0, 0, 0);
+      // (a row of L that is not finite: its R is not either, which k_gdn_chunks answers for)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) m[r] = fabsf(m[r]) < INFINITY ? m[r] : 0.f;
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         t = __builtin_amdgcn_mfma_f32_16x16x4f32(Ts[16 * wave + tl][16 * wave + 4 * g + r], m[r], t, 0, 0, 0);
@@ -437,6 +445,7 @@ __global__ void __launch_bounds__(768) k_gdn_chunks(GdnSeqArgs a, const char* ws
   __shared__ __align__(16) uint4 sS[4][2][64];              // S for the outputs: [k-step = wave][part][lane]
   __shared__ __align__(16) uint2 sR[NP][2][64][2], sE[NP][2][64][2], sD[2][2][64][2];   // [part][k-step][lane][tile of it]
   __shared__ __align__(16) uint2 sV[2][4][64];              // v: [row tile][row, 4 columns]
+  __shared__ int sBad[2][16];                               // the first row of each column that is not finite
   __shared__ __align__(16) float sF[2][4][GC];              // beta, beta e^G |k|^-1, e^(G_C - G) |k|^-1, e^G_C
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, tl = lane & 15;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), wave = wv & 3;
@@ -484,6 +493,7 @@ __global__ void __launch_bounds__(768) k_gdn_chunks(GdnSeqArgs a, const char* ws
       }
       sV[c & 1][wave][lane] = in.v;
       sF[c & 1][wave][lane] = in.f;
+      if (tid < 512 + 16) sBad[c & 1][tid - 512] = GC;
     };
     auto work = [&](int c, KeyIn& in, const KeyIn& next) {
       lds_barrier();                                         // B1
@@ -544,7 +554,10 @@ __global__ void __launch_bounds__(768) k_gdn_chunks(GdnSeqArgs a, const char* ws
         o[2] = mfma_b(in.at[ks][1], hi, o[2]);
       }
       load_a(min(c + 1, nc - 1), next, nk);
-      const f32x4 O = Y[0] + (o[0] + (o[1] + o[2]));
+      f32x4 O = Y[0] + (o[0] + (o[1] + o[2]));
+      const int bad = sBad[c & 1][tl] - (16 * wave + 4 * g);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) O[r] = r < bad ? O[r] : __builtin_nanf("");
       const int t0 = c0 + c * GC;
       const auto b = span(a.out + (size_t)t0 * rs, min(GC, c1 - t0) * (int)rs * 2);
 #pragma unroll
@@ -601,7 +614,19 @@ __global__ void __launch_bounds__(768) k_gdn_chunks(GdnSeqArgs a, const char* ws
     fe = *(const f32x4*)&sF[c & 1][2][16 * wave + 4 * g];
     eg = sF[c & 1][3][0];
   };
-  auto work = [&](int c, const uint4 (&t)[2][2], uint4 (&tnext)[2][2], auto nk) {
+  // entries out of range come back inside it; the first of the lane's four rows that has one (or `first`).  No branch:
+  // it would cost the loads in flight more than the selects.
+  auto into_range = [&](f32x4& x, int first) {
+#pragma unroll
+    for (int r = 3; r >= 0; --r) {
+      const float y = __builtin_amdgcn_fmed3f(x[r], -GDN_RANGE, GDN_RANGE);
+      first = x[r] == y ? first : min(first, 16 * wave + 4 * g + r);
+      x[r] = y;
+    }
+    return first;
+  };
+  // (inlined whatever its size: a call would have everything it refers to in scratch memory)
+  auto work = [&](int c, const uint4 (&t)[2][2], uint4 (&tnext)[2][2], auto nk) __attribute__((always_inline)) {
     const uint16_t* kt = kl[c & 1];
     uint2 p0[2], p1[2], pn[NP];
     uint4 sp[2];
@@ -625,6 +650,7 @@ __global__ void __launch_bounds__(768) k_gdn_chunks(GdnSeqArgs a, const char* ws
     f32x4 R;
 #pragma unroll
     for (int r = 0; r < 4; ++r) R[r] = fb[r] * v[r] - fx[r] * x[r];
+    int bad = into_range(R, GC);
     split4(R, pn);
 #pragma unroll
     for (int p = 0; p < NP; ++p) sR[p][wave >> 1][lane][wave & 1] = pn[p];
@@ -656,14 +682,16 @@ __global__ void __launch_bounds__(768) k_gdn_chunks(GdnSeqArgs a, const char* ws
         kf[ks][u] = make_uint4(y.x, y.y, z.x, z.y);
       }
     }
-    const f32x4 D = d[0] + (d[1] + d[2]);
+    f32x4 D = d[0] + (d[1] + d[2]);
+    bad = into_range(D, bad);
+    __hip_atomic_fetch_min(&sBad[c & 1][tl], bad, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     split4(D * fe, pn);
 #pragma unroll
     for (int p = 0; p < NP; ++p) sE[p][wave >> 1][lane][wave & 1] = pn[p];
     split4(D, p1);
 #pragma unroll
     for (int p = 0; p < 2; ++p) sD[p][wave >> 1][lane][wave & 1] = p1[p];
-    const float keep = eg;
+    const float eg0 = eg;
     lds_barrier();                                           // B3
     f32x4 up[2][2] = {};
     uint4 y[2][NP];
@@ -671,6 +699,7 @@ __global__ void __launch_bounds__(768) k_gdn_chunks(GdnSeqArgs a, const char* ws
     for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
       for (int p = 0; p < NP; ++p) y[ks][p] = *(const uint4*)sE[p][ks][lane];
+    const float keep = sBad[c & 1][tl] < GC ? __builtin_nanf("") : eg0;
     read_in(min(c + 1, nc - 1));
 #pragma unroll
     for (int p = NP - 1; p >= 0; --p)

@@ -253,3 +253,66 @@ def test_prefill_and_decode_in_one_graph(cuda):
         want = step(est)
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(got, want)) and torch.equal(gst, est), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("where", ["q", "k", "v", "a", "b"])
+@pytest.mark.parametrize("at", [0, 5, 22, 70, 127])
+def test_a_row_that_is_not_finite_leaves_the_rows_before_it(cuda, where, at):
+    """NaN or infinity in one row's q, k, v or gates: the rows before it are what they are without it, it and (but for q)
+    the rows after it are NaN where it reaches: the whole value head, or with v its own column; the other sequence and
+    the other heads as without it."""
+    clean = Case(cuda, [150, 40], seed=12)
+    ref, rst = clean.run()
+    c = Case(cuda, [150, 40], seed=12)
+    K, h = 128, 1                                                          # q/k head 1: value heads 2 and 3
+    hit = torch.zeros(4, 64, dtype=torch.bool)
+    if where == "q":
+        c.x[at, h * K + 3] = float("nan")
+        hit[2:] = True
+    elif where == "k":
+        c.x[at, (c.H + h) * K + 7] = float("inf")
+        hit[2:] = True
+    elif where == "v":
+        c.x[at, 2 * c.H * K + 2 * 64 + 9] = float("nan")
+        hit[2, 9] = True
+    else:
+        (c.a if where == "a" else c.b)[at, 3] = float("nan")
+        hit[3] = True
+    o, st = c.run()
+    assert torch.equal(o[:at], ref[:at]) and torch.equal(o[150:], ref[150:])
+    after = o[at:150].cpu()
+    assert torch.equal(after[:, ~hit], ref[at:150].cpu()[:, ~hit])
+    assert after[0][hit].isnan().all()
+    if where == "q":
+        assert torch.equal(o[at + 1:], ref[at + 1:]) and torch.equal(st, rst)
+    else:
+        assert after[:, hit].isnan().all()
+        s = st[c.slots[0]].cpu()
+        assert s[hit].isnan().all() and torch.equal(s[~hit], rst[c.slots[0]].cpu()[~hit])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,S", [(8, 1), (10, 1), (11, 1), (24, 8), (25, 8)])
+def test_rows_in_turn_and_chunks_at_the_rule_between_them(cuda, n, S):
+    """Row counts on either side of the one up to which the rows go one after another."""
+    c = Case(cuda, [n] * S, H=16 if S == 8 else 2, HV=32 if S == 8 else 4, V=128, seed=13)
+    c.check(*c.run(), *c.oracle())
+
+
+@pytest.mark.gpu
+def test_index_tensors_of_64_bits(cuda):
+    """int64 slots and bounds; a value past 32 bits is outside, not what its low half says; floats are refused."""
+    c = Case(cuda, [30, 4], seed=14)
+    ref, rst = c.oracle()
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    c.slots = c.slots.long()
+    o, st = c.run(status=status)
+    c.check(o, st, ref, rst)
+    assert status.item() == 0
+    c.slots[1] += 2 ** 32
+    o, st = c.run(status=status)
+    assert status.item() == 1 and o[30:].isnan().all() and not o[:30].isnan().any()
+    c.slots = c.slots.double()
+    with pytest.raises(ValueError, match="integers"):
+        c.run()
