@@ -27,6 +27,8 @@ def _check_cache(k_cache, v_cache, k_exp, v_exp, dtype):
     kind = k_cache.dtype
     if v_cache.shape != shape or v_cache.dtype != kind:
         raise ValueError("k_cache and v_cache must share one shape and type")
+    if not blocks * page * Hkv:
+        raise ValueError(f"a cache of shape {tuple(shape)} holds nothing")
     if D != 128 and D != 256 and D != 64:
         raise ValueError(f"head width {D} is not 64, 128 or 256")
     if kind == torch.float8_e4m3fn:
@@ -70,7 +72,7 @@ def kv_cache_write(key, value, k_cache, v_cache, slots, *, k_exp=None, v_exp=Non
 
     A negative slot is a padding row (skipped).  A slot past the cache is skipped and sets ``status`` (int32
     [1] on the device, zeroed by the caller), if given, to 1.  Slots of one call must differ: rows that share
-    one race, and either's elements may stay (a host tensor's are checked here)."""
+    one race, and what the slot then holds is undefined (a host tensor's are checked here)."""
     if key.dtype not in _TYPES or value.dtype != key.dtype or value.shape != key.shape:
         raise ValueError("key and value must be bf16 or fp16 tensors of one shape [T, Hkv, D]")
     blocks, page, Hkv, D, bs_k, bs_v = _check_cache(k_cache, v_cache, k_exp, v_exp, key.dtype)

@@ -316,3 +316,40 @@ def test_index_tensors_of_64_bits(cuda):
     c.slots = c.slots.double()
     with pytest.raises(ValueError, match="integers"):
         c.run()
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(cuda):
+    """Prefills on two streams together give what each gives alone (workspaces are the call's own)."""
+    cases = [Case(cuda, [300, 70], H=4, HV=8, V=128, seed=15 + i) for i in range(2)]
+    alone = [c.run() for c in cases]
+    args = []
+    for c in cases:
+        cu = torch.tensor(c.cu, dtype=torch.int32).to(cuda)
+        args.append([t.to(cuda) for t in (c.x, c.a, c.b, c.A, c.dt)] + [c.slots.to(cuda), cu])
+    states = [[c.state.to(cuda) for _ in range(6)] for c in cases]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in cases], [[], []]
+    for r in range(6):
+        for i, s in enumerate(streams):
+            x, a, b, A, dt, slots, cu = args[i]
+            with torch.cuda.stream(s):
+                got[i].append(gdn_prefill(x, a, b, A, dt, states[i][r], slots, cu, num_q_heads=4))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, alone[i][0]) for o in got[i]) and all(torch.equal(t, alone[i][1]) for t in states[i])
+
+
+@pytest.mark.gpu
+def test_many_sequences(cuda):
+    """As many sequences as a call takes, of 0 to 2 rows and one long one."""
+    g = torch.Generator().manual_seed(17)
+    for S, many in ((4096, 0), (500, 6000)):
+        news = torch.randint(0, 3, (S,), generator=g).tolist()
+        news[S // 2] += many
+        c = Case(cuda, news, H=1, HV=1, V=16, seed=18)
+        c.check(*c.run(), *c.oracle())
+    with pytest.raises(ValueError, match="4096"):
+        gdn_prefill(c.x.to(cuda), c.a.to(cuda), c.b.to(cuda), c.A.to(cuda), c.dt.to(cuda), c.state.to(cuda),
+                    torch.zeros(4097, dtype=torch.int32, device=cuda), torch.zeros(4098, dtype=torch.int32, device=cuda),
+                    num_q_heads=1)

@@ -456,3 +456,115 @@ def test_attention_mixed_batch_of_few_and_many_rows(cuda):
     c.check(*c.run())
     c = Case(cuda, FP, F8, [1] * 20 + [200], [30 + 7 * i for i in range(20)] + [250], 16, 4, 256, 64, seed=24)
     c.check(*c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("factor", [-1.0, 0.0, -30.0])
+@pytest.mark.parametrize("news,lens", [([1, 3], [600, 40]), ([70], [200])])
+def test_attention_of_negative_and_zero_scales(cuda, factor, news, lens):
+    """The largest score is the smallest product under a negative scale; under zero every visible token counts alike."""
+    c = Case(cuda, BF, BF, news, lens, 8, 2, 128, 16, seed=25)
+    c.scale *= factor
+    c.check(*c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("news,lens", [([1], [900]), ([1, 1, 1], [30, 200, 64]), ([5, 40], [333, 90])])
+def test_attention_of_many_heads_on_one(cuda, news, lens):
+    """64 query heads on one kv head: a token's rows are more than a tile of 16."""
+    for dtype, cache, D in ((BF, BF, 64), (FP, F8, 256)):
+        c = Case(cuda, dtype, cache, news, lens, 64, 1, D, 16, seed=26)
+        c.check(*c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S,many", [(70, 0), (70, 60), (5000, 0), (4200, 150)])
+def test_attention_of_many_sequences(cuda, S, many):
+    """More sequences than a wave has lanes, and than it has pairs of them: each row finds its own."""
+    g = torch.Generator().manual_seed(27)
+    news = torch.randint(0, 2, (S,), generator=g).tolist()
+    if many:
+        news[S // 3] = many
+    lens = [n + int(x) for n, x in zip(news, torch.randint(0, 40, (S,), generator=g))]
+    c = Case(cuda, BF, BF, news, [0] * S, 2, 1, 64, 8, seed=27)          # (the pages are filled here, in one call)
+    need = [-(-n // 8) for n in lens]
+    blocks = sum(need) + 1
+    c.k, c.v, _, _ = empty_cache(BF, blocks, 8, 1, 64, cuda)
+    perm, at, slots = torch.randperm(blocks, generator=g), 0, []
+    c.table = torch.full((S, max(need)), -1, dtype=torch.int32)
+    for s, n in enumerate(lens):
+        c.table[s, :need[s]] = perm[at:at + need[s]]
+        j = torch.arange(n)
+        slots.append(perm[at:at + need[s]][j // 8] * 8 + j % 8)
+        at += need[s]
+    k, v = (torch.randn(sum(lens), 1, 64, generator=g).to(BF) for _ in range(2))
+    kv_cache_write(k.to(cuda), v.to(cuda), c.k, c.v, torch.cat(slots).to(cuda))
+    c.ok, c.ov = ([to64(x) for x in t.split(lens)] for t in (k, v))
+    c.lens = lens
+    c.check(*c.run())
+
+
+@pytest.mark.gpu
+def test_bad_tables_and_values_in_a_split_call(cuda):
+    """As above where the tokens are cut into pieces: a bad block, length or value in one piece decides for the row."""
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    for news, lens in (([1, 1], [6000, 5000]), ([40, 1], [3000, 2000])):
+        c = Case(cuda, BF, BF, news, lens, 4, 2, 64, 16, seed=28)
+        n = news[0]
+        good = c.run(status=status)
+        assert status.item() == 0
+        table = c.table.clone()
+        table[0, 100] = 1 << 20
+        for kw in (dict(table=table), dict(lens=[c.table.shape[1] * 16 + 1, lens[1]])):
+            out, lse = c.run(status=status, **kw)
+            assert status.item() == 1 and out[:n].isnan().all() and lse[:, :n].isnan().all()
+            assert torch.equal(out[n:], good[0][n:]) and torch.equal(lse[:, n:], good[1][:, n:])
+            status.zero_()
+        c.v[int(c.table[0, 100]), 3, 1, 5] = float("nan")
+        out, lse = c.run(status=status)
+        hit = torch.zeros_like(out, dtype=torch.bool)
+        hit[:n, 2:, 5] = True
+        assert torch.equal(out.isnan(), hit) and torch.equal(out[~hit], good[0][~hit]) and torch.equal(lse, good[1])
+        assert status.item() == 0
+
+
+@pytest.mark.gpu
+def test_attention_over_an_empty_table(cuda):
+    """A table of no blocks: every row sees nothing; a length past it is refused."""
+    c = Case(cuda, BF, BF, [2, 30], [0, 0], 4, 2, 64, 16, seed=29)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    out, lse = c.run(table=c.table[:, :0], status=status)
+    assert (out == 0).all() and (lse == -float("inf")).all() and status.item() == 0
+    out, lse = c.run(table=c.table[:, :0], lens=[1, 0], status=status)
+    assert out[:2].isnan().all() and (out[2:] == 0).all() and status.item() == 1
+    for q, cu in ((c.q[:0], [0, 0, 0]), (c.q[:0], [0])):                  # no rows; no sequences
+        S = len(cu) - 1
+        out, lse = c.run(q=q, cu=cu, lens=[0] * S, table=c.table[:S])
+        assert out.shape == (0, 4, 64) and lse.shape == (4, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache", [BF, F8])
+@pytest.mark.parametrize("D,T", [(64, 33000), (256, 8301)])
+def test_many_rows_are_what_few_are(cuda, cache, D, T):
+    """Calls large enough for several rows a lane against the same rows in small calls, with padding among them."""
+    Hkv, page = 4, 16
+    g = torch.Generator().manual_seed(30)
+    key, value = (torch.randn(T, Hkv, D, generator=g).to(BF).to(cuda) for _ in range(2))
+    blocks = -(-T // page) + 3
+    slots = torch.randperm(blocks * page, generator=g)[:T].to(torch.int32)
+    slots[torch.randperm(T, generator=g)[:50]] = -1
+    slots = slots.to(cuda)
+    bits = lambda t: t.view(torch.uint8)  # noqa: E731
+    one, two = empty_cache(cache, blocks, page, Hkv, D, cuda), empty_cache(cache, blocks, page, Hkv, D, cuda)
+    kv_cache_write(key, value, one[0], one[1], slots, k_exp=one[2], v_exp=one[3])
+    for i in range(0, T, 3000):
+        kv_cache_write(key[i:i + 3000], value[i:i + 3000], two[0], two[1], slots[i:i + 3000], k_exp=two[2], v_exp=two[3])
+    assert all(torch.equal(bits(a), bits(b)) for a, b in zip(one, two) if a is not None)
+    whole = kv_cache_read(one[0], one[1], slots, k_exp=one[2], v_exp=one[3])
+    for i in range(0, T, 3000):
+        part = kv_cache_read(one[0], one[1], slots[i:i + 3000], k_exp=one[2], v_exp=one[3])
+        assert torch.equal(whole[0][i:i + 3000], part[0]) and torch.equal(whole[1][i:i + 3000], part[1])
+    if cache == BF:
+        used = slots >= 0
+        assert torch.equal(whole[0][used], key[used]) and (whole[0][~used] == 0).all()

@@ -176,3 +176,13 @@ def test_gdn_prefill_refuses_its_own_arguments():
                    (dict(initial=torch.zeros(2)), torch.tensor([0, 1, 3]))):
         with pytest.raises(ValueError):
             gdn_prefill(*call, cu, num_q_heads=1, **kw)
+
+
+@pytest.mark.parametrize("shape", [(0, 16, 2, 64), (4, 0, 2, 64), (4, 16, 0, 64)])
+def test_caches_that_hold_nothing_are_refused(shape):
+    k = torch.zeros(shape, dtype=BF)
+    with pytest.raises(ValueError, match="holds nothing"):
+        kv_cache_read(k, k, torch.arange(3))
+    with pytest.raises(ValueError, match="holds nothing"):
+        paged_attention(torch.zeros(3, 4, 64, dtype=BF), k, k, torch.zeros(2, 2, dtype=torch.int32),
+                        torch.zeros(2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), scale=1.0)
