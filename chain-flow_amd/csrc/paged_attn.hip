@@ -45,6 +45,7 @@ struct PagedArgs {
   int pshift;
   int T, H, Hkv, G, S, blocks, page, table_ld, max_blocks, causal;
   int piece, npiece, tiles;    // tokens a piece, pieces, row-tile slots
+  int spread;                  // on average at most one tile of k_attn_tiles a sequence
   int few;                     // rows (tokens * G) up to which a sequence is k_attn_rows' (0: none)
   int qsign;                   // of the scale: the sign goes into q, so that the scores' maximum scales
   float c;                     // |scale| log2(e)
@@ -91,11 +92,16 @@ template <int R, bool ROWS>
 __device__ __forceinline__ bool find_work(const PagedArgs& a, Work& w) {
   // (kv head, piece) groups and row tiles: consecutive workgroups go to the eight XCDs in turn, and each XCD
   // has its own L2, so a group's row tiles, which read the same tokens, are kept on one XCD (or an even share
-  // of the XCDs) where the group count allows
+  // of the XCDs) where the group count allows.  Where sequences have a tile each there is nothing to share, and
+  // with lengths that differ the late pieces are few: an odd stride spreads every group and every sequence over all
+  // XCDs (48 rows over 2,400 to 9,000 tokens, 2 kv heads, in 8 pieces: 61 us, 69 with a piece's rows on two XCDs)
   const int groups = a.Hkv * a.npiece;
   int g, t;
   const int b = blockIdx.x;
-  if (8 % groups == 0) {
+  if (ROWS || a.spread) {
+    g = b % (groups | 1);
+    t = b / (groups | 1);
+  } else if (8 % groups == 0) {
     const int per = 8 / groups, x = b % 8;
     g = x / per;
     t = b / 8 * per + x % per;
@@ -247,6 +253,9 @@ constexpr float LAZY = 8.f;   // log2 units the running maximum may lag behind (
 // row l % 32, and of every group of eight tokens the four with (t / 4) % 2 == l / 32.  Token tiles of TK go
 // global -> registers -> LDS one tile ahead (the 8-bit cache is widened on that way), double-buffered, one
 // barrier a tile.
+//   3,841 rows (16 / 4 heads of 256) over up to 9,001 tokens take 540 us: 755 TFLOP/s, 54% of a large matrix product's rate
+// (D = 128: 712).  Bound by the waves' own chain scores -> softmax -> products (MFMA busy 28% of the time, LDS 31%):
+// at D = 256 the accumulators leave room for two waves a SIMD, whose turns do not cover each other's exponentials.
 template <bool BF, bool F8, int D, int NW, int TK>
 __global__ void __launch_bounds__(NW * 64, 2) k_attn_tiles(PagedArgs a) {
   constexpr int R = NW * 32, NT = NW * 64;
@@ -471,8 +480,11 @@ __global__ void __launch_bounds__(NW * 64, 2) k_attn_tiles(PagedArgs a) {
 // Few rows: a tile of 16, one workgroup of four waves a (row tile, kv head, piece), each wave the tokens of
 // every fourth group of TG.  K goes from memory straight into the first operand's registers (16 tokens x
 // 64-byte segments a load), V through the wave's own rows of LDS for the transposed reads; both one group
-// ahead, 16 KB a wave (8 for D = 64 in 8 bits), with no branch around a load: behind one the compiler waits
-// for everything.  Waves do not wait for each other before the join of their (max, sum, O) at the end.
+// ahead, 16 KB a wave (an 8-bit cache: 8 at D = 64, else 16), with no branch around a load: behind one the compiler
+// waits for everything.  Waves do not wait for each other before the join of their (max, sum, O) at the end.
+//   Bound by memory latency: two workgroups a CU keep 128 KB in flight.  One row over 30,011 tokens (16 / 4 heads of
+// 256, 123 MB) 31 us, 4.0 TB/s, and the join 6 beside it; 48 rows over up to 9,000 (16 / 2 heads of 256) 132 us
+// together, 4.3 TB/s, and in 8 bits 99, where widening the elements shares the waves' time.
 template <bool BF>
 __device__ __forceinline__ f32x4 mfma16(const uint4& x, const uint4& y, f32x4 acc) {
   if constexpr (BF)
@@ -805,12 +817,15 @@ Plan plan(int T, int H, int Hkv, int D, int S, int max_len) {
   p.nrow = p.few ? S : (int)(packed / FEW_ROWS) + S;
   p.ntile = (int)(packed / tile_rows(D)) + S;
   // Pieces so that (row tiles) x (kv heads) x pieces fill the chip with the workgroups it holds at once, one a CU at
-  // D = 256 with many rows, else two; none from three quarters of a workgroup a CU on (244 of them, 3,841 rows over
-  // 9,001 tokens: cut in two 614 us, whole 551).  Pieces of 512 tokens at least where rows are few (one row over
-  // 30,011: 256 tokens 25 / 29 us at D = 64 / 128, 512 tokens 20 / 24), 256 where they are many.
+  // D = 256 with many rows, else two.  Many rows are left whole from three quarters of a workgroup a CU on (244 of
+  // them, 3,841 rows over 9,001 tokens: cut in two 614 us, whole 551); few rows are not (100 x 2 kv heads: whole 100
+  // us, in three 65; 64 x 4: 72, in two 55; 125 x 4: 129, in two 128).  More and shorter pieces of few rows lose
+  // again (48 x 2 kv heads, D = 128 in 8 bits: 3 pieces 65 us, 6 51, 8 61, 18 65).  Pieces of 512 tokens at least where
+  // rows are few (one row over 30,011: 256 tokens 25 / 29 us at D = 64 / 128, 512 tokens 20 / 24), 256 where they are
+  // many.
   const int fill = p.tiles && D == 256 ? 256 : 512, least = p.tiles ? 256 : 512;
   const long long items = (long long)Hkv * std::max<long long>(p.tiles ? (packed + tile_rows(D) - 1) / tile_rows(D) : S, std::min(S, T));
-  const long long want = items >= 192 ? 1 : (fill + items - 1) / items;
+  const long long want = p.tiles && items >= 192 ? 1 : (fill + items - 1) / items;
   long long piece = ((long long)max_len + want - 1) / want;
   piece = std::max<long long>(least, (piece + 63) / 64 * 64);
   p.npiece = (int)std::max(1ll, ((long long)max_len + piece - 1) / piece);
@@ -874,14 +889,16 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
   a.pmagic = (unsigned)((1ull << (31 + l)) / (unsigned)page + 1);
   hipStream_t st = (hipStream_t)stream;
   const long long groups = (long long)Hkv * p.npiece;
-  auto grid_of = [&](int tiles) {                 // (whole rounds of the XCD mapping)
+  a.spread = (long long)T * a.G <= (long long)tile_rows(D) * S;
+  auto grid_of = [&](int tiles, bool spread) {    // (whole rounds of the XCD mapping)
+    if (spread) return (groups | 1) * tiles;
     const long long per = 8 % groups == 0 ? 8 / groups : 1;
     return 8 % groups == 0 ? (tiles + per - 1) / per * 8 : groups * tiles;
   };
-  if (std::max(grid_of(p.nrow), grid_of(p.ntile)) > 0x7fffffffll) return CFH_E_UNSUPPORTED;
+  if (std::max(grid_of(p.nrow, true), grid_of(p.ntile, a.spread)) > 0x7fffffffll) return CFH_E_UNSUPPORTED;
   if (p.tiles) {
     a.tiles = p.ntile;
-    const dim3 grid((unsigned)grid_of(p.ntile));
+    const dim3 grid((unsigned)grid_of(p.ntile, a.spread));
     kv_dispatch(is_bf16, f8, D, [&](auto bf, auto e8, auto d) {
       constexpr int NW = tile_rows(d.value) / 32, TK = d.value == 256 ? 32 : 64;
       hipLaunchKernelGGL((k_attn_tiles<bf.value, e8.value, d.value, NW, TK>), grid, dim3(NW * 64), 0, st, a);
@@ -890,7 +907,7 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
   }
   if (p.rows) {
     a.tiles = p.nrow;
-    const dim3 grid((unsigned)grid_of(p.nrow));
+    const dim3 grid((unsigned)grid_of(p.nrow, true));
     kv_dispatch(is_bf16, f8, D, [&](auto bf, auto e8, auto d) {
       hipLaunchKernelGGL((k_attn_rows<bf.value, e8.value, d.value>), grid, dim3(256), 0, st, a);
     });
