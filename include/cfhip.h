@@ -492,12 +492,14 @@ int cfh_tree_greedy_accept(const void* logits, long long ld, int V, int n_rows, 
  * page Hkv D: the two may be views of one allocation), rows within a block contiguous.  With k_exp and
  * v_exp NULL the elements are 2-byte (bf16 or fp16: is_bf16); with both given they are e4m3, and byte
  * c = exp[blocks][page][Hkv], 1 to 254, is the scale 2^(c - 127) of its (slot, head).  Any page size; D in
- * {64, 128, 256}; blocks * page < 2^31.  Pointers 16-byte aligned, row strides multiples of 8 elements.
+ * {64, 128, 256}; blocks * page and page * Hkv * D < 2^31.  Pointers 16-byte aligned, row strides multiples of 8
+ * elements.  Limits past which a call returns "unsupported": T * Hkv (attention: T * H) < 2^30, max_blocks * page < 2^30,
+ * S <= 2^20.
  *
  * cfh_kv_write: rows key / value [T][Hkv][D] (row strides ld_k / ld_v, heads contiguous) into slots[T].
  * A negative slot is a padding row (skipped); one past the cache is skipped and sets status[0] to 1
- * (status: one int32 the caller zeroes, or NULL).  Two rows of one call in the same slot race: either's
- * elements may stay.  8-bit form: the scale is the least power of two, from 2^-126 up, that brings the
+ * (status: one int32 the caller zeroes, or NULL).  Two rows of one call in the same slot race: what it
+ * then holds is undefined.  8-bit form: the scale is the least power of two, from 2^-126 up, that brings the
  * row's largest finite magnitude to 448 or below; elements are x / scale rounded to nearest even (they end
  * at 240 where 256 times the scale exceeds the source type's largest value); NaN and infinities become
  * NaN. */
@@ -521,7 +523,8 @@ int cfh_kv_read(const void* k_cache, long long bs_k, const void* v_cache, long l
  * sequence are left as they were; a sequence whose bounds do not lie in [0, T] is skipped; one whose
  * length is negative or exceeds max_blocks * page, and rows that see a token of a block outside the cache,
  * give NaN; each of these sets status[0] to 1.  max_len: an upper bound of the lengths (it only plans how
- * the work is split).  ws: cfh_paged_attn_ws_bytes(...) bytes, 256-byte aligned (NULL where that is 0). */
+ * the work is split).  out may be q itself.  ws: cfh_paged_attn_ws_bytes(...) bytes of the same sizes and max_len,
+ * 256-byte aligned (NULL where that is 0), of the call's own until it ends. */
 int64_t cfh_paged_attn_ws_bytes(int T, int H, int Hkv, int D, int S, int max_len);
 int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, int is_bf16, const void* k_cache,
                    long long bs_k, const void* v_cache, long long bs_v, const uint8_t* k_exp, const uint8_t* v_exp,
@@ -534,7 +537,8 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
  * dt_bias, gates, normalisation, scale, ssm_state [nslots][HV][V][K] bf16 or fp32), each sequence from and
  * to its slot: S = exp(g) S; d = beta (v - S k); S += d k^T; o = S q.  The state is carried in fp32 and
  * rounded to the slot's type once, when the call ends; out [T][HV][V] bf16.  K == 128, V % 16 == 0,
- * S <= 4096.  Slot -1 is a padding sequence (nothing is read or written for it).  A slot outside the state
+ * S <= 4096, 2 H K + HV V <= 2^20.  A row that is not finite makes itself and its sequence's later rows and state NaN
+ * where it reaches (a NaN in v: its column), never an earlier row.  Slot -1 is a padding sequence (nothing is read or written for it).  A slot outside the state
  * or shared with another sequence of the call gives NaN rows, leaves the slot as it was and sets status[0]
  * to 1 (status: one int32 the caller zeroes, or NULL); checked on the device, so the calls never
  * synchronise and can be captured.
@@ -543,7 +547,8 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
  * cfh_gdn_prefill: sequence s has the rows cu_seqlens[s] .. cu_seqlens[s+1] (ascending) of mixed_qkv [T] (a sequence
  * whose bounds do not lie in [0, T] is skipped and sets status; one of no rows leaves its slot as it was;
  * rows of no sequence are left as they were).  initial [S] (or NULL: all 1): 0 = start from a zero state
- * instead of the slot's.  ws: cfh_gdn_prefill_ws_bytes(T, S, HV) bytes, 256-byte aligned. */
+ * instead of the slot's.  ws: cfh_gdn_prefill_ws_bytes(T, S, HV) bytes, 256-byte aligned (NULL where that is 0), of
+ * the call's own until it ends. */
 int cfh_gdn_decode(const void* mixed_qkv, const void* a, const void* b, const float* A_log, const float* dt_bias,
                    void* ssm_state, int state_bf16, int nslots, const int32_t* slots, int S, int H, int HV, int K,
                    int V, int use_l2norm, float scale, void* out, int32_t* status, void* stream);
