@@ -914,13 +914,19 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
     CFH_LAUNCH_CHECK();
   }
   if (p.npiece > 1) {
-    // up to 8 pieces a wave takes a (row, head) by itself, above that a workgroup of 16 (59 pieces of 16 rows and
-    // heads: 14 us with 4 waves)
-    const bool wide = p.npiece > 8;
-    const dim3 grid((unsigned)(wide ? (long long)T * H : ((long long)T * H + 3) / 4));
+    // Up to 8 pieces a wave takes a (row, head) by itself; above that a workgroup does, of 16 waves while there are few
+    // of them, else of 4 (the whole call, 16 / 4 waves a workgroup: 16 (row, head)s of 59 pieces 44.4 / 47.5 us, 192 of
+    // 18 27.4 / 29.1, 960 33.5 / 31.9, 1,712 of 16 48.5 / 42.9, 3,200 45.9 / 36.7; one wave: 63, 37, 37, 45, 37)
+    const long long rows = (long long)T * H;
     kv_dispatch(is_bf16, false, D, [&](auto bf, auto, auto d) {
-      if (wide) hipLaunchKernelGGL((k_attn_join<bf.value, d.value, 16>), grid, dim3(1024), 0, st, a);
-      else hipLaunchKernelGGL((k_attn_join<bf.value, d.value, 1>), grid, dim3(256), 0, st, a);
+      auto join = [&](auto w) {
+        constexpr int W = w.value;
+        const dim3 grid((unsigned)(W == 1 ? (rows + 3) / 4 : rows)), block(W == 1 ? 256 : W * 64);
+        hipLaunchKernelGGL((k_attn_join<bf.value, d.value, W>), grid, block, 0, st, a);
+      };
+      if (p.npiece <= 8) join(std::integral_constant<int, 1>{});
+      else if (rows <= 512) join(std::integral_constant<int, 16>{});
+      else join(std::integral_constant<int, 4>{});
     });
     CFH_LAUNCH_CHECK();
   }

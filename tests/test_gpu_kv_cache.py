@@ -568,3 +568,14 @@ def test_many_rows_are_what_few_are(cuda, cache, D, T):
     if cache == BF:
         used = slots >= 0
         assert torch.equal(whole[0][used], key[used]) and (whole[0][~used] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("new,length,H", [(40, 1300, 16), (2, 6000, 4), (40, 3000, 16), (37, 2900, 16)])
+def test_joins_of_few_and_many_pieces(cuda, D, new, length, H):
+    """Up to eight pieces of a row; more, of few rows and heads; more, of many: each joined by its own form."""
+    for dtype, cache in ((BF, BF), (FP, F8)):
+        c = Case(cuda, dtype, cache, [new, 1], [length, 40], H, 1, D, 16, seed=31)
+        c.check(*c.run())
+        c.check(*c.run(causal=False), causal=False)
