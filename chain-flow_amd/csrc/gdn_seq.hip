@@ -45,6 +45,9 @@ struct GdnSeqArgs {
   uint16_t* out;         // [T][HV][V] bf16
   int* status;
   int T, S, H, HV, V, ld, nslots, l2norm;
+  int few;               // k_gdn_rows takes the sequences of up to so many rows, the chunk kernels the others (0: all)
+  int step, plus;        // the chunks' places (chunk_start)
+  int nlong;             // sequences that k_gdn_chunks has workgroups for: all S, or as many as can have over `few` rows
   float scale;
 };
 
@@ -83,7 +86,7 @@ __global__ void __launch_bounds__(64) k_gdn_rows(GdnSeqArgs a) {
   const int t0 = a.cu ? a.cu[s] : s, t1 = a.cu ? a.cu[s + 1] : s + 1;
   const int ok = slot_verdict(a.slots, a.S, s, a.nslots);
   const bool rows = t0 >= 0 && t1 <= a.T && t0 <= t1;
-  if (ok == 0) return;
+  if (ok == 0 || (a.few && rows && t1 - t0 > a.few)) return;
   if (ok < 0 || !rows) {
     if (a.status && lane == 0) a.status[0] = 1;
     if (rows)
@@ -198,9 +201,10 @@ __device__ __forceinline__ void split4(const f32x4& x, uint2 (&p)[N]) {
   }
 }
 
-// Chunk slots: sequence s has those from floor(cu[s] / 64) + s on, ceil(n / 64) of them used, so no two
-// sequences share one.
-__device__ __forceinline__ int chunk_start(const int* cu, int s) { return cu[s] / GC + s; }
+// Chunk slots: a sequence in chunks, of n rows, uses the ceil(n / 64) from chunk_start on.  No two share one: with
+// floor(cu[s] / 64) + s sequences lie at least that many apart; with floor(cu[s] / (few + 1)), for few < 32, one of
+// more than `few` rows lies at least floor(n / (few + 1)) >= ceil(n / 64) before the next.
+__device__ __forceinline__ int chunk_start(const GdnSeqArgs& a, int s) { return a.cu[s] / a.step + a.plus * s; }
 
 // The order of a contraction over 32 k-slots, element e of lane group g: 16-row MFMA results (row 4 g + r of two
 // tiles, r = e % 4, tile e / 4) are operands as they stand.  The other operand follows it.
@@ -219,14 +223,14 @@ __global__ void __launch_bounds__(256) k_gdn_prep(GdnSeqArgs a, char* ws) {
   int s = 0, cnt = a.S;                            // the last sequence with chunk_start <= slot, 64 a step
   while (cnt > 1) {
     const int step = (cnt + 63) / 64, i = s + lane * step;
-    const unsigned long long m = __ballot(i < s + cnt && chunk_start(a.cu, i) <= slot);
+    const unsigned long long m = __ballot(i < s + cnt && chunk_start(a, i) <= slot);
     const int k = m ? 63 - __builtin_clzll(m) : 0;
     cnt = min(step, s + cnt - (s + k * step));
     s += k * step;
   }
   const int c0 = a.cu[s], c1 = a.cu[s + 1];
-  if (c0 < 0 || c0 > c1 || c1 > a.T) return;
-  const int chunk = slot - chunk_start(a.cu, s);
+  if (c0 < 0 || c0 > c1 || c1 > a.T || c1 - c0 <= a.few) return;
+  const int chunk = slot - chunk_start(a, s);
   if (chunk < 0 || chunk >= (c1 - c0 + GC - 1) / GC) return;
   const int t0 = c0 + chunk * GC, n = min(GC, c1 - t0);
   const int h = hv / (a.HV / a.H);
@@ -457,10 +461,26 @@ __global__ void __launch_bounds__(768) k_gdn_chunks(GdnSeqArgs a, const char* ws
   const int nsl = a.V / 16;
   // the column slices of a (sequence, value head) read the same chunks: on one XCD, whose L2 holds them
   const int pair = (blockIdx.x / 8 / nsl) * 8 + blockIdx.x % 8, sl = blockIdx.x / 8 % nsl;
-  if (pair >= a.S * a.HV) return;
-  const int s = pair / a.HV, hv = pair % a.HV;
+  if (pair >= a.nlong * a.HV) return;
+  int s = pair / a.HV;
+  const int hv = pair % a.HV;
+  if (a.nlong < a.S) {             // the s-th sequence in chunks, 64 a step
+    int skip = s, i = 0;
+    unsigned long long m = 0;
+    for (; i < a.S; i += 64) {
+      const int j = min(i + lane, a.S - 1), b0 = a.cu[j], b1 = a.cu[j + 1];
+      m = __ballot(i + lane < a.S && b0 >= 0 && b1 <= a.T && b1 - b0 > a.few);
+      const int n = __popcll(m);
+      if (skip < n) break;
+      skip -= n;
+    }
+    if (i >= a.S) return;
+    for (; skip; --skip) m &= m - 1;
+    s = i + __builtin_ctzll(m);
+  }
   const int c0 = a.cu[s], c1 = a.cu[s + 1];
   const bool rows = c0 >= 0 && c0 <= c1 && c1 <= a.T;
+  if (rows && a.few && c1 - c0 <= a.few) return;
   const int ok = slot_verdict(a.slots, a.S, s, a.nslots);
   if (ok == 0) return;
   if (ok < 0 || !rows) {
@@ -471,7 +491,7 @@ __global__ void __launch_bounds__(768) k_gdn_chunks(GdnSeqArgs a, const char* ws
   }
   if (c0 == c1) return;
   const int h = hv / (a.HV / a.H), nc = (c1 - c0 + GC - 1) / GC;
-  const char* const wb = ws + ((size_t)chunk_start(a.cu, s) * a.HV + hv) * GW_BYTES;
+  const char* const wb = ws + ((size_t)chunk_start(a, s) * a.HV + hv) * GW_BYTES;
   auto place = [&](int c) { return wb + (size_t)c * a.HV * GW_BYTES; };
   // (chunks past the last one: the last one again)
   auto rows_of = [&](int c) {      // the chunk's rows of mixed_qkv
@@ -739,16 +759,22 @@ __global__ void __launch_bounds__(768) k_gdn_chunks(GdnSeqArgs a, const char* ws
   }
 }
 
-// Whether the rows go one after another (k_gdn_rows): up to 8 a sequence on average, and 2 more for each round of
-// workgroups that k_gdn_chunks takes, one a CU (32 value heads of 128; one after another / in chunks: one sequence of
-// 8 rows 12.3 / 13.9 us, of 12 16.7 / 14.0; eight of 16 27.9 / 40.9, of 24 38.2 / 42.0, of 32 48.7 / 42.0).
-constexpr int GDN_ROWS_MAX = 8, GDN_CUS = 256;
-inline bool rows_in_turn(long long T, long long S, int HV, int V) {
+// The rows up to which a sequence goes one after another (k_gdn_rows): 8, and 1 more for each round of workgroups that
+// k_gdn_chunks takes, one a CU (32 value heads of 128, calls one after another / in chunks: one sequence of 8 rows 12.3 /
+// 13.9 us, of 12 16.7 / 14.0; eight of 12 42 / 45, of 16 53 / 49, of 24 74 / 50; 32 of 14 108 / 145, of 20 148 / 148).
+// Lengths are known on the device only, so with more than one sequence and rows enough for a long one both forms are
+// launched, each for its sequences: 63 single rows beside 500 76 us, 603 when one form served all of a call.  Launches
+// without a sequence of theirs cost 3 to 16 us (two of 12, eight of 16).
+constexpr int GDN_ROWS_MIN = 9, GDN_ROWS_MAX = 16, GDN_CUS = 256;
+static_assert(GDN_ROWS_MAX < 32, "chunk slots");
+inline int few_rows(long long S, int HV, int V) {
   const long long rounds = std::min((S * HV * (V / 16) + GDN_CUS - 1) / GDN_CUS, 8ll);
-  return T <= (GDN_ROWS_MAX + 2 * rounds) * S;
+  return 8 + (int)rounds;                          // GDN_ROWS_MIN to GDN_ROWS_MAX
 }
 
-inline long long chunk_slots(int T, int S) { return (long long)T / GC + S; }
+// Chunk slots for sequences of more than `few` rows.
+inline long long slots_by_chunks(int T, int S) { return (long long)T / GC + S; }
+inline long long slots_by_rows(int T, int few) { return T / (few + 1) + 1; }
 
 constexpr int GDN_SEQS = 4096;   // sequences a call (every wave looks for its slot among theirs)
 
@@ -793,7 +819,8 @@ int cfh_gdn_decode(const void* mixed_qkv, const void* a, const void* b, const fl
 
 int64_t cfh_gdn_prefill_ws_bytes(int T, int S, int HV) {
   if (T < 0 || S < 0 || HV < 1) return -1;
-  return (long long)T <= (long long)GDN_ROWS_MAX * S ? 0 : chunk_slots(T, S) * HV * GW_BYTES;
+  if (T <= GDN_ROWS_MIN || S == 0) return 0;
+  return std::min(slots_by_chunks(T, S), slots_by_rows(T, GDN_ROWS_MIN)) * HV * GW_BYTES;
 }
 
 int cfh_gdn_prefill(const void* mixed_qkv, const void* a, const void* b, const float* A_log, const float* dt_bias,
@@ -809,9 +836,19 @@ int cfh_gdn_prefill(const void* mixed_qkv, const void* a, const void* b, const f
   g.cu = cu_seqlens;
   g.initial = initial;
   hipStream_t st = (hipStream_t)stream;
-  if (rows_in_turn(T, S, HV, V)) return launch_rows(g, state_bf16, st);
+  const int few = few_rows(S, HV, V);
+  if (T <= few) return launch_rows(g, state_bf16, st);
   if (!ws || (uintptr_t)ws % 256) return CFH_E_INVALID;
-  const long long prep = chunk_slots(T, S) * HV, blocks = ((long long)S * HV + 7) / 8 * 8 * (V / 16);
+  if (S > 1) {
+    g.few = few;
+    if (int rc = launch_rows(g, state_bf16, st)) return rc;
+  }
+  const bool by_rows = slots_by_rows(T, few) < slots_by_chunks(T, S);
+  g.step = by_rows ? few + 1 : GC;
+  g.plus = by_rows ? 0 : 1;
+  g.nlong = S > 1 ? std::min(S, T / (few + 1)) : 1;
+  const long long prep = (by_rows ? slots_by_rows(T, few) : slots_by_chunks(T, S)) * HV;
+  const long long blocks = ((long long)g.nlong * HV + 7) / 8 * 8 * (V / 16);
   if (prep > 0x7fffffffll || blocks > 0x7fffffffll) return CFH_E_UNSUPPORTED;
   hipLaunchKernelGGL(k_gdn_prep, dim3((unsigned)prep), dim3(256), 0, st, g, (char*)ws);
   CFH_LAUNCH_CHECK();

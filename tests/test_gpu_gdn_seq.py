@@ -293,7 +293,7 @@ def test_a_row_that_is_not_finite_leaves_the_rows_before_it(cuda, where, at):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("n,S", [(8, 1), (10, 1), (11, 1), (24, 8), (25, 8)])
+@pytest.mark.parametrize("n,S", [(8, 1), (9, 1), (10, 1), (11, 1), (16, 8), (17, 8), (24, 8), (25, 8)])
 def test_rows_in_turn_and_chunks_at_the_rule_between_them(cuda, n, S):
     """Row counts on either side of the one up to which the rows go one after another."""
     c = Case(cuda, [n] * S, H=16 if S == 8 else 2, HV=32 if S == 8 else 4, V=128, seed=13)
@@ -353,3 +353,42 @@ def test_many_sequences(cuda):
         gdn_prefill(c.x.to(cuda), c.a.to(cuda), c.b.to(cuda), c.A.to(cuda), c.dt.to(cuda), c.state.to(cuda),
                     torch.zeros(4097, dtype=torch.int32, device=cuda), torch.zeros(4098, dtype=torch.int32, device=cuda),
                     num_q_heads=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("state", [torch.float32, BF])
+@pytest.mark.parametrize("news", [[1] * 63 + [300], [200] + [1] * 40 + [65, 10, 11], [3, 64, 0, 1, 129, 24, 25, 2], [11, 10, 12] * 7])
+def test_short_and_long_sequences_in_one_call(cuda, news, state):
+    """Each sequence by the form for its own length, whatever the others': decode rows beside prompts; with a padding
+    entry, a foreign slot and a shared one of either length, and rows of no sequence."""
+    c = Case(cuda, news, state=state, seed=19)
+    ref, rst = c.oracle()
+    c.check(*c.run(), ref, rst)
+    long, short = int(np.argmax(news)), int(np.argmin([n or 99 for n in news]))
+    for s in (long, short):
+        for bad in (-1, len(news) + 3):
+            keep = c.slots.clone()
+            c.slots[s] = bad
+            status = torch.zeros(1, dtype=torch.int32, device=cuda)
+            out = torch.full((sum(news), c.A.shape[0], 64), 7.0, dtype=BF, device=cuda)
+            o, st = c.run(status=status, out=out)
+            at = slice(c.cu[s], c.cu[s + 1])
+            assert status.item() == (bad != -1)
+            assert (o[at] == 7).all() if bad == -1 else o[at].isnan().all()
+            assert torch.equal(st[keep[s]].cpu(), c.state[keep[s]])
+            rows = torch.ones(sum(news), dtype=torch.bool)
+            rows[at] = False
+            assert rel_err(to64(o.cpu()[rows]), ref[rows.numpy()]) < TOL[BF]
+            c.slots = keep
+
+
+@pytest.mark.gpu
+def test_bounds_with_one_sequence_of_no_rows(cuda):
+    """One sequence that has no rows of a query that has: nothing but the status of its slot."""
+    c = Case(cuda, [90], seed=20)
+    for slot, want in ((0, 0), (9, 1), (-1, 0)):
+        c.slots = torch.tensor([slot], dtype=torch.int32)
+        status = torch.zeros(1, dtype=torch.int32, device=cuda)
+        out = torch.full((90, 4, 64), 7.0, dtype=BF, device=cuda)
+        o, st = c.run(status=status, out=out, cu=[40, 40])
+        assert status.item() == want and (o == 7).all() and torch.equal(st.cpu(), c.state)

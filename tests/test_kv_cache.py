@@ -186,3 +186,26 @@ def test_caches_that_hold_nothing_are_refused(shape):
     with pytest.raises(ValueError, match="holds nothing"):
         paged_attention(torch.zeros(3, 4, 64, dtype=BF), k, k, torch.zeros(2, 2, dtype=torch.int32),
                         torch.zeros(2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), scale=1.0)
+
+
+def test_gdn_prefill_workspace_covers_every_split():
+    """The chunks of sequences of more than `few` rows, at the places either rule gives them, fit the workspace and do
+    not overlap; decode-like calls of many sequences need no more than their rows do."""
+    rng = np.random.default_rng(0)
+    per = _lib.lib().cfh_gdn_prefill_ws_bytes(64, 1, 1) // 2
+    for _ in range(300):
+        few = int(rng.integers(9, 17))
+        news = rng.choice([0, 1, few, few + 1, 63, 64, 65, 128, 129, 500], size=int(rng.integers(1, 40)))
+        cu = np.concatenate([[int(rng.integers(0, 3))], news]).cumsum()
+        T, S = int(cu[-1] + rng.integers(0, 3)), len(news)
+        slots = _lib.lib().cfh_gdn_prefill_ws_bytes(T, S, 1) // per
+        by_rows = T // (few + 1) + 1 < T // 64 + S
+        used = []
+        for s, n in enumerate(news):
+            start = cu[s] // (few + 1) if by_rows else cu[s] // 64 + s
+            if n > few:
+                used += range(start, start + -(-int(n) // 64))
+        assert len(set(used)) == len(used)
+        if T > few:
+            assert max(used, default=0) < slots
+    assert _lib.lib().cfh_gdn_prefill_ws_bytes(4096, 4096, 1) // per <= 4096 // 10 + 1
