@@ -61,7 +61,8 @@ __device__ __forceinline__ int page_of(const PagedArgs& a, int j) { return (int)
 template <int R>
 __device__ __forceinline__ bool find_tile(const PagedArgs& a, int slot, int& s, int& tile) {
   const int lane = threadIdx.x & 63;
-  auto start = [&](int i) { return (int)(((long long)a.cu[i] * a.G) / R) + i; };   // (of bounds past T: any value)
+  // (bounds outside the query as its ends: times G they would pass 32 bits, and start would no longer ascend)
+  auto start = [&](int i) { return min(max(a.cu[i], 0), a.T) * a.G / R + i; };
   int lo = 0, n = a.S;                       // the last i in [lo, lo + n) with start(i) <= slot
   while (n > 1) {
     const int step = (n + 63) / 64, i = lo + lane * step;
