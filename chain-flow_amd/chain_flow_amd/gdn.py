@@ -150,7 +150,8 @@ def gdn_prefill(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, cu_seqlens, *
     (from zero where ``initial`` [S] bool is given and false) and leaves its state there, rounded to the
     slot's type once.  Layout, gates and slots as in ``gdn_decode``; the state a draft tree's roots start
     from (``tree_gdn_vllm``'s prefix slot).  -> o [T, HV, V] bf16.  ``cfh_gdn_prefill``, no host
-    synchronisation; rows of no sequence stay as they were in ``out``."""
+    synchronisation; rows of no sequence stay as they were in ``out``.  A sequence whose bounds do not lie in [0, T] is
+    skipped, and where a bound falls below the one before it that sequence and all behind it are; ``status`` is set."""
     H = int(num_q_heads)
     x, a, b, A_log, dt_bias, slots, out, dev = _seq_args(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, H, out, status)
     S, T = slots.shape[0], x.shape[0]

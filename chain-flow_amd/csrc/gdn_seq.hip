@@ -28,6 +28,7 @@
 #include "cfh_gdn.h"
 #include "cfh_host.h"
 #include "cfh_kernels.h"
+#include "cfh_seq.h"
 #include "cfh_tr.h"
 
 namespace {
@@ -44,6 +45,8 @@ struct GdnSeqArgs {
   const uint8_t* initial;  // [S] or null: 0 = start from zero instead of the slot
   uint16_t* out;         // [T][HV][V] bf16
   int* status;
+  int* whole;            // the sequences before the first bound that falls (cfh_seq.h); null: one sequence
+  int known;             // by k_ascending; else k_gdn_rows sets it for the chunk kernels
   int T, S, H, HV, V, ld, nslots, l2norm;
   int few;               // k_gdn_rows takes the sequences of up to so many rows, the chunk kernels the others (0: all)
   int step, plus;        // the chunks' places (chunk_start)
@@ -84,8 +87,10 @@ __global__ void __launch_bounds__(64) k_gdn_rows(GdnSeqArgs a) {
   const int hv = u % a.HV, s = u / a.HV;
   const int lane = threadIdx.x, p = lane & 15, r0 = vs * 16 + (lane >> 4) * 4;
   const int t0 = a.cu ? a.cu[s] : s, t1 = a.cu ? a.cu[s + 1] : s + 1;
+  const int whole = !a.cu ? a.S : a.known ? *a.whole : ascending(a.cu, a.S);
+  if (a.whole && !a.known && blockIdx.x == 0 && lane == 0) *a.whole = whole;
   const int ok = slot_verdict(a.slots, a.S, s, a.nslots);
-  const bool rows = t0 >= 0 && t1 <= a.T && t0 <= t1;
+  const bool rows = s < whole && t0 >= 0 && t1 <= a.T && t0 <= t1;
   if (ok == 0 || (a.few && rows && t1 - t0 > a.few)) return;
   if (ok < 0 || !rows) {
     if (a.status && lane == 0) a.status[0] = 1;
@@ -180,6 +185,7 @@ constexpr int GC = 64;                             // rows a chunk
 // [row tile][k-step][part][lane] 16 B; then the rows' factors, fp32 [4][64], and e^G_C
 constexpr int GW_ATT = 4 * 2 * 2 * 64 * 16, GW_VEC = 2 * GW_ATT;
 constexpr int GW_BYTES = GW_VEC + 4 * GC * 4 + 256;
+constexpr int GW_WHOLE = GW_VEC + (4 * GC + 1) * 4;   // GdnSeqArgs::whole, in the first place's spare bytes
 
 constexpr float GDN_RANGE = 0x1.fep127f;           // the largest finite bf16
 
@@ -220,16 +226,10 @@ __global__ void __launch_bounds__(256) k_gdn_prep(GdnSeqArgs a, char* ws) {
   __shared__ double Gs[GC];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, tl = lane & 15;
   const int slot = blockIdx.x / a.HV, hv = blockIdx.x % a.HV;
-  int s = 0, cnt = a.S;                            // the last sequence with chunk_start <= slot, 64 a step
-  while (cnt > 1) {
-    const int step = (cnt + 63) / 64, i = s + lane * step;
-    const unsigned long long m = __ballot(i < s + cnt && chunk_start(a, i) <= slot);
-    const int k = m ? 63 - __builtin_clzll(m) : 0;
-    cnt = min(step, s + cnt - (s + k * step));
-    s += k * step;
-  }
+  const int whole = a.whole ? *a.whole : a.S;
+  const int s = last_where(whole, [&](int i) { return chunk_start(a, i) <= slot; });
   const int c0 = a.cu[s], c1 = a.cu[s + 1];
-  if (c0 < 0 || c0 > c1 || c1 > a.T || c1 - c0 <= a.few) return;
+  if (s >= whole || c0 < 0 || c0 > c1 || c1 > a.T || c1 - c0 <= a.few) return;
   const int chunk = slot - chunk_start(a, s);
   if (chunk < 0 || chunk >= (c1 - c0 + GC - 1) / GC) return;
   const int t0 = c0 + chunk * GC, n = min(GC, c1 - t0);
@@ -463,23 +463,23 @@ __global__ void __launch_bounds__(768) k_gdn_chunks(GdnSeqArgs a, const char* ws
   const int pair = (blockIdx.x / 8 / nsl) * 8 + blockIdx.x % 8, sl = blockIdx.x / 8 % nsl;
   if (pair >= a.nlong * a.HV) return;
   int s = pair / a.HV;
-  const int hv = pair % a.HV;
+  const int hv = pair % a.HV, whole = a.whole ? *a.whole : a.S;
   if (a.nlong < a.S) {             // the s-th sequence in chunks, 64 a step
     int skip = s, i = 0;
     unsigned long long m = 0;
-    for (; i < a.S; i += 64) {
-      const int j = min(i + lane, a.S - 1), b0 = a.cu[j], b1 = a.cu[j + 1];
-      m = __ballot(i + lane < a.S && b0 >= 0 && b1 <= a.T && b1 - b0 > a.few);
+    for (; i < whole; i += 64) {
+      const int j = min(i + lane, whole - 1), b0 = a.cu[j], b1 = a.cu[j + 1];
+      m = __ballot(i + lane < whole && b0 >= 0 && b1 <= a.T && b1 - b0 > a.few);
       const int n = __popcll(m);
       if (skip < n) break;
       skip -= n;
     }
-    if (i >= a.S) return;
+    if (i >= whole) return;
     for (; skip; --skip) m &= m - 1;
     s = i + __builtin_ctzll(m);
   }
   const int c0 = a.cu[s], c1 = a.cu[s + 1];
-  const bool rows = c0 >= 0 && c0 <= c1 && c1 <= a.T;
+  const bool rows = s < whole && c0 >= 0 && c0 <= c1 && c1 <= a.T;
   if (rows && a.few && c1 - c0 <= a.few) return;
   const int ok = slot_verdict(a.slots, a.S, s, a.nslots);
   if (ok == 0) return;
@@ -841,6 +841,12 @@ int cfh_gdn_prefill(const void* mixed_qkv, const void* a, const void* b, const f
   if (!ws || (uintptr_t)ws % 256) return CFH_E_INVALID;
   if (S > 1) {
     g.few = few;
+    g.whole = (int*)((char*)ws + GW_WHOLE);
+    if (S > ASC_OWN) {
+      g.known = 1;
+      hipLaunchKernelGGL(k_ascending, dim3(1), dim3(1024), 0, st, cu_seqlens, S, g.whole);
+      CFH_LAUNCH_CHECK();
+    }
     if (int rc = launch_rows(g, state_bf16, st)) return rc;
   }
   const bool by_rows = slots_by_rows(T, few) < slots_by_chunks(T, S);

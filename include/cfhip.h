@@ -545,8 +545,8 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
  *
  * cfh_gdn_decode: one token a sequence, row s of mixed_qkv [S].
  * cfh_gdn_prefill: sequence s has the rows cu_seqlens[s] .. cu_seqlens[s+1] (ascending) of mixed_qkv [T] (a sequence
- * whose bounds do not lie in [0, T] is skipped and sets status; one of no rows leaves its slot as it was;
- * rows of no sequence are left as they were).  initial [S] (or NULL: all 1): 0 = start from a zero state
+ * whose bounds do not lie in [0, T] is skipped and sets status; where a bound falls below the one before it, that
+ * sequence and all behind it are; one of no rows leaves its slot as it was; rows of no sequence are left as they were).  initial [S] (or NULL: all 1): 0 = start from a zero state
  * instead of the slot's.  ws: cfh_gdn_prefill_ws_bytes(T, S, HV) bytes, 256-byte aligned (NULL where that is 0), of
  * the call's own until it ends. */
 int cfh_gdn_decode(const void* mixed_qkv, const void* a, const void* b, const float* A_log, const float* dt_bias,

@@ -1,4 +1,4 @@
-"""Edges of the committed prefix's calls on the GPU: saturated bounds."""
+"""Edges of the committed prefix's calls on the GPU: saturated bounds, bounds that fall."""
 from __future__ import annotations
 
 import numpy as np
@@ -6,9 +6,18 @@ import pytest
 import torch
 
 from chain_flow_amd.kv_cache import paged_attention
-from conftest import to64
+from conftest import rel_err, to64
 from oracle import kv_cache as okv
+from test_gpu_gdn_seq import TOL
+from test_gpu_gdn_seq import Case as GdnCase
 from test_gpu_kv_cache import BF, Case, close
+
+
+def poison(cuda, *nbytes):
+    """NaNs in the blocks that the allocator hands out next."""
+    held = [torch.full((max(n, 1),), 0xFF, dtype=torch.uint8, device=cuda) for n in nbytes]
+    torch.cuda.synchronize()
+    del held
 
 
 def check_first(c, out, lse, S, causal=True):
@@ -33,3 +42,40 @@ def test_attention_bounds_past_32_bits_skip_their_sequences_only(cuda, H, bounds
     o, lse = paged_attention(c.q, c.k, c.v, i32(c.table), i32(c.lens), torch.tensor(bounds), scale=c.scale, out=out, status=status)
     assert status.item() == 1 and (o[bounds[good]:] == 7).all()
     check_first(c, o, lse, good)
+
+
+# ---------------------------------------------------------------- bounds that fall
+FALLS = [
+    # news, bounds, sequences before the fall
+    ([100, 50, 50], [0, 100, -1000, 200], 1),
+    ([100, 50, 50], [0, 100, 60, 200], 1),
+    ([3, 2, 3], [0, 3, -7, 8], 1),
+    ([60, 1, 1, 90, 4], [0, 60, 61, 62, 20, 156], 3),
+    ([40, 30, 20], [0, 40, 70, -1], 2),
+    ([40, 30], [40, 0, 70], 0),
+    ([1] * 100 + [50], [*range(90), 3, *range(91, 101), 150], 89),
+    ([1] * 600 + [50], [*range(401), 3, *range(402, 601), 650], 400),
+    ([0] * 700 + [30] + [1] * 300, [0] * 701 + [30 + i for i in range(200)] + [1 + i for i in range(101)], 900),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("state", [torch.float32, BF])
+@pytest.mark.parametrize("news,bounds,good", FALLS)
+def test_prefill_stops_where_the_bounds_fall(cuda, news, bounds, good, state):
+    """The sequences before the first bound that falls below the one before it, and their slots, are what they are by
+    themselves; from it on sequences are skipped, their rows and slots left as they were, and the status word is set."""
+    c = GdnCase(cuda, news, state=state, seed=3)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    out = torch.full((sum(news), 4, 64), 7.0, dtype=BF, device=cuda)
+    poison(cuda, 1 << 24)
+    print(f"[prefill falls] {len(news)} sequences, {good} before it", flush=True)
+    o, st = c.run(out=out, status=status, cu=bounds)
+    assert status.item() == 1 and (o[bounds[good] if good else 0:] == 7).all()
+    others = np.setdiff1d(np.arange(len(news) + 3), c.slots.numpy()[:good])
+    assert torch.equal(st.cpu()[others], c.state[others])
+    if good:
+        c.cu, c.slots = c.cu[:good + 1], c.slots[:good]
+        ref, rst = c.oracle()
+        T = bounds[good]
+        assert rel_err(to64(o[:T]), ref[:T]) < TOL[BF] and rel_err(to64(st), rst) < TOL[state]
