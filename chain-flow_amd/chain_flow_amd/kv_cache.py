@@ -125,9 +125,10 @@ def paged_attention(query, k_cache, v_cache, block_table, seq_lens, cu_q, *, sca
 
     A row that sees no token gives 0 and -inf.  Rows of no sequence stay as they were in ``out``.  Lengths, tables
     and bounds are read on the device only: a negative length or one past the table, and rows that see a token of
-    a block outside the cache, give NaN; a sequence whose rows do not lie in the query is skipped; each sets
-    ``status`` (int32 [1], zeroed by the caller), if given, to 1.  ``max_len``: an upper bound of the lengths
-    (default: what the table holds); it only plans how the work is split."""
+    a block outside the cache, give NaN; a sequence whose rows do not lie in the query is skipped, and where a bound
+    falls below the one before it that sequence and all behind it are; each sets ``status`` (int32 [1], zeroed by
+    the caller), if given, to 1.  ``max_len``: an upper bound of the lengths (default: what the table holds); it only
+    plans how the work is split."""
     if query.dtype not in _TYPES:
         raise ValueError("query must be bf16 or fp16")
     blocks, page, Hkv, D, bs_k, bs_v = _check_cache(k_cache, v_cache, k_exp, v_exp, query.dtype)

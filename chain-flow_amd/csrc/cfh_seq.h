@@ -60,4 +60,43 @@ __global__ void __launch_bounds__(1024) k_ascending(const int* cu, int S, int* w
   }
 }
 
+// The last sequence i with pred(i, cu[i]) of those before the first bound that falls, and its bounds; s = -1 where there
+// is none.  pred holds up to some i and not behind it.  `whole`: k_ascending's count, or null: the bounds are looked over
+// on the way, 64 U of them at a time, which needs no load behind the first where one place holds them all.
+struct Seq { int s, c0, c1; };
+template <int U, typename F>
+__device__ __forceinline__ Seq find_looking(const int* cu, int S, F pred) {
+  const int lane = threadIdx.x & 63;
+  Seq f = {-1, 0, 0};
+  for (int b = 0; b < S; b += 64 * U) {
+    int x[U], y[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = min(b + 64 * u + lane, S - 1);
+      x[u] = cu[i];
+      y[u] = cu[i + 1];
+    }
+    bool on = true;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = b + 64 * u + lane;
+      const unsigned long long in = __ballot(i < S && pred(i, x[u])), fall = __ballot(x[u] > y[u]);
+      const unsigned long long m = on ? in & (fall ? (fall & -fall) - 1 : ~0ull) : 0;
+      if (m) {
+        const int k = 63 - __builtin_clzll(m);
+        f = {b + 64 * u + k, __builtin_amdgcn_readlane(x[u], k), __builtin_amdgcn_readlane(y[u], k)};
+      }
+      on = m == ~0ull;
+    }
+    if (!on) break;
+  }
+  return f;
+}
+template <typename F>
+__device__ __forceinline__ Seq find_seq(const int* cu, int S, const int* whole, F pred) {
+  if (!whole) return S <= 64 ? find_looking<1>(cu, S, pred) : find_looking<4>(cu, S, pred);
+  const int n = *whole, s = last_where(n, [&](int i) { return pred(i, cu[i]); });
+  return {s < n ? s : -1, cu[s], cu[s + 1]};
+}
+
 }  // namespace

@@ -20,6 +20,7 @@
 #include "cfh_host.h"
 #include "cfh_kernels.h"
 #include "cfh_kv.h"
+#include "cfh_seq.h"
 #include "cfh_tr.h"
 
 namespace {
@@ -37,6 +38,7 @@ struct PagedArgs {
   const int* table;            // [S][table_ld]
   const int* lens;             // [S]
   const int* cu;               // [S + 1]
+  const int* whole;            // the sequences before the first bound that falls, by k_ascending (null: look)
   int* status;
   float* po;                   // pieces' O [npiece][T][H][D] (npiece > 1)
   float2* pml;                 // pieces' (max in log2 units, sum) [npiece][T][H]
@@ -55,27 +57,6 @@ struct PagedArgs {
 __device__ __forceinline__ bool bounds_ok(const PagedArgs& a, int c0, int c1) { return c0 >= 0 && c0 <= c1 && c1 <= a.T; }
 
 __device__ __forceinline__ int page_of(const PagedArgs& a, int j) { return (int)(__umulhi((unsigned)j << 1, a.pmagic) >> a.pshift); }
-
-// Row-tile slot -> (sequence, tile): sequence s has the slots from floor(cu[s] G / R) + s on, at most
-// ceil(n G / R) of them used, so no two sequences share one.  A search over 64 sequences a step.
-template <int R>
-__device__ __forceinline__ bool find_tile(const PagedArgs& a, int slot, int& s, int& tile) {
-  const int lane = threadIdx.x & 63;
-  // (bounds outside the query as its ends: times G they would pass 32 bits, and start would no longer ascend)
-  auto start = [&](int i) { return min(max(a.cu[i], 0), a.T) * a.G / R + i; };
-  int lo = 0, n = a.S;                       // the last i in [lo, lo + n) with start(i) <= slot
-  while (n > 1) {
-    const int step = (n + 63) / 64, i = lo + lane * step;
-    const bool le = i < lo + n && start(i) <= slot;
-    const unsigned long long m = __ballot(le);
-    const int k = m ? 63 - __builtin_clzll(m) : 0;
-    n = min(step, lo + n - (lo + k * step));
-    lo += k * step;
-  }
-  s = lo;
-  tile = slot - start(lo);
-  return tile >= 0;
-}
 
 // What one workgroup works on: rows [r0, r0 + R) of the n * G packed rows of sequence s and kv head hk, and
 // the tokens [j0, j1) of one piece.
@@ -116,11 +97,17 @@ __device__ __forceinline__ bool find_work(const PagedArgs& a, Work& w) {
   if (g >= groups || t >= a.tiles) return false;
   w.hk = g % a.Hkv;
   w.piece = g / a.Hkv;
-  int tile = 0;
-  if (ROWS && a.few) w.s = t;      // (beside k_attn_tiles: one tile of a.few rows a sequence)
-  else if (!find_tile<R>(a, a.tiles - 1 - t, w.s, tile)) return false;   // (late rows see the most: first)
-  w.c0 = a.cu[w.s];
-  const int c1 = a.cu[w.s + 1];
+  // Row-tile slot -> (sequence, tile): sequence s has the slots from floor(cu[s] G / R) + s on, at most
+  // ceil(n G / R) of them used, so no two sequences share one.  (Bounds outside the query as its ends: times G they would
+  // pass 32 bits, and start would no longer ascend.)  Beside k_attn_tiles: one tile of a.few rows a sequence
+  const bool own = ROWS && a.few;
+  const int slot = own ? t : a.tiles - 1 - t;      // (late rows see the most: first)
+  auto start = [&](int i, int c) { return own ? i : min(max(c, 0), a.T) * a.G / R + i; };
+  const Seq f = find_seq(a.cu, a.S, a.whole, [&](int i, int c) { return start(i, c) <= slot; });
+  const int tile = slot - start(f.s, f.c0), c1 = f.c1;
+  if (f.s < 0 || tile < 0 || (own && tile)) return false;
+  w.s = f.s;
+  w.c0 = f.c0;
   if (!bounds_ok(a, w.c0, c1)) return false;
   w.n = c1 - w.c0;
   if (ROWS ? (a.few && (long long)w.n * a.G > a.few) : (long long)w.n * a.G <= a.few) return false;
@@ -725,16 +712,9 @@ __global__ void __launch_bounds__(W == 1 ? 256 : W * 64) k_attn_join(PagedArgs a
   const int at = W == 1 ? blockIdx.x * 4 + wave : blockIdx.x, part = W == 1 ? 0 : wave;
   const int t = at / a.H, h = at % a.H;
   if (t >= a.T) return;
-  int s = 0, n = a.S;                             // the last sequence with cu[s] <= t (64 a step)
-  while (n > 1) {
-    const int step = (n + 63) / 64, i = s + lane * step;
-    const unsigned long long mk = __ballot(i < s + n && a.cu[i] <= t);
-    const int k = mk ? 63 - __builtin_clzll(mk) : 0;
-    n = min(step, s + n - (s + k * step));
-    s += k * step;
-  }
-  const int c0 = a.cu[s], c1 = a.cu[s + 1];
-  if (t < c0 || t >= c1 || !bounds_ok(a, c0, c1)) return;   // a row of no sequence
+  const Seq f = find_seq(a.cu, a.S, a.whole, [&](int, int c) { return c <= t; });
+  const int s = f.s, c0 = f.c0, c1 = f.c1;
+  if (s < 0 || t < c0 || t >= c1 || !bounds_ok(a, c0, c1)) return;   // a row of no sequence
   int len = a.lens[s];
   if (len < 0 || len > (long long)a.max_blocks * a.page) len = 0;
   // the row's pieces: those that start below what it sees, and the first always
@@ -834,7 +814,21 @@ Plan plan(int T, int H, int Hkv, int D, int S, int max_len) {
   return p;
 }
 
-int64_t po_bytes(const Plan& p, int T, int H, int D) { return cfh::align256((size_t)p.npiece * T * H * D * sizeof(float)); }
+// Sequences up to which every workgroup looks over the bounds on its way to its sequence; k_ascending before the others
+// for more (300 of 500 tokens 51.9 us so and 55.4 with k_ascending, 1,000 of 300 tokens 119 and 115, 110 unchecked).
+constexpr int ASC_FIND = 512;
+
+// The workspace: the pieces' O, their (max, sum), and the count of sequences where k_ascending makes it.
+struct Space { int64_t pml, whole, all; };
+Space space(const Plan& p, int T, int H, int D, int S) {
+  Space w = {};
+  if (p.npiece > 1) {
+    w.pml = cfh::align256((size_t)p.npiece * T * H * D * sizeof(float));
+    w.whole = w.pml + cfh::align256((size_t)p.npiece * T * H * sizeof(float2));
+  }
+  w.all = w.whole + (S > ASC_FIND ? 256 : 0);
+  return w;
+}
 
 }  // namespace
 
@@ -843,9 +837,7 @@ extern "C" {
 int64_t cfh_paged_attn_ws_bytes(int T, int H, int Hkv, int D, int S, int max_len) {
   if (T < 0 || H < 1 || Hkv < 1 || H % Hkv || S < 0 || max_len < 0 || D < 1) return -1;
   if (T == 0 || S == 0) return 0;
-  const Plan p = plan(T, H, Hkv, D, S, max_len);
-  if (p.npiece == 1) return 0;
-  return po_bytes(p, T, H, D) + (int64_t)cfh::align256((size_t)p.npiece * T * H * sizeof(float2));
+  return space(plan(T, H, Hkv, D, S, max_len), T, H, D, S).all;
 }
 
 int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, int is_bf16, const void* k_cache,
@@ -871,7 +863,8 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
       o_ld < (long long)H * D || q_ld % 8 || o_ld % 8 || ((uintptr_t)q | (uintptr_t)out) % 16)
     return CFH_E_INVALID;
   const Plan p = plan(T, H, Hkv, D, S, max_len);
-  if (p.npiece > 1 && (!ws || (uintptr_t)ws % 256)) return CFH_E_INVALID;
+  const Space w = space(p, T, H, D, S);
+  if (w.all && (!ws || (uintptr_t)ws % 256)) return CFH_E_INVALID;
   PagedArgs a = {};
   a.q = (const u16*)q; a.out = (u16*)out; a.lse = lse; a.kc = k_cache; a.vc = v_cache; a.ke = k_exp; a.ve = v_exp;
   a.table = table; a.lens = seq_lens; a.cu = cu_q; a.status = status; a.q_ld = q_ld; a.o_ld = o_ld; a.bs_k = bs_k;
@@ -880,7 +873,7 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
   a.qsign = scale > 0.f ? 1 : scale < 0.f ? -1 : 0;
   a.c = scale == 0.f ? 1.f : fabsf(scale) * 1.44269504088896340736f;
   a.po = (float*)ws;
-  a.pml = (float2*)((char*)ws + (p.npiece > 1 ? po_bytes(p, T, H, D) : 0));
+  a.pml = (float2*)((char*)ws + w.pml);
   a.piece = p.piece; a.npiece = p.npiece; a.few = p.few;
   // j / page for j < 2^30 as j M >> (31 + l), 2^l >= page > 2^(l - 1), M = floor(2^(31 + l) / page) + 1 < 2^32: M is
   // above 2^(31 + l) / page by at most 1, which adds less than 2^30 / 2^(31 + l) < 1 / page to the quotient
@@ -897,6 +890,11 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
     return 8 % groups == 0 ? (tiles + per - 1) / per * 8 : groups * tiles;
   };
   if (std::max(grid_of(p.nrow, true), grid_of(p.ntile, a.spread)) > 0x7fffffffll) return CFH_E_UNSUPPORTED;
+  if (S > ASC_FIND) {
+    a.whole = (int*)((char*)ws + w.whole);
+    hipLaunchKernelGGL(k_ascending, dim3(1), dim3(1024), 0, st, cu_q, S, (int*)((char*)ws + w.whole));
+    CFH_LAUNCH_CHECK();
+  }
   if (p.tiles) {
     a.tiles = p.ntile;
     const dim3 grid((unsigned)grid_of(p.ntile, a.spread));

@@ -520,7 +520,8 @@ int cfh_kv_read(const void* k_cache, long long bs_k, const void* v_cache, long l
  * over kv head h / (H / Hkv); a row that sees nothing gives 0 and -inf.  causal = 0 with a draft tree's
  * nodes as rows gives the prefix_out / prefix_lse that cfh_tree_attn_merge takes.  Lengths, tables and
  * row bounds are read on the device only, so the call never synchronises and can be captured.  Rows of no
- * sequence are left as they were; a sequence whose bounds do not lie in [0, T] is skipped; one whose
+ * sequence are left as they were; a sequence whose bounds do not lie in [0, T] is skipped, and where a
+ * bound falls below the one before it that sequence and all behind it are; one whose
  * length is negative or exceeds max_blocks * page, and rows that see a token of a block outside the cache,
  * give NaN; each of these sets status[0] to 1.  max_len: an upper bound of the lengths (it only plans how
  * the work is split).  out may be q itself.  ws: cfh_paged_attn_ws_bytes(...) bytes of the same sizes and max_len,

@@ -27,6 +27,13 @@ def check_first(c, out, lse, S, causal=True):
     close(out[:T].contiguous(), lse[:, :T].contiguous(), *ref, max(c.lens[:S] + [1]), c.dtype)
 
 
+def wide(c, tokens):
+    """The case's table with room for `tokens` tokens a sequence: a call of that max_len is planned in pieces."""
+    table = torch.full((c.table.shape[0], max(c.table.shape[1], -(-tokens // c.page))), -1, dtype=torch.int32)
+    table[:, :c.table.shape[1]] = c.table
+    return table
+
+
 # ---------------------------------------------------------------- saturated bounds
 @pytest.mark.gpu
 @pytest.mark.parametrize("H,bounds", [(256, [0, 5, 2 ** 40, 2 ** 40]),                             # many rows a sequence
@@ -79,3 +86,22 @@ def test_prefill_stops_where_the_bounds_fall(cuda, news, bounds, good, state):
         ref, rst = c.oracle()
         T = bounds[good]
         assert rel_err(to64(o[:T]), ref[:T]) < TOL[BF] and rel_err(to64(st), rst) < TOL[state]
+
+
+# ---------------------------------------------------------------- attention where bounds fall
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [100, 3000])
+@pytest.mark.parametrize("news,bounds,good", FALLS)
+def test_attention_stops_where_the_bounds_fall(cuda, news, bounds, good, most):
+    """As the delta rule's.  Whole and in pieces."""
+    rng = np.random.default_rng(len(news))
+    lens = (np.asarray(news) + rng.integers(0, 30 if len(news) > 9 else 900, len(news))).tolist()
+    c = Case(cuda, BF, BF, news, lens, 4, 2, 64, 16, seed=2)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    out = torch.full_like(c.q, 7.0)
+    print(f"[attention falls] {len(news)} sequences, {good} before it", flush=True)
+    o, lse = c.run(cu=bounds, out=out, status=status, table=wide(c, most), max_len=most)
+    assert status.item() == 1 and (o[bounds[good] if good else 0:] == 7).all()
+    if good:
+        assert c.cu[:good + 1].tolist() == bounds[:good + 1]
+        check_first(c, o, lse, good)
