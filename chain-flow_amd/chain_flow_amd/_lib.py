@@ -103,6 +103,7 @@ SIGNATURES = {
     "cfh_gdn_prefill": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, C.c_float,
                              _VP, _VP, _VP, _VP]),
 }
+SIGNATURES.update({name + "_fresh": SIGNATURES[name] for name in ("cfh_gdn_decode", "cfh_gdn_prefill")})
 
 
 def lib():

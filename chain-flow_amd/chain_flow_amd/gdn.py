@@ -111,7 +111,7 @@ def _seq_args(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, H, out, status,
         raise ValueError("slots must be [S], S <= 4096")
     dev = _lib.device_of(mixed_qkv, a, b, A_log, dt_bias, ssm_state, status=status)
     if out is None:
-        out = mixed_qkv.new_empty((T, HV, V))
+        out = mixed_qkv.new_empty((T, HV, V)) if slots.shape[0] else mixed_qkv.new_zeros((T, HV, V))
     elif out.shape != (T, HV, V) or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.get_device() != dev:
         raise ValueError(f"out must be a contiguous bf16 [{T}, {HV}, {V}] tensor on cuda:{dev}")
     if A_log.dtype != torch.float32 or dt_bias.dtype != torch.float32:
@@ -127,16 +127,18 @@ def gdn_decode(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, *, num_q_heads
     dt_bias [HV], ssm_state [slots, HV, V, K] bf16 or fp32 (sequence s's slot slots[s] is updated in place).
     -> o [S, HV, V] bf16.  One launch of ``cfh_gdn_decode``, no host synchronisation.
 
-    Slot -1 marks a padding row: nothing is read or written for it (its row of ``out`` stays as it was).  A
+    Slot -1 marks a padding row: nothing is read or written for it (its row of ``out`` stays as it was, or is 0
+    without ``out``).  A
     slot outside ssm_state or shared by two rows gives NaN outputs, stays as it was, and sets ``status``
     (int32 [1] on the device, zeroed by the caller), if given, to 1."""
     H = int(num_q_heads)
     S = mixed_qkv.shape[0]
     if slots.shape != (S,):
         raise ValueError(f"slots must be [{S}]")
+    call = _lib.lib().cfh_gdn_decode_fresh if out is None else _lib.lib().cfh_gdn_decode
     x, a, b, A_log, dt_bias, slots, out, dev = _seq_args(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, H, out, status)
     nslots, HV, V, K = ssm_state.shape
-    _lib.check(_lib.lib().cfh_gdn_decode(
+    _lib.check(call(
         x.data_ptr(), a.data_ptr(), b.data_ptr(), A_log.data_ptr(), dt_bias.data_ptr(), ssm_state.data_ptr(),
         ssm_state.dtype == torch.bfloat16, nslots, slots.data_ptr(), S, H, HV, K, V, bool(use_qk_l2norm),
         float(K ** -0.5 if scale is None else scale), out.data_ptr(), _lib.ptr(status), _lib.stream_of(dev)), "cfh_gdn_decode")
@@ -150,9 +152,11 @@ def gdn_prefill(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, cu_seqlens, *
     (from zero where ``initial`` [S] bool is given and false) and leaves its state there, rounded to the
     slot's type once.  Layout, gates and slots as in ``gdn_decode``; the state a draft tree's roots start
     from (``tree_gdn_vllm``'s prefix slot).  -> o [T, HV, V] bf16.  ``cfh_gdn_prefill``, no host
-    synchronisation; rows of no sequence stay as they were in ``out``.  A sequence whose bounds do not lie in [0, T] is
+    synchronisation; rows of no sequence stay as they were in ``out``, and are 0 without it.  A sequence whose bounds do not lie in [0, T] is
     skipped, and where a bound falls below the one before it that sequence and all behind it are; ``status`` is set."""
     H = int(num_q_heads)
+    L = _lib.lib()
+    call = L.cfh_gdn_prefill_fresh if out is None else L.cfh_gdn_prefill
     x, a, b, A_log, dt_bias, slots, out, dev = _seq_args(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, H, out, status)
     S, T = slots.shape[0], x.shape[0]
     nslots, HV, V, K = ssm_state.shape
@@ -163,9 +167,8 @@ def gdn_prefill(mixed_qkv, a, b, A_log, dt_bias, ssm_state, slots, cu_seqlens, *
         if initial.shape != (S,) or initial.dtype not in (torch.bool, torch.uint8):
             raise ValueError(f"initial must be a bool [{S}] tensor")
         initial = initial.to(x.device).contiguous()
-    L = _lib.lib()
     ws = x.new_empty(L.cfh_gdn_prefill_ws_bytes(T, S, HV), dtype=torch.uint8)
-    _lib.check(L.cfh_gdn_prefill(
+    _lib.check(call(
         x.data_ptr(), a.data_ptr(), b.data_ptr(), A_log.data_ptr(), dt_bias.data_ptr(), ssm_state.data_ptr(),
         ssm_state.dtype == torch.bfloat16, nslots, slots.data_ptr(), cu.data_ptr(), _lib.ptr(initial), S, T, H, HV, K, V,
         bool(use_qk_l2norm), float(K ** -0.5 if scale is None else scale), out.data_ptr(), ws.data_ptr(), _lib.ptr(status),

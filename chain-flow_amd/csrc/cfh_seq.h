@@ -1,5 +1,7 @@
 // Sequences of rows given by bounds cu[0 .. S] on the device: sequence s has the rows cu[s] .. cu[s + 1].
 #pragma once
+#include <algorithm>
+
 #include "cfh_common.h"
 
 namespace {
@@ -45,7 +47,7 @@ __device__ __forceinline__ int first_fall(const int* cu, int S, int lo, int hi) 
   }
   return first;                                    // (behind hi - 1 the last place's again, which is found before)
 }
-__device__ __forceinline__ int ascending(const int* cu, int S) { return S == 1 ? 1 : first_fall(cu, S, 0, S); }
+__device__ __forceinline__ int ascending(const int* cu, int S) { return first_fall(cu, S, 0, S); }
 
 __global__ void __launch_bounds__(1024) k_ascending(const int* cu, int S, int* whole) {
   __shared__ int found[16];
@@ -98,5 +100,23 @@ __device__ __forceinline__ Seq find_seq(const int* cu, int S, const int* whole, 
   const int n = *whole, s = last_where(n, [&](int i) { return pred(i, cu[i]); });
   return {s < n ? s : -1, cu[s], cu[s + 1]};
 }
+
+// The rows of [0, T) that some sequence has, of the first n, whose bounds ascend: one range, as those that begin below 0
+// come first and those that end behind T last.
+struct Rows { int lo, hi; };
+__device__ __forceinline__ Rows covered(const int* cu, int n, int T) {
+  const int i0 = cu[0] < 0 ? last_where(n + 1, [&](int i) { return cu[i] < 0; }) + 1 : 0;
+  if (i0 > n || cu[i0] > T) return {0, 0};
+  return {cu[i0], cu[last_where(n + 1, [&](int i) { return cu[i] <= T; })]};
+}
+
+// f(row) for the rows of [0, T) outside a range, dealt out over `parts` workgroups.
+template <typename F>
+__device__ __forceinline__ void each_outside(const Rows& r, int T, int part, int parts, F f) {
+  for (int i = part; i < r.lo + T - r.hi; i += parts) f(i < r.lo ? i : i - r.lo + r.hi);
+}
+
+// Workgroups that clear such rows, of `bytes` in all: 32 KB each, as far as that goes.
+inline unsigned clearing(long long bytes) { return (unsigned)std::min(256ll, (bytes + 32767) / 32768); }
 
 }  // namespace

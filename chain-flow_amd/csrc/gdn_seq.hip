@@ -45,13 +45,15 @@ struct GdnSeqArgs {
   const uint8_t* initial;  // [S] or null: 0 = start from zero instead of the slot
   uint16_t* out;         // [T][HV][V] bf16
   int* status;
-  int* whole;            // the sequences before the first bound that falls (cfh_seq.h); null: one sequence
-  int known;             // by k_ascending; else k_gdn_rows sets it for the chunk kernels
   int T, S, H, HV, V, ld, nslots, l2norm;
   int few;               // k_gdn_rows takes the sequences of up to so many rows, the chunk kernels the others (0: all)
   int step, plus;        // the chunks' places (chunk_start)
   int nlong;             // sequences that k_gdn_chunks has workgroups for: all S, or as many as can have over `few` rows
   float scale;
+  int fresh;             // out holds nothing yet: rows of no sequence, skipped and padding ones become 0
+  int work;              // workgroups with a part of the work; those behind them clear rows of no sequence
+  int* whole;            // the sequences before the first bound that falls (cfh_seq.h); null: one sequence
+  int known;             // by k_ascending; else k_gdn_rows sets it for the chunk kernels
 };
 
 // softplus by log1p: with log(1 + exp(x)) a decay near 1 (x below -5, the usual ones) keeps few digits of its
@@ -72,16 +74,35 @@ __device__ __forceinline__ int slot_verdict(const int* slots, int S, int s, int 
   return (__ballot(same > 0) || mine < 0 || mine >= nslots) ? -1 : 1;
 }
 
+// A workgroup behind those of the work: its share of the rows of no sequence, as zeros (of a padding one where it is the
+// only one; beside others k_gdn_rows clears those).
+__device__ __forceinline__ void clear_outside(const GdnSeqArgs& a) {
+  const int n = a.HV * a.V / 8;
+  const bool none = a.S == 1 && a.slots[0] == -1;
+  const Rows r = none ? Rows{0, 0} : covered(a.cu, a.known ? *a.whole : ascending(a.cu, a.S), a.T);
+  each_outside(r, a.T, blockIdx.x - a.work, gridDim.x - a.work, [&](int t) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) ((uint4*)a.out)[(size_t)t * n + i] = make_uint4(0, 0, 0, 0);
+  });
+}
+
 // The simplest form, and the decode step: a wave takes 16 value rows of one (sequence, value head) and its
 // tokens one after another.  Lane 16 g + p holds an 8-element share of K of rows 4 g + (0..3) (cfh_gdn.h);
 // a dot product is 8 products and a 16-lane DPP sum.  No LDS and no barrier.
 //   A decode step reads and writes each state once and is bound by that: 61 sequences of 32 value heads with fp32
 // states (257 MB) 51.4 us, 5.0 TB/s, as a large copy; one sequence in bf16 4.4 us, a launch.
-template <typename T>
+// CLEAR: with workgroups behind the work's that clear rows of no sequence (beside the chunk kernels k_gdn_prep has them:
+// the branch in front of 128,000 short waves costs them 20 of 220 us).
+template <typename T, bool CLEAR>
 __global__ void __launch_bounds__(64) k_gdn_rows(GdnSeqArgs a) {
   constexpr int NR = sizeof(T) / 2;
   const int nvs = a.V / 16;
   int u = blockIdx.x;
+  if constexpr (CLEAR) {
+    if (u >= a.work) {
+      clear_outside(a);
+      return;
+    }
+  }
   const int vs = u % nvs;
   u /= nvs;
   const int hv = u % a.HV, s = u / a.HV;
@@ -91,12 +112,12 @@ __global__ void __launch_bounds__(64) k_gdn_rows(GdnSeqArgs a) {
   if (a.whole && !a.known && blockIdx.x == 0 && lane == 0) *a.whole = whole;
   const int ok = slot_verdict(a.slots, a.S, s, a.nslots);
   const bool rows = s < whole && t0 >= 0 && t1 <= a.T && t0 <= t1;
-  if (ok == 0 || (a.few && rows && t1 - t0 > a.few)) return;
-  if (ok < 0 || !rows) {
-    if (a.status && lane == 0) a.status[0] = 1;
+  if (ok ? a.few && rows && t1 - t0 > a.few : !a.fresh || !rows) return;
+  if (ok <= 0 || !rows) {          // (padding sequences of any length)
+    if (ok && a.status && lane == 0) a.status[0] = 1;
     if (rows)
       for (int t = t0; t < t1; ++t)
-        if (p < 4) a.out[((size_t)t * a.HV + hv) * a.V + r0 + p] = 0x7fc0;
+        if (p < 4) a.out[((size_t)t * a.HV + hv) * a.V + r0 + p] = ok ? 0x7fc0 : 0;
     return;
   }
   if (t0 == t1) return;
@@ -226,6 +247,10 @@ __global__ void __launch_bounds__(256) k_gdn_prep(GdnSeqArgs a, char* ws) {
   __shared__ double Gs[GC];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, tl = lane & 15;
   const int slot = blockIdx.x / a.HV, hv = blockIdx.x % a.HV;
+  if ((int)blockIdx.x >= a.work) {
+    clear_outside(a);
+    return;
+  }
   const int whole = a.whole ? *a.whole : a.S;
   const int s = last_where(whole, [&](int i) { return chunk_start(a, i) <= slot; });
   const int c0 = a.cu[s], c1 = a.cu[s + 1];
@@ -780,24 +805,83 @@ constexpr int GDN_SEQS = 4096;   // sequences a call (every wave looks for its s
 
 int seq_args(GdnSeqArgs& g, const void* mixed_qkv, const void* a, const void* b, const float* A_log,
              const float* dt_bias, void* ssm_state, int nslots, const int32_t* slots, int S, int T, int H, int HV, int K,
-             int V, int use_l2norm, float scale, void* out, int32_t* status) {
+             int V, int use_l2norm, float scale, void* out, int32_t* status, int fresh) {
   if (T < 0 || S < 0 || H < 1 || HV < H || HV % H || V < 16 || V % 16 || nslots < 1) return CFH_E_INVALID;
   if (K != GDN_DK || S > GDN_SEQS || 2ll * H * K + (long long)HV * V > 1 << 20) return CFH_E_UNSUPPORTED;
   if (T == 0 || S == 0) return CFH_OK;
   if (!mixed_qkv || !a || !b || !A_log || !dt_bias || !ssm_state || !slots || !out) return CFH_E_INVALID;
-  if (((uintptr_t)mixed_qkv | (uintptr_t)ssm_state) % 16 || (uintptr_t)out % 2) return CFH_E_INVALID;
+  if (((uintptr_t)mixed_qkv | (uintptr_t)ssm_state) % 16 || (uintptr_t)out % (fresh ? 16 : 2)) return CFH_E_INVALID;
   g.qkv = (const uint16_t*)mixed_qkv; g.ga = (const uint16_t*)a; g.gb = (const uint16_t*)b; g.A_log = A_log;
   g.dt_bias = dt_bias; g.state = ssm_state; g.slots = slots; g.out = (uint16_t*)out; g.status = status; g.T = T;
   g.S = S; g.H = H; g.HV = HV; g.V = V; g.ld = 2 * H * K + HV * V; g.nslots = nslots; g.l2norm = use_l2norm ? 1 : 0;
-  g.scale = scale;
+  g.scale = scale; g.fresh = fresh;
   return CFH_OK;
 }
 
-int launch_rows(const GdnSeqArgs& g, int state_bf16, hipStream_t st) {
+// Workgroups behind the work's that clear rows of no sequence.
+unsigned clearing_of(const GdnSeqArgs& g) { return g.fresh && g.cu ? clearing(2ll * g.T * g.HV * g.V) : 0; }
+
+int launch_rows(GdnSeqArgs& g, int state_bf16, bool clear, hipStream_t st) {
   const long long blocks = (long long)g.S * g.HV * (g.V / 16);
-  if (blocks > 0x7fffffffll) return CFH_E_UNSUPPORTED;
-  if (state_bf16) hipLaunchKernelGGL(k_gdn_rows<uint16_t>, dim3((unsigned)blocks), dim3(64), 0, st, g);
-  else hipLaunchKernelGGL(k_gdn_rows<float>, dim3((unsigned)blocks), dim3(64), 0, st, g);
+  if (blocks > 0x7fff0000ll) return CFH_E_UNSUPPORTED;
+  const unsigned more = clear ? clearing_of(g) : 0;
+  g.work = (int)blocks;
+  auto go = [&](auto k) { hipLaunchKernelGGL(k, dim3((unsigned)blocks + more), dim3(64), 0, st, g); };
+  if (more) state_bf16 ? go(k_gdn_rows<uint16_t, true>) : go(k_gdn_rows<float, true>);
+  else state_bf16 ? go(k_gdn_rows<uint16_t, false>) : go(k_gdn_rows<float, false>);
+  CFH_LAUNCH_CHECK();
+  return CFH_OK;
+}
+
+int decode(const void* mixed_qkv, const void* a, const void* b, const float* A_log, const float* dt_bias, void* ssm_state,
+           int state_bf16, int nslots, const int32_t* slots, int S, int H, int HV, int K, int V, int use_l2norm, float scale,
+           void* out, int32_t* status, void* stream, int fresh) {
+  GdnSeqArgs g = {};
+  if (int rc = seq_args(g, mixed_qkv, a, b, A_log, dt_bias, ssm_state, nslots, slots, S, S, H, HV, K, V, use_l2norm,
+                        scale, out, status, fresh))
+    return rc;
+  if (S == 0) return CFH_OK;
+  return launch_rows(g, state_bf16, false, (hipStream_t)stream);
+}
+
+int prefill(const void* mixed_qkv, const void* a, const void* b, const float* A_log, const float* dt_bias, void* ssm_state,
+            int state_bf16, int nslots, const int32_t* slots, const int32_t* cu_seqlens, const uint8_t* initial, int S,
+            int T, int H, int HV, int K, int V, int use_l2norm, float scale, void* out, void* ws, int32_t* status,
+            void* stream, int fresh) {
+  GdnSeqArgs g = {};
+  if (int rc = seq_args(g, mixed_qkv, a, b, A_log, dt_bias, ssm_state, nslots, slots, S, T, H, HV, K, V, use_l2norm,
+                        scale, out, status, fresh))
+    return rc;
+  if (S == 0 || T == 0) return CFH_OK;
+  if (!cu_seqlens) return CFH_E_INVALID;
+  g.cu = cu_seqlens;
+  g.initial = initial;
+  hipStream_t st = (hipStream_t)stream;
+  const int few = few_rows(S, HV, V);
+  if (T <= few) return launch_rows(g, state_bf16, true, st);
+  if (!ws || (uintptr_t)ws % 256) return CFH_E_INVALID;
+  if (S > 1) {
+    g.few = few;
+    g.whole = (int*)((char*)ws + GW_WHOLE);
+    if (S > ASC_OWN) {
+      g.known = 1;
+      hipLaunchKernelGGL(k_ascending, dim3(1), dim3(1024), 0, st, cu_seqlens, S, g.whole);
+      CFH_LAUNCH_CHECK();
+    }
+    if (int rc = launch_rows(g, state_bf16, false, st)) return rc;
+  }
+  const bool by_rows = slots_by_rows(T, few) < slots_by_chunks(T, S);
+  g.step = by_rows ? few + 1 : GC;
+  g.plus = by_rows ? 0 : 1;
+  g.nlong = S > 1 ? std::min(S, T / (few + 1)) : 1;
+  const long long prep = (by_rows ? slots_by_rows(T, few) : slots_by_chunks(T, S)) * HV;
+  const long long blocks = ((long long)g.nlong * HV + 7) / 8 * 8 * (V / 16);
+  if (prep > 0x7fff0000ll || blocks > 0x7fffffffll) return CFH_E_UNSUPPORTED;
+  g.work = (int)prep;
+  hipLaunchKernelGGL(k_gdn_prep, dim3((unsigned)prep + clearing_of(g)), dim3(256), 0, st, g, (char*)ws);
+  CFH_LAUNCH_CHECK();
+  if (state_bf16) hipLaunchKernelGGL(k_gdn_chunks<uint16_t>, dim3((unsigned)blocks), dim3(768), 0, st, g, (const char*)ws);
+  else hipLaunchKernelGGL(k_gdn_chunks<float>, dim3((unsigned)blocks), dim3(768), 0, st, g, (const char*)ws);
   CFH_LAUNCH_CHECK();
   return CFH_OK;
 }
@@ -809,12 +893,15 @@ extern "C" {
 int cfh_gdn_decode(const void* mixed_qkv, const void* a, const void* b, const float* A_log, const float* dt_bias,
                    void* ssm_state, int state_bf16, int nslots, const int32_t* slots, int S, int H, int HV, int K, int V,
                    int use_l2norm, float scale, void* out, int32_t* status, void* stream) {
-  GdnSeqArgs g = {};
-  if (int rc = seq_args(g, mixed_qkv, a, b, A_log, dt_bias, ssm_state, nslots, slots, S, S, H, HV, K, V, use_l2norm,
-                        scale, out, status))
-    return rc;
-  if (S == 0) return CFH_OK;
-  return launch_rows(g, state_bf16, (hipStream_t)stream);
+  return decode(mixed_qkv, a, b, A_log, dt_bias, ssm_state, state_bf16, nslots, slots, S, H, HV, K, V, use_l2norm, scale, out,
+                status, stream, 0);
+}
+
+int cfh_gdn_decode_fresh(const void* mixed_qkv, const void* a, const void* b, const float* A_log, const float* dt_bias,
+                         void* ssm_state, int state_bf16, int nslots, const int32_t* slots, int S, int H, int HV, int K, int V,
+                         int use_l2norm, float scale, void* out, int32_t* status, void* stream) {
+  return decode(mixed_qkv, a, b, A_log, dt_bias, ssm_state, state_bf16, nslots, slots, S, H, HV, K, V, use_l2norm, scale, out,
+                status, stream, 1);
 }
 
 int64_t cfh_gdn_prefill_ws_bytes(int T, int S, int HV) {
@@ -827,41 +914,16 @@ int cfh_gdn_prefill(const void* mixed_qkv, const void* a, const void* b, const f
                     void* ssm_state, int state_bf16, int nslots, const int32_t* slots, const int32_t* cu_seqlens,
                     const uint8_t* initial, int S, int T, int H, int HV, int K, int V, int use_l2norm, float scale,
                     void* out, void* ws, int32_t* status, void* stream) {
-  GdnSeqArgs g = {};
-  if (int rc = seq_args(g, mixed_qkv, a, b, A_log, dt_bias, ssm_state, nslots, slots, S, T, H, HV, K, V, use_l2norm,
-                        scale, out, status))
-    return rc;
-  if (S == 0 || T == 0) return CFH_OK;
-  if (!cu_seqlens) return CFH_E_INVALID;
-  g.cu = cu_seqlens;
-  g.initial = initial;
-  hipStream_t st = (hipStream_t)stream;
-  const int few = few_rows(S, HV, V);
-  if (T <= few) return launch_rows(g, state_bf16, st);
-  if (!ws || (uintptr_t)ws % 256) return CFH_E_INVALID;
-  if (S > 1) {
-    g.few = few;
-    g.whole = (int*)((char*)ws + GW_WHOLE);
-    if (S > ASC_OWN) {
-      g.known = 1;
-      hipLaunchKernelGGL(k_ascending, dim3(1), dim3(1024), 0, st, cu_seqlens, S, g.whole);
-      CFH_LAUNCH_CHECK();
-    }
-    if (int rc = launch_rows(g, state_bf16, st)) return rc;
-  }
-  const bool by_rows = slots_by_rows(T, few) < slots_by_chunks(T, S);
-  g.step = by_rows ? few + 1 : GC;
-  g.plus = by_rows ? 0 : 1;
-  g.nlong = S > 1 ? std::min(S, T / (few + 1)) : 1;
-  const long long prep = (by_rows ? slots_by_rows(T, few) : slots_by_chunks(T, S)) * HV;
-  const long long blocks = ((long long)g.nlong * HV + 7) / 8 * 8 * (V / 16);
-  if (prep > 0x7fffffffll || blocks > 0x7fffffffll) return CFH_E_UNSUPPORTED;
-  hipLaunchKernelGGL(k_gdn_prep, dim3((unsigned)prep), dim3(256), 0, st, g, (char*)ws);
-  CFH_LAUNCH_CHECK();
-  if (state_bf16) hipLaunchKernelGGL(k_gdn_chunks<uint16_t>, dim3((unsigned)blocks), dim3(768), 0, st, g, (const char*)ws);
-  else hipLaunchKernelGGL(k_gdn_chunks<float>, dim3((unsigned)blocks), dim3(768), 0, st, g, (const char*)ws);
-  CFH_LAUNCH_CHECK();
-  return CFH_OK;
+  return prefill(mixed_qkv, a, b, A_log, dt_bias, ssm_state, state_bf16, nslots, slots, cu_seqlens, initial, S, T, H, HV, K, V,
+                 use_l2norm, scale, out, ws, status, stream, 0);
+}
+
+int cfh_gdn_prefill_fresh(const void* mixed_qkv, const void* a, const void* b, const float* A_log, const float* dt_bias,
+                          void* ssm_state, int state_bf16, int nslots, const int32_t* slots, const int32_t* cu_seqlens,
+                          const uint8_t* initial, int S, int T, int H, int HV, int K, int V, int use_l2norm, float scale,
+                          void* out, void* ws, int32_t* status, void* stream) {
+  return prefill(mixed_qkv, a, b, A_log, dt_bias, ssm_state, state_bf16, nslots, slots, cu_seqlens, initial, S, T, H, HV, K, V,
+                 use_l2norm, scale, out, ws, status, stream, 1);
 }
 
 }  // extern "C"

@@ -559,6 +559,16 @@ int cfh_gdn_prefill(const void* mixed_qkv, const void* a, const void* b, const f
                     const uint8_t* initial, int S, int T, int H, int HV, int K, int V, int use_l2norm, float scale,
                     void* out, void* ws, int32_t* status, void* stream);
 
+/* The same into an output that holds nothing yet (16-byte aligned): rows that the calls above leave as they were (of
+ * padding and skipped sequences, and of none) become 0.  S = 0 writes nothing. */
+int cfh_gdn_decode_fresh(const void* mixed_qkv, const void* a, const void* b, const float* A_log, const float* dt_bias,
+                         void* ssm_state, int state_bf16, int nslots, const int32_t* slots, int S, int H, int HV, int K,
+                         int V, int use_l2norm, float scale, void* out, int32_t* status, void* stream);
+int cfh_gdn_prefill_fresh(const void* mixed_qkv, const void* a, const void* b, const float* A_log, const float* dt_bias,
+                          void* ssm_state, int state_bf16, int nslots, const int32_t* slots, const int32_t* cu_seqlens,
+                          const uint8_t* initial, int S, int T, int H, int HV, int K, int V, int use_l2norm, float scale,
+                          void* out, void* ws, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,4 +1,5 @@
-"""Edges of the committed prefix's calls on the GPU: saturated bounds, bounds that fall."""
+"""Edges of the committed prefix's calls on the GPU: saturated bounds, bounds that fall, rows of no sequence in fresh
+outputs."""
 from __future__ import annotations
 
 import numpy as np
@@ -105,3 +106,61 @@ def test_attention_stops_where_the_bounds_fall(cuda, news, bounds, good, most):
     if good:
         assert c.cu[:good + 1].tolist() == bounds[:good + 1]
         check_first(c, o, lse, good)
+
+
+# ---------------------------------------------------------------- rows of no sequence in fresh outputs
+OUTSIDE = [
+    # rows of the query, bounds, rows that sequences cover
+    (21, [3, 7, 16], (3, 16)),                # before, behind
+    (300, [0, 130, 131, 290], (0, 290)),
+    (9, [4, 4], (4, 4)),                      # one sequence of no rows
+    (40, [-5, 10, 30, 50], (10, 30)),         # sequences that are skipped
+    (40, [-5, 50], (0, 0)),
+    (40, [41, 50], (0, 0)),
+    (40, [0, 20, 5, 40], (0, 20)),            # a fall
+    (700, [2 + i for i in range(601)], (2, 602)),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,bounds,cover", OUTSIDE)
+def test_prefill_rows_of_no_sequence_are_zero_in_a_fresh_out(cuda, T, bounds, cover):
+    S = len(bounds) - 1
+    c = GdnCase(cuda, [T], seed=6)
+    c.state = torch.zeros(S + 1, 4, 64, 128)
+    c.slots = torch.arange(S, dtype=torch.int32)
+    a, b = cover
+    out = torch.full((T, 4, 64), 7.0, dtype=BF, device=cuda)
+    want = c.run(cu=bounds, out=out)[0]
+    assert (want[:a] == 7).all() and (want[b:] == 7).all()
+    poison(cuda, T * 4 * 64 * 2)
+    o, _ = c.run(cu=bounds)
+    assert (o[:a] == 0).all() and (o[b:] == 0).all() and torch.equal(o[a:b], want[a:b])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("news", [[5], [70], [3, 70, 1, 64], [1] * 9])
+def test_prefill_rows_of_a_padding_sequence_are_zero_in_a_fresh_out(cuda, news):
+    """Each sequence in turn a padding one (slot -1), short and long; and no sequence at all."""
+    for s in range(len(news)):
+        c = GdnCase(cuda, news, seed=7)
+        c.slots[s] = -1
+        poison(cuda, sum(news) * 4 * 64 * 2)
+        o, _ = c.run()
+        at = slice(c.cu[s], c.cu[s + 1])
+        assert (o[at] == 0).all() and o.isfinite().all()
+    c = GdnCase(cuda, news, seed=7)
+    c.slots = c.slots[:0]
+    poison(cuda, sum(news) * 4 * 64 * 2)
+    assert (c.run(cu=[0])[0] == 0).all()
+
+
+@pytest.mark.gpu
+def test_decode_rows_of_padding_are_zero_in_a_fresh_out(cuda):
+    c = GdnCase(cuda, [1] * 5, seed=8, slots=[4, -1, 0, -1, 6])
+    poison(cuda, 5 * 4 * 64 * 2)
+    o, st = c.run(decode=True)
+    ref, rst = c.oracle()
+    assert (o[1] == 0).all() and (o[3] == 0).all()
+    live = [0, 2, 4]
+    assert rel_err(to64(o[live]), ref[live]) < TOL[BF] and rel_err(to64(st), rst) < 1e-5

@@ -1,0 +1,20 @@
+"""The committed prefix's calls without a GPU: what their host side refuses and plans."""
+from __future__ import annotations
+
+from chain_flow_amd import _lib
+
+
+def test_gdn_calls_into_fresh_outputs_check_their_arguments():
+    """As the calls into outputs that hold something (stand-in addresses, never dereferenced); rows of zeros are written
+    16 bytes at a time."""
+    L = _lib.lib()
+    p = 4096
+
+    def dec(fn, S=3, out=p, K=128, slots=p):
+        return fn(p, p, p, p, p, p, 1, 9, slots, S, 2, 4, K, 128, 1, 0.1, out, None, None)
+    assert dec(L.cfh_gdn_decode_fresh, S=0) == 0 and dec(L.cfh_gdn_decode_fresh, K=64) == 2
+    assert dec(L.cfh_gdn_decode_fresh, slots=None) == 1 and dec(L.cfh_gdn_decode_fresh, out=p + 8) == 1
+
+    def pre(S=3, T=20, cu=p, out=p, ws=p):
+        return L.cfh_gdn_prefill_fresh(p, p, p, p, p, p, 1, 9, p, cu, None, S, T, 2, 4, 128, 128, 1, 0.1, out, ws, None, None)
+    assert pre(T=0) == 0 and pre(S=0) == 0 and pre(cu=None) == 1 and pre(out=p + 8) == 1 and pre(ws=None, T=200) == 1
