@@ -103,6 +103,7 @@ SIGNATURES = {
     "cfh_gdn_prefill": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, C.c_float,
                              _VP, _VP, _VP, _VP]),
 }
+SIGNATURES["cfh_paged_attn_fresh"] = (_I, SIGNATURES["cfh_paged_attn"][1][:-1] + [_I, _VP])
 SIGNATURES.update({name + "_fresh": SIGNATURES[name] for name in ("cfh_gdn_decode", "cfh_gdn_prefill")})
 
 

@@ -123,12 +123,12 @@ def paged_attention(query, k_cache, v_cache, block_table, seq_lens, cu_q, *, sca
     j < len and, if ``causal``, j <= len - n + i (the rows' own keys and values are the cache's last n, written
     before the call).  -> (out [T, H, D] of the query's type, lse [H, T] fp32: ``tree_attn_merge``'s prefix_lse).
 
-    A row that sees no token gives 0 and -inf.  Rows of no sequence stay as they were in ``out``.  Lengths, tables
-    and bounds are read on the device only: a negative length or one past the table, and rows that see a token of
-    a block outside the cache, give NaN; a sequence whose rows do not lie in the query is skipped, and where a bound
-    falls below the one before it that sequence and all behind it are; each sets ``status`` (int32 [1], zeroed by
-    the caller), if given, to 1.  ``max_len``: an upper bound of the lengths (default: what the table holds); it only
-    plans how the work is split."""
+    A row that sees no token gives 0 and -inf.  Rows of no sequence stay as they were in ``out`` (0 without it); their
+    lse is -inf.  Lengths, tables and bounds are read on the device only: a negative length or one past the table, and
+    rows that see a token of a block outside the cache, give NaN; a sequence whose rows do not lie in the query is
+    skipped, and where a bound falls below the one before it that sequence and all behind it are; each sets ``status``
+    (int32 [1], zeroed by the caller), if given, to 1.  ``max_len``: an upper bound of the lengths (default: what the
+    table holds); it only plans how the work is split."""
     if query.dtype not in _TYPES:
         raise ValueError("query must be bf16 or fp16")
     blocks, page, Hkv, D, bs_k, bs_v = _check_cache(k_cache, v_cache, k_exp, v_exp, query.dtype)
@@ -139,7 +139,8 @@ def paged_attention(query, k_cache, v_cache, block_table, seq_lens, cu_q, *, sca
     if seq_lens.shape != (S,) or cu_q.shape != (S + 1,) or block_table.dim() != 2 or block_table.shape[0] != S:
         raise ValueError("seq_lens must be [S], cu_q [S + 1] and block_table [S, blocks]")
     dev = _lib.device_of(query, k_cache, v_cache, k_exp, v_exp, status=status)
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = query.new_empty((T, H, D))
         o_ld = H * D
     else:
@@ -161,10 +162,13 @@ def paged_attention(query, k_cache, v_cache, block_table, seq_lens, cu_q, *, sca
     L = _lib.lib()
     nws = L.cfh_paged_attn_ws_bytes(T, H, Hkv, D, S, most)
     lse = query.new_empty((H, T), dtype=torch.float32)
+    if not S:
+        lse.fill_(float("-inf"))
+        return out.zero_() if fresh else out, lse
     ws = query.new_empty(nws, dtype=torch.uint8) if nws > 0 else None
-    _lib.check(L.cfh_paged_attn(
+    _lib.check(L.cfh_paged_attn_fresh(
         query.data_ptr(), q_ld, T, H, Hkv, D, query.dtype == torch.bfloat16, k_cache.data_ptr(), bs_k, v_cache.data_ptr(),
         bs_v, _lib.ptr(k_exp), _lib.ptr(v_exp), blocks, page, table.data_ptr(), max(table.stride(0), width), width,
         lens.data_ptr(), cu.data_ptr(), S, float(scale), bool(causal), most, out.data_ptr(), o_ld, lse.data_ptr(), _lib.ptr(ws),
-        _lib.ptr(status), _lib.stream_of(dev)), "cfh_paged_attn")
+        _lib.ptr(status), fresh, _lib.stream_of(dev)), "cfh_paged_attn")
     return out, lse

@@ -51,6 +51,8 @@ struct PagedArgs {
   int few;                     // rows (tokens * G) up to which a sequence is k_attn_rows' (0: none)
   int qsign;                   // of the scale: the sign goes into q, so that the scores' maximum scales
   float c;                     // |scale| log2(e)
+  int fresh;                   // lse (1), and out too (2), hold nothing yet: rows of no sequence become -inf and 0
+  int work;                    // workgroups with a part of the work; those behind them clear such rows
 };
 
 // Whether a sequence's rows lie in the query.
@@ -121,6 +123,17 @@ __device__ __forceinline__ bool find_work(const PagedArgs& a, Work& w) {
   w.j1 = w.piece + 1 == a.npiece ? w.jend : min(w.j0 + a.piece, w.jend);
   // a piece past the tile's tokens has nothing to do; the first one also answers for rows that see nothing
   return w.piece == 0 || w.j0 < w.j1;
+}
+
+// A workgroup behind those of the work: its share of the rows of no sequence.
+__device__ __forceinline__ void clear_outside(const PagedArgs& a, int D) {
+  const int n = a.H * D / 8;
+  const int whole = a.whole ? *a.whole : ascending(a.cu, a.S);
+  each_outside(covered(a.cu, whole, a.T), a.T, blockIdx.x - a.work, gridDim.x - a.work, [&](int t) {
+    for (int h = threadIdx.x; h < a.H; h += blockDim.x) a.lse[(size_t)h * a.T + t] = -INFINITY;
+    if (a.fresh & 2)
+      for (int i = threadIdx.x; i < n; i += blockDim.x) *(uint4*)(a.out + (size_t)t * a.o_ld + 8 * i) = make_uint4(0, 0, 0, 0);
+  });
 }
 
 // Sequences whose rows do not lie in the query are skipped: the status word says so.
@@ -256,6 +269,10 @@ __global__ void __launch_bounds__(NW * 64, 2) k_attn_tiles(PagedArgs a) {
   constexpr int OW = (R + 2 * TK + 31) / 32;
   __shared__ int first_bad;
   __shared__ unsigned odd[OW];
+  if (__builtin_expect((int)blockIdx.x >= a.work, 0)) {
+    clear_outside(a, D);
+    return;
+  }
   check_bounds(a);
   Work w;
   if (!find_work<R, false>(a, w)) return;         // (the whole workgroup)
@@ -498,6 +515,10 @@ __global__ void __launch_bounds__(256, 2) k_attn_rows(PagedArgs a) {
   __shared__ float2 ml[NW][16];
   __shared__ int first_bad;
   __shared__ unsigned odd[4];                     // (the tokens not all rows see: 16, and a group on either side)
+  if (__builtin_expect((int)blockIdx.x >= a.work, 0)) {
+    clear_outside(a, D);
+    return;
+  }
   check_bounds(a);
   Work w;
   if (!find_work<R, true>(a, w)) return;          // (the whole workgroup)
@@ -830,21 +851,11 @@ Space space(const Plan& p, int T, int H, int D, int S) {
   return w;
 }
 
-}  // namespace
-
-extern "C" {
-
-int64_t cfh_paged_attn_ws_bytes(int T, int H, int Hkv, int D, int S, int max_len) {
-  if (T < 0 || H < 1 || Hkv < 1 || H % Hkv || S < 0 || max_len < 0 || D < 1) return -1;
-  if (T == 0 || S == 0) return 0;
-  return space(plan(T, H, Hkv, D, S, max_len), T, H, D, S).all;
-}
-
-int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, int is_bf16, const void* k_cache,
-                   long long bs_k, const void* v_cache, long long bs_v, const uint8_t* k_exp, const uint8_t* v_exp,
-                   int blocks, int page, const int32_t* table, int table_ld, int max_blocks, const int32_t* seq_lens,
-                   const int32_t* cu_q, int S, float scale, int causal, int max_len, void* out, long long o_ld,
-                   float* lse, void* ws, int32_t* status, void* stream) {
+int attend(const void* q, long long q_ld, int T, int H, int Hkv, int D, int is_bf16, const void* k_cache,
+           long long bs_k, const void* v_cache, long long bs_v, const uint8_t* k_exp, const uint8_t* v_exp,
+           int blocks, int page, const int32_t* table, int table_ld, int max_blocks, const int32_t* seq_lens,
+           const int32_t* cu_q, int S, float scale, int causal, int max_len, void* out, long long o_ld,
+           float* lse, void* ws, int32_t* status, void* stream, int fresh) {
   if (T < 0 || S < 0 || H < 1 || Hkv < 1 || H % Hkv || blocks < 1 || page < 1 || max_blocks < 0 ||
       table_ld < max_blocks || max_len < 0)
     return CFH_E_INVALID;
@@ -870,6 +881,7 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
   a.table = table; a.lens = seq_lens; a.cu = cu_q; a.status = status; a.q_ld = q_ld; a.o_ld = o_ld; a.bs_k = bs_k;
   a.bs_v = bs_v; a.T = T; a.H = H; a.Hkv = Hkv; a.G = H / Hkv; a.S = S; a.blocks = blocks; a.page = page;
   a.table_ld = table_ld; a.max_blocks = max_blocks; a.causal = causal ? 1 : 0;
+  a.fresh = fresh;
   a.qsign = scale > 0.f ? 1 : scale < 0.f ? -1 : 0;
   a.c = scale == 0.f ? 1.f : fabsf(scale) * 1.44269504088896340736f;
   a.po = (float*)ws;
@@ -889,7 +901,8 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
     const long long per = 8 % groups == 0 ? 8 / groups : 1;
     return 8 % groups == 0 ? (tiles + per - 1) / per * 8 : groups * tiles;
   };
-  if (std::max(grid_of(p.nrow, true), grid_of(p.ntile, a.spread)) > 0x7fffffffll) return CFH_E_UNSUPPORTED;
+  if (std::max(grid_of(p.nrow, true), grid_of(p.ntile, a.spread)) > 0x7fff0000ll) return CFH_E_UNSUPPORTED;
+  const unsigned more = fresh ? clearing((long long)T * H * (fresh & 2 ? 2 * D + 4 : 4)) : 0;
   if (S > ASC_FIND) {
     a.whole = (int*)((char*)ws + w.whole);
     hipLaunchKernelGGL(k_ascending, dim3(1), dim3(1024), 0, st, cu_q, S, (int*)((char*)ws + w.whole));
@@ -897,7 +910,8 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
   }
   if (p.tiles) {
     a.tiles = p.ntile;
-    const dim3 grid((unsigned)grid_of(p.ntile, a.spread));
+    a.work = (int)grid_of(p.ntile, a.spread);
+    const dim3 grid(a.work + (p.rows ? 0 : more));
     kv_dispatch(is_bf16, f8, D, [&](auto bf, auto e8, auto d) {
       constexpr int NW = tile_rows(d.value) / 32, TK = d.value == 256 ? 32 : 64;
       hipLaunchKernelGGL((k_attn_tiles<bf.value, e8.value, d.value, NW, TK>), grid, dim3(NW * 64), 0, st, a);
@@ -906,7 +920,8 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
   }
   if (p.rows) {
     a.tiles = p.nrow;
-    const dim3 grid((unsigned)grid_of(p.nrow, true));
+    a.work = (int)grid_of(p.nrow, true);
+    const dim3 grid(a.work + more);
     kv_dispatch(is_bf16, f8, D, [&](auto bf, auto e8, auto d) {
       hipLaunchKernelGGL((k_attn_rows<bf.value, e8.value, d.value>), grid, dim3(256), 0, st, a);
     });
@@ -930,6 +945,36 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
     CFH_LAUNCH_CHECK();
   }
   return CFH_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t cfh_paged_attn_ws_bytes(int T, int H, int Hkv, int D, int S, int max_len) {
+  if (T < 0 || H < 1 || Hkv < 1 || H % Hkv || S < 0 || max_len < 0 || D < 1) return -1;
+  if (T == 0 || S == 0) return 0;
+  return space(plan(T, H, Hkv, D, S, max_len), T, H, D, S).all;
+}
+
+int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, int is_bf16, const void* k_cache,
+                   long long bs_k, const void* v_cache, long long bs_v, const uint8_t* k_exp, const uint8_t* v_exp,
+                   int blocks, int page, const int32_t* table, int table_ld, int max_blocks, const int32_t* seq_lens,
+                   const int32_t* cu_q, int S, float scale, int causal, int max_len, void* out, long long o_ld,
+                   float* lse, void* ws, int32_t* status, void* stream) {
+  return attend(q, q_ld, T, H, Hkv, D, is_bf16, k_cache, bs_k, v_cache, bs_v, k_exp, v_exp, blocks, page, table,
+                table_ld, max_blocks, seq_lens, cu_q, S, scale, causal, max_len, out, o_ld, lse, ws, status, stream, 0);
+}
+
+int cfh_paged_attn_fresh(const void* q, long long q_ld, int T, int H, int Hkv, int D, int is_bf16,
+                         const void* k_cache, long long bs_k, const void* v_cache, long long bs_v,
+                         const uint8_t* k_exp, const uint8_t* v_exp, int blocks, int page, const int32_t* table,
+                         int table_ld, int max_blocks, const int32_t* seq_lens, const int32_t* cu_q, int S,
+                         float scale, int causal, int max_len, void* out, long long o_ld, float* lse, void* ws,
+                         int32_t* status, int out_too, void* stream) {
+  return attend(q, q_ld, T, H, Hkv, D, is_bf16, k_cache, bs_k, v_cache, bs_v, k_exp, v_exp, blocks, page, table,
+                table_ld, max_blocks, seq_lens, cu_q, S, scale, causal, max_len, out, o_ld, lse, ws, status, stream,
+                out_too ? 3 : 1);
 }
 
 }  // extern "C"

@@ -532,6 +532,14 @@ int cfh_paged_attn(const void* q, long long q_ld, int T, int H, int Hkv, int D, 
                    int blocks, int page, const int32_t* table, int table_ld, int max_blocks, const int32_t* seq_lens,
                    const int32_t* cu_q, int S, float scale, int causal, int max_len, void* out, long long o_ld,
                    float* lse, void* ws, int32_t* status, void* stream);
+/* The same into an lse that holds nothing yet and, with out_too, such an out: rows that the call above leaves as they were (of
+ * skipped sequences and of none) get lse -inf, and out 0.  S = 0 writes nothing. */
+int cfh_paged_attn_fresh(const void* q, long long q_ld, int T, int H, int Hkv, int D, int is_bf16,
+                         const void* k_cache, long long bs_k, const void* v_cache, long long bs_v,
+                         const uint8_t* k_exp, const uint8_t* v_exp, int blocks, int page, const int32_t* table,
+                         int table_ld, int max_blocks, const int32_t* seq_lens, const int32_t* cu_q, int S,
+                         float scale, int causal, int max_len, void* out, long long o_ld, float* lse, void* ws,
+                         int32_t* status, int out_too, void* stream);
 
 /* ---------------------------------------------------------------- the committed prefix: recurrent state
  * The gated delta rule over committed tokens, in the layout of cfh_gdn_tree_vllm (mixed_qkv, a, b, A_log,

@@ -164,3 +164,33 @@ def test_decode_rows_of_padding_are_zero_in_a_fresh_out(cuda):
     assert (o[1] == 0).all() and (o[3] == 0).all()
     live = [0, 2, 4]
     assert rel_err(to64(o[live]), ref[live]) < TOL[BF] and rel_err(to64(st), rst) < 1e-5
+
+
+# ---------------------------------------------------------------- fresh attention outputs
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [100, 4000])
+@pytest.mark.parametrize("T,bounds,cover", OUTSIDE)
+def test_attention_rows_of_no_sequence_are_zero_in_a_fresh_out(cuda, T, bounds, cover, most):
+    """Without `out`, rows that no sequence has (or a skipped one) are 0, and their lse is -inf with and without it."""
+    S = len(bounds) - 1
+    c = Case(cuda, BF, BF, [0] * S, [20 + i % 50 for i in range(S)], 4, 2, 64, 16, seed=4)
+    q = torch.randn(T, 4, 64, device=cuda).to(BF)
+    a, b = cover
+    for given in (False, True):
+        poison(cuda, *[T * 4 * 64 * 2] * 2, *[T * 4 * 4] * 2)
+        out = torch.full_like(q, 7.0) if given else None
+        o, lse = c.run(q=q, cu=bounds, out=out, table=wide(c, most), max_len=most)
+        rest = torch.cat([o[:a], o[b:]])
+        assert (rest == (7 if given else 0)).all()
+        assert (lse[:, :a] == -np.inf).all() and (lse[:, b:] == -np.inf).all()
+        assert o[a:b].isfinite().all() and (lse[:, a:b] > -np.inf).all() or min(c.lens) < max(np.diff(bounds))
+        assert not o[a:b].isnan().any() and not lse[:, a:b].isnan().any()
+
+
+@pytest.mark.gpu
+def test_attention_of_no_sequences_is_zero(cuda):
+    c = Case(cuda, BF, BF, [0], [20], 4, 2, 64, 16, seed=5)
+    q = torch.randn(5, 4, 64, device=cuda).to(BF)
+    poison(cuda, 5 * 4 * 64 * 2, 5 * 4 * 4)
+    o, lse = c.run(q=q, cu=[0], lens=[], table=c.table[:0])
+    assert (o == 0).all() and (lse == -np.inf).all()

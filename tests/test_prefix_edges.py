@@ -18,3 +18,14 @@ def test_gdn_calls_into_fresh_outputs_check_their_arguments():
     def pre(S=3, T=20, cu=p, out=p, ws=p):
         return L.cfh_gdn_prefill_fresh(p, p, p, p, p, p, 1, 9, p, cu, None, S, T, 2, 4, 128, 128, 1, 0.1, out, ws, None, None)
     assert pre(T=0) == 0 and pre(S=0) == 0 and pre(cu=None) == 1 and pre(out=p + 8) == 1 and pre(ws=None, T=200) == 1
+
+
+def test_attention_into_fresh_outputs_checks_its_arguments():
+    L = _lib.lib()
+    p = 4096
+
+    def attn(S=2, T=3, out=p, lse=p, cu=p, max_len=80):
+        return L.cfh_paged_attn_fresh(p, 1024, T, 8, 4, 128, 1, p, 16 * 512, p, 16 * 512, None, None, 7, 16, p, 5, 5, p, cu,
+                                      S, 0.1, 1, max_len, out, 1024, lse, p, None, 1, None)
+    assert attn(T=0) == 0 and attn(S=0) == 0
+    assert attn(out=p + 8) == 1 and attn(lse=None) == 1 and attn(cu=None) == 1 and attn(max_len=-1) == 1
