@@ -249,6 +249,10 @@ __device__ __forceinline__ void add_odd(const PagedArgs& a, const Work& w, unsig
 }
 
 constexpr float LAZY = 8.f;   // log2 units the running maximum may lag behind (probabilities up to 2^8)
+// fp16 probabilities are taken 2^7 as large (up to 2^15, the statistics with them): it ends at 2^-24, and beside one
+// token with nearly all the weight, tens of thousands of others of 2^-25 each would vanish from the product with V.
+template <bool BF>
+constexpr float LIFT = BF ? 0.f : 7.f;
 
 // Many rows.  Wave v of a workgroup takes rows 32 v .. 32 v + 31 of its tile; lane l of a wave holds query
 // row l % 32, and of every group of eight tokens the four with (t / 4) % 2 == l / 32.  Token tiles of TK go
@@ -395,7 +399,7 @@ __global__ void __launch_bounds__(NW * 64, 2) k_attn_tiles(PagedArgs a) {
       for (int b = 0; b < TK / 32; ++b)
 #pragma unroll
         for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[b][e]);
-      mx = swap_max(mx) * a.c;
+      mx = swap_max(mx) * a.c - LIFT<BF>;
       if (__any(mx > m + LAZY || (m == -INFINITY && mx > m))) {
         const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
         l *= f;
@@ -636,7 +640,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_rows(PagedArgs a) {
         mx = fmaxf(mx, sc[u][e]);
       }
     mx = fmaxf(mx, __shfl_xor(mx, 16));
-    mx = swap_max(mx) * a.c;
+    mx = swap_max(mx) * a.c - LIFT<BF>;
     if (__any(mx > m + LAZY || (m == -INFINITY && mx > m))) {
       const float mn = fmaxf(m, mx), fac = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
       l *= fac;

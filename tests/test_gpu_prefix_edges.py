@@ -1,5 +1,5 @@
 """Edges of the committed prefix's calls on the GPU: saturated bounds, bounds that fall, rows of no sequence in fresh
-outputs."""
+outputs, probabilities far below the largest one."""
 from __future__ import annotations
 
 import numpy as np
@@ -11,7 +11,7 @@ from conftest import rel_err, to64
 from oracle import kv_cache as okv
 from test_gpu_gdn_seq import TOL
 from test_gpu_gdn_seq import Case as GdnCase
-from test_gpu_kv_cache import BF, Case, close
+from test_gpu_kv_cache import BF, F8, FP, Case, close
 
 
 def poison(cuda, *nbytes):
@@ -194,3 +194,34 @@ def test_attention_of_no_sequences_is_zero(cuda):
     poison(cuda, 5 * 4 * 64 * 2, 5 * 4 * 4)
     o, lse = c.run(q=q, cu=[0], lens=[], table=c.table[:0])
     assert (o == 0).all() and (lse == -np.inf).all()
+
+
+# ---------------------------------------------------------------- probabilities far below the largest
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache", [FP, F8])
+@pytest.mark.parametrize("T,D,split", [(1, 64, False), (40, 64, False), (40, 128, False), (40, 256, False), (1, 128, True)])
+def test_many_small_probabilities_beside_a_large_one(cuda, T, D, split, cache):
+    """fp16: one token takes nearly all the weight (the first, as a prompt's first token does) and each of 60,000 others
+    2^-25.5 of it; together they are 1.3e-3 of the result.  A probability enters the product with v as fp16 scaled by
+    2^7, so it loses at most 2^-25 2^-7, and a row at most L 2^-32 |v|."""
+    L = 60000
+    c = Case(cuda, FP, cache, [T], [L], 2, 1, D, 64, seed=9)
+    k, v = (t.view(torch.uint8 if cache == F8 else FP) for t in (c.k, c.v))
+    one = 0x38 if cache == F8 else 1.0                                      # (the byte of e4m3's 1)
+    blk = c.table[0].long().to(cuda)
+    k[blk], v[blk] = 0, one
+    if cache == F8:
+        c.ke[blk], c.ve[blk] = 127, 127
+    k[blk[0], 0, 0, 0] = one
+    v[blk[0], 0] = 0
+    c.ok, c.ov = [np.zeros((L, 1, D))], [np.ones((L, 1, D))]
+    c.ok[0][0, 0, 0], c.ov[0][0] = 1.0, 0.0
+    c.q.zero_()
+    c.q[:, :, 0] = 25.5 * np.log(2.0) / c.scale
+    out, lse = c.run(causal=False, max_len=L if split else 1)
+    ref, rlse, weight, reach = okv.attention(to64(c.q), c.ok, c.ov, c.lens, c.cu, c.scale, False)
+    u, score = 2.0 ** -11, (D * 2.0 ** -24 * reach).T[..., None]
+    bound = u * np.abs(ref) + (u + 2 * score + L * 2.0 ** -23) * weight + 2.0 ** -24 + L * 2.0 ** -32
+    off = np.abs(to64(out) - ref) / bound
+    print(f"[small probabilities] {cache} T={T} D={D}: {to64(out).max():.3e} for {ref.max():.3e}, {off.max():.3f} of its bound", flush=True)
+    assert off.max() <= 1.0 and np.abs(to64(lse) - rlse).max() <= score.max() + L * 2.0 ** -24 + 2.0 ** -22 * np.abs(rlse).max()
