@@ -37,11 +37,10 @@ def _check_cache(k_cache, v_cache, k_exp, v_exp, dtype):
                 raise ValueError(f"an 8-bit cache needs contiguous uint8 k_exp and v_exp [{blocks}, {page}, {Hkv}]")
     elif kind != dtype or k_exp is not None or v_exp is not None:
         raise ValueError(f"the cache must be {dtype} without exponents, or float8_e4m3fn with them")
-    (bs_k, *in_k), (bs_v, *in_v) = k_cache.stride(), v_cache.stride()
     row = Hkv * D
     inner = page * row
-    if blocks == 1:
-        bs_k = bs_v = inner
+    want = (inner, row, D, 1)
+    (bs_k, *in_k), (bs_v, *in_v) = _strides(k_cache, want), _strides(v_cache, want)
     want = [row, D, 1]
     if (in_k != want or in_v != want or bs_k < inner or bs_v < inner or (bs_k | bs_v) % 16
             or (k_cache.data_ptr() | v_cache.data_ptr()) % 16):
@@ -50,11 +49,19 @@ def _check_cache(k_cache, v_cache, k_exp, v_exp, dtype):
     return blocks, page, Hkv, D, bs_k, bs_v
 
 
+def _strides(t, want):
+    """A tensor's strides, those of dimensions of size one (which may be anything) as wanted."""
+    got = t.stride()
+    if 1 in t.shape:
+        got = tuple(w if n == 1 else g for n, g, w in zip(t.shape, got, want))
+    return got
+
+
 def _rows(t):
     """Rows [T, heads, D] with contiguous heads whose vector loads are aligned (copied where they are not), and
     their stride."""
     T, h, D = t.shape
-    ld, inner, one = t.stride()
+    ld, inner, one = _strides(t, (h * D, D, 1))
     if T < 2:
         ld = h * D
     if one != 1 or inner != D or ld < h * D or ld % 8 or t.data_ptr() % 16:
@@ -144,8 +151,10 @@ def paged_attention(query, k_cache, v_cache, block_table, seq_lens, cu_q, *, sca
         out = query.new_empty((T, H, D))
         o_ld = H * D
     else:
-        o_ld = out.stride(0) if T > 1 else H * D
-        if (out.shape != query.shape or out.dtype != query.dtype or out.get_device() != dev or out.stride()[1:] != (D, 1)
+        o_ld, *in_o = _strides(out, (H * D, D, 1)) if out.shape == query.shape else (0, 0)
+        if T < 2:
+            o_ld = H * D
+        if (out.dtype != query.dtype or out.get_device() != dev or in_o != [D, 1]
                 or o_ld < H * D or o_ld % 8 or out.data_ptr() % 16):
             raise ValueError(f"out must be a {query.dtype} [{T}, {H}, {D}] tensor on cuda:{dev} with contiguous heads, "
                              "16-byte aligned")

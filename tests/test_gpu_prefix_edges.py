@@ -1,5 +1,5 @@
 """Edges of the committed prefix's calls on the GPU: saturated bounds, bounds that fall, rows of no sequence in fresh
-outputs, probabilities far below the largest one."""
+outputs, probabilities far below the largest one, dimensions of size one."""
 from __future__ import annotations
 
 import numpy as np
@@ -225,3 +225,17 @@ def test_many_small_probabilities_beside_a_large_one(cuda, T, D, split, cache):
     off = np.abs(to64(out) - ref) / bound
     print(f"[small probabilities] {cache} T={T} D={D}: {to64(out).max():.3e} for {ref.max():.3e}, {off.max():.3f} of its bound", flush=True)
     assert off.max() <= 1.0 and np.abs(to64(lse) - rlse).max() <= score.max() + L * 2.0 ** -24 + 2.0 ** -22 * np.abs(rlse).max()
+
+
+# ---------------------------------------------------------------- dimensions of size one
+@pytest.mark.gpu
+def test_attention_strides_of_size_one_do_not_count(cuda):
+    """One kv head kept as [blocks, 1, page, D], one query head behind a wider stride: contiguous all the same."""
+    c = Case(cuda, BF, BF, [3, 1], [40, 9], 1, 1, 64, 16, seed=10)
+    want = c.run()
+    c.k, c.v = (t.transpose(1, 2).contiguous().transpose(1, 2) for t in (c.k, c.v))
+    c.k, c.v = (t.as_strided(t.shape, (1024, 64, 4096, 1)) for t in (c.k, c.v))
+    out = torch.zeros(4, 64, dtype=BF, device=cuda).as_strided((4, 1, 64), (64, 8, 1))
+    got = c.run(q=c.q.as_strided(c.q.shape, (64, 8, 1)), out=out)
+    assert got[0].data_ptr() == out.data_ptr()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -1,7 +1,11 @@
 """The committed prefix's calls without a GPU: what their host side refuses and plans."""
 from __future__ import annotations
 
+import pytest
+import torch
+
 from chain_flow_amd import _lib
+from chain_flow_amd.kv_cache import kv_cache_read, kv_cache_write
 
 
 def test_gdn_calls_into_fresh_outputs_check_their_arguments():
@@ -29,3 +33,20 @@ def test_attention_into_fresh_outputs_checks_its_arguments():
                                       S, 0.1, 1, max_len, out, 1024, lse, p, None, 1, None)
     assert attn(T=0) == 0 and attn(S=0) == 0
     assert attn(out=p + 8) == 1 and attn(lse=None) == 1 and attn(cu=None) == 1 and attn(max_len=-1) == 1
+
+
+@pytest.mark.parametrize("shape,strides", [((4, 8, 1, 64), (512, 64, 512, 1)),      # [blocks, Hkv, page, D] seen as pages
+                                           ((4, 1, 2, 64), (128, 999, 64, 1)), ((1, 8, 2, 64), (7, 128, 64, 1)),
+                                           ((4, 1, 1, 64), (64, 1, 3, 1))])
+def test_strides_of_dimensions_of_size_one_do_not_count(shape, strides):
+    """A cache that is contiguous but for what a stride over one element says passes (as far as a CPU's goes); one that
+    is not, with more than one element there, does not."""
+    k = torch.zeros(4096, dtype=torch.bfloat16).as_strided(shape, strides)
+    rows = torch.zeros(3, shape[2], 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="one GPU"):
+        kv_cache_read(k, k, torch.arange(3))
+    with pytest.raises(ValueError, match="one GPU"):
+        kv_cache_write(rows, rows, k, k, torch.arange(3))
+    wide = torch.zeros(1 << 14, dtype=torch.bfloat16).as_strided((4, 8, 2, 64), (1024, 64, 512, 1))
+    with pytest.raises(ValueError, match="contiguous"):
+        kv_cache_read(wide, wide, torch.arange(3))
