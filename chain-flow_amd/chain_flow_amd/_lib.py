@@ -100,6 +100,7 @@ SIGNATURES = {
     "cfh_gdn_decode": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _VP, _I, _I, _I, _I, _I, _I, C.c_float, _VP, _VP,
                             _VP]),
     "cfh_gdn_prefill_ws_bytes": (_I64, [_I, _I, _I]),
+    "cfh_gdn_prefill_plan": (_I, [_I, _I, _I, _I, _VP]),
     "cfh_gdn_prefill": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, C.c_float,
                              _VP, _VP, _VP, _VP]),
 }

@@ -792,14 +792,30 @@ __global__ void __launch_bounds__(768) k_gdn_chunks(GdnSeqArgs a, const char* ws
 // without a sequence of theirs cost 3 to 16 us (two of 12, eight of 16).
 constexpr int GDN_ROWS_MIN = 9, GDN_ROWS_MAX = 16, GDN_CUS = 256;
 static_assert(GDN_ROWS_MAX < 32, "chunk slots");
-inline int few_rows(long long S, int HV, int V) {
-  const long long rounds = std::min((S * HV * (V / 16) + GDN_CUS - 1) / GDN_CUS, 8ll);
-  return 8 + (int)rounds;                          // GDN_ROWS_MIN to GDN_ROWS_MAX
-}
 
-// Chunk slots for sequences of more than `few` rows.
+// Places of chunks by either rule of chunk_start.
 inline long long slots_by_chunks(int T, int S) { return (long long)T / GC + S; }
 inline long long slots_by_rows(int T, int few) { return T / (few + 1) + 1; }
+inline long long places(int T, int S, int few) { return std::min(slots_by_chunks(T, S), slots_by_rows(T, few)); }
+
+// How a prefill is split, from what the host knows.
+struct PrefillPlan {
+  int few;               // rows up to which a sequence goes one after another
+  int step, plus;        // chunk_start
+  int nlong;             // sequences of more rows, at most
+  long long places;      // chunks they use, at most
+};
+PrefillPlan prefill_plan(int T, int S, int HV, int V) {
+  PrefillPlan p;
+  const long long rounds = ((long long)S * HV * (V / 16) + GDN_CUS - 1) / GDN_CUS;
+  p.few = (int)std::min<long long>(GDN_ROWS_MIN - 1 + std::max(1ll, rounds), GDN_ROWS_MAX);
+  const bool by_rows = slots_by_rows(T, p.few) < slots_by_chunks(T, S);
+  p.step = by_rows ? p.few + 1 : GC;
+  p.plus = by_rows ? 0 : 1;
+  p.nlong = S > 1 ? std::min(S, T / (p.few + 1)) : 1;
+  p.places = places(T, S, p.few);
+  return p;
+}
 
 constexpr int GDN_SEQS = 4096;   // sequences a call (every wave looks for its slot among theirs)
 
@@ -857,11 +873,11 @@ int prefill(const void* mixed_qkv, const void* a, const void* b, const float* A_
   g.cu = cu_seqlens;
   g.initial = initial;
   hipStream_t st = (hipStream_t)stream;
-  const int few = few_rows(S, HV, V);
-  if (T <= few) return launch_rows(g, state_bf16, true, st);
+  const PrefillPlan p = prefill_plan(T, S, HV, V);
+  if (T <= p.few) return launch_rows(g, state_bf16, true, st);
   if (!ws || (uintptr_t)ws % 256) return CFH_E_INVALID;
   if (S > 1) {
-    g.few = few;
+    g.few = p.few;
     g.whole = (int*)((char*)ws + GW_WHOLE);
     if (S > ASC_OWN) {
       g.known = 1;
@@ -870,11 +886,10 @@ int prefill(const void* mixed_qkv, const void* a, const void* b, const float* A_
     }
     if (int rc = launch_rows(g, state_bf16, false, st)) return rc;
   }
-  const bool by_rows = slots_by_rows(T, few) < slots_by_chunks(T, S);
-  g.step = by_rows ? few + 1 : GC;
-  g.plus = by_rows ? 0 : 1;
-  g.nlong = S > 1 ? std::min(S, T / (few + 1)) : 1;
-  const long long prep = (by_rows ? slots_by_rows(T, few) : slots_by_chunks(T, S)) * HV;
+  g.step = p.step;
+  g.plus = p.plus;
+  g.nlong = p.nlong;
+  const long long prep = p.places * HV;
   const long long blocks = ((long long)g.nlong * HV + 7) / 8 * 8 * (V / 16);
   if (prep > 0x7fff0000ll || blocks > 0x7fffffffll) return CFH_E_UNSUPPORTED;
   g.work = (int)prep;
@@ -907,7 +922,15 @@ int cfh_gdn_decode_fresh(const void* mixed_qkv, const void* a, const void* b, co
 int64_t cfh_gdn_prefill_ws_bytes(int T, int S, int HV) {
   if (T < 0 || S < 0 || HV < 1) return -1;
   if (T <= GDN_ROWS_MIN || S == 0) return 0;
-  return std::min(slots_by_chunks(T, S), slots_by_rows(T, GDN_ROWS_MIN)) * HV * GW_BYTES;
+  return places(T, S, GDN_ROWS_MIN) * HV * GW_BYTES;   // (a larger `few` needs no more)
+}
+
+int cfh_gdn_prefill_plan(int T, int S, int HV, int V, int32_t* plan) {
+  if (T < 0 || S < 1 || HV < 1 || V < 16 || !plan) return CFH_E_INVALID;
+  if (S > GDN_SEQS || (long long)HV * V > 1 << 20) return CFH_E_UNSUPPORTED;
+  const PrefillPlan p = prefill_plan(T, S, HV, V);
+  plan[0] = p.few; plan[1] = p.step; plan[2] = p.plus; plan[3] = p.nlong; plan[4] = (int)p.places;
+  return CFH_OK;
 }
 
 int cfh_gdn_prefill(const void* mixed_qkv, const void* a, const void* b, const float* A_log, const float* dt_bias,

@@ -566,8 +566,11 @@ int cfh_gdn_prefill(const void* mixed_qkv, const void* a, const void* b, const f
                     void* ssm_state, int state_bf16, int nslots, const int32_t* slots, const int32_t* cu_seqlens,
                     const uint8_t* initial, int S, int T, int H, int HV, int K, int V, int use_l2norm, float scale,
                     void* out, void* ws, int32_t* status, void* stream);
+/* How cfh_gdn_prefill splits a call of these sizes: plan[5] = the rows up to which a sequence goes row by row; a longer
+ * one's first chunk lies in place floor(cu_seqlens[s] / plan[1]) + plan[2] s of the workspace; such sequences at most; places. */
+int cfh_gdn_prefill_plan(int T, int S, int HV, int V, int32_t* plan);
 
-/* The same into an output that holds nothing yet (16-byte aligned): rows that the calls above leave as they were (of
+/* cfh_gdn_decode and cfh_gdn_prefill into an output that holds nothing yet (16-byte aligned): rows that those leave as they were (of
  * padding and skipped sequences, and of none) become 0.  S = 0 writes nothing. */
 int cfh_gdn_decode_fresh(const void* mixed_qkv, const void* a, const void* b, const float* A_log, const float* dt_bias,
                          void* ssm_state, int state_bf16, int nslots, const int32_t* slots, int S, int H, int HV, int K,

@@ -1,6 +1,9 @@
 """The committed prefix's calls without a GPU: what their host side refuses and plans."""
 from __future__ import annotations
 
+import ctypes
+
+import numpy as np
 import pytest
 import torch
 
@@ -50,3 +53,31 @@ def test_strides_of_dimensions_of_size_one_do_not_count(shape, strides):
     wide = torch.zeros(1 << 14, dtype=torch.bfloat16).as_strided((4, 8, 2, 64), (1024, 64, 512, 1))
     with pytest.raises(ValueError, match="contiguous"):
         kv_cache_read(wide, wide, torch.arange(3))
+
+
+def test_prefill_plan_places_every_chunk_in_the_workspace():
+    """The split that the launches use: the rows of a sequence that go one after another stay in the rule's range and grow
+    with the work, chunks of longer sequences lie apart and inside the workspace, and no more sequences are long than
+    have workgroups."""
+    L = _lib.lib()
+    rng = np.random.default_rng(1)
+    plan = (ctypes.c_int32 * 5)()
+    seen = set()
+    for _ in range(2000):
+        HV, V = int(rng.choice([1, 2, 8, 32])), int(rng.choice([16, 64, 128, 256]))
+        edges = [0, 1, 8, 9, 10, 11, 15, 16, 17, 18, 63, 64, 65, 128, 129, 500]
+        news = rng.choice(edges, size=int(rng.choice([1, 2, 5, 40, 300])), p=None if rng.random() < 0.5 else
+                          np.r_[[0.3, 0.3], [0.4 / 14] * 14])
+        cu = np.concatenate([[int(rng.integers(0, 30))], news]).cumsum()
+        T, S = int(cu[-1] + rng.integers(0, 30)), len(news)
+        assert L.cfh_gdn_prefill_plan(T, S, HV, V, plan) == 0
+        few, step, plus, nlong, places = plan
+        seen.add(few)
+        assert 9 <= few <= 16
+        at = [c for s, n in enumerate(news) if n > few for c in range(cu[s] // step + plus * s, cu[s] // step + plus * s - (-n // 64))]
+        assert len(set(at)) == len(at) and max(at, default=-1) < places
+        assert sum(n > few for n in news) <= nlong or T <= few
+        if T > few:
+            assert places * HV * 34048 <= L.cfh_gdn_prefill_ws_bytes(T, S, HV)
+    assert {9, 16} <= seen
+    assert L.cfh_gdn_prefill_plan(5, 0, 1, 16, plan) == 1 and L.cfh_gdn_prefill_plan(5, 4097, 1, 16, plan) == 2
