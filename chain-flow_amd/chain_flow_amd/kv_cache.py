@@ -20,6 +20,12 @@ from chain_flow_amd import _lib
 _TYPES = (torch.bfloat16, torch.float16)
 
 
+def _laid(t, want):
+    """Whether a tensor's strides behind the first are as wanted; those over a single element may be anything."""
+    got = t.stride()[1:]
+    return got == want or all(n == 1 or g == w for n, g, w in zip(t.shape[1:], got, want))
+
+
 def _check_cache(k_cache, v_cache, k_exp, v_exp, dtype):
     """-> (blocks, page, Hkv, D, block strides of k and v) of a cache that serves rows of ``dtype``."""
     shape = k_cache.shape
@@ -39,32 +45,21 @@ def _check_cache(k_cache, v_cache, k_exp, v_exp, dtype):
         raise ValueError(f"the cache must be {dtype} without exponents, or float8_e4m3fn with them")
     row = Hkv * D
     inner = page * row
-    want = (inner, row, D, 1)
-    (bs_k, *in_k), (bs_v, *in_v) = _strides(k_cache, want), _strides(v_cache, want)
-    want = [row, D, 1]
-    if (in_k != want or in_v != want or bs_k < inner or bs_v < inner or (bs_k | bs_v) % 16
+    want = (row, D, 1)
+    bs_k, bs_v = (inner, inner) if blocks == 1 else (k_cache.stride(0), v_cache.stride(0))
+    if (not _laid(k_cache, want) or not _laid(v_cache, want) or bs_k < inner or bs_v < inner or (bs_k | bs_v) % 16
             or (k_cache.data_ptr() | v_cache.data_ptr()) % 16):
         raise ValueError("cache blocks must be contiguous [page, Hkv, D], on strides of 16 elements and 16-byte "
                          "boundaries")
     return blocks, page, Hkv, D, bs_k, bs_v
 
 
-def _strides(t, want):
-    """A tensor's strides, those of dimensions of size one (which may be anything) as wanted."""
-    got = t.stride()
-    if 1 in t.shape:
-        got = tuple(w if n == 1 else g for n, g, w in zip(t.shape, got, want))
-    return got
-
-
 def _rows(t):
     """Rows [T, heads, D] with contiguous heads whose vector loads are aligned (copied where they are not), and
     their stride."""
     T, h, D = t.shape
-    ld, inner, one = _strides(t, (h * D, D, 1))
-    if T < 2:
-        ld = h * D
-    if one != 1 or inner != D or ld < h * D or ld % 8 or t.data_ptr() % 16:
+    ld = t.stride(0) if T > 1 else h * D
+    if not _laid(t, (D, 1)) or ld < h * D or ld % 8 or t.data_ptr() % 16:
         t, ld = _lib.aligned(t.contiguous()), h * D
     return t, ld
 
@@ -151,10 +146,8 @@ def paged_attention(query, k_cache, v_cache, block_table, seq_lens, cu_q, *, sca
         out = query.new_empty((T, H, D))
         o_ld = H * D
     else:
-        o_ld, *in_o = _strides(out, (H * D, D, 1)) if out.shape == query.shape else (0, 0)
-        if T < 2:
-            o_ld = H * D
-        if (out.dtype != query.dtype or out.get_device() != dev or in_o != [D, 1]
+        o_ld = out.stride(0) if T > 1 else H * D
+        if (out.shape != query.shape or out.dtype != query.dtype or out.get_device() != dev or not _laid(out, (D, 1))
                 or o_ld < H * D or o_ld % 8 or out.data_ptr() % 16):
             raise ValueError(f"out must be a {query.dtype} [{T}, {H}, {D}] tensor on cuda:{dev} with contiguous heads, "
                              "16-byte aligned")
