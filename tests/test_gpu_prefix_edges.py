@@ -1,11 +1,12 @@
 """Edges of the committed prefix's calls on the GPU: saturated bounds, bounds that fall, rows of no sequence in fresh
-outputs, probabilities far below the largest one, dimensions of size one."""
+outputs, probabilities far below the largest one, dimensions of size one, captured calls."""
 from __future__ import annotations
 
 import numpy as np
 import pytest
 import torch
 
+from chain_flow_amd.gdn import gdn_prefill
 from chain_flow_amd.kv_cache import paged_attention
 from conftest import rel_err, to64
 from oracle import kv_cache as okv
@@ -239,3 +240,54 @@ def test_attention_strides_of_size_one_do_not_count(cuda):
     got = c.run(q=c.q.as_strided(c.q.shape, (64, 8, 1)), out=out)
     assert got[0].data_ptr() == out.data_ptr()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# ---------------------------------------------------------------- captured, with bounds that change between replays
+@pytest.mark.gpu
+@pytest.mark.parametrize("S", [5, 300, 700])
+def test_a_captured_call_follows_its_bounds(cuda, S):
+    """One graph of an attention (whose out and lse it makes) and a prefill; before each replay the bounds are others:
+    all rows, none, rows of no sequence on either side, a fall, ends outside the query.  Every replay equals the eager
+    calls."""
+    news = [1 + i % 3 for i in range(S)]
+    news[S // 2] = 60
+    T = sum(news)
+    c = Case(cuda, BF, BF, [0] * S, [70 + i % 9 for i in range(S)], 4, 2, 64, 16, seed=11)
+    g = GdnCase(cuda, [T], H=1, HV=2, V=16, seed=12)
+    state = torch.randn(S, 2, 16, 128, device=cuda)
+    q = torch.randn(T, 4, 64, device=cuda).to(BF)
+    d = lambda t: t.to(cuda)  # noqa: E731
+    x, a, b, A, dt, slots = d(g.x), d(g.a), d(g.b), d(g.A), d(g.dt), torch.arange(S, dtype=torch.int32, device=cuda)
+    table, lens = wide(c, 3000).to(cuda), torch.tensor(c.lens, dtype=torch.int32, device=cuda)
+    whole = torch.tensor([0, *np.cumsum(news)], dtype=torch.int32)
+    fall, low, late = whole.clone(), whole - 3, whole + 3
+    fall[S // 3:] -= 7
+    cu = whole.to(cuda)
+    st, status = state.clone(), torch.zeros(1, dtype=torch.int32, device=cuda)
+
+    def step(st, status):
+        o, lse = paged_attention(q, c.k, c.v, table, lens, cu, scale=c.scale, status=status)
+        return o, lse, gdn_prefill(x, a, b, A, dt, st, slots, cu, num_q_heads=1, status=status)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(st, status)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(st, status)
+    for name, bounds in (("whole", whole), ("fall", fall), ("none", whole * 0 + 5), ("low", low), ("whole", whole),
+                         ("late", late)):
+        print(f"[captured bounds] S={S} {name}", flush=True)
+        cu.copy_(bounds)
+        st.copy_(state)
+        status.zero_()
+        graph.replay()
+        got = [t.clone() for t in (*outs, st, status)]
+        est, estat = state.clone(), torch.zeros_like(status)
+        want = (*step(est, estat), est, estat)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, w) for p, w in zip(got, want)), name
+        assert status.item() == (name in ("fall", "low", "late")) and all(t.isfinite().all() for t in (got[0], got[2]))
