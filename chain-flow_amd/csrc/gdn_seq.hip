@@ -438,7 +438,8 @@ __global__ void __launch_bounds__(256) k_gdn_prep(GdnSeqArgs a, char* ws) {
 
 // S through the chunks of one (sequence, value head), 16 value columns, in a chain that no other workgroup can
 // shorten: what counts is the time from one chunk's S to the next one's, 1.6 us (8,000 rows of 32 value heads: 125
-// chunks in 200 us on all CUs; five prompts of up to 300 rows 37).  Waves 0 - 3 carry the chain, waves
+// chunks in 200 us on all CUs; five prompts of up to 300 rows 39: 1,280 workgroups, one a CU, so five rounds of up to
+// five chunks and their ramps).  Waves 0 - 3 carry the chain, waves
 // 4 - 7 compute the outputs beside it, waves 8 - 11 bring K, v and the rows' factors into LDS.  Three barriers a
 // chunk.
 //   B1  every chain wave multiplies all of K with its own 32 k rows of S (from registers), the partial products

@@ -10,7 +10,8 @@
 // border cannot fall to its other side.  It costs no precision: e4m3's relative step is the same in every
 // binade, and the up to one binade left unused at the top is one of 15.  The format has no infinity:
 // NaN and infinite elements are stored as NaN.  Where 256 * 2^E is above the source type's largest value
-// the elements end at 240 (still within half a step), so that every finite value reads back finite.
+// the elements end at 240 (off by up to 15.9 scales, less than 2^-4 of the value), so that every finite value reads back
+// finite.
 #include "cfh_host.h"
 #include "cfh_kv.h"
 
@@ -18,8 +19,9 @@ namespace {
 
 // Groups of D / 8 lanes take the key and the value of one (row, head), 8 elements a lane: 16-byte accesses of the
 // 2-byte side, 8-byte ones of the 8-bit side; N of them a group, their loads in flight together.
-//   Bound by memory: 16,000 rows of 4 heads of 256 into an 8-bit cache (98 MB, scattered slots) 22.5 us, 4.4 TB/s; 40,000
-// such rows back (246 MB) 41 us, 6.0 TB/s, where a copy of 256 MB makes 5.4.  32 rows: 3.3 us, a launch.
+//   Bound by memory: 16,000 rows of 4 heads of 256 into an 8-bit cache (98 MB, scattered slots) 20.4 us, 4.8 TB/s; 40,000
+// such rows back (246 MB) 48.5 us, 5.1 TB/s, as a copy of 1 GiB (where every call writes the same 164 MB, which the
+// last cache partly holds, 41).  32 rows: 3.5 us, a launch.
 struct KvRowsArgs {
   const u16* key; const u16* value;          // [T][Hkv][D], row strides ld_k / ld_v
   u16* out_key; u16* out_value;              // (reading)

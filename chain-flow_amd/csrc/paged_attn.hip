@@ -12,7 +12,9 @@
 // a lane then holds one query row's scores, the running maximum and sum of its softmax are lane-local but
 // for one exchange, and the probabilities are already where the next MFMA wants its second operand
 // (O^T += V^T P^T), only in another order of the tokens, which the first operand's loads follow.
-// Probabilities are rounded to the 2-byte type once for that product; statistics and sums are fp32.
+// Probabilities are rounded to the 2-byte type once for that product, whose matrix instructions take no wider operand at
+// this rate: half a step (2^-8, 2^-11) of each, so at most that much of sum p |v|, beside the same half step of the
+// rounded output (errors of 2.3e-3 for 1.7e-3 with bf16).  Scores, statistics and sums are fp32.
 //   k_attn_tiles  many rows: workgroups of NW waves x 32 rows over tiles of tokens staged in LDS
 //   k_attn_rows   few rows (decode): one tile of 16 rows, each wave its own tokens, no barrier but the join's
 // The long axis is cut into pieces of `piece` tokens where the rows alone do not fill the chip; k_attn_join
@@ -258,9 +260,11 @@ constexpr float LIFT = BF ? 0.f : 7.f;
 // row l % 32, and of every group of eight tokens the four with (t / 4) % 2 == l / 32.  Token tiles of TK go
 // global -> registers -> LDS one tile ahead (the 8-bit cache is widened on that way), double-buffered, one
 // barrier a tile.
-//   3,841 rows (16 / 4 heads of 256) over up to 9,001 tokens take 540 us: 755 TFLOP/s, 54% of a large matrix product's rate
-// (D = 128: 712).  Bound by the waves' own chain scores -> softmax -> products (MFMA busy 28% of the time, LDS 31%):
-// at D = 256 the accumulators leave room for two waves a SIMD, whose turns do not cover each other's exponentials.
+//   3,841 rows (16 / 4 heads of 256) over up to 9,001 tokens take 540 us: 760 TFLOP/s, 54% of a large matrix product's rate
+// (D = 128: 720).  244 workgroups of 3,551 to 9,001 tokens, one a CU: over the longest one's time the CUs work 69.5% of
+// it, at 78% of the product's rate while they do.  That rest is the waves' own chain scores -> softmax -> products (matrix
+// instructions busy 28% of the time, LDS 31%): at D = 256 the accumulators leave room for two waves a SIMD, whose turns do
+// not cover each other's exponentials.  The kernel for D = 256 spills 8 vector registers (8-bit cache: 6).
 template <bool BF, bool F8, int D, int NW, int TK>
 __global__ void __launch_bounds__(NW * 64, 2) k_attn_tiles(PagedArgs a) {
   constexpr int R = NW * 32, NT = NW * 64;
@@ -491,9 +495,11 @@ __global__ void __launch_bounds__(NW * 64, 2) k_attn_tiles(PagedArgs a) {
 // 64-byte segments a load), V through the wave's own rows of LDS for the transposed reads; both one group
 // ahead, 16 KB a wave (an 8-bit cache: 8 at D = 64, else 16), with no branch around a load: behind one the compiler
 // waits for everything.  Waves do not wait for each other before the join of their (max, sum, O) at the end.
-//   Bound by memory latency: two workgroups a CU keep 128 KB in flight.  One row over 30,011 tokens (16 / 4 heads of
-// 256, 123 MB) 31 us, 4.0 TB/s, and the join 6 beside it; 48 rows over up to 9,000 (16 / 2 heads of 256) 132 us
-// together, 4.3 TB/s, and in 8 bits 99, where widening the elements shares the waves' time.
+//   Bound by memory latency: one row over 30,011 tokens (16 / 4 heads of 256, 123 MB) is 236 workgroups, one a CU, with 64 KB
+// in flight: 38.5 us, 3.2 TB/s, and the join 5 beside it; 48 rows over up to 9,000 (16 / 2 heads of 256), two workgroups a
+// CU with 128 KB, 131 us together, 4.3 TB/s, and in 8 bits 97, where widening the elements shares the waves' time and
+// 17 vector and 9 scalar registers spill (D = 128 in 8 bits: 8 scalar ones).  At D = 64 (and 128 in 2 bytes) 48 bytes a
+// lane of scratch memory are no spill but add_odd's arrays, touched only where a value is not finite.
 template <bool BF>
 __device__ __forceinline__ f32x4 mfma16(const uint4& x, const uint4& y, f32x4 acc) {
   if constexpr (BF)
@@ -823,8 +829,10 @@ Plan plan(int T, int H, int Hkv, int D, int S, int max_len) {
   p.nrow = p.few ? S : (int)(packed / FEW_ROWS) + S;
   p.ntile = (int)(packed / tile_rows(D)) + S;
   // Pieces so that (row tiles) x (kv heads) x pieces fill the chip with the workgroups it holds at once, one a CU at
-  // D = 256 with many rows, else two.  Many rows are left whole from three quarters of a workgroup a CU on (244 of
-  // them, 3,841 rows over 9,001 tokens: cut in two 614 us, whole 551); few rows are not (100 x 2 kv heads: whole 100
+  // D = 256 with many rows, else two.  Many rows are left whole from three quarters of a workgroup a CU on
+  // (9,001 tokens, 16 / 4 heads of 256, whole / cut by the rule below / best cut: 128 workgroups 529 / 313 / 313, 160 531 /
+  // 578 / 412, 192 531 / 585 / 501, 208 530 / 588 / 525, 256 553 / 607 / 607; at D = 128, where two workgroups share a CU,
+  // cutting wins up to 256 of them and loses at 320: 192 in two 183 for 227, 256 198 for 228, 320 290 for 276); few rows are not (100 x 2 kv heads: whole 100
   // us, in three 65; 64 x 4: 72, in two 55; 125 x 4: 129, in two 128).  More and shorter pieces of few rows lose
   // again (48 x 2 kv heads, D = 128 in 8 bits: 3 pieces 65 us, 6 51, 8 61, 18 65).  Pieces of 512 tokens at least where
   // rows are few (one row over 30,011: 256 tokens 25 / 29 us at D = 64 / 128, 512 tokens 20 / 24), 256 where they are

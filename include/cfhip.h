@@ -557,7 +557,8 @@ int cfh_paged_attn_fresh(const void* q, long long q_ld, int T, int H, int Hkv, i
  * whose bounds do not lie in [0, T] is skipped and sets status; where a bound falls below the one before it, that
  * sequence and all behind it are; one of no rows leaves its slot as it was; rows of no sequence are left as they were).  initial [S] (or NULL: all 1): 0 = start from a zero state
  * instead of the slot's.  ws: cfh_gdn_prefill_ws_bytes(T, S, HV) bytes, 256-byte aligned (NULL where that is 0), of
- * the call's own until it ends. */
+ * the call's own until it ends: 34,048 for each value head and place, of which there are the lesser of T / 64 + S and
+ * T / 10 + 1 (8,000 rows of one prompt and 32 value heads: 137 MB; 131,072 rows: 2.2 GB). */
 int cfh_gdn_decode(const void* mixed_qkv, const void* a, const void* b, const float* A_log, const float* dt_bias,
                    void* ssm_state, int state_bf16, int nslots, const int32_t* slots, int S, int H, int HV, int K,
                    int V, int use_l2norm, float scale, void* out, int32_t* status, void* stream);
