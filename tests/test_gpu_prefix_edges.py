@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+from chain_flow_amd import _lib
 from chain_flow_amd.gdn import gdn_prefill
 from chain_flow_amd.kv_cache import paged_attention
 from conftest import rel_err, to64
@@ -195,6 +196,28 @@ def test_attention_of_no_sequences_is_zero(cuda):
     poison(cuda, 5 * 4 * 64 * 2, 5 * 4 * 4)
     o, lse = c.run(q=q, cu=[0], lens=[], table=c.table[:0])
     assert (o == 0).all() and (lse == -np.inf).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [100, 3000])
+def test_the_plain_c_call_leaves_rows_of_no_sequence(cuda, most):
+    """cfh_paged_attn itself writes no row of out or lse that no sequence has; in the others it is the Python call."""
+    c = Case(cuda, BF, BF, [4, 30], [50, 90], 4, 2, 64, 16, seed=13)
+    q = torch.randn(50, 4, 64, device=cuda).to(BF)
+    bounds, table = [7, 11, 41], wide(c, most).to(cuda)
+    o, lse = c.run(q=q, cu=bounds, table=table, max_len=most)
+    out, lse2 = torch.full_like(q, 7.0), torch.full((4, 50), 7.0, device=cuda)
+    lens, cu = (torch.tensor(x, dtype=torch.int32, device=cuda) for x in (c.lens, bounds))
+    L = _lib.lib()
+    ws = torch.empty(max(1, L.cfh_paged_attn_ws_bytes(50, 4, 2, 64, 2, most)), dtype=torch.uint8, device=cuda)
+    blocks, stride = c.k.shape[0], c.k.stride(0)
+    rc = L.cfh_paged_attn(q.data_ptr(), 256, 50, 4, 2, 64, 1, c.k.data_ptr(), stride, c.v.data_ptr(), stride, None, None, blocks,
+                          16, table.data_ptr(), table.shape[1], table.shape[1], lens.data_ptr(), cu.data_ptr(), 2, c.scale, 1, most,
+                          out.data_ptr(), 256, lse2.data_ptr(), ws.data_ptr(), None, _lib.stream_handle())
+    torch.cuda.synchronize()
+    assert rc == 0
+    assert (out[:7] == 7).all() and (out[41:] == 7).all() and (lse2[:, :7] == 7).all() and (lse2[:, 41:] == 7).all()
+    assert torch.equal(out[7:41], o[7:41]) and torch.equal(lse2[:, 7:41], lse[:, 7:41])
 
 
 # ---------------------------------------------------------------- probabilities far below the largest
