@@ -6,7 +6,9 @@
   (``_tree_suffix_eager`` / ``fused_suffix_merge``, patch lines 403-575, 2793-3121): the tree rows'
   ancestor-masked attention merged into ``output`` with the prefix half by log-sum-exp;
 * ``tree_greedy_accept`` -- ``tree_rejection_sample`` (patch lines 510-550): row argmax + greedy
-  descent.
+  descent;
+* ``tree_sample_accept`` -- the same walk with every row's token drawn from the target's filtered
+  probabilities by a given uniform number (temperature, top-k, top-p a request).
 """
 from __future__ import annotations
 
@@ -128,3 +130,72 @@ def tree_greedy_accept(logits, cu_num_draft_tokens, cu_num_sampled_tokens, draft
         csg.data_ptr(), draft.data_ptr(), par.data_ptr(), B, max_spec_len, out.data_ptr(), path.data_ptr(),
         ln.data_ptr(), ra.data_ptr(), ws.data_ptr(), _lib.stream_handle()), "cfh_tree_greedy_accept")
     return out, path[:, :max_spec_len], ln
+
+
+def _counts_fit(cd, cs, R, D, max_spec_len):
+    """Whether host-side cumulative draft and row counts describe requests of n drafts and n + 1 rows (or none of either)."""
+    import numpy as np
+    nd, ns = (np.diff(np.concatenate([[0], np.asarray(c, dtype=np.int64)])) for c in (cd, cs))
+    return not ((nd < 0).any() or nd.max(initial=0) > max_spec_len or ((ns != nd + 1) & ((ns != 0) | (nd != 0))).any()
+                or int(cs[-1]) > R or int(cd[-1]) > D)
+
+
+def tree_sample_accept(logits, cu_num_draft_tokens, cu_num_sampled_tokens, draft_token_ids, tree_parents,
+                       max_spec_len: int, uniforms, temperature, *, top_k=None, top_p=None, status=None):
+    """``tree_greedy_accept`` for sampled requests: row r's target token is drawn by uniforms[r] in [0, 1) from its logits
+    under its request's ``temperature`` [B] (fp32; 0: the largest logit), ``top_k`` [B] (int32; 0, or None: off) and
+    ``top_p`` [B] (fp32; 1, or None: off); the walk from a request's root row steps to the first child that holds the
+    drawn token and ends with the token that no child holds.  Drafts count as certain (a beam search's are), so that what is
+    emitted is distributed as the target's own samples.
+
+    A row's tokens are ordered by logit, ties by the lower index; NaN and -inf are none.  Of exp((x - max) / temperature) the
+    first top_k are kept, of those the shortest prefix that has top_p of their sum (one token at least), and the token
+    is the first at which the running sum exceeds uniforms[r] times what is kept.  Sums are held in 64 bits.  A row
+    without any token gives none: its walk ends there.  Uniforms outside [0, 1) count as the nearest in it, NaN as 0; a
+    temperature that is not above 0 as 0.
+
+    logits [rows, V] (bf16 / fp16; rows may be strided); cumulative (inclusive) draft and row counts a request (n drafts have n + 1
+    rows; a request of no rows and drafts is padding); draft ids and local parents (-1 = root).  -> (output_token_ids
+    [B, max_spec_len + 1] int32, -1 padded; accepted_path [B, max_spec_len]; accepted_len [B]; logprobs [B, max_spec_len
+    + 1] fp32, 0 padded: the log of what each emitted token's probability was, after the filters).  Counts are
+    read on the device only (host ones are checked here): a request whose counts do not fit the rows or drafts, and all
+    behind counts that fall, emit nothing and set ``status`` (int32 [1] on the device, zeroed by the caller), if given, to 1."""
+    if logits.dtype not in (torch.bfloat16, torch.float16) or logits.dim() != 2 or logits.numel() == 0:
+        raise ValueError("logits must be bf16 / fp16 [rows, V]")
+    R, V = logits.shape
+    ld = logits.stride(0) if R > 1 else V
+    if (V > 1 and logits.stride(1) != 1) or ld < V:
+        raise ValueError("logits must have contiguous rows")
+    max_spec_len = int(max_spec_len)
+    if max_spec_len < 0:
+        raise ValueError(f"max_spec_len {max_spec_len} is negative")
+    B, D = len(cu_num_draft_tokens), len(draft_token_ids)
+    if len(cu_num_sampled_tokens) != B or len(tree_parents) != D:
+        raise ValueError("draft and row counts must be of one length, and draft ids and parents of another")
+    dev = _lib.device_of(logits, status=status)
+    for name, t, n, kinds in (("uniforms", uniforms, R, (torch.float32,)), ("temperature", temperature, B, (torch.float32,)),
+                              ("top_k", top_k, B, (torch.int32, torch.int64)), ("top_p", top_p, B, (torch.float32,))):
+        if t is None and name[:3] == "top":
+            continue
+        if t.shape != (n,) or t.dtype not in kinds or t.get_device() != dev:
+            raise ValueError(f"{name} must be {' or '.join(str(k) for k in kinds)} [{n}] on cuda:{dev}")
+    cd, cs = _host(cu_num_draft_tokens), _host(cu_num_sampled_tokens)
+    if B and cd is not None and cs is not None and not _counts_fit(cd, cs, R, D, max_spec_len):
+        raise ValueError("cumulative draft / row counts inconsistent with the logits rows, the drafts and max_spec_len")
+    index = lambda t: _lib.index32(t if isinstance(t, torch.Tensor) else torch.as_tensor(t, dtype=torch.int64), dev)  # noqa: E731
+    draft, par, cdg, csg = (index(t) for t in (draft_token_ids, tree_parents, cu_num_draft_tokens, cu_num_sampled_tokens))
+    uniforms, temperature = uniforms.contiguous(), temperature.contiguous()
+    top_k = None if top_k is None else _lib.index32(top_k, dev)
+    top_p = None if top_p is None else top_p.contiguous()
+    out = torch.empty(B, max_spec_len + 1, dtype=torch.int32, device=logits.device)
+    path = torch.empty(B, max_spec_len, dtype=torch.int32, device=logits.device)
+    ln = torch.empty(B, dtype=torch.int32, device=logits.device)
+    lps = torch.empty(B, max_spec_len + 1, dtype=torch.float32, device=logits.device)
+    L = _lib.lib()
+    ws = torch.empty(int(L.cfh_tree_sample_ws_bytes(R)), dtype=torch.uint8, device=logits.device)
+    _lib.check(L.cfh_tree_sample_accept(
+        logits.data_ptr(), ld, V, R, logits.dtype == torch.bfloat16, cdg.data_ptr(), csg.data_ptr(), _lib.ptr(draft),
+        _lib.ptr(par), D, B, max_spec_len, uniforms.data_ptr(), temperature.data_ptr(), _lib.ptr(top_k), _lib.ptr(top_p),
+        out.data_ptr(), path.data_ptr(), ln.data_ptr(), lps.data_ptr(), ws.data_ptr(), _lib.ptr(status),
+        _lib.stream_of(dev)), "cfh_tree_sample_accept")
+    return out, path, ln, lps

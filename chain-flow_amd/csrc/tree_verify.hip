@@ -10,6 +10,7 @@
 #include <type_traits>
 
 #include "cfh_kernels.h"
+#include "cfh_walk.h"
 
 namespace {
 
@@ -398,35 +399,11 @@ __global__ void __launch_bounds__(64) k_tree_descent(DescentArgs a) {
   for (int i = threadIdx.x; i <= a.max_spec; i += blockDim.x) ot[i] = -1;
   for (int i = threadIdx.x; i < a.max_spec; i += blockDim.x) pt[i] = -1;
   __syncthreads();
-  // the walk: at each level the wave tests 64 nodes at a time for (parent == cur, token == the
-  // row's argmax); the lowest matching index is the first child in draft order
   const int lane = threadIdx.x;
-  int cur = -1, pos = 0;
-  for (int step = 0; step <= a.max_spec; ++step) {
-    const int tok = lds ? s_arg[cur + 1] : a.row_argmax[s0 + cur + 1];
-    if (lane == 0) ot[pos] = tok;
-    int nxt = -1;
-    if (pos < a.max_spec) {
-      for (int i0 = 0; i0 < n; i0 += 64) {
-        const int i = i0 + lane;
-        bool hit = false;
-        if (i < n) {
-          const int pi = lds ? s_par[i] : a.parents[d0 + i];
-          const int ti = lds ? s_tok[i] : a.draft[d0 + i];
-          hit = pi == cur && ti == tok;
-        }
-        const unsigned long long m = __ballot(hit);
-        if (m) {
-          nxt = i0 + __ffsll((long long)m) - 1;
-          break;
-        }
-      }
-    }
-    if (nxt < 0) break;
-    if (lane == 0) pt[pos] = nxt;
-    cur = nxt;
-    ++pos;
-  }
+  const int pos = walk_tree(
+      n, a.max_spec, [&](int row) { return lds ? s_arg[row] : a.row_argmax[s0 + row]; },
+      [&](int i) { return lds ? s_par[i] : a.parents[d0 + i]; }, [&](int i) { return lds ? s_tok[i] : a.draft[d0 + i]; },
+      [&](int p, int, int tok) { if (lane == 0) ot[p] = tok; }, [&](int p, int node) { if (lane == 0) pt[p] = node; });
   if (lane == 0) a.len[r] = pos;
 }
 

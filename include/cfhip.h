@@ -486,6 +486,25 @@ int cfh_tree_greedy_accept(const void* logits, long long ld, int V, int n_rows, 
                            int max_spec, int32_t* out_tokens, int32_t* accepted_path, int32_t* accepted_len,
                            int32_t* row_argmax, void* ws, void* stream);
 
+/* Sampled tree verify: cfh_tree_greedy_accept with row r's token drawn by uniforms[r] in [0, 1) (others: the nearest;
+ * NaN: 0) from its logits under its request's temperature (not above 0: the largest logit), top_k (NULL, or below 1: off)
+ * and top_p (NULL, or 1 and above: off).  Tokens in order of logit, ties by index, NaN and -inf none: w = exp((x - max) /
+ * temperature); the first top_k; of those the shortest prefix of at least top_p times their sum (one token at least);
+ * the first whose running sum exceeds uniforms[r] times what is kept.  Sums in 64 bits.  A row without a token ends its walk.
+ *   cu_draft, cu_sampled [B]: inclusive cumulative drafts and rows (n drafts, n + 1 rows; 0 and 0: a padding request);
+ *   draft_ids, parents [n_drafts] (local parents, -1 = root); uniforms [n_rows]; temperature, top_k, top_p [B].
+ *   out_tokens [B][max_spec + 1] and accepted_path [B][max_spec] (-1 padded), accepted_len [B], out_logprobs [B][max_spec
+ *   + 1] (0 padded): the log of the emitted tokens' probabilities after the filters.
+ * A request whose counts do not lie in the rows and drafts, and all behind counts that fall, get no token and set status[0]
+ * to 1 (status: one int32 the caller zeroes, or NULL).  V <= 2^24.  ws: cfh_tree_sample_ws_bytes(n_rows) bytes, 16-byte
+ * aligned, of the call's own until it ends. */
+int64_t cfh_tree_sample_ws_bytes(int n_rows);
+int cfh_tree_sample_accept(const void* logits, long long ld, int V, int n_rows, int is_bf16, const int32_t* cu_draft,
+                           const int32_t* cu_sampled, const int32_t* draft_ids, const int32_t* parents, int n_drafts, int B,
+                           int max_spec, const float* uniforms, const float* temperature, const int32_t* top_k,
+                           const float* top_p, int32_t* out_tokens, int32_t* accepted_path, int32_t* accepted_len,
+                           float* out_logprobs, void* ws, int32_t* status, void* stream);
+
 /* ---------------------------------------------------------------- the committed prefix: paged cache
  * The key / value cache of a target's attention layers: k_cache, v_cache [blocks][page][Hkv][D], slot n =
  * row n % page of block n / page; block strides bs_k / bs_v in elements (multiples of 16, at least

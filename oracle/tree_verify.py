@@ -122,6 +122,59 @@ def greedy_descent(row_argmax, cu_draft, cu_sampled, draft, parents, max_spec):
     return out, path, ln
 
 
+def sampled_token(x, T, k, P, u):
+    """One row x [V] (float64): (token, log of its probability after the filters); (-1, 0) without a token.  Tokens in
+    order of (x descending, index ascending), NaN and -inf none; w = exp((x - max) / T), 1 at the largest; the first k
+    (k < 1: all); the shortest prefix of at least P times their sum (P >= 1: all); the first whose running sum exceeds u
+    times what is kept.  Running sums by np.cumsum over the ordered tokens, one token at a time."""
+    x = np.asarray(x, dtype=np.float64) + 0.0
+    idx = np.flatnonzero(~np.isnan(x) & (x != -np.inf))
+    if not len(idx):
+        return -1, 0.0
+    idx = idx[np.argsort(-x[idx], kind="stable")]
+    v = x[idx]
+    if not T > 0:
+        return int(idx[0]), 0.0
+    with np.errstate(invalid="ignore", over="ignore"):
+        w = np.where(v == v[0], 1.0, 0.0 if np.isinf(v[0]) else np.exp((v - v[0]) / T))
+    if k is not None and 0 < k < len(w):
+        w = w[:k]
+    cum = np.cumsum(w)
+    if P is not None and P < 1:
+        n = int(np.searchsorted(cum, P * cum[-1], side="left")) + 1       # the first with cum >= P total
+        w, cum = w[:max(n, 1)], cum[:max(n, 1)]
+    u = 0.0 if not u > 0 else min(float(u), 1.0 - 2.0 ** -24)
+    i = min(int(np.searchsorted(cum, u * cum[-1], side="right")), int((w > 0).sum()) - 1)
+    return int(idx[i]), float(np.log(w[i] / cum[-1]))
+
+
+def sampled_descent(logits, cu_draft, cu_sampled, draft, parents, max_spec, u, T, k=None, P=None):
+    """``greedy_descent`` with each row's ``sampled_token`` under its request's T, k, P: (out_tokens, path, length, logprobs
+    [B, max_spec + 1], 0 padded).  A row without a token ends its walk; a request of no rows emits nothing."""
+    B = len(cu_draft)
+    out = np.full((B, max_spec + 1), -1, dtype=np.int64)
+    path = np.full((B, max_spec), -1, dtype=np.int64)
+    ln, lps = np.zeros(B, dtype=np.int64), np.zeros((B, max_spec + 1))
+    for r in range(B):
+        d0, s0 = (0 if r == 0 else int(c[r - 1]) for c in (cu_draft, cu_sampled))
+        n = int(cu_draft[r]) - d0
+        if int(cu_sampled[r]) == s0:
+            continue
+        cur = -1
+        for pos in range(max_spec + 1):
+            row = s0 + cur + 1
+            tok, lp = sampled_token(logits[row], T[r], None if k is None else k[r], None if P is None else P[r], u[row])
+            if tok < 0:
+                break
+            out[r, pos], lps[r, pos] = tok, lp
+            here = [i for i in range(n) if parents[d0 + i] == cur and draft[d0 + i] == tok]
+            if pos == max_spec or not here:
+                break
+            path[r, pos] = cur = here[0]
+            ln[r] = pos + 1
+    return out, path, ln, lps
+
+
 def first_argmax(logits):
     """torch.argmax: the first index of the maximum of each row."""
     return np.argmax(logits, axis=-1)
