@@ -30,6 +30,12 @@ class VaeDims(C.Structure):
                 ("heads", C.c_int), ("max_rows", C.c_int)]
 
 
+class KvPool(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("k", "v", "k_exp", "v_exp")]
+                + [(n, C.c_longlong) for n in ("ls_k", "ls_v", "bs_k", "bs_v", "ls_k_exp", "ls_v_exp")]
+                + [(n, C.c_int) for n in ("layers", "blocks", "page", "heads", "dim")])
+
+
 _VP = C.c_void_p
 _I = C.c_int
 _I64 = C.c_int64
@@ -100,6 +106,10 @@ SIGNATURES = {
     "cfh_paged_attn_ws_bytes": (_I64, [_I, _I, _I, _I, _I, _I]),
     "cfh_paged_attn": (_I, [_VP, _I64, _I, _I, _I, _I, _I, _VP, _I64, _VP, _I64, _VP, _VP, _I, _I, _VP, _I, _I, _VP,
                             _VP, _I, C.c_float, _I, _I, _VP, _I64, _VP, _VP, _VP, _VP]),
+    "cfh_kv_commit": (_I, [C.POINTER(KvPool), _VP, _I, _I, _VP, _VP, _I, _I, _VP, _I, _VP, _VP]),
+    "cfh_kv_fork": (_I, [_VP, _I, _I, _VP, _I, _VP, _I, _I, _VP, _VP, _I, _VP, _VP]),
+    "cfh_kv_resize_ws_bytes": (_I64, [_I, _I, _I]),
+    "cfh_kv_resize": (_I, [C.POINTER(KvPool), _VP, _I, _I, _VP, _I, _VP, _I, _I, _VP, _VP, _VP, _VP]),
     "cfh_gdn_decode": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _VP, _I, _I, _I, _I, _I, _I, C.c_float, _VP, _VP,
                             _VP]),
     "cfh_gdn_prefill_ws_bytes": (_I64, [_I, _I, _I]),

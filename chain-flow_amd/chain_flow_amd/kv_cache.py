@@ -4,7 +4,8 @@
 * ``kv_cache_read`` -- slots back as rows of the model's type;
 * ``paged_attention`` -- new rows (a prefill chunk, single tokens, a draft tree's nodes) over each
   sequence's pages; with ``causal=False`` and a tree's nodes it gives the prefix half that
-  ``tree_attn_merge`` merges with.
+  ``tree_attn_merge`` merges with;
+* ``kv_cache_commit`` -- a draft tree's accepted rows moved together, in the caches of all layers.
 
 A cache is [blocks, page, Hkv, D] of the model's type (bf16 or fp16), or of ``torch.float8_e4m3fn`` with a
 byte [blocks, page, Hkv] (uint8) per slot and head: byte c, 1 to 254, stands for the scale 2^(c - 127).  Slot n is row
@@ -52,6 +53,62 @@ def _check_cache(k_cache, v_cache, k_exp, v_exp, dtype):
         raise ValueError("cache blocks must be contiguous [page, Hkv, D], on strides of 16 elements and 16-byte "
                          "boundaries")
     return blocks, page, Hkv, D, bs_k, bs_v
+
+
+def _check_pool(k_cache, v_cache, k_exp, v_exp):
+    """-> the ``KvPool`` of a cache, or of the caches of several layers [layers, blocks, page, Hkv, D]."""
+    shape, kind = k_cache.shape, k_cache.dtype
+    if v_cache.shape != shape or v_cache.dtype != kind:
+        raise ValueError("k_cache and v_cache must share one shape and type")
+    if len(shape) == 4:
+        layers, (blocks, page, Hkv, D) = 1, shape
+        ls_k = ls_v = 0
+        sk, sv = k_cache.stride(), v_cache.stride()
+    elif len(shape) == 5:
+        layers, blocks, page, Hkv, D = shape
+        (ls_k, *sk), (ls_v, *sv) = k_cache.stride(), v_cache.stride()
+    else:
+        raise ValueError("a cache must be [blocks, page, Hkv, D], or with the layers before")
+    if not layers * blocks * page * Hkv:
+        raise ValueError(f"a cache of shape {tuple(shape)} holds nothing")
+    if D != 128 and D != 256 and D != 64:
+        raise ValueError(f"head width {D} is not 64, 128 or 256")
+    f8 = kind == torch.float8_e4m3fn
+    lk = lv = 0
+    if f8:
+        for e in (k_exp, v_exp):
+            if e is None or e.dtype != torch.uint8 or e.shape != shape[:-1] or not (e[0] if layers > 1 else e).is_contiguous():
+                raise ValueError(f"an 8-bit cache needs uint8 k_exp and v_exp {tuple(shape[:-1])}, contiguous in a layer")
+        if layers > 1:
+            lk, lv = k_exp.stride(0), v_exp.stride(0)
+            if min(lk, lv) < blocks * page * Hkv:
+                raise ValueError("layers of scale bytes must not overlap")
+    elif kind not in _TYPES or k_exp is not None or v_exp is not None:
+        raise ValueError("the cache must be bf16 or fp16 without exponents, or float8_e4m3fn with them")
+    row = Hkv * D
+    inner = page * row
+    sizes, want = (page, Hkv, D), (row, D, 1)
+    laid = all(n == 1 or (a == w and b == w) for n, a, b, w in zip(sizes, sk[1:], sv[1:], want))
+    bs_k, bs_v = (inner, inner) if blocks == 1 else (sk[0], sv[0])
+    if (not laid or bs_k < inner or bs_v < inner or (bs_k | bs_v | ls_k | ls_v) % 16
+            or any(ls < inner or (ls < (blocks - 1) * bs + inner and bs < (layers - 1) * ls + inner)
+                   for ls, bs in ((ls_k, bs_k), (ls_v, bs_v)) if layers > 1) or (k_cache.data_ptr() | v_cache.data_ptr()) % 16):
+        raise ValueError("cache blocks must be contiguous [page, Hkv, D], blocks and layers on strides of 16 elements and "
+                         "16-byte boundaries")
+    return _lib.KvPool(k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_exp), _lib.ptr(v_exp), ls_k, ls_v, bs_k, bs_v,
+                       lk, lv, layers, blocks, page, Hkv, D)
+
+
+def _table(block_table, dev):
+    """A block table [S, W] as int32 rows for the device, and their stride."""
+    table = block_table
+    if table.dtype != torch.int32 or table.get_device() != dev:
+        table = _lib.index32(table, dev)
+    S, W = table.shape
+    ld = table.stride(0) if S > 1 else W
+    if (W > 1 and table.stride(1) != 1) or ld < W:
+        table, ld = table.contiguous(), W
+    return table, ld
 
 
 def _rows(t):
@@ -174,3 +231,29 @@ def paged_attention(query, k_cache, v_cache, block_table, seq_lens, cu_q, *, sca
         lens.data_ptr(), cu.data_ptr(), S, float(scale), bool(causal), most, out.data_ptr(), o_ld, lse.data_ptr(), _lib.ptr(ws),
         _lib.ptr(status), fresh, _lib.stream_of(dev)), "cfh_paged_attn")
     return out, lse
+
+
+def kv_cache_commit(k_cache, v_cache, block_table, seq_lens, path, path_len, *, k_exp=None, v_exp=None, status=None) -> None:
+    """The accepted rows of draft trees moved together, in place: sequence s, with seq_lens[s] tokens before its tree's
+    rows, gets node path[s][i]'s row (position seq_lens[s] + path[s][i]) at position seq_lens[s] + i, for i <
+    path_len[s].  ``path`` [S, P] and ``path_len`` [S] are the accept's accepted_path and accepted_len (nodes ascend along a
+    path, as parents come before children).  The cache may be that of several layers, [layers, blocks, page, Hkv, D] (with
+    exponents [layers, blocks, page, Hkv]): all of them in one launch.
+
+    Rows behind the accepted ones keep what they held.  Lengths, tables and paths are read on the device only: a sequence
+    whose path does not ascend or is longer than P, or whose rows do not lie in the table and the cache, is left as it
+    was and sets ``status`` (int32 [1], zeroed by the caller), if given, to 1; path_len below 1 moves nothing.  Sequences
+    must not share the pages they move rows in (``kv_pages_resize`` gives each its own)."""
+    pool = _check_pool(k_cache, v_cache, k_exp, v_exp)
+    if seq_lens.dim() != 1 or path.dim() != 2 or block_table.dim() != 2:
+        raise ValueError("seq_lens must be [S], path [S, P] and block_table [S, blocks]")
+    S, P = path.shape
+    if seq_lens.shape[0] != S or path_len.shape != (S,) or block_table.shape[0] != S:
+        raise ValueError(f"seq_lens and path_len must be [{S}] and block_table [{S}, blocks], as path is [{S}, {P}]")
+    dev = _lib.device_of(k_cache, v_cache, k_exp, v_exp, status=status)
+    table, t_ld = _table(block_table, dev)
+    nodes, p_ld = _table(path, dev)
+    lens, count = _lib.index32(seq_lens, dev), _lib.index32(path_len, dev)
+    _lib.check(_lib.lib().cfh_kv_commit(
+        pool, table.data_ptr(), t_ld, table.shape[1], lens.data_ptr(), nodes.data_ptr(), p_ld, P, count.data_ptr(), S,
+        _lib.ptr(status), _lib.stream_of(dev)), "cfh_kv_commit")

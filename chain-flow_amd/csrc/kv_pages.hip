@@ -1,0 +1,433 @@
+// The pages of the paged key / value cache on MI355X: accepted rows moved together, pages shared between sequences, taken
+// and given back.  A pool's book-keeping is three tensors: table [S][W] (the pages of each sequence, -1: none), room [S]
+// (tokens that a sequence's pages are for: it holds ceil(room / page) of them) and ref [blocks] (sequences that hold a page;
+// 0: free).  Everything is decided on the device, in an order that the sequences give (the lowest free page first), so
+// that a call never synchronises, can be captured, and gives the same table every time.
+#include <type_traits>
+
+#include "cfh_host.h"
+#include "cfh_seq.h"
+
+namespace {
+
+// One part of the cache (keys, values) of all layers, in bytes.
+struct Part { char* p; uint8_t* ex; long long ls, bs, es; };   // base, scale bytes, strides of a layer, a block, a layer's scales
+
+struct PoolArgs {
+  Part part[2];
+  int layers, blocks, page, Hkv;
+  int row;                   // bytes of a token's heads
+  bool f8;
+};
+
+// ---------------------------------------------------------------------------- accepted rows
+// Node path[s][i] of sequence s, row lens[s] + path[s][i], becomes row lens[s] + i, in every layer.  The nodes ascend, so
+// row i never lies behind its source and no source lies before the row in hand: a thread that moves one 16-byte column
+// of all rows in order, whole batches read before they are written, needs no other thread.
+struct CommitArgs {
+  PoolArgs c;
+  const int* table;          // [S][table_ld]
+  const int* lens;           // [S]
+  const int* path;           // [S][path_ld]
+  const int* count;          // [S]
+  int* status;
+  int table_ld, W, path_ld, most;
+};
+
+constexpr int COMMIT_ROWS = 64;   // path entries whose slots lie in LDS at a time
+constexpr int COMMIT_BATCH = 8;   // rows a thread has in flight
+
+__global__ void __launch_bounds__(256) k_commit(CommitArgs a) {
+  __shared__ int src[COMMIT_ROWS], dst[COMMIT_ROWS];
+  __shared__ int bad;
+  const int s = blockIdx.y, n = a.count[s], len = a.lens[s];
+  if (n <= 0) return;                                // nothing accepted, or padding
+  const int* path = a.path + (size_t)s * a.path_ld;
+  const int* table = a.table + (size_t)s * a.table_ld;
+  // the whole path first: ascending nodes whose rows the table holds
+  if (threadIdx.x == 0) bad = n > a.most || len < 0;
+  __syncthreads();
+  const long long limit = (long long)a.W * a.c.page;
+  auto slot_of = [&](long long pos) {                // -1: not in the cache
+    const int blk = pos < limit ? table[pos / a.c.page] : -1;
+    return blk < 0 || blk >= a.c.blocks ? -1 : blk * a.c.page + (int)(pos % a.c.page);
+  };
+  if (!bad)
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const int p = path[i];
+      if (p < (i ? path[i - 1] + 1 : 0) || slot_of((long long)len + p) < 0 || slot_of((long long)len + i) < 0) bad = 1;
+    }
+  __syncthreads();
+  if (bad) {
+    if (threadIdx.x == 0 && a.status) a.status[0] = 1;
+    return;
+  }
+  const int cols = a.c.row / 16, per = cols + (a.c.f8 ? a.c.Hkv : 0);
+  const int item = blockIdx.x * blockDim.x + threadIdx.x, unit = item / per, col = item - unit * per;
+  const bool live = unit < 2 * a.c.layers;
+  const Part q = unit & 1 ? a.c.part[1] : a.c.part[0];
+  const size_t layer = live ? unit >> 1 : 0;
+  for (int i0 = 0; i0 < n; i0 += COMMIT_ROWS) {
+    const int m = min(COMMIT_ROWS, n - i0);
+    __syncthreads();
+    if (threadIdx.x < m) {
+      src[threadIdx.x] = slot_of((long long)len + path[i0 + threadIdx.x]);
+      dst[threadIdx.x] = slot_of((long long)len + i0 + threadIdx.x);
+    }
+    __syncthreads();
+    if (!live) continue;
+    for (int i = 0; i < m; i += COMMIT_BATCH) {
+      if (col < cols) {
+        uint4 x[COMMIT_BATCH];
+        auto at = [&](int slot) {
+          return (uint4*)(q.p + layer * q.ls + (size_t)(slot / a.c.page) * q.bs + (size_t)(slot % a.c.page) * a.c.row) + col;
+        };
+#pragma unroll
+        for (int u = 0; u < COMMIT_BATCH; ++u) x[u] = *at(src[min(i + u, m - 1)]);
+#pragma unroll
+        for (int u = 0; u < COMMIT_BATCH; ++u)
+          if (i + u < m) *at(dst[i + u]) = x[u];
+      } else {
+        uint8_t x[COMMIT_BATCH];
+        auto at = [&](int slot) { return q.ex + layer * q.es + (size_t)slot * a.c.Hkv + (col - cols); };
+#pragma unroll
+        for (int u = 0; u < COMMIT_BATCH; ++u) x[u] = *at(src[min(i + u, m - 1)]);
+#pragma unroll
+        for (int u = 0; u < COMMIT_BATCH; ++u)
+          if (i + u < m) *at(dst[i + u]) = x[u];
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------- fork
+// Row dst[i] of the table lets go of its pages and shares row src[i]'s (src -1: none).  No source is a destination
+// of another pair and destinations differ (pairs that break this are skipped), so that pairs need no order; holders
+// are counted by atomic additions, whose order does not matter.
+struct ForkArgs {
+  int* table;
+  int* room;
+  int* ref;
+  const int* src;            // [n]
+  const int* dst;
+  int* status;
+  int table_ld, W, S, blocks, page, n;
+};
+
+__global__ void __launch_bounds__(256) k_fork(ForkArgs a) {
+  __shared__ int clash;
+  const int i = blockIdx.x, t = threadIdx.x, from = a.src[i], to = a.dst[i];
+  if (to == -1) return;                              // padding
+  if (t == 0) clash = 0;
+  __syncthreads();
+  for (int j = t; j < a.n; j += blockDim.x)
+    if (j != i && (a.dst[j] == to || (from >= 0 && a.dst[j] == from))) clash = 1;
+  __syncthreads();
+  const long long limit = (long long)a.W * a.page;
+  const bool in = to >= 0 && to < a.S && from >= -1 && from < a.S;
+  const int had_room = in ? a.room[to] : -1, new_room = in ? (from >= 0 ? a.room[from] : 0) : -1;
+  if (clash || had_room < 0 || new_room < 0 || had_room > limit || new_room > limit) {
+    if (t == 0 && a.status) a.status[0] = 1;
+    return;
+  }
+  if (from == to) return;
+  int* row = a.table + (size_t)to * a.table_ld;
+  const int* other = a.table + (size_t)max(from, 0) * a.table_ld;
+  const int had = (int)(((long long)had_room + a.page - 1) / a.page), want = (int)(((long long)new_room + a.page - 1) / a.page);
+  for (int j = t; j < max(had, want); j += blockDim.x) {
+    int now = -1;
+    if (j < had) {
+      const int p = row[j];
+      if (p >= 0 && p < a.blocks) atomicSub(&a.ref[p], 1);
+      else if (a.status) a.status[0] = 1;
+    }
+    if (j < want) {
+      now = other[j];
+      if (now >= 0 && now < a.blocks) atomicAdd(&a.ref[now], 1);
+      else if (a.status) a.status[0] = 1;
+    }
+    row[j] = now;
+  }
+  __syncthreads();
+  if (t == 0) a.room[to] = new_room;
+}
+
+// ---------------------------------------------------------------------------- resize
+struct ResizeArgs {
+  PoolArgs c;
+  int* table;
+  int* room;
+  int* ref;
+  const int* new_room;
+  int* status;
+  int4* plan;                // [S]: first place in `fresh` (-1: refused), page to copy (-1: none), pages kept, tokens in the copied one
+  int* fresh;                // pages taken, in order
+  int table_ld, W, S, pieces;
+};
+
+constexpr int RS_MAX = 4096;      // sequences of a call
+constexpr int RS_T = 1024;
+constexpr int RS_FAR = 0x3fffffff; // a place behind every page
+
+// Pages that a sequence has, wants and keeps.
+struct Span { int had, want, kept, part; bool ok, pad; };
+__device__ __forceinline__ Span span_of(const ResizeArgs& a, int s) {
+  const long long limit = (long long)a.W * a.c.page;
+  const int now = a.room[s], want = a.new_room[s];
+  Span x = {};
+  x.pad = want < 0;
+  x.ok = !x.pad && now >= 0 && now <= limit && want <= limit;
+  if (x.ok) {
+    x.had = (int)(((long long)now + a.c.page - 1) / a.c.page);
+    x.want = (int)(((long long)want + a.c.page - 1) / a.c.page);
+    x.kept = min(x.had, x.want);
+    x.part = want > now ? now % a.c.page : 0;
+  }
+  return x;
+}
+
+// First: pages behind the new rooms are let go of.
+__global__ void __launch_bounds__(64) k_release(ResizeArgs a) {
+  const int s = blockIdx.x;
+  const Span x = span_of(a, s);
+  if (!x.ok) {
+    if (!x.pad && threadIdx.x == 0 && a.status) a.status[0] = 1;
+    return;
+  }
+  int* row = a.table + (size_t)s * a.table_ld;
+  for (int j = x.want + (int)threadIdx.x; j < x.had; j += 64) {
+    const int p = row[j];
+    if (p >= 0 && p < a.c.blocks) atomicSub(&a.ref[p], 1);
+    else if (a.status) a.status[0] = 1;
+    row[j] = -1;
+  }
+}
+
+// The sum of v over the threads before this one, and over all of them.
+__device__ __forceinline__ long long scan_before(int v, long long* tmp, long long& all) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  long long run = v;
+  for (int off = 1; off < 64; off <<= 1) {
+    const long long o = __shfl_up(run, off);
+    if (lane >= off) run += o;
+  }
+  __syncthreads();
+  if (lane == 63) tmp[wave] = run;
+  __syncthreads();
+  long long before = 0;
+  all = 0;
+  for (int w = 0; w < RS_T / 64; ++w) {
+    if (w < wave) before += tmp[w];
+    all += tmp[w];
+  }
+  return before + run - v;
+}
+
+// Then, in one workgroup: what each sequence needs, in order, and the lowest free pages for it.  A shared last page
+// that is filled in part is copied before its sequence grows: by all but the last of its holders.
+__global__ void __launch_bounds__(RS_T) k_plan(ResizeArgs a) {
+  __shared__ int tails[RS_MAX];      // the shared page a sequence would write into, -1: none
+  __shared__ long long tmp[RS_T / 64];
+  __shared__ int used;
+  const int t = threadIdx.x;
+  if (t == 0) used = 0;
+  for (int s = t; s < a.S; s += RS_T) {
+    const Span x = span_of(a, s);
+    int tail = -1;
+    if (x.ok && x.part) {
+      tail = a.table[(size_t)s * a.table_ld + x.kept - 1];
+      if (tail < 0 || tail >= a.c.blocks) {
+        if (a.status) a.status[0] = 1;
+        tail = -2;                                   // no such page: refused
+      } else if (a.ref[tail] <= 1) {
+        tail = -1;
+      }
+    }
+    tails[s] = tail;
+  }
+  __syncthreads();
+  long long total = 0;                               // (what is asked for may pass 32 bits; what is free does not)
+  for (int s0 = 0; s0 < a.S; s0 += RS_T) {
+    const int s = s0 + t;
+    int need = 0, tail = -1;
+    Span x = {};
+    if (s < a.S) {
+      x = span_of(a, s);
+      tail = tails[s];
+      if (tail == -2) x.ok = false;
+      if (x.ok) need = x.want - x.kept;
+      if (x.ok && tail >= 0) {
+        int before = 0;
+        for (int j = 0; j < s; ++j) before += tails[j] == tail;
+        if (a.ref[tail] - before > 1) ++need;
+      }
+    }
+    long long all;
+    const int at = (int)min(total + scan_before(need, tmp, all), (long long)RS_FAR);
+    if (s < a.S) {
+      const bool copied = x.ok && need > x.want - x.kept;
+      // (-2: keeps its shared page, if those before it copied it)
+      a.plan[s] = make_int4(x.ok ? at : -1, copied ? tail : x.ok && tail >= 0 ? -2 : -1, x.kept, x.part);
+    }
+    total += all;
+  }
+  // the lowest free pages
+  long long base = 0;
+  for (int p0 = 0; p0 < a.c.blocks && base < total; p0 += 4 * RS_T) {
+    int is[4], n = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int p = p0 + 4 * t + e;
+      is[e] = p < a.c.blocks && a.ref[p] == 0;
+      n += is[e];
+    }
+    long long all, at = base + scan_before(n, tmp, all);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (is[e]) {
+        if (at < total) a.fresh[at] = p0 + 4 * t + e;
+        ++at;
+      }
+    base += all;
+  }
+  const int have = (int)min(base, total);
+  __syncthreads();
+  for (int s = t; s < a.S; s += RS_T) {
+    int4 p = a.plan[s];
+    if (p.x < 0) continue;
+    const Span x = span_of(a, s);
+    const int need = x.want - x.kept + (p.y >= 0);
+    if ((need > 0 || p.y == -2) && p.x + need > have) {
+      a.plan[s].x = -1;
+      if (a.status) a.status[0] = 1;
+      continue;
+    }
+    if (p.y >= 0) atomicSub(&a.ref[p.y], 1);
+    if (need > 0) atomicMax(&used, p.x + need);
+  }
+  __syncthreads();
+  for (int i = t; i < min(used, have); i += RS_T) a.ref[a.fresh[i]] = 1;
+}
+
+// Last: tables and rooms (y = 0), and the copies, a piece of a page of one layer's keys or values each.
+constexpr int PIECE = 16384;
+
+__global__ void __launch_bounds__(256) k_fill(ResizeArgs a) {
+  const int s = blockIdx.x, t = threadIdx.x;
+  const int4 p = a.plan[s];
+  if (p.x < 0) return;
+  if (blockIdx.y == 0) {
+    const int want = (int)(((long long)a.new_room[s] + a.c.page - 1) / a.c.page), j0 = p.z - (p.y >= 0);
+    for (int j = j0 + t; j < want; j += 256) a.table[(size_t)s * a.table_ld + j] = a.fresh[p.x + j - j0];
+    if (t == 0) a.room[s] = a.new_room[s];
+    return;
+  }
+  if (p.y < 0) return;
+  const int unit = (blockIdx.y - 1) / a.pieces, piece = (blockIdx.y - 1) % a.pieces;
+  const Part q = unit & 1 ? a.c.part[1] : a.c.part[0];
+  const size_t layer = unit >> 1;
+  const int to = a.fresh[p.x], bytes = p.w * a.c.row;
+  const char* src = q.p + layer * q.ls + (size_t)p.y * q.bs;
+  char* dst = q.p + layer * q.ls + (size_t)to * q.bs;
+  for (int o = piece * PIECE + t * 16; o < min(bytes, (piece + 1) * PIECE); o += 256 * 16) *(uint4*)(dst + o) = *(const uint4*)(src + o);
+  if (a.c.f8 && piece == 0) {
+    const size_t per = (size_t)a.c.page * a.c.Hkv;
+    const uint8_t* es = q.ex + layer * q.es + p.y * per;
+    uint8_t* ed = q.ex + layer * q.es + to * per;
+    for (int o = t; o < p.w * a.c.Hkv; o += 256) ed[o] = es[o];
+  }
+}
+
+int pool_of(const cfh_kv_pool* c, PoolArgs& a) {
+  if (!c || c->layers < 1 || c->blocks < 1 || c->page < 1 || c->heads < 1) return CFH_E_INVALID;
+  if ((c->dim != 64 && c->dim != 128 && c->dim != 256) || (long long)c->blocks * c->page > 0x7fffffffll ||
+      (long long)c->page * c->heads * c->dim > 0x3fffffffll)
+    return CFH_E_UNSUPPORTED;
+  const bool f8 = c->k_exp || c->v_exp;
+  const int es = f8 ? 1 : 2;
+  const long long inner = (long long)c->page * c->heads * c->dim, scales = (long long)c->blocks * c->page * c->heads;
+  if (!c->k || !c->v || (f8 && (!c->k_exp || !c->v_exp)) || ((uintptr_t)c->k | (uintptr_t)c->v) % 16) return CFH_E_INVALID;
+  const void* base[2] = {c->k, c->v};
+  uint8_t* ex[2] = {c->k_exp, c->v_exp};
+  const long long ls[2] = {c->ls_k, c->ls_v}, bs[2] = {c->bs_k, c->bs_v}, xs[2] = {c->ls_k_exp, c->ls_v_exp};
+  for (int i = 0; i < 2; ++i) {
+    if (bs[i] < inner || bs[i] % 16) return CFH_E_INVALID;
+    // layers around the blocks, or blocks around the layers
+    if (c->layers > 1 && (ls[i] < inner || ls[i] % 16 || (ls[i] < (c->blocks - 1) * bs[i] + inner && bs[i] < (c->layers - 1) * ls[i] + inner) ||
+                          (f8 && xs[i] < scales)))
+      return CFH_E_INVALID;
+    a.part[i] = {(char*)base[i], ex[i], ls[i] * es, bs[i] * es, xs[i]};
+  }
+  a.layers = c->layers; a.blocks = c->blocks; a.page = c->page; a.Hkv = c->heads; a.row = c->heads * c->dim * es; a.f8 = f8;
+  return CFH_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int cfh_kv_commit(const cfh_kv_pool* pool, const int32_t* table, int table_ld, int max_blocks, const int32_t* seq_lens,
+                  const int32_t* path, int path_ld, int max_path, const int32_t* path_len, int S, int32_t* status,
+                  void* stream) {
+  CommitArgs a = {};
+  if (int rc = pool_of(pool, a.c)) return rc;
+  if (S < 0 || max_path < 0 || max_blocks < 0) return CFH_E_INVALID;
+  if (S == 0 || max_path == 0) return CFH_OK;
+  if (!table || !seq_lens || !path || !path_len || table_ld < max_blocks || path_ld < max_path) return CFH_E_INVALID;
+  if (S > 65535) return CFH_E_UNSUPPORTED;
+  a.table = table; a.lens = seq_lens; a.path = path; a.count = path_len; a.status = status;
+  a.table_ld = table_ld; a.W = max_blocks; a.path_ld = path_ld; a.most = max_path;
+  const long long items = 2ll * a.c.layers * (a.c.row / 16 + (a.c.f8 ? a.c.Hkv : 0));
+  if (items > 0x3fffffffll) return CFH_E_UNSUPPORTED;
+  hipLaunchKernelGGL(k_commit, dim3((unsigned)((items + 255) / 256), S), dim3(256), 0, (hipStream_t)stream, a);
+  CFH_LAUNCH_CHECK();
+  return CFH_OK;
+}
+
+int cfh_kv_fork(int32_t* table, int table_ld, int max_blocks, int32_t* room, int S, int32_t* ref, int blocks, int page,
+                const int32_t* src, const int32_t* dst, int n, int32_t* status, void* stream) {
+  if (n < 0 || S < 0 || blocks < 1 || page < 1 || max_blocks < 0 || table_ld < max_blocks) return CFH_E_INVALID;
+  if (max_blocks > RS_FAR || (long long)max_blocks * page > 0x7fffffffll) return CFH_E_UNSUPPORTED;
+  if (n == 0) return CFH_OK;
+  if (!table || !room || !ref || !src || !dst) return CFH_E_INVALID;
+  if (n > 65535) return CFH_E_UNSUPPORTED;
+  ForkArgs a = {table, room, ref, src, dst, status, table_ld, max_blocks, S, blocks, page, n};
+  hipLaunchKernelGGL(k_fork, dim3(n), dim3(256), 0, (hipStream_t)stream, a);
+  CFH_LAUNCH_CHECK();
+  return CFH_OK;
+}
+
+int64_t cfh_kv_resize_ws_bytes(int S, int max_blocks, int blocks) {
+  if (S < 0 || max_blocks < 0 || blocks < 1) return -1;
+  return 16ll * S + 4 * std::min((long long)blocks, (long long)S * max_blocks);
+}
+
+int cfh_kv_resize(const cfh_kv_pool* pool, int32_t* table, int table_ld, int max_blocks, int32_t* room, int S, int32_t* ref,
+                  int blocks, int page, const int32_t* new_room, void* ws, int32_t* status, void* stream) {
+  ResizeArgs a = {};
+  if (pool) {
+    if (int rc = pool_of(pool, a.c)) return rc;
+    if (a.c.blocks != blocks || a.c.page != page) return CFH_E_INVALID;
+  }
+  if (S < 0 || blocks < 1 || page < 1 || max_blocks < 0 || table_ld < max_blocks) return CFH_E_INVALID;
+  if (S == 0) return CFH_OK;
+  if (!table || !room || !ref || !new_room || !ws || (uintptr_t)ws % 16) return CFH_E_INVALID;
+  if (S > RS_MAX || max_blocks > RS_FAR || blocks > RS_FAR || (long long)max_blocks * page > 0x7fffffffll) return CFH_E_UNSUPPORTED;
+  a.c.blocks = blocks; a.c.page = page;
+  a.table = table; a.room = room; a.ref = ref; a.new_room = new_room; a.status = status;
+  a.plan = (int4*)ws; a.fresh = (int*)(a.plan + S);
+  a.table_ld = table_ld; a.W = max_blocks; a.S = S;
+  a.pieces = pool ? (int)(((long long)page * a.c.row + PIECE - 1) / PIECE) : 0;
+  const long long copies = 2ll * a.c.layers * a.pieces;
+  if (copies > 65534) return CFH_E_UNSUPPORTED;
+  hipStream_t st = (hipStream_t)stream;
+  hipLaunchKernelGGL(k_release, dim3(S), dim3(64), 0, st, a);
+  CFH_LAUNCH_CHECK();
+  hipLaunchKernelGGL(k_plan, dim3(1), dim3(RS_T), 0, st, a);
+  CFH_LAUNCH_CHECK();
+  hipLaunchKernelGGL(k_fill, dim3(S, (unsigned)(1 + copies)), dim3(256), 0, st, a);
+  CFH_LAUNCH_CHECK();
+  return CFH_OK;
+}
+
+}  // extern "C"

@@ -560,6 +560,49 @@ int cfh_paged_attn_fresh(const void* q, long long q_ld, int T, int H, int Hkv, i
                          float scale, int causal, int max_len, void* out, long long o_ld, float* lse, void* ws,
                          int32_t* status, int out_too, void* stream);
 
+/* ---------------------------------------------------------------- the committed prefix: the cache's pages
+ * The caches of all attention layers, on one block table: keys k, values v [layers][blocks][page][heads][dim] as the
+ * single cache above (2-byte elements, or e4m3 with both k_exp and v_exp [layers][blocks][page][heads]); strides of a layer
+ * (ls, unused where there is one layer) and a block (bs) in elements, multiples of 16, of a layer's scales (ls_exp) in bytes. */
+typedef struct cfh_kv_pool {
+  void *k, *v;
+  uint8_t *k_exp, *v_exp;
+  long long ls_k, ls_v, bs_k, bs_v, ls_k_exp, ls_v_exp;
+  int layers, blocks, page, heads, dim;
+} cfh_kv_pool;
+
+/* The accepted rows of a draft tree moved together, in every layer: sequence s, with seq_lens[s] tokens before the tree's
+ * rows, has node path[s][i]'s row (position seq_lens[s] + path[s][i]) moved to position seq_lens[s] + i, i < path_len[s].
+ * table [S][table_ld] (max_blocks usable), path [S][path_ld] (max_path usable): what the accept calls return.  Nodes
+ * ascend.  path_len below 1: nothing to do.  A path that does not ascend or is longer than max_path, and rows outside the
+ * table or the cache: the sequence is left as it was and status[0] set to 1 (status: one int32 the caller zeroes, or NULL).
+ * Sequences must not share the pages they move rows in. */
+int cfh_kv_commit(const cfh_kv_pool* pool, const int32_t* table, int table_ld, int max_blocks, const int32_t* seq_lens,
+                  const int32_t* path, int path_ld, int max_path, const int32_t* path_len, int S, int32_t* status,
+                  void* stream);
+
+/* Book-keeping of pages: table [S][table_ld] (max_blocks usable) holds each sequence's pages (-1: none), room [S] the tokens
+ * they are for (a sequence holds the first ceil(room / page) entries of its row), ref [blocks] how many sequences hold a
+ * page (0: free).  All three are updated in place, on the device.
+ *
+ * cfh_kv_fork: for each i < n, sequence dst[i] lets go of its pages and shares those of sequence src[i] (-1: holds none),
+ * with its room.  dst -1: padding.  Destinations must differ, and no source may be another pair's destination: such pairs,
+ * and ones whose sequences or rooms do not lie in the table, are skipped and set status.  Entries that are no page of the
+ * cache set status and count for none.
+ *
+ * cfh_kv_resize: every sequence gets the pages for new_room[s] tokens (negative: left as it is): pages behind are let go of,
+ * missing ones taken, the lowest free ones first, in order of the sequences and of their places.  Where a sequence grows
+ * and its last page is filled in part (room % page) and shared, all but the last of the growing holders that could not
+ * keep it get a copy of its own: pool (NULL: no copies, only the book-keeping; else its blocks and page are these) says
+ * where the rows lie.  Where the free pages end, that sequence and all behind it that need one are left as they were
+ * (status), as are ones whose rooms do not lie in the table.  S <= 4096.  ws: cfh_kv_resize_ws_bytes(S,
+ * max_blocks, blocks) bytes, 16-byte aligned, of the call's own until it ends. */
+int cfh_kv_fork(int32_t* table, int table_ld, int max_blocks, int32_t* room, int S, int32_t* ref, int blocks, int page,
+                const int32_t* src, const int32_t* dst, int n, int32_t* status, void* stream);
+int64_t cfh_kv_resize_ws_bytes(int S, int max_blocks, int blocks);
+int cfh_kv_resize(const cfh_kv_pool* pool, int32_t* table, int table_ld, int max_blocks, int32_t* room, int S, int32_t* ref,
+                  int blocks, int page, const int32_t* new_room, void* ws, int32_t* status, void* stream);
+
 /* ---------------------------------------------------------------- the committed prefix: recurrent state
  * The gated delta rule over committed tokens, in the layout of cfh_gdn_tree_vllm (mixed_qkv, a, b, A_log,
  * dt_bias, gates, normalisation, scale, ssm_state [nslots][HV][V][K] bf16 or fp32), each sequence from and
