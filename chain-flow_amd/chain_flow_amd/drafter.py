@@ -15,7 +15,7 @@ import torch
 from chain_flow_amd import _lib
 from chain_flow_amd.config import TreeFlowConfig, TreeVAEFlowConfig
 from chain_flow_amd.flow import FusedFlow
-from chain_flow_amd.head import GEMV_ROWS, PathHead, ShortlistHead, row_topk
+from chain_flow_amd.head import GEMV_ROWS, PathHead, QuantHead, ShortlistHead, row_topk
 from chain_flow_amd.vae import HiddenVAE
 
 
@@ -34,11 +34,18 @@ class Drafter:
     (``cf/vllm_plugin/flow_proposer.py:1113-1184``): one head pass over the marginal hiddens of every
     depth picks M shortlist rows (``twopass_shared``: one set for all depths, else one per depth;
     ``twopass_seed``: scored with the seed path's residual and markov bias), and each depth
-    rescores only those rows, renormalised over them."""
+    rescores only those rows, renormalised over them.
+
+    ``head_bits`` = 4 holds the head (shortlisted lm_head and markov.w2) at 4 bits with a scale for each ``head_group``
+    columns (``QuantHead``: a quarter of the bytes a depth reads); its search is the one-pass one."""
 
     def __init__(self, cfg: TreeFlowConfig, weights: dict, shortlist: torch.Tensor | None, device="cuda",
                  path_trim: bool = True, twopass_m: int = 0, twopass_shared: bool = True,
-                 twopass_seed: bool = False):
+                 twopass_seed: bool = False, head_bits: int = 16, head_group: int = 64):
+        if head_bits not in (4, 16):
+            raise ValueError(f"head_bits={head_bits} is not 16 or 4")
+        if head_bits == 4 and twopass_m:
+            raise ValueError("the two-pass candidate head gathers fp16 rows: a head of 4 bits is searched in one pass")
         self.cfg = cfg
         dev = torch.device(device)
         if dev.type == "cuda" and dev.index is None:
@@ -55,8 +62,9 @@ class Drafter:
         self.flow = FusedFlow(cfg, weights, device=dev)
         self.path = PathHead(weights, weights["embed_tokens.weight"], cfg.path_order,
                              cfg.path_ffn_multiplier, dev)
-        self.head = ShortlistHead(weights["lm_head.weight"].to(dev, torch.float16), shortlist,
-                                  weights["markov.w1.weight"], weights["markov.w2.weight"])
+        head = (weights["lm_head.weight"].to(dev, torch.float16), shortlist, weights["markov.w1.weight"],
+                weights["markov.w2.weight"])
+        self.head = ShortlistHead(*head) if head_bits == 16 else QuantHead(*head, group=head_group)
         self.order = cfg.path_order
         if twopass_m and not 0 < twopass_m < self.head.n:
             raise ValueError(f"two-pass M={twopass_m} must be below the head's {self.head.n} rows")

@@ -408,6 +408,127 @@ def row_topk(logits: torch.Tensor, k: int):
     return vals, ids, lse
 
 
+def quantize4(w: torch.Tensor, group: int = 64, rows: torch.Tensor | None = None, w2: torch.Tensor | None = None):
+    """fp16 weights [V, d] (the columns of ``w2`` [V, r] behind theirs, if given; only ``rows`` [n], if given) at 4 bits ->
+    (weight uint8 [n, (d + r) / 2], scale fp16 [n, (d + r) / group]).
+
+    A byte holds two columns, the even one in its low half, as whole numbers 0 .. 15 that stand for themselves less 8.  A
+    scale is the least fp16 value whose seven reach the largest magnitude of its ``group`` (32, 64 or 128) columns, so that no
+    weight is off by more than half a scale; a group with a NaN or an infinity has a NaN scale.  d and r must be
+    multiples of ``group``, d + r of 128."""
+    if group not in (32, 64, 128):
+        raise ValueError(f"group {group} is not 32, 64 or 128")
+    for t in (w, w2):
+        if t is not None and (t.dtype != torch.float16 or t.dim() != 2 or not t.numel()):
+            raise ValueError("weights must be fp16 [V, d]")
+    V, d = w.shape
+    r = 0 if w2 is None else w2.shape[1]
+    if (w2 is not None and w2.shape[0] != V) or d % group or r % group or (d + r) % 128:
+        raise ValueError(f"{d} and {r} columns must be multiples of the group of {group} together of 128, with as many rows")
+    dev = _lib.device_of(w, w2)
+    if rows is not None:
+        if rows.dim() != 1 or (rows.numel() and (int(rows.min()) < 0 or int(rows.max()) >= V)):
+            raise ValueError(f"rows must be [n] of the {V} weight rows")
+        rows = _lib.index32(rows, dev)
+    n = V if rows is None else rows.shape[0]
+    w = _lib.aligned(w.contiguous())
+    w2 = None if w2 is None else _lib.aligned(w2.contiguous())
+    weight = torch.empty(n, (d + r) // 2, dtype=torch.uint8, device=w.device)
+    scale = torch.empty(n, (d + r) // group, dtype=torch.float16, device=w.device)
+    _lib.check(_lib.lib().cfh_quantize4(w.data_ptr(), _lib.ptr(w2), _lib.ptr(rows), n, d, r, group, weight.data_ptr(),
+                                        scale.data_ptr(), _lib.stream_of(dev)), "cfh_quantize4")
+    return weight, scale
+
+
+def matvec4(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, *, table: torch.Tensor | None = None,
+            ids: torch.Tensor | None = None, ids_stride: int = 1, out: torch.Tensor | None = None) -> torch.Tensor:
+    """fp16(x @ w.T) [M, n] of fp16 rows x [M, d] (rows may be strided) with 4-bit weights as ``quantize4`` makes them: weight
+    uint8 [n, K / 2], scale fp16 [n, K / group], K a multiple of 128, the group of 32, 64 or 128 columns being K over the
+    scales' columns.  Products and sums are fp32.  The weights are read once for up to 16 rows.
+
+    With ``table`` [V, r] fp16 and ``ids`` (int32; row m's at m * ids_stride), row ids[m] of the table (outside it: the nearest)
+    stands behind x's d columns, d + r = K."""
+    if x.dtype != torch.float16 or x.dim() != 2 or weight.dtype != torch.uint8 or weight.dim() != 2 or \
+            scale.dtype != torch.float16 or scale.dim() != 2:
+        raise ValueError("x must be fp16 [M, d], weight uint8 [n, K / 2] and scale fp16 [n, K / group]")
+    M, d = x.shape
+    n, K = weight.shape[0], 2 * weight.shape[1]
+    groups = scale.shape[1]
+    if scale.shape[0] != n or not groups or K % groups or K // groups not in (32, 64, 128) or K % 128 or K > 65536:
+        raise ValueError(f"scale {tuple(scale.shape)} must be [{n}, {K} / 32, 64 or 128], and {K} columns a multiple of 128 up to 65,536")
+    r = 0
+    if (table is None) != (ids is None):
+        raise ValueError("table and ids go together")
+    if table is not None:
+        if table.dtype != torch.float16 or table.dim() != 2 or not table.numel() or ids.dtype != torch.int32 or ids.dim() != 1 or \
+                ids_stride < 1 or ids.shape[0] < (M - 1) * ids_stride + 1:
+            raise ValueError("table must be fp16 [V, r] and ids int32 with one for each row")
+        r = table.shape[1]
+    if d + r != K or d % 8:
+        raise ValueError(f"x has {d} columns, the table {r}: the weights take {K}, and x's must be a multiple of 8")
+    dev = _lib.device_of(x, weight, scale, table, ids)
+    ld_x = x.stride(0) if M > 1 else d
+    if x.stride(1) != 1 or ld_x < d or ld_x % 8 or x.data_ptr() % 16:
+        x, ld_x = _lib.aligned(x.contiguous()), d
+    if not weight.is_contiguous() or weight.data_ptr() % 16:
+        weight = _lib.aligned(weight.contiguous())
+    if not scale.is_contiguous() or scale.data_ptr() % 16:
+        scale = _lib.aligned(scale.contiguous())
+    if table is not None:
+        table, ids = _lib.aligned(table.contiguous()), ids.contiguous()
+    if out is None:
+        out = x.new_empty((M, n))
+    elif out.shape != (M, n) or out.dtype != torch.float16 or out.get_device() != dev or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous fp16 [{M}, {n}] tensor on cuda:{dev}")
+    _lib.check(_lib.lib().cfh_matvec4(
+        x.data_ptr(), ld_x, M, d, weight.data_ptr(), K // 2, scale.data_ptr(), groups, K // groups, n, _lib.ptr(table),
+        0 if table is None else table.shape[0], _lib.ptr(ids), ids_stride, r, out.data_ptr(), n, _lib.stream_of(dev)),
+        "cfh_matvec4")
+    return out
+
+
+class QuantHead:
+    """``ShortlistHead`` at 4 bits: the shortlisted rows of lm_head and, behind their columns, of markov.w2 as ``quantize4``
+    weights (174 MB for 62,642 rows at d = 5120, r = 256, groups of 64, against 673 MB), so that a row's logit is one product
+    of [h, w1[prev]] and is rounded once.  The drafts it makes differ from the fp16 head's; what the target's verify
+    accepts of them is distributed as before."""
+
+    def __init__(self, lm_w: torch.Tensor, shortlist: torch.Tensor | None, w1: torch.Tensor | None = None,
+                 w2: torch.Tensor | None = None, group: int = 64):
+        if lm_w.dtype != torch.float16 or not lm_w.is_cuda:
+            raise ValueError("lm_w must be a CUDA fp16 [V, d] tensor")
+        if (w1 is None) != (w2 is None):
+            raise ValueError("markov w1 and w2 go together")
+        self.V, self.d = lm_w.shape
+        self.sl = None if shortlist is None else _i32(shortlist.to(lm_w.device))
+        self.w1 = None if w1 is None else w1.to(lm_w.device, torch.float16).contiguous()
+        self.r = 0 if w1 is None else int(self.w1.shape[1])
+        self.weight, self.scale = quantize4(lm_w, group, self.sl, None if w2 is None else w2.to(lm_w.device, torch.float16))
+        self.n = self.weight.shape[0]
+        self.group = group
+        self.image = None
+        self._zero = None
+
+    map = ShortlistHead.map
+
+    def logits(self, h: torch.Tensor, prev: torch.Tensor | None = None, prev_stride: int = 1,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+        """h [M, d] fp16, prev (global ids) -> fp16 logits [M, n] (head + markov bias; without ``prev`` the head's alone)."""
+        if self.w1 is None:
+            return matvec4(h, self.weight, self.scale, out=out)
+        if prev is None:                       # a row of zeros for the markov columns
+            if self._zero is None:
+                self._zero = torch.zeros(1, self.r, dtype=torch.float16, device=h.device)
+            return matvec4(h, self.weight, self.scale, table=self._zero, out=out,
+                           ids=torch.zeros(h.shape[0], dtype=torch.int32, device=h.device))
+        return matvec4(h, self.weight, self.scale, table=self.w1, ids=prev.reshape(-1).to(torch.int32), ids_stride=prev_stride, out=out)
+
+    def topk(self, h: torch.Tensor, k: int, prev: torch.Tensor | None = None, prev_stride: int = 1,
+             logits: torch.Tensor | None = None):
+        """-> (log-prob values [M, k] f32, shortlist-local ids [M, k] int32, lse [M] f32), as ``ShortlistHead.topk``."""
+        return row_topk(self.logits(h, prev, prev_stride, logits), k)
+
+
 def pack_linear(w: torch.Tensor) -> torch.Tensor:
     """Row-major [n, k] 2-byte weight -> MFMA tile order (same shape, new storage)."""
     w = w.contiguous()

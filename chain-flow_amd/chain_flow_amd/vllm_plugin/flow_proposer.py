@@ -17,7 +17,8 @@ Mirrors ``chain_flow.vllm_plugin.flow_proposer.FlowDrafterProposer`` (``cf/vllm_
   ``:2326-2357``);
 * the head is the two-pass candidate head by default (``CF_TWOPASS_M=8192``, ``CF_TWOPASS_SHARED=1``,
   ``CF_TWOPASS_SEED=0``; ``:1113-1184``, ``cf/defaults.py:123-127``), dropped when M does not fit
-  the head unless it was asked for;
+  the head unless it was asked for; ``CF_HEAD_BITS=4`` (16) holds the head at 4 bits and searches it
+  in one pass;
 * the context lives in a device ring per batch slot (``_ring_write`` / ``_ring_gather``,
   ``:916-961``; ``cfh_ring_step``), with the slot lifecycle of ``_ctx_gpu`` (``:2045-2105``: a new
   request resets or seeds its slot, a request moved by vLLM's batch condense carries its history),
@@ -229,6 +230,13 @@ class FlowDrafterProposer:
         self.twopass_m = int(os.environ.get("CF_TWOPASS_M", "8192") or 0)
         self.twopass_shared = os.environ.get("CF_TWOPASS_SHARED", "1") == "1"
         self.twopass_seed = os.environ.get("CF_TWOPASS_SEED", "0") == "1"
+        self.head_bits = int(os.environ.get("CF_HEAD_BITS", "16") or 16)
+        if self.head_bits not in (4, 16):
+            raise ValueError(f"CF_HEAD_BITS={self.head_bits} is not 16 or 4")
+        if self.head_bits == 4:
+            if self._twopass_explicit and self.twopass_m:
+                raise ValueError("CF_HEAD_BITS=4 searches the head in one pass: it does not go with CF_TWOPASS_M")
+            self.twopass_m = 0
         self.async_spec = os.environ.get("CF_ASYNC_SPEC", "0") == "1"
         self.drafter: Drafter | None = None
         self._target = None
@@ -294,7 +302,8 @@ class FlowDrafterProposer:
             self.twopass_m, self.twopass_shared = 0, False
         self.drafter = Drafter(cfg, weights, None if sl is None else sl.to(self.dev), device=self.dev,
                                path_trim=self.path_trim, twopass_m=self.twopass_m,
-                               twopass_shared=self.twopass_shared, twopass_seed=self.twopass_seed)
+                               twopass_shared=self.twopass_shared, twopass_seed=self.twopass_seed,
+                               head_bits=self.head_bits)
         self.ctx_size = cfg.context_size
         # rows one request can append per step: the committed token plus every accepted draft
         self.kmax = (self.tree_depth + 1) if self.branching else (self.K + 1)

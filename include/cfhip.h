@@ -273,6 +273,24 @@ int cfh_head_logits(const void* h, int M, int d, const void* W, const int32_t* s
 int cfh_row_topk(const void* logits, int M, int n, int k, float* vals, int32_t* ids, float* lse,
                  void* stream);
 
+/* The head at 4 bits.  Weight rows w [n][ld_w bytes]: column 2 i in the low half of byte i, column 2 i + 1 in its high half, as
+ * whole numbers 0 .. 15 that stand for themselves less 8; scale [n][ld_s] fp16, one for `group` (32, 64 or 128) columns.
+ *
+ * cfh_quantize4: fp16 rows w [.][d], their columns followed by w2 [.][r]'s (r = 0: none), taken through rows [n] (NULL: as they
+ * are), into q [n][(d + r) / 2] and scale [n][(d + r) / group]: the least fp16 scale whose seven reach the group's
+ * largest magnitude, weights rounded to nearest even, off by half a scale at most.  A group with a NaN or an infinity has a NaN
+ * scale.  d and r multiples of group, d + r of 128.
+ *
+ * cfh_matvec4: y[m][j] = fp16(sum over the K = d + r columns of scale * (w[j][k] - 8) * x[m][k]), sums in fp32; x [M][ld_x] fp16
+ * holds the first d columns, the r behind them are row a_ids[m * a_ids_stride] (below 0 and past a_rows: the nearest) of a
+ * [a_rows][r] (r = 0: none).  Any M; K a multiple of 128, at most 65,536, d and r of 8; the weights are read once for up to 16
+ * rows.  x, w, a 16-byte aligned, ld_x a multiple of 8, ld_w of 16; scale aligned to 256 / group bytes, ld_s a multiple of 128 / group. */
+int cfh_quantize4(const void* w, const void* w2, const int32_t* rows, int n, int d, int r, int group, uint8_t* q, void* scale,
+                  void* stream);
+int cfh_matvec4(const void* x, long long ld_x, int M, int d, const uint8_t* w, int ld_w, const void* scale, int ld_s, int group,
+                int n, const void* a, int a_rows, const int32_t* a_ids, int a_ids_stride, int r, void* y, long long ld_y,
+                void* stream);
+
 /* Bytes of the candidate workspace `ws` that cfh_head_topk / cfh_head_gemm_topk need for M rows,
  * n shortlist columns and top-k (-1 if out of range). */
 int64_t cfh_head_ws_bytes(int M, int n, int k);

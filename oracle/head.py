@@ -79,3 +79,26 @@ def margins(x, k):
     up = np.concatenate([np.full(v.shape[:-1] + (1,), np.inf), v[..., :-2] - v[..., 1:-1]], -1)
     dn = v[..., :-1] - v[..., 1:]
     return np.minimum(up[..., :k], dn[..., :k])
+
+
+def quantize4(w, group):
+    """w [n, K] float64 (fp16 values) -> (whole numbers [n, K] in 0 .. 15 that stand for themselves less 8, scales [n,
+    K / group]): the least fp16 scale whose seven reach the group's largest magnitude, weights to nearest even."""
+    w = np.asarray(w, dtype=np.float64)
+    g = w.reshape(len(w), -1, group)
+    most = np.abs(g).max(-1)
+    s = (most / 7).astype(np.float16)
+    up = np.nextafter(s, np.float16(np.inf))
+    s = np.where(s.astype(np.float64) * 7 < most, up, s).astype(np.float64)
+    q = np.rint(np.divide(g, s[..., None], out=np.zeros_like(g), where=s[..., None] > 0))
+    return (np.clip(q, -7, 7) + 8).reshape(w.shape).astype(np.int64), s
+
+
+def dequant4(q, s):
+    """The weights that whole numbers and scales stand for, float64."""
+    return (q - 8.0) * np.repeat(s, q.shape[1] // s.shape[1], 1)
+
+
+def unpack4(b):
+    """Bytes [n, K / 2] -> whole numbers [n, K], the even column in a byte's low half."""
+    return np.stack([b & 15, b >> 4], -1).reshape(len(b), -1).astype(np.int64)
