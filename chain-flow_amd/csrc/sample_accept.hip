@@ -26,9 +26,7 @@
 
 namespace {
 
-constexpr int SA_T = 1024, SA_W = SA_T / 64;   // threads and waves of a row
-constexpr int SA_GROUPS = 65536 / (4 * SA_T);  // groups of 4 values a thread: 16
-constexpr int SA_CELLS = SA_GROUPS * SA_W;     // (group, wave): 256 values each, in the order's order
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
 
 struct SampleArgs {
   const u16* logits;
@@ -43,59 +41,84 @@ struct SampleArgs {
   float* lp;                 // [R]
 };
 
-// Order-preserving 16-bit key of a logit (-0 as 0); -1: no token (NaN, -inf).
+// Order position o of a 16-bit value: 0 the largest NaN pattern of a positive sign, then descending, +0 at 32,767, -0 behind it.
+__device__ __forceinline__ int raw_of(int o) { return o < 0x8000 ? 0x7fff - o : o; }
 template <bool BF>
-__device__ __forceinline__ int key_of(unsigned x) {
-  constexpr unsigned INF = BF ? 0x7f80u : 0x7c00u;
-  const unsigned mag = x & 0x7fffu;
-  if (mag > INF || x == (0x8000u | INF)) return -1;
-  if (mag == 0) return 0x8000;
-  return (int)(x & 0x8000u ? 0xffffu - x : x | 0x8000u);
-}
-template <bool BF>
-__device__ __forceinline__ double value_of(int key) {
-  const unsigned x = key & 0x8000 ? key & 0x7fffu : 0xffffu - (unsigned)key;
+__device__ __forceinline__ double value_of(int o) {
+  const unsigned x = (unsigned)raw_of(o);
   if constexpr (BF) return (double)__uint_as_float(x << 16);
   else return (double)__builtin_bit_cast(_Float16, (u16)x);
 }
+// Positions of numbers above -inf: the first and the last.
+template <bool BF> constexpr int O_FIRST = 0x7fff - (BF ? 0x7f80 : 0x7c00);
+template <bool BF> constexpr int O_LAST = 0x8000 + (BF ? 0x7f80 : 0x7c00) - 1;
 
-__device__ __forceinline__ double shfl_up_d(double v, int d) { return __shfl_up(v, d); }
-
-// What a row's searches share.
-struct Row {
-  double m, T;
-  int key_max;
-  bool wide;                 // 32-bit counts of one half of the values at a time (see k_sample_rows)
-};
-
-// The weight of a value: 1 at the largest, nothing else beside an infinite one.
-template <bool BF>
-__device__ __forceinline__ double weight_of(const Row& r, int key) {
-  if (key == r.key_max) return 1.0;
-  if (isinf(r.m)) return 0.0;
-  return exp((value_of<BF>(key) - r.m) / r.T);
+// 2^t in 64 bits, t <= 0: t = q / 32 + g, 2^(q / 32) by exponent and a table of 32, 2^g by the exponential series to the 6th power
+// (its next term is below 4e-18 for |g| <= 1 / 64).  0 from 2^-1100 on.
+__device__ __forceinline__ double pow2(const double* table, double t) {
+  t = fmax(t, -1100.0);
+  const double q = rint(t * 32.0), z = fma(q, -1.0 / 32.0, t) * 0.693147180559945309417;
+  double p = 1.0 / 720.0;
+  p = fma(p, z, 1.0 / 120.0);
+  p = fma(p, z, 1.0 / 24.0);
+  p = fma(p, z, 1.0 / 6.0);
+  p = fma(p, z, 0.5);
+  p = fma(p, z, 1.0);
+  p = fma(p, z, 1.0);
+  const int i = (int)q;
+  return ldexp(table[i & 31] * p, i >> 5);
+}
+// The table: 2^(i / 32), the series to the 20th power.
+__device__ __forceinline__ double pow2_of_32(int i) {
+  const double z = (double)i * (0.693147180559945309417 / 32.0);
+  double p = 1.0;
+  for (int n = 20; n >= 1; --n) p = fma(p * z, 1.0 / (double)n, 1.0);
+  return p;
 }
 
-// Counts of the four values at order positions 4096 g + 4 t .. + 3 (position o = value 65535 - o).  hist[w] holds
-// value w + 32768's count in its high half and value w's in its low one, or, `wide`, the whole count of one of the two.
-__device__ __forceinline__ void counts_of(const unsigned* hist, bool wide, int g, int t, unsigned (&c)[4]) {
-  const int o = (g & 7) * 4 * SA_T + 4 * t;
-  const uint4 w = *(const uint4*)(hist + 32768 - 4 - o);
-  const unsigned v[4] = {w.w, w.z, w.y, w.x};
-#pragma unroll
-  for (int e = 0; e < 4; ++e) c[e] = wide ? v[e] : g < 8 ? v[e] >> 16 : v[e] & 0xffffu;
+// Running sums over the wave's lanes, each with its own, by DPP: steps of 1, 2, 4 and 8 within a row of 16 lanes, then the
+// rows' last lanes (a step costs a few cycles; by ds_bpermute, some hundred).
+enum { DPP_SHR1 = 0x111, DPP_SHR2 = 0x112, DPP_SHR4 = 0x114, DPP_SHR8 = 0x118, DPP_BCAST15 = 0x142, DPP_BCAST31 = 0x143 };
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int moved(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved(double v) {
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+  const unsigned lo = moved<CTRL, ROWS>((int)u), hi = moved<CTRL, ROWS>((int)(u >> 32));
+  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
 }
-
+template <typename N>
+__device__ __forceinline__ N scan64(N v) {
+  v += moved<DPP_SHR1, 0xf>(v);
+  v += moved<DPP_SHR2, 0xf>(v);
+  v += moved<DPP_SHR4, 0xf>(v);
+  v += moved<DPP_SHR8, 0xf>(v);
+  v += moved<DPP_BCAST15, 0xa>(v);
+  v += moved<DPP_BCAST31, 0xc>(v);
+  return v;
+}
 // The place where a running count or sum passes a goal: the value, and what stands before it.
-struct Place { int key; unsigned count; double w, before_m; long long before_n; };
+struct Place { int o; unsigned count; double w, before_m; int before_n; };
 
-template <bool BF, bool VEC>
-__global__ void __launch_bounds__(SA_T) k_sample_rows(SampleArgs a) {
-  __shared__ __attribute__((aligned(16))) unsigned hist[32768];
-  __shared__ double cell_m[SA_CELLS];
-  __shared__ int cell_n[SA_CELLS];
-  __shared__ int s_int[SA_W], s_key[SA_W];
+// One workgroup of T threads a row.  BITS: a value's count in LDS, 32 / BITS values a word (the low bits of the value name the
+// word, the high ones the field).  The counts are right where they add up to V: one that leaves its BITS takes 2^BITS from its
+// own and adds at most 1 to the next, so that the sum only falls.  Then (a constant row, a masked one) half of the values
+// are counted at a time, in twice the bits, which V cannot leave: 8 bits and 64 KB for V < 65,536, 16 bits and 128 KB
+// above.  The row is read again, from the caches, for the drawn token's index.
+template <bool BF, bool VEC, int T, int BITS>
+__global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
+  constexpr int W = T / 64, LOG = BITS == 8 ? 14 : 15, WORDS = 1 << LOG;
+  constexpr int GROUPS = 65536 / (4 * T), CELLS = GROUPS * W;   // a cell: a wave's 256 values of a group, in the order
+  constexpr int AHEAD = VEC ? 8 : 2;                           // vectors a thread has in flight
+  static_assert(CELLS == 256, "a lane searches four cells");
+  __shared__ __attribute__((aligned(16))) unsigned hist[WORDS];
+  __shared__ double cell_m[CELLS];                   // sums of the cells, then up to and with each
+  __shared__ int cell_n[CELLS];
+  constexpr int MANT = BF ? 7 : 10;                  // bits of a binade's values
+  __shared__ double table[32], ratio[0x8000 >> MANT];
+  __shared__ int s_int[W];
   __shared__ Place s_place;
+  __shared__ int s_cell, s_rank;
   const int row = blockIdx.x, t = threadIdx.x, wave = t >> 6, lane = t & 63;
   // request b > 0 has the rows cu_rows[b - 1] .. cu_rows[b], the first those below cu_rows[0]
   int b = 0;
@@ -103,267 +126,444 @@ __global__ void __launch_bounds__(SA_T) k_sample_rows(SampleArgs a) {
     const Seq f = find_looking<1>(a.cu_rows, a.B - 1, [&](int, int c) { return c <= row; });
     b = f.s >= 0 && row < f.c1 ? f.s + 1 : -1;
   }
+  auto give = [&](int tok, float lp) __attribute__((always_inline)) { a.tok[row] = tok; a.lp[row] = lp; };
   if (b < 0) {                                       // a row of no request
-    if (t == 0) { a.tok[row] = -1; a.lp[row] = 0.f; }
+    if (t == 0) give(-1, 0.f);
+    return;
+  }
+  const u16* x = a.logits + (size_t)row * a.ld;
+  const int V = a.V;
+  auto load8 = [&](int j) __attribute__((always_inline)) {   // eight logits from 8 j on
+    if constexpr (VEC) return *(const v4u*)(x + (size_t)8 * j);
+    v4u w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = x[(size_t)8 * j + 2 * i] | (unsigned)x[(size_t)8 * j + 2 * i + 1] << 16;
+    return w;
+  };
+  const int whole = V / 8;                           // vectors of eight; the row's last logits are one more, from `tail`
+  v4u tail = {};                                     // (the last logit again behind the row's end)
+  if (V % 8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tail[i] = x[min(8 * whole + 2 * i, V - 1)] | (unsigned)x[min(8 * whole + 2 * i + 1, V - 1)] << 16;
+  }
+  // f(j, eight logits) for this thread's whole vectors j, AHEAD of them in flight
+  auto each = [&](auto f) __attribute__((always_inline)) {
+    if (!whole) return;
+    v4u ring[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) ring[i] = load8(min(t + i * T, whole - 1));
+#pragma unroll 1
+    for (int j = t; j < whole; j += AHEAD * T) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const v4u w = ring[i];
+        ring[i] = load8(min(j + (i + AHEAD) * T, whole - 1));
+        if (j + i * T < whole) f(j + i * T, w);
+      }
+    }
+  };
+
+  bool wide = false;
+  int half = 0;                                      // (wide) the top bit of the values whose counts hist holds
+  auto clear = [&]() __attribute__((always_inline)) {
+    for (int i = t; i < WORDS / 4; i += T) ((uint4*)hist)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+  };
+  // n tokens of value v counted in the narrow fields (few operations: they are what counting costs)
+  auto add = [&](unsigned v, unsigned n) __attribute__((always_inline)) {
+    atomicAdd(&hist[v & (WORDS - 1)], BITS == 16 ? n * ((v >> 15) * 0xffffu + 1) : n << ((v >> 11) & 24));
+  };
+  // whether a wave has one and the same value everywhere (a mask): counted one by one, each would wait for the others
+  auto one_value = [&](v4u w, unsigned& v) __attribute__((always_inline)) {
+    const unsigned first = __builtin_amdgcn_readfirstlane(w[0]);
+    v = first & 0xffffu;
+    return __ballot(w[0] != first) == 0 && first >> 16 == v && __ballot(w[1] != first || w[2] != first || w[3] != first) == 0;
+  };
+  auto count_half = [&](int h) __attribute__((always_inline)) {
+    half = h;
+    clear();
+    auto add_wide = [&](unsigned v, unsigned n) __attribute__((always_inline)) {
+      if (v == 0x8000u) v = 0;                       // -0 counts as +0
+      if ((int)(v >> 15) == h) atomicAdd(&hist[v & (WORDS - 1)], n << (((v & 0x7fffu) >> LOG) * (2 * BITS & 31)));
+    };
+#pragma unroll 1
+    for (int j = t; j < whole; j += T) {
+      const v4u w = load8(j);
+      unsigned v;
+      if (one_value(w, v)) {
+        const unsigned long long on = __ballot(true);
+        if (lane == __builtin_ctzll(on)) add_wide(v, 8u * __builtin_popcountll(on));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) add_wide(w[i >> 1] >> (16 * (i & 1)) & 0xffffu, 1u);
+      }
+    }
+    if (t < V % 8) add_wide(x[8 * whole + t], 1u);
+    __syncthreads();
+  };
+  // counts of the four values at order positions 4 (T g + tt) .. + 3; those that are no numbers above -inf: see `number`
+  auto counts_of = [&](int g, int tt, unsigned (&c)[4]) {
+    const int o = 4 * (g * T + tt), raw = o < 0x8000 ? 0x7fff - o - 3 : o;      // the lowest of the four patterns
+    const uint4 w = *(const uint4*)(hist + (raw & (WORDS - 1)));
+    const unsigned v[4] = {w.x, w.y, w.z, w.w};
+    const int bits = wide ? 2 * BITS : BITS, shift = (wide ? raw & 0x7fff : raw) >> LOG;
+    const unsigned mask = bits == 32 ? ~0u : (1u << bits) - 1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[e] = v[o < 0x8000 ? 3 - e : e] >> (bits == 32 ? 0 : shift * bits) & mask;
+  };
+  auto number = [&](int g, int tt, unsigned (&c)[4]) {
+    const int o = 4 * (g * T + tt);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[e] = o + e >= O_FIRST<BF> && o + e <= O_LAST<BF> ? c[e] : 0;
+  };
+  int top = -1;
+  double m = 0.0, rate = 0.0;
+  // Weights of the values at order positions o .. o + 3, o a multiple of 4: they lie in one binade, a step apart, so that each is
+  // the one before times 2^(-step / T).  1 at the largest (none lies above it), 0 beside an infinite one.
+  auto weights = [&](int o, double (&w)[4]) __attribute__((always_inline)) {
+    const int base = max(o, top);
+    double x = pow2(table, base == top ? 0.0 : isinf(m) ? -INFINITY : (value_of<BF>(base) - m) * rate);
+    const double r = ratio[(raw_of(base) & 0x7fff) >> MANT];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      w[e] = x;
+      x = o + e >= top ? x * r : x;
+    }
+  };
+  // The same from the narrow counts, for all cells: each word is read once, and most are 0 in a whole wave.  (The positive
+  // values' order runs against their words'.)
+  auto cells_narrow = [&]() __attribute__((always_inline)) {
+    constexpr int F = 32 / BITS, BLOCKS = WORDS / (4 * T);
+    int all = 0;
+#pragma unroll 2
+    for (int k = 0; k < BLOCKS; ++k) {
+      const uint4 q = ((const uint4*)hist)[k * T + t];
+      if (!__ballot((q.x | q.y | q.z | q.w) != 0)) continue;
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
+        const bool pos = f < F / 2;
+        constexpr unsigned M = (1u << BITS) - 1;
+        const unsigned v[4] = {q.x >> (f * BITS) & M, q.y >> (f * BITS) & M, q.z >> (f * BITS) & M, q.w >> (f * BITS) & M};
+        unsigned c[4] = {pos ? v[3] : v[0], pos ? v[2] : v[1], pos ? v[1] : v[2], pos ? v[0] : v[3]};
+        int n = (int)(c[0] + c[1] + c[2] + c[3]);
+        if (!__ballot(n != 0)) continue;
+        all += n;
+        const int at = f * BLOCKS + k, raw = 4 * (at * T + t), o = pos ? 0x7fff - 3 - raw : raw;
+        if (o < O_FIRST<BF> || o + 3 > O_LAST<BF>) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[e] = o + e >= O_FIRST<BF> && o + e <= O_LAST<BF> ? c[e] : 0;
+          n = (int)(c[0] + c[1] + c[2] + c[3]);
+        }
+        double s = 0.0;
+        if (n) {
+          double w[4];
+          weights(o, w);
+          s = c[0] * w[0] + c[1] * w[1] + (c[2] * w[2] + c[3] * w[3]);
+        }
+        n = scan64(n);
+        s = scan64(s);
+        const int cell = pos ? (GROUPS / 2 - 1 - at) * W + W - 1 - wave : at * W + wave;
+        if (lane == 63) { cell_n[cell] = n; cell_m[cell] = s; }
+      }
+    }
+    return all;
+  };
+  // counts and weights of the cells of groups g0 .. g1 - 1
+  auto cells = [&](int g0, int g1) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int g = g0; g < g1; ++g) {
+      unsigned c[4];
+      int n = 0;
+      double s = 0.0;
+      counts_of(g, t, c);
+      if (__ballot((c[0] | c[1] | c[2] | c[3]) != 0)) {
+        number(g, t, c);
+        n = (int)(c[0] + c[1] + c[2] + c[3]);
+        if (n) {
+          double w[4];
+          weights(4 * (g * T + t), w);
+          s = c[0] * w[0] + c[1] * w[1] + (c[2] * w[2] + c[3] * w[3]);
+        }
+        n = scan64(n);
+        s = scan64(s);
+      }
+      if (lane == 63) { cell_n[g * W + wave] = n; cell_m[g * W + wave] = s; }
+    }
+  };
+
+  // the counts, and the largest number: the largest pattern as a signed number, where that is one
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  s16x2 most = {-32768, -32768};
+  if (t < 32) table[t] = pow2_of_32(t);
+  if (t < CELLS) { cell_n[t] = 0; cell_m[t] = 0.0; }
+  clear();
+  each([&](int, v4u w) __attribute__((always_inline)) {
+    unsigned v;
+    if (one_value(w, v)) {
+      const unsigned long long on = __ballot(true);
+      if (lane == __builtin_ctzll(on)) add(v, 8u * __builtin_popcountll(on));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        add(w[i] & 0xffffu, 1u);
+        add(w[i] >> 16, 1u);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned u = w[i];
+      most = __builtin_elementwise_max(most, __builtin_bit_cast(s16x2, u));
+    }
+  });
+  int high = max((int)most[0], (int)most[1]);
+  if (t < V % 8) {
+    const unsigned v = x[8 * whole + t];
+    add(v, 1u);
+    high = max(high, (int)(short)v);
+  }
+  // the largest of v over the workgroup
+  auto over_all = [&](int v) __attribute__((always_inline)) {
+    for (int off = 32; off >= 1; off >>= 1) v = max(v, __shfl_xor(v, off));
+    __syncthreads();
+    if (lane == 0) s_int[wave] = v;
+    __syncthreads();
+    for (int w = 0; w < W; ++w) v = max(v, s_int[w]);
+    return v;
+  };
+  constexpr int INF = BF ? 0x7f80 : 0x7c00;
+  high = over_all(high);
+  if (t == 0) {                                      // -0 counts as +0
+    const unsigned w = hist[0], at = (0x8000 >> LOG) * BITS, c = w >> at & ((1u << BITS) - 1);
+    hist[0] = w - (c << at) + c;
+  }
+  if (high < 0 || high > INF) {                      // no positive pattern, or a positive NaN: the numbers alone, in their order
+    int best = -65536;
+    auto look = [&](int v) __attribute__((always_inline)) {
+      const int o = v < 0x8000 ? 0x7fff - v : v == 0x8000 ? 0x7fff : v;
+      if (o >= O_FIRST<BF> && o <= O_LAST<BF>) best = max(best, -o);
+    };
+    each([&](int, v4u w) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) look(w[i >> 1] >> (16 * (i & 1)) & 0xffff);
+    });
+    if (t < V % 8) look(x[8 * whole + t]);
+    best = over_all(best);
+    top = best > -65536 ? -best : -1;
+  } else {
+    top = 0x7fff - high;
+  }
+  __syncthreads();
+  if (top < 0) {                                     // nothing to draw from
+    if (t == 0) give(-1, 0.f);
     return;
   }
   const float Tf = a.temp[b];
   const bool greedy = !(Tf > 0.f);
-  Row r;
-  r.T = Tf;
-  r.wide = false;
-  const u16* x = a.logits + (size_t)row * a.ld;
-  const int V = a.V, nvec = (V + 7) / 8;
-
-  // eight logits from 8 j on, -inf behind the row's end
-  auto load8 = [&](int j, unsigned (&e)[8]) {
-    constexpr unsigned NONE = BF ? 0xff80u : 0xfc00u;
-    if (VEC && 8 * j + 8 <= V) {
-      const uint4 w = *(const uint4*)(x + (size_t)8 * j);
-      const unsigned q[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { e[2 * i] = q[i] & 0xffffu; e[2 * i + 1] = q[i] >> 16; }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = 8 * j + i < V ? x[(size_t)8 * j + i] : NONE;
-    }
-  };
-  // counts of the row's values (half < 0: all, packed; else of the values whose top bit is `half`); the largest key and
-  // the number of tokens counted
-  auto count = [&](int half, int& key_max, int& n) {
-    for (int i = t; i < 32768 / 4; i += SA_T) ((uint4*)hist)[i] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    int mine = -1, num = 0;
-    for (int j = t; j < nvec; j += SA_T) {
-      unsigned e[8];
-      load8(j, e);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int k = key_of<BF>(e[i]);
-        mine = max(mine, k);
-        if (k < 0 || (half >= 0 && k >> 15 != half)) continue;
-        ++num;
-        if (!greedy) atomicAdd(&hist[k & 0x7fff], half < 0 && k >> 15 ? 0x10000u : 1u);
-      }
-    }
-    for (int off = 32; off >= 1; off >>= 1) {
-      mine = max(mine, __shfl_xor(mine, off));
-      num += __shfl_xor(num, off);
-    }
-    if (lane == 0) { s_key[wave] = mine; s_int[wave] = num; }
-    __syncthreads();
-    key_max = -1;
-    n = 0;
-    for (int w = 0; w < SA_W; ++w) { key_max = max(key_max, s_key[w]); n += s_int[w]; }
-    __syncthreads();
-  };
-  // count and weight of every cell of the groups g0 .. g1 - 1; -> tokens in them
-  auto cells = [&](int g0, int g1) {
-    for (int g = g0; g < g1; ++g) {
-      unsigned c[4];
-      counts_of(hist, r.wide, g, t, c);
-      int n = (int)(c[0] + c[1] + c[2] + c[3]);
-      double m = 0.0;
-      if (n)
-        for (int e = 0; e < 4; ++e)
-          if (c[e]) m += c[e] * weight_of<BF>(r, 65535 - (g * 4 * SA_T + 4 * t + e));
-      for (int off = 32; off >= 1; off >>= 1) {
-        n += __shfl_xor(n, off);
-        m += __shfl_xor(m, off);
-      }
-      if (lane == 0) { cell_n[g * SA_W + wave] = n; cell_m[g * SA_W + wave] = m; }
-    }
-  };
-  int held = -1;                                     // (wide) the half whose counts hist holds
-  auto hold = [&](int half) {
-    if (!r.wide || held == half) return;
-    int km, n;
-    count(half, km, n);
-    held = half;
-  };
-
-  int total;
-  count(-1, r.key_max, total);
-  if (r.key_max < 0) {                               // nothing to draw from
-    if (t == 0) { a.tok[row] = -1; a.lp[row] = 0.f; }
-    return;
+  m = value_of<BF>(top);
+  rate = greedy ? 0.0 : 1.4426950408889634074 / (double)Tf;
+  if (t < (0x8000 >> MANT)) {                        // 2^(-step / T) of every binade
+    const int o = 0x7fff - (t << MANT);
+    ratio[t] = isinf(m) ? 0.0 : pow2(table, (value_of<BF>(o) - value_of<BF>(o - 1)) * rate);
   }
-  r.m = value_of<BF>(r.key_max);
-  int key = r.key_max;
-  unsigned rank = 0;
-  double lp = 0.0;
-  if (!greedy) {
-    cells(0, SA_GROUPS);
+  __syncthreads();
+  int all = cells_narrow();
+  for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off);
+  if (lane == 0) s_int[wave] = all;
+  __syncthreads();
+  all = 0;
+  for (int w = 0; w < W; ++w) all += s_int[w];
+  if (all != V) {
+    wide = true;
+    for (int h = 1; h >= 0; --h) {
+      __syncthreads();
+      count_half(h);
+      cells(h ? GROUPS / 2 : 0, h ? GROUPS : GROUPS / 2);
+    }
     __syncthreads();
-    int sum = 0;
-    for (int i = lane; i < SA_CELLS; i += 64) sum += cell_n[i];
-    for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
-    // A value that 65,536 tokens have leaves its 16 bits: a low half's carry makes the sum 65,535 too small, a high
-    // half's 65,536, so that the sum is right only where no count left its half.  Then each half of the values is counted in 32 bits.
-    if (sum != total) {
-      r.wide = true;
-      for (int half = 1; half >= 0; --half) {
-        __syncthreads();
-        hold(half);
-        cells(half ? 0 : 8, half ? 8 : 16);
-      }
-      __syncthreads();
+  }
+
+  // One wave finds the places (where counts are wide, all waves help it to the half that it looks at).
+  if (wave == 0) {
+    int n[4], ns = 0;
+    double s[4], ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ns += cell_n[lane * 4 + i]; ss += cell_m[lane * 4 + i];
+      n[i] = ns; s[i] = ss;
     }
-    // The first value at which the running sum (by_n: count) reaches goal_m (goal_n), strictly passing it if `past`; the
-    // last one of any weight where rounding leaves none.  Only the first `end_n` tokens of the order count.
-    auto find = [&](bool by_n, long long goal_n, double goal_m, bool past, long long end_n) {
-      __shared__ int s_cell;
-      __shared__ double s_m;
-      __shared__ long long s_n;
-      if (wave == 0) {
-        constexpr int PER = SA_CELLS / 64;
-        long long n[PER], nl = 0;
-        double m[PER], ml = 0.0;
-        for (int i = 0; i < PER; ++i) {
-          nl += cell_n[lane * PER + i]; ml += cell_m[lane * PER + i];
-          n[i] = nl; m[i] = ml;
-        }
-        long long ns = nl;
-        double ms = ml;
-        for (int off = 1; off < 64; off <<= 1) {
-          const long long on = __shfl_up(ns, off);
-          const double om = shfl_up_d(ms, off);
-          if (lane >= off) { ns += on; ms += om; }
-        }
-        // sums before this lane's cells: the lane before's inclusive ones
-        long long nb = __shfl_up(ns, 1);
-        double mb = shfl_up_d(ms, 1);
-        if (lane == 0) { nb = 0; mb = 0.0; }
-        int hit = -1, last = -1;
-        for (int i = PER - 1; i >= 0; --i) {
-          const long long n0 = nb + (i ? n[i - 1] : 0);
-          const int here = (int)(nb + n[i] - n0);
-          if (!here || n0 >= end_n || (!by_n && !(m[i] > (i ? m[i - 1] : 0.0)))) continue;
-          if (last < 0) last = lane * PER + i;
-          if (by_n ? nb + n[i] >= goal_n : past ? mb + m[i] > goal_m : mb + m[i] >= goal_m) hit = lane * PER + i;
-        }
-        const unsigned long long any = __ballot(hit >= 0), some = __ballot(last >= 0);
-        const int from = any ? __ffsll((long long)any) - 1 : 63 - __builtin_clzll(some);
-        const int cell = __shfl(any ? hit : last, from);
-        if (lane == cell / PER) {
-          const int i = cell % PER;
-          s_cell = cell;
-          s_m = mb + (i ? m[i - 1] : 0.0);
-          s_n = nb + (i ? n[i - 1] : 0);
-        }
-      }
-      __syncthreads();
-      const int cell = s_cell, g = cell / SA_W;
-      hold(g < 8);
-      if (wave == 0) {
-        const int tt = (cell % SA_W) * 64 + lane;
-        unsigned c[4];
-        counts_of(hist, r.wide, g, tt, c);
-        double w[4], ml = 0.0;
-        long long nl = 0;
-        for (int e = 0; e < 4; ++e) {
-          w[e] = c[e] ? weight_of<BF>(r, 65535 - (g * 4 * SA_T + 4 * tt + e)) : 0.0;
-          ml += c[e] * w[e];
-          nl += c[e];
-        }
-        long long ns = nl;
-        double ms = ml;
-        for (int off = 1; off < 64; off <<= 1) {
-          const long long on = __shfl_up(ns, off);
-          const double om = shfl_up_d(ms, off);
-          if (lane >= off) { ns += on; ms += om; }
-        }
-        long long nb = __shfl_up(ns, 1);
-        double mb = shfl_up_d(ms, 1);
-        if (lane == 0) { nb = 0; mb = 0.0; }
-        nb += s_n;
-        mb += s_m;
-        int hit = -1, last = -1;
-        Place ph = {}, pl = {};
-        for (int e = 0; e < 4; ++e) {
-          if (c[e] && nb < end_n && (by_n || w[e] > 0.0)) {
-            const Place p = {65535 - (g * 4 * SA_T + 4 * tt + e), c[e], w[e], mb, nb};
-            pl = p;
-            last = e;
-            const double m1 = mb + c[e] * w[e];
-            if (hit < 0 && (by_n ? nb + c[e] >= goal_n : past ? m1 > goal_m : m1 >= goal_m)) { hit = e; ph = p; }
-          }
-          nb += c[e];
-          mb += c[e] * w[e];
-        }
-        const unsigned long long any = __ballot(hit >= 0), some = __ballot(last >= 0);
-        const int from = any ? __ffsll((long long)any) - 1 : 63 - __builtin_clzll(some);
-        if (lane == from) s_place = any ? ph : pl;
-      }
-      __syncthreads();
-      const Place p = s_place;
-      __syncthreads();
-      return p;
-    };
-    long long kept_n = total;
-    double kept_m;
-    const int k = a.top_k ? a.top_k[b] : 0;
-    if (k > 0 && k < kept_n) kept_n = k;
-    {
-      const Place p = find(true, kept_n, 0.0, false, kept_n);
-      kept_m = p.before_m + (double)(kept_n - p.before_n) * p.w;
+    const int nb = scan64(ns) - ns;
+    double sb = __shfl_up(scan64(ss), 1);            // (as the lanes before add up, to the bit)
+    if (lane == 0) sb = 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { cell_n[lane * 4 + i] = nb + n[i]; cell_m[lane * 4 + i] = sb + s[i]; }
+  }
+  __syncthreads();
+  // Up to three searches, each for the first value at which the running sum (of counts: by_n) reaches a goal, or passes it
+  // (the draw), or the last one of any weight where rounding leaves none, among the first kept_n tokens: the cut of k, the
+  // cut of P, the draw.
+  int kept_n = cell_n[CELLS - 1], rank = 0;
+  double kept_m = cell_m[CELLS - 1];
+  float lp = 0.f;
+  Place p = {};
+#pragma unroll 1
+  for (int stage = 0; stage < 3; ++stage) {
+    bool by_n = false;
+    double goal = 0.0;
+    if (stage == 0) {
+      const int k = greedy ? 1 : a.top_k ? a.top_k[b] : 0;
+      if (k < 1 || (k >= kept_n && !greedy)) continue;
+      by_n = true;
+      kept_n = k;
+    } else if (stage == 1) {
+      const float P = a.top_p ? a.top_p[b] : 1.f;
+      if (!(P < 1.f)) continue;
+      goal = (double)P * kept_m;
+    } else {
+      const float u = a.u[row];
+      goal = (u > 0.f ? (double)fminf(u, 0x1.fffffep-1f) : 0.0) * kept_m;
     }
-    const float P = a.top_p ? a.top_p[b] : 1.f;
-    if (P < 1.f) {
-      const double goal = (double)P * kept_m;
-      const Place p = find(false, 0, goal, false, kept_n);
+    const bool past = stage == 2;
+    if (wave == 0) {
+      int hit = -1, last = -1;
+#pragma unroll
+      for (int i = 3; i >= 0; --i) {
+        const int c = lane * 4 + i, n1 = cell_n[c], n0 = c ? cell_n[c - 1] : 0;
+        const double m1 = cell_m[c], m0 = c ? cell_m[c - 1] : 0.0;
+        if (n1 == n0 || n0 >= kept_n || (!by_n && !(m1 > m0))) continue;
+        if (last < 0) last = c;
+        if (by_n ? n1 >= kept_n : past ? m1 > goal : m1 >= goal) hit = c;
+      }
+      const unsigned long long any = __ballot(hit >= 0), some = __ballot(last >= 0);
+      const int c = any ? __builtin_amdgcn_readlane(hit, __builtin_ctzll(any))
+                        : __builtin_amdgcn_readlane(last, some ? 63 - __builtin_clzll(some) : 0);
+      if (lane == 0) s_cell = max(c, 0);
+    }
+    if (wide) {                                      // (all waves help the first to the half that it looks at)
+      __syncthreads();
+      if (half != (s_cell >= CELLS / 2)) count_half(!half);
+    }
+    if (wave == 0) {
+      const int cell = s_cell, g = cell / W, tt = cell % W * 64 + lane;
+      unsigned c[4];
+      counts_of(g, tt, c);
+      number(g, tt, c);
+      const int ns = (int)(c[0] + c[1] + c[2] + c[3]);
+      double w[4] = {}, ss = 0.0;
+      if (ns) {
+        weights(4 * (g * T + tt), w);
+        ss = c[0] * w[0] + c[1] * w[1] + (c[2] * w[2] + c[3] * w[3]);
+      }
+      int nb = scan64(ns) - ns + (cell ? cell_n[cell - 1] : 0);
+      double mb = __shfl_up(scan64(ss), 1);
+      if (lane == 0) mb = 0.0;
+      mb += cell ? cell_m[cell - 1] : 0.0;
+      int eh = -1, el = -1, n0[4];                   // the first place that reaches the goal, the last of any weight
+      double m0[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const double m1 = mb + c[e] * w[e];
+        n0[e] = nb;
+        m0[e] = mb;
+        if (c[e] && nb < kept_n && (by_n || w[e] > 0.0)) {
+          el = e;
+          if (eh < 0 && (by_n ? nb + (int)c[e] >= kept_n : past ? m1 > goal : m1 >= goal)) eh = e;
+        }
+        nb += c[e];
+        mb = m1;
+      }
+      const unsigned long long any = __ballot(eh >= 0), some = __ballot(el >= 0);
+      const int e = any ? eh : el;
+      if (lane == (any ? __builtin_ctzll(any) : 63 - __builtin_clzll(some))) {
+        auto pick = [&](const auto& v) __attribute__((always_inline)) { return e == 0 ? v[0] : e == 1 ? v[1] : e == 2 ? v[2] : v[3]; };
+        s_place = {4 * (g * T + tt) + e, pick(c), pick(w), pick(m0), pick(n0)};
+      }
+    }
+    __syncthreads();
+    p = s_place;
+    __syncthreads();
+    if (greedy) break;
+    const int most = min((int)p.count, kept_n - p.before_n);
+    if (stage == 0) {
+      kept_m = p.before_m + (double)most * p.w;
+    } else if (stage == 1) {
       const double more = ceil((goal - p.before_m) / p.w);
-      const long long most = min((long long)p.count, kept_n - p.before_n);
-      const long long i = more >= (double)most ? most : more >= 1.0 ? (long long)more : 1;
+      const int i = more >= (double)most ? most : more >= 1.0 ? (int)more : 1;
       kept_n = p.before_n + i;
       kept_m = p.before_m + (double)i * p.w;
+    } else {
+      const double past_n = floor((goal - p.before_m) / p.w);
+      rank = past_n >= (double)(most - 1) ? most - 1 : past_n > 0.0 ? (int)past_n : 0;
+      lp = (float)log(p.w / kept_m);
     }
-    const float u = a.u[row];
-    const double goal = (u > 0.f ? (double)fminf(u, 0x1.fffffep-1f) : 0.0) * kept_m;
-    const Place p = find(false, 0, goal, true, kept_n);
-    const double past = floor((goal - p.before_m) / p.w);
-    const long long most = min((long long)p.count, kept_n - p.before_n) - 1;
-    key = p.key;
-    rank = (unsigned)(past >= (double)most ? most : past > 0.0 ? (long long)past : 0);
-    lp = log(p.w / kept_m);
   }
-  // the index of the rank-th token that has the value: each wave counts its part of the row, the one that holds it looks again
-  const int per = (nvec + SA_W - 1) / SA_W, j0 = wave * per, j1 = min(nvec, j0 + per);
-  int num = 0;
-  for (int j = j0 + lane; j < j1; j += 64) {
-    unsigned e[8];
-    load8(j, e);
+
+  // The index of the rank-th token of that value: where it is alone, the one; else how many each 64 vectors hold, in
+  // order, in the counts' place (2^24 tokens: 32,768 words and one for the tail), and those 64 again.
+  const unsigned raw = (unsigned)raw_of(p.o), both = raw | raw << 16, care = p.o == 0x7fff ? 0x7fff7fffu : ~0u;   // (0 and -0)
+  auto mask_of = [&](v4u w) __attribute__((always_inline)) {   // bit i: the i-th of eight has it
+    unsigned hits = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) num += key_of<BF>(e[i]) == key;
+    for (int i = 0; i < 8; ++i) hits |= (unsigned)(((w[i >> 1] ^ both) & care) >> (16 * (i & 1)) << 16 == 0) << i;
+    return hits;
+  };
+  auto any_of = [&](v4u w) __attribute__((always_inline)) {    // whether one of eight has it: a half of the least is 0
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 least = {0xffff, 0xffff};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned u = (w[i] ^ both) & care;
+      least = __builtin_elementwise_min(least, __builtin_bit_cast(u16x2, u));
+    }
+    return least[0] == 0 || least[1] == 0;
+  };
+  const int steps = (whole + 63) / 64;               // (the tail: step `steps`)
+  const unsigned tail_hits = V % 8 ? mask_of(tail) & ((1u << V % 8) - 1) : 0;
+  if (p.count == 1) {
+    each([&](int j, v4u w) __attribute__((always_inline)) {
+      if (any_of(w)) give(8 * j + __builtin_ctz(mask_of(w)), lp);
+    });
+    if (t == 0 && tail_hits) give(8 * whole + __builtin_ctz(tail_hits), lp);
+    return;
   }
-  for (int off = 32; off >= 1; off >>= 1) num += __shfl_xor(num, off);
-  if (lane == 0) s_int[wave] = num;
+  each([&](int j, v4u w) __attribute__((always_inline)) {
+    int n = 0;
+    if (__ballot(any_of(w))) {
+      const unsigned hits = mask_of(w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) n += __builtin_popcountll(__ballot(hits >> i & 1));
+    }
+    if (lane == 0) hist[j >> 6] = n;
+  });
   __syncthreads();
-  unsigned before = 0;
-  for (int w = 0; w < wave; ++w) before += s_int[w];
-  if (rank < before || rank >= before + (unsigned)num) return;
-  for (int j = j0; j < j1; j += 64) {
-    unsigned e[8];
-    int hits = 0;
-    if (j + lane < j1) {
-      load8(j + lane, e);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) hits += key_of<BF>(e[i]) == key;
-    }
-    int run = hits;
-    for (int off = 1; off < 64; off <<= 1) {
-      const int o = __shfl_up(run, off);
-      if (lane >= off) run += o;
-    }
-    const unsigned first = before + run - hits;
-    if (hits && rank >= first && rank < first + hits) {
-      unsigned left = rank - first;
-      for (int i = 0; i < 8; ++i)
-        if (key_of<BF>(e[i]) == key && left-- == 0) { a.tok[row] = 8 * (j + lane) + i; a.lp[row] = (float)lp; }
-    }
-    before += __shfl(run, 63);
-    if (before > rank) break;
+  const int per = (steps + T - 1) / T;
+  int mine = 0;
+  for (int i = t * per; i < min(steps, (t + 1) * per); ++i) mine += hist[i];
+  int upto = scan64(mine);
+  if (lane == 63) s_int[wave] = upto;
+  if (t == 0) { s_cell = steps; s_rank = -1; }
+  __syncthreads();
+  int all_steps = 0;
+  for (int w = 0; w < W; ++w) {
+    if (w < wave) upto += s_int[w];
+    all_steps += s_int[w];
   }
+  if (rank < upto && rank >= upto - mine) {
+    int left = rank - (upto - mine), i = t * per;
+    while (left >= (int)hist[i]) left -= hist[i++];
+    s_cell = i;
+    s_rank = left;
+  }
+  __syncthreads();
+  if (wave) return;
+  const bool last = s_cell == steps;                 // none of the whole vectors: in the tail
+  const int j = s_cell * 64 + lane;
+  const unsigned hits = last ? lane == 0 ? tail_hits : 0 : j < whole ? mask_of(load8(j)) : 0;
+  const int own = __builtin_popcount(hits);
+  int left = (last ? rank - all_steps : s_rank) - (scan64(own) - own);
+  if (left < 0 || left >= own) return;
+  unsigned h = hits;
+  for (; left > 0; --left) h &= h - 1;
+  give(8 * (last ? whole : j) + __builtin_ctz(h), lp);
 }
 
 struct WalkArgs {
@@ -380,6 +580,8 @@ struct WalkArgs {
   int* status;
   int B, R, D, max_spec;
 };
+
+constexpr int WALK_LDS = 1024;   // drafts of a request staged in LDS
 
 // One wave a request; counts that do not lie in the rows and drafts refuse the request (one of no rows: padding).
 __global__ void __launch_bounds__(64) k_sample_walk(WalkArgs a) {
@@ -400,10 +602,17 @@ __global__ void __launch_bounds__(64) k_sample_walk(WalkArgs a) {
     }
     return;
   }
+  __shared__ int s_par[WALK_LDS], s_draft[WALK_LDS], s_tok[WALK_LDS + 1];
+  const bool lds = n <= WALK_LDS;
+  if (lds)
+    for (int i = lane; i <= n; i += 64) {
+      s_tok[i] = a.tok[s0 + i];
+      if (i < n) { s_par[i] = a.parents[d0 + i]; s_draft[i] = a.draft[d0 + i]; }
+    }
   __syncthreads();                                   // (one wave: the stores above are out before those below)
   const int pos = walk_tree(
-      (int)n, a.max_spec, [&](int row) { return a.tok[s0 + row]; }, [&](int i) { return a.parents[d0 + i]; },
-      [&](int i) { return a.draft[d0 + i]; },
+      (int)n, a.max_spec, [&](int row) { return lds ? s_tok[row] : a.tok[s0 + row]; },
+      [&](int i) { return lds ? s_par[i] : a.parents[d0 + i]; }, [&](int i) { return lds ? s_draft[i] : a.draft[d0 + i]; },
       [&](int p, int row, int tok) { if (lane == 0) { ot[p] = tok; ol[p] = a.lp[s0 + row]; } },
       [&](int p, int node) { if (lane == 0) pt[p] = node; });
   if (lane == 0) a.len[b] = pos;
@@ -432,7 +641,9 @@ int cfh_tree_sample_accept(const void* logits, long long ld, int V, int n_rows, 
   SampleArgs s = {(const u16*)logits, ld, V, n_rows, B, cu_sampled, uniforms, temperature, top_k, top_p, tok, lp};
   const bool vec = ld % 8 == 0 && ((uintptr_t)logits & 15) == 0;
   auto launch = [&](auto bf, auto v) {
-    hipLaunchKernelGGL((k_sample_rows<bf.value, v.value>), dim3(n_rows), dim3(SA_T), 0, st, s);
+    constexpr bool BF = bf.value, VEC = v.value;
+    if (V < 65536) hipLaunchKernelGGL((k_sample_rows<BF, VEC, 512, 8>), dim3(n_rows), dim3(512), 0, st, s);
+    else hipLaunchKernelGGL((k_sample_rows<BF, VEC, 1024, 16>), dim3(n_rows), dim3(1024), 0, st, s);
   };
   if (is_bf16) vec ? launch(std::true_type{}, std::true_type{}) : launch(std::true_type{}, std::false_type{});
   else vec ? launch(std::false_type{}, std::true_type{}) : launch(std::false_type{}, std::false_type{});
