@@ -21,18 +21,22 @@ from chain_flow_amd.kv_cache import _check_pool
 
 def _check_pages(block_table, room, ref, page, status):
     """-> (S, W, row stride, blocks, device index) of a pool's book-keeping."""
-    if block_table.dim() != 2 or ref.dim() != 1 or room.shape != block_table.shape[:1]:
-        raise ValueError("block_table must be [S, W], room [S] and ref [blocks]")
-    if any(t.dtype != torch.int32 for t in (block_table, room, ref)):
+    i32 = torch.int32
+    if block_table.dtype != i32 or room.dtype != i32 or ref.dtype != i32:
         raise ValueError("block_table, room and ref must be int32: they are updated in place")
-    S, W = block_table.shape
-    ld = block_table.stride(0) if S > 1 else W
-    if ((W > 1 and block_table.stride(1) != 1) or ld < W or not room.is_contiguous() or not ref.is_contiguous()
-            or not ref.shape[0]):
+    shape = block_table.shape
+    if len(shape) != 2 or ref.dim() != 1 or room.shape != shape[:1]:
+        raise ValueError("block_table must be [S, W], room [S] and ref [blocks]")
+    S, W = shape
+    blocks = ref.shape[0]
+    ld, one = block_table.stride()
+    if S < 2:
+        ld = W
+    if (one != 1 and W > 1) or ld < W or not room.is_contiguous() or not ref.is_contiguous() or not blocks:
         raise ValueError("block_table must have contiguous rows, room and ref be contiguous, and ref hold a page")
     if page < 1:
         raise ValueError(f"a page of {page} tokens")
-    return S, W, ld, ref.shape[0], _lib.device_of(block_table, room, ref, status=status)
+    return S, W, ld, blocks, _lib.device_of(block_table, room, ref, status=status)
 
 
 def kv_pages_fork(block_table, room, ref, src, dst, *, page: int, status=None) -> None:

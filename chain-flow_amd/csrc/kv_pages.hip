@@ -3,12 +3,15 @@
 // (tokens that a sequence's pages are for: it holds ceil(room / page) of them) and ref [blocks] (sequences that hold a page;
 // 0: free).  Everything is decided on the device, in an order that the sequences give (the lowest free page first), so
 // that a call never synchronises, can be captured, and gives the same table every time.
+#include <algorithm>
 #include <type_traits>
 
 #include "cfh_host.h"
-#include "cfh_seq.h"
+#include "cfh_scan.h"
 
 namespace {
+
+typedef unsigned v4u __attribute__((ext_vector_type(4)));   // (arrays of uint4, a union, go to memory)
 
 // One part of the cache (keys, values) of all layers, in bytes.
 struct Part { char* p; uint8_t* ex; long long ls, bs, es; };   // base, scale bytes, strides of a layer, a block, a layer's scales
@@ -19,6 +22,12 @@ struct PoolArgs {
   int row;                   // bytes of a token's heads
   bool f8;
 };
+
+// Keys (0) or values (1), field by field: the array taken by a lane's index would go to memory.
+__device__ __forceinline__ Part part_of(const PoolArgs& c, int i) {
+  const Part &k = c.part[0], &v = c.part[1];
+  return {i ? v.p : k.p, i ? v.ex : k.ex, i ? v.ls : k.ls, i ? v.bs : k.bs, i ? v.es : k.es};
+}
 
 // ---------------------------------------------------------------------------- accepted rows
 // Node path[s][i] of sequence s, row lens[s] + path[s][i], becomes row lens[s] + i, in every layer.  The nodes ascend, so
@@ -48,14 +57,15 @@ __global__ void __launch_bounds__(256) k_commit(CommitArgs a) {
   if (threadIdx.x == 0) bad = n > a.most || len < 0;
   __syncthreads();
   const long long limit = (long long)a.W * a.c.page;
-  auto slot_of = [&](long long pos) {                // -1: not in the cache
+  auto slot_of = [&](long long pos) __attribute__((always_inline)) {                // -1: not in the cache
     const int blk = pos < limit ? table[pos / a.c.page] : -1;
     return blk < 0 || blk >= a.c.blocks ? -1 : blk * a.c.page + (int)(pos % a.c.page);
   };
   if (!bad)
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
-      const int p = path[i];
-      if (p < (i ? path[i - 1] + 1 : 0) || slot_of((long long)len + p) < 0 || slot_of((long long)len + i) < 0) bad = 1;
+      const int p = path[i], from = slot_of((long long)len + max(p, 0)), to = slot_of((long long)len + i);
+      if (p < (i ? path[i - 1] + 1 : 0) || from < 0 || to < 0) bad = 1;
+      if (i < COMMIT_ROWS) { src[i] = from; dst[i] = to; }
     }
   __syncthreads();
   if (bad) {
@@ -65,22 +75,24 @@ __global__ void __launch_bounds__(256) k_commit(CommitArgs a) {
   const int cols = a.c.row / 16, per = cols + (a.c.f8 ? a.c.Hkv : 0);
   const int item = blockIdx.x * blockDim.x + threadIdx.x, unit = item / per, col = item - unit * per;
   const bool live = unit < 2 * a.c.layers;
-  const Part q = unit & 1 ? a.c.part[1] : a.c.part[0];
+  const Part q = part_of(a.c, unit & 1);
   const size_t layer = live ? unit >> 1 : 0;
   for (int i0 = 0; i0 < n; i0 += COMMIT_ROWS) {
     const int m = min(COMMIT_ROWS, n - i0);
-    __syncthreads();
-    if (threadIdx.x < m) {
-      src[threadIdx.x] = slot_of((long long)len + path[i0 + threadIdx.x]);
-      dst[threadIdx.x] = slot_of((long long)len + i0 + threadIdx.x);
+    if (i0) {
+      __syncthreads();
+      if (threadIdx.x < m) {
+        src[threadIdx.x] = slot_of((long long)len + path[i0 + threadIdx.x]);
+        dst[threadIdx.x] = slot_of((long long)len + i0 + threadIdx.x);
+      }
+      __syncthreads();
     }
-    __syncthreads();
     if (!live) continue;
     for (int i = 0; i < m; i += COMMIT_BATCH) {
       if (col < cols) {
-        uint4 x[COMMIT_BATCH];
-        auto at = [&](int slot) {
-          return (uint4*)(q.p + layer * q.ls + (size_t)(slot / a.c.page) * q.bs + (size_t)(slot % a.c.page) * a.c.row) + col;
+        v4u x[COMMIT_BATCH];
+        auto at = [&](int slot) __attribute__((always_inline)) {
+          return (v4u*)(q.p + layer * q.ls + (size_t)(slot / a.c.page) * q.bs + (size_t)(slot % a.c.page) * a.c.row) + col;
         };
 #pragma unroll
         for (int u = 0; u < COMMIT_BATCH; ++u) x[u] = *at(src[min(i + u, m - 1)]);
@@ -89,7 +101,7 @@ __global__ void __launch_bounds__(256) k_commit(CommitArgs a) {
           if (i + u < m) *at(dst[i + u]) = x[u];
       } else {
         uint8_t x[COMMIT_BATCH];
-        auto at = [&](int slot) { return q.ex + layer * q.es + (size_t)slot * a.c.Hkv + (col - cols); };
+        auto at = [&](int slot) __attribute__((always_inline)) { return q.ex + layer * q.es + (size_t)slot * a.c.Hkv + (col - cols); };
 #pragma unroll
         for (int u = 0; u < COMMIT_BATCH; ++u) x[u] = *at(src[min(i + u, m - 1)]);
 #pragma unroll
@@ -161,6 +173,7 @@ struct ResizeArgs {
   const int* new_room;
   int* status;
   int4* plan;                // [S]: first place in `fresh` (-1: refused), page to copy (-1: none), pages kept, tokens in the copied one
+  int* copies;               // [S + 1]: how many sequences have a page copied, and which
   int* fresh;                // pages taken, in order
   int table_ld, W, S, pieces;
 };
@@ -168,6 +181,11 @@ struct ResizeArgs {
 constexpr int RS_MAX = 4096;      // sequences of a call
 constexpr int RS_T = 1024;
 constexpr int RS_FAR = 0x3fffffff; // a place behind every page
+// Up to so many table entries (and RS_T sequences) one workgroup does all of it, in one launch; above, the entries are let go of
+// and filled in by a workgroup a sequence, in launches before and behind.  A pair of calls that grows and shrinks 48
+// sequences of 567 entries: 14.7 us so, 23.9 in three launches each (200 of 304: 15.9, 23.8; 1,000 of 223: 22.0, 24.9); a pair in
+// which every page changes hands 53 and 37 (104 and 48; 358 and 121).
+constexpr long long RS_ONE = 65536;
 
 // Pages that a sequence has, wants and keeps.
 struct Span { int had, want, kept, part; bool ok, pad; };
@@ -186,6 +204,15 @@ __device__ __forceinline__ Span span_of(const ResizeArgs& a, int s) {
   return x;
 }
 
+// An entry behind its sequence's new room: the page has one holder less.
+__device__ __forceinline__ void let_go(const ResizeArgs& a, int s, int j) {
+  int* entry = a.table + (size_t)s * a.table_ld + j;
+  const int p = *entry;
+  if (p >= 0 && p < a.c.blocks) atomicSub(&a.ref[p], 1);
+  else if (a.status) a.status[0] = 1;
+  *entry = -1;
+}
+
 // First: pages behind the new rooms are let go of.
 __global__ void __launch_bounds__(64) k_release(ResizeArgs a) {
   const int s = blockIdx.x;
@@ -194,28 +221,19 @@ __global__ void __launch_bounds__(64) k_release(ResizeArgs a) {
     if (!x.pad && threadIdx.x == 0 && a.status) a.status[0] = 1;
     return;
   }
-  int* row = a.table + (size_t)s * a.table_ld;
-  for (int j = x.want + (int)threadIdx.x; j < x.had; j += 64) {
-    const int p = row[j];
-    if (p >= 0 && p < a.c.blocks) atomicSub(&a.ref[p], 1);
-    else if (a.status) a.status[0] = 1;
-    row[j] = -1;
-  }
+  for (int j = x.want + (int)threadIdx.x; j < x.had; j += 64) let_go(a, s, j);
 }
 
-// The sum of v over the threads before this one, and over all of them.
-__device__ __forceinline__ long long scan_before(int v, long long* tmp, long long& all) {
+// The sum of v over the threads before this one, and over all of them (exact as doubles: below 2^53).
+__device__ __forceinline__ double scan_before(int v, double* tmp, double& all) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  long long run = v;
-  for (int off = 1; off < 64; off <<= 1) {
-    const long long o = __shfl_up(run, off);
-    if (lane >= off) run += o;
-  }
+  const double run = scan64((double)v);
   __syncthreads();
   if (lane == 63) tmp[wave] = run;
   __syncthreads();
-  long long before = 0;
+  double before = 0;
   all = 0;
+#pragma unroll
   for (int w = 0; w < RS_T / 64; ++w) {
     if (w < wave) before += tmp[w];
     all += tmp[w];
@@ -223,14 +241,43 @@ __device__ __forceinline__ long long scan_before(int v, long long* tmp, long lon
   return before + run - v;
 }
 
+// The last i in [0, n) with first[i] <= v (first[0] = 0, ascending).
+__device__ __forceinline__ int last_at(const int* first, int n, int v) {
+  int lo = 0;
+  for (int step = RS_T / 2; step; step /= 2)
+    if (lo + step < n && first[lo + step] <= v) lo += step;
+  return lo;
+}
+
 // Then, in one workgroup: what each sequence needs, in order, and the lowest free pages for it.  A shared last page
-// that is filled in part is copied before its sequence grows: by all but the last of its holders.
+// that is filled in part is copied before its sequence grows: by all but the last of its holders.  ONE: letting go and filling in,
+// too.
+template <bool ONE>
 __global__ void __launch_bounds__(RS_T) k_plan(ResizeArgs a) {
   __shared__ int tails[RS_MAX];      // the shared page a sequence would write into, -1: none
-  __shared__ long long tmp[RS_T / 64];
-  __shared__ int used;
+  __shared__ int first[ONE ? RS_T : 1];
+  __shared__ double tmp[RS_T / 64];
+  __shared__ int used, copied_n;
   const int t = threadIdx.x;
-  if (t == 0) used = 0;
+  if (t == 0) used = copied_n = 0;
+  if constexpr (ONE) {
+    const Span x = t < a.S ? span_of(a, t) : Span{};
+    if (t < a.S && !x.ok && !x.pad && a.status) a.status[0] = 1;
+    double all;
+    const double at = scan_before(x.ok ? x.had - x.kept : 0, tmp, all);
+    const int n = (int)all;                          // (at most RS_ONE entries)
+    first[t] = (int)at;
+    __syncthreads();
+    for (int i0 = t; i0 < n; i0 += 4 * RS_T)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * RS_T;
+        if (i >= n) break;
+        const int s = last_at(first, a.S, i);
+        let_go(a, s, (int)(((long long)a.new_room[s] + a.c.page - 1) / a.c.page) + i - first[s]);
+      }
+    __syncthreads();
+  }
   for (int s = t; s < a.S; s += RS_T) {
     const Span x = span_of(a, s);
     int tail = -1;
@@ -246,7 +293,7 @@ __global__ void __launch_bounds__(RS_T) k_plan(ResizeArgs a) {
     tails[s] = tail;
   }
   __syncthreads();
-  long long total = 0;                               // (what is asked for may pass 32 bits; what is free does not)
+  double total = 0;                                  // (what is asked for may pass 32 bits; what is free does not)
   for (int s0 = 0; s0 < a.S; s0 += RS_T) {
     const int s = s0 + t;
     int need = 0, tail = -1;
@@ -262,38 +309,46 @@ __global__ void __launch_bounds__(RS_T) k_plan(ResizeArgs a) {
         if (a.ref[tail] - before > 1) ++need;
       }
     }
-    long long all;
-    const int at = (int)min(total + scan_before(need, tmp, all), (long long)RS_FAR);
+    double all;
+    const int at = (int)fmin(total + scan_before(need, tmp, all), (double)RS_FAR);
     if (s < a.S) {
       const bool copied = x.ok && need > x.want - x.kept;
       // (-2: keeps its shared page, if those before it copied it)
       a.plan[s] = make_int4(x.ok ? at : -1, copied ? tail : x.ok && tail >= 0 ? -2 : -1, x.kept, x.part);
     }
+    if constexpr (ONE) first[t] = at;
     total += all;
   }
-  // the lowest free pages
-  long long base = 0;
-  for (int p0 = 0; p0 < a.c.blocks && base < total; p0 += 4 * RS_T) {
-    int is[4], n = 0;
+  // the lowest free pages, 16 counts a thread and step
+  constexpr int PER = 16;
+  double base = 0;
+  for (int p0 = 0; p0 < a.c.blocks && base < total; p0 += PER * RS_T) {
+    const int at0 = p0 + PER * t;
+    int ref[PER];
+    if (at0 + PER <= a.c.blocks) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int p = p0 + 4 * t + e;
-      is[e] = p < a.c.blocks && a.ref[p] == 0;
-      n += is[e];
+      for (int e = 0; e < PER; e += 4) __builtin_memcpy(ref + e, a.ref + at0 + e, 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < PER; ++e) ref[e] = at0 + e < a.c.blocks ? a.ref[at0 + e] : 1;
     }
-    long long all, at = base + scan_before(n, tmp, all);
+    int n = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (is[e]) {
-        if (at < total) a.fresh[at] = p0 + 4 * t + e;
-        ++at;
+    for (int e = 0; e < PER; ++e) n += ref[e] == 0;
+    double all, at = base + scan_before(n, tmp, all);
+    int to = (int)at;                                // (below 2^30: so many pages at most)
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+      if (ref[e] == 0) {
+        if (to < total) a.fresh[to] = at0 + e;
+        ++to;
       }
     base += all;
   }
-  const int have = (int)min(base, total);
+  const int have = (int)fmin(base, total);
   __syncthreads();
   for (int s = t; s < a.S; s += RS_T) {
-    int4 p = a.plan[s];
+    const int4 p = a.plan[s];
     if (p.x < 0) continue;
     const Span x = span_of(a, s);
     const int need = x.want - x.kept + (p.y >= 0);
@@ -302,39 +357,66 @@ __global__ void __launch_bounds__(RS_T) k_plan(ResizeArgs a) {
       if (a.status) a.status[0] = 1;
       continue;
     }
-    if (p.y >= 0) atomicSub(&a.ref[p.y], 1);
+    if (p.y >= 0) {
+      atomicSub(&a.ref[p.y], 1);
+      a.copies[1 + atomicAdd(&copied_n, 1)] = s;
+    }
     if (need > 0) atomicMax(&used, p.x + need);
+    if constexpr (ONE) a.room[s] = a.new_room[s];
   }
   __syncthreads();
-  for (int i = t; i < min(used, have); i += RS_T) a.ref[a.fresh[i]] = 1;
+  if (t == 0) a.copies[0] = copied_n;
+  for (int i = t; i < used; i += RS_T) {             // (what is used was had: no place behind)
+    const int page = a.fresh[i];
+    a.ref[page] = 1;
+    if constexpr (ONE) {
+      const int s = last_at(first, a.S, i);
+      const int4 p = a.plan[s];
+      a.table[(size_t)s * a.table_ld + p.z - (p.y >= 0) + i - p.x] = page;
+    }
+  }
 }
 
-// Last: tables and rooms (y = 0), and the copies, a piece of a page of one layer's keys or values each.
-constexpr int PIECE = 16384;
-
-__global__ void __launch_bounds__(256) k_fill(ResizeArgs a) {
+// The tables and rooms, where they are not filled in above.
+__global__ void __launch_bounds__(64) k_fill(ResizeArgs a) {
   const int s = blockIdx.x, t = threadIdx.x;
   const int4 p = a.plan[s];
   if (p.x < 0) return;
-  if (blockIdx.y == 0) {
-    const int want = (int)(((long long)a.new_room[s] + a.c.page - 1) / a.c.page), j0 = p.z - (p.y >= 0);
-    for (int j = j0 + t; j < want; j += 256) a.table[(size_t)s * a.table_ld + j] = a.fresh[p.x + j - j0];
-    if (t == 0) a.room[s] = a.new_room[s];
-    return;
-  }
-  if (p.y < 0) return;
-  const int unit = (blockIdx.y - 1) / a.pieces, piece = (blockIdx.y - 1) % a.pieces;
-  const Part q = unit & 1 ? a.c.part[1] : a.c.part[0];
-  const size_t layer = unit >> 1;
-  const int to = a.fresh[p.x], bytes = p.w * a.c.row;
-  const char* src = q.p + layer * q.ls + (size_t)p.y * q.bs;
-  char* dst = q.p + layer * q.ls + (size_t)to * q.bs;
-  for (int o = piece * PIECE + t * 16; o < min(bytes, (piece + 1) * PIECE); o += 256 * 16) *(uint4*)(dst + o) = *(const uint4*)(src + o);
-  if (a.c.f8 && piece == 0) {
-    const size_t per = (size_t)a.c.page * a.c.Hkv;
-    const uint8_t* es = q.ex + layer * q.es + p.y * per;
-    uint8_t* ed = q.ex + layer * q.es + to * per;
-    for (int o = t; o < p.w * a.c.Hkv; o += 256) ed[o] = es[o];
+  const int want = (int)(((long long)a.new_room[s] + a.c.page - 1) / a.c.page), j0 = p.z - (p.y >= 0);
+  for (int j = j0 + t; j < want; j += 64) a.table[(size_t)s * a.table_ld + j] = a.fresh[p.x + j - j0];
+  if (t == 0) a.room[s] = a.new_room[s];
+}
+
+// Last, the copies: a piece of a page of one layer's keys or values at a time.
+constexpr int PIECE = 16384;
+
+__global__ void __launch_bounds__(256) k_copy(ResizeArgs a) {
+  const int t = threadIdx.x, units = 2 * a.c.layers * a.pieces;
+  const long long all = (long long)a.copies[0] * units;
+  for (long long item = blockIdx.x; item < all; item += gridDim.x) {
+    const int s = a.copies[1 + item / units], rest = (int)(item % units), unit = rest / a.pieces, piece = rest % a.pieces;
+    const int4 p = a.plan[s];
+    const Part q = part_of(a.c, unit & 1);
+    const size_t layer = unit >> 1;
+    const int to = a.fresh[p.x], bytes = p.w * a.c.row, end = min(bytes, (piece + 1) * PIECE);
+    const char* src = q.p + layer * q.ls + (size_t)p.y * q.bs;
+    char* dst = q.p + layer * q.ls + (size_t)to * q.bs;
+    if (piece * PIECE >= bytes) continue;
+    constexpr int N = PIECE / (256 * 16);
+    v4u x[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = *(const v4u*)(src + min(piece * PIECE + (i * 256 + t) * 16, end - 16));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int o = piece * PIECE + (i * 256 + t) * 16;
+      if (o < end) *(v4u*)(dst + o) = x[i];
+    }
+    if (a.c.f8 && piece == 0) {
+      const size_t per = (size_t)a.c.page * a.c.Hkv;
+      const uint8_t* es = q.ex + layer * q.es + p.y * per;
+      uint8_t* ed = q.ex + layer * q.es + to * per;
+      for (int o = t; o < p.w * a.c.Hkv; o += 256) ed[o] = es[o];
+    }
   }
 }
 
@@ -399,7 +481,7 @@ int cfh_kv_fork(int32_t* table, int table_ld, int max_blocks, int32_t* room, int
 
 int64_t cfh_kv_resize_ws_bytes(int S, int max_blocks, int blocks) {
   if (S < 0 || max_blocks < 0 || blocks < 1) return -1;
-  return 16ll * S + 4 * std::min((long long)blocks, (long long)S * max_blocks);
+  return 16ll * S + 4 * (S + 1ll) + 4 * std::min((long long)blocks, (long long)S * max_blocks);
 }
 
 int cfh_kv_resize(const cfh_kv_pool* pool, int32_t* table, int table_ld, int max_blocks, int32_t* room, int S, int32_t* ref,
@@ -415,17 +497,25 @@ int cfh_kv_resize(const cfh_kv_pool* pool, int32_t* table, int table_ld, int max
   if (S > RS_MAX || max_blocks > RS_FAR || blocks > RS_FAR || (long long)max_blocks * page > 0x7fffffffll) return CFH_E_UNSUPPORTED;
   a.c.blocks = blocks; a.c.page = page;
   a.table = table; a.room = room; a.ref = ref; a.new_room = new_room; a.status = status;
-  a.plan = (int4*)ws; a.fresh = (int*)(a.plan + S);
+  a.plan = (int4*)ws; a.copies = (int*)(a.plan + S); a.fresh = a.copies + S + 1;
   a.table_ld = table_ld; a.W = max_blocks; a.S = S;
   a.pieces = pool ? (int)(((long long)page * a.c.row + PIECE - 1) / PIECE) : 0;
-  const long long copies = 2ll * a.c.layers * a.pieces;
-  if (copies > 65534) return CFH_E_UNSUPPORTED;
+  if (2ll * a.c.layers * a.pieces > 0x7fffffffll) return CFH_E_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(k_release, dim3(S), dim3(64), 0, st, a);
-  CFH_LAUNCH_CHECK();
-  hipLaunchKernelGGL(k_plan, dim3(1), dim3(RS_T), 0, st, a);
-  CFH_LAUNCH_CHECK();
-  hipLaunchKernelGGL(k_fill, dim3(S, (unsigned)(1 + copies)), dim3(256), 0, st, a);
+  if (S <= RS_T && (long long)S * max_blocks <= RS_ONE) {
+    hipLaunchKernelGGL(k_plan<true>, dim3(1), dim3(RS_T), 0, st, a);
+    CFH_LAUNCH_CHECK();
+  } else {
+    hipLaunchKernelGGL(k_release, dim3(S), dim3(64), 0, st, a);
+    CFH_LAUNCH_CHECK();
+    hipLaunchKernelGGL(k_plan<false>, dim3(1), dim3(RS_T), 0, st, a);
+    CFH_LAUNCH_CHECK();
+    hipLaunchKernelGGL(k_fill, dim3(S), dim3(64), 0, st, a);
+    CFH_LAUNCH_CHECK();
+  }
+  if (!pool) return CFH_OK;
+  const long long items = 2ll * S * a.c.layers * a.pieces;
+  hipLaunchKernelGGL(k_copy, dim3((unsigned)std::min(items, 1024ll)), dim3(256), 0, st, a);
   CFH_LAUNCH_CHECK();
   return CFH_OK;
 }

@@ -3,16 +3,22 @@
 //
 //   y[m][n] = sum_g s[n][g] sum_{k in group g} (u[n][k] - 8) x[m][k],   u in 0 .. 15
 //
-// Weight rows are u[n][K / 2] bytes, column 2 i in the low half of byte i; scales s[n][K / group] fp16; x and y fp16.  The
-// whole numbers u - 8 are exact in fp16, products and sums are fp32 (MFMA), each group's sum is scaled in fp32, and the
-// result is rounded once.
+// Weight rows are u[n][K / 2] bytes, column 2 i in the low half of byte i; scales s[n][K / group] fp16; x and y fp16.  Four bits
+// moved to bits 6 .. 9 of 0x4c00 are the fp16 number 16 + u, so a group's sum is
+//     sum (16 + u) x  -  24 sum x
+// with the second term, the same for all weight rows, as what the products are added to: two operations for two weights,
+// and no subtraction.  Products are exact in fp32 and sums are fp32 (MFMA); the magnitudes that meet are at most six times
+// those of (u - 8) x on average, 2^-21 of the sum of |s x| a group, far below the one rounding of the result to fp16.
 //
-// A wave takes 16 weight rows and 128 columns a step: 16 bytes a lane (row lane % 16, columns 32 (lane / 16) ..), 4 x 4
-// words of the four lanes of a row exchanged so that word j of lane (n, kg) holds columns 32 j + 8 kg .. + 7 of the step:
-// one 16 x 16 x 32 MFMA a word, and no MFMA mixes groups of 32 columns or more.
+// A wave takes 16 weight rows and 256 columns at a time, in two loads of 8 rows and 128 bytes each: whole lines (a bare read
+// of such a matrix reached 5.9 TB/s so, 5.2 with 16 rows and 64 bytes a load).  Lanes 8 apart exchange halves, so that lane
+// (n, kg) has 32 bytes of row n.  With groups below 128 columns they are 64 kg .. of the 256, and the 4 x 4 words of the four lanes of a
+// row are exchanged too, so that an MFMA's 32 columns lie side by side and mix no groups; with 128 they are columns 32 kg .. of both
+// halves, and the MFMAs take them as they are.
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "cfh_host.h"
 #include "cfh_common.h"
@@ -23,10 +29,8 @@ typedef unsigned short u16;
 typedef unsigned v4u __attribute__((ext_vector_type(4)));
 typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
 
-constexpr int MV_W = 8;          // waves a workgroup
-constexpr int MV_PF = 4;         // steps a wave has in flight
 constexpr int MV_ROWS = 16;      // rows of x a launch at most
-constexpr int MV_LDS = 150 * 1024;
+constexpr long long MV_LDS = 158 * 1024, MV_HALF = 79 * 1024;   // one workgroup a compute unit, two
 
 struct MvArgs {
   const h16* x;                  // [M][ld_x]
@@ -37,19 +41,17 @@ struct MvArgs {
   h16* y;                        // [M][ld_y]
   long long ld_x, ld_y;
   int ids_stride, a_rows, r;
-  int M, d, K, n, ld_w, ld_s, ks; // K = d + r columns; waves a tile of 16 weight rows
+  int M, d, K, n, ld_w, ld_s;    // K = d + r columns
+  int ks, chunk;                 // waves a tile of 16 weight rows; steps of 128 columns whose x lies in LDS at a time
 };
 
-// The eight weights of a word as whole numbers in fp16, in the order 0 4 1 5 2 6 3 7: 0x6400 + u is 1024 + u.
-__device__ __forceinline__ h16x8 whole8(unsigned w) {
-  h16x8 out;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const h16x2 v = __builtin_bit_cast(h16x2, ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u) - (h16x2){(h16)1032.f, (h16)1032.f};
-    out[2 * i] = v[0];
-    out[2 * i + 1] = v[1];
-  }
-  return out;
+// The eight weights of a word as fp16 numbers 16 + u, in the order 0 4 1 5 2 6 3 7.  (`e` is 0x4c004c00 in a vector register
+// and the mask in a scalar one: and-or is then one operation, which takes no literals.)
+__device__ __forceinline__ h16x8 plus16(unsigned w, unsigned e) {
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  constexpr unsigned M = 0x03c003c0u;
+  const u32x4 v = {(w << 6 & M) | e, (w << 2 & M) | e, (w >> 2 & M) | e, (w >> 6 & M) | e};
+  return __builtin_bit_cast(h16x8, v);
 }
 
 // Words of four lanes (kg = lane / 16) transposed: word j of lane kg becomes word kg of lane j.
@@ -68,70 +70,153 @@ __device__ __forceinline__ void swap4(unsigned (&w)[4]) {
   s16(w[2], w[3]);
 }
 
-// G: columns a scale.
-template <int G>
-__global__ void __launch_bounds__(MV_W * 64) k_matvec4(MvArgs a) {
-  extern __shared__ __attribute__((aligned(16))) h16 xs[];     // [M][K + 8], eights of columns in the order 0 4 1 5 2 6 3 7
-  __shared__ f32x4 part[MV_W][64];
+// G: columns a scale; NW waves.
+template <int G, int NW>
+__global__ void __launch_bounds__(NW * 64, 4) k_matvec4(MvArgs a) {
+  // x [M][chunk columns + 8], eights of them in the order 0 4 1 5 2 6 3 7; behind it -24 times its sums [columns / G][16 rows]
+  extern __shared__ __attribute__((aligned(16))) h16 xs[];
   constexpr int S = 128 / G;     // scales a step
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, kg = lane >> 4;
-  const int tile = blockIdx.x * (MV_W / a.ks) + wave / a.ks, part_k = wave % a.ks;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, kg = lane >> 4;
+  const int tile = blockIdx.x * (NW / a.ks) + wave / a.ks, part_k = wave % a.ks;
   const int steps = a.K / 128, s0 = steps * part_k / a.ks, s1 = steps * (part_k + 1) / a.ks;
   const int col = tile * 16 + (lane & 15);
   const size_t row = min(col, a.n - 1);              // (lanes behind the last row read it again)
-  const v4u* w = (const v4u*)(a.w + row * a.ld_w) + kg;
-  const h16* sc = a.s + row * a.ld_s;
-  v4u buf[MV_PF];
-  struct Sc { h16 v[S]; } sbuf[MV_PF];
-  auto fetch = [&](int p, int st) {
-    const int c = min(st, s1 - 1);
-    buf[p] = w[c * 4];
-    sbuf[p] = *(const Sc*)(sc + c * S);
-  };
-  if (s1 > s0) {
-#pragma unroll
-    for (int p = 0; p < MV_PF; ++p) fetch(p, s0 + p);
+  struct __attribute__((packed, aligned(256 / G))) Sc { h16 v[S]; };
+  struct __attribute__((packed, aligned(256 / G))) Sc2 { unsigned v[S]; };   // of two steps (as words: halves would be taken apart,
+                                                                             // and so waited for, where they are loaded)
+  const h16* sc = a.s + row * a.ld_s + s0 * S;
+  // an odd step first, by 64 bytes of each of the 16 rows; then pairs of steps, the next one in flight
+  const bool odd = (s1 - s0) % 2;
+  const int pairs = (s1 - s0) / 2;
+  struct Pair { v4u lo, hi; Sc2 s; };                // rows lane % 8 and 8 more
+  const int unit = G < 128 ? lane / 8 : kg + 4 * (lane / 8 % 2), r8 = tile * 16 + lane % 8;
+  const v4u* lo = (const v4u*)(a.w + (size_t)min(r8, a.n - 1) * a.ld_w) + (s0 + odd) * 4 + unit;
+  const v4u* hi = (const v4u*)(a.w + (size_t)min(r8 + 8, a.n - 1) * a.ld_w) + (s0 + odd) * 4 + unit;
+  v4u first = {};
+  Sc first_s = {};
+  if (odd) {
+    first = ((const v4u*)(a.w + row * a.ld_w))[s0 * 4 + kg];
+    first_s = *(const Sc*)sc;
+    sc += S;
   }
-  const int ldx = a.K + 8, eights = a.K / 8;
-  for (int i = threadIdx.x; i < a.M * eights; i += MV_W * 64) {
-    const int m = i / eights, k = (i - m * eights) * 8;
-    h16x8 v;
-    if (k < a.d) v = *(const h16x8*)(a.x + m * a.ld_x + k);
-    else v = *(const h16x8*)(a.a + (size_t)min(max(a.ids[m * a.ids_stride], 0), a.a_rows - 1) * a.r + (k - a.d));
-    *(h16x8*)(xs + m * ldx + k) = __builtin_shufflevector(v, v, 0, 4, 1, 5, 2, 6, 3, 7);
-  }
-  __syncthreads();
-  const int m = lane & 15;
-  const h16* xr = xs + (m < a.M ? m : 0) * ldx + kg * 8;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int st = s0; st < s1; st += MV_PF) {
+  Pair next = {};
+  if (pairs) next = {lo[0], hi[0], *(const Sc2*)sc};
+
+  // x's columns 128 c0 .. 128 c1 into LDS
+  const int ldx = a.chunk * 128 + 8;
+  float* sums = (float*)(xs + a.M * ldx);
+  auto stage = [&](int c0, int c1) __attribute__((always_inline)) {
+    constexpr int XB = 4;                            // eights of columns a thread has in flight
+    const int eights = (c1 - c0) * 16, all = a.M * eights;
+    for (int i0 = threadIdx.x; i0 < all; i0 += XB * NW * 64) {
+      h16x8 v[XB];
+      int to[XB], at[XB];
 #pragma unroll
-    for (int p = 0; p < MV_PF; ++p) {
-      unsigned q[4] = {buf[p][0], buf[p][1], buf[p][2], buf[p][3]};
-      const Sc s = sbuf[p];
-      const int here = st + p;
-      fetch(p, here + MV_PF);
-      swap4(q);
-      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+      for (int u = 0; u < XB; ++u) {
+        const int i = min(i0 + u * NW * 64, all - 1), m = i / eights, here = (i - m * eights) * 8, k = c0 * 128 + here;
+        to[u] = m * ldx + here;
+        at[u] = here / G * 16 + m;
+        v[u] = k < a.d ? *(const h16x8*)(a.x + m * a.ld_x + k)
+                       : *(const h16x8*)(a.a + (size_t)min(max(a.ids[m * a.ids_stride], 0), a.a_rows - 1) * a.r + (k - a.d));
+      }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        sum = mfma_f16(*(const h16x8*)(xr + min(here, s1 - 1) * 128 + j * 32), whole8(q[j]), sum);
-        if ((j + 1) % (G / 32) == 0) {
-          const float f = here < s1 ? (float)s.v[j / (G / 32)] : 0.f;
+      for (int u = 0; u < XB; ++u) {
+        *(h16x8*)(xs + to[u]) = __builtin_shufflevector(v[u], v[u], 0, 4, 1, 5, 2, 6, 3, 7);
+        float f = 0.f;                               // (whole groups of G / 8 lanes lie within or behind the last)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] = here < s1 ? fmaf(f, sum[e], acc[e]) : acc[e];
-          sum = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+        for (int e = 0; e < 8; ++e) f += (float)v[u][e];
+        f += dpp_f32<DPP_XOR1>(f);
+        f += dpp_f32<DPP_XOR2>(f);
+        if (G >= 64) f += dpp_f32<DPP_HMIRROR>(f);
+        if (G >= 128) f += dpp_f32<DPP_MIRROR>(f);
+        if (threadIdx.x % (G / 8) == 0 && i0 + u * NW * 64 < all) sums[at[u]] = -24.f * f;
       }
     }
+    __syncthreads();
+  };
+  const int m = lane & 15;
+  const h16* const x0 = xs + (m < a.M ? m : 0) * ldx + kg * (G < 128 ? 8 : 32);
+  const f32x4* const sum0 = (const f32x4*)sums + kg;
+  const h16* xr = x0;
+  const f32x4* sr = sum0;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  unsigned e16 = 0x4c004c00u;
+  asm("" : "+v"(e16));
+  auto scaled = [&](float f, const f32x4& sum) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = fmaf(f, sum[e], acc[e]);
+  };
+  auto one_step = [&]() __attribute__((always_inline)) {
+    unsigned q[4] = {first[0], first[1], first[2], first[3]};
+    if (G < 128) swap4(q);
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j % (G / 32) == 0) sum = sr[j / (G / 32) * 4];
+      sum = mfma_f16(*(const h16x8*)(xr + j * (G < 128 ? 32 : 8)), plus16(q[j], e16), sum);
+      if ((j + 1) % (G / 32) == 0) scaled((float)first_s.v[j / (G / 32)], sum);
+    }
+    xr += 128;
+    sr += S * 4;
+  };
+  auto two_steps = [&](const Pair& b) __attribute__((always_inline)) {
+    constexpr int ROR8 = 0x128;                      // lanes 8 apart
+    unsigned q[2][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      q[0][j] = __builtin_amdgcn_update_dpp((int)b.lo[j], (int)b.hi[j], ROR8, 0xf, 0xc, false);
+      q[1][j] = __builtin_amdgcn_update_dpp((int)b.hi[j], (int)b.lo[j], ROR8, 0xf, 0x3, false);
+    }
+    if (G < 128) {
+      swap4(q[0]);
+      swap4(q[1]);
+    }
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {                    // 32 columns each
+      if (i % (G / 32) == 0) sum = sr[i / (G / 32) * 4];
+      const unsigned word = G < 128 ? q[i & 1][i >> 1] : q[i >> 2][i & 3];
+      sum = mfma_f16(*(const h16x8*)(xr + (G < 128 ? i * 32 : i / 4 * 128 + i % 4 * 8)), plus16(word, e16), sum);
+      if ((i + 1) % (G / 32) == 0) {
+        const int at = i / (G / 32);
+        scaled((float)__builtin_bit_cast(h16, (u16)(b.s.v[at / 2] >> (16 * (at % 2)))), sum);
+      }
+    }
+    xr += 256;
+    sr += 2 * S * 4;
+  };
+  // the first chunk has the odd step; split waves have one chunk, of all columns
+  for (int c0 = 0, c1; c0 < steps; c0 = c1) {
+    const int extra = c0 == 0 && odd && a.ks == 1;
+    c1 = a.ks > 1 ? steps : min(steps, c0 + extra + (a.chunk - extra) / 2 * 2);
+    if (c0) __syncthreads();                         // (the chunk before is done with)
+    stage(c0, c1);
+    const int skip = a.ks > 1 ? s0 : 0;
+    xr = x0 + skip * 128;
+    sr = sum0 + skip * S * 4;
+    if (c0 == 0 && odd) one_step();
+    // (the last pair of all: behind the loop, which has no branch around its loads)
+    const int here = (a.ks > 1 ? pairs : (c1 - c0 - extra) / 2) - (c1 == steps ? 1 : 0);
+    for (int i = 0; i < here; ++i) {
+      const Pair now = next;
+      lo += 8;
+      hi += 8;
+      sc += 2 * S;
+      next = {*lo, *hi, *(const Sc2*)sc};
+      asm volatile("" ::: "memory");                 // (the loads together, not each where its words are used)
+      two_steps(now);
+    }
   }
+  if (pairs) two_steps(next);
   if (a.ks > 1) {                // the waves of a tile joined in their order
-    part[wave][lane] = acc;
+    f32x4* part = (f32x4*)xs;    // (x's place: NW KB)
+    __syncthreads();
+    part[wave * 64 + lane] = acc;
     __syncthreads();
     if (part_k) return;
     for (int i = 1; i < a.ks; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] += part[wave + i][lane][e];
+      for (int e = 0; e < 4; ++e) acc[e] += part[(wave + i) * 64 + lane][e];
   }
   if (col >= a.n) return;
 #pragma unroll
@@ -215,25 +300,40 @@ int cfh_matvec4(const void* x, long long ld_x, int M, int d, const uint8_t* w, i
       ld_s % (128 / group) || (uintptr_t)x % 16 || (uintptr_t)w % 16 || (uintptr_t)scale % (256 / group))
     return CFH_E_INVALID;
   if (r > 0 && (!a || !a_ids || a_rows < 1 || (uintptr_t)a % 16 || r % 8)) return CFH_E_INVALID;
-  const int most = (int)std::min<long long>(MV_ROWS, MV_LDS / ((K + 8) * 2));
-  if (most < 1) return CFH_E_UNSUPPORTED;
-  const long long tiles = ((long long)n + 15) / 16;
-  int ks = 1;
-  while (ks < MV_W && tiles * ks < 2048) ks *= 2;
-  for (int m0 = 0; m0 < M; m0 += most) {
+  const long long tiles = ((long long)n + 15) / 16, steps = K / 128;
+  auto lds_of = [&](int rows, long long c) { return rows * (c * 128 + 8) * 2 + c * 128 / group * 64; };
+  for (int m0 = 0, rows; m0 < M; m0 += rows) {
+    rows = std::min(MV_ROWS, M - m0);
     MvArgs v = {};
-    v.M = std::min(most, M - m0);
     v.x = (const h16*)x + m0 * ld_x; v.ld_x = ld_x; v.d = d; v.K = (int)K; v.n = n;
     v.w = w; v.ld_w = ld_w; v.s = (const h16*)scale; v.ld_s = ld_s;
     v.a = (const h16*)a; v.a_rows = a_rows; v.r = r; v.ids = a_ids + (long long)m0 * a_ids_stride; v.ids_stride = a_ids_stride;
-    v.y = (h16*)y + m0 * ld_y; v.ld_y = ld_y; v.ks = ks;
-    const dim3 grid((unsigned)((tiles * ks + MV_W - 1) / MV_W)), block(MV_W * 64);
-    const size_t lds = (size_t)v.M * (K + 8) * 2;
-    const hipStream_t st = (hipStream_t)stream;
-    auto* fn = group == 32 ? k_matvec4<32> : group == 64 ? k_matvec4<64> : k_matvec4<128>;
-    if (lds > 49152) CFH_HIP(hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    hipLaunchKernelGGL(fn, grid, block, lds, st, v);
-    CFH_LAUNCH_CHECK();
+    v.y = (h16*)y + m0 * ld_y; v.ld_y = ld_y;
+    auto launch = [&](auto g, auto nw) -> int {
+      constexpr int NW = nw.value;
+      int ks = 1;
+      while (ks < NW && tiles * ks < 200 * NW) ks *= 2;
+      long long c = steps;
+      if (ks > 1) {
+        while (rows > 1 && lds_of(rows, c) > MV_LDS) rows = (rows + 1) / 2;
+        if (lds_of(rows, c) > MV_LDS) ks = 1;
+      }
+      if (ks == 1)
+        while (lds_of(rows, c) > MV_HALF) c = (c + 1) / 2;
+      v.M = rows; v.ks = ks; v.chunk = (int)c;
+      const size_t lds = std::max<size_t>(lds_of(rows, c), ks > 1 ? (size_t)NW * 1024 : (size_t)0);
+      auto* fn = k_matvec4<g.value, NW>;
+      if (lds > 49152) CFH_HIP(hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+      hipLaunchKernelGGL(fn, dim3((unsigned)((tiles * ks + NW - 1) / NW)), dim3(NW * 64), lds, (hipStream_t)stream, v);
+      CFH_LAUNCH_CHECK();
+      return CFH_OK;
+    };
+    auto of_group = [&](auto nw) {
+      return group == 32 ? launch(std::integral_constant<int, 32>{}, nw) : group == 64 ? launch(std::integral_constant<int, 64>{}, nw)
+                                                                              : launch(std::integral_constant<int, 128>{}, nw);
+    };
+    const bool big = lds_of(rows, steps) > MV_HALF;
+    if (int rc = big ? of_group(std::integral_constant<int, 16>{}) : of_group(std::integral_constant<int, 8>{})) return rc;
   }
   return CFH_OK;
 }
