@@ -173,7 +173,7 @@ struct ResizeArgs {
   const int* new_room;
   int* status;
   int4* plan;                // [S]: first place in `fresh` (-1: refused), page to copy (-1: none), pages kept, tokens in the copied one
-  int* copies;               // [S + 1]: how many sequences have a page copied, and which
+  int4* copies;              // [S + 1]: how many pages are copied (x of the first), then from, to, tokens of each
   int* fresh;                // pages taken, in order
   int table_ld, W, S, pieces;
 };
@@ -359,13 +359,13 @@ __global__ void __launch_bounds__(RS_T) k_plan(ResizeArgs a) {
     }
     if (p.y >= 0) {
       atomicSub(&a.ref[p.y], 1);
-      a.copies[1 + atomicAdd(&copied_n, 1)] = s;
+      a.copies[1 + atomicAdd(&copied_n, 1)] = make_int4(p.y, a.fresh[p.x], p.w, 0);   // (in any order)
     }
     if (need > 0) atomicMax(&used, p.x + need);
     if constexpr (ONE) a.room[s] = a.new_room[s];
   }
   __syncthreads();
-  if (t == 0) a.copies[0] = copied_n;
+  if (t == 0) a.copies[0].x = copied_n;
   for (int i = t; i < used; i += RS_T) {             // (what is used was had: no place behind)
     const int page = a.fresh[i];
     a.ref[page] = 1;
@@ -392,15 +392,15 @@ constexpr int PIECE = 16384;
 
 __global__ void __launch_bounds__(256) k_copy(ResizeArgs a) {
   const int t = threadIdx.x, units = 2 * a.c.layers * a.pieces;
-  const long long all = (long long)a.copies[0] * units;
+  const long long all = (long long)a.copies[0].x * units;
   for (long long item = blockIdx.x; item < all; item += gridDim.x) {
-    const int s = a.copies[1 + item / units], rest = (int)(item % units), unit = rest / a.pieces, piece = rest % a.pieces;
-    const int4 p = a.plan[s];
+    const int4 p = a.copies[1 + item / units];
+    const int rest = (int)(item % units), unit = rest / a.pieces, piece = rest % a.pieces;
     const Part q = part_of(a.c, unit & 1);
     const size_t layer = unit >> 1;
-    const int to = a.fresh[p.x], bytes = p.w * a.c.row, end = min(bytes, (piece + 1) * PIECE);
-    const char* src = q.p + layer * q.ls + (size_t)p.y * q.bs;
-    char* dst = q.p + layer * q.ls + (size_t)to * q.bs;
+    const int bytes = p.z * a.c.row, end = min(bytes, (piece + 1) * PIECE);
+    const char* src = q.p + layer * q.ls + (size_t)p.x * q.bs;
+    char* dst = q.p + layer * q.ls + (size_t)p.y * q.bs;
     if (piece * PIECE >= bytes) continue;
     constexpr int N = PIECE / (256 * 16);
     v4u x[N];
@@ -413,9 +413,9 @@ __global__ void __launch_bounds__(256) k_copy(ResizeArgs a) {
     }
     if (a.c.f8 && piece == 0) {
       const size_t per = (size_t)a.c.page * a.c.Hkv;
-      const uint8_t* es = q.ex + layer * q.es + p.y * per;
-      uint8_t* ed = q.ex + layer * q.es + to * per;
-      for (int o = t; o < p.w * a.c.Hkv; o += 256) ed[o] = es[o];
+      const uint8_t* es = q.ex + layer * q.es + p.x * per;
+      uint8_t* ed = q.ex + layer * q.es + p.y * per;
+      for (int o = t; o < p.z * a.c.Hkv; o += 256) ed[o] = es[o];
     }
   }
 }
@@ -481,7 +481,7 @@ int cfh_kv_fork(int32_t* table, int table_ld, int max_blocks, int32_t* room, int
 
 int64_t cfh_kv_resize_ws_bytes(int S, int max_blocks, int blocks) {
   if (S < 0 || max_blocks < 0 || blocks < 1) return -1;
-  return 16ll * S + 4 * (S + 1ll) + 4 * std::min((long long)blocks, (long long)S * max_blocks);
+  return 16ll * S + 16 * (S + 1ll) + 4 * std::min((long long)blocks, (long long)S * max_blocks);
 }
 
 int cfh_kv_resize(const cfh_kv_pool* pool, int32_t* table, int table_ld, int max_blocks, int32_t* room, int S, int32_t* ref,
@@ -497,7 +497,7 @@ int cfh_kv_resize(const cfh_kv_pool* pool, int32_t* table, int table_ld, int max
   if (S > RS_MAX || max_blocks > RS_FAR || blocks > RS_FAR || (long long)max_blocks * page > 0x7fffffffll) return CFH_E_UNSUPPORTED;
   a.c.blocks = blocks; a.c.page = page;
   a.table = table; a.room = room; a.ref = ref; a.new_room = new_room; a.status = status;
-  a.plan = (int4*)ws; a.copies = (int*)(a.plan + S); a.fresh = a.copies + S + 1;
+  a.plan = (int4*)ws; a.copies = a.plan + S; a.fresh = (int*)(a.copies + S + 1);
   a.table_ld = table_ld; a.W = max_blocks; a.S = S;
   a.pieces = pool ? (int)(((long long)page * a.c.row + PIECE - 1) / PIECE) : 0;
   if (2ll * a.c.layers * a.pieces > 0x7fffffffll) return CFH_E_UNSUPPORTED;
@@ -515,7 +515,7 @@ int cfh_kv_resize(const cfh_kv_pool* pool, int32_t* table, int table_ld, int max
   }
   if (!pool) return CFH_OK;
   const long long items = 2ll * S * a.c.layers * a.pieces;
-  hipLaunchKernelGGL(k_copy, dim3((unsigned)std::min(items, 1024ll)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(k_copy, dim3((unsigned)std::min(items, 4096ll)), dim3(256), 0, st, a);
   CFH_LAUNCH_CHECK();
   return CFH_OK;
 }

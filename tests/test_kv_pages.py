@@ -80,7 +80,7 @@ def test_pages_refusals_without_a_device():
     with pytest.raises(ValueError, match="one GPU"):
         kv_pages_fork(table, room, ref, ids, ids, page=4)
     L, p = _lib.lib(), 4096      # stand-in addresses: never dereferenced, the checks fail first
-    assert L.cfh_kv_resize_ws_bytes(3, 4, 10) == 48 + 16 + 40 and L.cfh_kv_resize_ws_bytes(3, 4, 100) == 48 + 16 + 48
+    assert L.cfh_kv_resize_ws_bytes(3, 4, 10) == 48 + 64 + 40 and L.cfh_kv_resize_ws_bytes(3, 4, 100) == 48 + 64 + 48
     assert L.cfh_kv_resize_ws_bytes(-1, 4, 10) == L.cfh_kv_resize_ws_bytes(3, 4, 0) == -1
 
     def fork(ld=4, W=4, S=3, blocks=10, page=4, n=2, src=p):
