@@ -88,9 +88,9 @@ struct Place { int o; unsigned count; double w, before_m; int before_n; };
 template <bool BF, bool VEC, int T, int BITS>
 __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
   constexpr int W = T / 64, LOG = BITS == 8 ? 14 : 15, WORDS = 1 << LOG;
-  constexpr int GROUPS = 65536 / (4 * T), CELLS = GROUPS * W;   // a cell: a wave's 256 values of a group, in the order
+  constexpr int N = 8, GROUPS = 65536 / (N * T), CELLS = GROUPS * W;   // a cell: a wave's 64 x N values of a group, in the order
   constexpr int AHEAD = VEC ? 8 : 2;                           // vectors a thread has in flight
-  static_assert(CELLS == 256, "a lane searches four cells");
+  static_assert(CELLS == 128, "a lane searches two cells");
   __shared__ __attribute__((aligned(16))) unsigned hist[WORDS];
   __shared__ double cell_m[CELLS];                   // sums of the cells, then up to and with each
   __shared__ int cell_n[CELLS];
@@ -98,8 +98,10 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
   __shared__ double table[32], ratio[0x8000 >> MANT];
   __shared__ int s_int[W];
   __shared__ Place s_place;
-  __shared__ int s_cell, s_rank;
+  __shared__ int s_half[3], s_cell, s_rank;
+  __shared__ double s_kept;
   const int row = blockIdx.x, t = threadIdx.x, wave = t >> 6, lane = t & 63;
+  for (int i = t; i < WORDS / 4; i += T) ((uint4*)hist)[i] = make_uint4(0, 0, 0, 0);   // (while the bounds arrive)
   // request b > 0 has the rows cu_rows[b - 1] .. cu_rows[b], the first those below cu_rows[0]
   int b = 0;
   if (row >= a.cu_rows[0]) {
@@ -111,6 +113,8 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
     if (t == 0) give(-1, 0.f);
     return;
   }
+  const float Tf = a.temp[b], u = a.u[row], P = a.top_p ? a.top_p[b] : 1.f;   // (here, so that they arrive during the count)
+  const int K = a.top_k ? a.top_k[b] : 0;
   const u16* x = a.logits + (size_t)row * a.ld;
   const int V = a.V;
   auto load8 = [&](int j) __attribute__((always_inline)) {   // eight logits from 8 j on
@@ -145,10 +149,6 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
 
   bool wide = false;
   int half = 0;                                      // (wide) the top bit of the values whose counts hist holds
-  auto clear = [&]() __attribute__((always_inline)) {
-    for (int i = t; i < WORDS / 4; i += T) ((uint4*)hist)[i] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-  };
   // n tokens of value v counted in the narrow fields (few operations: they are what counting costs)
   auto add = [&](unsigned v, unsigned n) __attribute__((always_inline)) {
     atomicAdd(&hist[v & (WORDS - 1)], BITS == 16 ? n * ((v >> 15) * 0xffffu + 1) : n << ((v >> 11) & 24));
@@ -161,7 +161,8 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
   };
   auto count_half = [&](int h) __attribute__((always_inline)) {
     half = h;
-    clear();
+    for (int i = t; i < WORDS / 4; i += T) ((uint4*)hist)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
     auto add_wide = [&](unsigned v, unsigned n) __attribute__((always_inline)) {
       if (v == 0x8000u) v = 0;                       // -0 counts as +0
       if ((int)(v >> 15) == h) atomicAdd(&hist[v & (WORDS - 1)], n << (((v & 0x7fffu) >> LOG) * (2 * BITS & 31)));
@@ -181,92 +182,111 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
     if (t < V % 8) add_wide(x[8 * whole + t], 1u);
     __syncthreads();
   };
-  // counts of the four values at order positions 4 (T g + tt) .. + 3; those that are no numbers above -inf: see `number`
-  auto counts_of = [&](int g, int tt, unsigned (&c)[4]) {
-    const int o = 4 * (g * T + tt), raw = o < 0x8000 ? 0x7fff - o - 3 : o;      // the lowest of the four patterns
-    const uint4 w = *(const uint4*)(hist + (raw & (WORDS - 1)));
-    const unsigned v[4] = {w.x, w.y, w.z, w.w};
+  // counts of the N values at order positions N (T g + tt) .., 0 for those that are no numbers above -inf
+  auto counts_of = [&](int g, int tt, unsigned (&c)[N]) __attribute__((always_inline)) {
+    const int o = N * (g * T + tt), raw = o < 0x8000 ? 0x7fff - o - (N - 1) : o;      // the lowest of the patterns
+    const uint4* w = (const uint4*)(hist + (raw & (WORDS - 1)));
+    const uint4 w0 = w[0], w1 = w[1];
+    const unsigned v[N] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
     const int bits = wide ? 2 * BITS : BITS, shift = (wide ? raw & 0x7fff : raw) >> LOG;
     const unsigned mask = bits == 32 ? ~0u : (1u << bits) - 1;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) c[e] = v[o < 0x8000 ? 3 - e : e] >> (bits == 32 ? 0 : shift * bits) & mask;
-  };
-  auto number = [&](int g, int tt, unsigned (&c)[4]) {
-    const int o = 4 * (g * T + tt);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) c[e] = o + e >= O_FIRST<BF> && o + e <= O_LAST<BF> ? c[e] : 0;
+    for (int e = 0; e < N; ++e) {
+      const unsigned n = v[o < 0x8000 ? N - 1 - e : e] >> (bits == 32 ? 0 : shift * bits) & mask;
+      c[e] = o + e >= O_FIRST<BF> && o + e <= O_LAST<BF> ? n : 0;
+    }
   };
   int top = -1;
   double m = 0.0, rate = 0.0;
-  // Weights of the values at order positions o .. o + 3, o a multiple of 4: they lie in one binade, a step apart, so that each is
-  // the one before times 2^(-step / T).  1 at the largest (none lies above it), 0 beside an infinite one.
-  auto weights = [&](int o, double (&w)[4]) __attribute__((always_inline)) {
+  // f(e, weight) for the values at order positions o .. o + N - 1, o a multiple of N: they lie in one binade, a step apart, so that
+  // each is the one before times 2^(-step / T).  1 at the largest (none lies above it), 0 beside an infinite one.
+  auto weights = [&](int o, auto f) __attribute__((always_inline)) {
     const int base = max(o, top);
     double x = pow2(table, base == top ? 0.0 : isinf(m) ? -INFINITY : (value_of<BF>(base) - m) * rate);
     const double r = ratio[(raw_of(base) & 0x7fff) >> MANT];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      w[e] = x;
+    for (int e = 0; e < N; ++e) {
+      f(e, x);
       x = o + e >= top ? x * r : x;
     }
   };
-  // The same from the narrow counts, for all cells: each word is read once, and most are 0 in a whole wave.  (The positive
-  // values' order runs against their words'.)
+  // the weight of the tokens counted there: where the whole wave lies below the largest, a polynomial in the step's ratio
+  auto weight_of = [&](int o, const unsigned (&c)[N]) __attribute__((always_inline)) {
+    double s = 0.0;
+    if (__ballot(o < top)) {
+      weights(o, [&](int e, double w) __attribute__((always_inline)) { s = fma((double)c[e], w, s); });
+    } else {
+      const double r = ratio[(raw_of(o) & 0x7fff) >> MANT];
+#pragma unroll
+      for (int e = N - 1; e >= 0; --e) s = fma(s, r, (double)c[e]);
+      s *= pow2(table, isinf(m) ? o == top ? 0.0 : -INFINITY : (value_of<BF>(o) - m) * rate);
+    }
+    return s;
+  };
+  // All cells from the narrow counts: each word is read once, and most are 0 in a whole wave.  (The positive values' order runs
+  // against their words'.)  -> this thread's tokens, numbers or not
   auto cells_narrow = [&]() __attribute__((always_inline)) {
-    constexpr int F = 32 / BITS, BLOCKS = WORDS / (4 * T);
+    constexpr int F = 32 / BITS, BLOCKS = WORDS / (N * T);
     int all = 0;
 #pragma unroll 2
     for (int k = 0; k < BLOCKS; ++k) {
-      const uint4 q = ((const uint4*)hist)[k * T + t];
-      if (!__ballot((q.x | q.y | q.z | q.w) != 0)) continue;
+      const uint4 q0 = ((const uint4*)hist)[2 * (k * T + t)], q1 = ((const uint4*)hist)[2 * (k * T + t) + 1];
+      const unsigned q[N] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
+      if (!__ballot((q[0] | q[1] | q[2] | q[3] | q[4] | q[5] | q[6] | q[7]) != 0)) continue;
+      int cn[F] = {};
+      double cs[F] = {};
 #pragma unroll
       for (int f = 0; f < F; ++f) {
         const bool pos = f < F / 2;
-        constexpr unsigned M = (1u << BITS) - 1;
-        const unsigned v[4] = {q.x >> (f * BITS) & M, q.y >> (f * BITS) & M, q.z >> (f * BITS) & M, q.w >> (f * BITS) & M};
-        unsigned c[4] = {pos ? v[3] : v[0], pos ? v[2] : v[1], pos ? v[1] : v[2], pos ? v[0] : v[3]};
-        int n = (int)(c[0] + c[1] + c[2] + c[3]);
+        unsigned c[N];
+        int n = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          c[e] = q[pos ? N - 1 - e : e] >> (f * BITS) & ((1u << BITS) - 1);
+          n += (int)c[e];
+        }
         if (!__ballot(n != 0)) continue;
         all += n;
-        const int at = f * BLOCKS + k, raw = 4 * (at * T + t), o = pos ? 0x7fff - 3 - raw : raw;
-        if (o < O_FIRST<BF> || o + 3 > O_LAST<BF>) {
+        const int at = f * BLOCKS + k, raw = N * (at * T + t), o = pos ? 0x7fff - (N - 1) - raw : raw;
+        if (o < O_FIRST<BF> || o + N - 1 > O_LAST<BF>) {
+          n = 0;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) c[e] = o + e >= O_FIRST<BF> && o + e <= O_LAST<BF> ? c[e] : 0;
-          n = (int)(c[0] + c[1] + c[2] + c[3]);
+          for (int e = 0; e < N; ++e) {
+            c[e] = o + e >= O_FIRST<BF> && o + e <= O_LAST<BF> ? c[e] : 0;
+            n += (int)c[e];
+          }
         }
-        double s = 0.0;
-        if (n) {
-          double w[4];
-          weights(o, w);
-          s = c[0] * w[0] + c[1] * w[1] + (c[2] * w[2] + c[3] * w[3]);
-        }
-        n = scan64(n);
-        s = scan64(s);
-        const int cell = pos ? (GROUPS / 2 - 1 - at) * W + W - 1 - wave : at * W + wave;
-        if (lane == 63) { cell_n[cell] = n; cell_m[cell] = s; }
+        cn[f] = n;
+        if (n) cs[f] = weight_of(o, c);
       }
+      // the F cells' sums at once: halves and rows of lanes exchanged, so that a cell's are in lanes 64 / F f .. + 15
+      if constexpr (F == 4) {
+        swap_add<32>(cn[0], cn[2]); swap_add<32>(cn[1], cn[3]); swap_add<16>(cn[0], cn[1]);
+        swap_add<32>(cs[0], cs[2]); swap_add<32>(cs[1], cs[3]); swap_add<16>(cs[0], cs[1]);
+      } else {
+        swap_add<32>(cn[0], cn[1]); swap_add<16>(cn[0], 0);
+        swap_add<32>(cs[0], cs[1]); swap_add<16>(cs[0], 0.0);
+      }
+      cn[0] = row_scan(cn[0]);
+      cs[0] = row_scan(cs[0]);
+      const int f = lane / (64 / F), at = f * BLOCKS + k;
+      const int cell = f < F / 2 ? (GROUPS / 2 - 1 - at) * W + W - 1 - wave : at * W + wave;
+      if (lane % (64 / F) == 15) { cell_n[cell] = cn[0]; cell_m[cell] = cs[0]; }
     }
     return all;
   };
-  // counts and weights of the cells of groups g0 .. g1 - 1
+  // the cells of groups g0 .. g1 - 1
   auto cells = [&](int g0, int g1) __attribute__((always_inline)) {
 #pragma unroll 1
     for (int g = g0; g < g1; ++g) {
-      unsigned c[4];
-      int n = 0;
-      double s = 0.0;
+      unsigned c[N];
       counts_of(g, t, c);
-      if (__ballot((c[0] | c[1] | c[2] | c[3]) != 0)) {
-        number(g, t, c);
-        n = (int)(c[0] + c[1] + c[2] + c[3]);
-        if (n) {
-          double w[4];
-          weights(4 * (g * T + t), w);
-          s = c[0] * w[0] + c[1] * w[1] + (c[2] * w[2] + c[3] * w[3]);
-        }
-        n = scan64(n);
-        s = scan64(s);
-      }
+      int n = 0;
+#pragma unroll
+      for (int e = 0; e < N; ++e) n += (int)c[e];
+      double s = n ? weight_of(N * (g * T + t), c) : 0.0;
+      n = scan64(n);
+      s = scan64(s);
       if (lane == 63) { cell_n[g * W + wave] = n; cell_m[g * W + wave] = s; }
     }
   };
@@ -276,7 +296,7 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
   s16x2 most = {-32768, -32768};
   if (t < 32) table[t] = pow2_of_32(t);
   if (t < CELLS) { cell_n[t] = 0; cell_m[t] = 0.0; }
-  clear();
+  __syncthreads();
   each([&](int, v4u w) __attribute__((always_inline)) {
     unsigned v;
     if (one_value(w, v)) {
@@ -337,7 +357,6 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
     if (t == 0) give(-1, 0.f);
     return;
   }
-  const float Tf = a.temp[b];
   const bool greedy = !(Tf > 0.f);
   m = value_of<BF>(top);
   rate = greedy ? 0.0 : 1.4426950408889634074 / (double)Tf;
@@ -346,135 +365,119 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
     ratio[t] = isinf(m) ? 0.0 : pow2(table, (value_of<BF>(o) - value_of<BF>(o - 1)) * rate);
   }
   __syncthreads();
-  int all = cells_narrow();
-  for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off);
-  if (lane == 0) s_int[wave] = all;
-  __syncthreads();
-  all = 0;
-  for (int w = 0; w < W; ++w) all += s_int[w];
-  if (all != V) {
-    wide = true;
-    for (int h = 1; h >= 0; --h) {
-      __syncthreads();
-      count_half(h);
-      cells(h ? GROUPS / 2 : 0, h ? GROUPS : GROUPS / 2);
-    }
+  Place p = {top, 0, 1.0, 0.0, 0};                   // (as a greedy request's: the first of the largest)
+  int rank = 0;
+  double kept_m = 1.0;
+  if (!greedy) {
+    int all = cells_narrow();
+    for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off);
+    if (lane == 0) s_int[wave] = all;
     __syncthreads();
-  }
-
-  // One wave finds the places (where counts are wide, all waves help it to the half that it looks at).
-  if (wave == 0) {
-    int n[4], ns = 0;
-    double s[4], ss = 0.0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      ns += cell_n[lane * 4 + i]; ss += cell_m[lane * 4 + i];
-      n[i] = ns; s[i] = ss;
-    }
-    const int nb = scan64(ns) - ns;
-    double sb = __shfl_up(scan64(ss), 1);            // (as the lanes before add up, to the bit)
-    if (lane == 0) sb = 0.0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { cell_n[lane * 4 + i] = nb + n[i]; cell_m[lane * 4 + i] = sb + s[i]; }
-  }
-  __syncthreads();
-  // Up to three searches, each for the first value at which the running sum (of counts: by_n) reaches a goal, or passes it
-  // (the draw), or the last one of any weight where rounding leaves none, among the first kept_n tokens: the cut of k, the
-  // cut of P, the draw.
-  int kept_n = cell_n[CELLS - 1], rank = 0;
-  double kept_m = cell_m[CELLS - 1];
-  float lp = 0.f;
-  Place p = {};
-#pragma unroll 1
-  for (int stage = 0; stage < 3; ++stage) {
-    bool by_n = false;
-    double goal = 0.0;
-    if (stage == 0) {
-      const int k = greedy ? 1 : a.top_k ? a.top_k[b] : 0;
-      if (k < 1 || (k >= kept_n && !greedy)) continue;
-      by_n = true;
-      kept_n = k;
-    } else if (stage == 1) {
-      const float P = a.top_p ? a.top_p[b] : 1.f;
-      if (!(P < 1.f)) continue;
-      goal = (double)P * kept_m;
-    } else {
-      const float u = a.u[row];
-      goal = (u > 0.f ? (double)fminf(u, 0x1.fffffep-1f) : 0.0) * kept_m;
-    }
-    const bool past = stage == 2;
-    if (wave == 0) {
-      int hit = -1, last = -1;
-#pragma unroll
-      for (int i = 3; i >= 0; --i) {
-        const int c = lane * 4 + i, n1 = cell_n[c], n0 = c ? cell_n[c - 1] : 0;
-        const double m1 = cell_m[c], m0 = c ? cell_m[c - 1] : 0.0;
-        if (n1 == n0 || n0 >= kept_n || (!by_n && !(m1 > m0))) continue;
-        if (last < 0) last = c;
-        if (by_n ? n1 >= kept_n : past ? m1 > goal : m1 >= goal) hit = c;
+    all = 0;
+    for (int w = 0; w < W; ++w) all += s_int[w];
+    if (all != V) {
+      wide = true;
+      for (int h = 1; h >= 0; --h) {
+        __syncthreads();
+        count_half(h);
+        cells(h ? GROUPS / 2 : 0, h ? GROUPS : GROUPS / 2);
       }
-      const unsigned long long any = __ballot(hit >= 0), some = __ballot(last >= 0);
-      const int c = any ? __builtin_amdgcn_readlane(hit, __builtin_ctzll(any))
-                        : __builtin_amdgcn_readlane(last, some ? 63 - __builtin_clzll(some) : 0);
-      if (lane == 0) s_cell = max(c, 0);
-    }
-    if (wide) {                                      // (all waves help the first to the half that it looks at)
       __syncthreads();
-      if (half != (s_cell >= CELLS / 2)) count_half(!half);
     }
-    if (wave == 0) {
-      const int cell = s_cell, g = cell / W, tt = cell % W * 64 + lane;
-      unsigned c[4];
-      counts_of(g, tt, c);
-      number(g, tt, c);
-      const int ns = (int)(c[0] + c[1] + c[2] + c[3]);
-      double w[4] = {}, ss = 0.0;
-      if (ns) {
-        weights(4 * (g * T + tt), w);
-        ss = c[0] * w[0] + c[1] * w[1] + (c[2] * w[2] + c[3] * w[3]);
-      }
-      int nb = scan64(ns) - ns + (cell ? cell_n[cell - 1] : 0);
-      double mb = __shfl_up(scan64(ss), 1);
-      if (lane == 0) mb = 0.0;
-      mb += cell ? cell_m[cell - 1] : 0.0;
-      int eh = -1, el = -1, n0[4];                   // the first place that reaches the goal, the last of any weight
-      double m0[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const double m1 = mb + c[e] * w[e];
-        n0[e] = nb;
-        m0[e] = mb;
-        if (c[e] && nb < kept_n && (by_n || w[e] > 0.0)) {
-          el = e;
-          if (eh < 0 && (by_n ? nb + (int)c[e] >= kept_n : past ? m1 > goal : m1 >= goal)) eh = e;
+    // One wave finds the places (where counts are wide, the others help it to the half that it looks at): up to three searches,
+    // each for the first value at which the running sum (of counts: by_n) reaches a goal, or passes it (the draw), or the last
+    // one of any weight where rounding leaves none, among the first kept_n tokens: the cut of k, the cut of P, the draw.
+    if (wave == 0 || wide) {
+      const int n0 = cell_n[2 * lane], n1 = n0 + cell_n[2 * lane + 1], up_n = scan64(n1), from_n = up_n - n1;
+      const double s0 = cell_m[2 * lane], s1 = s0 + cell_m[2 * lane + 1], up_m = scan64(s1);
+      double from_m = __shfl_up(up_m, 1);            // (as the lanes before add up, to the bit)
+      if (lane == 0) from_m = 0.0;
+      const int upto_n[3] = {from_n, from_n + n0, up_n};          // up to the lane's two cells, between them and behind them
+      const double upto_m[3] = {from_m, from_m + s0, up_m};
+      int kept_n = __builtin_amdgcn_readlane(up_n, 63);
+      kept_m = from_lane(up_m, 63);
+#pragma unroll 1
+      for (int stage = 0; stage < 3; ++stage) {
+        const bool by_n = stage == 0, past = stage == 2;
+        double goal = 0.0;
+        if (by_n) {
+          if (K < 1 || K >= kept_n) continue;
+          kept_n = K;
+        } else if (!past) {
+          if (!(P < 1.f)) continue;
+          goal = (double)P * kept_m;
+        } else {
+          goal = (u > 0.f ? (double)fminf(u, 0x1.fffffep-1f) : 0.0) * kept_m;
         }
-        nb += c[e];
-        mb = m1;
+        int hit = -1, last = -1;
+#pragma unroll
+        for (int i = 1; i >= 0; --i) {
+          if (upto_n[i + 1] == upto_n[i] || upto_n[i] >= kept_n || (!by_n && !(upto_m[i + 1] > upto_m[i]))) continue;
+          if (last < 0) last = i;
+          if (by_n ? upto_n[i + 1] >= kept_n : past ? upto_m[i + 1] > goal : upto_m[i + 1] >= goal) hit = i;
+        }
+        const unsigned long long any = __ballot(hit >= 0), some = __ballot(last >= 0);
+        const int at = any ? __builtin_ctzll(any) : some ? 63 - __builtin_clzll(some) : 0;
+        const int i = max(__builtin_amdgcn_readlane(any ? hit : last, at), 0);
+        if (wide) {                                  // (wave 0's: kept_n and the rest are its own)
+          if (t == 0) s_half[stage] = at >= 32;
+          __syncthreads();
+          if (half != s_half[stage]) count_half(!half);
+          if (wave) continue;
+        }
+        const int cell = 2 * at + i, g = cell / W, tt = cell % W * 64 + lane, o = N * (g * T + tt);
+        unsigned c[N];
+        counts_of(g, tt, c);
+        int ns = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) ns += (int)c[e];
+        double w[N] = {}, ss = 0.0;
+        if (ns) weights(o, [&](int e, double x) __attribute__((always_inline)) { w[e] = x; ss = fma((double)c[e], x, ss); });
+        int nb = scan64(ns) - ns + __builtin_amdgcn_readlane(i ? upto_n[1] : upto_n[0], at);
+        double mb = __shfl_up(scan64(ss), 1);
+        if (lane == 0) mb = 0.0;
+        mb += from_lane(i ? upto_m[1] : upto_m[0], at);
+        Place first = {-1, 0, 0.0, 0.0, 0}, end = first;   // the first place that reaches the goal, the last of any weight
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const double m1 = fma((double)c[e], w[e], mb);
+          const bool in = c[e] && nb < kept_n && (by_n || w[e] > 0.0);
+          const bool hit = in && first.o < 0 && (by_n ? nb + (int)c[e] >= kept_n : past ? m1 > goal : m1 >= goal);
+          first.o = hit ? o + e : first.o; first.count = hit ? c[e] : first.count; first.w = hit ? w[e] : first.w;
+          first.before_m = hit ? mb : first.before_m; first.before_n = hit ? nb : first.before_n;
+          end.o = in ? o + e : end.o; end.count = in ? c[e] : end.count; end.w = in ? w[e] : end.w;
+          end.before_m = in ? mb : end.before_m; end.before_n = in ? nb : end.before_n;
+          nb += (int)c[e];
+          mb = m1;
+        }
+        const unsigned long long reach = __ballot(first.o >= 0), weigh = __ballot(end.o >= 0);
+        const int from = reach ? __builtin_ctzll(reach) : weigh ? 63 - __builtin_clzll(weigh) : 0;
+        if (!reach) first = end;
+        p.o = __builtin_amdgcn_readlane(first.o, from);
+        p.count = __builtin_amdgcn_readlane(first.count, from);
+        p.w = from_lane(first.w, from);
+        p.before_m = from_lane(first.before_m, from);
+        p.before_n = __builtin_amdgcn_readlane(first.before_n, from);
+        const int most = min((int)p.count, kept_n - p.before_n);
+        if (by_n) {
+          kept_m = p.before_m + (double)most * p.w;
+        } else if (!past) {
+          const double more = ceil((goal - p.before_m) / p.w);
+          const int i = more >= (double)most ? most : more >= 1.0 ? (int)more : 1;
+          kept_n = p.before_n + i;
+          kept_m = p.before_m + (double)i * p.w;
+        } else {
+          const double over = floor((goal - p.before_m) / p.w);
+          rank = over >= (double)(most - 1) ? most - 1 : over > 0.0 ? (int)over : 0;
+        }
       }
-      const unsigned long long any = __ballot(eh >= 0), some = __ballot(el >= 0);
-      const int e = any ? eh : el;
-      if (lane == (any ? __builtin_ctzll(any) : 63 - __builtin_clzll(some))) {
-        auto pick = [&](const auto& v) __attribute__((always_inline)) { return e == 0 ? v[0] : e == 1 ? v[1] : e == 2 ? v[2] : v[3]; };
-        s_place = {4 * (g * T + tt) + e, pick(c), pick(w), pick(m0), pick(n0)};
-      }
+      if (t == 0) { s_place = p; s_rank = rank; s_kept = kept_m; }
     }
     __syncthreads();
     p = s_place;
+    rank = s_rank;
+    kept_m = s_kept;
     __syncthreads();
-    if (greedy) break;
-    const int most = min((int)p.count, kept_n - p.before_n);
-    if (stage == 0) {
-      kept_m = p.before_m + (double)most * p.w;
-    } else if (stage == 1) {
-      const double more = ceil((goal - p.before_m) / p.w);
-      const int i = more >= (double)most ? most : more >= 1.0 ? (int)more : 1;
-      kept_n = p.before_n + i;
-      kept_m = p.before_m + (double)i * p.w;
-    } else {
-      const double past_n = floor((goal - p.before_m) / p.w);
-      rank = past_n >= (double)(most - 1) ? most - 1 : past_n > 0.0 ? (int)past_n : 0;
-      lp = (float)log(p.w / kept_m);
-    }
   }
 
   // The index of the rank-th token of that value: where it is alone, the one; else how many each 64 vectors hold, in
@@ -497,12 +500,13 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
     return least[0] == 0 || least[1] == 0;
   };
   const int steps = (whole + 63) / 64;               // (the tail: step `steps`)
+  auto found = [&](int tok) __attribute__((always_inline)) { give(tok, (float)log(p.w / kept_m)); };
   const unsigned tail_hits = V % 8 ? mask_of(tail) & ((1u << V % 8) - 1) : 0;
   if (p.count == 1) {
     each([&](int j, v4u w) __attribute__((always_inline)) {
-      if (any_of(w)) give(8 * j + __builtin_ctz(mask_of(w)), lp);
+      if (any_of(w)) found(8 * j + __builtin_ctz(mask_of(w)));
     });
-    if (t == 0 && tail_hits) give(8 * whole + __builtin_ctz(tail_hits), lp);
+    if (t == 0 && tail_hits) found(8 * whole + __builtin_ctz(tail_hits));
     return;
   }
   each([&](int j, v4u w) __attribute__((always_inline)) {
@@ -543,7 +547,7 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
   if (left < 0 || left >= own) return;
   unsigned h = hits;
   for (; left > 0; --left) h &= h - 1;
-  give(8 * (last ? whole : j) + __builtin_ctz(h), lp);
+  found(8 * (last ? whole : j) + __builtin_ctz(h));
 }
 
 struct WalkArgs {
