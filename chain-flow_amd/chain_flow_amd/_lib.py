@@ -71,7 +71,7 @@ SIGNATURES = {
     "cfh_tree_accept_ws_bytes": (_I64, [_I]),
     "cfh_tree_greedy_accept": (_I, [_VP, C.c_longlong, _I, _I, _I, _VP, _VP, _VP, _VP, _I, _I, _VP, _VP, _VP, _VP,
                                     _VP, _VP]),
-    "cfh_tree_sample_ws_bytes": (_I64, [_I]),
+    "cfh_tree_sample_ws_bytes": (_I64, [_I, _I]),
     "cfh_tree_sample_accept": (_I, [_VP, C.c_longlong, _I, _I, _I, _VP, _VP, _VP, _VP, _I, _I, _I, _VP, _VP, _VP, _VP,
                                     _VP, _VP, _VP, _VP, _VP, _VP, _VP]),
     "cfh_cand_ws_bytes": (_I64, [_I, _I]),

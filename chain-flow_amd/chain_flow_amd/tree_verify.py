@@ -192,7 +192,7 @@ def tree_sample_accept(logits, cu_num_draft_tokens, cu_num_sampled_tokens, draft
     ln = torch.empty(B, dtype=torch.int32, device=logits.device)
     lps = torch.empty(B, max_spec_len + 1, dtype=torch.float32, device=logits.device)
     L = _lib.lib()
-    ws = torch.empty(int(L.cfh_tree_sample_ws_bytes(R)), dtype=torch.uint8, device=logits.device)
+    ws = torch.empty(int(L.cfh_tree_sample_ws_bytes(R, V)), dtype=torch.uint8, device=logits.device)
     _lib.check(L.cfh_tree_sample_accept(
         logits.data_ptr(), ld, V, R, logits.dtype == torch.bfloat16, cdg.data_ptr(), csg.data_ptr(), _lib.ptr(draft),
         _lib.ptr(par), D, B, max_spec_len, uniforms.data_ptr(), temperature.data_ptr(), _lib.ptr(top_k), _lib.ptr(top_p),

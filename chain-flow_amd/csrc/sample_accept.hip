@@ -40,7 +40,16 @@ struct SampleArgs {
   const float* top_p;        // [B] or null
   int* tok;                  // [R]
   float* lp;                 // [R]
+  int parts;                 // of a row, counted on their own before (1: none)
+  unsigned* part_counts;     // [R][parts][PART_WORDS]
+  int* part_high;            // [R][parts]
 };
+struct Range { int from, to; };
+__device__ __forceinline__ Range part_range(int vectors, int part, int parts) {
+  const int per = (vectors + parts - 1) / parts;
+  return {min(part * per, vectors), min((part + 1) * per, vectors)};
+}
+constexpr int PART_WORDS = 32768;   // a part's counts: those of k_sample_rows with 16 bits a value
 
 // Order position o of a 16-bit value: 0 the largest NaN pattern of a positive sign, then descending, +0 at 32,767, -0 behind it.
 __device__ __forceinline__ int raw_of(int o) { return o < 0x8000 ? 0x7fff - o : o; }
@@ -80,16 +89,119 @@ __device__ __forceinline__ double pow2_of_32(int i) {
 // The place where a running count or sum passes a goal: the value, and what stands before it.
 struct Place { int o; unsigned count; double w, before_m; int before_n; };
 
+// Eight logits from 8 j on.
+template <bool VEC>
+__device__ __forceinline__ v4u load8(const u16* x, int j) {
+  if constexpr (VEC) return *(const v4u*)(x + (size_t)8 * j);
+  v4u w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = x[(size_t)8 * j + 2 * i] | (unsigned)x[(size_t)8 * j + 2 * i + 1] << 16;
+  return w;
+}
+// f(j, eight logits) for this thread's vectors j of from .. to - 1, AHEAD of them in flight.
+template <bool VEC, int T, typename F>
+__device__ __forceinline__ void each_of(const u16* x, int from, int to, F f) {
+  constexpr int AHEAD = VEC ? 8 : 2;
+  if (from >= to) return;
+  v4u ring[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) ring[i] = load8<VEC>(x, min(from + (int)threadIdx.x + i * T, to - 1));
+#pragma unroll 1
+  for (int j = from + threadIdx.x; j < to; j += AHEAD * T) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const v4u w = ring[i];
+      ring[i] = load8<VEC>(x, min(j + (i + AHEAD) * T, to - 1));
+      if (j + i * T < to) f(j + i * T, w);
+    }
+  }
+}
+// Whether a wave has one and the same value everywhere (a mask): counted one by one, each would wait for the others.
+__device__ __forceinline__ bool one_value(v4u w, unsigned& v) {
+  const unsigned first = __builtin_amdgcn_readfirstlane(w[0]);
+  v = first & 0xffffu;
+  return __ballot(w[0] != first) == 0 && first >> 16 == v && __ballot(w[1] != first || w[2] != first || w[3] != first) == 0;
+}
+// The narrow counts of the vectors from .. to - 1 and of the n_tail logits behind them (few operations a logit: they are what
+// counting costs).  -> the thread's largest pattern as a signed number: the largest number, where there is a positive one
+template <bool VEC, int T, int BITS>
+__device__ __forceinline__ int count_narrow(const u16* x, int from, int to, int n_tail, unsigned* hist) {
+  constexpr int WORDS = BITS == 8 ? 1 << 14 : 1 << 15;
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  s16x2 most = {-32768, -32768};
+  auto add = [&](unsigned v, unsigned n) __attribute__((always_inline)) {
+    atomicAdd(&hist[v & (WORDS - 1)], BITS == 16 ? n * ((v >> 15) * 0xffffu + 1) : n << ((v >> 11) & 24));
+  };
+  each_of<VEC, T>(x, from, to, [&](int, v4u w) __attribute__((always_inline)) {
+    unsigned v;
+    if (one_value(w, v)) {
+      const unsigned long long on = __ballot(true);
+      if ((threadIdx.x & 63) == __builtin_ctzll(on)) add(v, 8u * __builtin_popcountll(on));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        add(w[i] & 0xffffu, 1u);
+        add(w[i] >> 16, 1u);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned u = w[i];
+      most = __builtin_elementwise_max(most, __builtin_bit_cast(s16x2, u));
+    }
+  });
+  int high = max((int)most[0], (int)most[1]);
+  if ((int)threadIdx.x < n_tail) {
+    const unsigned v = x[(size_t)8 * to + threadIdx.x];
+    add(v, 1u);
+    high = max(high, (int)(short)v);
+  }
+  return high;
+}
+// The largest of v over W waves.
+template <int W>
+__device__ __forceinline__ int over_all(int v, int* s_int) {
+  for (int off = 32; off >= 1; off >>= 1) v = max(v, __shfl_xor(v, off));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s_int[threadIdx.x >> 6] = v;
+  __syncthreads();
+  for (int w = 0; w < W; ++w) v = max(v, s_int[w]);
+  return v;
+}
+
+// Few long rows leave most CUs idle, and a CU counts a logit a lane and 10 cycles: then each row is counted in parts, a
+// workgroup a part, and k_sample_rows adds the parts' counts up.
+template <bool VEC>
+__global__ void __launch_bounds__(1024, 4) k_sample_parts(SampleArgs a) {
+  __shared__ __attribute__((aligned(16))) unsigned hist[PART_WORDS];
+  __shared__ int s_int[16];
+  const int row = blockIdx.x, part = blockIdx.y, t = threadIdx.x, whole = a.V / 8;
+  const u16* x = a.logits + (size_t)row * a.ld;
+  for (int i = t; i < PART_WORDS / 4; i += 1024) ((uint4*)hist)[i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  const Range r = part_range(whole, part, a.parts);
+  int high = count_narrow<VEC, 1024, 16>(x, r.from, r.to, part == a.parts - 1 ? a.V % 8 : 0, hist);
+  high = over_all<16>(high, s_int);                  // (and the counts are whole)
+  const size_t at = (size_t)row * a.parts + part;
+  uint4* out = (uint4*)(a.part_counts + at * PART_WORDS);
+  for (int i = t; i < PART_WORDS / 4; i += 1024) out[i] = ((uint4*)hist)[i];
+  if (t == 0) a.part_high[at] = high;
+}
+
 // One workgroup of T threads a row.  BITS: a value's count in LDS, 32 / BITS values a word (the low bits of the value name the
 // word, the high ones the field).  The counts are right where they add up to V: one that leaves its BITS takes 2^BITS from its
 // own and adds at most 1 to the next, so that the sum only falls.  Then (a constant row, a masked one) half of the values
 // are counted at a time, in twice the bits, which V cannot leave: 8 bits and 64 KB for V < 65,536, 16 bits and 128 KB
 // above.  The row is read again, from the caches, for the drawn token's index.
+// 8 bits below 65,536 values, as two workgroups then share a CU (1,968 rows of 32,000 logits: 90 us in fp16, 76 in bf16; with
+// 1,024 threads and 16 bits 136 and 125).  What bounds a row of 248,320 bf16 logits on its CU: 17 us of counting (an LDS atomic a logit, a wave's 64 in
+// 10 cycles), 2.2 the cells (fp16: 4.2, more values are in use), 2.1 a search (one wave's latency), 4 the index.  1,968 rows
+// of 32,000: 12 us a row and CU in fp16, 1.4 TB/s; the stages of two rows overlap there, and the searches' latency and the
+// weights of many values are what remains.
 template <bool BF, bool VEC, int T, int BITS>
 __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
   constexpr int W = T / 64, LOG = BITS == 8 ? 14 : 15, WORDS = 1 << LOG;
   constexpr int N = 8, GROUPS = 65536 / (N * T), CELLS = GROUPS * W;   // a cell: a wave's 64 x N values of a group, in the order
-  constexpr int AHEAD = VEC ? 8 : 2;                           // vectors a thread has in flight
   static_assert(CELLS == 128, "a lane searches two cells");
   __shared__ __attribute__((aligned(16))) unsigned hist[WORDS];
   __shared__ double cell_m[CELLS];                   // sums of the cells, then up to and with each
@@ -101,7 +213,9 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
   __shared__ int s_half[3], s_cell, s_rank;
   __shared__ double s_kept;
   const int row = blockIdx.x, t = threadIdx.x, wave = t >> 6, lane = t & 63;
-  for (int i = t; i < WORDS / 4; i += T) ((uint4*)hist)[i] = make_uint4(0, 0, 0, 0);   // (while the bounds arrive)
+  const bool in_parts = T == 1024 && a.parts > 1;
+  if (!in_parts)
+    for (int i = t; i < WORDS / 4; i += T) ((uint4*)hist)[i] = make_uint4(0, 0, 0, 0);   // (while the bounds arrive)
   // request b > 0 has the rows cu_rows[b - 1] .. cu_rows[b], the first those below cu_rows[0]
   int b = 0;
   if (row >= a.cu_rows[0]) {
@@ -117,48 +231,14 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
   const int K = a.top_k ? a.top_k[b] : 0;
   const u16* x = a.logits + (size_t)row * a.ld;
   const int V = a.V;
-  auto load8 = [&](int j) __attribute__((always_inline)) {   // eight logits from 8 j on
-    if constexpr (VEC) return *(const v4u*)(x + (size_t)8 * j);
-    v4u w;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = x[(size_t)8 * j + 2 * i] | (unsigned)x[(size_t)8 * j + 2 * i + 1] << 16;
-    return w;
-  };
   const int whole = V / 8;                           // vectors of eight; the row's last logits are one more, from `tail`
   v4u tail = {};                                     // (the last logit again behind the row's end)
   if (V % 8) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) tail[i] = x[min(8 * whole + 2 * i, V - 1)] | (unsigned)x[min(8 * whole + 2 * i + 1, V - 1)] << 16;
   }
-  // f(j, eight logits) for this thread's whole vectors j, AHEAD of them in flight
-  auto each = [&](auto f) __attribute__((always_inline)) {
-    if (!whole) return;
-    v4u ring[AHEAD];
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) ring[i] = load8(min(t + i * T, whole - 1));
-#pragma unroll 1
-    for (int j = t; j < whole; j += AHEAD * T) {
-#pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        const v4u w = ring[i];
-        ring[i] = load8(min(j + (i + AHEAD) * T, whole - 1));
-        if (j + i * T < whole) f(j + i * T, w);
-      }
-    }
-  };
-
   bool wide = false;
   int half = 0;                                      // (wide) the top bit of the values whose counts hist holds
-  // n tokens of value v counted in the narrow fields (few operations: they are what counting costs)
-  auto add = [&](unsigned v, unsigned n) __attribute__((always_inline)) {
-    atomicAdd(&hist[v & (WORDS - 1)], BITS == 16 ? n * ((v >> 15) * 0xffffu + 1) : n << ((v >> 11) & 24));
-  };
-  // whether a wave has one and the same value everywhere (a mask): counted one by one, each would wait for the others
-  auto one_value = [&](v4u w, unsigned& v) __attribute__((always_inline)) {
-    const unsigned first = __builtin_amdgcn_readfirstlane(w[0]);
-    v = first & 0xffffu;
-    return __ballot(w[0] != first) == 0 && first >> 16 == v && __ballot(w[1] != first || w[2] != first || w[3] != first) == 0;
-  };
   auto count_half = [&](int h) __attribute__((always_inline)) {
     half = h;
     for (int i = t; i < WORDS / 4; i += T) ((uint4*)hist)[i] = make_uint4(0, 0, 0, 0);
@@ -169,7 +249,7 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
     };
 #pragma unroll 1
     for (int j = t; j < whole; j += T) {
-      const v4u w = load8(j);
+      const v4u w = load8<VEC>(x, j);
       unsigned v;
       if (one_value(w, v)) {
         const unsigned long long on = __ballot(true);
@@ -291,47 +371,27 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
     }
   };
 
-  // the counts, and the largest number: the largest pattern as a signed number, where that is one
-  typedef short s16x2 __attribute__((ext_vector_type(2)));
-  s16x2 most = {-32768, -32768};
   if (t < 32) table[t] = pow2_of_32(t);
   if (t < CELLS) { cell_n[t] = 0; cell_m[t] = 0.0; }
   __syncthreads();
-  each([&](int, v4u w) __attribute__((always_inline)) {
-    unsigned v;
-    if (one_value(w, v)) {
-      const unsigned long long on = __ballot(true);
-      if (lane == __builtin_ctzll(on)) add(v, 8u * __builtin_popcountll(on));
-    } else {
+  int high = -32768;
+  if (in_parts) {
+    constexpr int PER = WORDS / (4 * T);
+    const v4u* part = (const v4u*)(a.part_counts + (size_t)row * a.parts * PART_WORDS) + t;
+    v4u sum[PER] = {};
+#pragma unroll 2
+    for (int p = 0; p < a.parts; ++p) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        add(w[i] & 0xffffu, 1u);
-        add(w[i] >> 16, 1u);
-      }
+      for (int k = 0; k < PER; ++k) sum[k] += part[(size_t)p * (PART_WORDS / 4) + k * T];
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const unsigned u = w[i];
-      most = __builtin_elementwise_max(most, __builtin_bit_cast(s16x2, u));
-    }
-  });
-  int high = max((int)most[0], (int)most[1]);
-  if (t < V % 8) {
-    const unsigned v = x[8 * whole + t];
-    add(v, 1u);
-    high = max(high, (int)(short)v);
+    for (int k = 0; k < PER; ++k) ((v4u*)hist)[k * T + t] = sum[k];
+    if (t < a.parts) high = a.part_high[(size_t)row * a.parts + t];
+  } else {
+    high = count_narrow<VEC, T, BITS>(x, 0, whole, V % 8, hist);
   }
-  // the largest of v over the workgroup
-  auto over_all = [&](int v) __attribute__((always_inline)) {
-    for (int off = 32; off >= 1; off >>= 1) v = max(v, __shfl_xor(v, off));
-    __syncthreads();
-    if (lane == 0) s_int[wave] = v;
-    __syncthreads();
-    for (int w = 0; w < W; ++w) v = max(v, s_int[w]);
-    return v;
-  };
   constexpr int INF = BF ? 0x7f80 : 0x7c00;
-  high = over_all(high);
+  high = over_all<W>(high, s_int);
   if (t == 0) {                                      // -0 counts as +0
     const unsigned w = hist[0], at = (0x8000 >> LOG) * BITS, c = w >> at & ((1u << BITS) - 1);
     hist[0] = w - (c << at) + c;
@@ -342,12 +402,12 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
       const int o = v < 0x8000 ? 0x7fff - v : v == 0x8000 ? 0x7fff : v;
       if (o >= O_FIRST<BF> && o <= O_LAST<BF>) best = max(best, -o);
     };
-    each([&](int, v4u w) __attribute__((always_inline)) {
+    each_of<VEC, T>(x, 0, whole, [&](int, v4u w) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) look(w[i >> 1] >> (16 * (i & 1)) & 0xffff);
     });
     if (t < V % 8) look(x[8 * whole + t]);
-    best = over_all(best);
+    best = over_all<W>(best, s_int);
     top = best > -65536 ? -best : -1;
   } else {
     top = 0x7fff - high;
@@ -499,24 +559,38 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
     }
     return least[0] == 0 || least[1] == 0;
   };
-  const int steps = (whole + 63) / 64;               // (the tail: step `steps`)
+  Range in = {0, whole};
+  bool with_tail = V % 8 != 0, alone = p.count == 1;
+  if (in_parts) {                                    // the part that has it (a part holds fewer than 2^16 logits)
+    int n = 0;
+    if (lane < a.parts) {
+      const unsigned w = a.part_counts[((size_t)row * a.parts + lane) * PART_WORDS + (raw & (PART_WORDS - 1))];
+      n = p.o == 0x7fff ? (w & 0xffffu) + (w >> 16) : w >> (raw >> 15) * 16 & 0xffffu;
+    }
+    const int upto = scan64(n), part = __builtin_ctzll(__ballot(upto > rank));
+    rank -= __builtin_amdgcn_readlane(upto - n, part);
+    alone = __builtin_amdgcn_readlane(n, part) == 1;
+    in = part_range(whole, part, a.parts);
+    with_tail = with_tail && part == a.parts - 1;
+  }
+  const int steps = (in.to - in.from + 63) / 64;     // (the tail: step `steps`)
   auto found = [&](int tok) __attribute__((always_inline)) { give(tok, (float)log(p.w / kept_m)); };
-  const unsigned tail_hits = V % 8 ? mask_of(tail) & ((1u << V % 8) - 1) : 0;
-  if (p.count == 1) {
-    each([&](int j, v4u w) __attribute__((always_inline)) {
+  const unsigned tail_hits = with_tail ? mask_of(tail) & ((1u << V % 8) - 1) : 0;
+  if (alone) {
+    each_of<VEC, T>(x, in.from, in.to, [&](int j, v4u w) __attribute__((always_inline)) {
       if (any_of(w)) found(8 * j + __builtin_ctz(mask_of(w)));
     });
     if (t == 0 && tail_hits) found(8 * whole + __builtin_ctz(tail_hits));
     return;
   }
-  each([&](int j, v4u w) __attribute__((always_inline)) {
+  each_of<VEC, T>(x, in.from, in.to, [&](int j, v4u w) __attribute__((always_inline)) {
     int n = 0;
     if (__ballot(any_of(w))) {
       const unsigned hits = mask_of(w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) n += __builtin_popcountll(__ballot(hits >> i & 1));
     }
-    if (lane == 0) hist[j >> 6] = n;
+    if (lane == 0) hist[(j - in.from) >> 6] = n;
   });
   __syncthreads();
   const int per = (steps + T - 1) / T;
@@ -540,8 +614,8 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
   __syncthreads();
   if (wave) return;
   const bool last = s_cell == steps;                 // none of the whole vectors: in the tail
-  const int j = s_cell * 64 + lane;
-  const unsigned hits = last ? lane == 0 ? tail_hits : 0 : j < whole ? mask_of(load8(j)) : 0;
+  const int j = in.from + s_cell * 64 + lane;
+  const unsigned hits = last ? lane == 0 ? tail_hits : 0 : j < in.to ? mask_of(load8<VEC>(x, j)) : 0;
   const int own = __builtin_popcount(hits);
   int left = (last ? rank - all_steps : s_rank) - (scan64(own) - own);
   if (left < 0 || left >= own) return;
@@ -602,11 +676,23 @@ __global__ void __launch_bounds__(64) k_sample_walk(WalkArgs a) {
   if (lane == 0) a.len[b] = pos;
 }
 
+// How many parts a row is counted in.  The whole call over 248,320 logits: 6 rows 34.8 us in one part, 31.4 in 2, 29.3 in 4, 34.6
+// in 8 (a part's counts are 128 KB to read for the row's CU, 1.4 us); 24 rows 37.2 and 30.5 in 4, 36 rows 38.4 and 35.1, 41 rows of
+// other filters 41.2 and 40.7, 82 rows 42 and 50.  A part's counts stay below 2^16.
+int parts_of(int n_rows, int V) {
+  const int parts = max(4, V / 65528 + 1);
+  return n_rows <= 24 && V >= 65536 && parts <= 8 ? parts : 1;
+}
+
 }  // namespace
 
 extern "C" {
 
-int64_t cfh_tree_sample_ws_bytes(int n_rows) { return n_rows < 0 ? -1 : (int64_t)n_rows * 8; }
+int64_t cfh_tree_sample_ws_bytes(int n_rows, int V) {
+  if (n_rows < 0 || V <= 0) return -1;
+  const int parts = parts_of(n_rows, V);
+  return ((int64_t)n_rows * 8 + 15) / 16 * 16 + (parts > 1 ? (int64_t)n_rows * parts * (PART_WORDS * 4 + 4) : 0);
+}
 
 int cfh_tree_sample_accept(const void* logits, long long ld, int V, int n_rows, int is_bf16, const int32_t* cu_draft,
                            const int32_t* cu_sampled, const int32_t* draft_ids, const int32_t* parents, int n_drafts, int B,
@@ -622,8 +708,16 @@ int cfh_tree_sample_accept(const void* logits, long long ld, int V, int n_rows, 
   hipStream_t st = (hipStream_t)stream;
   int* tok = (int*)ws;
   float* lp = (float*)(tok + n_rows);
-  SampleArgs s = {(const u16*)logits, ld, V, n_rows, B, cu_sampled, uniforms, temperature, top_k, top_p, tok, lp};
-  const bool vec = ld % 8 == 0 && ((uintptr_t)logits & 15) == 0;
+  const int parts = parts_of(n_rows, V);
+  unsigned* part_counts = (unsigned*)((char*)ws + ((size_t)n_rows * 8 + 15) / 16 * 16);
+  SampleArgs s = {(const u16*)logits, ld, V, n_rows, B, cu_sampled, uniforms, temperature, top_k, top_p, tok, lp, parts,
+                  part_counts, (int*)(part_counts + (size_t)n_rows * parts * PART_WORDS)};
+  const bool vec = (n_rows == 1 || ld % 8 == 0) && ((uintptr_t)logits & 15) == 0;
+  if (parts > 1) {
+    if (vec) hipLaunchKernelGGL(k_sample_parts<true>, dim3(n_rows, parts), dim3(1024), 0, st, s);
+    else hipLaunchKernelGGL(k_sample_parts<false>, dim3(n_rows, parts), dim3(1024), 0, st, s);
+    CFH_LAUNCH_CHECK();
+  }
   auto launch = [&](auto bf, auto v) {
     constexpr bool BF = bf.value, VEC = v.value;
     if (V < 65536) hipLaunchKernelGGL((k_sample_rows<BF, VEC, 512, 8>), dim3(n_rows), dim3(512), 0, st, s);

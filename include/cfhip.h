@@ -514,9 +514,9 @@ int cfh_tree_greedy_accept(const void* logits, long long ld, int V, int n_rows, 
  *   out_tokens [B][max_spec + 1] and accepted_path [B][max_spec] (-1 padded), accepted_len [B], out_logprobs [B][max_spec
  *   + 1] (0 padded): the log of the emitted tokens' probabilities after the filters.
  * A request whose counts do not lie in the rows and drafts, and all behind counts that fall, get no token and set status[0]
- * to 1 (status: one int32 the caller zeroes, or NULL).  V <= 2^24.  ws: cfh_tree_sample_ws_bytes(n_rows) bytes, 16-byte
+ * to 1 (status: one int32 the caller zeroes, or NULL).  V <= 2^24.  ws: cfh_tree_sample_ws_bytes(n_rows, V) bytes, 16-byte
  * aligned, of the call's own until it ends. */
-int64_t cfh_tree_sample_ws_bytes(int n_rows);
+int64_t cfh_tree_sample_ws_bytes(int n_rows, int V);
 int cfh_tree_sample_accept(const void* logits, long long ld, int V, int n_rows, int is_bf16, const int32_t* cu_draft,
                            const int32_t* cu_sampled, const int32_t* draft_ids, const int32_t* parents, int n_drafts, int B,
                            int max_spec, const float* uniforms, const float* temperature, const int32_t* top_k,

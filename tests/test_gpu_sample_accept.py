@@ -129,6 +129,29 @@ def test_rows_of_infinities_nan_and_nothing(cuda, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("R,V", [(1, 65536), (24, 65605), (25, 65605), (130, 65541), (3, 262144), (2, 530000)])
+def test_long_rows_counted_whole_and_in_parts(cuda, R, V, dtype):
+    """Few long rows are counted by several workgroups, more of them by one each: odd rows and drawn tokens in the first part,
+    the last one and the last logits behind whole vectors."""
+    inf, nan = float("inf"), float("nan")
+    rng = np.random.default_rng(R + V)
+    x = torch.randn(R, V, generator=torch.Generator().manual_seed(R)).mul(3).to(dtype)
+    odd = [lambda r: r.fill_(0.0)[::2].fill_(-0.0), lambda r: r.fill_(-2.0)[V - 1:].fill_(9.0), lambda r: r.fill_(nan),
+           lambda r: r.fill_(-inf)[:1].fill_(-5.0), lambda r: r.fill_(-1.0)[::3].fill_(nan), lambda r: r[::5].fill_(inf),
+           lambda r: r[V // 2:].fill_(torch.finfo(dtype).min), lambda r: r.fill_(-0.5)[V - 3:].fill_(-0.25)]
+    for i in range(R if R < 24 else 0, R):
+        if i % 3 == 0:
+            odd[i // 3 % len(odd)](x[i])
+    if R < 24:
+        odd[1](x[0])
+    T = rng.choice([0.0, 0.7, 1.0, 40.0], R)
+    print(f"[sample accept] long rows {R} x {V} {dtype}", flush=True)
+    _check(x, np.zeros(R, np.int64), np.arange(1, R + 1), [], [], 0, rng.random(R), T, rng.integers(0, 2 * V, R),
+           rng.random(R) * 1.3, cuda)
+
+
+@pytest.mark.gpu
 def test_uniforms_at_and_past_their_ends(cuda):
     x = torch.randn(8, 501, generator=torch.Generator().manual_seed(4)).bfloat16()
     u = [0.0, -1.0, float("nan"), 1.0, 7.0, float("inf"), 1 - 2.0 ** -24, 2.0 ** -30]

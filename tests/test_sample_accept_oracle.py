@@ -107,4 +107,4 @@ def test_refusals_without_a_device():
     assert call(logits=None) == call(ld=7) == call(V=0) == call(rows=0) == call(drafts=-1) == call(B=-1) == 1
     assert call(spec=-1) == call(u=None) == call(T=None) == call(path=None) == call(ws=None) == call(ids=None) == 1
     assert call(V=(1 << 24) + 1, ld=1 << 25) == 2
-    assert L.cfh_tree_sample_ws_bytes(5) == 40 and L.cfh_tree_sample_ws_bytes(-1) == -1
+    assert L.cfh_tree_sample_ws_bytes(5, 64) >= 40 and L.cfh_tree_sample_ws_bytes(-1, 64) == L.cfh_tree_sample_ws_bytes(5, 0) == -1
