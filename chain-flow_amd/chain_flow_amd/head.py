@@ -444,7 +444,8 @@ def matvec4(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, *, table
             ids: torch.Tensor | None = None, ids_stride: int = 1, out: torch.Tensor | None = None) -> torch.Tensor:
     """fp16(x @ w.T) [M, n] of fp16 rows x [M, d] (rows may be strided) with 4-bit weights as ``quantize4`` makes them: weight
     uint8 [n, K / 2], scale fp16 [n, K / group], K a multiple of 128, the group of 32, 64 or 128 columns being K over the
-    scales' columns.  Products and sums are fp32.  The weights are read once for up to 16 rows.
+    scales' columns.  Products and sums are fp32 (a row with a NaN or an infinity is
+    NaN throughout: all of a group's columns are in one sum).  The weights are read once for up to 16 rows.
 
     With ``table`` [V, r] fp16 and ``ids`` (int32; row m's at m * ids_stride), row ids[m] of the table (outside it: the nearest)
     stands behind x's d columns, d + r = K."""
@@ -507,7 +508,8 @@ class QuantHead:
         self.n = self.weight.shape[0]
         self.group = group
         self.image = None
-        self._zero = None
+        # the markov columns of a row without prev (made here: a buffer made in a captured call would be the graph's)
+        self._zero = torch.zeros(1, self.r, dtype=torch.float16, device=lm_w.device) if self.r else None
 
     map = ShortlistHead.map
 
@@ -516,9 +518,7 @@ class QuantHead:
         """h [M, d] fp16, prev (global ids) -> fp16 logits [M, n] (head + markov bias; without ``prev`` the head's alone)."""
         if self.w1 is None:
             return matvec4(h, self.weight, self.scale, out=out)
-        if prev is None:                       # a row of zeros for the markov columns
-            if self._zero is None:
-                self._zero = torch.zeros(1, self.r, dtype=torch.float16, device=h.device)
+        if prev is None:
             return matvec4(h, self.weight, self.scale, table=self._zero, out=out,
                            ids=torch.zeros(h.shape[0], dtype=torch.int32, device=h.device))
         return matvec4(h, self.weight, self.scale, table=self.w1, ids=prev.reshape(-1).to(torch.int32), ids_stride=prev_stride, out=out)

@@ -1,8 +1,8 @@
 """The 4-bit head on the GPU against float64: quantised weights equal, products within the roundings.
 
-A product's whole numbers and fp16 values multiply exactly in fp32.  A group's G terms are added in fp32 in some order: off by
-at most G 2^-23 of the sum of their magnitudes (2^-23 a step also where a unit truncates); the scaled groups by as much
-a group, one more for the scaling; then one rounding to fp16, 2^-11 of the value (2^-25 below its normal range)."""
+A product's whole numbers and fp16 values multiply exactly in fp32.  (The kernel's are u + 16, and 24 times a group's sum of x is
+taken off: the bound for |u - 8| alone is the stricter one.)  A group's G terms are added in fp32 in some order: off by
+at most G 2^-23 of the sum of their magnitudes (2^-23 a step also where a unit truncates); the scaled groups by as much a group, one more for the scaling; then one rounding to fp16, 2^-11 of the value (2^-25 below its normal range)."""
 from __future__ import annotations
 
 import numpy as np
@@ -202,3 +202,25 @@ def test_products_in_a_graph(cuda):
         torch.cuda.synchronize()
         print(f"[matvec4 graph] replay {i}", flush=True)
         assert torch.equal(y, want)
+
+
+@pytest.mark.gpu
+def test_head_first_used_in_a_graph(cuda):
+    """Logits without previous tokens, captured before any eager use: eager calls before the first replay are right."""
+    g = torch.Generator().manual_seed(3)
+    lm, w1, w2 = (torch.randn(*s, generator=g).half().to(cuda) for s in ((500, 256), (500, 128), (500, 128)))
+    h = torch.randn(3, 256, generator=g).half().to(cuda)
+    head = QuantHead(lm, None, w1, w2)
+    matvec4(h, *quantize4(lm))                     # (loads the library)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = head.logits(h)
+    eager = head.logits(h).clone()
+    for i in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        print(f"[4-bit head in a graph] replay {i}", flush=True)
+        assert torch.equal(y, eager) and torch.equal(head.logits(h), eager)
+    _close(eager, np.concatenate([to64(h), np.zeros((3, 128))], 1),
+           ohead.dequant4(ohead.unpack4(head.weight.cpu().numpy()), to64(head.scale)), 64)
