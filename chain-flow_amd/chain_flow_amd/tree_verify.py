@@ -177,7 +177,7 @@ def tree_sample_accept(logits, cu_num_draft_tokens, cu_num_sampled_tokens, draft
                               ("top_k", top_k, B, (torch.int32, torch.int64)), ("top_p", top_p, B, (torch.float32,))):
         if t is None and name[:3] == "top":
             continue
-        if t.shape != (n,) or t.dtype not in kinds or t.get_device() != dev:
+        if not isinstance(t, torch.Tensor) or t.shape != (n,) or t.dtype not in kinds or t.get_device() != dev:
             raise ValueError(f"{name} must be {' or '.join(str(k) for k in kinds)} [{n}] on cuda:{dev}")
     cd, cs = _host(cu_num_draft_tokens), _host(cu_num_sampled_tokens)
     if B and cd is not None and cs is not None and not _counts_fit(cd, cs, R, D, max_spec_len):

@@ -236,7 +236,7 @@ class FlowDrafterProposer:
         if self.head_bits == 4:
             if self._twopass_explicit and self.twopass_m:
                 raise ValueError("CF_HEAD_BITS=4 searches the head in one pass: it does not go with CF_TWOPASS_M")
-            self.twopass_m = 0
+            self.twopass_m, self.twopass_shared = 0, False
         self.async_spec = os.environ.get("CF_ASYNC_SPEC", "0") == "1"
         self.drafter: Drafter | None = None
         self._target = None

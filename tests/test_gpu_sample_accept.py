@@ -246,7 +246,7 @@ def test_refusals(cuda):
     u, T = torch.zeros(3, device=cuda), torch.ones(1, device=cuda)
     ok = ([2], [3], [1, 2], [-1, 0], 2)
     tree_sample_accept(x, *ok, u, T)
-    for bad in ((u[:2], T), (u.double(), T), (u.cpu(), T), (u, T.half()), (u, torch.ones(2, device=cuda))):
+    for bad in ((u[:2], T), (u.double(), T), (u.cpu(), T), (u, T.half()), (u, torch.ones(2, device=cuda)), (u, 1.0), ([0.5] * 3, T)):
         with pytest.raises(ValueError):
             tree_sample_accept(x, *ok, *bad)
     for kw in (dict(top_k=T), dict(top_p=u), dict(top_p=T.int()), dict(status=T)):
