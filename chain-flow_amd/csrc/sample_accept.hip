@@ -193,10 +193,10 @@ __global__ void __launch_bounds__(1024, 4) k_sample_parts(SampleArgs a) {
 // own and adds at most 1 to the next, so that the sum only falls.  Then (a constant row, a masked one) half of the values
 // are counted at a time, in twice the bits, which V cannot leave: 8 bits and 64 KB for V < 65,536, 16 bits and 128 KB
 // above.  The row is read again, from the caches, for the drawn token's index.
-// 8 bits below 65,536 values, as two workgroups then share a CU (1,968 rows of 32,000 logits: 90 us in fp16, 76 in bf16; with
-// 1,024 threads and 16 bits 136 and 125).  What bounds a row of 248,320 bf16 logits on its CU: 17 us of counting (an LDS atomic a logit, a wave's 64 in
-// 10 cycles), 2.2 the cells (fp16: 4.2, more values are in use), 2.1 a search (one wave's latency), 4 the index.  1,968 rows
-// of 32,000: 12 us a row and CU in fp16, 1.4 TB/s; the stages of two rows overlap there, and the searches' latency and the
+// 8 bits below 65,536 values, as two workgroups then share a CU (1,968 rows of 32,000 logits: 90 us in fp16, 76 in bf16, 136 and 125
+// with 1,024 threads and 16 bits; since then 85 and 70).  What bounds a row of 248,320 bf16 logits on its CU: 17 us of counting (an LDS atomic a logit, a wave's 64 in
+// 10 cycles), 2.2 the cells (fp16: 4.2, more values are in use), 1.5 a search (one wave's latency), 4 the index.  1,968 rows
+// of 32,000: 11 us a row and CU in fp16, 1.5 TB/s; the stages of two rows overlap there, and the searches' latency and the
 // weights of many values are what remains.
 template <bool BF, bool VEC, int T, int BITS>
 __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
@@ -262,18 +262,29 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
     if (t < V % 8) add_wide(x[8 * whole + t], 1u);
     __syncthreads();
   };
-  // counts of the N values at order positions N (T g + tt) .., 0 for those that are no numbers above -inf
-  auto counts_of = [&](int g, int tt, unsigned (&c)[N]) __attribute__((always_inline)) {
-    const int o = N * (g * T + tt), raw = o < 0x8000 ? 0x7fff - o - (N - 1) : o;      // the lowest of the patterns
-    const uint4* w = (const uint4*)(hist + (raw & (WORDS - 1)));
+  // counts of this lane's N values of a cell (the same one in the whole wave), 0 for those that are no numbers above -inf
+  auto counts_of = [&](int cell, unsigned (&c)[N]) __attribute__((always_inline)) {
+    const bool pos = cell < CELLS / 2;
+    const int o0 = cell * 64 * N, raw0 = pos ? 0x7fff - o0 - (64 * N - 1) : o0;      // its first position, its lowest pattern
+    const uint4* w = (const uint4*)(hist + (raw0 & (WORDS - 1)) + (pos ? 63 - lane : lane) * N);
     const uint4 w0 = w[0], w1 = w[1];
     const unsigned v[N] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-    const int bits = wide ? 2 * BITS : BITS, shift = (wide ? raw & 0x7fff : raw) >> LOG;
+    const int bits = wide ? 2 * BITS : BITS, field = (wide ? raw0 & 0x7fff : raw0) >> LOG;
+    const int shift = bits == 32 ? 0 : field * bits;
     const unsigned mask = bits == 32 ? ~0u : (1u << bits) - 1;
+    if (pos) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const unsigned n = v[o < 0x8000 ? N - 1 - e : e] >> (bits == 32 ? 0 : shift * bits) & mask;
-      c[e] = o + e >= O_FIRST<BF> && o + e <= O_LAST<BF> ? n : 0;
+      for (int e = 0; e < N; ++e) c[e] = v[N - 1 - e] >> shift & mask;
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) c[e] = v[e] >> shift & mask;
+    }
+    if (o0 < O_FIRST<BF> || o0 + 64 * N - 1 > O_LAST<BF>) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int o = o0 + N * lane + e;
+        c[e] = o >= O_FIRST<BF> && o <= O_LAST<BF> ? c[e] : 0;
+      }
     }
   };
   int top = -1;
@@ -359,15 +370,16 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
   auto cells = [&](int g0, int g1) __attribute__((always_inline)) {
 #pragma unroll 1
     for (int g = g0; g < g1; ++g) {
+      const int cell = __builtin_amdgcn_readfirstlane(g * W + wave);
       unsigned c[N];
-      counts_of(g, t, c);
+      counts_of(cell, c);
       int n = 0;
 #pragma unroll
       for (int e = 0; e < N; ++e) n += (int)c[e];
-      double s = n ? weight_of(N * (g * T + t), c) : 0.0;
+      double s = n ? weight_of(64 * N * cell + N * lane, c) : 0.0;
       n = scan64(n);
       s = scan64(s);
-      if (lane == 63) { cell_n[g * W + wave] = n; cell_m[g * W + wave] = s; }
+      if (lane == 63) { cell_n[cell] = n; cell_m[cell] = s; }
     }
   };
 
@@ -459,65 +471,81 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
 #pragma unroll 1
       for (int stage = 0; stage < 3; ++stage) {
         const bool by_n = stage == 0, past = stage == 2;
-        double goal = 0.0;
+        double goal = 0.0, below = 0.0;              // reached by a sum above `below`
         if (by_n) {
           if (K < 1 || K >= kept_n) continue;
           kept_n = K;
         } else if (!past) {
           if (!(P < 1.f)) continue;
-          goal = (double)P * kept_m;
+          goal = fmax((double)P * kept_m, 0x1p-60);  // (the first token at least: it weighs 1)
+          below = __longlong_as_double(__double_as_longlong(goal) - 1);
         } else {
-          goal = (u > 0.f ? (double)fminf(u, 0x1.fffffep-1f) : 0.0) * kept_m;
+          below = goal = (u > 0.f ? (double)fminf(u, 0x1.fffffep-1f) : 0.0) * kept_m;
         }
-        int hit = -1, last = -1;
+        // the first of the places that count and reach it, else the last that counts (a bit a lane)
+        auto choose = [](unsigned long long counts, unsigned long long reaches) __attribute__((always_inline)) {
+          reaches &= counts;
+          return reaches ? __builtin_ctzll(reaches) : counts ? 63 - __builtin_clzll(counts) : 0;
+        };
+        unsigned long long in[2], reach[2];
 #pragma unroll
-        for (int i = 1; i >= 0; --i) {
-          if (upto_n[i + 1] == upto_n[i] || upto_n[i] >= kept_n || (!by_n && !(upto_m[i + 1] > upto_m[i]))) continue;
-          if (last < 0) last = i;
-          if (by_n ? upto_n[i + 1] >= kept_n : past ? upto_m[i + 1] > goal : upto_m[i + 1] >= goal) hit = i;
+        for (int i = 0; i < 2; ++i) {
+          in[i] = __ballot(upto_n[i + 1] > upto_n[i] && upto_n[i] < kept_n && (by_n || upto_m[i + 1] > upto_m[i]));
+          reach[i] = in[i] & __ballot(by_n ? upto_n[i + 1] >= kept_n : upto_m[i + 1] > below);
         }
-        const unsigned long long any = __ballot(hit >= 0), some = __ballot(last >= 0);
-        const int at = any ? __builtin_ctzll(any) : some ? 63 - __builtin_clzll(some) : 0;
-        const int i = max(__builtin_amdgcn_readlane(any ? hit : last, at), 0);
+        const int at = choose(in[0] | in[1], reach[0] | reach[1]);
+        const int i = (reach[0] | reach[1]) ? !(reach[0] >> at & 1) : (int)(in[1] >> at & 1);
         if (wide) {                                  // (wave 0's: kept_n and the rest are its own)
           if (t == 0) s_half[stage] = at >= 32;
           __syncthreads();
           if (half != s_half[stage]) count_half(!half);
           if (wave) continue;
         }
-        const int cell = 2 * at + i, g = cell / W, tt = cell % W * 64 + lane, o = N * (g * T + tt);
+        const int cell = 2 * at + i, o = 64 * N * cell + N * lane;
         unsigned c[N];
-        counts_of(g, tt, c);
+        counts_of(cell, c);
         int ns = 0;
 #pragma unroll
         for (int e = 0; e < N; ++e) ns += (int)c[e];
-        double w[N] = {}, ss = 0.0;
-        if (ns) weights(o, [&](int e, double x) __attribute__((always_inline)) { w[e] = x; ss = fma((double)c[e], x, ss); });
-        int nb = scan64(ns) - ns + __builtin_amdgcn_readlane(i ? upto_n[1] : upto_n[0], at);
+        double w[N], ss = 0.0;
+        if (64 * N * cell < top) {
+          weights(o, [&](int e, double x) __attribute__((always_inline)) { w[e] = x; });
+        } else {
+          const double r = ratio[(raw_of(o) & 0x7fff) >> MANT];
+          w[0] = pow2(table, isinf(m) ? o == top ? 0.0 : -INFINITY : (value_of<BF>(o) - m) * rate);
+#pragma unroll
+          for (int e = 1; e < N; ++e) w[e] = w[e - 1] * r;
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          w[e] = c[e] ? w[e] : 0.0;
+          ss = fma((double)c[e], w[e], ss);
+        }
+        const int nb = scan64(ns) - ns + __builtin_amdgcn_readlane(i ? upto_n[1] : upto_n[0], at);
         double mb = __shfl_up(scan64(ss), 1);
         if (lane == 0) mb = 0.0;
         mb += from_lane(i ? upto_m[1] : upto_m[0], at);
-        Place first = {-1, 0, 0.0, 0.0, 0}, end = first;   // the first place that reaches the goal, the last of any weight
+        // the lane, then its N values a lane each
+        const bool counts = ns > 0 && nb < kept_n && (by_n || ss > 0.0);
+        const int from = choose(__ballot(counts), __ballot(by_n ? nb + ns >= kept_n : mb + ss > below));
+        unsigned ce = 0;
+        double we = 0.0;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-          const double m1 = fma((double)c[e], w[e], mb);
-          const bool in = c[e] && nb < kept_n && (by_n || w[e] > 0.0);
-          const bool hit = in && first.o < 0 && (by_n ? nb + (int)c[e] >= kept_n : past ? m1 > goal : m1 >= goal);
-          first.o = hit ? o + e : first.o; first.count = hit ? c[e] : first.count; first.w = hit ? w[e] : first.w;
-          first.before_m = hit ? mb : first.before_m; first.before_n = hit ? nb : first.before_n;
-          end.o = in ? o + e : end.o; end.count = in ? c[e] : end.count; end.w = in ? w[e] : end.w;
-          end.before_m = in ? mb : end.before_m; end.before_n = in ? nb : end.before_n;
-          nb += (int)c[e];
-          mb = m1;
+          const unsigned x = __builtin_amdgcn_readlane(c[e], from);
+          const double y = from_lane(w[e], from);
+          ce = lane == e ? x : ce;
+          we = lane == e ? y : we;
         }
-        const unsigned long long reach = __ballot(first.o >= 0), weigh = __ballot(end.o >= 0);
-        const int from = reach ? __builtin_ctzll(reach) : weigh ? 63 - __builtin_clzll(weigh) : 0;
-        if (!reach) first = end;
-        p.o = __builtin_amdgcn_readlane(first.o, from);
-        p.count = __builtin_amdgcn_readlane(first.count, from);
-        p.w = from_lane(first.w, from);
-        p.before_m = from_lane(first.before_m, from);
-        p.before_n = __builtin_amdgcn_readlane(first.before_n, from);
+        const int n1 = __builtin_amdgcn_readlane(nb, from) + row_scan((int)ce), n0 = n1 - (int)ce;
+        const double sum = row_scan((double)ce * we), m0 = from_lane(mb, from), m1 = m0 + sum;
+        const double before = m0 + moved<DPP_SHR1, 0xf>(sum);
+        const int pick = choose(__ballot(ce && n0 < kept_n && (by_n || we > 0.0)), __ballot(by_n ? n1 >= kept_n : m1 > below));
+        p.o = 64 * N * cell + N * from + pick;
+        p.count = __builtin_amdgcn_readlane(ce, pick);
+        p.w = from_lane(we, pick);
+        p.before_m = from_lane(before, pick);
+        p.before_n = __builtin_amdgcn_readlane(n0, pick);
         const int most = min((int)p.count, kept_n - p.before_n);
         if (by_n) {
           kept_m = p.before_m + (double)most * p.w;
