@@ -78,6 +78,7 @@ SIGNATURES = {
     "cfh_cand_topm": (_I, [_VP, C.c_longlong, _VP, _I, _I, _I, _I, _VP, _VP, _VP, _VP, _VP]),
     "cfh_head_logits": (_I, [_VP, _I, _I, _VP, _VP, _I, _VP, _VP, _I, _I, _VP, _VP, _VP]),
     "cfh_row_topk": (_I, [_VP, _I, _I, _I, _VP, _VP, _VP, _VP]),
+    "cfh_row_topk_sets": (_I, [_VP, _I, _I, _I, _VP, _VP, _VP, _VP, _VP]),
     "cfh_quantize4": (_I, [_VP, _VP, _VP, _I, _I, _I, _I, _VP, _VP, _VP]),
     "cfh_matvec4": (_I, [_VP, C.c_longlong, _I, _I, _VP, _I, _VP, _I, _I, _I, _VP, _I, _VP, _I, _I, _VP, C.c_longlong, _VP]),
     "cfh_head_ws_bytes": (_I64, [_I, _I, _I]),

@@ -37,7 +37,8 @@ class Drafter:
     rescores only those rows, renormalised over them.
 
     ``head_bits`` = 4 holds the head (shortlisted lm_head and markov.w2) at 4 bits with a scale for each ``head_group``
-    columns (``QuantHead``: a quarter of the bytes a depth reads); its search is the one-pass one."""
+    columns (``QuantHead``: a quarter of the bytes a depth reads, for up to 16 beams a depth; worth it up to some 40, requests times
+    width); its search is the one-pass one."""
 
     def __init__(self, cfg: TreeFlowConfig, weights: dict, shortlist: torch.Tensor | None, device="cuda",
                  path_trim: bool = True, twopass_m: int = 0, twopass_shared: bool = True,

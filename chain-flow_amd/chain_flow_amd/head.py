@@ -396,15 +396,21 @@ class GemmHead:
         return vals, ids, lse
 
 
-def row_topk(logits: torch.Tensor, k: int):
-    """Per-row log-softmax top-k of fp16 logits [M, n] -> (vals f32, ids int32, lse f32)."""
+def row_topk(logits: torch.Tensor, k: int, split: bool = False):
+    """Per-row log-softmax top-k of fp16 logits [M, n] -> (vals f32, ids int32, lse f32).  ``split``: a row's columns over many
+    workgroups, for few long rows; the same ids, lse but for the order of an fp32 sum."""
     M, n = logits.shape
     logits = logits.contiguous()
     vals = torch.empty(M, k, dtype=torch.float32, device=logits.device)
     ids = torch.empty(M, k, dtype=torch.int32, device=logits.device)
     lse = torch.empty(M, dtype=torch.float32, device=logits.device)
-    _lib.check(_lib.lib().cfh_row_topk(logits.data_ptr(), M, n, k, vals.data_ptr(), ids.data_ptr(),
-                                       lse.data_ptr(), _lib.stream_handle()), "cfh_row_topk")
+    args = (logits.data_ptr(), M, n, k, vals.data_ptr(), ids.data_ptr(), lse.data_ptr())
+    L = _lib.lib()
+    if split:
+        ws = torch.empty(max(int(L.cfh_head_ws_bytes(M, n, k)), 16), dtype=torch.uint8, device=logits.device)
+        _lib.check(L.cfh_row_topk_sets(*args, ws.data_ptr(), _lib.stream_handle()), "cfh_row_topk_sets")
+    else:
+        _lib.check(L.cfh_row_topk(*args, _lib.stream_handle()), "cfh_row_topk")
     return vals, ids, lse
 
 
@@ -491,7 +497,8 @@ def matvec4(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, *, table
 class QuantHead:
     """``ShortlistHead`` at 4 bits: the shortlisted rows of lm_head and, behind their columns, of markov.w2 as ``quantize4``
     weights (174 MB for 62,642 rows at d = 5120, r = 256, groups of 64, against 673 MB), so that a row's logit is one product
-    of [h, w1[prev]] and is rounded once.  The drafts it makes differ from the fp16 head's; what the target's verify
+    of [h, w1[prev]] and is rounded once.  A depth's top k of those rows takes 40 us where the fp16 head's takes 110 (1 to 8 rows;
+    49 and 113 at 16); every 16 rows read the weights again (32 rows: 89 and 112, 48: 126 and 112).  The drafts it makes differ from the fp16 head's; what the target's verify
     accepts of them is distributed as before."""
 
     def __init__(self, lm_w: torch.Tensor, shortlist: torch.Tensor | None, w1: torch.Tensor | None = None,
@@ -526,7 +533,7 @@ class QuantHead:
     def topk(self, h: torch.Tensor, k: int, prev: torch.Tensor | None = None, prev_stride: int = 1,
              logits: torch.Tensor | None = None):
         """-> (log-prob values [M, k] f32, shortlist-local ids [M, k] int32, lse [M] f32), as ``ShortlistHead.topk``."""
-        return row_topk(self.logits(h, prev, prev_stride, logits), k)
+        return row_topk(self.logits(h, prev, prev_stride, logits), k, split=True)
 
 
 def pack_linear(w: torch.Tensor) -> torch.Tensor:

@@ -38,6 +38,17 @@ __device__ __forceinline__ double from_lane(double v, int lane) {
   return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
 }
 
+// the largest of the wave's unsigned numbers, for all lanes
+__device__ __forceinline__ unsigned wave_largest(unsigned v) {
+  v = max(v, (unsigned)moved<DPP_SHR1, 0xf>((int)v));
+  v = max(v, (unsigned)moved<DPP_SHR2, 0xf>((int)v));
+  v = max(v, (unsigned)moved<DPP_SHR4, 0xf>((int)v));
+  v = max(v, (unsigned)moved<DPP_SHR8, 0xf>((int)v));
+  v = max(v, (unsigned)moved<DPP_BCAST15, 0xa>((int)v));
+  v = max(v, (unsigned)moved<DPP_BCAST31, 0xc>((int)v));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
 // Two sums over lanes in the operations of one: with a's odd groups of L lanes exchanged for b's even ones, a + b is a's two
 // halves' sum in the even groups and b's in the odd ones.
 template <int L>

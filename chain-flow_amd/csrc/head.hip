@@ -19,6 +19,7 @@
 // kernel combines the blocks into the row's log-sum-exp and top-k.
 #include <limits.h>
 
+#include "cfh_scan.h"
 #include "cfh_wide.h"
 
 namespace {
@@ -520,6 +521,66 @@ __global__ void __launch_bounds__(TK_THREADS) k_topk(TopkArgs a) {
     vals[r] = ok ? bv - lse : -INFINITY;
     ids[r] = ok ? bi : -1;
   });
+}
+
+// The same in two launches, for rows that are few and long: a wave takes 512 columns of a row, eight a lane, as 32-bit keys that
+// order like (value, lower column first), sorts its lanes' eights and takes the k best off their heads; k_merge_wave joins the
+// sets.  One workgroup a row spends 76 us on 62,642 columns; this and the join 8 (1 to 16 rows).
+constexpr int TS_COLS = 512;
+
+__global__ void __launch_bounds__(256) k_topk_sets(TopkArgs a, void* ws, int nsets) {
+  const int lane = threadIdx.x & 63, set = blockIdx.x * 4 + (threadIdx.x >> 6), m = blockIdx.y;
+  if (set >= nsets) return;
+  const uint16_t* L = (const uint16_t*)a.logits + (size_t)m * a.ld + (size_t)set * TS_COLS;
+  const int n = min(TS_COLS, a.n - set * TS_COLS);
+  constexpr int N = TS_COLS / 64;
+  unsigned raw[N], key[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) raw[i] = L[min(i * 64 + lane, n - 1)];
+  float mx = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int at = i * 64 + lane;
+    const bool nan = (raw[i] & 0x7fffu) > 0x7c00u;
+    const unsigned order = raw[i] & 0x8000u ? ~raw[i] & 0xffffu : raw[i] | 0x8000u;
+    key[i] = at < n && !nan ? order << 16 | (0xffffu - at) : 0;             // (0: none)
+    if (at < n) mx = fmaxf(mx, (float)__builtin_bit_cast(h16, (uint16_t)raw[i]));
+  }
+  mx = wave_max(mx);
+  float se = 0.f;
+  if (mx != -INFINITY) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i * 64 + lane < n) se += expf((float)__builtin_bit_cast(h16, (uint16_t)raw[i]) - mx);
+    se = wave_sum(se);
+  }
+  auto order2 = [&](int i, int j) { const unsigned x = max(key[i], key[j]); key[j] = min(key[i], key[j]); key[i] = x; };
+  order2(0, 1); order2(2, 3); order2(4, 5); order2(6, 7);
+  order2(0, 2); order2(1, 3); order2(4, 6); order2(5, 7);
+  order2(1, 2); order2(5, 6);
+  order2(0, 4); order2(1, 5); order2(2, 6); order2(3, 7);
+  order2(2, 4); order2(3, 5);
+  order2(1, 2); order2(3, 4); order2(5, 6);
+  unsigned mine = 0;
+  for (int r = 0; r < a.k; ++r) {
+    const unsigned best = wave_largest(key[0]);
+    if (lane == r) mine = best;
+    if (key[0] == best) {
+#pragma unroll
+      for (int i = 0; i < N - 1; ++i) key[i] = key[i + 1];
+      key[N - 1] = 0;
+    }
+  }
+  const Cands cd = carve_cands(ws, a.M, nsets, a.k);
+  const size_t base = (size_t)m * nsets + set;
+  if (lane < a.k) {
+    const unsigned o = mine >> 16;
+    const uint16_t v = o & 0x8000u ? o & 0x7fffu : ~o & 0xffffu;
+    cd.cv[base * a.k + lane] = mine ? (float)__builtin_bit_cast(h16, v) : -INFINITY;
+    cd.ci[base * a.k + lane] = mine ? set * TS_COLS + (int)(0xffffu - (mine & 0xffffu)) : INT_MAX;
+  }
+  // (a NaN sum as the maximum's: the join takes only sums above 0)
+  if (lane == 0) { cd.cs[base * 2] = isnan(se) ? se : mx; cd.cs[base * 2 + 1] = isnan(se) ? 1.f : se; }
 }
 
 // ---------------------------------------------------------------------------- MFMA GEMM head
@@ -1554,6 +1615,18 @@ int cfh_row_topk(const void* logits, int M, int n, int k, float* vals, int32_t* 
   hipLaunchKernelGGL(k_topk, dim3(M), dim3(TK_THREADS), 0, (hipStream_t)stream, ta);
   CFH_LAUNCH_CHECK();
   return CFH_OK;
+}
+
+int cfh_row_topk_sets(const void* logits, int M, int n, int k, float* vals, int32_t* ids, float* lse, void* ws,
+                      void* stream) {
+  if (!logits || !vals || !ids || !ws || M < 1 || n < 1 || k < 1 || k > KMAX) return CFH_E_INVALID;
+  if (M > 65535) return CFH_E_UNSUPPORTED;
+  TopkArgs ta = {};
+  ta.logits = (const h16*)logits; ta.ld = n; ta.M = M; ta.n = n; ta.k = k;
+  const int nsets = (n + TS_COLS - 1) / TS_COLS;
+  hipLaunchKernelGGL(k_topk_sets, dim3((nsets + 3) / 4, M), dim3(256), 0, (hipStream_t)stream, ta, ws, nsets);
+  CFH_LAUNCH_CHECK();
+  return launch_merge(ws, M, nsets, k, vals, ids, lse, (hipStream_t)stream);
 }
 
 int cfh_head_topk(const void* h, int M, int d, const void* W, const int32_t* sl, int n, const void* a,

@@ -32,7 +32,8 @@ __device__ __forceinline__ Part part_of(const PoolArgs& c, int i) {
 // ---------------------------------------------------------------------------- accepted rows
 // Node path[s][i] of sequence s, row lens[s] + path[s][i], becomes row lens[s] + i, in every layer.  The nodes ascend, so
 // row i never lies behind its source and no source lies before the row in hand: a thread that moves one 16-byte column
-// of all rows in order, whole batches read before they are written, needs no other thread.
+// of all rows in order, whole batches read before they are written, needs no other thread.  Bound by round trips (lengths, path
+// and table, rows), not bytes: one path in 8 layers of 4 x 256 bf16 4.9 us, 48 in 16 layers of 2 x 128 e4m3 (2.5 MB) 5.8.
 struct CommitArgs {
   PoolArgs c;
   const int* table;          // [S][table_ld]
@@ -115,7 +116,8 @@ __global__ void __launch_bounds__(256) k_commit(CommitArgs a) {
 // ---------------------------------------------------------------------------- fork
 // Row dst[i] of the table lets go of its pages and shares row src[i]'s (src -1: none).  No source is a destination
 // of another pair and destinations differ (pairs that break this are skipped), so that pairs need no order; holders
-// are counted by atomic additions, whose order does not matter.
+// are counted by atomic additions, whose order does not matter.  A workgroup a pair, two round trips through the table: 30,011
+// tokens' 469 pages shared by 8 sequences 5.4 us, 24 prompts of 13 pages by 4 each 4.2.
 struct ForkArgs {
   int* table;
   int* room;
@@ -249,7 +251,7 @@ __device__ __forceinline__ int last_at(const int* first, int n, int v) {
   return lo;
 }
 
-// Then, in one workgroup: what each sequence needs, in order, and the lowest free pages for it.  A shared last page
+// Then, in one workgroup, as every place depends on those before it: what each sequence needs, in order, and the lowest free pages for it.  A shared last page
 // that is filled in part is copied before its sequence grows: by all but the last of its holders.  ONE: letting go and filling in,
 // too.
 template <bool ONE>
@@ -387,7 +389,9 @@ __global__ void __launch_bounds__(64) k_fill(ResizeArgs a) {
   if (t == 0) a.room[s] = a.new_room[s];
 }
 
-// Last, the copies: a piece of a page of one layer's keys or values at a time.
+// Last, the copies: a piece of a page of one layer's keys or values at a time.  96 pages in 8 layers (29 of their 64 rows of 4 x 256
+// bf16 on average: 180 MB in and out) 27 us, 6.6 TB/s.  At most 4,096 workgroups, as the number of copies is known here only:
+// those and a plan without copies take 55.3 and 6.9 us, with 1,024 of them 56.1 and 6.6, with 16,384 54.3 and 9.2.
 constexpr int PIECE = 16384;
 
 __global__ void __launch_bounds__(256) k_copy(ResizeArgs a) {

@@ -70,7 +70,10 @@ __device__ __forceinline__ void swap4(unsigned (&w)[4]) {
   s16(w[2], w[3]);
 }
 
-// G: columns a scale; NW waves.
+// G: columns a scale; NW waves.  Bound by the weights' bytes where they are many: 62,642 rows of 2,560 columns, one row of x, 16.0
+// us (5.2 TB/s); of 5,376, four rows, 32.9 (5.5); by the launch, x's way into LDS and the joined parts where they are few: 8,191 rows of
+// 4,096, 16 rows of x, 10.4 us for 19 MB.  A step of 128 columns costs a wave some 57 operations beside its loads, so that two
+// steps' loads in flight are enough (four: 18.3 -> 20.5 us for one row of x, as registers leave fewer waves).
 template <int G, int NW>
 __global__ void __launch_bounds__(NW * 64, 4) k_matvec4(MvArgs a) {
   // x [M][chunk columns + 8], eights of them in the order 0 4 1 5 2 6 3 7; behind it -24 times its sums [columns / G][16 rows]
@@ -106,7 +109,7 @@ __global__ void __launch_bounds__(NW * 64, 4) k_matvec4(MvArgs a) {
   const int ldx = a.chunk * 128 + 8;
   float* sums = (float*)(xs + a.M * ldx);
   auto stage = [&](int c0, int c1) __attribute__((always_inline)) {
-    constexpr int XB = 4;                            // eights of columns a thread has in flight
+    constexpr int XB = 4;                            // eights of columns a thread has in flight (16 rows of 4,096: 10.8 us; 2: 12.0)
     const int eights = (c1 - c0) * 16, all = a.M * eights;
     for (int i0 = threadIdx.x; i0 < all; i0 += XB * NW * 64) {
       h16x8 v[XB];
@@ -235,7 +238,7 @@ struct QuantArgs {
   int n, d, r, group;
 };
 
-// eight columns a thread, group / 8 threads a group
+// Eight columns a thread, group / 8 threads a group: run once, when a head is laid out.
 __global__ void __launch_bounds__(256) k_quantize4(QuantArgs a) {
   const int K = a.d + a.r, per = K / 8;
   const size_t all = (size_t)a.n * per;
@@ -311,6 +314,9 @@ int cfh_matvec4(const void* x, long long ld_x, int M, int d, const uint8_t* w, i
     v.y = (h16*)y + m0 * ld_y; v.ld_y = ld_y;
     auto launch = [&](auto g, auto nw) -> int {
       constexpr int NW = nw.value;
+      // K split over a workgroup's waves until there are 200 workgroups: 16 rows times 8,191 x 4,096, 11.7 us in 8 parts, 14.4 in
+      // 4, 18.0 in 16.  Unsplit, x that two workgroups of a compute unit cannot both hold comes in chunks (16 rows of 5,376: 47
+      // us; in two launches of 8 rows 77).
       int ks = 1;
       while (ks < NW && tiles * ks < 200 * NW) ks *= 2;
       long long c = steps;
@@ -332,6 +338,7 @@ int cfh_matvec4(const void* x, long long ld_x, int M, int d, const uint8_t* w, i
       return group == 32 ? launch(std::integral_constant<int, 32>{}, nw) : group == 64 ? launch(std::integral_constant<int, 64>{}, nw)
                                                                               : launch(std::integral_constant<int, 128>{}, nw);
     };
+    // 16 waves share x where two workgroups of 8 do not fit: 62,642 x 5,376, 8 rows 39.2 us (of 8 waves 40.6), 16 rows 47.1 (50.3)
     const bool big = lds_of(rows, steps) > MV_HALF;
     if (int rc = big ? of_group(std::integral_constant<int, 16>{}) : of_group(std::integral_constant<int, 8>{})) return rc;
   }

@@ -169,8 +169,8 @@ __device__ __forceinline__ int over_all(int v, int* s_int) {
   return v;
 }
 
-// Few long rows leave most CUs idle, and a CU counts a logit a lane and 10 cycles: then each row is counted in parts, a
-// workgroup a part, and k_sample_rows adds the parts' counts up.
+// Few long rows leave most CUs idle, and a CU counts 64 logits in 10 cycles: then each row is counted in parts, a workgroup a
+// part, and k_sample_rows adds the parts' counts up (6 rows of 248,320 in 4 parts: 10 us here and 15.7 there, 31 in one).
 template <bool VEC>
 __global__ void __launch_bounds__(1024, 4) k_sample_parts(SampleArgs a) {
   __shared__ __attribute__((aligned(16))) unsigned hist[PART_WORDS];
@@ -669,7 +669,8 @@ struct WalkArgs {
 
 constexpr int WALK_LDS = 1024;   // drafts of a request staged in LDS
 
-// One wave a request; counts that do not lie in the rows and drafts refuse the request (one of no rows: padding).
+// One wave a request: round trips, the walk itself in LDS (one request 3.8 us, 48 5.6).  Counts that do not lie in the rows and
+// drafts refuse the request (one of no rows: padding).
 __global__ void __launch_bounds__(64) k_sample_walk(WalkArgs a) {
   const int b = blockIdx.x, lane = threadIdx.x;
   const long long d0 = b ? a.cu_draft[b - 1] : 0, d1 = a.cu_draft[b], s0 = b ? a.cu_rows[b - 1] : 0, s1 = a.cu_rows[b];

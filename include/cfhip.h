@@ -273,6 +273,11 @@ int cfh_head_logits(const void* h, int M, int d, const void* W, const int32_t* s
 int cfh_row_topk(const void* logits, int M, int n, int k, float* vals, int32_t* ids, float* lse,
                  void* stream);
 
+/* cfh_row_topk in two launches, a row's columns over many workgroups: ws of cfh_head_ws_bytes(M, n, k) bytes, 16-byte aligned, of the
+ * call's own until it ends.  The same order; lse and vals differ from cfh_row_topk's by the order of an fp32 sum.  M <= 65,535. */
+int cfh_row_topk_sets(const void* logits, int M, int n, int k, float* vals, int32_t* ids, float* lse, void* ws,
+                      void* stream);
+
 /* The head at 4 bits.  Weight rows w [n][ld_w bytes]: column 2 i in the low half of byte i, column 2 i + 1 in its high half, as
  * whole numbers 0 .. 15 that stand for themselves less 8; scale [n][ld_s] fp16, one for `group` (32, 64 or 128) columns.
  *

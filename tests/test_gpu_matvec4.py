@@ -12,7 +12,7 @@ import torch
 from conftest import to64
 from chain_flow_amd.config import flownet
 from chain_flow_amd.drafter import Drafter
-from chain_flow_amd.head import QuantHead, ShortlistHead, matvec4, quantize4
+from chain_flow_amd.head import QuantHead, ShortlistHead, matvec4, quantize4, row_topk
 from chain_flow_amd.weights import make_weights, synthetic_context
 from oracle import beam as obeam
 from oracle import head as ohead
@@ -153,6 +153,41 @@ def test_head_of_4_bits(cuda):
     order = torch.sort(ls, dim=1, descending=True, stable=True)
     assert torch.equal(ids.long(), order.indices[:, :5]) and (vals.double() - order.values[:, :5]).abs().max() < 1e-4
     assert torch.equal(head.map(ids).cpu(), sl[ids.cpu().long()])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,n", [(1, 1), (2, 15), (3, 511), (1, 512), (4, 513), (1, 62642), (5, 4099), (300, 2049), (2, 300001)])
+@pytest.mark.parametrize("k", [1, 4, 16])
+def test_split_top_k(cuda, M, n, k):
+    """A row's top k over many workgroups: ids equal to a stable sort's (lower column first among equals), -1 past the numbers."""
+    x = (torch.randn(M, n, generator=torch.Generator().manual_seed(n)) * 4).half()
+    x[0] = x[0].mul(2).round().div(2)              # many equal ones
+    if n > 20:
+        x[0, 5], x[0, n - 1], x[M - 1, 3] = float("nan"), float("-inf"), float("-inf")
+    if M > 2:
+        x[1] = float("-inf")
+        x[2] = float("nan")
+    print(f"[split top-k] {M} x {n} k {k}", flush=True)
+    vals, ids, lse = (t.cpu() for t in row_topk(x.to(cuda), k, split=True))
+    assert torch.equal(ids, row_topk(x.to(cuda), k)[1].cpu())
+    v = to64(x)
+    for m in range(M):
+        order = np.argsort(np.where(np.isnan(v[m]), np.inf, -v[m]), kind="stable")
+        order = order[: int((~np.isnan(v[m])).sum())][:k]
+        assert ids[m, : len(order)].tolist() == order.tolist() and (ids[m, len(order):] == -1).all()
+        if np.isnan(v[m]).all() or np.isneginf(v[m]).all():
+            assert not torch.isfinite(lse[m])
+        elif np.isnan(v[m]).any():
+            assert torch.isnan(lse[m])
+        else:
+            top = v[m].max()
+            want = top + np.log(np.exp(v[m] - top).sum())
+            # exponentials within 2^-22, n of them added in fp32 by 8 a lane, lanes and sets, the log and a sum: below 2^-17 of 1
+            tol = 2.0 ** -17 + abs(want) * 2.0 ** -22
+            assert abs(float(lse[m]) - want) <= tol
+            got = vals[m, : len(order)].double().numpy()
+            want = v[m][order] - want
+            assert (np.abs(got - want)[np.isfinite(want)] <= tol + np.abs(want[np.isfinite(want)]) * 2.0 ** -23).all()
 
 
 @pytest.mark.gpu
