@@ -220,15 +220,16 @@ def test_many_requests(cuda):
 
 
 @pytest.mark.gpu
-def test_graph_replays_follow_their_inputs(cuda):
-    x, cu_d, cu_r, draft, par, rng = _case([6, 3], 5000, torch.bfloat16, 21)
+@pytest.mark.parametrize("V", [5000, 70001])
+def test_graph_replays_follow_their_inputs(cuda, V):
+    x, cu_d, cu_r, draft, par, rng = _case([6, 3], V, torch.bfloat16, 21)
     ints = lambda v: torch.tensor(np.asarray(v), dtype=torch.int32, device=cuda)                  # noqa: E731
     xg, u = x.to(cuda), torch.rand(x.shape[0], device=cuda)
     args = (ints(cu_d), ints(cu_r), ints(draft), ints(par), 6, u, torch.tensor([1.0, 0.7], device=cuda))
     tree_sample_accept(xg, *args)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
+    with torch.inference_mode(), torch.cuda.graph(graph):    # (as the draft graphs: captures of one mode go together)
         out = tree_sample_accept(xg, *args)
     for i in range(4):
         print(f"[sample accept] replay {i}", flush=True)

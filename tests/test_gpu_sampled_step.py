@@ -146,7 +146,7 @@ def test_sampled_steps(cuda, how, kind):
         with torch.cuda.stream(stream):
             if how == "graph" and i == 1:          # (the first step is an eager one; capturing runs nothing)
                 graph = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(graph):
+                with torch.inference_mode(), torch.cuda.graph(graph):    # (as the draft graphs: captures of one mode go together)
                     server.step()
             if graph is not None:
                 graph.replay()
