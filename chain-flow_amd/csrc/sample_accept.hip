@@ -43,6 +43,7 @@ struct SampleArgs {
   int parts;                 // of a row, counted on their own before (1: none)
   unsigned* part_counts;     // [R][parts][PART_WORDS]
   int* part_high;            // [R][parts]
+  int* part_masked;          // [R][parts]
 };
 struct Range { int from, to; };
 __device__ __forceinline__ Range part_range(int vectors, int part, int parts) {
@@ -98,14 +99,15 @@ __device__ __forceinline__ v4u load8(const u16* x, int j) {
   for (int i = 0; i < 4; ++i) w[i] = x[(size_t)8 * j + 2 * i] | (unsigned)x[(size_t)8 * j + 2 * i + 1] << 16;
   return w;
 }
-// f(j, eight logits) for this thread's vectors j of from .. to - 1, AHEAD of them in flight.
-template <bool VEC, int T, typename F>
-__device__ __forceinline__ void each_of(const u16* x, int from, int to, F f) {
+// f(j, eight logits) for this thread's vectors j of from .. to - 1, AHEAD of them in flight; meanwhile() while the first arrive.
+template <bool VEC, int T, typename F, typename G>
+__device__ __forceinline__ void each_of(const u16* x, int from, int to, F f, G meanwhile) {
   constexpr int AHEAD = VEC ? 8 : 2;
-  if (from >= to) return;
+  if (from >= to) return meanwhile();
   v4u ring[AHEAD];
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) ring[i] = load8<VEC>(x, min(from + (int)threadIdx.x + i * T, to - 1));
+  meanwhile();
 #pragma unroll 1
   for (int j = from + threadIdx.x; j < to; j += AHEAD * T) {
 #pragma unroll
@@ -116,27 +118,63 @@ __device__ __forceinline__ void each_of(const u16* x, int from, int to, F f) {
     }
   }
 }
+template <bool VEC, int T, typename F>
+__device__ __forceinline__ void each_of(const u16* x, int from, int to, F f) {
+  each_of<VEC, T>(x, from, to, f, []() {});
+}
 // Whether a wave has one and the same value everywhere (a mask): counted one by one, each would wait for the others.
 __device__ __forceinline__ bool one_value(v4u w, unsigned& v) {
   const unsigned first = __builtin_amdgcn_readfirstlane(w[0]);
   v = first & 0xffffu;
   return __ballot(w[0] != first) == 0 && first >> 16 == v && __ballot(w[1] != first || w[2] != first || w[3] != first) == 0;
 }
+// The likely mask of a row: the lowest of 64 logits spread over it, where two have it and it is below 0 (NONE: there is none).
+// Tokens of that value are counted apart, in 32 bits: lanes that added to one count would wait for each other, and its count
+// would leave the narrow fields (248,320 logits, every second -inf: 41 rows in 45 us, 378 without).  Any value is as right.
+constexpr unsigned NONE = 0x10000;
+__device__ __forceinline__ unsigned sample_of(const u16* x, int V) { return x[(long long)(threadIdx.x & 63) * (V - 1) / 63]; }
+template <bool BF>
+__device__ __forceinline__ unsigned mask_of_sample(unsigned v) {
+  const unsigned lowest = wave_largest(v <= (BF ? 0xff80u : 0xfc00u) ? v : 0);   // (negative patterns ascend as values fall; no NaN)
+  return lowest > 0x8000u && __builtin_popcountll(__ballot(v == lowest)) > 1 ? lowest : NONE;
+}
 // The narrow counts of the vectors from .. to - 1 and of the n_tail logits behind them (few operations a logit: they are what
-// counting costs).  -> the thread's largest pattern as a signed number: the largest number, where there is a positive one
-template <bool VEC, int T, int BITS>
-__device__ __forceinline__ int count_narrow(const u16* x, int from, int to, int n_tail, unsigned* hist) {
+// counting costs), but for those of value h, the likely mask: to the thread's n_h.  -> the thread's largest pattern as a signed number: the
+// largest number, where there is a positive one
+template <bool BF, bool VEC, int T, int BITS>
+__device__ __forceinline__ int count_narrow(const u16* x, int from, int to, int n_tail, unsigned* hist, unsigned sample, unsigned& h,
+                                            int& n_h) {
   constexpr int WORDS = BITS == 8 ? 1 << 14 : 1 << 15;
   typedef short s16x2 __attribute__((ext_vector_type(2)));
   s16x2 most = {-32768, -32768};
   auto add = [&](unsigned v, unsigned n) __attribute__((always_inline)) {
     atomicAdd(&hist[v & (WORDS - 1)], BITS == 16 ? n * ((v >> 15) * 0xffffu + 1) : n << ((v >> 11) & 24));
   };
+  n_h = 0;
   each_of<VEC, T>(x, from, to, [&](int, v4u w) __attribute__((always_inline)) {
+    bool masked = false;
+    if (h != NONE) {
+      typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+      u16x2 low = {0, 0};                            // the lowest, as there is one below 0
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned u = w[i];
+        low = __builtin_elementwise_max(low, __builtin_bit_cast(u16x2, u));
+      }
+      masked = low[0] >= h || low[1] >= h;
+    }
     unsigned v;
     if (one_value(w, v)) {
       const unsigned long long on = __ballot(true);
-      if ((threadIdx.x & 63) == __builtin_ctzll(on)) add(v, 8u * __builtin_popcountll(on));
+      if (v == h) n_h += 8;
+      else if ((threadIdx.x & 63) == __builtin_ctzll(on)) add(v, 8u * __builtin_popcountll(on));
+    } else if (__ballot(masked)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const unsigned v = w[i >> 1] >> (16 * (i & 1)) & 0xffffu;
+        if (v == h) ++n_h;
+        else add(v, 1u);
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -149,11 +187,12 @@ __device__ __forceinline__ int count_narrow(const u16* x, int from, int to, int 
       const unsigned u = w[i];
       most = __builtin_elementwise_max(most, __builtin_bit_cast(s16x2, u));
     }
-  });
+  }, [&]() __attribute__((always_inline)) { h = mask_of_sample<BF>(sample); });
   int high = max((int)most[0], (int)most[1]);
   if ((int)threadIdx.x < n_tail) {
     const unsigned v = x[(size_t)8 * to + threadIdx.x];
-    add(v, 1u);
+    if (v == h) ++n_h;
+    else add(v, 1u);
     high = max(high, (int)(short)v);
   }
   return high;
@@ -168,24 +207,39 @@ __device__ __forceinline__ int over_all(int v, int* s_int) {
   for (int w = 0; w < W; ++w) v = max(v, s_int[w]);
   return v;
 }
+// The sum of v over W waves.
+template <int W>
+__device__ __forceinline__ int sum_over_all(int v, int* s_int) {
+  v = scan64(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) s_int[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0;
+  for (int w = 0; w < W; ++w) v += s_int[w];
+  return v;
+}
 
 // Few long rows leave most CUs idle, and a CU counts 64 logits in 10 cycles: then each row is counted in parts, a workgroup a
 // part, and k_sample_rows adds the parts' counts up (6 rows of 248,320 in 4 parts: 10 us here and 15.7 there, 31 in one).
-template <bool VEC>
+template <bool BF, bool VEC>
 __global__ void __launch_bounds__(1024, 4) k_sample_parts(SampleArgs a) {
   __shared__ __attribute__((aligned(16))) unsigned hist[PART_WORDS];
   __shared__ int s_int[16];
   const int row = blockIdx.x, part = blockIdx.y, t = threadIdx.x, whole = a.V / 8;
   const u16* x = a.logits + (size_t)row * a.ld;
   for (int i = t; i < PART_WORDS / 4; i += 1024) ((uint4*)hist)[i] = make_uint4(0, 0, 0, 0);
+  const unsigned sample = sample_of(x, a.V);
   __syncthreads();
   const Range r = part_range(whole, part, a.parts);
-  int high = count_narrow<VEC, 1024, 16>(x, r.from, r.to, part == a.parts - 1 ? a.V % 8 : 0, hist);
+  unsigned h;
+  int masked;
+  int high = count_narrow<BF, VEC, 1024, 16>(x, r.from, r.to, part == a.parts - 1 ? a.V % 8 : 0, hist, sample, h, masked);
   high = over_all<16>(high, s_int);                  // (and the counts are whole)
+  masked = sum_over_all<16>(masked, s_int);
   const size_t at = (size_t)row * a.parts + part;
   uint4* out = (uint4*)(a.part_counts + at * PART_WORDS);
   for (int i = t; i < PART_WORDS / 4; i += 1024) out[i] = ((uint4*)hist)[i];
-  if (t == 0) a.part_high[at] = high;
+  if (t == 0) { a.part_high[at] = high; a.part_masked[at] = masked; }
 }
 
 // One workgroup of T threads a row.  BITS: a value's count in LDS, 32 / BITS values a word (the low bits of the value name the
@@ -193,11 +247,10 @@ __global__ void __launch_bounds__(1024, 4) k_sample_parts(SampleArgs a) {
 // own and adds at most 1 to the next, so that the sum only falls.  Then (a constant row, a masked one) half of the values
 // are counted at a time, in twice the bits, which V cannot leave: 8 bits and 64 KB for V < 65,536, 16 bits and 128 KB
 // above.  The row is read again, from the caches, for the drawn token's index.
-// 8 bits below 65,536 values, as two workgroups then share a CU (1,968 rows of 32,000 logits: 90 us in fp16, 76 in bf16, 136 and 125
-// with 1,024 threads and 16 bits; since then 85 and 70).  What bounds a row of 248,320 bf16 logits on its CU: 17 us of counting (an LDS atomic a logit, a wave's 64 in
-// 10 cycles), 2.2 the cells (fp16: 4.2, more values are in use), 1.5 a search (one wave's latency), 4 the index.  1,968 rows
-// of 32,000: 11 us a row and CU in fp16, 1.5 TB/s; the stages of two rows overlap there, and the searches' latency and the
-// weights of many values are what remains.
+// What bounds a row of 248,320 bf16 logits on its CU: 17 us of counting (an LDS atomic a logit, a wave's 64 in 10 cycles), 2.2 the
+// cells (fp16: 4.2, more values are in use), 1.5 a search (one wave's latency), 4 the index.  1,968 rows of 32,000: 11 us a row and
+// CU in fp16, 1.5 TB/s; the stages of two rows overlap there, and the searches' latency and the weights of many values
+// are what remains.
 template <bool BF, bool VEC, int T, int BITS>
 __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
   constexpr int W = T / 64, LOG = BITS == 8 ? 14 : 15, WORDS = 1 << LOG;
@@ -208,7 +261,7 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
   __shared__ int cell_n[CELLS];
   constexpr int MANT = BF ? 7 : 10;                  // bits of a binade's values
   __shared__ double table[32], ratio[0x8000 >> MANT];
-  __shared__ int s_int[W];
+  __shared__ int s_int[W], s_masked[W];
   __shared__ Place s_place;
   __shared__ int s_half[3], s_cell, s_rank;
   __shared__ double s_kept;
@@ -216,6 +269,9 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
   const bool in_parts = T == 1024 && a.parts > 1;
   if (!in_parts)
     for (int i = t; i < WORDS / 4; i += T) ((uint4*)hist)[i] = make_uint4(0, 0, 0, 0);   // (while the bounds arrive)
+  const u16* x = a.logits + (size_t)row * a.ld;
+  const int V = a.V;
+  const unsigned sample = sample_of(x, V);
   // request b > 0 has the rows cu_rows[b - 1] .. cu_rows[b], the first those below cu_rows[0]
   int b = 0;
   if (row >= a.cu_rows[0]) {
@@ -229,8 +285,6 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
   }
   const float Tf = a.temp[b], u = a.u[row], P = a.top_p ? a.top_p[b] : 1.f;   // (here, so that they arrive during the count)
   const int K = a.top_k ? a.top_k[b] : 0;
-  const u16* x = a.logits + (size_t)row * a.ld;
-  const int V = a.V;
   const int whole = V / 8;                           // vectors of eight; the row's last logits are one more, from `tail`
   v4u tail = {};                                     // (the last logit again behind the row's end)
   if (V % 8) {
@@ -238,6 +292,8 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
     for (int i = 0; i < 4; ++i) tail[i] = x[min(8 * whole + 2 * i, V - 1)] | (unsigned)x[min(8 * whole + 2 * i + 1, V - 1)] << 16;
   }
   bool wide = false;
+  unsigned h = NONE;                                 // the value that hist does not hold, and its tokens (a thread's, then the row's)
+  int n_h = 0;
   int half = 0;                                      // (wide) the top bit of the values whose counts hist holds
   auto count_half = [&](int h) __attribute__((always_inline)) {
     half = h;
@@ -278,6 +334,10 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
     } else {
 #pragma unroll
       for (int e = 0; e < N; ++e) c[e] = v[e] >> shift & mask;
+    }
+    if (h - o0 < 64u * N) {                          // (a value below 0 is its own position)
+#pragma unroll
+      for (int e = 0; e < N; ++e) c[e] += (int)h == o0 + N * lane + e ? n_h : 0;
     }
     if (o0 < O_FIRST<BF> || o0 + 64 * N - 1 > O_LAST<BF>) {
 #pragma unroll
@@ -398,10 +458,15 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
     }
 #pragma unroll
     for (int k = 0; k < PER; ++k) ((v4u*)hist)[k * T + t] = sum[k];
-    if (t < a.parts) high = a.part_high[(size_t)row * a.parts + t];
+    if (t < a.parts) {
+      high = a.part_high[(size_t)row * a.parts + t];
+      n_h = a.part_masked[(size_t)row * a.parts + t];
+    }
+    h = mask_of_sample<BF>(sample);
   } else {
-    high = count_narrow<VEC, T, BITS>(x, 0, whole, V % 8, hist);
+    high = count_narrow<BF, VEC, T, BITS>(x, 0, whole, V % 8, hist, sample, h, n_h);
   }
+  const unsigned masked = h;
   constexpr int INF = BF ? 0x7f80 : 0x7c00;
   high = over_all<W>(high, s_int);
   if (t == 0) {                                      // -0 counts as +0
@@ -441,14 +506,15 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
   int rank = 0;
   double kept_m = 1.0;
   if (!greedy) {
-    int all = cells_narrow();
-    for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off);
-    if (lane == 0) s_int[wave] = all;
+    int all = scan64(cells_narrow() + n_h);
+    n_h = scan64(n_h);
+    if (lane == 63) { s_int[wave] = all; s_masked[wave] = n_h; }
     __syncthreads();
-    all = 0;
-    for (int w = 0; w < W; ++w) all += s_int[w];
+    all = n_h = 0;
+    for (int w = 0; w < W; ++w) { all += s_int[w]; n_h += s_masked[w]; }
     if (all != V) {
       wide = true;
+      h = NONE;                                      // (counted with the others)
       for (int h = 1; h >= 0; --h) {
         __syncthreads();
         count_half(h);
@@ -460,8 +526,21 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
     // each for the first value at which the running sum (of counts: by_n) reaches a goal, or passes it (the draw), or the last
     // one of any weight where rounding leaves none, among the first kept_n tokens: the cut of k, the cut of P, the draw.
     if (wave == 0 || wide) {
-      const int n0 = cell_n[2 * lane], n1 = n0 + cell_n[2 * lane + 1], up_n = scan64(n1), from_n = up_n - n1;
-      const double s0 = cell_m[2 * lane], s1 = s0 + cell_m[2 * lane + 1], up_m = scan64(s1);
+      int n0 = cell_n[2 * lane], n1 = cell_n[2 * lane + 1];
+      double s0 = cell_m[2 * lane], s1 = cell_m[2 * lane + 1];
+      const int o_h = (int)h;
+      if (o_h >= 0x8000 && o_h <= O_LAST<BF> && o_h / (128 * N) == lane) {   // (-inf is no token)
+        const double sum = (double)n_h * pow2(table, o_h == top ? 0.0 : isinf(m) ? -INFINITY : (value_of<BF>(o_h) - m) * rate);
+        const bool second = o_h / (64 * N) % 2;
+        n0 += second ? 0 : n_h;
+        n1 += second ? n_h : 0;
+        s0 += second ? 0.0 : sum;
+        s1 += second ? sum : 0.0;
+      }
+      n1 += n0;
+      s1 += s0;
+      const int up_n = scan64(n1), from_n = up_n - n1;
+      const double up_m = scan64(s1);
       double from_m = __shfl_up(up_m, 1);            // (as the lanes before add up, to the bit)
       if (lane == 0) from_m = 0.0;
       const int upto_n[3] = {from_n, from_n + n0, up_n};          // up to the lane's two cells, between them and behind them
@@ -593,7 +672,8 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
     int n = 0;
     if (lane < a.parts) {
       const unsigned w = a.part_counts[((size_t)row * a.parts + lane) * PART_WORDS + (raw & (PART_WORDS - 1))];
-      n = p.o == 0x7fff ? (w & 0xffffu) + (w >> 16) : w >> (raw >> 15) * 16 & 0xffffu;
+      n = raw == masked ? a.part_masked[(size_t)row * a.parts + lane]
+                   : p.o == 0x7fff ? (w & 0xffffu) + (w >> 16) : w >> (raw >> 15) * 16 & 0xffffu;
     }
     const int upto = scan64(n), part = __builtin_ctzll(__ballot(upto > rank));
     rank -= __builtin_amdgcn_readlane(upto - n, part);
@@ -647,9 +727,9 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
   const int own = __builtin_popcount(hits);
   int left = (last ? rank - all_steps : s_rank) - (scan64(own) - own);
   if (left < 0 || left >= own) return;
-  unsigned h = hits;
-  for (; left > 0; --left) h &= h - 1;
-  found(8 * (last ? whole : j) + __builtin_ctz(h));
+  unsigned rest = hits;
+  for (; left > 0; --left) rest &= rest - 1;
+  found(8 * (last ? whole : j) + __builtin_ctz(rest));
 }
 
 struct WalkArgs {
@@ -720,7 +800,7 @@ extern "C" {
 int64_t cfh_tree_sample_ws_bytes(int n_rows, int V) {
   if (n_rows < 0 || V <= 0) return -1;
   const int parts = parts_of(n_rows, V);
-  return ((int64_t)n_rows * 8 + 15) / 16 * 16 + (parts > 1 ? (int64_t)n_rows * parts * (PART_WORDS * 4 + 4) : 0);
+  return ((int64_t)n_rows * 8 + 15) / 16 * 16 + (parts > 1 ? (int64_t)n_rows * parts * (PART_WORDS * 4 + 8) : 0);
 }
 
 int cfh_tree_sample_accept(const void* logits, long long ld, int V, int n_rows, int is_bf16, const int32_t* cu_draft,
@@ -740,16 +820,22 @@ int cfh_tree_sample_accept(const void* logits, long long ld, int V, int n_rows, 
   const int parts = parts_of(n_rows, V);
   unsigned* part_counts = (unsigned*)((char*)ws + ((size_t)n_rows * 8 + 15) / 16 * 16);
   SampleArgs s = {(const u16*)logits, ld, V, n_rows, B, cu_sampled, uniforms, temperature, top_k, top_p, tok, lp, parts,
-                  part_counts, (int*)(part_counts + (size_t)n_rows * parts * PART_WORDS)};
+                  part_counts, (int*)(part_counts + (size_t)n_rows * parts * PART_WORDS),
+                  (int*)(part_counts + (size_t)n_rows * parts * (PART_WORDS + 1))};
   const bool vec = (n_rows == 1 || ld % 8 == 0) && ((uintptr_t)logits & 15) == 0;
   if (parts > 1) {
-    if (vec) hipLaunchKernelGGL(k_sample_parts<true>, dim3(n_rows, parts), dim3(1024), 0, st, s);
-    else hipLaunchKernelGGL(k_sample_parts<false>, dim3(n_rows, parts), dim3(1024), 0, st, s);
+    auto* fn = is_bf16 ? (vec ? k_sample_parts<true, true> : k_sample_parts<true, false>)
+                       : (vec ? k_sample_parts<false, true> : k_sample_parts<false, false>);
+    hipLaunchKernelGGL(fn, dim3(n_rows, parts), dim3(1024), 0, st, s);
     CFH_LAUNCH_CHECK();
   }
+  // 8 bits let two workgroups share a CU: 1,968 rows of 32,000 logits 87 us in fp16 and 72 in bf16, with 16 bits 129 and 118; 492 rows 31 and
+  // 27, 42 and 38; 246 rows (a CU each) 24 and 22 either way.  But a value that more than 255 have sends its row to the wide
+  // counts (1,968 rows of 32,000 bf16 logits around -6: 192 us), so they are for many rows, and in bf16 for up to 32,768 values.
+  const bool narrow = V < 65536 && n_rows > 256 && (!is_bf16 || V <= 32768);
   auto launch = [&](auto bf, auto v) {
     constexpr bool BF = bf.value, VEC = v.value;
-    if (V < 65536) hipLaunchKernelGGL((k_sample_rows<BF, VEC, 512, 8>), dim3(n_rows), dim3(512), 0, st, s);
+    if (narrow) hipLaunchKernelGGL((k_sample_rows<BF, VEC, 512, 8>), dim3(n_rows), dim3(512), 0, st, s);
     else hipLaunchKernelGGL((k_sample_rows<BF, VEC, 1024, 16>), dim3(n_rows), dim3(1024), 0, st, s);
   };
   if (is_bf16) vec ? launch(std::true_type{}, std::true_type{}) : launch(std::true_type{}, std::false_type{});

@@ -152,6 +152,50 @@ def test_long_rows_counted_whole_and_in_parts(cuda, R, V, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V", [5000, 60001, 70001])
+def test_rows_masked_here_and_there(cuda, V, dtype):
+    """A constrained request's logits: most or some of them -inf, the type's lowest value, a large negative number or the row's
+    own lowest one, in no runs; temperatures from ones that drop what is masked to ones at which it counts as much as the rest."""
+    lowest, far = torch.finfo(dtype).min, torch.tensor(-1.0e4).to(dtype).item()
+    g = torch.Generator().manual_seed(V)
+    rows = [(m, d) for m in (float("-inf"), lowest, far, -3.5, -0.0) for d in (0.03, 0.5, 0.97, 0.9999)] + [(float("nan"), 0.6)]
+    R = len(rows) + (6 if V == 70001 else 0)       # (more than 24 long rows are counted whole)
+    x = torch.randn(R, V, generator=g).mul(2).to(dtype)
+    x[-1], x[-2] = x[-1].abs() + 1, -x[-2].abs() - 1
+    for i, (m, d) in enumerate(rows):
+        x[i] = torch.where(torch.rand(V, generator=g) < d, torch.tensor(m).to(dtype), x[i])
+    rng = np.random.default_rng(V)
+    print(f"[sample accept] masked rows {R} x {V} {dtype}", flush=True)
+    for n in (R, 20):
+        for T in (1.0, 0.0, 3.0e4, 1e38):
+            k = rng.integers(0, 2 * V, n) * (rng.random(n) < 0.7)
+            _check(x[:n], np.zeros(n, np.int64), np.arange(1, n + 1), [], [], 0, rng.random(n), [T] * n, k,
+                   np.where(rng.random(n) < 0.5, 1.0, rng.random(n)), cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V", [4096, 8203, 32768])
+def test_many_rows_of_every_kind(cuda, V, dtype):
+    """More rows than CUs: narrower counts, which clustered and constant rows leave."""
+    R = 264
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(R, V, generator=g).to(dtype)
+    kinds = [lambda r: r.mul_(2.5), lambda r: r.mul_(0.3).sub_(6), lambda r: r.mul_(0.01).add_(3), lambda r: r.fill_(-1.25),
+             lambda r: r[::2].fill_(torch.finfo(dtype).min), lambda r: r[: V // 2].fill_(float("-inf")), lambda r: r.fill_(0.0)[::3].fill_(-0.0),
+             lambda r: r.fill_(float("-inf")), lambda r: r[::7].fill_(float("nan")), lambda r: r.fill_(-2.0)[1::2].fill_(-1.0),
+             lambda r: r.fill_(7.0)[5:9].fill_(8.0)]
+    for i in range(R):
+        kinds[i % len(kinds)](x[i])
+    rng = np.random.default_rng(V)
+    print(f"[sample accept] rows of every kind {R} x {V} {dtype}", flush=True)
+    T = rng.choice([0.0, 0.5, 1.0, 30.0], R)
+    _check(x, np.zeros(R, np.int64), np.arange(1, R + 1), [], [], 0, rng.random(R), T, rng.integers(0, V, R) * (rng.random(R) < 0.6),
+           np.where(rng.random(R) < 0.4, 1.0, rng.random(R)), cuda)
+
+
+@pytest.mark.gpu
 def test_uniforms_at_and_past_their_ends(cuda):
     x = torch.randn(8, 501, generator=torch.Generator().manual_seed(4)).bfloat16()
     u = [0.0, -1.0, float("nan"), 1.0, 7.0, float("inf"), 1 - 2.0 ** -24, 2.0 ** -30]
