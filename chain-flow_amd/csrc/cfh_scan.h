@@ -10,10 +10,13 @@ enum { DPP_SHR1 = 0x111, DPP_SHR2 = 0x112, DPP_SHR4 = 0x114, DPP_SHR8 = 0x118, D
 template <int CTRL, int ROWS>
 __device__ __forceinline__ int moved(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
 template <int CTRL, int ROWS>
-__device__ __forceinline__ double moved(double v) {
-  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+__device__ __forceinline__ unsigned long long moved(unsigned long long u) {
   const unsigned lo = moved<CTRL, ROWS>((int)u), hi = moved<CTRL, ROWS>((int)(u >> 32));
-  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+  return (unsigned long long)hi << 32 | lo;
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved(double v) {
+  return __builtin_bit_cast(double, moved<CTRL, ROWS>(__builtin_bit_cast(unsigned long long, v)));
 }
 template <typename N>
 __device__ __forceinline__ N row_scan(N v) {
