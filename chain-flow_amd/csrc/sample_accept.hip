@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
   // request b > 0 has the rows cu_rows[b - 1] .. cu_rows[b], the first those below cu_rows[0]
   int b = 0;
   if (row >= a.cu_rows[0]) {
-    const Seq f = find_looking<1>(a.cu_rows, a.B - 1, [&](int, int c) { return c <= row; });
+    const Seq f = find_seq(a.cu_rows, a.B - 1, nullptr, [&](int, int c) { return c <= row; });
     b = f.s >= 0 && row < f.c1 ? f.s + 1 : -1;
   }
   auto give = [&](int tok, float lp) __attribute__((always_inline)) { a.tok[row] = tok; a.lp[row] = lp; };
