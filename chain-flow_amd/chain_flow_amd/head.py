@@ -408,7 +408,7 @@ def row_topk(logits: torch.Tensor, k: int, split: bool = False):
     L = _lib.lib()
     if split:
         ws = torch.empty(max(int(L.cfh_head_ws_bytes(M, n, k)), 16), dtype=torch.uint8, device=logits.device)
-        _lib.check(L.cfh_row_topk_sets(*args, ws.data_ptr(), _lib.stream_handle()), "cfh_row_topk_sets")
+        _lib.check(L.cfh_row_topk_sets(*args, ws.data_ptr(), _lib.stream_of(logits.get_device())), "cfh_row_topk_sets")
     else:
         _lib.check(L.cfh_row_topk(*args, _lib.stream_handle()), "cfh_row_topk")
     return vals, ids, lse

@@ -77,7 +77,8 @@ def _check_pool(k_cache, v_cache, k_exp, v_exp):
     lk = lv = 0
     if f8:
         for e in (k_exp, v_exp):
-            if e is None or e.dtype != torch.uint8 or e.shape != shape[:-1] or not (e[0] if layers > 1 else e).is_contiguous():
+            if (e is None or e.dtype != torch.uint8 or e.shape != shape[:-1]
+                    or (e.stride()[-3:] != (page * Hkv, Hkv, 1) and not (e[0] if layers > 1 else e).is_contiguous())):
                 raise ValueError(f"an 8-bit cache needs uint8 k_exp and v_exp {tuple(shape[:-1])}, contiguous in a layer")
         if layers > 1:
             lk, lv = k_exp.stride(0), v_exp.stride(0)
@@ -87,15 +88,19 @@ def _check_pool(k_cache, v_cache, k_exp, v_exp):
         raise ValueError("the cache must be bf16 or fp16 without exponents, or float8_e4m3fn with them")
     row = Hkv * D
     inner = page * row
-    sizes, want = (page, Hkv, D), (row, D, 1)
-    laid = all(n == 1 or (a == w and b == w) for n, a, b, w in zip(sizes, sk[1:], sv[1:], want))
+    want = (row, D, 1)
+    laid = (tuple(sk[1:]) == want and tuple(sv[1:]) == want) or all(
+        n == 1 or (a == w and b == w) for n, a, b, w in zip((page, Hkv, D), sk[1:], sv[1:], want))
     bs_k, bs_v = (inner, inner) if blocks == 1 else (sk[0], sv[0])
-    if (not laid or bs_k < inner or bs_v < inner or (bs_k | bs_v | ls_k | ls_v) % 16
-            or any(ls < inner or (ls < (blocks - 1) * bs + inner and bs < (layers - 1) * ls + inner)
-                   for ls, bs in ((ls_k, bs_k), (ls_v, bs_v)) if layers > 1) or (k_cache.data_ptr() | v_cache.data_ptr()) % 16):
+    apart = layers == 1 or (                       # layers around the blocks, or blocks around the layers
+        ls_k >= inner and ls_v >= inner
+        and (ls_k >= (blocks - 1) * bs_k + inner or bs_k >= (layers - 1) * ls_k + inner)
+        and (ls_v >= (blocks - 1) * bs_v + inner or bs_v >= (layers - 1) * ls_v + inner))
+    k_ptr, v_ptr = k_cache.data_ptr(), v_cache.data_ptr()
+    if (not laid or not apart or bs_k < inner or bs_v < inner or (bs_k | bs_v | ls_k | ls_v) % 16 or (k_ptr | v_ptr) % 16):
         raise ValueError("cache blocks must be contiguous [page, Hkv, D], blocks and layers on strides of 16 elements and "
                          "16-byte boundaries")
-    return _lib.KvPool(k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_exp), _lib.ptr(v_exp), ls_k, ls_v, bs_k, bs_v,
+    return _lib.KvPool(k_ptr, v_ptr, _lib.ptr(k_exp), _lib.ptr(v_exp), ls_k, ls_v, bs_k, bs_v,
                        lk, lv, layers, blocks, page, Hkv, D)
 
 
