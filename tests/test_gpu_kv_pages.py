@@ -257,6 +257,37 @@ def test_commit_refuses_a_sequence_at_a_time(cuda):
 
 
 @pytest.mark.gpu
+def test_pages_behind_4_gib(cuda):
+    """Copies and moved rows whose offsets pass 32 bits, in bytes and (of the last layer) in elements."""
+    layers, blocks, page, Hkv, D = 2, 70001, 16, 8, 256
+    print("[pages] behind 4 GiB", flush=True)
+    k, v = (torch.zeros(layers, blocks, page, Hkv, D, dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    table = torch.full((2, 3), -1, dtype=torch.int32, device=cuda)
+    room, ref = torch.zeros(2, dtype=torch.int32, device=cuda), torch.ones(blocks, dtype=torch.int32, device=cuda)
+    free = [69990, 69995, 70000]
+    ref[free] = 0
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    kv_pages_resize(table, room, ref, _i32([21, 0], cuda), page=page, status=status)
+    assert table[0].tolist() == free[:2] + [-1]
+    for c in (k, v):
+        for p in free[:2]:
+            c[:, p] = torch.randn(layers, page, Hkv, D, device=cuda).to(torch.bfloat16)
+    kv_pages_fork(table, room, ref, _i32([0], cuda), _i32([1], cuda), page=page, status=status)
+    kv_pages_resize(table, room, ref, _i32([-1, 26], cuda), page=page, k_cache=k, v_cache=v, status=status)
+    torch.cuda.synchronize()
+    assert int(status) == 0 and table[1].tolist() == [free[0], free[2], -1]
+    for c in (k, v):
+        assert torch.equal(c[:, free[2], :5], c[:, free[1], :5]) and not c[:, free[2], 5:].any()
+    rows = torch.randn(layers, 5, Hkv, D, device=cuda).to(torch.bfloat16)
+    k[:, free[2], 5:10], v[:, free[2], 5:10] = rows, rows * 2
+    kv_cache_commit(k, v, table[1:], _i32([21], cuda), _i32([[1, 4]], cuda), _i32([2], cuda), status=status)
+    torch.cuda.synchronize()
+    assert int(status) == 0
+    for c, r in ((k, rows), (v, rows * 2)):
+        assert torch.equal(c[:, free[2], 5:7], r[:, [1, 4]]) and torch.equal(c[:, free[2], 7:10], r[:, 2:])
+
+
+@pytest.mark.gpu
 def test_pages_in_a_graph(cuda):
     """A captured step -- grow, commit, shrink, fork -- replayed over pools that change between replays."""
     page, W, S, blocks, P = 4, 12, 6, 80, 3

@@ -259,3 +259,25 @@ def test_head_first_used_in_a_graph(cuda):
         assert torch.equal(y, eager) and torch.equal(head.logits(h), eager)
     _close(eager, np.concatenate([to64(h), np.zeros((3, 128))], 1),
            ohead.dequant4(ohead.unpack4(head.weight.cpu().numpy()), to64(head.scale)), 64)
+
+
+@pytest.mark.gpu
+def test_drafts_over_4_bits_in_a_graph(cuda):
+    cfg = flownet(512, layers=1, flow_steps=2)
+    W = make_weights(cfg, 2048, init="test", base_seed=3)
+    dr = Drafter(cfg, {k: v.to(cuda) for k, v in W.items()}, None, device=cuda, head_bits=4)
+    pred = dr.predict_hidden(synthetic_context(3, cfg.context_size, 512, seed=2).to(cuda))
+    known = torch.tensor([3, 500, 2000], device=cuda)
+    draft = lambda: (dr.beam_chains(None, known, 5, 4, pred=pred), dr.beam_tree(None, known, 4, 4, 3, pred=pred))   # noqa: E731
+    draft()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.inference_mode(), torch.cuda.graph(graph):
+        out = draft()
+    for i in range(3):
+        known.copy_(torch.tensor([7 * i + 1, 40 * i, 2047 - i]))
+        want = [w.clone() for w in draft()]
+        graph.replay()
+        torch.cuda.synchronize()
+        print(f"[4-bit drafts in a graph] replay {i}", flush=True)
+        assert all(torch.equal(a, b) for a, b in zip(out, want))

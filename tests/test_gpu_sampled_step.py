@@ -175,3 +175,29 @@ def test_sampled_steps(cuda, how, kind):
     # requests end: every page is free again
     kv_pages_resize(server.table, server.room, server.ref, torch.zeros(S, dtype=torch.int32), page=PAGE, status=server.status)
     assert int(server.ref.abs().sum()) == 0 and (server.table == -1).all() and int(server.status) == 0
+
+
+@pytest.mark.gpu
+def test_two_servers_at_once(cuda):
+    """Two of them on streams of their own, steps in turn and no waiting in between: neither finds the other's workspaces."""
+    rng = np.random.default_rng(3)
+    servers, texts, roots, streams = [], [], [], [torch.cuda.Stream() for _ in range(2)]
+    print("[sampled steps] two at once", flush=True)
+    for i in range(2):
+        servers.append(_Server(cuda, ("bf16", "fp8")[i]))
+        prompts = [[int(t) for t in rng.integers(0, V, n)] for n in (5 + i, 8)]
+        servers[i].prompts(prompts)
+        texts.append([list(prompts[s // 3]) for s in range(S)])
+        roots.append([int(t) for t in rng.integers(0, V, S)])
+        servers[i].root.copy_(torch.tensor(roots[i]))
+    for step in range(3):
+        draws = [torch.tensor(rng.random(S * (N + 1)), dtype=torch.float32).to(cuda) for _ in range(2)]
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                servers[i].u.copy_(draws[i])
+                servers[i].step()
+        torch.cuda.synchronize()
+        for i in range(2):
+            servers[i].check(texts[i], roots[i])
+        print(f"[sampled steps] step {step}", flush=True)
