@@ -279,18 +279,31 @@ __global__ void __launch_bounds__(RS_T) k_plan(ResizeArgs a) {
   constexpr int MOST = ONE ? RS_T : RS_MAX;
   __shared__ int tails[MOST];        // the shared page a sequence would write into, -1: none
   __shared__ Shared<2 * MOST> shared;
-  __shared__ int first[ONE ? RS_T : 1];
+  // ONE: a sequence a thread, what others need of it in LDS, as are the first pages taken (a pair of calls for 48 sequences in a
+  // graph: 18.4 us, 20.0 through memory; 96 copied pages: this kernel 10.4 for 12.0)
+  constexpr int QUICK = ONE ? 4096 : 1;
+  __shared__ int first[ONE ? RS_T : 1], quick[QUICK];
+  __shared__ int4 plans[ONE ? RS_T : 1];
   __shared__ double tmp[RS_T / 64];
   __shared__ int used, copied_n;
   const int t = threadIdx.x;
   if (t == 0) used = copied_n = 0;
+  Span mine = {};
+  if (ONE && t < a.S) mine = span_of(a, t);
+  auto span = [&](int s) __attribute__((always_inline)) { return ONE ? mine : span_of(a, s); };
+  auto plan = [&](int s) __attribute__((always_inline)) -> int4& {
+    if constexpr (ONE) return plans[s];
+    else return a.plan[s];
+  };
+  auto fresh = [&](int i) __attribute__((always_inline)) { return i < QUICK && ONE ? quick[i] : a.fresh[i]; };
   if constexpr (ONE) {
-    const Span x = t < a.S ? span_of(a, t) : Span{};
+    const Span x = mine;
     if (t < a.S && !x.ok && !x.pad && a.status) a.status[0] = 1;
     double all;
     const double at = scan_before((double)(x.ok ? x.had - x.kept : 0), tmp, all);
     const int n = (int)all;                          // (at most RS_ONE entries)
     first[t] = (int)at;
+    tails[t] = x.want;
     __syncthreads();
     for (int i0 = t; i0 < n; i0 += 4 * RS_T)
 #pragma unroll
@@ -298,13 +311,13 @@ __global__ void __launch_bounds__(RS_T) k_plan(ResizeArgs a) {
         const int i = i0 + u * RS_T;
         if (i >= n) break;
         const int s = last_at(first, a.S, i);
-        let_go(a, s, (int)(((long long)a.new_room[s] + a.c.page - 1) / a.c.page) + i - first[s]);
+        let_go(a, s, tails[s] + i - first[s]);
       }
     __syncthreads();
   }
   bool any = false;
   for (int s = t; s < a.S; s += RS_T) {
-    const Span x = span_of(a, s);
+    const Span x = span(s);
     int tail = -1;
     if (x.ok && x.part) {
       tail = a.table[(size_t)s * a.table_ld + x.kept - 1];
@@ -335,7 +348,7 @@ __global__ void __launch_bounds__(RS_T) k_plan(ResizeArgs a) {
     int need = 0, tail = -1;
     Span x = {};
     if (s < a.S) {
-      x = span_of(a, s);
+      x = span(s);
       tail = tails[s];
       if (tail == -2) x.ok = false;
       if (x.ok) need = x.want - x.kept;
@@ -349,7 +362,7 @@ __global__ void __launch_bounds__(RS_T) k_plan(ResizeArgs a) {
     if (s < a.S) {
       const bool copied = x.ok && need > x.want - x.kept;
       // (-2: keeps its shared page, if those before it copied it)
-      a.plan[s] = make_int4(x.ok ? at : -1, copied ? tail : x.ok && tail >= 0 ? -2 : -1, x.kept, x.part);
+      plan(s) = make_int4(x.ok ? at : -1, copied ? tail : x.ok && tail >= 0 ? -2 : -1, x.kept, x.part);
     }
     if constexpr (ONE) first[t] = at;
     total += all;
@@ -382,7 +395,11 @@ __global__ void __launch_bounds__(RS_T) k_plan(ResizeArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (ref[4 * q + e] == 0) {
-          if (to < total) a.fresh[to] = p0 + q * Q + 4 * t + e;
+          if (to < total) {
+            const int page = p0 + q * Q + 4 * t + e;
+            if (ONE && to < QUICK) quick[to] = page;
+            else a.fresh[to] = page;
+          }
           ++to;
         }
       base += (double)(all >> (16 * q) & 0xffff);
@@ -391,18 +408,18 @@ __global__ void __launch_bounds__(RS_T) k_plan(ResizeArgs a) {
   const int have = (int)fmin(base, total);
   __syncthreads();
   for (int s = t; s < a.S; s += RS_T) {
-    const int4 p = a.plan[s];
+    const int4 p = plan(s);
     if (p.x < 0) continue;
-    const Span x = span_of(a, s);
+    const Span x = span(s);
     const int need = x.want - x.kept + (p.y >= 0);
     if ((need > 0 || p.y == -2) && p.x + need > have) {
-      a.plan[s].x = -1;
+      plan(s).x = -1;
       if (a.status) a.status[0] = 1;
       continue;
     }
     if (p.y >= 0) {
       atomicSub(&a.ref[p.y], 1);
-      a.copies[1 + atomicAdd(&copied_n, 1)] = make_int4(p.y, a.fresh[p.x], p.w, 0);   // (in any order)
+      a.copies[1 + atomicAdd(&copied_n, 1)] = make_int4(p.y, fresh(p.x), p.w, 0);   // (in any order)
     }
     if (need > 0) atomicMax(&used, p.x + need);
     if constexpr (ONE) a.room[s] = a.new_room[s];
@@ -410,11 +427,11 @@ __global__ void __launch_bounds__(RS_T) k_plan(ResizeArgs a) {
   __syncthreads();
   if (t == 0) a.copies[0].x = copied_n;
   for (int i = t; i < used; i += RS_T) {             // (what is used was had: no place behind)
-    const int page = a.fresh[i];
+    const int page = fresh(i);
     a.ref[page] = 1;
     if constexpr (ONE) {
       const int s = last_at(first, a.S, i);
-      const int4 p = a.plan[s];
+      const int4 p = plans[s];
       a.table[(size_t)s * a.table_ld + p.z - (p.y >= 0) + i - p.x] = page;
     }
   }
