@@ -185,8 +185,8 @@ constexpr int RS_T = 1024;
 constexpr int RS_FAR = 0x3fffffff; // a place behind every page
 // Up to so many table entries (and RS_T sequences) one workgroup does all of it, in one launch; above, the entries are let go of
 // and filled in by a workgroup a sequence, in launches before and behind.  A pair of calls that grows and shrinks 48
-// sequences of 567 entries: 14.7 us so, 23.9 in three launches each (200 of 304: 15.9, 23.8; 1,000 of 223: 22.0, 24.9); a pair in
-// which every page changes hands 53 and 37 (104 and 48; 358 and 121).
+// sequences of 567 entries: 14.8 us so, 25.3 in three launches each (200 of 304: 15.7, 26.5; 1,000 of 223: 19.9, 26.4); a pair in
+// which every page changes hands 41 and 34 (79 and 41; 266 and 89).
 constexpr long long RS_ONE = 65536;
 
 // Pages that a sequence has, wants and keeps.
