@@ -542,7 +542,8 @@ __global__ void __launch_bounds__(256) k_topk_sets(TopkArgs a, void* ws, int nse
   for (int i = 0; i < N; ++i) {
     const int at = i * 64 + lane;
     const bool nan = (raw[i] & 0x7fffu) > 0x7c00u;
-    const unsigned order = raw[i] & 0x8000u ? ~raw[i] & 0xffffu : raw[i] | 0x8000u;
+    const unsigned v = raw[i] == 0x8000u ? 0 : raw[i];                      // (-0 and +0 are equal: the lower column of them)
+    const unsigned order = v & 0x8000u ? ~v & 0xffffu : v | 0x8000u;
     key[i] = at < n && !nan ? order << 16 | (0xffffu - at) : 0;             // (0: none)
     if (at < n) mx = fmaxf(mx, (float)__builtin_bit_cast(h16, (uint16_t)raw[i]));
   }

@@ -281,3 +281,22 @@ def test_drafts_over_4_bits_in_a_graph(cuda):
         torch.cuda.synchronize()
         print(f"[4-bit drafts in a graph] replay {i}", flush=True)
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [1, 3, 16])
+def test_split_top_k_takes_both_zeros_as_equal(cuda, k):
+    """-0 and +0 are equal numbers: the lower column comes first, within 512 columns and between."""
+    g = torch.Generator().manual_seed(k)
+    x = -(torch.rand(4, 1700, generator=g) + 0.5).half()
+    x[0, 3], x[0, 7] = -0.0, 0.0                                   # -0 before +0, at the cut of k = 1
+    x[1, 600], x[1, 5], x[1, 601] = 0.0, -0.0, -0.0
+    at = torch.randperm(1700, generator=g)[:60]
+    x[2, at] = torch.where(torch.rand(60, generator=g) < 0.5, -0.0, 0.0).half()
+    x[3] = torch.where(torch.rand(1700, generator=g) < 0.9, -0.0, 0.0).half()
+    vals, ids, _ = (t.cpu() for t in row_topk(x.to(cuda), k, split=True))
+    print(f"[split top-k] zeros, k {k}: {ids[:, 0].tolist()}", flush=True)
+    want = np.argsort(-to64(x), axis=1, kind="stable")[:, :k]
+    assert ids.tolist() == want.tolist()
+    full = row_topk(x.to(cuda), k)
+    assert torch.equal(ids, full[1].cpu()) and (vals - full[0].cpu()).abs().max() < 1e-5
