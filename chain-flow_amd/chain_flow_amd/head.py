@@ -398,7 +398,7 @@ class GemmHead:
 
 def row_topk(logits: torch.Tensor, k: int, split: bool = False):
     """Per-row log-softmax top-k of fp16 logits [M, n] -> (vals f32, ids int32, lse f32).  ``split``: a row's columns over many
-    workgroups, for few long rows; the same ids, lse but for the order of an fp32 sum."""
+    workgroups, for few long rows; the same ids, lse but for the order of an fp32 sum (a row with a NaN: NaN)."""
     M, n = logits.shape
     logits = logits.contiguous()
     vals = torch.empty(M, k, dtype=torch.float32, device=logits.device)

@@ -538,10 +538,12 @@ __global__ void __launch_bounds__(256) k_topk_sets(TopkArgs a, void* ws, int nse
 #pragma unroll
   for (int i = 0; i < N; ++i) raw[i] = L[min(i * 64 + lane, n - 1)];
   float mx = -INFINITY;
+  bool none = false;                                                        // (a NaN, in columns that the row has)
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int at = i * 64 + lane;
     const bool nan = (raw[i] & 0x7fffu) > 0x7c00u;
+    none |= nan;
     const unsigned v = raw[i] == 0x8000u ? 0 : raw[i];                      // (-0 and +0 are equal: the lower column of them)
     const unsigned order = v & 0x8000u ? ~v & 0xffffu : v | 0x8000u;
     key[i] = at < n && !nan ? order << 16 | (0xffffu - at) : 0;             // (0: none)
@@ -580,7 +582,8 @@ __global__ void __launch_bounds__(256) k_topk_sets(TopkArgs a, void* ws, int nse
     cd.cv[base * a.k + lane] = mine ? (float)__builtin_bit_cast(h16, v) : -INFINITY;
     cd.ci[base * a.k + lane] = mine ? set * TS_COLS + (int)(0xffffu - (mine & 0xffffu)) : INT_MAX;
   }
-  // (a NaN sum as the maximum's: the join takes only sums above 0)
+  // a NaN sum (of an infinity, or with a NaN among columns that hold nothing else) as the maximum's: the join takes only sums above 0
+  if (__ballot(none)) se = NAN;
   if (lane == 0) { cd.cs[base * 2] = isnan(se) ? se : mx; cd.cs[base * 2 + 1] = isnan(se) ? 1.f : se; }
 }
 

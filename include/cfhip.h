@@ -274,7 +274,8 @@ int cfh_row_topk(const void* logits, int M, int n, int k, float* vals, int32_t* 
                  void* stream);
 
 /* cfh_row_topk in two launches, a row's columns over many workgroups: ws of cfh_head_ws_bytes(M, n, k) bytes, 16-byte aligned, of the
- * call's own until it ends.  The same order; lse and vals differ from cfh_row_topk's by the order of an fp32 sum.  M <= 65,535. */
+ * call's own until it ends.  The same order; lse and vals differ from cfh_row_topk's by the order of an fp32 sum, and are NaN for
+ * every row with a NaN (cfh_row_topk can miss one that no number above -inf stands beside in its thread).  M <= 65,535. */
 int cfh_row_topk_sets(const void* logits, int M, int n, int k, float* vals, int32_t* ids, float* lse, void* ws,
                       void* stream);
 

@@ -300,3 +300,20 @@ def test_split_top_k_takes_both_zeros_as_equal(cuda, k):
     assert ids.tolist() == want.tolist()
     full = row_topk(x.to(cuda), k)
     assert torch.equal(ids, full[1].cpu()) and (vals - full[0].cpu()).abs().max() < 1e-5
+
+
+@pytest.mark.gpu
+def test_split_top_k_of_columns_without_a_number(cuda):
+    """A NaN anywhere makes a row's log-sum-exp NaN, as a softmax's, also where 512 columns hold nothing else."""
+    x = torch.randn(6, 2000, generator=torch.Generator().manual_seed(1)).half()
+    x[0, 512:1024] = float("nan")
+    x[1, 512:1024] = float("-inf")
+    x[1, 700] = float("nan")
+    x[2, 1536:] = float("nan")
+    x[3, 10] = float("nan")
+    x[4, 512:1024] = float("-inf")                                 # (no NaN: finite)
+    print("[split top-k] sets of NaN", flush=True)
+    vals, ids, lse = (t.cpu() for t in row_topk(x.to(cuda), 4, split=True))
+    assert torch.isnan(lse).tolist() == [True] * 4 + [False] * 2 and torch.isnan(vals[:4]).all() and torch.isfinite(vals[4:]).all()
+    v = to64(x)
+    assert ids.tolist() == np.argsort(np.where(np.isnan(v), np.inf, -v), axis=1, kind="stable")[:, :4].tolist()
