@@ -450,8 +450,8 @@ def matvec4(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, *, table
             ids: torch.Tensor | None = None, ids_stride: int = 1, out: torch.Tensor | None = None) -> torch.Tensor:
     """fp16(x @ w.T) [M, n] of fp16 rows x [M, d] (rows may be strided) with 4-bit weights as ``quantize4`` makes them: weight
     uint8 [n, K / 2], scale fp16 [n, K / group], K a multiple of 128, the group of 32, 64 or 128 columns being K over the
-    scales' columns.  Products and sums are fp32 (a row with a NaN or an infinity is
-    NaN throughout: all of a group's columns are in one sum).  The weights are read once for up to 16 rows.
+    scales' columns.  Products and sums are fp32, of the products with the weights themselves (a weight of zero adds nothing, however
+    large its column; an infinity times it is NaN, as ever).  The weights are read once for up to 16 rows.
 
     With ``table`` [V, r] fp16 and ``ids`` (int32; row m's at m * ids_stride), row ids[m] of the table (outside it: the nearest)
     stands behind x's d columns, d + r = K."""

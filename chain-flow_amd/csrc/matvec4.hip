@@ -4,11 +4,11 @@
 //   y[m][n] = sum_g s[n][g] sum_{k in group g} (u[n][k] - 8) x[m][k],   u in 0 .. 15
 //
 // Weight rows are u[n][K / 2] bytes, column 2 i in the low half of byte i; scales s[n][K / group] fp16; x and y fp16.  Four bits
-// moved to bits 6 .. 9 of 0x4c00 are the fp16 number 16 + u, so a group's sum is
-//     sum (16 + u) x  -  24 sum x
-// with the second term, the same for all weight rows, as what the products are added to: two operations for two weights,
-// and no subtraction.  Products are exact in fp32 and sums are fp32 (MFMA); the magnitudes that meet are at most six times
-// those of (u - 8) x on average, 2^-21 of the sum of |s x| a group, far below the one rounding of the result to fp16.
+// as the last of 0x6400 are the fp16 number 1024 + u, and at bits 4 .. 7 of 0x5400 64 + u: one shift a word, and two operations
+// (and-or, a packed addition of -1032 or -72, which is exact) for two weights.  Products are exact in fp32 and sums are fp32 (MFMA),
+// of the terms (u - 8) x themselves: G adds of at most 2^-23 of the sum of their magnitudes a group.  (16 + u, with 24 sum x
+// taken off behind the products, takes no fewer operations, and a column whose weight is 8 would cost 24 |x| 2^-24 of the
+// sum: with an x of 60,000 beside ones of 1, many times the rounding to fp16.)
 //
 // A wave takes 16 weight rows and 256 columns at a time, in two loads of 8 rows and 128 bytes each: whole lines (a bare read
 // of such a matrix reached 5.9 TB/s so, 5.2 with 16 rows and 64 bytes a load).  Lanes 8 apart exchange halves, so that lane
@@ -45,13 +45,21 @@ struct MvArgs {
   int ks, chunk;                 // waves a tile of 16 weight rows; steps of 128 columns whose x lies in LDS at a time
 };
 
-// The eight weights of a word as fp16 numbers 16 + u, in the order 0 4 1 5 2 6 3 7.  (`e` is 0x4c004c00 in a vector register
-// and the mask in a scalar one: and-or is then one operation, which takes no literals.)
-__device__ __forceinline__ h16x8 plus16(unsigned w, unsigned e) {
-  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-  constexpr unsigned M = 0x03c003c0u;
-  const u32x4 v = {(w << 6 & M) | e, (w << 2 & M) | e, (w >> 2 & M) | e, (w >> 6 & M) | e};
-  return __builtin_bit_cast(h16x8, v);
+// The eight weights of a word as fp16 numbers u - 8, in the order 0 4 1 5 2 6 3 7.  (`e` is 0x64006400 and 0x54005400 in vector
+// registers and the masks in scalar ones: and-or is then one operation, which takes no literals.)
+struct Exponents { unsigned at0, at4; };
+__device__ __forceinline__ h16x8 less8(unsigned w, const Exponents& e) {
+  auto low = [&](unsigned v) __attribute__((always_inline)) {    // bits 0 .. 3 of both halves
+    const unsigned u = (v & 0x000f000fu) | e.at0;
+    return __builtin_bit_cast(h16x2, u) + h16x2{(h16)-1032.f, (h16)-1032.f};
+  };
+  auto high = [&](unsigned v) __attribute__((always_inline)) {   // bits 4 .. 7
+    const unsigned u = (v & 0x00f000f0u) | e.at4;
+    return __builtin_bit_cast(h16x2, u) + h16x2{(h16)-72.f, (h16)-72.f};
+  };
+  const unsigned w8 = w >> 8;
+  const h16x2 a = low(w), b = high(w), c = low(w8), d = high(w8);
+  return __builtin_shufflevector(__builtin_shufflevector(a, b, 0, 1, 2, 3), __builtin_shufflevector(c, d, 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 // Words of four lanes (kg = lane / 16) transposed: word j of lane kg becomes word kg of lane j.
@@ -70,13 +78,14 @@ __device__ __forceinline__ void swap4(unsigned (&w)[4]) {
   s16(w[2], w[3]);
 }
 
-// G: columns a scale; NW waves.  Bound by the weights' bytes where they are many: 62,642 rows of 2,560 columns, one row of x, 16.0
-// us (5.2 TB/s); of 5,376, four rows, 32.9 (5.5); by the launch, x's way into LDS and the joined parts where they are few: 8,191 rows of
-// 4,096, 16 rows of x, 10.4 us for 19 MB.  A step of 128 columns costs a wave some 57 operations beside its loads, so that two
-// steps' loads in flight are enough (four: 18.3 -> 20.5 us for one row of x, as registers leave fewer waves).
+// G: columns a scale; NW waves.  Bound by the weights' bytes where they are many: 62,642 rows of 2,560 columns, one row of x, 18-20
+// us with the weights in memory (4.0-4.5 TB/s), 15 where the caches hold them from the call before (5.5); of 5,376, four rows, 42
+// (4.3) and 31 (5.8).  By the launch, x's way into LDS and the joined parts where they are few: 8,191 rows of 4,096, 16 rows of x, 10
+// us for 19 MB, 8.5 from the caches.  A step of 128 columns costs a wave 52 to 70 vector operations (61 with groups of 64) beside its
+// loads, so that two steps' loads in flight are enough (four cost one row of x 2 us, as registers leave fewer waves).
 template <int G, int NW>
 __global__ void __launch_bounds__(NW * 64, 4) k_matvec4(MvArgs a) {
-  // x [M][chunk columns + 8], eights of them in the order 0 4 1 5 2 6 3 7; behind it -24 times its sums [columns / G][16 rows]
+  // x [M][chunk columns + 8], eights of them in the order 0 4 1 5 2 6 3 7
   extern __shared__ __attribute__((aligned(16))) h16 xs[];
   constexpr int S = 128 / G;     // scales a step
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, kg = lane >> 4;
@@ -107,44 +116,30 @@ __global__ void __launch_bounds__(NW * 64, 4) k_matvec4(MvArgs a) {
 
   // x's columns 128 c0 .. 128 c1 into LDS
   const int ldx = a.chunk * 128 + 8;
-  float* sums = (float*)(xs + a.M * ldx);
   auto stage = [&](int c0, int c1) __attribute__((always_inline)) {
-    constexpr int XB = 4;                            // eights of columns a thread has in flight (16 rows of 4,096: 10.8 us; 2: 12.0)
+    constexpr int XB = 4;                            // eights of columns a thread has in flight (16 rows of 4,096: 9.7 us; 2: 10.2; 8: 9.7)
     const int eights = (c1 - c0) * 16, all = a.M * eights;
     for (int i0 = threadIdx.x; i0 < all; i0 += XB * NW * 64) {
       h16x8 v[XB];
-      int to[XB], at[XB];
+      int to[XB];
 #pragma unroll
       for (int u = 0; u < XB; ++u) {
         const int i = min(i0 + u * NW * 64, all - 1), m = i / eights, here = (i - m * eights) * 8, k = c0 * 128 + here;
         to[u] = m * ldx + here;
-        at[u] = here / G * 16 + m;
         v[u] = k < a.d ? *(const h16x8*)(a.x + m * a.ld_x + k)
                        : *(const h16x8*)(a.a + (size_t)min(max(a.ids[m * a.ids_stride], 0), a.a_rows - 1) * a.r + (k - a.d));
       }
 #pragma unroll
-      for (int u = 0; u < XB; ++u) {
-        *(h16x8*)(xs + to[u]) = __builtin_shufflevector(v[u], v[u], 0, 4, 1, 5, 2, 6, 3, 7);
-        float f = 0.f;                               // (whole groups of G / 8 lanes lie within or behind the last)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f += (float)v[u][e];
-        f += dpp_f32<DPP_XOR1>(f);
-        f += dpp_f32<DPP_XOR2>(f);
-        if (G >= 64) f += dpp_f32<DPP_HMIRROR>(f);
-        if (G >= 128) f += dpp_f32<DPP_MIRROR>(f);
-        if (threadIdx.x % (G / 8) == 0 && i0 + u * NW * 64 < all) sums[at[u]] = -24.f * f;
-      }
+      for (int u = 0; u < XB; ++u) *(h16x8*)(xs + to[u]) = __builtin_shufflevector(v[u], v[u], 0, 4, 1, 5, 2, 6, 3, 7);
     }
     __syncthreads();
   };
   const int m = lane & 15;
   const h16* const x0 = xs + (m < a.M ? m : 0) * ldx + kg * (G < 128 ? 8 : 32);
-  const f32x4* const sum0 = (const f32x4*)sums + kg;
   const h16* xr = x0;
-  const f32x4* sr = sum0;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  unsigned e16 = 0x4c004c00u;
-  asm("" : "+v"(e16));
+  Exponents ex = {0x64006400u, 0x54005400u};
+  asm("" : "+v"(ex.at0), "+v"(ex.at4));
   auto scaled = [&](float f, const f32x4& sum) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] = fmaf(f, sum[e], acc[e]);
@@ -155,12 +150,11 @@ __global__ void __launch_bounds__(NW * 64, 4) k_matvec4(MvArgs a) {
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (j % (G / 32) == 0) sum = sr[j / (G / 32) * 4];
-      sum = mfma_f16(*(const h16x8*)(xr + j * (G < 128 ? 32 : 8)), plus16(q[j], e16), sum);
+      if (j % (G / 32) == 0) sum = {0.f, 0.f, 0.f, 0.f};
+      sum = mfma_f16(*(const h16x8*)(xr + j * (G < 128 ? 32 : 8)), less8(q[j], ex), sum);
       if ((j + 1) % (G / 32) == 0) scaled((float)first_s.v[j / (G / 32)], sum);
     }
     xr += 128;
-    sr += S * 4;
   };
   auto two_steps = [&](const Pair& b) __attribute__((always_inline)) {
     constexpr int ROR8 = 0x128;                      // lanes 8 apart
@@ -177,16 +171,15 @@ __global__ void __launch_bounds__(NW * 64, 4) k_matvec4(MvArgs a) {
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {                    // 32 columns each
-      if (i % (G / 32) == 0) sum = sr[i / (G / 32) * 4];
+      if (i % (G / 32) == 0) sum = {0.f, 0.f, 0.f, 0.f};
       const unsigned word = G < 128 ? q[i & 1][i >> 1] : q[i >> 2][i & 3];
-      sum = mfma_f16(*(const h16x8*)(xr + (G < 128 ? i * 32 : i / 4 * 128 + i % 4 * 8)), plus16(word, e16), sum);
+      sum = mfma_f16(*(const h16x8*)(xr + (G < 128 ? i * 32 : i / 4 * 128 + i % 4 * 8)), less8(word, ex), sum);
       if ((i + 1) % (G / 32) == 0) {
         const int at = i / (G / 32);
         scaled((float)__builtin_bit_cast(h16, (u16)(b.s.v[at / 2] >> (16 * (at % 2)))), sum);
       }
     }
     xr += 256;
-    sr += 2 * S * 4;
   };
   // the first chunk has the odd step; split waves have one chunk, of all columns
   for (int c0 = 0, c1; c0 < steps; c0 = c1) {
@@ -194,9 +187,7 @@ __global__ void __launch_bounds__(NW * 64, 4) k_matvec4(MvArgs a) {
     c1 = a.ks > 1 ? steps : min(steps, c0 + extra + (a.chunk - extra) / 2 * 2);
     if (c0) __syncthreads();                         // (the chunk before is done with)
     stage(c0, c1);
-    const int skip = a.ks > 1 ? s0 : 0;
-    xr = x0 + skip * 128;
-    sr = sum0 + skip * S * 4;
+    xr = x0 + (a.ks > 1 ? s0 : 0) * 128;
     if (c0 == 0 && odd) one_step();
     // (the last pair of all: behind the loop, which has no branch around its loads)
     const int here = (a.ks > 1 ? pairs : (c1 - c0 - extra) / 2) - (c1 == steps ? 1 : 0);
@@ -304,7 +295,7 @@ int cfh_matvec4(const void* x, long long ld_x, int M, int d, const uint8_t* w, i
     return CFH_E_INVALID;
   if (r > 0 && (!a || !a_ids || a_rows < 1 || (uintptr_t)a % 16 || r % 8)) return CFH_E_INVALID;
   const long long tiles = ((long long)n + 15) / 16, steps = K / 128;
-  auto lds_of = [&](int rows, long long c) { return rows * (c * 128 + 8) * 2 + c * 128 / group * 64; };
+  auto lds_of = [](int rows, long long c) { return rows * (c * 128 + 8) * 2; };
   for (int m0 = 0, rows; m0 < M; m0 += rows) {
     rows = std::min(MV_ROWS, M - m0);
     MvArgs v = {};
@@ -314,9 +305,9 @@ int cfh_matvec4(const void* x, long long ld_x, int M, int d, const uint8_t* w, i
     v.y = (h16*)y + m0 * ld_y; v.ld_y = ld_y;
     auto launch = [&](auto g, auto nw) -> int {
       constexpr int NW = nw.value;
-      // K split over a workgroup's waves until there are 200 workgroups: 16 rows times 8,191 x 4,096, 11.7 us in 8 parts, 14.4 in
-      // 4, 18.0 in 16.  Unsplit, x that two workgroups of a compute unit cannot both hold comes in chunks (16 rows of 5,376: 47
-      // us; in two launches of 8 rows 77).
+      // K split over a workgroup's waves until there are 200 workgroups: 16 rows times 8,191 x 4,096, 9.7 us in 8 parts, 11.7 in
+      // 4, 14.7 in 16, 29 in one; one row times 62,642 x 2,560, 18.1 in one, 20.6 in 2.  Unsplit, x that two workgroups of a compute
+      // unit cannot both hold comes in chunks (16 rows of 5,376: 48 us; in two launches of 8 rows 82).
       int ks = 1;
       while (ks < NW && tiles * ks < 200 * NW) ks *= 2;
       long long c = steps;
@@ -338,7 +329,8 @@ int cfh_matvec4(const void* x, long long ld_x, int M, int d, const uint8_t* w, i
       return group == 32 ? launch(std::integral_constant<int, 32>{}, nw) : group == 64 ? launch(std::integral_constant<int, 64>{}, nw)
                                                                               : launch(std::integral_constant<int, 128>{}, nw);
     };
-    // 16 waves share x where two workgroups of 8 do not fit: 62,642 x 5,376, 8 rows 39.2 us (of 8 waves 40.6), 16 rows 47.1 (50.3)
+    // 16 waves share x where two workgroups of 8 do not fit: 62,642 x 5,376, 16 rows 47.9 us (of 8 waves 48.5), with the weights in
+    // the caches 36.2 (40.3); 8 rows 46.1 (45.3), 33.5 (35.4)
     const bool big = lds_of(rows, steps) > MV_HALF;
     if (int rc = big ? of_group(std::integral_constant<int, 16>{}) : of_group(std::integral_constant<int, 8>{})) return rc;
   }

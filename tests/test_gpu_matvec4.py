@@ -1,7 +1,6 @@
 """The 4-bit head on the GPU against float64: quantised weights equal, products within the roundings.
 
-A product's whole numbers and fp16 values multiply exactly in fp32.  (The kernel's are u + 16, and 24 times a group's sum of x is
-taken off: the bound for |u - 8| alone is the stricter one.)  A group's G terms are added in fp32 in some order: off by
+A product's whole numbers and fp16 values multiply exactly in fp32.  A group's G terms are added in fp32 in some order: off by
 at most G 2^-23 of the sum of their magnitudes (2^-23 a step also where a unit truncates); the scaled groups by as much a group, one more for the scaling; then one rounding to fp16, 2^-11 of the value (2^-25 below its normal range)."""
 from __future__ import annotations
 
@@ -317,3 +316,29 @@ def test_split_top_k_of_columns_without_a_number(cuda):
     assert torch.isnan(lse).tolist() == [True] * 4 + [False] * 2 and torch.isnan(vals[:4]).all() and torch.isfinite(vals[4:]).all()
     v = to64(x)
     assert ids.tolist() == np.argsort(np.where(np.isnan(v), np.inf, -v), axis=1, kind="stable")[:, :4].tolist()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,n,K", [(1, 40, 128), (4, 129, 5376), (16, 33, 640), (3, 8191, 2560)])
+def test_products_beside_large_columns(cuda, M, n, K, group):
+    """The bound holds with the weights' own magnitudes: a weight of zero takes nothing from a column, however large it is,
+    and rows of x far from zero lose nothing to what their weights cancel."""
+    g = torch.Generator().manual_seed(M * K + group)
+    for size in (1000.0, 8000.0, 60000.0):
+        w, s, W = _weights(n, K, group, M + n, "cpu")
+        x = torch.randn(M, K, generator=g).half()
+        at = torch.arange(K) % group == int(size) % group              # a column a group, of either sign, whose weights are 0
+        x[:, at] = torch.where(torch.rand(M, int(at.sum()), generator=g) < 0.5, -size, size).half()
+        u = torch.from_numpy(ohead.unpack4(w.numpy()).astype(np.uint8))
+        u[:, at] = 8
+        w = u[:, ::2] | u[:, 1::2] << 4
+        W = ohead.dequant4(u.numpy(), to64(s))
+        assert np.array_equal(ohead.unpack4(w.numpy()), u.numpy())
+        y = matvec4(x.to(cuda), w.to(cuda), s.to(cuda))
+        print(f"[matvec4] columns of {size:.0f}, M={M} n={n} K={K} G={group}: {_close(y, x.numpy(), W, group):.2f} of the bound", flush=True)
+    x = (torch.randn(M, K, generator=g) + 200).half()
+    s = (s.float() * 2.0 ** -6).half()
+    W = ohead.dequant4(u.numpy(), to64(s))
+    y = matvec4(x.to(cuda), w.to(cuda), s.to(cuda))
+    print(f"[matvec4] rows around 200, M={M} n={n} K={K} G={group}: {_close(y, x.numpy(), W, group):.2f} of the bound", flush=True)
