@@ -482,10 +482,12 @@ __global__ void __launch_bounds__(256) k_copy(ResizeArgs a) {
   }
 }
 
+constexpr long long PAGE_MOST = 0x40000000ll - PIECE;   // elements of a page: its last piece ends within 32 bits
+
 int pool_of(const cfh_kv_pool* c, PoolArgs& a) {
   if (!c || c->layers < 1 || c->blocks < 1 || c->page < 1 || c->heads < 1) return CFH_E_INVALID;
   if ((c->dim != 64 && c->dim != 128 && c->dim != 256) || (long long)c->blocks * c->page > 0x7fffffffll ||
-      (long long)c->page * c->heads * c->dim > 0x3fffffffll)
+      (long long)c->page * c->heads * c->dim > PAGE_MOST)
     return CFH_E_UNSUPPORTED;
   const bool f8 = c->k_exp || c->v_exp;
   const int es = f8 ? 1 : 2;

@@ -587,7 +587,8 @@ int cfh_paged_attn_fresh(const void* q, long long q_ld, int T, int H, int Hkv, i
 /* ---------------------------------------------------------------- the committed prefix: the cache's pages
  * The caches of all attention layers, on one block table: keys k, values v [layers][blocks][page][heads][dim] as the
  * single cache above (2-byte elements, or e4m3 with both k_exp and v_exp [layers][blocks][page][heads]); strides of a layer
- * (ls, unused where there is one layer) and a block (bs) in elements, multiples of 16, of a layer's scales (ls_exp) in bytes. */
+ * (ls, unused where there is one layer) and a block (bs) in elements, multiples of 16, of a layer's scales (ls_exp) in bytes.
+ * blocks * page < 2^31, page * heads * dim <= 2^30 - 16,384. */
 typedef struct cfh_kv_pool {
   void *k, *v;
   uint8_t *k_exp, *v_exp;

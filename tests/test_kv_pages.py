@@ -133,3 +133,17 @@ def test_pool_refusals_without_a_device():
     assert commit(p_ld=4) == commit(t_ld=3) == commit(S=-1) == commit(path=None) == commit(k=None) == commit(k_exp=p) == 1
     assert commit(bs_k=511) == commit(bs_v=520) == commit(ls_k=2552) == commit(ls_v=512) == commit(ls_k=2544) == commit(k=p + 8) == commit(layers=0) == 1
     assert commit(dim=96) == commit(blocks=1 << 30) == commit(S=65536) == 2
+
+
+def test_pages_end_within_32_bits():
+    """A page is copied in pieces of 16 KB whose ends are 32-bit numbers: the largest pages, whose last piece would end behind
+    them, are refused by every call that takes a pool."""
+    L, p = _lib.lib(), 4096
+
+    def calls(page):
+        pool = _lib.KvPool(p, p, None, None, 0, 0, page * 64, page * 64, 0, 0, 1, 1, page, 1, 64)
+        return (L.cfh_kv_resize(pool, p, 4, 4, p, 0, p, 1, page, p, p, None, None),
+                L.cfh_kv_commit(pool, p, 4, 4, p, p, 5, 5, p, 0, None, None))
+    last = (2 ** 30 - 16384) // 64
+    assert calls(last) == (0, 0) and (last * 128 + 16383) // 16384 * 16384 < 2 ** 31
+    assert calls(last + 1) == calls((2 ** 30 - 1) // 64) == (2, 2)
