@@ -342,3 +342,33 @@ def test_products_beside_large_columns(cuda, M, n, K, group):
     W = ohead.dequant4(u.numpy(), to64(s))
     y = matvec4(x.to(cuda), w.to(cuda), s.to(cuda))
     print(f"[matvec4] rows around 200, M={M} n={n} K={K} G={group}: {_close(y, x.numpy(), W, group):.2f} of the bound", flush=True)
+
+
+@pytest.mark.gpu
+def test_drafts_over_4_bits_equal_the_oracles(cuda):
+    """Chains and trees over the 4-bit head, token for token and parent for parent.  No two candidates of the search are within
+    0.05 of each other (hiddens are chosen so; logits of up to 32 are rounded by 2^-7 at most), so nothing else passes."""
+    cfg = flownet(512, layers=1, flow_steps=2)
+    W = make_weights(cfg, 4096, init="test", base_seed=1)
+    W["lm_head.weight"] = (W["lm_head.weight"].float() * 8).half()
+    sl = torch.randperm(4096, generator=torch.Generator().manual_seed(2))[:1024].sort().values.to(torch.int32)
+    dr = Drafter(cfg, {k: v.to(cuda) for k, v in W.items()}, sl.to(cuda), device=cuda, head_bits=4, head_group=32)
+    pred = torch.randn(2, 8, 512, generator=torch.Generator().manual_seed(2203)).half()
+    known0 = torch.tensor([int(sl[7]), int(sl[100])])
+    print("[4-bit drafts] against the oracle's search", flush=True)
+    chains = dr.beam_chains(None, known0.to(cuda), 5, 4, pred=pred.to(cuda)).cpu()
+    tree = dr.beam_tree(None, known0.to(cuda), 4, 4, 4, pred=pred.to(cuda)).cpu()
+    D = ohead.dequant4(ohead.unpack4(dr.head.weight.cpu().numpy()), to64(dr.head.scale))
+    W64 = {k: to64(v) for k, v in W.items()}
+    sl64, w1 = sl.long().numpy(), to64(dr.head.w1)
+
+    def score(h, prev):
+        x = np.concatenate([np.asarray(h, dtype=np.float64), w1[np.clip(prev, 0, None)]], 1)
+        return (x @ D.T).astype(np.float16).astype(np.float64)
+    resid = lambda lp, nl: ohead.path_residual(W64, W64["embed_tokens.weight"], lp, nl, cfg.path_order)    # noqa: E731
+    args = (to64(pred), known0.numpy(), sl64, 4)
+    ref, trace = obeam.beam_chains(*args, 5, cfg.path_order, score, resid, return_trace=True)
+    ref_tree, more = obeam.beam_tree(*args, 4, 4, cfg.path_order, score, resid, return_trace=True)
+    assert min(ohead.margins(t[what], 4).min() for t in trace + more for what in ("lp", "cand")) > 0.05
+    assert chains.tolist() == ref.tolist()
+    assert tree.tolist() == ref_tree.tolist()
