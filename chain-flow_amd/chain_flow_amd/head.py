@@ -399,6 +399,10 @@ class GemmHead:
 def row_topk(logits: torch.Tensor, k: int, split: bool = False):
     """Per-row log-softmax top-k of fp16 logits [M, n] -> (vals f32, ids int32, lse f32).  ``split``: a row's columns over many
     workgroups, for few long rows; the same ids, lse but for the order of an fp32 sum (a row with a NaN: NaN)."""
+    if logits.dtype != torch.float16 or logits.dim() != 2:
+        raise ValueError("logits must be fp16 [M, n]")
+    if not logits.is_cuda:
+        raise ValueError("logits must lie on a GPU")
     M, n = logits.shape
     logits = logits.contiguous()
     vals = torch.empty(M, k, dtype=torch.float32, device=logits.device)
@@ -407,8 +411,9 @@ def row_topk(logits: torch.Tensor, k: int, split: bool = False):
     args = (logits.data_ptr(), M, n, k, vals.data_ptr(), ids.data_ptr(), lse.data_ptr())
     L = _lib.lib()
     if split:
+        dev = _lib.device_of(logits)
         ws = torch.empty(max(int(L.cfh_head_ws_bytes(M, n, k)), 16), dtype=torch.uint8, device=logits.device)
-        _lib.check(L.cfh_row_topk_sets(*args, ws.data_ptr(), _lib.stream_of(logits.get_device())), "cfh_row_topk_sets")
+        _lib.check(L.cfh_row_topk_sets(*args, ws.data_ptr(), _lib.stream_of(dev)), "cfh_row_topk_sets")
     else:
         _lib.check(L.cfh_row_topk(*args, _lib.stream_handle()), "cfh_row_topk")
     return vals, ids, lse

@@ -7,7 +7,7 @@ import torch
 
 from chain_flow_amd import _lib
 from chain_flow_amd.drafter import Drafter
-from chain_flow_amd.head import QuantHead, matvec4, quantize4
+from chain_flow_amd.head import QuantHead, matvec4, quantize4, row_topk
 from oracle import head as ohead
 
 
@@ -63,3 +63,11 @@ def test_refusals_without_a_device():
         return L.cfh_quantize4(w, w2, None, n, d, r, group, q, s, None)
     assert qt(n=0) == 0 and qt(w=None) == qt(w=p + 2) == qt(q=None) == qt(s=None) == qt(group=0) == qt(r=64, d=192) == 1
     assert qt(d=96) == qt(d=192) == qt(d=160, r=96, w2=p) == 2
+
+
+@pytest.mark.parametrize("split", [False, True])
+def test_row_topk_refusals(split):
+    x = torch.zeros(2, 256, dtype=torch.float16)
+    for bad in (x, x.bfloat16(), x.float(), x[0]):                    # (host memory, other types, one row)
+        with pytest.raises(ValueError, match="logits"):
+            row_topk(bad, 4, split=split)
