@@ -243,10 +243,10 @@ __global__ void __launch_bounds__(1024, 4) k_sample_parts(SampleArgs a) {
 }
 
 // One workgroup of T threads a row.  BITS: a value's count in LDS, 32 / BITS values a word (the low bits of the value name the
-// word, the high ones the field).  The counts are right where they add up to V: one that leaves its BITS takes 2^BITS from its
-// own and adds at most 1 to the next, so that the sum only falls.  Then (a constant row, a masked one) half of the values
-// are counted at a time, in twice the bits, which V cannot leave: 8 bits and 64 KB for V < 65,536, 16 bits and 128 KB
-// above.  The row is read again, from the caches, for the drawn token's index.
+// word, the high ones the field).  The counts are right where they add up to V: one that leaves its BITS takes 2^BITS from its own
+// for each 1 that it adds to the next, so that the sum only falls.  Then (a constant row, values that crowd) half of them
+// are counted at a time, in twice the bits, which V cannot leave.  8 bits (64 KB) are for many rows of V < 65,536, 16 bits (128 KB)
+// for all others (the rule and what both cost stand at the launch).  The row is read again, from the caches, for the drawn token's index.
 // What bounds a row of 248,320 bf16 logits on its CU: 17 us of counting (an LDS atomic a logit, a wave's 64 in 10 cycles), 2.2 the
 // cells (fp16: 4.2, more values are in use), 1.5 a search (one wave's latency), 4 the index.  1,968 rows of 32,000: 11 us a row and
 // CU in fp16, 1.5 TB/s; the stages of two rows overlap there, and the searches' latency and the weights of many values
@@ -295,13 +295,13 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
   unsigned h = NONE;                                 // the value that hist does not hold, and its tokens (a thread's, then the row's)
   int n_h = 0;
   int half = 0;                                      // (wide) the top bit of the values whose counts hist holds
-  auto count_half = [&](int h) __attribute__((always_inline)) {
-    half = h;
+  auto count_half = [&](int top_bit) __attribute__((always_inline)) {
+    half = top_bit;
     for (int i = t; i < WORDS / 4; i += T) ((uint4*)hist)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     auto add_wide = [&](unsigned v, unsigned n) __attribute__((always_inline)) {
       if (v == 0x8000u) v = 0;                       // -0 counts as +0
-      if ((int)(v >> 15) == h) atomicAdd(&hist[v & (WORDS - 1)], n << (((v & 0x7fffu) >> LOG) * (2 * BITS & 31)));
+      if ((int)(v >> 15) == top_bit) atomicAdd(&hist[v & (WORDS - 1)], n << (((v & 0x7fffu) >> LOG) * (2 * BITS & 31)));
     };
 #pragma unroll 1
     for (int j = t; j < whole; j += T) {
@@ -515,10 +515,10 @@ __global__ void __launch_bounds__(T, 4) k_sample_rows(SampleArgs a) {
     if (all != V) {
       wide = true;
       h = NONE;                                      // (counted with the others)
-      for (int h = 1; h >= 0; --h) {
+      for (int top_bit = 1; top_bit >= 0; --top_bit) {
         __syncthreads();
-        count_half(h);
-        cells(h ? GROUPS / 2 : 0, h ? GROUPS : GROUPS / 2);
+        count_half(top_bit);
+        cells(top_bit ? GROUPS / 2 : 0, top_bit ? GROUPS : GROUPS / 2);
       }
       __syncthreads();
     }
@@ -786,8 +786,10 @@ __global__ void __launch_bounds__(64) k_sample_walk(WalkArgs a) {
 }
 
 // How many parts a row is counted in.  The whole call over 248,320 logits: 6 rows 34.8 us in one part, 31.4 in 2, 29.3 in 4, 34.6
-// in 8 (a part's counts are 128 KB to read for the row's CU, 1.4 us); 24 rows 37.2 and 30.5 in 4, 36 rows 38.4 and 35.1, 41 rows of
-// other filters 41.2 and 40.7, 82 rows 42 and 50.  A part's counts stay below 2^16.
+// in 8 (a part's counts are 128 KB to read for the row's CU, 1.4 us).  One part and 4 by rows, bf16 with k and P (deviation 2.5
+// around 0; 0.7 around -6): 6 rows 37.8 and 32.4 us; 61.0 and 52.2.  24 rows 38.6 and 33.4; 62.5 and 54.5.  36 rows 39.9 and 37.9; 63.5
+// and 57.5.  64 rows 39.7 and 39.9; 63.9 and 59.4.  82 rows 42.0 and 49.1; 65.3 and 69.4.  (So parts lose above 64 rows, and 25 to
+// 64 would gain 0 to 6 us by them.)  A part's counts stay below 2^16.
 int parts_of(int n_rows, int V) {
   const int parts = max(4, V / 65528 + 1);
   return n_rows <= 24 && V >= 65536 && parts <= 8 ? parts : 1;
@@ -829,9 +831,11 @@ int cfh_tree_sample_accept(const void* logits, long long ld, int V, int n_rows, 
     hipLaunchKernelGGL(fn, dim3(n_rows, parts), dim3(1024), 0, st, s);
     CFH_LAUNCH_CHECK();
   }
-  // 8 bits let two workgroups share a CU: 1,968 rows of 32,000 logits 87 us in fp16 and 72 in bf16, with 16 bits 129 and 118; 492 rows 31 and
-  // 27, 42 and 38; 246 rows (a CU each) 24 and 22 either way.  But a value that more than 255 have sends its row to the wide
-  // counts (1,968 rows of 32,000 bf16 logits around -6: 192 us), so they are for many rows, and in bf16 for up to 32,768 values.
+  // 8 bits let two workgroups share a CU, but a value that more than 255 have sends its row to the wide counts.  8 and 16 bits over
+  // 1,968 rows of 32,000 logits with k and P: fp16 102 and 161 us around 0, 100 and 164 around -6, 105 and 172 of deviation 0.7 there.
+  // bf16, whose values are eight times as far apart: 91 and 150 around 0, where they lie densest, but 207 and 165 of deviation 1.5 around -6,
+  // 170 and 150 of 3 around 8.  300 rows, fp16 30 and 40; bf16 25 and 37 around 0, 56 and 40 around -6.  (The host cannot tell where the
+  // logits lie: bf16 takes the side that gains the more.)  246 rows (a CU each) take the same either way.
   const bool narrow = V < 65536 && n_rows > 256 && (!is_bf16 || V <= 32768);
   auto launch = [&](auto bf, auto v) {
     constexpr bool BF = bf.value, VEC = v.value;
