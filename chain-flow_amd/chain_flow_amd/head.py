@@ -503,7 +503,8 @@ class QuantHead:
     """``ShortlistHead`` at 4 bits: the shortlisted rows of lm_head and, behind their columns, of markov.w2 as ``quantize4``
     weights (174 MB for 62,642 rows at d = 5120, r = 256, groups of 64, against 673 MB), so that a row's logit is one product
     of [h, w1[prev]] and is rounded once.  A depth's top k of those rows takes 40 us where the fp16 head's takes 110 (1 to 8 rows;
-    49 and 113 at 16); every 16 rows read the weights again (32 rows: 89 and 112, 48: 126 and 112).  The drafts it makes differ from the fp16 head's; what the target's verify
+    47 and 111 at 16); every 16 rows read the weights again (32 rows: 87 and 112, 48: 124 and 112, 64: 162 and 112), so that it is for up
+    to some 40 rows: fp16 rows are not kept, and nothing falls back to them.  The drafts it makes differ from the fp16 head's; what the target's verify
     accepts of them is distributed as before."""
 
     def __init__(self, lm_w: torch.Tensor, shortlist: torch.Tensor | None, w1: torch.Tensor | None = None,

@@ -18,7 +18,8 @@ Mirrors ``chain_flow.vllm_plugin.flow_proposer.FlowDrafterProposer`` (``cf/vllm_
 * the head is the two-pass candidate head by default (``CF_TWOPASS_M=8192``, ``CF_TWOPASS_SHARED=1``,
   ``CF_TWOPASS_SEED=0``; ``:1113-1184``, ``cf/defaults.py:123-127``), dropped when M does not fit
   the head unless it was asked for; ``CF_HEAD_BITS=4`` (16) holds the head at 4 bits and searches it
-  in one pass;
+  in one pass, for the whole process: for servers of up to some 10 requests at width 4 (beyond, each
+  16 beams read the weights again, and the fp16 head with ``CF_TWOPASS_M=0`` is faster);
 * the context lives in a device ring per batch slot (``_ring_write`` / ``_ring_gather``,
   ``:916-961``; ``cfh_ring_step``), with the slot lifecycle of ``_ctx_gpu`` (``:2045-2105``: a new
   request resets or seeds its slot, a request moved by vLLM's batch condense carries its history),

@@ -186,7 +186,8 @@ constexpr int RS_FAR = 0x3fffffff; // a place behind every page
 // Up to so many table entries (and RS_T sequences) one workgroup does all of it, in one launch; above, the entries are let go of
 // and filled in by a workgroup a sequence, in launches before and behind.  A pair of calls that grows and shrinks 48
 // sequences of 567 entries: 14.8 us so, 25.3 in three launches each (200 of 304: 15.7, 26.5; 1,000 of 223: 19.9, 26.4); a pair in
-// which every page changes hands 41 and 34 (79 and 41; 266 and 89).
+// which every page changes hands 41 and 34 (79 and 41; 266 and 89).  The cost goes with the pages that change, which the host does not
+// know: the rule takes the side of growing by a step's rows and back, which every step does, and loses where prompts come and go.
 constexpr long long RS_ONE = 65536;
 
 // Pages that a sequence has, wants and keeps.
@@ -448,8 +449,8 @@ __global__ void __launch_bounds__(64) k_fill(ResizeArgs a) {
 }
 
 // Last, the copies: a piece of a page of one layer's keys or values at a time.  96 pages in 8 layers (29 of their 64 rows of 4 x 256
-// bf16 on average: 180 MB in and out) 27 us, 6.6 TB/s.  At most 4,096 workgroups, as the number of copies is known here only:
-// those and a plan without copies take 55.3 and 6.9 us, with 1,024 of them 56.1 and 6.6, with 16,384 54.3 and 9.2.
+// bf16 on average: 180 MB in and out) 41 us, 4.4 TB/s, with the pages in memory; 27 over one pool again and again.  At most 4,096 workgroups, as the number of copies is known here only:
+// the whole call and a plan without copies take 55.3 and 6.9 us, with 1,024 of them 56.1 and 6.6, with 16,384 54.3 and 9.2.
 constexpr int PIECE = 16384;
 
 __global__ void __launch_bounds__(256) k_copy(ResizeArgs a) {
